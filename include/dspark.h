@@ -587,6 +587,49 @@ int dspark_argmax_accept(const void* logits, int64_t ld, int64_t M, int64_t V, c
                          int32_t* target_tokens, int32_t* n_accepted, void* workspace, size_t workspace_bytes,
                          dspark_stream stream);
 
+/* ------------------------------------------------------------------ sampled rounds (temperature > 0) */
+
+/*
+ * The probabilities a token is sampled from, fp32 [rows, V] (row stride ldo):
+ *   w = exp((x - max x) / temperature) over the row (0 for -inf and NaN logits; with a +inf logit 1 for
+ *   those and 0 for the rest); of the top_k largest (0: all) those tokens before which, in falling order,
+ *   less than top_p of their mass lies (1: all); out = w / their sum on these, 0 elsewhere. Equal logits
+ *   are ordered by index. A row with nothing but -inf and NaN gives zeros.
+ * logits bf16 or fp16 [rows, V] (row stride ld, any alignment), V <= 524280, rows <= 65535. Weights and
+ * sums are fp64. workspace >= dspark_sampling_workspace(rows, V, 0) bytes, 256-byte aligned, of any content.
+ * Covers the reference's truncate_probs (sampling.py) with the softmax before it.
+ */
+size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences);
+
+int dspark_sampling_probs(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V, double temperature,
+                          int64_t top_k, double top_p, float* out, int64_t ldo, void* workspace,
+                          size_t workspace_bytes, dspark_stream stream);
+
+/*
+ * The accept rule of a sampled round (speculative sampling) for a batch of sequences, with p_i the row
+ * dspark_sampling_probs forms of logits row i, in fp64:
+ *   draft i is accepted while all before it are and u_i * q_i(draft_i) < p_i(draft_i);
+ *   n = the first one refused (the number of drafts if none is);
+ *   tokens = the n accepted drafts, one token drawn from max(p_n - q_n, 0) (from p_n where no draft was
+ *   refused or that is zero throughout), then -1. Drawn: the first token whose running sum, by index, is
+ *   over u_last times the whole sum (0 where p_n is zero throughout).
+ * logits     bf16 or fp16 [sequences, drafts + 1, V], strides ld_seq / ld_row, any alignment
+ * draft      int32 [sequences, drafts] (drafts <= 255); one outside 0..V-1 is refused, p = 0
+ * draft_probs fp32 [sequences, drafts, V], strides q_seq / q_row (nullable: q = 1 at the drafted token)
+ * draft_lens int32 [sequences] (nullable = drafts), clamped to 0..drafts: the drafts of a padded batch
+ * uniforms   [sequences, drafts + 1] in [0, 1), fp32 or (uniforms_f64) fp64; the last one draws the token
+ * n_accepted int32 [sequences]; tokens int32 [sequences, drafts + 1]; draft_p fp32 [sequences, drafts]
+ *            (p_i(draft_i) of every draft, those after the first refused one too)
+ * workspace >= dspark_sampling_workspace(sequences * (drafts + 1), V, sequences) bytes, 256-byte aligned,
+ * of any content. The sampling counterpart of dspark_argmax_accept (generate.py's sampling accept).
+ */
+int dspark_speculative_verify(int dtype, const void* logits, int64_t ld_seq, int64_t ld_row, int64_t sequences,
+                              int64_t drafts, int64_t V, const int32_t* draft, const float* draft_probs,
+                              int64_t q_seq, int64_t q_row, const int32_t* draft_lens, const void* uniforms,
+                              int uniforms_f64, double temperature, int64_t top_k, double top_p,
+                              int32_t* n_accepted, int32_t* tokens, float* draft_p, void* workspace,
+                              size_t workspace_bytes, dspark_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,251 @@
+// Sampling from next-token logits (gfx950): the truncated softmax of a row and the accept rule of a
+// sampled speculative round, both from 16-bit logits x[0..V).
+//
+//   w_v = exp((x_v - max x) / T), 0 where x_v is -inf or NaN (max = +inf: 1 where x_v = +inf, else 0)
+//   K   = the top_k largest logits (all without top_k), Z_K the sum of w over K
+//   N   = the tokens of K, in falling order, before which less than top_p * Z_K lies
+//   p_v = w_v / Z on N with Z the sum of w over N, else 0; equal logits are ordered by index
+//   accept draft i:  u_i * q_i(x_i) < p_i(x_i)        (q = 1 at the drafted token without draft_probs)
+//   n = the first draft refused (or the number of drafts); the token after them is drawn from
+//   r_v = max(p_v - q_v, 0) of row n, from p of row n where there was no draft or r is zero throughout:
+//   the first v whose running sum of r passes u_last times the whole sum.
+//
+// Every weight is formed and summed in 64 bits, in an order that depends on the sizes alone: which
+// token a random number falls on is decided by differences that fp32 sums over 1e5 tokens do not hold
+// (a token of probability 1e-5 is 1e2 units of an fp32 sum of 1 wide). Vector fp64 runs at the rate of
+// fp32 here, so the exponential (a degree-10 polynomial) costs less than reading the logits does.
+//
+// A row is cut into segments of 512 logits, one wave load of 16 bytes a lane. The first pass leaves the
+// maximum of each segment and its sum of weights against that maximum; whatever follows works on these
+// few hundred values and re-reads single segments:
+//   - the normaliser of a row is the join of its segments;
+//   - a cut needs a threshold. 16-bit logits have at most 2^16 values, so the weight mass above a value is
+//     a sum over distinct values of count * weight: integer counts in LDS, joined in falling order. Only
+//     segments whose maximum can reach the threshold are read: for top_k the k-th largest segment
+//     maximum bounds it from below, for top_p the weight (1 - top_p) S / V (what lies below all
+//     together weighs less than (1 - top_p) S);
+//   - the drawn token is found by a scan over segments, then inside one.
+// Segments start at 16-byte addresses, not at the row's start: a row of odd length behind another one
+// still loads 16 bytes a lane, and only its first and last 8 logits element by element.
+#pragma once
+
+#include "dspark_common.h"
+
+namespace dspark {
+
+constexpr int kSegVals = 512;          // logits of a segment
+constexpr int kMaxSegs = 1024;         // segments of a row: one LDS slot each in the kernels of a row
+constexpr int kMaxDraft = 255;         // drafts of a sequence
+constexpr int kBins = 8192;            // distinct logit values counted at a time
+constexpr int kRowThreads = 512;       // threads of the kernels that work on one row or sequence
+
+struct SampleArgs {
+  const u16* x;                        // logits
+  long ldb, ldr;                       // strides of a sequence, of a row inside it
+  int rows, per, V, nseg;              // rows in all, rows of a sequence
+  double c;                            // log2(e) / T
+  double top_p;
+  int top_k;                           // 0: none
+  float* segm;                         // [rows][nseg] segment maxima
+  double* segs;                        // [rows][nseg] segment sums
+};
+
+struct RowInfo {                       // what the later kernels need of a row
+  double z;                            // sum of the kept weights (0: nothing to draw from)
+  double px;                           // the drafted token's probability
+  float m;                             // the row's maximum
+  int thr, cut;                        // kept: key > thr, or key == thr and index <= cut
+  int pad;
+};
+
+struct VerifyIn {
+  const int32_t* draft;                // [sequences][per - 1]
+  const float* q;                      // draft probabilities, or null
+  long qb, qr;                         // strides of a sequence, of a draft
+  const int32_t* lens;                 // drafts of each sequence, or null
+  const void* u;                       // uniforms [sequences][per]
+  int u64;                             // uniforms in 64 bits
+  int32_t* n;                          // accepted
+  int32_t* tokens;                     // [sequences][per]
+  float* px;                           // [sequences][per - 1]
+};
+
+// ---------------------------------------------------------------- values and keys
+
+template <bool HALF>
+__device__ __forceinline__ float val(u32 bits) {
+  if constexpr (HALF) return (float)__builtin_bit_cast(_Float16, (u16)bits);
+  else return bf2f(bits);
+}
+
+template <bool HALF>
+constexpr u32 kInfBits = HALF ? 0x7C00u : 0x7F80u;
+
+// Order of the logits as integers: NaN counts as -inf, -0 as +0.
+template <bool HALF>
+__device__ __forceinline__ int key_of(u32 b) {
+  if ((b & 0x7FFFu) > kInfBits<HALF>) b = 0x8000u | kInfBits<HALF>;
+  if (b == 0x8000u) b = 0;
+  return (int)((b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u));
+}
+template <bool HALF>
+constexpr int kLowKey = (int)(~(0x8000u | kInfBits<HALF>) & 0xFFFFu);  // the key of -inf
+template <bool HALF>
+__device__ __forceinline__ float val_of_key(int k) {
+  return val<HALF>((k & 0x8000) ? (u32)k & 0x7FFFu : ~(u32)k & 0xFFFFu);
+}
+template <bool HALF>
+__device__ __forceinline__ int key_of_float(float f) {
+  if constexpr (HALF) return key_of<HALF>(__builtin_bit_cast(u16, (_Float16)f));
+  else return key_of<HALF>(f2bf(f));
+}
+
+// 2^d for d <= 0: the interpolation of 2^f on [-1/2, 1/2] in 11 Chebyshev nodes (within 5e-15 of itself,
+// exact at 0), times a power of two; 0 below 2^-1075.
+__device__ __forceinline__ double exp2_neg(double d) {
+  d = __builtin_fmax(d, -1080.0);
+  const double n = __builtin_rint(d), f = d - n;
+  double p = 6.4224123393201308e-09;
+  p = __builtin_fma(p, f, 1.02053706737851e-07);
+  p = __builtin_fma(p, f, 1.3219110032865315e-06);
+  p = __builtin_fma(p, f, 1.5252674086943783e-05);
+  p = __builtin_fma(p, f, 0.00015403523472909156);
+  p = __builtin_fma(p, f, 0.0013333558203519715);
+  p = __builtin_fma(p, f, 0.0096181291126410592);
+  p = __builtin_fma(p, f, 0.055504108664584259);
+  p = __builtin_fma(p, f, 0.24022650695899311);
+  p = __builtin_fma(p, f, 0.69314718055994884);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+
+// The weight of a logit against a maximum m (a NaN logit fails both tests and its NaN argument is taken
+// for the smaller operand: 0).
+__device__ __forceinline__ double weight(float x, float m, double c) {
+  if (x == m) return x > -INFINITY ? 1.0 : 0.0;
+  return exp2_neg(((double)x - (double)m) * c);
+}
+
+// ---------------------------------------------------------------- wave reductions (DPP)
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_d(double v) {
+  const u32x2_t b = __builtin_bit_cast(u32x2_t, v);
+  u32x2_t r;
+  r[0] = (u32)__builtin_amdgcn_update_dpp(0, (int)b[0], CTRL, ROWS, 0xF, true);
+  r[1] = (u32)__builtin_amdgcn_update_dpp(0, (int)b[1], CTRL, ROWS, 0xF, true);
+  return __builtin_bit_cast(double, r);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {  // max with the shifted value, -inf where there is none
+  const int lo = __builtin_bit_cast(int, -INFINITY);
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(lo, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
+}
+
+// Running sums over the lanes of a wave: shifts inside rows of 16 lanes, then the last lane of row 0
+// and 2 into the next row, then that of the lower half into the upper.
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp_d<0x111, 0xF>(v);
+  v += dpp_d<0x112, 0xF>(v);
+  v += dpp_d<0x114, 0xF>(v);
+  v += dpp_d<0x118, 0xF>(v);
+  v += dpp_d<0x142, 0xA>(v);
+  v += dpp_d<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_i<0x111, 0xF>(v);
+  v += dpp_i<0x112, 0xF>(v);
+  v += dpp_i<0x114, 0xF>(v);
+  v += dpp_i<0x118, 0xF>(v);
+  v += dpp_i<0x142, 0xA>(v);
+  v += dpp_i<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const u32x2_t b = __builtin_bit_cast(u32x2_t, v);
+  u32x2_t r;
+  r[0] = (u32)__builtin_amdgcn_readlane((int)b[0], lane);
+  r[1] = (u32)__builtin_amdgcn_readlane((int)b[1], lane);
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wave_total(double v) { return lane_value(wave_scan(v), 63); }
+__device__ __forceinline__ float wave_max(float v) {
+  v = dpp_max<0x111, 0xF>(v);
+  v = dpp_max<0x112, 0xF>(v);
+  v = dpp_max<0x114, 0xF>(v);
+  v = dpp_max<0x118, 0xF>(v);
+  v = dpp_max<0x142, 0xA>(v);
+  v = dpp_max<0x143, 0xC>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// Running sums over the threads of a workgroup, in thread order; `total` is the whole sum.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* waves, V& total) {
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const V in = wave_scan(v);
+  if ((threadIdx.x & 63) == 63) waves[w] = in;
+  __syncthreads();
+  V before = 0, all = 0;
+  for (int i = 0; i < nw; ++i) {
+    if (i == w) before = all;
+    all += waves[i];
+  }
+  __syncthreads();
+  total = all;
+  return before + in;
+}
+
+// ---------------------------------------------------------------- segments
+
+// Where a row's first logit lies inside its first 16 bytes: logit v is value v + off of the segments.
+__device__ __forceinline__ int row_off(const u16* row) { return (int)((reinterpret_cast<uintptr_t>(row) >> 1) & 7); }
+
+// The 8 logits of a lane of segment `seg` (first index v0 = 512 seg + 8 lane - off), -inf outside the row.
+template <bool HALF>
+__device__ __forceinline__ u32x4_t load8(const u16* row, int v0, int V) {
+  if (v0 >= 0 && v0 + 8 <= V) return ldg128(row + v0);
+  constexpr u32 ninf = 0x8000u | kInfBits<HALF>;
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int a = v0 + 2 * i, b = a + 1;
+    const u32 lo = (a >= 0 && a < V) ? row[a] : ninf, hi = (b >= 0 && b < V) ? row[b] : ninf;
+    r[i] = lo | (hi << 16);
+  }
+  return r;
+}
+__device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >> 1] >> (16 * (j & 1))) & 0xFFFFu; }
+
+__device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int row) {
+  return a.x + (long)(row / a.per) * a.ldb + (long)(row % a.per) * a.ldr;
+}
+
+// The normaliser of a row without a cut, and its maximum: the join of its segments over a workgroup.
+__device__ __forceinline__ double join_segments(const float* segm, const double* segs, int nseg, double c, float* red_f,
+                                                double* red_d, float& m) {
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  float mx = -INFINITY;
+  for (int s = threadIdx.x; s < nseg; s += blockDim.x) mx = fmaxf(mx, segm[s]);
+  mx = wave_max(mx);
+  if ((threadIdx.x & 63) == 0) red_f[w] = mx;
+  __syncthreads();
+  for (int i = 0; i < nw; ++i) mx = fmaxf(mx, red_f[i]);
+  double z = 0;
+  for (int s = threadIdx.x; s < nseg; s += blockDim.x) z += segs[s] * weight(segm[s], mx, c);
+  z = wave_total(z);
+  if ((threadIdx.x & 63) == 0) red_d[w] = z;
+  __syncthreads();
+  z = 0;
+  for (int i = 0; i < nw; ++i) z += red_d[i];
+  __syncthreads();
+  m = mx;
+  return z;
+}
+
+}  // namespace dspark

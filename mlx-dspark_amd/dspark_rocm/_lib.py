@@ -20,6 +20,7 @@ c_int = ctypes.c_int
 c_i64 = ctypes.c_int64
 c_size_t = ctypes.c_size_t
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 c_char_p = ctypes.c_char_p
 c_i64_p = ctypes.POINTER(ctypes.c_int64)
 
@@ -183,6 +184,12 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_argmax_accept_workspace": (c_size_t, [c_i64, c_i64]),
     "dspark_argmax_accept": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
                                      c_size_t, c_void_p]),
+    "dspark_sampling_workspace": (c_size_t, [c_i64, c_i64, c_i64]),
+    "dspark_sampling_probs": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_double, c_i64, c_double, c_void_p, c_i64,
+                                      c_void_p, c_size_t, c_void_p]),
+    "dspark_speculative_verify": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64,
+                                          c_i64, c_void_p, c_void_p, c_int, c_double, c_i64, c_double, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -6,6 +6,7 @@ These are the product path: every function here launches a hand-written gfx950 k
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -869,3 +870,152 @@ def argmax_accept(logits: torch.Tensor, draft: torch.Tensor, target_tokens: torc
         raise ValueError("argmax_accept: draft must be a contiguous int32 tensor on the logits' device")
     _lib.call("dspark_argmax_accept", _ptr(logits), logits.stride(0), M, V, _ptr(draft) if m else None, m,
               _ptr(target_tokens), _ptr(n_accepted), _ptr(workspace), workspace.numel(), _stream(logits))
+
+
+# ---------------------------------------------------------------------------- sampled rounds
+
+LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1}    # dspark_dtype codes
+
+
+def _on_device(device: torch.device):
+    """The device as the current one for the block (a launch needs its stream's device to be)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _no_autograd(what: str, *ts: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise ValueError(f"{what}: has no backward pass; detach its inputs or use torch.no_grad()")
+
+
+def _one_device(what: str, first: torch.Tensor, *ts) -> None:
+    if not first.is_cuda:
+        raise ValueError("dspark kernels need tensors on a ROCm device (cuda:N)")
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
+    t, k, p = float(temperature), int(top_k or 0), float(top_p)
+    if not 1e-30 <= t <= 1e30:
+        raise ValueError(f"temperature={temperature}: a positive number (greedy rounds: argmax_accept)")
+    if k < 0 or not 0.0 < p <= 1.0:
+        raise ValueError(f"top_k={top_k} (0 or more), top_p={top_p} (over 0, up to 1)")
+    return t, k, p
+
+
+def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> torch.Tensor:
+    nbytes = _lib.load().dspark_sampling_workspace(rows, vocab, sequences)
+    if nbytes == 0:
+        raise ValueError(f"{rows} rows of {vocab} logits (up to 65535 rows of 524280)")
+    if ws is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if ws.numel() * ws.element_size() < nbytes or ws.device != device or not ws.is_contiguous():
+        raise ValueError(f"workspace: {nbytes} contiguous bytes on {device} needed")
+    return ws
+
+
+def sampling_workspace_bytes(rows: int, vocab: int, sequences: int = 0) -> int:
+    """Workspace bytes of :func:`sampling_probs` over ``rows`` rows, or of :func:`speculative_verify`
+    over ``sequences`` sequences of ``rows`` rows together."""
+    return int(_lib.load().dspark_sampling_workspace(rows, vocab, sequences))
+
+
+def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                   out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The probabilities a token is sampled from, fp32 [..., V]: softmax of ``logits / temperature``
+    (bf16 or fp16 [..., V]) over the ``top_k`` largest logits (0: all), of these over the tokens before
+    which less than ``top_p`` of their mass lies, 0 elsewhere. Equal logits are ordered by index; a row
+    of nothing but -inf and NaN gives zeros. What a drafter samples its tokens from and hands to
+    :func:`speculative_verify`. ``out`` contiguous; ``workspace`` (any content) of
+    :func:`sampling_workspace_bytes`, else allocated."""
+    _one_device("sampling_probs", logits, out, workspace)
+    dt = LOGIT_DTYPES.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"sampling_probs: logits {logits.dtype} (bfloat16 or float16)")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"sampling_probs: logits {tuple(logits.shape)}")
+    _no_autograd("sampling_probs", logits)
+    t, k, p = _sampler(temperature, top_k, top_p)
+    V = logits.shape[-1]
+    x = logits.reshape(-1, V)
+    if x.stride(1) != 1 or x.stride(0) < V:
+        x = x.contiguous()
+    rows = x.shape[0]
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    elif out.dtype != torch.float32 or out.shape != logits.shape or not out.is_contiguous():
+        raise ValueError(f"sampling_probs: out must be contiguous fp32 {tuple(logits.shape)}")
+    if rows:
+        ws = _sampling_workspace(workspace, logits.device, rows, V, 0)
+        with _on_device(logits.device):
+            _lib.call("dspark_sampling_probs", dt, x.data_ptr(), x.stride(0), rows, V, t, k, p, out.data_ptr(), V,
+                      ws.data_ptr(), ws.numel() * ws.element_size(), _stream(x))
+    return out
+
+
+def _ints(what: str, name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must be int32 or int64 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if t.dtype == torch.int64:              # an id past 32 bits stays one that no vocabulary has
+        t = t.clamp(-1, 2 ** 31 - 1)
+    return t.to(torch.int32).contiguous()
+
+
+def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torch.Tensor, *,
+                       draft_probs: torch.Tensor | None = None, draft_lens: torch.Tensor | None = None,
+                       temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                       workspace: torch.Tensor | None = None):
+    """The accept rule of a sampled round: ``(n_accepted int32 [B], tokens int32 [B, m + 1], draft_p fp32
+    [B, m])`` for the logits bf16 / fp16 [B, m + 1, V] of ``[anchor] + m drafts`` per sequence, with p the
+    rows :func:`sampling_probs` forms of them (in 64 bits).
+
+    Draft i is accepted while all before it are and ``uniforms[b, i] * q < p`` at the drafted token
+    (``draft_probs`` fp32 [B, m, V], normalised as the drafter sampled from it; None: q = 1, a drafter
+    without probabilities). ``tokens`` are the accepted drafts, then one drawn with ``uniforms[b, m]``
+    from ``max(p - q, 0)`` of the refused row, or from p of the row after the last draft, then -1; the
+    committed tokens then follow p whatever the drafter proposed. ``draft_p``: p of every draft.
+    ``draft_lens`` [B] (padded batches): how many drafts each sequence has. ``uniforms`` [B, m + 1] fp32 or
+    fp64 in [0, 1). Drafts outside the vocabulary are refused. m up to 255."""
+    what = "speculative_verify"
+    _one_device(what, logits, draft, uniforms, draft_probs, draft_lens, workspace)
+    dt = LOGIT_DTYPES.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"{what}: logits {logits.dtype} (bfloat16 or float16)")
+    if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
+        raise ValueError(f"{what}: logits must be [B, drafts + 1, V], got {list(logits.shape)}")
+    B, R, V = logits.shape
+    m = R - 1
+    if m > 255:
+        raise ValueError(f"{what}: {m} drafts (up to 255)")
+    if uniforms.dtype not in (torch.float32, torch.float64) or tuple(uniforms.shape) != (B, R):
+        raise ValueError(f"{what}: uniforms must be fp32 or fp64 [{B}, {R}], got {uniforms.dtype} {list(uniforms.shape)}")
+    t, k, p = _sampler(temperature, top_k, top_p)
+    draft = _ints(what, "draft", draft, (B, m))
+    q = q_seq = q_row = 0
+    if draft_probs is not None:
+        if draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (B, m, V):
+            raise ValueError(f"{what}: draft_probs must be fp32 [{B}, {m}, {V}], got {draft_probs.dtype} {list(draft_probs.shape)}")
+        _no_autograd(what, draft_probs)
+        if draft_probs.stride(2) != 1:
+            draft_probs = draft_probs.contiguous()
+        q, q_seq, q_row = draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1)
+    _no_autograd(what, logits)
+    if draft_lens is not None:
+        draft_lens = _ints(what, "draft_lens", draft_lens, (B,))
+    x = logits if logits.stride(2) == 1 else logits.contiguous()
+    u = uniforms.contiguous()
+    dev = logits.device
+    n = torch.empty(B, dtype=torch.int32, device=dev)
+    tokens = torch.empty((B, R), dtype=torch.int32, device=dev)
+    draft_p = torch.empty((B, m), dtype=torch.float32, device=dev)
+    if B:
+        ws = _sampling_workspace(workspace, dev, B * R, V, B)
+        with _on_device(dev):
+            _lib.call("dspark_speculative_verify", dt, x.data_ptr(), x.stride(0), x.stride(1), B, m, V, draft.data_ptr(),
+                      q or None, q_seq, q_row, None if draft_lens is None else draft_lens.data_ptr(), u.data_ptr(),
+                      int(u.dtype == torch.float64), t, k, p, n.data_ptr(), tokens.data_ptr(), draft_p.data_ptr(),
+                      ws.data_ptr(), ws.numel() * ws.element_size(), _stream(x))
+    return n, tokens, draft_p

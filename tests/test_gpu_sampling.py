@@ -1,0 +1,236 @@
+"""GPU: sampling_probs and speculative_verify against the oracle in 64 bits.
+
+Counts and tokens are equal. A probability is one fp64 value rounded to fp32: half a step of it (2^-24)
+beside the fp64 error of two weights (5e-15 of the polynomial, |argument| 2^-53 <= 1.2e-13 each) and sums."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import sampling_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def close(got, want):
+    got, want = _np(got), np.asarray(want)
+    assert got.shape == want.shape
+    assert (np.abs(got - want) <= want * (2.0 ** -24 + 1e-12) + 2.0 ** -150).all(), np.abs(got - want).max()
+
+
+def rows(g, n, V, dtype, kind="plain"):
+    x = 3.0 * torch.randn(n, V, generator=g)
+    if kind == "ties":
+        x = torch.round(x)
+    elif kind == "same":
+        x = torch.full((n, V), -1.25)
+    elif kind == "masked":                               # most of the row cut off, as a grammar does; type's lowest too
+        x = torch.where(torch.rand(n, V, generator=g) < 0.97, float("-inf"), x)
+        x[:, ::7] = torch.finfo(dtype).min
+        x[:, V // 2] = 0.5
+    elif kind == "zeros":                                # +0 and -0 are equal logits
+        x = torch.where(torch.rand(n, V, generator=g) < 0.5, 0.0, -0.0)
+    elif kind == "odd":                                  # values that are not finite
+        x[:, ::5] = float("nan")
+        x[:, 1::5] = float("-inf")
+        if n > 1:
+            x[1, V // 3] = x[1, -1] = float("inf")
+        if n > 2:
+            x[2] = float("-inf")
+        if n > 3:
+            x[3] = float("nan")
+    elif kind == "far":                                  # the whole range of the type, tiny values among them
+        x = x * torch.exp2(torch.randint(-20, 4, (n, V), generator=g).float())
+    return x.to(dtype)
+
+
+CUTS = [dict(), dict(top_k=1), dict(top_k=20), dict(top_p=0.9), dict(top_k=50, top_p=0.8), dict(top_p=1e-9),
+        dict(temperature=0.25, top_p=0.999), dict(temperature=3.0, top_k=700)]
+
+
+@pytest.mark.parametrize("kind", ["plain", "ties", "same", "masked", "zeros", "odd", "far"])
+@pytest.mark.parametrize("n,V,dtype", [(4, 1, "bf16"), (4, 7, "f16"), (4, 511, "bf16"), (4, 513, "f16"), (4, 5000, "bf16"),
+                                       (5, 50257, "f16"), (4, 151936, "bf16")])
+def test_probs(dev, n, V, dtype, kind):
+    from dspark_rocm import ops
+
+    x = rows(torch.Generator().manual_seed(V + n), n, V, DT[dtype], kind)
+    for kw in CUTS:
+        got = ops.sampling_probs(x.to(dev), **kw)
+        assert got.dtype == torch.float32
+        close(got, np.stack([ref.probs(r, **kw) for r in _np(x)]))
+
+
+def test_probs_of_the_longest_row(dev):
+    from dspark_rocm import ops
+
+    x = rows(torch.Generator().manual_seed(0), 1, 524280, torch.bfloat16)
+    for kw in (dict(), dict(top_p=0.97), dict(top_k=1000, top_p=0.9)):
+        close(ops.sampling_probs(x.to(dev), **kw), ref.probs(_np(x)[0], **kw)[None])
+    with pytest.raises(ValueError):
+        ops.sampling_probs(torch.zeros(1, 524281, dtype=torch.bfloat16, device=dev))
+
+
+def _drafts(g, x, kind, m):
+    """Drafts from a distribution near the target's, and it."""
+    B, _, V = x.shape
+    q = torch.softmax(torch.nan_to_num(x[:, :m].float(), 0.0, 5.0, -30.0).clamp(-30, 30) + torch.randn(B, m, V, generator=g), -1)
+    d = torch.multinomial(q.reshape(-1, V), 1, generator=g).reshape(B, m) if m else torch.zeros(B, 0, dtype=torch.int64)
+    return d.to(torch.int32), q
+
+
+@pytest.mark.parametrize("kind", ["plain", "ties", "masked", "odd"])
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("B,m,V,dtype", [(1, 0, 8192, "bf16"), (3, 1, 1, "bf16"), (2, 4, 9, "f16"), (5, 3, 777, "bf16"),
+                                         (1, 15, 32003, "f16"), (7, 2, 4096, "bf16"), (2, 3, 151936, "bf16")])
+def test_verify(dev, B, m, V, dtype, kind, dense):
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(B * 1000 + m * 10 + V)
+    x = rows(g, B * (m + 1), V, DT[dtype], kind).reshape(B, m + 1, V)
+    d, q = _drafts(g, x, kind, m)
+    seen = set()
+    for i, kw in enumerate(CUTS):
+        u = torch.rand(B, m + 1, generator=g, dtype=torch.float64 if i % 2 else torch.float32)
+        lens = torch.randint(0, m + 1, (B,), generator=g) if i % 3 == 2 else None
+        got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev) if dense else None,
+                                     draft_lens=None if lens is None else lens.to(dev), **kw)
+        want = ref.verify(_np(x), d.numpy(), u.numpy(), q.numpy() if dense else None, None if lens is None else lens.numpy(), **kw)
+        assert np.array_equal(got[0].cpu().numpy(), want[0]), (kw, got[0], want[0])
+        assert np.array_equal(got[1].cpu().numpy(), want[1]), (kw, got[1], want[1])
+        close(got[2], want[2])
+        seen.update(want[0].tolist())
+    assert len(seen) > 1 or not (dense and kind == "plain" and m > 1 and V > 9)     # drafts are taken and refused
+
+
+def test_verify_takes_what_the_reference_would_index(dev):
+    """Drafts outside the vocabulary, lengths outside the batch, random numbers at and past both ends, the same
+    token drafted twice, int64 drafts: refused, clamped or drawn, and nothing read out of range."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(5)
+    x = rows(g, 12, 1000, torch.bfloat16).reshape(3, 4, 1000)
+    best = x.float().argmax(-1)[:, :3]
+    for d in (torch.tensor([[-1, 5, 5]] * 3), torch.tensor([[1000, 0, 0]] * 3), torch.tensor([[2 ** 31 - 1, 0, 0]] * 3),
+              torch.tensor([[2 ** 32 + 7, 0, 0]] * 3), best):
+        for u in (torch.zeros(3, 4), torch.full((3, 4), 1.0 - 2.0 ** -24), torch.full((3, 4), 1.0), torch.full((3, 4), 2.0)):
+            for lens in (None, torch.tensor([-4, 1, 99])):
+                for dense in (False, True):
+                    q = torch.softmax(x[:, :3].float(), -1)
+                    for kw in (dict(), dict(top_k=5)):
+                        got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev) if dense else None,
+                                                     draft_lens=None if lens is None else lens.to(dev), **kw)
+                        want = ref.verify(_np(x), d.clamp(-1, 2 ** 31 - 1).numpy(), u.numpy(), q.numpy() if dense else None,
+                                          None if lens is None else lens.numpy(), **kw)
+                        assert np.array_equal(got[0].cpu().numpy(), want[0])
+                        if dense and not kw:
+                            continue        # p = q but for their roundings: the rest is the roundings' own pattern
+                        assert np.array_equal(got[1].cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("cut", [dict(), dict(top_k=30, top_p=0.9)])
+def test_views_and_strides(dev, cut):
+    """Rows at any address and stride: a column slice from an odd column, sequences and rows exchanged, a
+    transposed vocabulary, expanded logits; draft probabilities a slice too."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(9)
+    big = rows(g, 20, 3001, torch.bfloat16).reshape(4, 5, 3001).to(dev)
+    u = torch.rand(5, 4, generator=g).to(dev)
+    for x in (big[:, :, 3:2999].transpose(0, 1), big[:, :, :1001].transpose(0, 1),
+              big.transpose(1, 2).contiguous().transpose(1, 2).transpose(0, 1), big[:1].expand(4, 5, 3001).transpose(0, 1)):
+        V = x.shape[2]
+        d, q = _drafts(g, x.cpu(), "plain", 3)
+        wide = torch.zeros(5, 3, V + 3, device=dev)
+        wide[:, :, 1:V + 1] = q.to(dev)
+        got = ops.speculative_verify(x, d.to(dev), u, draft_probs=wide[:, :, 1:V + 1], **cut)
+        want = ref.verify(_np(x), d.numpy(), _np(u), q.numpy(), **cut)
+        assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1])
+        close(got[2], want[2])
+        close(ops.sampling_probs(x[:, 0], **cut), np.stack([ref.probs(r, **cut) for r in _np(x[:, 0])]))
+
+
+def test_out_and_workspace(dev):
+    """out is written and nothing beside it; a workspace of any content serves, one too small or misplaced does not."""
+    from dspark_rocm import ops
+
+    x = rows(torch.Generator().manual_seed(2), 3, 1003, torch.float16).to(dev)
+    buf = torch.full((3 * 1003 + 2,), 7.0, device=dev)
+    out = buf[1:-1].view(3, 1003)
+    need = ops.sampling_workspace_bytes(3, 1003)
+    ws = torch.full((need,), 0xFF, dtype=torch.uint8, device=dev)
+    for kw in CUTS:
+        assert ops.sampling_probs(x, out=out, workspace=ws, **kw) is out
+        close(out, np.stack([ref.probs(r, **kw) for r in _np(x)]))
+        assert buf[0] == 7 and buf[-1] == 7
+    for bad in (dict(workspace=ws[:-1]), dict(workspace=ws.cpu()), dict(out=out.t()), dict(out=out.half()), dict(out=out[:2])):
+        with pytest.raises(ValueError):
+            ops.sampling_probs(x, **bad)
+
+
+def test_refusals(dev):
+    from dspark_rocm import ops
+
+    x = torch.zeros(2, 3, 10, dtype=torch.bfloat16, device=dev)
+    d, u = torch.zeros(2, 2, dtype=torch.int32, device=dev), torch.zeros(2, 3, device=dev)
+    for bad in (dict(draft_probs=torch.zeros(2, 2, 9, device=dev)), dict(draft_probs=torch.zeros(2, 2, 10, device=dev).half()),
+                dict(draft_lens=torch.zeros(3, dtype=torch.int32, device=dev)), dict(draft_lens=torch.zeros(2, device=dev)),
+                dict(draft_probs=torch.zeros(2, 2, 10)), dict(temperature=0.0), dict(top_p=0.0),
+                dict(draft_probs=torch.zeros(2, 2, 10, device=dev, requires_grad=True))):
+        with pytest.raises(ValueError):
+            ops.speculative_verify(x, d, u, **bad)
+    for args in ((x[0], d, u), (x, d[:, :1], u), (x, d.float(), u), (x, d, u[:, :2]), (x, d, u.half()), (x, d.cpu(), u)):
+        with pytest.raises(ValueError):
+            ops.speculative_verify(*args)
+    for f in (lambda: ops.speculative_verify(x.float(), d, u), lambda: ops.sampling_probs(x.float())):
+        with pytest.raises(TypeError):
+            f()
+    assert ops.sampling_probs(x[:0]).shape == (0, 3, 10)
+    assert [tuple(t.shape) for t in ops.speculative_verify(x[:0], d[:0], u[:0])] == [(0,), (0, 3), (0, 2)]
+
+
+@pytest.mark.parametrize("cut", [dict(), dict(top_k=20, top_p=0.9)])
+def test_streams_and_graphs(dev, cut):
+    """On another stream; two captured graphs replayed in turn with the program's own calls between."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(4)
+    sets = []
+    for _ in range(2):
+        x = rows(g, 8, 20000, torch.bfloat16).reshape(2, 4, 20000)
+        d, q = _drafts(g, x, "plain", 3)
+        sets.append([t.to(dev) for t in (x, d, torch.rand(2, 4, generator=g), q)])
+    call = lambda s: ops.speculative_verify(s[0], s[1], s[2], draft_probs=s[3], **cut)
+    want = [[t.clone() for t in call(s)] for s in sets]
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        outs = [call(s) for s in sets]
+    other.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(a, b) for a, b in zip(w, o))
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = call(s)
+        graphs.append((graph, o))
+    for _ in range(3):
+        for (graph, o), w in zip(graphs, want):
+            for t in o:
+                t.zero_()
+            graph.replay()
+            call(sets[0])
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(w, o))
+    sets[0][2].copy_(torch.rand(2, 4, generator=g))         # new random numbers in place, as a serving loop draws them
+    graphs[0][0].replay()
+    assert all(torch.equal(a, b) for a, b in zip(call(sets[0]), graphs[0][1]))
