@@ -35,7 +35,7 @@ typedef void* dspark_stream; /* hipStream_t */
 enum dspark_dtype {
   DSPARK_DTYPE_BF16 = 0,
   DSPARK_DTYPE_F16 = 1,
-  DSPARK_DTYPE_F32 = 2   /* dspark_qmm_dequantize only */
+  DSPARK_DTYPE_F32 = 2   /* dspark_qmm_dequantize, dspark_rope, the plain rows of dspark_kv_* */
 };
 
 enum dspark_status {
@@ -629,6 +629,50 @@ int dspark_speculative_verify(int dtype, const void* logits, int64_t ld_seq, int
                               int uniforms_f64, double temperature, int64_t top_k, double top_p,
                               int32_t* n_accepted, int32_t* tokens, float* draft_p, void* workspace,
                               size_t workspace_bytes, dspark_stream stream);
+
+/* ------------------------------------------------------------------ rotary positions, quantized cache rows */
+
+/*
+ * Rotary positions of queries [B, Hq, L, D] and keys [B, Hk, L, D] (Hk = 0: queries alone) in one launch:
+ *   a_i = position * freqs[i], i < dims / 2
+ *   (y1, y2) = scale * (x1 cos a_i - x2 sin a_i, x1 sin a_i + x2 cos a_i)
+ * for the pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved, of the first dims values of a head; the
+ * other D - dims are copied. fp32 with the angle reduced in fp64, rounded once to dtype (bf16, fp16, fp32).
+ * Strides (batch, head, row) in elements, unit stride along D; 16-byte accesses where every address and
+ * stride allows, else single values. y may be x itself (the same address and strides), not overlap it
+ * otherwise. positions: int32 or (positions_i64) int64 of row (b, l) at b * stride[0] + l * stride[1];
+ * NULL: pos0 + l. freqs fp64 [dims / 2] on the device, in radians a position.
+ * D <= 1024, dims even and <= 256, B * L <= 2^24. Covers mx.fast.rope as mlx-lm's layers call it
+ * (traditional or not, dims below the head, offset and freqs arrays), which dspark_qk_norm_rope_kv fuses
+ * for one layout.
+ */
+int dspark_rope(int dtype, const void* q, const int64_t q_strides[3], int64_t Hq, const void* k,
+                const int64_t k_strides[3], int64_t Hk, int64_t B, int64_t L, int64_t D, int64_t dims, int interleaved,
+                const double* freqs, float scale, const void* positions, int positions_i64,
+                const int64_t position_strides[2], int64_t pos0, void* q_out, const int64_t q_out_strides[3], void* k_out,
+                const int64_t k_out_strides[3], dspark_stream stream);
+
+/*
+ * Rows into a quantized cache (mlx-lm QuantizedKVCache layout), keys and values in one launch. Of each two
+ * arguments [0] is the keys', [1] the values'; strides are (batch, head, row) triples, keys then values.
+ * Per group of 64 values of x [B, H, T, D] (bf16, fp16 or fp32), every step one fp32 operation:
+ *   scale = (max - min) * fl(1 / (2^bits - 1)) and bias = min, rounded to cache_dtype (bf16 or fp16);
+ *   field = clamp(round_half_even((x - bias) / scale), 0, 2^bits - 1), a scale of 0 dividing as 1
+ * (dspark_qk_norm_rope_kv_quantized's rule but for the quotient by 2^bits - 1). A NaN makes its group's scale and bias NaN, its fields 0.
+ * words uint32 [B, H, T, D * bits / 32], scales and biases [B, H, T, D / 64] (shared strides), unit stride
+ * along the last dim: rows of a cache view. D % 64 == 0, group_size 64, 2 * B * H <= 65535.
+ */
+int dspark_kv_quantize(int x_dtype, const void* const x[2], const int64_t x_strides[6], int cache_dtype,
+                       uint32_t* const words[2], void* const scales[2], void* const biases[2],
+                       const int64_t word_strides[6], const int64_t scale_strides[6], int64_t B, int64_t H, int64_t T,
+                       int64_t D, int bits, int group_size, dspark_stream stream);
+
+/* Such rows read back: out = scale * field (rounded to fp32) + bias (rounded to fp32), rounded to
+ * out_dtype (bf16, fp16 or fp32); the same arguments, out [B, H, T, D] with its own strides. */
+int dspark_kv_dequantize(int cache_dtype, const uint32_t* const words[2], const void* const scales[2],
+                         const void* const biases[2], const int64_t word_strides[6], const int64_t scale_strides[6],
+                         int64_t B, int64_t H, int64_t T, int64_t D, int bits, int group_size, int out_dtype,
+                         void* const out[2], const int64_t out_strides[6], dspark_stream stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,278 @@
+// Rows quantized into a key/value cache as they are written, and the cache read back (gfx950), both
+// tensors of a layer in one launch.
+//
+// A group is 64 values of a row; its scale and bias are rounded to the cache's type, its fields come from
+// the rounded ones, every step one fp32 operation (dspark_rocm.quant.quantize_rows on this GPU, bit for
+// bit: torch's quotient by a constant is the product with its rounded reciprocal here, so the fused
+// q/k/v kernel, which divides, rounds about one scale in 2^16 to the other side):
+//   scale = T((max - min) * fl(1 / (2^bits - 1))), bias = T(min), f = clamp(round_half_even((x - bias) / scale))
+// with a scale of 0 dividing as 1; read back: T'(fl(f * scale) + bias). A NaN in a group makes its scale and
+// bias NaN and its fields 0.
+//
+// Bound by bytes: 8 lanes hold a group, 8 values a lane (16 bytes of a 16-bit row), the group's extremes
+// joined over the 8 lanes with DPP.
+#include "dspark_common.h"
+
+// A product and a sum stay two roundings: a fused one does not overflow between them.
+#pragma clang fp contract(off)
+
+namespace dspark {
+namespace {
+
+constexpr int kKvThreads = 256;
+
+struct KvSide {                                // keys or values
+  char* x;                                     // plain rows (read, or the output of a read back)
+  long xb, xh, xt;                             // strides of batch, head, row, in elements
+  u32* w;
+  u16* s;
+  u16* b;
+  long wb, wh, wt, sb, sh, st;
+};
+
+struct KvArgs {
+  KvSide side[2];
+  int B, H, D8;                                // D8 = D / 8
+  u32 items;                                   // rows * D8 of one head
+};
+
+template <int DT>
+__device__ __forceinline__ float kv_get(u32 bits) {
+  if constexpr (DT == DSPARK_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (u16)bits);
+  else return bf2f(bits);
+}
+template <int DT>
+__device__ __forceinline__ u16 kv_put(float v) {
+  if constexpr (DT == DSPARK_DTYPE_F16) return __builtin_bit_cast(u16, (_Float16)v);
+  else return f2bf(v);
+}
+
+// Joined over each aligned group of 8 lanes, in all of them (the exchanges of sum8_lanes).
+__device__ __forceinline__ float min8_lanes(float v) {
+  v = fminf(v, dpp_mov<0xB1>(v));
+  v = fminf(v, dpp_mov<0x4E>(v));
+  return fminf(v, dpp_mov<0x141>(v));
+}
+__device__ __forceinline__ float max8_lanes(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v));
+  v = fmaxf(v, dpp_mov<0x4E>(v));
+  return fmaxf(v, dpp_mov<0x141>(v));
+}
+
+// SRC: type of the rows; DST: type of scales and biases; ALIGNED: 16-byte rows, 8-byte words
+template <int SRC, int DST, int BITS, bool ALIGNED>
+__global__ __launch_bounds__(kKvThreads) void kv_quantize_kernel(const KvArgs a) {
+  const u32 i = blockIdx.x * kKvThreads + threadIdx.x;
+  if (i >= a.items) return;                    // whole groups: items is a multiple of 8
+  const int bh = blockIdx.y % (a.B * a.H), b = bh / a.H, h = bh % a.H;
+  const KvSide& s = a.side[blockIdx.y >= (unsigned)(a.B * a.H)];
+  const u32 t = i / (u32)a.D8, c = i - t * a.D8;
+  float v[8];
+  const long at = b * s.xb + h * s.xh + (long)t * s.xt + 8 * c;
+  if constexpr (SRC == DSPARK_DTYPE_F32) {
+    const float* x = reinterpret_cast<const float*>(s.x) + at;
+    if constexpr (ALIGNED) {
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(x), hi = *reinterpret_cast<const f32x4_t*>(x + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = lo[j];
+        v[4 + j] = hi[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = x[j];
+    }
+  } else {
+    const u16* x = reinterpret_cast<const u16*>(s.x) + at;
+    if constexpr (ALIGNED) {
+      const u32x4_t r = ldg128(x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = kv_get<SRC>(r[j] & 0xFFFFu);
+        v[2 * j + 1] = kv_get<SRC>(r[j] >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = kv_get<SRC>(x[j]);
+    }
+  }
+  constexpr float kLevels = (float)((1 << BITS) - 1);
+  float lo = v[0], hi = v[0], bad = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    lo = fminf(lo, v[j]);
+    hi = fmaxf(hi, v[j]);
+    bad = v[j] != v[j] ? 1.f : bad;
+  }
+  lo = min8_lanes(lo);
+  hi = max8_lanes(hi);
+  if (max8_lanes(bad) != 0.f) lo = hi = __builtin_nanf("");
+  const u16 sbits = kv_put<DST>((hi - lo) * (1.0f / kLevels)), bbits = kv_put<DST>(lo);
+  const float sc = kv_get<DST>(sbits), bias = kv_get<DST>(bbits);
+  const float div = sc == 0.f ? 1.f : sc;
+  u32 f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    f[j] = (u32)fminf(fmaxf(rintf(__fdiv_rn(v[j] - bias, div)), 0.f), kLevels);
+  u32* w = s.w + b * s.wb + h * s.wh + (long)t * s.wt + (BITS / 4) * c;
+  if constexpr (BITS == 8) {
+    const u32x2_t two = {f[0] | (f[1] << 8) | (f[2] << 16) | (f[3] << 24), f[4] | (f[5] << 8) | (f[6] << 16) | (f[7] << 24)};
+    if constexpr (ALIGNED) {
+      *reinterpret_cast<u32x2_t*>(w) = two;
+    } else {
+      w[0] = two[0];
+      w[1] = two[1];
+    }
+  } else {
+    u32 one = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) one |= f[j] << (4 * j);
+    *w = one;
+  }
+  if ((c & 7) == 0) {
+    const long g = b * s.sb + h * s.sh + (long)t * s.st + (c >> 3);
+    s.s[g] = sbits;
+    s.b[g] = bbits;
+  }
+}
+
+// SRC: type of scales and biases; DST: type of the rows written; ALIGNED as above
+template <int SRC, int DST, int BITS, bool ALIGNED>
+__global__ __launch_bounds__(kKvThreads) void kv_dequantize_kernel(const KvArgs a) {
+  const u32 i = blockIdx.x * kKvThreads + threadIdx.x;
+  if (i >= a.items) return;
+  const int bh = blockIdx.y % (a.B * a.H), b = bh / a.H, h = bh % a.H;
+  const KvSide& s = a.side[blockIdx.y >= (unsigned)(a.B * a.H)];
+  const u32 t = i / (u32)a.D8, c = i - t * a.D8;
+  const u32* w = s.w + b * s.wb + h * s.wh + (long)t * s.wt + (BITS / 4) * c;
+  u32x2_t f;
+  if constexpr (BITS == 8) {
+    if constexpr (ALIGNED) f = ldg64(w);
+    else f = u32x2_t{w[0], w[1]};
+  } else {
+    f = u32x2_t{w[0], 0};
+  }
+  const long g = b * s.sb + h * s.sh + (long)t * s.st + (c >> 3);
+  const float sc = kv_get<SRC>(s.s[g]), bias = kv_get<SRC>(s.b[g]);
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const u32 q = BITS == 8 ? (f[j >> 2] >> (8 * (j & 3))) & 0xFFu : (f[0] >> (4 * j)) & 0xFu;
+    v[j] = (float)q * sc + bias;
+  }
+  const long at = b * s.xb + h * s.xh + (long)t * s.xt + 8 * c;
+  if constexpr (DST == DSPARK_DTYPE_F32) {
+    float* y = reinterpret_cast<float*>(s.x) + at;
+    if constexpr (ALIGNED) {
+      *reinterpret_cast<f32x4_t*>(y) = f32x4_t{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4_t*>(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = v[j];
+    }
+  } else {
+    u16* y = reinterpret_cast<u16*>(s.x) + at;
+    if constexpr (ALIGNED) {
+      u32x4_t o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = (u32)kv_put<DST>(v[2 * j]) | ((u32)kv_put<DST>(v[2 * j + 1]) << 16);
+      *reinterpret_cast<u32x4_t*>(y) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = kv_put<DST>(v[j]);
+    }
+  }
+}
+
+template <bool WRITE, int A, int C, int BITS, bool AL>
+void launch_kv(const KvArgs& a, hipStream_t s) {
+  const dim3 grid((a.items + kKvThreads - 1) / kKvThreads, (unsigned)(2 * a.B * a.H)), block(kKvThreads);
+  if constexpr (WRITE) hipLaunchKernelGGL((kv_quantize_kernel<A, C, BITS, AL>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((kv_dequantize_kernel<A, C, BITS, AL>), grid, block, 0, s, a);
+}
+
+template <bool WRITE, int A, int C>
+void launch_kv(const KvArgs& a, int bits, bool al, hipStream_t s) {
+  if (bits == 8) al ? launch_kv<WRITE, A, C, 8, true>(a, s) : launch_kv<WRITE, A, C, 8, false>(a, s);
+  else al ? launch_kv<WRITE, A, C, 4, true>(a, s) : launch_kv<WRITE, A, C, 4, false>(a, s);
+}
+
+// The arguments both directions share; `al`: everything a wide access touches is aligned for it.
+int kv_args(const char* what, int x_dtype, int c_dtype, void* const x[2], const int64_t x_strides[6], uint32_t* const words[2],
+            void* const scales[2], void* const biases[2], const int64_t w_strides[6], const int64_t s_strides[6], int64_t B,
+            int64_t H, int64_t T, int64_t D, int bits, int group_size, KvArgs& a, bool& al) {
+  if (!x || !x_strides || !words || !scales || !biases || !w_strides || !s_strides) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  if (bits != 4 && bits != 8) return fail(DSPARK_ERR_UNSUPPORTED, "%s: bits=%d (4 or 8)", what, bits);
+  if (group_size != 64) return fail(DSPARK_ERR_UNSUPPORTED, "%s: group_size=%d (64)", what, group_size);
+  if ((c_dtype != DSPARK_DTYPE_BF16 && c_dtype != DSPARK_DTYPE_F16) ||
+      (x_dtype != DSPARK_DTYPE_BF16 && x_dtype != DSPARK_DTYPE_F16 && x_dtype != DSPARK_DTYPE_F32))
+    return fail(DSPARK_ERR_UNSUPPORTED, "%s: rows of dtype %d, a cache of dtype %d", what, x_dtype, c_dtype);
+  if (D < 64 || D % 64 || D > 4096) return fail(DSPARK_ERR_SHAPE, "%s: head_dim %lld (a multiple of 64 up to 4096)", what, (long long)D);
+  if (B < 1 || H < 1 || B > 32767 || H > 32767 || 2 * B * H > 65535 || T < 1 || T > (1LL << 31) / D * 4)
+    return fail(DSPARK_ERR_SHAPE, "%s: B=%lld H=%lld rows=%lld", what, (long long)B, (long long)H, (long long)T);
+  const int es = x_dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  al = true;
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i] || !words[i] || !scales[i] || !biases[i]) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+    if (!aligned(x[i], es) || !aligned(words[i], 4) || !aligned(scales[i], 2) || !aligned(biases[i], 2))
+      return fail(DSPARK_ERR_ALIGN, "%s: tensors need the alignment of their type", what);
+    const int64_t *xs = x_strides + 3 * i, *ws = w_strides + 3 * i, *ss = s_strides + 3 * i;
+    al = al && aligned(x[i], 16) && aligned(words[i], 8);
+    for (int j = 0; j < 3; ++j) al = al && xs[j] % (16 / es) == 0 && ws[j] % 2 == 0;
+    a.side[i] = KvSide{static_cast<char*>(x[i]), xs[0], xs[1], xs[2], words[i], static_cast<u16*>(scales[i]),
+                       static_cast<u16*>(biases[i]), ws[0], ws[1], ws[2], ss[0], ss[1], ss[2]};
+  }
+  a.B = (int)B;
+  a.H = (int)H;
+  a.D8 = (int)(D / 8);
+  a.items = (u32)(T * (D / 8));
+  return DSPARK_OK;
+}
+
+template <bool WRITE>
+void launch_types(const KvArgs& a, int x_dtype, int c_dtype, int bits, bool al, hipStream_t s) {
+  constexpr int bf = DSPARK_DTYPE_BF16, hf = DSPARK_DTYPE_F16, f = DSPARK_DTYPE_F32;
+  const bool ch = c_dtype == hf;
+  if constexpr (WRITE) {
+    if (x_dtype == bf) ch ? launch_kv<WRITE, bf, hf>(a, bits, al, s) : launch_kv<WRITE, bf, bf>(a, bits, al, s);
+    else if (x_dtype == hf) ch ? launch_kv<WRITE, hf, hf>(a, bits, al, s) : launch_kv<WRITE, hf, bf>(a, bits, al, s);
+    else ch ? launch_kv<WRITE, f, hf>(a, bits, al, s) : launch_kv<WRITE, f, bf>(a, bits, al, s);
+  } else {
+    if (x_dtype == bf) ch ? launch_kv<WRITE, hf, bf>(a, bits, al, s) : launch_kv<WRITE, bf, bf>(a, bits, al, s);
+    else if (x_dtype == hf) ch ? launch_kv<WRITE, hf, hf>(a, bits, al, s) : launch_kv<WRITE, bf, hf>(a, bits, al, s);
+    else ch ? launch_kv<WRITE, hf, f>(a, bits, al, s) : launch_kv<WRITE, bf, f>(a, bits, al, s);
+  }
+}
+
+}  // namespace
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" int dspark_kv_quantize(int x_dtype, const void* const x[2], const int64_t x_strides[6], int cache_dtype,
+                                  uint32_t* const words[2], void* const scales[2], void* const biases[2],
+                                  const int64_t word_strides[6], const int64_t scale_strides[6], int64_t B, int64_t H,
+                                  int64_t T, int64_t D, int bits, int group_size, dspark_stream stream) {
+  KvArgs a;
+  bool al;
+  const int st = kv_args("kv_quantize", x_dtype, cache_dtype, const_cast<void* const*>(x), x_strides, words, scales, biases,
+                         word_strides, scale_strides, B, H, T, D, bits, group_size, a, al);
+  if (st) return st;
+  launch_types<true>(a, x_dtype, cache_dtype, bits, al, static_cast<hipStream_t>(stream));
+  return check_launch("kv_quantize");
+}
+
+extern "C" int dspark_kv_dequantize(int cache_dtype, const uint32_t* const words[2], const void* const scales[2],
+                                    const void* const biases[2], const int64_t word_strides[6],
+                                    const int64_t scale_strides[6], int64_t B, int64_t H, int64_t T, int64_t D, int bits,
+                                    int group_size, int out_dtype, void* const out[2], const int64_t out_strides[6],
+                                    dspark_stream stream) {
+  KvArgs a;
+  bool al;
+  const int st = kv_args("kv_dequantize", out_dtype, cache_dtype, out, out_strides, const_cast<uint32_t* const*>(words),
+                         const_cast<void* const*>(scales), const_cast<void* const*>(biases), word_strides, scale_strides, B,
+                         H, T, D, bits, group_size, a, al);
+  if (st) return st;
+  launch_types<false>(a, out_dtype, cache_dtype, bits, al, static_cast<hipStream_t>(stream));
+  return check_launch("kv_dequantize");
+}

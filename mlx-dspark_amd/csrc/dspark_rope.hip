@@ -1,0 +1,197 @@
+// Rotary positions of queries and keys in one launch (gfx950).
+//
+//   a_i = position * freqs_i,   (y1, y2) = scale * (x1 cos a_i - x2 sin a_i, x1 sin a_i + x2 cos a_i)
+// for the pairs (i, i + half) or, interleaved, (2i, 2i + 1) of a head's first 2 half values; the others
+// are copied. cos and sin of a position serve every head of its row: a workgroup forms them once for its
+// rows in LDS. The angle is reduced in fp64, in turns: at position 1e6 an fp32 product is off by 0.06 rad,
+// the fp64 one by 1e-10. The rotation is fp32, rounded once to the tensors' type.
+//
+// Bound by the bytes of x and y: 16 bytes a lane and access where addresses and strides allow, else one
+// value (the same code at a width of one).
+#include "dspark_common.h"
+
+namespace dspark {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeHalf = 128;                 // pairs of a head
+constexpr int kRopeTab = 512;                  // (cos, sin) pairs of a workgroup
+
+struct RopeSide {                              // queries or keys
+  const char* x;
+  char* y;
+  long xb, xh, xl, yb, yh, yl;                 // strides of batch, head, row
+};
+
+struct RopeArgs {
+  RopeSide s[2];
+  int heads0, heads;                           // of s[0], of both
+  int B, L, D, half, rows;                     // rows = B * L
+  int per;                                     // items of a head
+  int rot;                                     // of these, items that rotate
+  int tok;                                     // rows of a workgroup
+  const void* pos;
+  int pos64;
+  long pb, pl;                                 // strides of the positions
+  long pos0;                                   // without pos: row l stands at pos0 + l
+  const double* freqs;
+  float scale;
+};
+
+template <int DT> struct Elem;
+template <> struct Elem<DSPARK_DTYPE_BF16> {
+  using t = u16;
+  static __device__ __forceinline__ float get(u16 v) { return bf2f(v); }
+  static __device__ __forceinline__ u16 put(float v) { return f2bf(v); }
+};
+template <> struct Elem<DSPARK_DTYPE_F16> {
+  using t = u16;
+  static __device__ __forceinline__ float get(u16 v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ u16 put(float v) { return __builtin_bit_cast(u16, (_Float16)v); }
+};
+template <> struct Elem<DSPARK_DTYPE_F32> {
+  using t = float;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+// An item is W pairs (half layout: W values of each half; interleaved: the W values of W / 2 pairs, at
+// W = 1 one pair) or W copied values.
+template <int DT, int W, bool INTER>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::t;
+  using P = Pack<T, W>;
+  __shared__ float2 tab[kRopeTab];
+  const int r0 = blockIdx.x * a.tok, nr = min(a.tok, a.rows - r0);
+  for (int i = threadIdx.x; i < nr * a.half; i += kRopeThreads) {
+    const int r = r0 + i / a.half, f = i % a.half, b = r / a.L, l = r % a.L;
+    long p = a.pos0 + l;
+    if (a.pos) {
+      const long at = b * a.pb + l * a.pl;
+      p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : (long)static_cast<const int32_t*>(a.pos)[at];
+    }
+    const double turns = (double)p * (a.freqs[f] * 0.15915494309189535);
+    float sn, cs;
+    sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &sn, &cs);
+    tab[i] = make_float2(cs * a.scale, sn * a.scale);
+  }
+  __syncthreads();
+  const int per_row = a.heads * a.per, n = nr * per_row;
+  for (int i = blockIdx.y * kRopeThreads + threadIdx.x; i < n; i += gridDim.y * kRopeThreads) {
+    const int tr = i / per_row, j = i - tr * per_row;
+    int h = j / a.per;
+    const int c = j - h * a.per;
+    const int r = r0 + tr, b = r / a.L, l = r - b * a.L;
+    const int side = h >= a.heads0;
+    h -= side ? a.heads0 : 0;
+    const RopeSide& s = a.s[side];
+    const T* x = reinterpret_cast<const T*>(s.x) + b * s.xb + h * s.xh + l * s.xl;
+    T* y = reinterpret_cast<T*>(s.y) + b * s.yb + h * s.yh + l * s.yl;
+    const float2* t = tab + tr * a.half;
+    if (c >= a.rot) {                          // beyond the rotated part
+      const int d = 2 * a.half + (c - a.rot) * W;
+      *reinterpret_cast<P*>(y + d) = *reinterpret_cast<const P*>(x + d);
+    } else if constexpr (!INTER) {
+      const int d = c * W;
+      P x1 = *reinterpret_cast<const P*>(x + d), x2 = *reinterpret_cast<const P*>(x + d + a.half);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float2 cs = t[d + e];
+        const float u = E::get(x1.v[e]), v = E::get(x2.v[e]);
+        x1.v[e] = E::put(u * cs.x - v * cs.y);
+        x2.v[e] = E::put(u * cs.y + v * cs.x);
+      }
+      *reinterpret_cast<P*>(y + d) = x1;
+      *reinterpret_cast<P*>(y + d + a.half) = x2;
+    } else if constexpr (W == 1) {
+      const float2 cs = t[c];
+      const float u = E::get(x[2 * c]), v = E::get(x[2 * c + 1]);
+      y[2 * c] = E::put(u * cs.x - v * cs.y);
+      y[2 * c + 1] = E::put(u * cs.y + v * cs.x);
+    } else {
+      const int d = c * W;
+      P v = *reinterpret_cast<const P*>(x + d);
+#pragma unroll
+      for (int e = 0; e < W; e += 2) {
+        const float2 cs = t[(d + e) >> 1];
+        const float p = E::get(v.v[e]), q = E::get(v.v[e + 1]);
+        v.v[e] = E::put(p * cs.x - q * cs.y);
+        v.v[e + 1] = E::put(p * cs.y + q * cs.x);
+      }
+      *reinterpret_cast<P*>(y + d) = v;
+    }
+  }
+}
+
+template <int DT, int W>
+void launch_rope(RopeArgs a, bool inter, hipStream_t s) {
+  a.rot = inter ? (W == 1 ? a.half : 2 * a.half / W) : a.half / W;
+  a.per = a.rot + (a.D - 2 * a.half) / W;
+  // rows of a workgroup: a table of up to 512 (cos, sin), one row where there are few
+  a.tok = a.rows >= 1024 ? kRopeTab / kRopeHalf : 1;
+  const unsigned gx = (unsigned)((a.rows + a.tok - 1) / a.tok);
+  const unsigned most = (unsigned)((a.tok * a.heads * a.per + kRopeThreads - 1) / kRopeThreads);
+  const unsigned gy = gx >= 512 ? 1u : (most < 512 / gx ? most : (512 / gx ? 512 / gx : 1u));
+  if (inter) hipLaunchKernelGGL((rope_kernel<DT, W, true>), dim3(gx, gy), dim3(kRopeThreads), 0, s, a);
+  else hipLaunchKernelGGL((rope_kernel<DT, W, false>), dim3(gx, gy), dim3(kRopeThreads), 0, s, a);
+}
+
+}  // namespace
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" int dspark_rope(int dtype, const void* q, const int64_t q_strides[3], int64_t Hq, const void* k,
+                           const int64_t k_strides[3], int64_t Hk, int64_t B, int64_t L, int64_t D, int64_t dims,
+                           int interleaved, const double* freqs, float scale, const void* positions, int positions_i64,
+                           const int64_t position_strides[2], int64_t pos0, void* q_out, const int64_t q_out_strides[3],
+                           void* k_out, const int64_t k_out_strides[3], dspark_stream stream) {
+  const char* what = "rope";
+  if (!q || !q_out || !q_strides || !q_out_strides || !freqs || (positions && !position_strides) ||
+      (Hk > 0 && (!k || !k_out || !k_strides || !k_out_strides)))
+    return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  if (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F16 && dtype != DSPARK_DTYPE_F32)
+    return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+  if (D < 2 || D > 1024 || dims < 2 || dims > 2 * kRopeHalf || dims % 2 || dims > D)
+    return fail(DSPARK_ERR_SHAPE, "%s: head_dim %lld (2..1024), rotated part %lld (even, up to it and to 256)", what, (long long)D, (long long)dims);
+  if (B < 1 || L < 1 || B * L > (1 << 24) || B > (1 << 24) || L > (1 << 24) || Hq < 1 || Hk < 0 || Hq + Hk > 4096)
+    return fail(DSPARK_ERR_SHAPE, "%s: B=%lld L=%lld Hq=%lld Hk=%lld", what, (long long)B, (long long)L, (long long)Hq, (long long)Hk);
+  const int64_t es = dtype == DSPARK_DTYPE_F32 ? 4 : 2, wide = 16 / es;
+  RopeArgs a = {};
+  bool vec = D % wide == 0 && (interleaved ? dims : dims / 2) % wide == 0;
+  for (int i = 0; i < (Hk ? 2 : 1); ++i) {
+    const void* x = i ? k : q;
+    void* y = i ? k_out : q_out;
+    const int64_t *xs = i ? k_strides : q_strides, *ys = i ? k_out_strides : q_out_strides;
+    if (!aligned(x, es) || !aligned(y, es)) return fail(DSPARK_ERR_ALIGN, "%s: tensors need the alignment of their type", what);
+    vec = vec && aligned(x, 16) && aligned(y, 16);
+    for (int j = 0; j < 3; ++j) vec = vec && xs[j] % wide == 0 && ys[j] % wide == 0;
+    a.s[i] = RopeSide{static_cast<const char*>(x), static_cast<char*>(y), xs[0], xs[1], xs[2], ys[0], ys[1], ys[2]};
+  }
+  a.heads0 = (int)Hq;
+  a.heads = (int)(Hq + Hk);
+  a.B = (int)B;
+  a.L = (int)L;
+  a.D = (int)D;
+  a.half = (int)(dims / 2);
+  a.rows = (int)(B * L);
+  a.pos = positions;
+  a.pos64 = positions_i64;
+  a.pb = positions ? position_strides[0] : 0;
+  a.pl = positions ? position_strides[1] : 0;
+  a.pos0 = pos0;
+  a.freqs = freqs;
+  a.scale = scale;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool in = interleaved != 0;
+  if (dtype == DSPARK_DTYPE_BF16) vec ? launch_rope<DSPARK_DTYPE_BF16, 8>(a, in, s) : launch_rope<DSPARK_DTYPE_BF16, 1>(a, in, s);
+  else if (dtype == DSPARK_DTYPE_F16) vec ? launch_rope<DSPARK_DTYPE_F16, 8>(a, in, s) : launch_rope<DSPARK_DTYPE_F16, 1>(a, in, s);
+  else vec ? launch_rope<DSPARK_DTYPE_F32, 4>(a, in, s) : launch_rope<DSPARK_DTYPE_F32, 1>(a, in, s);
+  return check_launch(what);
+}

@@ -23,6 +23,7 @@ c_float = ctypes.c_float
 c_double = ctypes.c_double
 c_char_p = ctypes.c_char_p
 c_i64_p = ctypes.POINTER(ctypes.c_int64)
+c_void_pp = ctypes.POINTER(ctypes.c_void_p)
 
 STATUS = {
     0: "DSPARK_OK",
@@ -190,6 +191,13 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_speculative_verify": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64,
                                           c_i64, c_void_p, c_void_p, c_int, c_double, c_i64, c_double, c_void_p,
                                           c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "dspark_rope": (c_int, [c_int, c_void_p, c_i64_p, c_i64, c_void_p, c_i64_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
+                            c_void_p, c_float, c_void_p, c_int, c_i64_p, c_i64, c_void_p, c_i64_p, c_void_p, c_i64_p,
+                            c_void_p]),
+    "dspark_kv_quantize": (c_int, [c_int, c_void_pp, c_i64_p, c_int, c_void_pp, c_void_pp, c_void_pp, c_i64_p, c_i64_p,
+                                   c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_void_p]),
+    "dspark_kv_dequantize": (c_int, [c_int, c_void_pp, c_void_pp, c_void_pp, c_i64_p, c_i64_p, c_i64, c_i64, c_i64, c_i64,
+                                     c_int, c_int, c_int, c_void_pp, c_i64_p, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -101,6 +101,22 @@ def scaled_dot_product_attention(q, k, v, *, scale, mask=None, sinks=None, **kw)
 STOCK = scaled_dot_product_attention
 
 
+def read_back_kernel(q, q_keys, q_values, bits, group_size) -> bool:
+    """Whether ``ops.dequantize_kv`` reads these triples back (the same bits in one launch): cache views
+    on q's GPU as the quantized caches keep them, nothing recording gradients."""
+    ts = (*q_keys, *q_values)
+    if not all(isinstance(t, torch.Tensor) for t in (q, *ts)) or not ops.eager_inference(q, *ts):
+        return False
+    (kw, ks, kb), (vw, vs, vb) = q_keys, q_values
+    if kw.dim() != 4 or bits not in ops.KV_BITS or group_size != ops.GROUP or kw.shape[3] * 32 // bits % ops.GROUP:
+        return False
+    groups = (*kw.shape[:3], kw.shape[3] * 32 // bits // ops.GROUP)
+    return (kw.numel() > 0 and kw.dtype in (torch.int32, torch.uint32) and vw.dtype == kw.dtype and vw.shape == kw.shape
+            and ks.dtype in ops.KV_CACHE_DTYPES and 2 * kw.shape[0] * kw.shape[1] <= 65535
+            and all(t.dtype == ks.dtype and tuple(t.shape) == groups for t in (ks, kb, vs, vb))
+            and all(t.stride(3) == 1 for t in ts) and ks.stride() == kb.stride() and vs.stride() == vb.stride())
+
+
 def quantized_scaled_dot_product_attention(q, q_keys, q_values, *, scale, mask=None, group_size: int = 64,
                                            bits: int = 8):
     """Attention over quantized K/V triples (words, scales, biases), the helper mlx-lm's
@@ -116,7 +132,11 @@ def quantized_scaled_dot_product_attention(q, q_keys, q_values, *, scale, mask=N
         g = vals.reshape(*lead, -1, group_size)
         return (g * s.to(torch.float32).unsqueeze(-1) + b.to(torch.float32).unsqueeze(-1)).reshape(*lead, -1)
 
-    return _stock_sdpa(q.to(torch.float32), deq(q_keys), deq(q_values), scale=scale, mask=mask).to(q.dtype)
+    if read_back_kernel(q, q_keys, q_values, bits, group_size):
+        k, v = ops.dequantize_kv(q_keys, q_values, bits=bits, group_size=group_size)
+    else:
+        k, v = deq(q_keys), deq(q_values)
+    return _stock_sdpa(q.to(torch.float32), k, v, scale=scale, mask=mask).to(q.dtype)
 
 
 QUANTIZED_STOCK = quantized_scaled_dot_product_attention

@@ -17,6 +17,8 @@ from __future__ import annotations
 
 import torch
 
+from . import ops
+
 STEP = 256
 
 
@@ -127,11 +129,26 @@ class QuantizedKVCache:
         t = keys.shape[2]
         if self.offset + t > self.capacity:
             self._grow(self.offset + t)
-        for dst, src in ((self.keys, keys), (self.values, values)):
-            for buf, part in zip(dst, quantize_rows(src, self.bits, self.group_size, self.dtype)):
-                buf[:, :, self.offset:self.offset + t] = part
+        if self._kernel(keys, values):
+            rows = lambda trip: tuple(a[:, :, self.offset:self.offset + t] for a in trip)
+            ops.quantize_kv(keys, values, rows(self.keys), rows(self.values), bits=self.bits, group_size=self.group_size)
+        else:
+            for dst, src in ((self.keys, keys), (self.values, values)):
+                for buf, part in zip(dst, quantize_rows(src, self.bits, self.group_size, self.dtype)):
+                    buf[:, :, self.offset:self.offset + t] = part
         self.offset += t
         return self.fetch()
+
+    def _kernel(self, keys: torch.Tensor, values: torch.Tensor) -> bool:
+        """Whether ``ops.quantize_kv`` writes these rows (the same bits in one launch): rows and cache on
+        one GPU, whole rows of the cache's own shape, nothing recording gradients."""
+        if not ops.eager_inference(keys, values, *self.keys, *self.values):
+            return False
+        return (keys.shape == values.shape and keys.dim() == 4 and keys.dtype == values.dtype
+                and keys.dtype in ops.DEQUANT_DTYPES and self.dtype in ops.KV_CACHE_DTYPES and keys.shape[2] > 0
+                and tuple(keys.shape[:2]) == (self.batch, self.kv_heads) and keys.shape[3] == self.head_dim
+                and 2 * self.batch * self.kv_heads <= 65535
+                and all(t.device == keys.device for t in (values, *self.keys, *self.values)))
 
     def reserve(self, t: int) -> None:
         """Make room for ``t`` more rows at ``offset`` (a kernel then writes them in place)."""

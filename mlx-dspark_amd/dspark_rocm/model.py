@@ -28,12 +28,13 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 from torch import nn
 
 from . import _lib, fast, ops
+from . import rope as rope_tables
 from ._lib import load as _lib_load
 from .kv_cache import KVCache, QuantizedKVCache
 from .nn import QuantizedLinear
@@ -52,6 +53,20 @@ class ModelArgs:
     rope_theta: float = 1e6
     bits: int = 8
     lm_head_bits: int = 8
+    rope_scaling: dict | None = field(default=None, hash=False)     # rope.frequencies' scaling
+    rope_traditional: bool = False      # pairs (2i, 2i + 1) instead of (i, i + dims / 2)
+    rope_dims: int | None = None        # values of a head that are rotated (None: all)
+
+    @property
+    def fused_rope(self) -> bool:
+        """Whether the fused q/k-norm + RoPE + cache-write kernel rotates as this target does: half split,
+        the whole head, frequencies of the base alone."""
+        kind = (self.rope_scaling or {}).get("rope_type", (self.rope_scaling or {}).get("type", "default"))
+        return kind == "default" and not self.rope_traditional and self.rope_dims in (None, self.head_dim)
+
+    def rope_table(self, device) -> tuple[torch.Tensor, float]:
+        """The frequencies (fp64, on ``device``) and the factor of the rotated values."""
+        return rope_tables.frequencies(self.rope_dims or self.head_dim, self.rope_theta, self.rope_scaling, device=device)
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -109,6 +124,7 @@ class Attention(nn.Module):
         self.q_proj, self.k_proj, self.v_proj, self.o_proj = q, k, v, o
         self.register_buffer("q_norm", q_norm)
         self.register_buffer("k_norm", k_norm)
+        self._rope = None               # (frequencies, factor) of a target that needs its table
 
     def forward(self, x: torch.Tensor, cache: KVCache) -> torch.Tensor:
         a = self.args
@@ -127,8 +143,7 @@ class Attention(nn.Module):
             q = rms_norm(q.reshape(B, L, hq, d), self.q_norm, a.rms_norm_eps).transpose(1, 2)
             k = rms_norm(k.reshape(B, L, hk, d), self.k_norm, a.rms_norm_eps).transpose(1, 2)
             v = v.reshape(B, L, hk, d).transpose(1, 2)
-            q = rope(q, cache.offset, a.rope_theta)
-            k = rope(k, cache.offset, a.rope_theta)
+            q, k = self._rotate(q, k, cache.offset)
             keys, values = cache.update_and_fetch(k, v)
         mask = "causal" if L > 1 else None
         if hasattr(cache, "bits"):
@@ -141,12 +156,24 @@ class Attention(nn.Module):
             out = fast.scaled_dot_product_attention(q.contiguous(), keys, values, scale=d ** -0.5, mask=mask)
         return self.o_proj(out.transpose(1, 2).reshape(B, L, hq * d))
 
+    def _rotate(self, q: torch.Tensor, k: torch.Tensor, pos0: int):
+        """q and k [B, H, L, D] at positions pos0 ..; targets the fused kernel does not rotate for go by
+        their frequency table, in one launch on the GPU."""
+        a = self.args
+        if a.fused_rope:
+            return rope(q, pos0, a.rope_theta), rope(k, pos0, a.rope_theta)
+        if self._rope is None or self._rope[0].device != q.device:
+            self._rope = a.rope_table(q.device)
+        freqs, scale = self._rope
+        if ops.eager_inference(q, k) and q.dtype in ops.ROPE_DTYPES:
+            return ops.rope(q, k, freqs, pos0, interleaved=a.rope_traditional, scale=scale)
+        return tuple(rope_tables.rotate(t, freqs, pos0, interleaved=a.rope_traditional, scale=scale) for t in (q, k))
 
     def _fused_kv(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache) -> bool:
         """Whether one launch norms and rotates q and k and writes k and v into a plain bf16 cache."""
         a = self.args
         hq, hk, d = a.num_attention_heads, a.num_key_value_heads, a.head_dim
-        if type(cache) is not KVCache or q.dim() != 3 or q.shape[0] != 1 or d % 8 or not 8 <= d <= 256:
+        if not a.fused_rope or type(cache) is not KVCache or q.dim() != 3 or q.shape[0] != 1 or d % 8 or not 8 <= d <= 256:
             return False
         L = q.shape[1]
         return (tuple(q.shape) == (1, L, hq * d) and tuple(k.shape) == tuple(v.shape) == (1, L, hk * d)
@@ -318,6 +345,12 @@ class VerifyEngine:
         # residual add that forms it (no copy), [max_rows, n_tap * H]; see set_tap
         self.tap: tuple[int, ...] = ()
         self.fused = e(max_rows, 0)
+        # targets whose rotation the fused kernel does not have: the table, and rows between the norm, the
+        # rotation and the cache
+        self.rope = None
+        if not a.fused_rope:
+            self.rope = a.rope_table(dev)
+            self.qn, self.kn = e(max_rows, hq * d), e(max_rows, hk * d)
         self.attn_ws = torch.empty(max(ops.attention_workspace_bound(1, hq, hk, d, max_rows), 16), dtype=torch.uint8,
                                    device=dev)
 
@@ -398,7 +431,7 @@ class VerifyEngine:
         caller's to make (:meth:`_native_layers`)."""
         a, m = self.args, self.model
         head = self._packed.get(id(m.lm_head))
-        if head is None or (head.n, head.k) != (a.vocab_size, a.hidden_size) or len(cache) != len(m.layers):
+        if self.rope is not None or head is None or (head.n, head.k) != (a.vocab_size, a.hidden_size) or len(cache) != len(m.layers):
             return False
         if not cache or not self._norm_fits(m.norm, a.hidden_size):
             return False
@@ -501,20 +534,24 @@ class VerifyEngine:
             self._qmm(y, [at.q_proj, at.k_proj, at.v_proj], [self.q[:M], self.k[:M], self.v[:M]])
             att = self.att[:M]
             ostr = (M * hq * d, d, hq * d)
-            if hasattr(c, "bits"):      # quantized cache: rows quantized as written, attention on the triples
+            if self.rope is not None:
+                self._rotate_and_write(M, at, c, pos0, qatt)
+            elif hasattr(c, "bits"):    # quantized cache: rows quantized as written
                 ops.qk_norm_rope_kv_quantized(self.q[:M], self.k[:M], self.v[:M], at.q_norm, at.k_norm, heads=hq,
                                               kv_heads=hk, head_dim=d, eps=eps, rope_base=a.rope_theta, pos0=pos0,
                                               q_out=qatt[0], k_cache=tuple(t[0] for t in c.keys),
                                               v_cache=tuple(t[0] for t in c.values), bits=c.bits,
                                               group_size=c.group_size)
+            else:
+                ops.qk_norm_rope_kv(self.q[:M], self.k[:M], self.v[:M], at.q_norm, at.k_norm, heads=hq,
+                                    kv_heads=hk, head_dim=d, eps=eps, rope_base=a.rope_theta, pos0=pos0,
+                                    q_out=qatt[0], k_cache=c.keys[0], v_cache=c.values[0])
+            if hasattr(c, "bits"):      # attention on the triples
                 ops.verify_attention_quantized(qatt, tuple(t[:, :, :L] for t in c.keys),
                                                tuple(t[:, :, :L] for t in c.values), scale=d ** -0.5, causal=M > 1,
                                                bits=c.bits, group_size=c.group_size, out=att, out_strides=ostr,
                                                workspace=self.attn_ws)
             else:
-                ops.qk_norm_rope_kv(self.q[:M], self.k[:M], self.v[:M], at.q_norm, at.k_norm, heads=hq,
-                                    kv_heads=hk, head_dim=d, eps=eps, rope_base=a.rope_theta, pos0=pos0,
-                                    q_out=qatt[0], k_cache=c.keys[0], v_cache=c.values[0])
                 ops.verify_attention_into(qatt, c.keys[:, :, :L], c.values[:, :, :L], att, ostr, scale=d ** -0.5,
                                           causal=M > 1, workspace=self.attn_ws)
             self._qmm(att, [at.o_proj], [r])
@@ -529,6 +566,24 @@ class VerifyEngine:
             self._qmm(self.hm[:M], [mlp.down_proj], [r])
         ops.rmsnorm(hcur, m.norm, eps, residual=r, h_out=stream_out(len(m.layers) - 1), out=y)
         self._qmm(y, [m.lm_head], [self.logits[:M]])
+
+    def _rotate_and_write(self, M: int, at: Attention, c, pos0: int, qatt: torch.Tensor) -> None:
+        """q/k norm, rotation by the table and the cache write of M rows, op by op."""
+        a = self.args
+        hq, hk, d, eps = a.num_attention_heads, a.num_key_value_heads, a.head_dim, a.rms_norm_eps
+        freqs, scale = self.rope
+        heads = lambda t, h: t[:M].view(1, M, h, d).transpose(1, 2)
+        rows = lambda trip: tuple(t[:, :, pos0:pos0 + M] for t in trip)
+        for x, y, w, h in ((self.q, self.qn, at.q_norm, hq), (self.k, self.kn, at.k_norm, hk)):
+            ops.rmsnorm(x[:M].view(M * h, d), w, eps, out=y[:M].view(M * h, d))
+        q, k, v = heads(self.qn, hq), heads(self.kn, hk), heads(self.v, hk)
+        quantized = hasattr(c, "bits")
+        ops.rope(q, k, freqs, pos0, interleaved=a.rope_traditional, scale=scale, q_out=qatt,
+                 k_out=k if quantized else c.keys[:, :, pos0:pos0 + M])
+        if quantized:
+            ops.quantize_kv(k, v, rows(c.keys), rows(c.values), bits=c.bits, group_size=c.group_size)
+        else:
+            c.values[:, :, pos0:pos0 + M].copy_(v)
 
 
 class Target:
@@ -627,6 +682,47 @@ class Target:
         self.rollback(cache, len(draft) - n)
         fused = self._fused_rows(M, tap)
         return n, list(draft[:n]) + [int(tt[n])], None if fused is None else fused[:, :n + 1]
+
+
+    def sampled_round(self, pending: int, draft: list[int], cache: list[KVCache], tap=None, *,
+                      draft_probs: torch.Tensor | None = None, uniforms: torch.Tensor | None = None,
+                      generator: torch.Generator | None = None, temperature: float = 1.0, top_k: int = 0,
+                      top_p: float = 1.0):
+        """One speculative round at a temperature (the reference's sampling accept, generate.py): verify
+        [pending] + draft, accept on the device by the rule of ``ops.speculative_verify``, one host read,
+        rollback of the rejected rows. Returns what :meth:`greedy_round` does; the token after the accepted
+        drafts is drawn so that the committed tokens follow the target's (truncated) distribution.
+
+        ``draft_probs`` fp32 [m, V]: what each draft was sampled from (``ops.sampling_probs`` of the
+        drafter's logits); None for drafts without probabilities. ``uniforms`` [m + 1] in [0, 1), else
+        drawn with ``generator`` on the engine's device."""
+        e = self.engine
+        m = len(draft)
+        M = 1 + m
+        if M > self.max_rows:
+            raise ValueError(f"verify width {M} > {self.max_rows}")
+        dev = e.ids.device
+        V = self.model.args.vocab_size
+        # whatever the round would refuse is refused before the caches take the rows
+        if not all(0 <= int(t) < V for t in (pending, *draft)):
+            raise ValueError(f"tokens outside the vocabulary of {V}: {[pending, *draft]}")
+        if uniforms is None:
+            uniforms = torch.rand(M, generator=generator, device=dev)
+        elif uniforms.dtype not in (torch.float32, torch.float64) or uniforms.numel() != M:
+            raise ValueError(f"uniforms: {M} fp32 or fp64 numbers, got {uniforms.dtype} {list(uniforms.shape)}")
+        if draft_probs is not None and (draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (m, V)
+                                        or draft_probs.requires_grad):
+            raise ValueError(f"draft_probs: fp32 [{m}, {V}] without gradients, got {draft_probs.dtype} {list(draft_probs.shape)}")
+        ops.check_sampler(temperature, top_k, top_p)
+        probs = None if draft_probs is None else draft_probs.to(dev)[None]
+        logits, fused = self.verify(torch.tensor([[pending] + list(draft)], dtype=torch.int64), cache, tap)
+        _, tokens, _ = ops.speculative_verify(logits, torch.tensor([list(draft)], dtype=torch.int32, device=dev).view(1, m),
+                                              uniforms.to(dev).view(1, M), draft_probs=probs, temperature=temperature,
+                                              top_k=top_k, top_p=top_p)
+        out = [t for t in tokens[0].tolist() if t >= 0]         # the round's one host read
+        n = len(out) - 1
+        self.rollback(cache, m - n)
+        return n, out, None if fused is None else fused[:, :n + 1]
 
 
 def prefill_plain(target: Target, ids: torch.Tensor, cache: list[KVCache], chunk: int | None = None,

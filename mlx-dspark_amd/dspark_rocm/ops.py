@@ -897,7 +897,8 @@ def _one_device(what: str, first: torch.Tensor, *ts) -> None:
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
 
 
-def _sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
+def check_sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
+    """The sampler's settings as the kernels take them; ValueError where they refuse them."""
     t, k, p = float(temperature), int(top_k or 0), float(top_p)
     if not 1e-30 <= t <= 1e30:
         raise ValueError(f"temperature={temperature}: a positive number (greedy rounds: argmax_accept)")
@@ -938,7 +939,7 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"sampling_probs: logits {tuple(logits.shape)}")
     _no_autograd("sampling_probs", logits)
-    t, k, p = _sampler(temperature, top_k, top_p)
+    t, k, p = check_sampler(temperature, top_k, top_p)
     V = logits.shape[-1]
     x = logits.reshape(-1, V)
     if x.stride(1) != 1 or x.stride(0) < V:
@@ -992,7 +993,7 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
         raise ValueError(f"{what}: {m} drafts (up to 255)")
     if uniforms.dtype not in (torch.float32, torch.float64) or tuple(uniforms.shape) != (B, R):
         raise ValueError(f"{what}: uniforms must be fp32 or fp64 [{B}, {R}], got {uniforms.dtype} {list(uniforms.shape)}")
-    t, k, p = _sampler(temperature, top_k, top_p)
+    t, k, p = check_sampler(temperature, top_k, top_p)
     draft = _ints(what, "draft", draft, (B, m))
     q = q_seq = q_row = 0
     if draft_probs is not None:
@@ -1019,3 +1020,169 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
                       int(u.dtype == torch.float64), t, k, p, n.data_ptr(), tokens.data_ptr(), draft_p.data_ptr(),
                       ws.data_ptr(), ws.numel() * ws.element_size(), _stream(x))
     return n, tokens, draft_p
+
+
+# ---------------------------------------------------------------------------- rotary positions, quantized cache rows
+
+_I64x2, _I64x6, _Ptrx2 = ctypes.c_int64 * 2, ctypes.c_int64 * 6, ctypes.c_void_p * 2
+ROPE_DTYPES = DEQUANT_DTYPES
+
+
+def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors of non-negative strides meet."""
+    end = lambda t: t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+def _no_repeats(what: str, out: torch.Tensor) -> None:
+    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{what}: the output is an expanded view ({list(out.shape)}, strides {list(out.stride())})")
+
+
+def _rope_out(name: str, x: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.dtype != x.dtype or out.shape != x.shape or out.stride(3) != 1:
+        raise ValueError(f"rope: {name} must be {x.dtype} {list(x.shape)} with unit last stride")
+    _no_repeats("rope", out)
+    if _spans_meet(x, out) and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()):
+        raise ValueError(f"rope: {name} overlaps its input (in place: the same view)")
+    return out
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions, *, interleaved: bool = False,
+         scale: float = 1.0, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotary positions of queries [B, Hq, L, D] and keys [B, Hk, L, D] (or None) in one launch ->
+    ``(q, k)`` rotated. bf16, fp16 or fp32, any batch / head / row strides, unit stride along D.
+
+    ``freqs`` fp64 [dims / 2] (:func:`dspark_rocm.rope.frequencies`): radians a position of the pairs
+    (i, i + dims / 2), or (2i, 2i + 1) when ``interleaved``, of a head's first ``dims`` values, which
+    ``scale`` multiplies; the rest is copied. ``positions``: an int (row l stands at ``positions + l``), or
+    an int32 / int64 tensor [L] or [B or 1, L or 1] with the position of every row, as tree rows need. The
+    angle is reduced in fp64; one rounding to the tensors' type. ``q_out`` / ``k_out``: where to write,
+    e.g. a cache's rows, or q and k themselves."""
+    _one_device("rope", q, k, freqs, q_out, k_out)
+    dt = ROPE_DTYPES.get(q.dtype)
+    if dt is None or (k is not None and k.dtype != q.dtype):
+        raise TypeError(f"rope: q {q.dtype}, k {None if k is None else k.dtype} (one of bfloat16, float16, float32)")
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], *q.shape[2:]))):
+        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(q.shape)} and {None if k is None else list(k.shape)}")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= min(128, q.shape[3] // 2):
+        raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(freqs.shape)}")
+    if k is None and k_out is not None:
+        raise ValueError("rope: k_out without k")
+    _no_autograd("rope", q, *(() if k is None else (k,)))
+    B, Hq, L, D = q.shape
+    freqs = freqs.contiguous()
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    pos, pos64, ps, pos0 = None, 0, None, 0
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device or positions.dim() not in (1, 2):
+            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L] on {q.device}, got {positions.dtype} {list(positions.shape)}")
+        try:
+            at = positions.expand(B, L)
+        except RuntimeError:
+            raise ValueError(f"rope: positions {list(positions.shape)} for {B} sequences of {L} rows") from None
+        pos, pos64, ps = positions.data_ptr(), int(positions.dtype == torch.int64), _I64x2(at.stride(0), at.stride(1))
+    else:
+        pos0 = int(positions)
+    q_out = _rope_out("q_out", q, q_out)
+    if k is not None:
+        k_out = _rope_out("k_out", k, k_out)
+    if q.numel() or (k is not None and k.numel()):
+        Hk = 0 if k is None else k.shape[1]
+        with _on_device(q.device):
+            _lib.call("dspark_rope", dt, q.data_ptr(), _i64x3(q), Hq, k.data_ptr() if Hk else None, _i64x3(k) if Hk else None,
+                      Hk, B, L, D, 2 * freqs.numel(), int(bool(interleaved)), freqs.data_ptr(), float(scale), pos, pos64, ps,
+                      pos0, q_out.data_ptr(), _i64x3(q_out), k_out.data_ptr() if Hk else None, _i64x3(k_out) if Hk else None,
+                      _stream(q))
+    return q_out, k_out
+
+
+KV_CACHE_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _kv_pair(what: str, keys, values, bits: int, group_size: int, shape=None):
+    """Checks of a (words, scales, biases) pair of cache views; (B, H, T, D), the type's code and the
+    argument arrays the C ABI takes."""
+    if bits not in KV_BITS or group_size != GROUP:
+        raise ValueError(f"{what}: bits={bits} (4 or 8), group_size={group_size} (64)")
+    kw, ks, kb = keys
+    vw, vs, vb = values
+    if kw.dim() != 4:
+        raise ValueError(f"{what}: words must be [B, H, rows, D * bits / 32], got {list(kw.shape)}")
+    B, H, T, W = kw.shape
+    D = W * 32 // bits
+    if D % GROUP or D == 0 or (shape is not None and tuple(shape) != (B, H, T, D)):
+        raise ValueError(f"{what}: words {list(kw.shape)} at {bits} bits" + ("" if shape is None else f" for rows {list(shape)}"))
+    if ks.dtype not in KV_CACHE_DTYPES:
+        raise TypeError(f"{what}: scales {ks.dtype} (bfloat16 or float16)")
+    for w, s, b in ((kw, ks, kb), (vw, vs, vb)):
+        _require_packed(w)
+        if s.dtype != ks.dtype or b.dtype != ks.dtype:
+            raise TypeError(f"{what}: scales and biases of {ks.dtype}, {s.dtype} and {b.dtype}")
+        if w.shape != kw.shape or s.shape != (B, H, T, D // GROUP) or b.shape != s.shape:
+            raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
+        if w.stride(3) != 1 or s.stride(3) != 1 or s.stride() != b.stride():
+            raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
+    if 2 * B * H > 65535:
+        raise ValueError(f"{what}: {B} x {H} heads (up to 32767)")
+    strides = lambda a, b: _I64x6(*a.stride()[:3], *b.stride()[:3])
+    arrays = (_Ptrx2(kw.data_ptr(), vw.data_ptr()), _Ptrx2(ks.data_ptr(), vs.data_ptr()), _Ptrx2(kb.data_ptr(), vb.data_ptr()),
+              strides(kw, vw), strides(ks, vs))
+    return (B, H, T, D), KV_CACHE_DTYPES[ks.dtype], arrays
+
+
+def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bits: int, group_size: int = GROUP) -> None:
+    """Quantize ``keys`` / ``values`` [B, H, T, D] (bf16, fp16 or fp32, any strides) into the cache rows
+    ``k_rows`` / ``v_rows``: (words int32 [B, H, T, D*bits/32], scales [B, H, T, D/64], biases) views of a
+    quantized cache, scales in bf16 or fp16. The values of :func:`dspark_rocm.quant.quantize_rows`, bit for
+    bit (a group with a NaN gets a NaN scale and bias), both tensors in one launch."""
+    what = "quantize_kv"
+    _one_device(what, keys, values, *k_rows, *v_rows)
+    dt = DEQUANT_DTYPES.get(keys.dtype)
+    if dt is None or values.dtype != keys.dtype:
+        raise TypeError(f"{what}: rows {keys.dtype} and {values.dtype} (one of bfloat16, float16, float32)")
+    if keys.shape != values.shape:
+        raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)}")
+    _no_autograd(what, keys, values)
+    (B, H, T, D), cache_dt, (w, s, b, ws, ss) = _kv_pair(what, k_rows, v_rows, bits, group_size, keys.shape)
+    for t in (*k_rows, *v_rows):
+        _no_repeats(what, t)
+    if keys.stride(3) != 1:
+        keys = keys.contiguous()
+    if values.stride(3) != 1:
+        values = values.contiguous()
+    if B * H * T:
+        with _on_device(keys.device):
+            _lib.call("dspark_kv_quantize", dt, _Ptrx2(keys.data_ptr(), values.data_ptr()),
+                      _I64x6(*keys.stride()[:3], *values.stride()[:3]), cache_dt, w, s, b, ws, ss, B, H, T, D, bits,
+                      group_size, _stream(keys))
+
+
+def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: torch.dtype = torch.float32, out=None):
+    """A quantized cache (or rows of it) read back: the triples of :func:`quantize_kv` -> ``(keys, values)``
+    [B, H, T, D] of ``dtype``, ``scale * field + bias`` with an fp32 product rounded, then an fp32 sum
+    rounded, then rounded to ``dtype``; both tensors in one launch. ``out``: two tensors to write."""
+    what = "dequantize_kv"
+    kw = keys[0]
+    _one_device(what, *keys, *values, *(out or ()))
+    if dtype not in DEQUANT_DTYPES:
+        raise TypeError(f"{what}: dtype {dtype} (bfloat16, float16 or float32)")
+    (B, H, T, D), cache_dt, (w, s, b, ws, ss) = _kv_pair(what, keys, values, bits, group_size)
+    if out is None:
+        k, v = torch.empty((B, H, T, D), dtype=dtype, device=kw.device), torch.empty((B, H, T, D), dtype=dtype, device=kw.device)
+    else:
+        k, v = out
+        for t in (k, v):
+            if t.dtype != dtype or tuple(t.shape) != (B, H, T, D) or t.stride(3) != 1:
+                raise ValueError(f"{what}: out must be two {dtype} [{B}, {H}, {T}, {D}] with unit last stride")
+            _no_repeats(what, t)
+    if B * H * T:
+        with _on_device(kw.device):
+            _lib.call("dspark_kv_dequantize", cache_dt, w, s, b, ws, ss, B, H, T, D, bits, group_size, DEQUANT_DTYPES[dtype],
+                      _Ptrx2(k.data_ptr(), v.data_ptr()), _I64x6(*k.stride()[:3], *v.stride()[:3]), _stream(kw))
+    return k, v

@@ -97,5 +97,5 @@ def test_host_checks():
         ops.speculative_verify(x, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 3))
     for bad in (dict(temperature=0), dict(temperature=-1.0), dict(top_k=-3), dict(top_p=0.0), dict(top_p=1.01)):
         with pytest.raises(ValueError):
-            ops._sampler(**{**dict(temperature=1.0, top_k=0, top_p=1.0), **bad})
+            ops.check_sampler(**{**dict(temperature=1.0, top_k=0, top_p=1.0), **bad})
     assert ops.sampling_workspace_bytes(16, 151936, 1) > 16 * 297 * 12
