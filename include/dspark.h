@@ -601,9 +601,20 @@ int dspark_argmax_accept(const void* logits, int64_t ld, int64_t M, int64_t V, c
  */
 size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences);
 
-int dspark_sampling_probs(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V, double temperature,
-                          int64_t top_k, double top_p, float* out, int64_t ldo, void* workspace,
-                          size_t workspace_bytes, dspark_stream stream);
+typedef struct dspark_sampling_probs_args { /* every field is 8 bytes */
+  int64_t dtype;
+  const void* logits;
+  int64_t ld, rows, V;
+  double temperature;
+  int64_t top_k;
+  double top_p;
+  float* out;
+  int64_t ldo;
+  void* workspace;
+  int64_t workspace_bytes;
+} dspark_sampling_probs_args;
+
+int dspark_sampling_probs(const dspark_sampling_probs_args* args, dspark_stream stream);
 
 /*
  * The accept rule of a sampled round (speculative sampling) for a batch of sequences, with p_i the row
@@ -623,12 +634,27 @@ int dspark_sampling_probs(int dtype, const void* logits, int64_t ld, int64_t row
  * workspace >= dspark_sampling_workspace(sequences * (drafts + 1), V, sequences) bytes, 256-byte aligned,
  * of any content. The sampling counterpart of dspark_argmax_accept (generate.py's sampling accept).
  */
-int dspark_speculative_verify(int dtype, const void* logits, int64_t ld_seq, int64_t ld_row, int64_t sequences,
-                              int64_t drafts, int64_t V, const int32_t* draft, const float* draft_probs,
-                              int64_t q_seq, int64_t q_row, const int32_t* draft_lens, const void* uniforms,
-                              int uniforms_f64, double temperature, int64_t top_k, double top_p,
-                              int32_t* n_accepted, int32_t* tokens, float* draft_p, void* workspace,
-                              size_t workspace_bytes, dspark_stream stream);
+typedef struct dspark_speculative_verify_args { /* every field is 8 bytes */
+  int64_t dtype;
+  const void* logits;
+  int64_t ld_seq, ld_row, sequences, drafts, V;
+  const int32_t* draft;
+  const float* draft_probs;
+  int64_t q_seq, q_row;
+  const int32_t* draft_lens;
+  const void* uniforms;
+  int64_t uniforms_f64;
+  double temperature;
+  int64_t top_k;
+  double top_p;
+  int32_t* n_accepted;
+  int32_t* tokens;
+  float* draft_p;
+  void* workspace;
+  int64_t workspace_bytes;
+} dspark_speculative_verify_args;
+
+int dspark_speculative_verify(const dspark_speculative_verify_args* args, dspark_stream stream);
 
 /* ------------------------------------------------------------------ rotary positions, quantized cache rows */
 
@@ -646,15 +672,25 @@ int dspark_speculative_verify(int dtype, const void* logits, int64_t ld_seq, int
  * (traditional or not, dims below the head, offset and freqs arrays), which dspark_qk_norm_rope_kv fuses
  * for one layout.
  */
-int dspark_rope(int dtype, const void* q, const int64_t q_strides[3], int64_t Hq, const void* k,
-                const int64_t k_strides[3], int64_t Hk, int64_t B, int64_t L, int64_t D, int64_t dims, int interleaved,
-                const double* freqs, float scale, const void* positions, int positions_i64,
-                const int64_t position_strides[2], int64_t pos0, void* q_out, const int64_t q_out_strides[3], void* k_out,
-                const int64_t k_out_strides[3], dspark_stream stream);
+typedef struct dspark_rope_args { /* every field is 8 bytes; strides are (batch, head, row) */
+  int64_t dtype;
+  const void* q;
+  void* q_out;
+  int64_t q_strides[3], q_out_strides[3], Hq;
+  const void* k;
+  void* k_out;
+  int64_t k_strides[3], k_out_strides[3], Hk;
+  int64_t B, L, D, dims, interleaved;
+  const double* freqs;
+  double scale;
+  const void* positions;
+  int64_t positions_i64, position_strides[2], pos0;
+} dspark_rope_args;
+
+int dspark_rope(const dspark_rope_args* args, dspark_stream stream);
 
 /*
- * Rows into a quantized cache (mlx-lm QuantizedKVCache layout), keys and values in one launch. Of each two
- * arguments [0] is the keys', [1] the values'; strides are (batch, head, row) triples, keys then values.
+ * Rows into a quantized cache (mlx-lm QuantizedKVCache layout), keys and values in one launch.
  * Per group of 64 values of x [B, H, T, D] (bf16, fp16 or fp32), every step one fp32 operation:
  *   scale = (max - min) * fl(1 / (2^bits - 1)) and bias = min, rounded to cache_dtype (bf16 or fp16);
  *   field = clamp(round_half_even((x - bias) / scale), 0, 2^bits - 1), a scale of 0 dividing as 1
@@ -662,17 +698,24 @@ int dspark_rope(int dtype, const void* q, const int64_t q_strides[3], int64_t Hq
  * words uint32 [B, H, T, D * bits / 32], scales and biases [B, H, T, D / 64] (shared strides), unit stride
  * along the last dim: rows of a cache view. D % 64 == 0, group_size 64, 2 * B * H <= 65535.
  */
-int dspark_kv_quantize(int x_dtype, const void* const x[2], const int64_t x_strides[6], int cache_dtype,
-                       uint32_t* const words[2], void* const scales[2], void* const biases[2],
-                       const int64_t word_strides[6], const int64_t scale_strides[6], int64_t B, int64_t H, int64_t T,
-                       int64_t D, int bits, int group_size, dspark_stream stream);
+typedef struct dspark_kv_side { /* keys or values; strides are (batch, head, row) */
+  void* x;                      /* plain rows: read by dspark_kv_quantize, written by dspark_kv_dequantize */
+  int64_t x_strides[3];
+  uint32_t* words;
+  void* scales;
+  void* biases;
+  int64_t word_strides[3], scale_strides[3];
+} dspark_kv_side;
 
-/* Such rows read back: out = scale * field (rounded to fp32) + bias (rounded to fp32), rounded to
- * out_dtype (bf16, fp16 or fp32); the same arguments, out [B, H, T, D] with its own strides. */
-int dspark_kv_dequantize(int cache_dtype, const uint32_t* const words[2], const void* const scales[2],
-                         const void* const biases[2], const int64_t word_strides[6], const int64_t scale_strides[6],
-                         int64_t B, int64_t H, int64_t T, int64_t D, int bits, int group_size, int out_dtype,
-                         void* const out[2], const int64_t out_strides[6], dspark_stream stream);
+typedef struct dspark_kv_args { /* every field is 8 bytes */
+  int64_t x_dtype, cache_dtype, B, H, T, D, bits, group_size;
+  dspark_kv_side keys, values;
+} dspark_kv_args;
+
+int dspark_kv_quantize(const dspark_kv_args* args, dspark_stream stream);
+
+/* Such rows read back: x = scale * field (rounded to fp32) + bias (rounded to fp32), rounded to x_dtype. */
+int dspark_kv_dequantize(const dspark_kv_args* args, dspark_stream stream);
 
 #ifdef __cplusplus
 }

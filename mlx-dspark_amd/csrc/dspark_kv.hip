@@ -198,29 +198,29 @@ void launch_kv(const KvArgs& a, int bits, bool al, hipStream_t s) {
 }
 
 // The arguments both directions share; `al`: everything a wide access touches is aligned for it.
-int kv_args(const char* what, int x_dtype, int c_dtype, void* const x[2], const int64_t x_strides[6], uint32_t* const words[2],
-            void* const scales[2], void* const biases[2], const int64_t w_strides[6], const int64_t s_strides[6], int64_t B,
-            int64_t H, int64_t T, int64_t D, int bits, int group_size, KvArgs& a, bool& al) {
-  if (!x || !x_strides || !words || !scales || !biases || !w_strides || !s_strides) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-  if (bits != 4 && bits != 8) return fail(DSPARK_ERR_UNSUPPORTED, "%s: bits=%d (4 or 8)", what, bits);
-  if (group_size != 64) return fail(DSPARK_ERR_UNSUPPORTED, "%s: group_size=%d (64)", what, group_size);
-  if ((c_dtype != DSPARK_DTYPE_BF16 && c_dtype != DSPARK_DTYPE_F16) ||
-      (x_dtype != DSPARK_DTYPE_BF16 && x_dtype != DSPARK_DTYPE_F16 && x_dtype != DSPARK_DTYPE_F32))
-    return fail(DSPARK_ERR_UNSUPPORTED, "%s: rows of dtype %d, a cache of dtype %d", what, x_dtype, c_dtype);
+int kv_args(const char* what, const dspark_kv_args* p, KvArgs& a, bool& al) {
+  if (!p) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  const int64_t B = p->B, H = p->H, T = p->T, D = p->D, xdt = p->x_dtype, cdt = p->cache_dtype;
+  if (p->bits != 4 && p->bits != 8) return fail(DSPARK_ERR_UNSUPPORTED, "%s: bits=%lld (4 or 8)", what, (long long)p->bits);
+  if (p->group_size != 64) return fail(DSPARK_ERR_UNSUPPORTED, "%s: group_size=%lld (64)", what, (long long)p->group_size);
+  if ((cdt != DSPARK_DTYPE_BF16 && cdt != DSPARK_DTYPE_F16) ||
+      (xdt != DSPARK_DTYPE_BF16 && xdt != DSPARK_DTYPE_F16 && xdt != DSPARK_DTYPE_F32))
+    return fail(DSPARK_ERR_UNSUPPORTED, "%s: rows of dtype %lld, a cache of dtype %lld", what, (long long)xdt, (long long)cdt);
   if (D < 64 || D % 64 || D > 4096) return fail(DSPARK_ERR_SHAPE, "%s: head_dim %lld (a multiple of 64 up to 4096)", what, (long long)D);
   if (B < 1 || H < 1 || B > 32767 || H > 32767 || 2 * B * H > 65535 || T < 1 || T > (1LL << 31) / D * 4)
     return fail(DSPARK_ERR_SHAPE, "%s: B=%lld H=%lld rows=%lld", what, (long long)B, (long long)H, (long long)T);
-  const int es = x_dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  const int es = xdt == DSPARK_DTYPE_F32 ? 4 : 2;
   al = true;
   for (int i = 0; i < 2; ++i) {
-    if (!x[i] || !words[i] || !scales[i] || !biases[i]) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-    if (!aligned(x[i], es) || !aligned(words[i], 4) || !aligned(scales[i], 2) || !aligned(biases[i], 2))
+    const dspark_kv_side& k = i ? p->values : p->keys;
+    if (!k.x || !k.words || !k.scales || !k.biases) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+    if (!aligned(k.x, es) || !aligned(k.words, 4) || !aligned(k.scales, 2) || !aligned(k.biases, 2))
       return fail(DSPARK_ERR_ALIGN, "%s: tensors need the alignment of their type", what);
-    const int64_t *xs = x_strides + 3 * i, *ws = w_strides + 3 * i, *ss = s_strides + 3 * i;
-    al = al && aligned(x[i], 16) && aligned(words[i], 8);
-    for (int j = 0; j < 3; ++j) al = al && xs[j] % (16 / es) == 0 && ws[j] % 2 == 0;
-    a.side[i] = KvSide{static_cast<char*>(x[i]), xs[0], xs[1], xs[2], words[i], static_cast<u16*>(scales[i]),
-                       static_cast<u16*>(biases[i]), ws[0], ws[1], ws[2], ss[0], ss[1], ss[2]};
+    al = al && aligned(k.x, 16) && aligned(k.words, 8);
+    for (int j = 0; j < 3; ++j) al = al && k.x_strides[j] % (16 / es) == 0 && k.word_strides[j] % 2 == 0;
+    a.side[i] = KvSide{static_cast<char*>(k.x), k.x_strides[0], k.x_strides[1], k.x_strides[2], k.words,
+                       static_cast<u16*>(k.scales), static_cast<u16*>(k.biases), k.word_strides[0], k.word_strides[1],
+                       k.word_strides[2], k.scale_strides[0], k.scale_strides[1], k.scale_strides[2]};
   }
   a.B = (int)B;
   a.H = (int)H;
@@ -249,30 +249,20 @@ void launch_types(const KvArgs& a, int x_dtype, int c_dtype, int bits, bool al, 
 
 using namespace dspark;
 
-extern "C" int dspark_kv_quantize(int x_dtype, const void* const x[2], const int64_t x_strides[6], int cache_dtype,
-                                  uint32_t* const words[2], void* const scales[2], void* const biases[2],
-                                  const int64_t word_strides[6], const int64_t scale_strides[6], int64_t B, int64_t H,
-                                  int64_t T, int64_t D, int bits, int group_size, dspark_stream stream) {
+extern "C" int dspark_kv_quantize(const dspark_kv_args* p, dspark_stream stream) {
   KvArgs a;
   bool al;
-  const int st = kv_args("kv_quantize", x_dtype, cache_dtype, const_cast<void* const*>(x), x_strides, words, scales, biases,
-                         word_strides, scale_strides, B, H, T, D, bits, group_size, a, al);
+  const int st = kv_args("kv_quantize", p, a, al);
   if (st) return st;
-  launch_types<true>(a, x_dtype, cache_dtype, bits, al, static_cast<hipStream_t>(stream));
+  launch_types<true>(a, (int)p->x_dtype, (int)p->cache_dtype, (int)p->bits, al, static_cast<hipStream_t>(stream));
   return check_launch("kv_quantize");
 }
 
-extern "C" int dspark_kv_dequantize(int cache_dtype, const uint32_t* const words[2], const void* const scales[2],
-                                    const void* const biases[2], const int64_t word_strides[6],
-                                    const int64_t scale_strides[6], int64_t B, int64_t H, int64_t T, int64_t D, int bits,
-                                    int group_size, int out_dtype, void* const out[2], const int64_t out_strides[6],
-                                    dspark_stream stream) {
+extern "C" int dspark_kv_dequantize(const dspark_kv_args* p, dspark_stream stream) {
   KvArgs a;
   bool al;
-  const int st = kv_args("kv_dequantize", out_dtype, cache_dtype, out, out_strides, const_cast<uint32_t* const*>(words),
-                         const_cast<void* const*>(scales), const_cast<void* const*>(biases), word_strides, scale_strides, B,
-                         H, T, D, bits, group_size, a, al);
+  const int st = kv_args("kv_dequantize", p, a, al);
   if (st) return st;
-  launch_types<false>(a, out_dtype, cache_dtype, bits, al, static_cast<hipStream_t>(stream));
+  launch_types<false>(a, (int)p->x_dtype, (int)p->cache_dtype, (int)p->bits, al, static_cast<hipStream_t>(stream));
   return check_launch("kv_dequantize");
 }

@@ -26,7 +26,7 @@ struct RopeSide {                              // queries or keys
 struct RopeArgs {
   RopeSide s[2];
   int heads0, heads;                           // of s[0], of both
-  int B, L, D, half, rows;                     // rows = B * L
+  int L, D, half, rows;                        // rows = B * L
   int per;                                     // items of a head
   int rot;                                     // of these, items that rotate
   int tok;                                     // rows of a workgroup
@@ -147,28 +147,25 @@ void launch_rope(RopeArgs a, bool inter, hipStream_t s) {
 
 using namespace dspark;
 
-extern "C" int dspark_rope(int dtype, const void* q, const int64_t q_strides[3], int64_t Hq, const void* k,
-                           const int64_t k_strides[3], int64_t Hk, int64_t B, int64_t L, int64_t D, int64_t dims,
-                           int interleaved, const double* freqs, float scale, const void* positions, int positions_i64,
-                           const int64_t position_strides[2], int64_t pos0, void* q_out, const int64_t q_out_strides[3],
-                           void* k_out, const int64_t k_out_strides[3], dspark_stream stream) {
+extern "C" int dspark_rope(const dspark_rope_args* p, dspark_stream stream) {
   const char* what = "rope";
-  if (!q || !q_out || !q_strides || !q_out_strides || !freqs || (positions && !position_strides) ||
-      (Hk > 0 && (!k || !k_out || !k_strides || !k_out_strides)))
-    return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-  if (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F16 && dtype != DSPARK_DTYPE_F32)
-    return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+  if (!p || !p->q || !p->q_out || !p->freqs || (p->Hk > 0 && (!p->k || !p->k_out))) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  const int64_t dt = p->dtype, B = p->B, L = p->L, D = p->D, dims = p->dims, Hq = p->Hq, Hk = p->Hk;
+  if (dt != DSPARK_DTYPE_BF16 && dt != DSPARK_DTYPE_F16 && dt != DSPARK_DTYPE_F32)
+    return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %lld", what, (long long)dt);
   if (D < 2 || D > 1024 || dims < 2 || dims > 2 * kRopeHalf || dims % 2 || dims > D)
     return fail(DSPARK_ERR_SHAPE, "%s: head_dim %lld (2..1024), rotated part %lld (even, up to it and to 256)", what, (long long)D, (long long)dims);
-  if (B < 1 || L < 1 || B * L > (1 << 24) || B > (1 << 24) || L > (1 << 24) || Hq < 1 || Hk < 0 || Hq + Hk > 4096)
+  if (B < 1 || L < 1 || B > (1 << 24) || L > (1 << 24) || B * L > (1 << 24) || Hq < 1 || Hk < 0 || Hq > 4096 || Hk > 4096 ||
+      Hq + Hk > 4096)
     return fail(DSPARK_ERR_SHAPE, "%s: B=%lld L=%lld Hq=%lld Hk=%lld", what, (long long)B, (long long)L, (long long)Hq, (long long)Hk);
-  const int64_t es = dtype == DSPARK_DTYPE_F32 ? 4 : 2, wide = 16 / es;
+  const int64_t es = dt == DSPARK_DTYPE_F32 ? 4 : 2, wide = 16 / es;
+  const bool inter = p->interleaved != 0;
   RopeArgs a = {};
-  bool vec = D % wide == 0 && (interleaved ? dims : dims / 2) % wide == 0;
+  bool vec = D % wide == 0 && (inter ? dims : dims / 2) % wide == 0;
   for (int i = 0; i < (Hk ? 2 : 1); ++i) {
-    const void* x = i ? k : q;
-    void* y = i ? k_out : q_out;
-    const int64_t *xs = i ? k_strides : q_strides, *ys = i ? k_out_strides : q_out_strides;
+    const void* x = i ? p->k : p->q;
+    void* y = i ? p->k_out : p->q_out;
+    const int64_t *xs = i ? p->k_strides : p->q_strides, *ys = i ? p->k_out_strides : p->q_out_strides;
     if (!aligned(x, es) || !aligned(y, es)) return fail(DSPARK_ERR_ALIGN, "%s: tensors need the alignment of their type", what);
     vec = vec && aligned(x, 16) && aligned(y, 16);
     for (int j = 0; j < 3; ++j) vec = vec && xs[j] % wide == 0 && ys[j] % wide == 0;
@@ -176,22 +173,20 @@ extern "C" int dspark_rope(int dtype, const void* q, const int64_t q_strides[3],
   }
   a.heads0 = (int)Hq;
   a.heads = (int)(Hq + Hk);
-  a.B = (int)B;
   a.L = (int)L;
   a.D = (int)D;
   a.half = (int)(dims / 2);
   a.rows = (int)(B * L);
-  a.pos = positions;
-  a.pos64 = positions_i64;
-  a.pb = positions ? position_strides[0] : 0;
-  a.pl = positions ? position_strides[1] : 0;
-  a.pos0 = pos0;
-  a.freqs = freqs;
-  a.scale = scale;
+  a.pos = p->positions;
+  a.pos64 = p->positions_i64 != 0;
+  a.pb = p->position_strides[0];
+  a.pl = p->position_strides[1];
+  a.pos0 = p->pos0;
+  a.freqs = p->freqs;
+  a.scale = (float)p->scale;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool in = interleaved != 0;
-  if (dtype == DSPARK_DTYPE_BF16) vec ? launch_rope<DSPARK_DTYPE_BF16, 8>(a, in, s) : launch_rope<DSPARK_DTYPE_BF16, 1>(a, in, s);
-  else if (dtype == DSPARK_DTYPE_F16) vec ? launch_rope<DSPARK_DTYPE_F16, 8>(a, in, s) : launch_rope<DSPARK_DTYPE_F16, 1>(a, in, s);
-  else vec ? launch_rope<DSPARK_DTYPE_F32, 4>(a, in, s) : launch_rope<DSPARK_DTYPE_F32, 1>(a, in, s);
+  if (dt == DSPARK_DTYPE_BF16) vec ? launch_rope<DSPARK_DTYPE_BF16, 8>(a, inter, s) : launch_rope<DSPARK_DTYPE_BF16, 1>(a, inter, s);
+  else if (dt == DSPARK_DTYPE_F16) vec ? launch_rope<DSPARK_DTYPE_F16, 8>(a, inter, s) : launch_rope<DSPARK_DTYPE_F16, 1>(a, inter, s);
+  else vec ? launch_rope<DSPARK_DTYPE_F32, 4>(a, inter, s) : launch_rope<DSPARK_DTYPE_F32, 1>(a, inter, s);
   return check_launch(what);
 }

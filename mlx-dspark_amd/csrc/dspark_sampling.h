@@ -37,7 +37,9 @@ constexpr int kSegVals = 512;          // logits of a segment
 constexpr int kMaxSegs = 1024;         // segments of a row: one LDS slot each in the kernels of a row
 constexpr int kMaxDraft = 255;         // drafts of a sequence
 constexpr int kBins = 8192;            // distinct logit values counted at a time
-constexpr int kRowThreads = 512;       // threads of the kernels that work on one row or sequence
+constexpr int kRowThreads = 1024;      // threads of the kernels that work on one row or sequence
+
+constexpr int kNoTies = -8;            // a cut below every index, those before a row's first logit too
 
 struct SampleArgs {
   const u16* x;                        // logits
@@ -119,11 +121,10 @@ __device__ __forceinline__ double exp2_neg(double d) {
   return __builtin_ldexp(p, (int)n);
 }
 
-// The weight of a logit against a maximum m (a NaN logit fails both tests and its NaN argument is taken
-// for the smaller operand: 0).
+// The weight of a logit against a maximum m over -inf (1 where they are equal, infinities too; a NaN logit's
+// NaN argument is taken for the smaller operand: 0). Straight code: the weights of a lane's 8 logits overlap.
 __device__ __forceinline__ double weight(float x, float m, double c) {
-  if (x == m) return x > -INFINITY ? 1.0 : 0.0;
-  return exp2_neg(((double)x - (double)m) * c);
+  return exp2_neg(x == m ? 0.0 : ((double)x - (double)m) * c);
 }
 
 // ---------------------------------------------------------------- wave reductions (DPP)

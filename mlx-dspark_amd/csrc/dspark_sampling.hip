@@ -32,7 +32,7 @@ __global__ __launch_bounds__(kStatThreads) void sample_segments_kernel(const Sam
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += weight(val<HALF>(bits_of(v[i], j)), m, a.c);
       s = wave_total(s);
-      if (lane == 0) a.segs[at] = s;
+      if (lane == 0) a.segs[at] = m > -INFINITY ? s : 0.0;
     }
     if (lane == 0) a.segm[at] = m;
   }
@@ -59,14 +59,22 @@ __device__ __forceinline__ void count_keys(const SampleArgs& a, const u16* x, in
   for (int i = threadIdx.x; i <= hi - lo; i += kRowThreads) sh.bins[i] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 63;
-  for (int i = uniform(threadIdx.x >> 6); i < nlist; i += kRowThreads / 64) {
-    const int s = sh.list[i];
-    if (sh.skey[s] < lo) continue;
-    const u32x4_t v = load8<HALF>(x, s * kSegVals + 8 * lane - off, a.V);
+  constexpr int kWaves = kRowThreads / 64, kAhead = 4;    // segments of a wave whose loads are out together
+  for (int i0 = uniform(threadIdx.x >> 6); i0 < nlist; i0 += kAhead * kWaves) {
+    u32x4_t v[kAhead];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = key_of<HALF>(bits_of(v, j));
-      if (k >= lo && k <= hi) atomicAdd(&sh.bins[hi - k], 1);
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * kWaves;
+      if (i < nlist) v[u] = load8<HALF>(x, sh.list[i] * kSegVals + 8 * lane - off, a.V);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u * kWaves >= nlist) break;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = key_of<HALF>(bits_of(v[u], j));
+        if (k >= lo && k <= hi) atomicAdd(&sh.bins[hi - k], 1);
+      }
     }
   }
   __syncthreads();
@@ -97,7 +105,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int row, RowS
   if (!(out.m > -INFINITY)) {           // nothing to draw from
     out.z = 0;
     out.thr = 1 << 16;
-    out.cut = -1;
+    out.cut = kNoTies;
     return out;
   }
   const int top = key_of_float<HALF>(out.m);
@@ -233,7 +241,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int row, RowS
   }
   out.thr = thr;
   out.z = z;
-  out.cut = ties ? a.V : -1;            // without a threshold value (thr = kb - 1) no token has that key
+  out.cut = ties ? a.V : kNoTies;            // without a threshold value (thr = kb - 1) no token has that key
   if (keep < ties) {                    // the index of the last kept token of the threshold's value
     const int lane = t & 63;
     for (int i = uniform(t >> 6); i < nlist; i += kRowThreads / 64) {
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
     __shared__ double red_d[kRowThreads / 64];
     r.z = join_segments(a.segm + (long)row * a.nseg, a.segs + (long)row * a.nseg, a.nseg, a.c, red_f, red_d, r.m);
     r.thr = kLowKey<HALF>;
-    r.cut = -1;
+    r.cut = kNoTies;
     r.pad = 0;
   }
   if (threadIdx.x == 0) {
@@ -418,16 +426,29 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SampleAr
   double all = 0, end = 0, s0 = 0, s1 = 0;
   for (int tries = 0; tries < 2; ++tries) {
     if constexpr (CUT) {
-      for (int s = uniform(t >> 6); s < a.nseg; s += kRowThreads / 64) {
-        double w[8], sum = 0;
-        if (r.z > 0 && skey[s] >= r.thr) {
-          const int v0 = s * kSegVals + 8 * lane - off;
-          rest8<HALF>(a, r, load8<HALF>(x, v0, a.V), v0, mode, q, skip, w);
+      constexpr int kWaves = kRowThreads / 64, kAhead = 4;
+      for (int i0 = uniform(t >> 6); i0 < a.nseg; i0 += kAhead * kWaves) {
+        u32x4_t v[kAhead];
+        bool on[kAhead];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum += w[j];
-          sum = wave_total(sum);
+        for (int k = 0; k < kAhead; ++k) {
+          const int s = i0 + k * kWaves;
+          on[k] = s < a.nseg && r.z > 0 && skey[s] >= r.thr;
+          if (on[k]) v[k] = load8<HALF>(x, s * kSegVals + 8 * lane - off, a.V);
         }
-        if (lane == 0) sums[s] = sum;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int s = i0 + k * kWaves;
+          if (s >= a.nseg) break;
+          double w[8], sum = 0;
+          if (on[k]) {
+            rest8<HALF>(a, r, v[k], s * kSegVals + 8 * lane - off, mode, q, skip, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += w[j];
+            sum = wave_total(sum);
+          }
+          if (lane == 0) sums[s] = sum;
+        }
       }
     } else {
       for (int s = t; s < a.nseg; s += kRowThreads)
@@ -558,14 +579,14 @@ constexpr int64_t kMaxVocab = (int64_t)kMaxSegs * kSegVals - 8;
 
 bool shape_ok(int64_t rows, int64_t V) { return rows >= 1 && rows <= 65535 && V >= 1 && V <= kMaxVocab; }
 
-int sample_args(const char* what, int dtype, const void* logits, int64_t rows, int64_t V, double temperature, int64_t top_k,
-                double top_p, void* ws, size_t ws_bytes, const Layout& l, SampleArgs& a) {
+int sample_args(const char* what, int64_t dtype, const void* logits, int64_t rows, int64_t V, double temperature, int64_t top_k,
+                double top_p, void* ws, int64_t ws_bytes, const Layout& l, SampleArgs& a) {
   if (!logits || !ws) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-  if (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F16) return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 logits)", what, dtype);
+  if (dtype != DSPARK_DTYPE_BF16 && dtype != DSPARK_DTYPE_F16) return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %lld (bf16 or fp16 logits)", what, (long long)dtype);
   if (!(temperature >= 1e-30 && temperature <= 1e30)) return fail(DSPARK_ERR_ARG, "%s: temperature %g (greedy: argmax_accept)", what, temperature);
   if (!(top_p > 0.0 && top_p <= 1.0) || top_k < 0) return fail(DSPARK_ERR_ARG, "%s: top_k %lld, top_p %g", what, (long long)top_k, top_p);
   if (!aligned(logits, 2) || !aligned(ws, 256)) return fail(DSPARK_ERR_ALIGN, "%s: logits need 2-byte, the workspace 256-byte alignment", what);
-  if (ws_bytes < l.bytes) return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes, l.bytes);
+  if (ws_bytes < (int64_t)l.bytes) return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %lld < %zu bytes", what, (long long)ws_bytes, l.bytes);
   char* w = static_cast<char*>(ws);
   a.x = static_cast<const u16*>(logits);
   a.rows = (int)rows;
@@ -621,68 +642,65 @@ extern "C" size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t seq
   return layout(rows, V, sequences).bytes;
 }
 
-extern "C" int dspark_sampling_probs(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V, double temperature,
-                                     int64_t top_k, double top_p, float* out, int64_t ldo, void* workspace,
-                                     size_t workspace_bytes, dspark_stream stream) {
+extern "C" int dspark_sampling_probs(const dspark_sampling_probs_args* p, dspark_stream stream) {
   const char* what = "sampling_probs";
-  if (!out) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-  if (!shape_ok(rows, V) || (rows > 1 && (ld < V || ldo < V)))
-    return fail(DSPARK_ERR_SHAPE, "%s: rows=%lld V=%lld ld=%lld", what, (long long)rows, (long long)V, (long long)ld);
-  if (!aligned(out, 4)) return fail(DSPARK_ERR_ALIGN, "%s: out needs 4-byte alignment", what);
-  const Layout l = layout(rows, V, 0);
+  if (!p || !p->out) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  if (!shape_ok(p->rows, p->V) || (p->rows > 1 && (p->ld < p->V || p->ldo < p->V)))
+    return fail(DSPARK_ERR_SHAPE, "%s: rows=%lld V=%lld ld=%lld", what, (long long)p->rows, (long long)p->V, (long long)p->ld);
+  if (!aligned(p->out, 4)) return fail(DSPARK_ERR_ALIGN, "%s: out needs 4-byte alignment", what);
+  const Layout l = layout(p->rows, p->V, 0);
   SampleArgs a;
-  const int st = sample_args(what, dtype, logits, rows, V, temperature, top_k, top_p, workspace, workspace_bytes, l, a);
+  const int st = sample_args(what, p->dtype, p->logits, p->rows, p->V, p->temperature, p->top_k, p->top_p, p->workspace,
+                             p->workspace_bytes, l, a);
   if (st) return st;
-  a.ldb = ld;
+  a.ldb = p->ld;
   a.ldr = 0;
   a.per = 1;
-  RowInfo* info = reinterpret_cast<RowInfo*>(static_cast<char*>(workspace) + l.info);
+  RowInfo* info = reinterpret_cast<RowInfo*>(static_cast<char*>(p->workspace) + l.info);
   const bool cut = a.top_k || a.top_p < 1.0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == DSPARK_DTYPE_F16) cut ? probs<true, true>(a, info, out, ldo, s) : probs<true, false>(a, info, out, ldo, s);
-  else cut ? probs<false, true>(a, info, out, ldo, s) : probs<false, false>(a, info, out, ldo, s);
+  if (p->dtype == DSPARK_DTYPE_F16) cut ? probs<true, true>(a, info, p->out, p->ldo, s) : probs<true, false>(a, info, p->out, p->ldo, s);
+  else cut ? probs<false, true>(a, info, p->out, p->ldo, s) : probs<false, false>(a, info, p->out, p->ldo, s);
   return check_launch(what);
 }
 
-extern "C" int dspark_speculative_verify(int dtype, const void* logits, int64_t ld_seq, int64_t ld_row, int64_t sequences,
-                                         int64_t drafts, int64_t V, const int32_t* draft, const float* draft_probs,
-                                         int64_t q_seq, int64_t q_row, const int32_t* draft_lens, const void* uniforms,
-                                         int uniforms_f64, double temperature, int64_t top_k, double top_p,
-                                         int32_t* n_accepted, int32_t* tokens, float* draft_p, void* workspace,
-                                         size_t workspace_bytes, dspark_stream stream) {
+extern "C" int dspark_speculative_verify(const dspark_speculative_verify_args* p, dspark_stream stream) {
   const char* what = "speculative_verify";
-  if (!uniforms || !n_accepted || !tokens || (drafts > 0 && (!draft || !draft_p)))
+  if (!p || !p->uniforms || !p->n_accepted || !p->tokens || (p->drafts > 0 && (!p->draft || !p->draft_p)))
     return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
-  if (sequences < 1 || sequences > 65535 || drafts < 0 || drafts > kMaxDraft || !shape_ok(sequences * (drafts + 1), V))
-    return fail(DSPARK_ERR_SHAPE, "%s: sequences=%lld drafts=%lld V=%lld", what, (long long)sequences, (long long)drafts, (long long)V);
-  if (ld_seq < 0 || ld_row < 0 || (draft_probs && (q_seq < 0 || q_row < 0)))
+  if (p->sequences < 1 || p->sequences > 65535 || p->drafts < 0 || p->drafts > kMaxDraft ||
+      !shape_ok(p->sequences * (p->drafts + 1), p->V))
+    return fail(DSPARK_ERR_SHAPE, "%s: sequences=%lld drafts=%lld V=%lld", what, (long long)p->sequences,
+                (long long)p->drafts, (long long)p->V);
+  if (p->ld_seq < 0 || p->ld_row < 0 || (p->draft_probs && (p->q_seq < 0 || p->q_row < 0)))
     return fail(DSPARK_ERR_SHAPE, "%s: negative strides", what);
-  if (!aligned(uniforms, uniforms_f64 ? 8 : 4)) return fail(DSPARK_ERR_ALIGN, "%s: uniforms alignment", what);
-  const Layout l = layout(sequences * (drafts + 1), V, sequences);
+  if (!aligned(p->uniforms, p->uniforms_f64 ? 8 : 4)) return fail(DSPARK_ERR_ALIGN, "%s: uniforms alignment", what);
+  const int64_t rows = p->sequences * (p->drafts + 1);
+  const Layout l = layout(rows, p->V, p->sequences);
   SampleArgs a;
-  const int st = sample_args(what, dtype, logits, sequences * (drafts + 1), V, temperature, top_k, top_p, workspace,
-                             workspace_bytes, l, a);
+  const int st = sample_args(what, p->dtype, p->logits, rows, p->V, p->temperature, p->top_k, p->top_p, p->workspace,
+                             p->workspace_bytes, l, a);
   if (st) return st;
-  a.ldb = ld_seq;
-  a.ldr = ld_row;
-  a.per = (int)drafts + 1;
+  a.ldb = p->ld_seq;
+  a.ldr = p->ld_row;
+  a.per = (int)p->drafts + 1;
   VerifyIn in;
-  in.draft = draft;
-  in.q = drafts > 0 ? draft_probs : nullptr;
-  in.qb = q_seq;
-  in.qr = q_row;
-  in.lens = draft_lens;
-  in.u = uniforms;
-  in.u64 = uniforms_f64;
-  in.n = n_accepted;
-  in.tokens = tokens;
-  in.px = draft_p;
-  char* w = static_cast<char*>(workspace);
+  in.draft = p->draft;
+  in.q = p->drafts > 0 ? p->draft_probs : nullptr;
+  in.qb = p->q_seq;
+  in.qr = p->q_row;
+  in.lens = p->draft_lens;
+  in.u = p->uniforms;
+  in.u64 = p->uniforms_f64 != 0;
+  in.n = p->n_accepted;
+  in.tokens = p->tokens;
+  in.px = p->draft_p;
+  char* w = static_cast<char*>(p->workspace);
   RowInfo* info = reinterpret_cast<RowInfo*>(w + l.info);
   double* rest = reinterpret_cast<double*>(w + l.rest);
   const bool cut = a.top_k || a.top_p < 1.0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == DSPARK_DTYPE_F16) cut ? verify<true, true>(a, in, info, rest, s) : verify<true, false>(a, in, info, rest, s);
+  if (p->dtype == DSPARK_DTYPE_F16) cut ? verify<true, true>(a, in, info, rest, s) : verify<true, false>(a, in, info, rest, s);
   else cut ? verify<false, true>(a, in, info, rest, s) : verify<false, false>(a, in, info, rest, s);
   return check_launch(what);
 }

@@ -20,10 +20,8 @@ c_int = ctypes.c_int
 c_i64 = ctypes.c_int64
 c_size_t = ctypes.c_size_t
 c_float = ctypes.c_float
-c_double = ctypes.c_double
 c_char_p = ctypes.c_char_p
 c_i64_p = ctypes.POINTER(ctypes.c_int64)
-c_void_pp = ctypes.POINTER(ctypes.c_void_p)
 
 STATUS = {
     0: "DSPARK_OK",
@@ -186,18 +184,12 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_argmax_accept": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
                                      c_size_t, c_void_p]),
     "dspark_sampling_workspace": (c_size_t, [c_i64, c_i64, c_i64]),
-    "dspark_sampling_probs": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_double, c_i64, c_double, c_void_p, c_i64,
-                                      c_void_p, c_size_t, c_void_p]),
-    "dspark_speculative_verify": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64,
-                                          c_i64, c_void_p, c_void_p, c_int, c_double, c_i64, c_double, c_void_p,
-                                          c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "dspark_rope": (c_int, [c_int, c_void_p, c_i64_p, c_i64, c_void_p, c_i64_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
-                            c_void_p, c_float, c_void_p, c_int, c_i64_p, c_i64, c_void_p, c_i64_p, c_void_p, c_i64_p,
-                            c_void_p]),
-    "dspark_kv_quantize": (c_int, [c_int, c_void_pp, c_i64_p, c_int, c_void_pp, c_void_pp, c_void_pp, c_i64_p, c_i64_p,
-                                   c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_void_p]),
-    "dspark_kv_dequantize": (c_int, [c_int, c_void_pp, c_void_pp, c_void_pp, c_i64_p, c_i64_p, c_i64, c_i64, c_i64, c_i64,
-                                     c_int, c_int, c_int, c_void_pp, c_i64_p, c_void_p]),
+    # args: the bytes of the struct of 8-byte fields (include/dspark.h)
+    "dspark_sampling_probs": (c_int, [c_char_p, c_void_p]),
+    "dspark_speculative_verify": (c_int, [c_char_p, c_void_p]),
+    "dspark_rope": (c_int, [c_char_p, c_void_p]),
+    "dspark_kv_quantize": (c_int, [c_char_p, c_void_p]),
+    "dspark_kv_dequantize": (c_int, [c_char_p, c_void_p]),
 }
 
 _lock = threading.Lock()

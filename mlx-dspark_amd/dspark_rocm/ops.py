@@ -6,8 +6,8 @@ These are the product path: every function here launches a hand-written gfx950 k
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import struct
 
 import torch
 
@@ -873,13 +873,22 @@ def argmax_accept(logits: torch.Tensor, draft: torch.Tensor, target_tokens: torc
 
 
 # ---------------------------------------------------------------------------- sampled rounds
+#
+# The entry points from here on take one struct of 8-byte fields (include/dspark.h): packing it costs a tenth of
+# converting twenty arguments one by one, which is what a call of a few microseconds is made of.
 
 LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1}    # dspark_dtype codes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the stream's handle without a Stream object
 
 
-def _on_device(device: torch.device):
-    """The device as the current one for the block (a launch needs its stream's device to be)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call_on(dev: torch.device, name: str, args: bytes) -> None:
+    """``name(args, current stream of dev)`` with dev as the current device (a launch needs its stream's to be)."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None else _raw_stream(index))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _no_autograd(what: str, *ts: torch.Tensor) -> None:
@@ -889,17 +898,19 @@ def _no_autograd(what: str, *ts: torch.Tensor) -> None:
                 raise ValueError(f"{what}: has no backward pass; detach its inputs or use torch.no_grad()")
 
 
-def _one_device(what: str, first: torch.Tensor, *ts) -> None:
+def _one_device(what: str, first: torch.Tensor, *ts) -> torch.device:
     if not first.is_cuda:
         raise ValueError("dspark kernels need tensors on a ROCm device (cuda:N)")
+    dev = first.device
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
 
 
 def check_sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
     """The sampler's settings as the kernels take them; ValueError where they refuse them."""
-    t, k, p = float(temperature), int(top_k or 0), float(top_p)
+    t, k, p = float(temperature), min(int(top_k or 0), 1 << 31), float(top_p)
     if not 1e-30 <= t <= 1e30:
         raise ValueError(f"temperature={temperature}: a positive number (greedy rounds: argmax_accept)")
     if k < 0 or not 0.0 < p <= 1.0:
@@ -913,7 +924,7 @@ def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> to
         raise ValueError(f"{rows} rows of {vocab} logits (up to 65535 rows of 524280)")
     if ws is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if ws.numel() * ws.element_size() < nbytes or ws.device != device or not ws.is_contiguous():
+    if ws.numel() * ws.element_size() < nbytes or not ws.is_contiguous():
         raise ValueError(f"workspace: {nbytes} contiguous bytes on {device} needed")
     return ws
 
@@ -924,6 +935,9 @@ def sampling_workspace_bytes(rows: int, vocab: int, sequences: int = 0) -> int:
     return int(_lib.load().dspark_sampling_workspace(rows, vocab, sequences))
 
 
+_PROBS_ARGS = struct.Struct("=5qdqd4q")
+
+
 def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """The probabilities a token is sampled from, fp32 [..., V]: softmax of ``logits / temperature``
@@ -932,37 +946,40 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     of nothing but -inf and NaN gives zeros. What a drafter samples its tokens from and hands to
     :func:`speculative_verify`. ``out`` contiguous; ``workspace`` (any content) of
     :func:`sampling_workspace_bytes`, else allocated."""
-    _one_device("sampling_probs", logits, out, workspace)
+    dev = _one_device("sampling_probs", logits, out, workspace)
     dt = LOGIT_DTYPES.get(logits.dtype)
     if dt is None:
         raise TypeError(f"sampling_probs: logits {logits.dtype} (bfloat16 or float16)")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"sampling_probs: logits {tuple(logits.shape)}")
+    shape = logits.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"sampling_probs: logits {list(shape)}")
     _no_autograd("sampling_probs", logits)
     t, k, p = check_sampler(temperature, top_k, top_p)
-    V = logits.shape[-1]
-    x = logits.reshape(-1, V)
-    if x.stride(1) != 1 or x.stride(0) < V:
-        x = x.contiguous()
-    rows = x.shape[0]
+    V = shape[-1]
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    rows, (ld, unit) = x.shape[0], x.stride()
+    if unit != 1 or ld < V:
+        x, ld = x.contiguous(), V
     if out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-    elif out.dtype != torch.float32 or out.shape != logits.shape or not out.is_contiguous():
-        raise ValueError(f"sampling_probs: out must be contiguous fp32 {tuple(logits.shape)}")
+        out = torch.empty(shape, dtype=torch.float32, device=dev)
+    elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"sampling_probs: out must be contiguous fp32 {list(shape)}")
     if rows:
-        ws = _sampling_workspace(workspace, logits.device, rows, V, 0)
-        with _on_device(logits.device):
-            _lib.call("dspark_sampling_probs", dt, x.data_ptr(), x.stride(0), rows, V, t, k, p, out.data_ptr(), V,
-                      ws.data_ptr(), ws.numel() * ws.element_size(), _stream(x))
+        ws = _sampling_workspace(workspace, dev, rows, V, 0)
+        _call_on(dev, "dspark_sampling_probs",
+                 _PROBS_ARGS.pack(dt, x.data_ptr(), ld, rows, V, t, k, p, out.data_ptr(), V, ws.data_ptr(), ws.nbytes))
     return out
 
 
 def _ints(what: str, name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != shape:
+    if t.dtype is torch.int32 and t.shape == shape:
+        return t.contiguous()
+    if t.dtype is not torch.int64 or t.shape != shape:
         raise ValueError(f"{what}: {name} must be int32 or int64 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    if t.dtype == torch.int64:              # an id past 32 bits stays one that no vocabulary has
-        t = t.clamp(-1, 2 ** 31 - 1)
-    return t.to(torch.int32).contiguous()
+    return t.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()    # an id past 32 bits stays one that no vocabulary has
+
+
+_VERIFY_ARGS = struct.Struct("=14qdqd5q")
 
 
 def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torch.Tensor, *,
@@ -981,50 +998,56 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
     ``draft_lens`` [B] (padded batches): how many drafts each sequence has. ``uniforms`` [B, m + 1] fp32 or
     fp64 in [0, 1). Drafts outside the vocabulary are refused. m up to 255."""
     what = "speculative_verify"
-    _one_device(what, logits, draft, uniforms, draft_probs, draft_lens, workspace)
+    dev = _one_device(what, logits, draft, uniforms, draft_probs, draft_lens, workspace)
     dt = LOGIT_DTYPES.get(logits.dtype)
     if dt is None:
         raise TypeError(f"{what}: logits {logits.dtype} (bfloat16 or float16)")
-    if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
-        raise ValueError(f"{what}: logits must be [B, drafts + 1, V], got {list(logits.shape)}")
-    B, R, V = logits.shape
+    shape = logits.shape
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1:
+        raise ValueError(f"{what}: logits must be [B, drafts + 1, V], got {list(shape)}")
+    B, R, V = shape
     m = R - 1
     if m > 255:
         raise ValueError(f"{what}: {m} drafts (up to 255)")
-    if uniforms.dtype not in (torch.float32, torch.float64) or tuple(uniforms.shape) != (B, R):
+    u64 = uniforms.dtype is torch.float64
+    if not (u64 or uniforms.dtype is torch.float32) or uniforms.shape != (B, R):
         raise ValueError(f"{what}: uniforms must be fp32 or fp64 [{B}, {R}], got {uniforms.dtype} {list(uniforms.shape)}")
     t, k, p = check_sampler(temperature, top_k, top_p)
     draft = _ints(what, "draft", draft, (B, m))
     q = q_seq = q_row = 0
     if draft_probs is not None:
-        if draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (B, m, V):
+        if draft_probs.dtype is not torch.float32 or draft_probs.shape != (B, m, V):
             raise ValueError(f"{what}: draft_probs must be fp32 [{B}, {m}, {V}], got {draft_probs.dtype} {list(draft_probs.shape)}")
         _no_autograd(what, draft_probs)
-        if draft_probs.stride(2) != 1:
+        q_seq, q_row, unit = draft_probs.stride()
+        if unit != 1 and V > 1:
             draft_probs = draft_probs.contiguous()
-        q, q_seq, q_row = draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1)
+            q_seq, q_row, _ = draft_probs.stride()
+        q = draft_probs.data_ptr()
     _no_autograd(what, logits)
+    lens = 0
     if draft_lens is not None:
         draft_lens = _ints(what, "draft_lens", draft_lens, (B,))
-    x = logits if logits.stride(2) == 1 else logits.contiguous()
-    u = uniforms.contiguous()
-    dev = logits.device
+        lens = draft_lens.data_ptr()
+    ld_seq, ld_row, unit = logits.stride()
+    if unit != 1 and V > 1:
+        logits = logits.contiguous()
+        ld_seq, ld_row, _ = logits.stride()
+    uniforms = uniforms.contiguous()
     n = torch.empty(B, dtype=torch.int32, device=dev)
     tokens = torch.empty((B, R), dtype=torch.int32, device=dev)
     draft_p = torch.empty((B, m), dtype=torch.float32, device=dev)
     if B:
         ws = _sampling_workspace(workspace, dev, B * R, V, B)
-        with _on_device(dev):
-            _lib.call("dspark_speculative_verify", dt, x.data_ptr(), x.stride(0), x.stride(1), B, m, V, draft.data_ptr(),
-                      q or None, q_seq, q_row, None if draft_lens is None else draft_lens.data_ptr(), u.data_ptr(),
-                      int(u.dtype == torch.float64), t, k, p, n.data_ptr(), tokens.data_ptr(), draft_p.data_ptr(),
-                      ws.data_ptr(), ws.numel() * ws.element_size(), _stream(x))
+        _call_on(dev, "dspark_speculative_verify",
+                 _VERIFY_ARGS.pack(dt, logits.data_ptr(), ld_seq, ld_row, B, m, V, draft.data_ptr(), q, q_seq, q_row, lens,
+                                   uniforms.data_ptr(), u64, t, k, p, n.data_ptr(), tokens.data_ptr(), draft_p.data_ptr(),
+                                   ws.data_ptr(), ws.nbytes))
     return n, tokens, draft_p
 
 
 # ---------------------------------------------------------------------------- rotary positions, quantized cache rows
 
-_I64x2, _I64x6, _Ptrx2 = ctypes.c_int64 * 2, ctypes.c_int64 * 6, ctypes.c_void_p * 2
 ROPE_DTYPES = DEQUANT_DTYPES
 
 
@@ -1035,19 +1058,20 @@ def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _no_repeats(what: str, out: torch.Tensor) -> None:
-    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+    if 0 in out.stride() and any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise ValueError(f"{what}: the output is an expanded view ({list(out.shape)}, strides {list(out.stride())})")
 
 
-def _rope_out(name: str, x: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _check_rope_out(name: str, x: torch.Tensor, out: torch.Tensor) -> None:
     if out.dtype != x.dtype or out.shape != x.shape or out.stride(3) != 1:
         raise ValueError(f"rope: {name} must be {x.dtype} {list(x.shape)} with unit last stride")
     _no_repeats("rope", out)
     if _spans_meet(x, out) and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()):
         raise ValueError(f"rope: {name} overlaps its input (in place: the same view)")
-    return out
+
+
+_ROPE_ARGS = struct.Struct("=25qd5q")
+_NO_KEYS = (0,) * 9
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions, *, interleaved: bool = False,
@@ -1061,79 +1085,100 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
     an int32 / int64 tensor [L] or [B or 1, L or 1] with the position of every row, as tree rows need. The
     angle is reduced in fp64; one rounding to the tensors' type. ``q_out`` / ``k_out``: where to write,
     e.g. a cache's rows, or q and k themselves."""
-    _one_device("rope", q, k, freqs, q_out, k_out)
-    dt = ROPE_DTYPES.get(q.dtype)
-    if dt is None or (k is not None and k.dtype != q.dtype):
-        raise TypeError(f"rope: q {q.dtype}, k {None if k is None else k.dtype} (one of bfloat16, float16, float32)")
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (q.shape[0], *q.shape[2:]))):
-        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(q.shape)} and {None if k is None else list(k.shape)}")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= min(128, q.shape[3] // 2):
+    dev = _one_device("rope", q, k, freqs, q_out, k_out)
+    dtype, shape = q.dtype, q.shape
+    dt = ROPE_DTYPES.get(dtype)
+    if dt is None or (k is not None and k.dtype != dtype):
+        raise TypeError(f"rope: q {dtype}, k {None if k is None else k.dtype} (one of bfloat16, float16, float32)")
+    if len(shape) != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (shape[0], *shape[2:]))):
+        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(shape)} and {None if k is None else list(k.shape)}")
+    B, Hq, L, D = shape
+    half = freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not 1 <= half <= min(128, D // 2):
         raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(freqs.shape)}")
     if k is None and k_out is not None:
         raise ValueError("rope: k_out without k")
     _no_autograd("rope", q, *(() if k is None else (k,)))
-    B, Hq, L, D = q.shape
     freqs = freqs.contiguous()
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
-    pos, pos64, ps, pos0 = None, 0, None, 0
+    pos, pos64, pb, pl, pos0 = 0, 0, 0, 0, 0
     if isinstance(positions, torch.Tensor):
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device or positions.dim() not in (1, 2):
-            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L] on {q.device}, got {positions.dtype} {list(positions.shape)}")
-        try:
-            at = positions.expand(B, L)
-        except RuntimeError:
-            raise ValueError(f"rope: positions {list(positions.shape)} for {B} sequences of {L} rows") from None
-        pos, pos64, ps = positions.data_ptr(), int(positions.dtype == torch.int64), _I64x2(at.stride(0), at.stride(1))
+        ps = positions.shape
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev or len(ps) not in (1, 2):
+            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L] on {dev}, got {positions.dtype} {list(ps)}")
+        if ps[-1] not in (1, L) or (len(ps) == 2 and ps[0] not in (1, B)):
+            raise ValueError(f"rope: positions {list(ps)} for {B} sequences of {L} rows")
+        pos, pos64, st = positions.data_ptr(), int(positions.dtype is torch.int64), positions.stride()
+        pl = st[-1] if ps[-1] > 1 else 0
+        pb = st[0] if len(ps) == 2 and ps[0] > 1 else 0
     else:
         pos0 = int(positions)
-    q_out = _rope_out("q_out", q, q_out)
+        if abs(pos0) >= 1 << 52:
+            raise ValueError(f"rope: position {pos0}")
+    sq = q.stride()
+    if sq[3] != 1:
+        q = q.contiguous()
+        sq = q.stride()
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dtype, device=dev)
+    else:
+        _check_rope_out("q_out", q, q_out)
+    so = q_out.stride()
+    keys = _NO_KEYS
     if k is not None:
-        k_out = _rope_out("k_out", k, k_out)
-    if q.numel() or (k is not None and k.numel()):
-        Hk = 0 if k is None else k.shape[1]
-        with _on_device(q.device):
-            _lib.call("dspark_rope", dt, q.data_ptr(), _i64x3(q), Hq, k.data_ptr() if Hk else None, _i64x3(k) if Hk else None,
-                      Hk, B, L, D, 2 * freqs.numel(), int(bool(interleaved)), freqs.data_ptr(), float(scale), pos, pos64, ps,
-                      pos0, q_out.data_ptr(), _i64x3(q_out), k_out.data_ptr() if Hk else None, _i64x3(k_out) if Hk else None,
-                      _stream(q))
+        sk = k.stride()
+        if sk[3] != 1:
+            k = k.contiguous()
+            sk = k.stride()
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+        else:
+            _check_rope_out("k_out", k, k_out)
+        if k.numel():
+            sko = k_out.stride()
+            keys = (k.data_ptr(), k_out.data_ptr(), sk[0], sk[1], sk[2], sko[0], sko[1], sko[2], k.shape[1])
+    if q.numel() or keys is not _NO_KEYS:
+        _call_on(dev, "dspark_rope",
+                 _ROPE_ARGS.pack(dt, q.data_ptr(), q_out.data_ptr(), sq[0], sq[1], sq[2], so[0], so[1], so[2], Hq, *keys, B, L,
+                                 D, 2 * half, bool(interleaved), freqs.data_ptr(), scale, pos, pos64, pb, pl, pos0))
     return q_out, k_out
 
 
 KV_CACHE_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_KV_ARGS = struct.Struct("=34q")
 
 
-def _kv_pair(what: str, keys, values, bits: int, group_size: int, shape=None):
-    """Checks of a (words, scales, biases) pair of cache views; (B, H, T, D), the type's code and the
-    argument arrays the C ABI takes."""
+def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple, cache_dtype) -> tuple:
+    """The fields of one ``dspark_kv_side``: plain rows x and the (words, scales, biases) they belong to."""
+    w, s, b = trip
+    _require_packed(w)
+    if s.dtype != cache_dtype or b.dtype != cache_dtype:
+        raise TypeError(f"{what}: scales and biases of {cache_dtype}, {s.dtype} and {b.dtype}")
+    ws, ss = w.stride(), s.stride()
+    if w.shape != words or s.shape != groups or b.shape != groups:
+        raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
+    if ws[3] != 1 or ss[3] != 1 or ss != b.stride():
+        if groups[3] > 1 or ws[3] != 1 or ss[:3] != b.stride()[:3]:
+            raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
+    xs = x.stride()
+    return (x.data_ptr(), xs[0], xs[1], xs[2], w.data_ptr(), s.data_ptr(), b.data_ptr(), ws[0], ws[1], ws[2], ss[0], ss[1], ss[2])
+
+
+def _kv_shape(what: str, keys, bits: int, group_size: int):
+    """((B, H, T, D), shape of the scales, their type) of a triple of cache views."""
     if bits not in KV_BITS or group_size != GROUP:
         raise ValueError(f"{what}: bits={bits} (4 or 8), group_size={group_size} (64)")
-    kw, ks, kb = keys
-    vw, vs, vb = values
+    kw = keys[0]
     if kw.dim() != 4:
         raise ValueError(f"{what}: words must be [B, H, rows, D * bits / 32], got {list(kw.shape)}")
     B, H, T, W = kw.shape
     D = W * 32 // bits
-    if D % GROUP or D == 0 or (shape is not None and tuple(shape) != (B, H, T, D)):
-        raise ValueError(f"{what}: words {list(kw.shape)} at {bits} bits" + ("" if shape is None else f" for rows {list(shape)}"))
-    if ks.dtype not in KV_CACHE_DTYPES:
-        raise TypeError(f"{what}: scales {ks.dtype} (bfloat16 or float16)")
-    for w, s, b in ((kw, ks, kb), (vw, vs, vb)):
-        _require_packed(w)
-        if s.dtype != ks.dtype or b.dtype != ks.dtype:
-            raise TypeError(f"{what}: scales and biases of {ks.dtype}, {s.dtype} and {b.dtype}")
-        if w.shape != kw.shape or s.shape != (B, H, T, D // GROUP) or b.shape != s.shape:
-            raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
-        if w.stride(3) != 1 or s.stride(3) != 1 or s.stride() != b.stride():
-            raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
+    if D % GROUP or D == 0:
+        raise ValueError(f"{what}: words {list(kw.shape)} at {bits} bits")
+    if keys[1].dtype not in KV_CACHE_DTYPES:
+        raise TypeError(f"{what}: scales {keys[1].dtype} (bfloat16 or float16)")
     if 2 * B * H > 65535:
         raise ValueError(f"{what}: {B} x {H} heads (up to 32767)")
-    strides = lambda a, b: _I64x6(*a.stride()[:3], *b.stride()[:3])
-    arrays = (_Ptrx2(kw.data_ptr(), vw.data_ptr()), _Ptrx2(ks.data_ptr(), vs.data_ptr()), _Ptrx2(kb.data_ptr(), vb.data_ptr()),
-              strides(kw, vw), strides(ks, vs))
-    return (B, H, T, D), KV_CACHE_DTYPES[ks.dtype], arrays
+    return (B, H, T, D), (B, H, T, D // GROUP), keys[1].dtype
 
 
 def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bits: int, group_size: int = GROUP) -> None:
@@ -1142,25 +1187,25 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     quantized cache, scales in bf16 or fp16. The values of :func:`dspark_rocm.quant.quantize_rows`, bit for
     bit (a group with a NaN gets a NaN scale and bias), both tensors in one launch."""
     what = "quantize_kv"
-    _one_device(what, keys, values, *k_rows, *v_rows)
+    dev = _one_device(what, keys, values, *k_rows, *v_rows)
     dt = DEQUANT_DTYPES.get(keys.dtype)
     if dt is None or values.dtype != keys.dtype:
         raise TypeError(f"{what}: rows {keys.dtype} and {values.dtype} (one of bfloat16, float16, float32)")
-    if keys.shape != values.shape:
-        raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)}")
+    (B, H, T, D), groups, cdt = _kv_shape(what, k_rows, bits, group_size)
+    if keys.shape != (B, H, T, D) or values.shape != keys.shape:
+        raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)} for rows [{B}, {H}, {T}, {D}]")
     _no_autograd(what, keys, values)
-    (B, H, T, D), cache_dt, (w, s, b, ws, ss) = _kv_pair(what, k_rows, v_rows, bits, group_size, keys.shape)
-    for t in (*k_rows, *v_rows):
-        _no_repeats(what, t)
     if keys.stride(3) != 1:
         keys = keys.contiguous()
     if values.stride(3) != 1:
         values = values.contiguous()
+    words = k_rows[0].shape
+    for t in (*k_rows, *v_rows):
+        _no_repeats(what, t)
+    args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt),
+            *_kv_side(what, values, v_rows, words, groups, cdt))
     if B * H * T:
-        with _on_device(keys.device):
-            _lib.call("dspark_kv_quantize", dt, _Ptrx2(keys.data_ptr(), values.data_ptr()),
-                      _I64x6(*keys.stride()[:3], *values.stride()[:3]), cache_dt, w, s, b, ws, ss, B, H, T, D, bits,
-                      group_size, _stream(keys))
+        _call_on(dev, "dspark_kv_quantize", _KV_ARGS.pack(*args))
 
 
 def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: torch.dtype = torch.float32, out=None):
@@ -1168,21 +1213,22 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     [B, H, T, D] of ``dtype``, ``scale * field + bias`` with an fp32 product rounded, then an fp32 sum
     rounded, then rounded to ``dtype``; both tensors in one launch. ``out``: two tensors to write."""
     what = "dequantize_kv"
-    kw = keys[0]
-    _one_device(what, *keys, *values, *(out or ()))
-    if dtype not in DEQUANT_DTYPES:
+    dev = _one_device(what, *keys, *values, *(out or ()))
+    dt = DEQUANT_DTYPES.get(dtype)
+    if dt is None:
         raise TypeError(f"{what}: dtype {dtype} (bfloat16, float16 or float32)")
-    (B, H, T, D), cache_dt, (w, s, b, ws, ss) = _kv_pair(what, keys, values, bits, group_size)
+    shape, groups, cdt = _kv_shape(what, keys, bits, group_size)
     if out is None:
-        k, v = torch.empty((B, H, T, D), dtype=dtype, device=kw.device), torch.empty((B, H, T, D), dtype=dtype, device=kw.device)
+        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     else:
         k, v = out
-        for t in (k, v):
-            if t.dtype != dtype or tuple(t.shape) != (B, H, T, D) or t.stride(3) != 1:
-                raise ValueError(f"{what}: out must be two {dtype} [{B}, {H}, {T}, {D}] with unit last stride")
+        for t in out:
+            if t.dtype != dtype or t.shape != shape or t.stride(3) != 1:
+                raise ValueError(f"{what}: out must be two {dtype} {list(shape)} with unit last stride")
             _no_repeats(what, t)
-    if B * H * T:
-        with _on_device(kw.device):
-            _lib.call("dspark_kv_dequantize", cache_dt, w, s, b, ws, ss, B, H, T, D, bits, group_size, DEQUANT_DTYPES[dtype],
-                      _Ptrx2(k.data_ptr(), v.data_ptr()), _I64x6(*k.stride()[:3], *v.stride()[:3]), _stream(kw))
+    words = keys[0].shape
+    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt),
+            *_kv_side(what, v, values, words, groups, cdt))
+    if shape[0] * shape[1] * shape[2]:
+        _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v

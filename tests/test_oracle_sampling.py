@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -58,14 +56,18 @@ def _lib():
     (dict(ws=(1 << 20) + 16), -3), (dict(logits=(1 << 20) + 1), -3), (dict(out=(1 << 20) + 2), -3)])
 def test_sampling_probs_refuses(change, status):
     """Refused on the host: the pointers are never followed."""
+    from dspark_rocm import ops
+
     lib = _lib()
     fake = 1 << 20
     a = dict(dtype=0, logits=fake, ld=100, rows=3, V=100, temperature=1.0, top_k=0, top_p=1.0, out=fake, ws=fake, nbytes=0)
     a.update(change)
     need = lib.dspark_sampling_workspace(a["rows"], a["V"], 0)
     assert (need == 0) == (status == -2 and "ld" not in change)
-    st = lib.dspark_sampling_probs(a["dtype"], a["logits"], a["ld"], a["rows"], a["V"], a["temperature"], a["top_k"],
-                                   a["top_p"], a["out"], 100, a["ws"], max(need + a["nbytes"], 0), None)
+    st = lib.dspark_sampling_probs(ops._PROBS_ARGS.pack(a["dtype"], a["logits"] or 0, a["ld"], a["rows"], a["V"], a["temperature"],
+                                                        a["top_k"], a["top_p"], a["out"] or 0, 100, a["ws"] or 0,
+                                                        max(need + a["nbytes"], 0)), None)
+    assert lib.dspark_sampling_probs(None, None) == -1
     assert st == status and lib.dspark_last_error()
 
 
@@ -75,15 +77,18 @@ def test_sampling_probs_refuses(change, status):
     (dict(temperature=0.0), -1), (dict(top_p=-0.1), -1), (dict(ld=-5), -2), (dict(nbytes=-1), -4), (dict(u=(1 << 20) + 2), -3),
     (dict(u=(1 << 20) + 4, f64=1), -3)])
 def test_speculative_verify_refuses(change, status):
+    from dspark_rocm import ops
+
     lib = _lib()
     fake = 1 << 20
     a = dict(dtype=0, ld=100, B=2, m=3, V=100, draft=fake, u=fake, f64=0, temperature=1.0, top_p=1.0, n=fake, tokens=fake,
              px=fake, nbytes=0)
     a.update(change)
     need = lib.dspark_sampling_workspace(a["B"] * (a["m"] + 1), a["V"], max(a["B"], 0))
-    st = lib.dspark_speculative_verify(a["dtype"], fake, 4 * a["ld"], a["ld"], a["B"], a["m"], a["V"], a["draft"], None, 0, 0,
-                                       None, a["u"], a["f64"], a["temperature"], 0, a["top_p"], a["n"], a["tokens"], a["px"],
-                                       fake, max(need + a["nbytes"], 0), None)
+    st = lib.dspark_speculative_verify(ops._VERIFY_ARGS.pack(
+        a["dtype"], fake, 4 * a["ld"], a["ld"], a["B"], a["m"], a["V"], a["draft"] or 0, 0, 0, 0, 0, a["u"] or 0, a["f64"],
+        a["temperature"], 0, a["top_p"], a["n"] or 0, a["tokens"] or 0, a["px"] or 0, fake, max(need + a["nbytes"], 0)), None)
+    assert lib.dspark_speculative_verify(None, None) == -1
     assert st == status and lib.dspark_last_error()
 
 

@@ -94,25 +94,21 @@ def test_which_targets_need_a_table():
         hash(a)
 
 
-def _i64(*v):
-    import ctypes
-
-    return (ctypes.c_int64 * len(v))(*v)
-
-
 @pytest.mark.parametrize("change,status", [
     (dict(q=None), -1), (dict(out=None), -1), (dict(freqs=None), -1), (dict(k=None), -1), (dict(dtype=3), -6), (dict(D=1), -2),
     (dict(D=1026), -2), (dict(dims=258, D=512), -2), (dict(dims=66), -2), (dict(dims=7), -2), (dict(dims=0), -2), (dict(B=0), -2),
     (dict(L=0), -2), (dict(B=1 << 13, L=1 << 13), -2), (dict(Hq=0), -2), (dict(Hk=-1), -2), (dict(Hq=5000), -2),
-    (dict(q=(1 << 20) + 1), -3), (dict(pos=1 << 20, ps=None), -1)])
+    (dict(q=(1 << 20) + 1), -3)])
 def test_rope_refuses(change, status):
     """Refused on the host: the pointers are never followed."""
     fake = 1 << 20
-    a = dict(dtype=0, q=fake, Hq=2, k=fake, Hk=1, B=1, L=3, D=64, dims=64, freqs=fake, pos=None, ps=None, out=fake)
+    a = dict(dtype=0, q=fake, Hq=2, k=fake, Hk=1, B=1, L=3, D=64, dims=64, freqs=fake, out=fake)
     a.update(change)
-    st3 = _i64(64, 64, 64)
-    st = _lib.load().dspark_rope(a["dtype"], a["q"], st3, a["Hq"], a["k"], st3, a["Hk"], a["B"], a["L"], a["D"], a["dims"], 0,
-                                 a["freqs"], 1.0, a["pos"], 0, a["ps"], 0, a["out"], st3, fake, st3, None)
+    six = (64,) * 6
+    st = _lib.load().dspark_rope(ops._ROPE_ARGS.pack(a["dtype"], a["q"] or 0, a["out"] or 0, *six, a["Hq"], a["k"] or 0, fake, *six,
+                                                     a["Hk"], a["B"], a["L"], a["D"], a["dims"], 0, a["freqs"] or 0, 1.0, 0, 0, 0,
+                                                     0, 0), None)
+    assert _lib.load().dspark_rope(None, None) == -1
     assert st == status and _lib.load().dspark_last_error()
 
 
@@ -122,20 +118,15 @@ def test_rope_refuses(change, status):
     (dict(w=0), -1), (dict(x=(1 << 20) + 1), -3), (dict(w=(1 << 20) + 2), -3)])
 @pytest.mark.parametrize("write", [True, False])
 def test_kv_refuses(change, status, write):
-    import ctypes
-
     fake = 1 << 20
     a = dict(x_dtype=0, c_dtype=0, x=fake, w=fake, B=1, H=2, T=5, D=64, bits=8, group=64)
     a.update(change)
-    two = lambda v: (ctypes.c_void_p * 2)(v, fake)
-    st6 = _i64(64, 64, 64, 64, 64, 64)
     lib = _lib.load()
-    if write:
-        st = lib.dspark_kv_quantize(a["x_dtype"], two(a["x"]), st6, a["c_dtype"], two(a["w"]), two(fake), two(fake), st6, st6,
-                                    a["B"], a["H"], a["T"], a["D"], a["bits"], a["group"], None)
-    else:
-        st = lib.dspark_kv_dequantize(a["c_dtype"], two(a["w"]), two(fake), two(fake), st6, st6, a["B"], a["H"], a["T"], a["D"],
-                                      a["bits"], a["group"], a["x_dtype"], two(a["x"]), st6, None)
+    call = lib.dspark_kv_quantize if write else lib.dspark_kv_dequantize
+    side = lambda x, w: (x, 64, 64, 64, w, fake, fake, 64, 64, 64, 64, 64, 64)
+    st = call(ops._KV_ARGS.pack(a["x_dtype"], a["c_dtype"], a["B"], a["H"], a["T"], a["D"], a["bits"], a["group"],
+                                *side(a["x"], a["w"]), *side(fake, fake)), None)
+    assert call(None, None) == -1
     assert st == status and lib.dspark_last_error()
 
 
