@@ -12,8 +12,8 @@
 //
 // Every weight is formed and summed in 64 bits, in an order that depends on the sizes alone: which
 // token a random number falls on is decided by differences that fp32 sums over 1e5 tokens do not hold
-// (a token of probability 1e-5 is 1e2 units of an fp32 sum of 1 wide). Vector fp64 runs at the rate of
-// fp32 here, so the exponential (a degree-10 polynomial) costs less than reading the logits does.
+// (a token of probability 1e-5 is 1e2 units of an fp32 sum of 1 wide). An fp64 instruction takes 8 cycles a
+// wave here; a weight takes 16 of them, of which 10 are its polynomial.
 //
 // A row is cut into segments of 512 logits, one wave load of 16 bytes a lane. The first pass leaves the
 // maximum of each segment and its sum of weights against that maximum; whatever follows works on these
@@ -38,6 +38,8 @@ constexpr int kMaxSegs = 1024;         // segments of a row: one LDS slot each i
 constexpr int kMaxDraft = 255;         // drafts of a sequence
 constexpr int kBins = 8192;            // distinct logit values counted at a time
 constexpr int kRowThreads = 1024;      // threads of the kernels that work on one row or sequence
+constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kListed = 256;           // kept tokens of a row that are written out one by one
 
 constexpr int kNoTies = -8;            // a cut below every index, those before a row's first logit too
 
@@ -50,14 +52,15 @@ struct SampleArgs {
   int top_k;                           // 0: none
   float* segm;                         // [rows][nseg] segment maxima
   double* segs;                        // [rows][nseg] segment sums
+  int* arrived;                        // [sequences] workgroups that are done, cleared by the first launch
 };
 
-struct RowInfo {                       // what the later kernels need of a row
+struct RowInfo {                       // what is sampled from of a row
   double z;                            // sum of the kept weights (0: nothing to draw from)
   double px;                           // the drafted token's probability
   float m;                             // the row's maximum
   int thr, cut;                        // kept: key > thr, or key == thr and index <= cut
-  int pad;
+  int listed;                          // kept tokens written out one by one, or -1
 };
 
 struct VerifyIn {
@@ -122,10 +125,12 @@ __device__ __forceinline__ double exp2_neg(double d) {
 }
 
 // The weight of a logit against a maximum m over -inf (1 where they are equal, infinities too; a NaN logit's
-// NaN argument is taken for the smaller operand: 0). Straight code: the weights of a lane's 8 logits overlap.
-__device__ __forceinline__ double weight(float x, float m, double c) {
-  return exp2_neg(x == m ? 0.0 : ((double)x - (double)m) * c);
+// NaN argument is taken for the smaller operand: 0); mc = -m c. Straight code: the weights of a lane's 8
+// logits overlap.
+__device__ __forceinline__ double weight(float x, float m, double c, double mc) {
+  return exp2_neg(x == m ? 0.0 : __builtin_fma((double)x, c, mc));
 }
+__device__ __forceinline__ double weight(float x, float m, double c) { return weight(x, m, c, -(double)m * c); }
 
 // ---------------------------------------------------------------- wave reductions (DPP)
 
@@ -146,6 +151,10 @@ __device__ __forceinline__ float dpp_max(float v) {  // max with the shifted val
   const int lo = __builtin_bit_cast(int, -INFINITY);
   return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(lo, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false)));
 }
+
+// The value of the lane before (0 in lane 0): a shift of the whole wave by one.
+__device__ __forceinline__ double lane_before(double v) { return dpp_d<0x138, 0xF>(v); }
+__device__ __forceinline__ int lane_before(int v) { return dpp_i<0x138, 0xF>(v); }
 
 // Running sums over the lanes of a wave: shifts inside rows of 16 lanes, then the last lane of row 0
 // and 2 into the next row, then that of the lower half into the upper.
@@ -185,9 +194,10 @@ __device__ __forceinline__ float wave_max(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Running sums over the threads of a workgroup, in thread order; `total` is the whole sum.
+// Running sums over the threads of a workgroup, in thread order: what lies before a thread (returned) and up
+// to it (`upto`), the whole in `total`. `waves`: a slot a wave, free again after the next barrier.
 template <typename V>
-__device__ __forceinline__ V block_scan(V v, V* waves, V& total) {
+__device__ __forceinline__ V block_scan(V v, V* waves, V& upto, V& total) {
   const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const V in = wave_scan(v);
   if ((threadIdx.x & 63) == 63) waves[w] = in;
@@ -199,7 +209,25 @@ __device__ __forceinline__ V block_scan(V v, V* waves, V& total) {
   }
   __syncthreads();
   total = all;
-  return before + in;
+  upto = before + in;
+  return before + lane_before(in);
+}
+
+// ---------------------------------------------------------------- between workgroups of a launch
+
+// Written through to, and read from, where every XCD sees it.
+template <typename V>
+__device__ __forceinline__ void put_far(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V>
+__device__ __forceinline__ V get_far(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// True in every thread of the workgroup that arrives last of `n`; what the others put before it is there to get.
+__device__ __forceinline__ bool arrives_last(int* counter, int n, int* slot) {
+  __builtin_amdgcn_s_waitcnt(0);       // this thread's stores are complete
+  __syncthreads();
+  if (threadIdx.x == 0) *slot = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+  __syncthreads();
+  return *slot;
 }
 
 // ---------------------------------------------------------------- segments
@@ -223,30 +251,18 @@ __device__ __forceinline__ u32x4_t load8(const u16* row, int v0, int V) {
 }
 __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >> 1] >> (16 * (j & 1))) & 0xFFFFu; }
 
-__device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int row) {
-  return a.x + (long)(row / a.per) * a.ldb + (long)(row % a.per) * a.ldr;
-}
+__device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int seq, int i) { return a.x + seq * a.ldb + i * a.ldr; }
 
-// The normaliser of a row without a cut, and its maximum: the join of its segments over a workgroup.
-__device__ __forceinline__ double join_segments(const float* segm, const double* segs, int nseg, double c, float* red_f,
-                                                double* red_d, float& m) {
-  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+// Maximum and normaliser of a row without a cut, the join of its segments, by one wave.
+__device__ __forceinline__ double join_wave(const float* segm, const double* segs, int nseg, double c, float& m) {
+  const int lane = threadIdx.x & 63;
   float mx = -INFINITY;
-  for (int s = threadIdx.x; s < nseg; s += blockDim.x) mx = fmaxf(mx, segm[s]);
+  for (int s = lane; s < nseg; s += 64) mx = fmaxf(mx, segm[s]);
   mx = wave_max(mx);
-  if ((threadIdx.x & 63) == 0) red_f[w] = mx;
-  __syncthreads();
-  for (int i = 0; i < nw; ++i) mx = fmaxf(mx, red_f[i]);
   double z = 0;
-  for (int s = threadIdx.x; s < nseg; s += blockDim.x) z += segs[s] * weight(segm[s], mx, c);
-  z = wave_total(z);
-  if ((threadIdx.x & 63) == 0) red_d[w] = z;
-  __syncthreads();
-  z = 0;
-  for (int i = 0; i < nw; ++i) z += red_d[i];
-  __syncthreads();
+  for (int s = lane; s < nseg; s += 64) z += segs[s] * weight(segm[s], mx, c);
   m = mx;
-  return z;
+  return mx > -INFINITY ? wave_total(z) : 0.0;
 }
 
 }  // namespace dspark
