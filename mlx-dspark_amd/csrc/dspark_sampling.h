@@ -36,10 +36,10 @@ namespace dspark {
 constexpr int kSegVals = 512;          // logits of a segment
 constexpr int kMaxSegs = 1024;         // segments of a row: one LDS slot each in the kernels of a row
 constexpr int kMaxDraft = 255;         // drafts of a sequence
-constexpr int kBins = 8192;            // distinct logit values counted at a time
+constexpr int kBins = 30720;           // distinct logit values counted at a time: most of the LDS
 constexpr int kRowThreads = 1024;      // threads of the kernels that work on one row or sequence
 constexpr int kRowWaves = kRowThreads / 64;
-constexpr int kListed = 256;           // kept tokens of a row that are written out one by one
+constexpr int kListed = 256;           // candidates of a row that are sorted instead of counted
 
 constexpr int kNoTies = -8;            // a cut below every index, those before a row's first logit too
 
@@ -60,7 +60,7 @@ struct RowInfo {                       // what is sampled from of a row
   double px;                           // the drafted token's probability
   float m;                             // the row's maximum
   int thr, cut;                        // kept: key > thr, or key == thr and index <= cut
-  int listed;                          // kept tokens written out one by one, or -1
+  int pad;
 };
 
 struct VerifyIn {
@@ -86,23 +86,33 @@ __device__ __forceinline__ float val(u32 bits) {
 template <bool HALF>
 constexpr u32 kInfBits = HALF ? 0x7C00u : 0x7F80u;
 
-// Order of the logits as integers: NaN counts as -inf, -0 as +0.
+// The order of the logits as integers: the magnitude's bits with their sign, so +0 and -0 are equal. A NaN lies
+// outside [kLowKey, -kLowKey], the keys of the infinities.
 template <bool HALF>
-__device__ __forceinline__ int key_of(u32 b) {
-  if ((b & 0x7FFFu) > kInfBits<HALF>) b = 0x8000u | kInfBits<HALF>;
-  if (b == 0x8000u) b = 0;
-  return (int)((b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u));
-}
-template <bool HALF>
-constexpr int kLowKey = (int)(~(0x8000u | kInfBits<HALF>) & 0xFFFFu);  // the key of -inf
+constexpr int kLowKey = -(int)kInfBits<HALF>;
 template <bool HALF>
 __device__ __forceinline__ float val_of_key(int k) {
-  return val<HALF>((k & 0x8000) ? (u32)k & 0x7FFFu : ~(u32)k & 0xFFFFu);
+  return val<HALF>(k < 0 ? 0x8000u | (u32)-k : (u32)k);
 }
 template <bool HALF>
 __device__ __forceinline__ int key_of_float(float f) {
-  if constexpr (HALF) return key_of<HALF>(__builtin_bit_cast(u16, (_Float16)f));
-  else return key_of<HALF>(f2bf(f));
+  int b;
+  if constexpr (HALF) b = (int16_t)__builtin_bit_cast(u16, (_Float16)f);
+  else b = (int16_t)f2bf(f);
+  return b < 0 ? -(b & 0x7FFF) : b;
+}
+
+// The keys of a lane's 8 logits, two at a time.
+typedef int16_t i16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void keys8(const u32x4_t& v, int (&k)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32 two = v[i];              // a value of its own: the cast of a vector's element takes the first one
+    const i16x2_t b = __builtin_bit_cast(i16x2_t, two), s = b >> (int16_t)15;
+    const i16x2_t r = ((b & (int16_t)0x7FFF) ^ s) - s;
+    k[2 * i] = r[0];
+    k[2 * i + 1] = r[1];
+  }
 }
 
 // 2^d for d <= 0: the interpolation of 2^f on [-1/2, 1/2] in 11 Chebyshev nodes (within 5e-15 of itself,
@@ -239,15 +249,15 @@ __device__ __forceinline__ int row_off(const u16* row) { return (int)((reinterpr
 template <bool HALF>
 __device__ __forceinline__ u32x4_t load8(const u16* row, int v0, int V) {
   if (v0 >= 0 && v0 + 8 <= V) return ldg128(row + v0);
-  constexpr u32 ninf = 0x8000u | kInfBits<HALF>;
-  u32x4_t r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int a = v0 + 2 * i, b = a + 1;
-    const u32 lo = (a >= 0 && a < V) ? row[a] : ninf, hi = (b >= 0 && b < V) ? row[b] : ninf;
-    r[i] = lo | (hi << 16);
+  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {        // a row's ends: one at a time, the first shifted down to the lowest bits
+    const int v = v0 + i;
+    const uint64_t b = v >= 0 && v < V ? row[v] : 0x8000u | kInfBits<HALF>;
+    lo = lo >> 16 | hi << 48;
+    hi = hi >> 16 | b << 48;
   }
-  return r;
+  return u32x4_t{(u32)lo, (u32)(lo >> 32), (u32)hi, (u32)(hi >> 32)};
 }
 __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >> 1] >> (16 * (j & 1))) & 0xFFFFu; }
 

@@ -52,53 +52,73 @@ constexpr int kAhead = 4;              // segments of a wave whose loads are out
 struct RowShared {
   union {
     int bins[kBins];
-    struct {
-      uint64_t cand[kListed];          // key << 32 | ~index: the larger the earlier in falling order
+    struct {                           // a few candidates, one by one
+      uint64_t cand[kListed];          // (key + 2^15) << 32 | ~index: the larger the earlier in falling order
       uint64_t sorted[kListed];
+      double w[kListed], r[kListed];   // weights in falling order; what is drawn from, by index
+      int order[kListed];              // the kept tokens by index
     };
   };
   int skey[kMaxSegs];                  // key of each segment's maximum
-  int list[kMaxSegs];                  // the segments that may hold a kept token, in order
+  int list[kMaxSegs];                  // the segments that may hold a kept token, in no order
   int cnt[kMaxSegs];
   double red_d[kRowWaves];
   float red_f[kRowWaves];
   int red_i[kRowWaves];
-  int owner, key, keep, ties, kb, cut, ncand, last;
-  double z, px;
+  int owner, key, keep, ties, cut, nlist, ncand, last, token;
+  double z;
 };
 
-// The largest key that at least k of the n (<= kMaxSegs) values reach, bit by bit: one wave, 16 values a lane.
-__device__ __forceinline__ int kth_key(const int* v, int n, int k) {
-  const int lane = threadIdx.x & 63;
-  int mine[kMaxSegs / 64];
-#pragma unroll
-  for (int i = 0; i < kMaxSegs / 64; ++i) mine[i] = 64 * i + lane < n ? v[64 * i + lane] : -1;
-  int key = 0;
-  for (int bit = 1 << 15; bit; bit >>= 1) {
+// The largest key that at least k of the n (<= kMaxSegs) values reach: 4 bits a round, a wave for each of the 16
+// keys a round tries. `counts`: a slot a wave.
+__device__ __forceinline__ int kth_key(const int* v, int n, int k, int* counts) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int key = -(1 << 15);
+  for (int shift = 12; shift >= 0; shift -= 4) {
+    const int tried = key + (wave << shift);
     int c = 0;
-#pragma unroll
-    for (int i = 0; i < kMaxSegs / 64; ++i)
-      if (64 * i < n) c += __popcll(__ballot(mine[i] >= (key | bit)));
-    if (c >= k) key |= bit;
+    for (int i = 0; i < n; i += 64) c += __popcll(__ballot(i + lane < n && v[i + lane] >= tried));
+    if (lane == 0) counts[wave] = c;
+    __syncthreads();
+    const unsigned long long enough = __ballot(lane < kRowWaves && counts[lane & (kRowWaves - 1)] >= k);
+    key += (enough ? 63 - __clzll(enough) : 0) << shift;
+    __syncthreads();
   }
   return key;
 }
 
-// Calls f(segment's place in the list, its 8 logits of this lane) for every listed segment, a wave at a time.
+// The segments whose maximum reaches `lo`, into sh.list; their number in sh.nlist (0 on entry).
+__device__ __forceinline__ int list_segments(RowShared& sh, int nseg, int lo) {
+  const int t = threadIdx.x, lane = t & 63;
+  const bool f = t < nseg && sh.skey[t] >= lo;                 // kMaxSegs <= kRowThreads
+  const unsigned long long on = __ballot(f);
+  int base = 0;
+  if (on) {
+    if (lane == 0) base = atomicAdd(&sh.nlist, __popcll(on));
+    base = __builtin_amdgcn_readfirstlane(base);
+    if (f) sh.list[base + __popcll(on & ((1ull << lane) - 1))] = t;
+  }
+  __syncthreads();
+  return sh.nlist;
+}
+
+// Calls f(segment, its 8 logits of this lane) for every listed segment, a wave at a time.
 template <bool HALF, typename F>
 __device__ __forceinline__ void each_listed(const SampleArgs& a, const u16* x, int off, const int* list, int nlist, F&& f) {
   const int lane = threadIdx.x & 63;
   for (int i0 = uniform(threadIdx.x >> 6); i0 < nlist; i0 += kAhead * kRowWaves) {
     u32x4_t v[kAhead];
+    int s[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * kRowWaves;
-      if (i < nlist) v[u] = load8<HALF>(x, list[i] * kSegVals + 8 * lane - off, a.V);
+      s[u] = i < nlist ? uniform(list[i]) : -1;
+      if (s[u] >= 0) v[u] = load8<HALF>(x, s[u] * kSegVals + 8 * lane - off, a.V);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (i0 + u * kRowWaves >= nlist) break;
-      f(i0 + u * kRowWaves, v[u]);
+      if (s[u] < 0) break;
+      f(s[u], v[u]);
     }
   }
 }
@@ -110,51 +130,98 @@ __device__ __forceinline__ void count_keys(const SampleArgs& a, const u16* x, in
   for (int i = threadIdx.x; i <= hi - lo; i += kRowThreads) sh.bins[i] = 0;
   __syncthreads();
   each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) {
+    int k[8];
+    keys8(v, k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int k = key_of<HALF>(bits_of(v, j));
-      if (k >= lo && k <= hi) atomicAdd(&sh.bins[hi - k], 1);
+      const u32 b = (u32)(hi - k[j]);
+      if (b <= (u32)(hi - lo)) atomicAdd(&sh.bins[b], 1);
     }
   });
   __syncthreads();
 }
 
-// The part of one row that is sampled from: its threshold and normaliser (RowInfo), and px of token `draft`.
-// Up to kListed of its tokens are written out as (index, weight) in falling order.
+// The weights of falling keys, one after another: inside an octave the values are evenly spaced, so each weight is
+// the one before times a constant. A power of two is formed anew at each octave's end.
 template <bool HALF>
-__device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int ri, int draft, RowShared& sh, int* out_idx,
-                                              double* out_w) {
+struct FallingWeights {
+  int key, left;
+  double w, ratio;
+  __device__ __forceinline__ void start(int k, float m, double c, double mc) {
+    constexpr int kOctave = HALF ? 1024 : 128;
+    const float x = val_of_key<HALF>(k);
+    key = k;
+    w = weight(x, m, c, mc);
+    left = k > 0 ? ((k - 1) & (kOctave - 1)) + 1 : kOctave - (-k & (kOctave - 1));
+    ratio = exp2_neg(((double)val_of_key<HALF>(k - 1) - (double)x) * c);
+  }
+  __device__ __forceinline__ void next(float m, double c, double mc) {
+    if (--left == 0) start(key - 1, m, c, mc);
+    else {
+      w *= ratio;
+      --key;
+    }
+  }
+};
+
+// p of a token of logit x (-inf for one outside the vocabulary)
+template <bool HALF>
+__device__ __forceinline__ double px_of(const SampleArgs& a, const RowInfo& r, int v, float x) {
+  if (!(x > -INFINITY && r.z > 0)) return 0;          // NaN too
+  const int k = key_of_float<HALF>(x);
+  return k > r.thr || (k == r.thr && v <= r.cut) ? weight(x, r.m, a.c) / r.z : 0;
+}
+
+// Four values a lane, in thread order over the 256 of one wave: their running sums' start and the whole.
+__device__ __forceinline__ double scan4(const double (&v)[4], double& total) {
+  const double in = wave_scan((v[0] + v[1]) + (v[2] + v[3]));
+  total = lane_value(in, 63);
+  return lane_before(in);
+}
+
+enum { kDrawRow = 0, kDrawRest = 1, kDrawOther = 2 };   // r = p, max(p - q, 0), p without one token
+
+struct DrawIn {                        // what a row's own draw goes by
+  int mode, skip;                      // mode < 0: none
+  const float* q;
+  double u;
+};
+
+// The part of one row that is sampled from: its threshold and normaliser (RowInfo), and px of token `draft`. Where
+// the candidates are few, the token drawn from the row too (d.mode >= 0; -1 where it was not).
+template <bool HALF>
+__device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, RowShared& sh,
+                                              int& token) {
   const int t = threadIdx.x, lane = t & 63;
   const u16* x = row_ptr(a, seq, ri);
   const int off = row_off(x);
   const long row = (long)seq * a.per + ri;
   const float sm = t < a.nseg ? a.segm[row * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
   const double ss = !a.top_k && t < a.nseg ? a.segs[row * a.nseg + t] : 0;
-  const u32 dbits = draft >= 0 && draft < a.V ? x[draft] : 0x8000u | kInfBits<HALF>;
+  const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
   RowInfo out;
+  token = -1;
   float mx = wave_max(sm);
   if (lane == 0) sh.red_f[t >> 6] = mx;
   if (t < a.nseg) sh.skey[t] = key_of_float<HALF>(sm);
-  if (t == 0) {
-    sh.ncand = 0;
-    sh.px = 0;
-  }
+  if (t == 0) sh.ncand = sh.nlist = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) mx = fmaxf(mx, sh.red_f[i]);
   out.m = mx;
   out.px = 0;
-  out.listed = -1;
+  out.pad = 0;
   if (!(mx > -INFINITY)) {              // nothing to draw from
     out.z = 0;
     out.thr = 1 << 16;
     out.cut = kNoTies;
-    out.listed = 0;
+    token = 0;
     return out;
   }
+  const double mc = -(double)mx * a.c;
   double total = 0;                     // of the whole row; needed where the mass itself is cut
   if (!a.top_k) {
-    const double part = wave_total(ss * weight(sm, mx, a.c));
+    const double part = wave_total(ss * weight(sm, mx, a.c, mc));
     if (lane == 0) sh.red_d[t >> 6] = part;
     __syncthreads();
 #pragma unroll
@@ -163,62 +230,50 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
   const int top = key_of_float<HALF>(mx);
 
   // a key that every kept token reaches
-  if (a.top_k && a.nseg < a.top_k && a.nseg <= kMaxSegs / 8) {
+  int kb = kLowKey<HALF>;
+  if (!a.top_k) {
+    // tokens of weight (1 - top_p) S / V or less: all together less than (1 - top_p) S. One key of room for the
+    // rounding to 16 bits.
+    const double w = (1.0 - a.top_p) * total / (double)a.V;
+    kb = key_of_float<HALF>((float)((double)mx + log2(w) / a.c)) - 1;
+  } else if (a.nseg >= a.top_k) {
+    kb = kth_key(sh.skey, a.nseg, a.top_k, sh.red_i);
+  } else if (8 * a.nseg >= a.top_k && a.nseg <= kMaxSegs / 8) {
     // few segments: the maxima of groups of 8 lanes instead
     for (int s = uniform(t >> 6); s < a.nseg; s += kRowWaves) {
       const u32x4_t v = load8<HALF>(x, s * kSegVals + 8 * lane - off, a.V);
-      int k = key_of<HALF>(bits_of(v, 0));
+      int ks[8], k = kLowKey<HALF>;
+      keys8(v, ks);
 #pragma unroll
-      for (int j = 1; j < 8; ++j) k = max(k, key_of<HALF>(bits_of(v, j)));
+      for (int j = 0; j < 8; ++j) k = max(k, ks[j] <= top ? ks[j] : k);
       k = max(k, dpp_i<0xB1, 0xF>(k));   // the exchanges of sum8_lanes
       k = max(k, dpp_i<0x4E, 0xF>(k));
       k = max(k, dpp_i<0x141, 0xF>(k));
       if ((lane & 7) == 0) sh.cnt[8 * s + (lane >> 3)] = k;
     }
     __syncthreads();
-    if (t < 64) {
-      const int kb = 8 * a.nseg >= a.top_k ? kth_key(sh.cnt, 8 * a.nseg, a.top_k) : 0;
-      if (t == 0) sh.kb = min(max(kb, kLowKey<HALF> + 1), top);
-    }
-  } else if (t < 64) {
-    int kb = 0;
-    if (a.top_k) {
-      if (a.nseg >= a.top_k) kb = kth_key(sh.skey, a.nseg, a.top_k);
-    } else {
-      // tokens of weight (1 - top_p) S / V or less: all together less than (1 - top_p) S. One key of room
-      // for the rounding to 16 bits.
-      const double w = (1.0 - a.top_p) * total / (double)a.V;
-      kb = key_of_float<HALF>((float)((double)mx + log2(w) / a.c)) - 1;
-    }
-    if (t == 0) sh.kb = min(max(kb, kLowKey<HALF> + 1), top);
+    kb = kth_key(sh.cnt, 8 * a.nseg, a.top_k, sh.red_i);
   }
-  __syncthreads();
-  const int kb = sh.kb;
-  int nlist;
-  {
-    const int f = t < a.nseg && sh.skey[t] >= kb;
-    int upto;
-    const int at = block_scan(f, sh.red_i, upto, nlist);
-    if (f) sh.list[at] = t;
-  }
-  __syncthreads();
+  kb = min(max(kb, kLowKey<HALF> + 1), top);
+  int nlist = list_segments(sh, a.nseg, kb);
 
-  // few candidates: sort them
-  if (nlist <= kAhead * kRowWaves) {
-    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int i, const u32x4_t& v) {
-      const int v0 = sh.list[i] * kSegVals + 8 * lane - off;
-      int n = 0;
+  // Few candidates are sorted. A top_k leaves little more than that many; a mass alone may leave most of a segment,
+  // so that only rows where few segments reach are tried.
+  if (nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves)) {
+    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
+      const int v0 = s * kSegVals + 8 * lane - off;
+      int n = 0, ks[8];
+      keys8(v, ks);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) n += key_of<HALF>(bits_of(v, j)) >= kb;
+      for (int j = 0; j < 8; ++j) n += ks[j] >= kb && ks[j] <= top;
       const int upto = wave_scan(n);
       int base = 0;
       if (lane == 63) base = atomicAdd(&sh.ncand, upto);
       int at = __builtin_amdgcn_readlane(base, 63) + upto - n;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int k = key_of<HALF>(bits_of(v, j));
-        if (k >= kb) {
-          if (at < kListed) sh.cand[at] = (uint64_t)(u32)k << 32 | (u32)~(v0 + j);
+        if (ks[j] >= kb && ks[j] <= top) {
+          if (at < kListed) sh.cand[at] = (uint64_t)(u32)(ks[j] + (1 << 15)) << 32 | (u32)~(v0 + j);
           ++at;
         }
       }
@@ -233,35 +288,91 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
         sh.sorted[r] = me;
       }
       __syncthreads();
-      const uint64_t me = t < n ? sh.sorted[t] : 0;
-      const int key = (int)(me >> 32), idx = (int)~(u32)me;
-      const double w = t < n && !(a.top_k && t >= a.top_k) ? weight(val_of_key<HALF>(key), mx, a.c) : 0.0;
-      double upto, zk;
-      const double before = block_scan(w, sh.red_d, upto, zk);
-      const double goal = a.top_p * (a.top_k ? zk : total);
-      const int nk = a.top_k ? min(a.top_k, n) : n;
-      if (t == 0) sh.keep = nk;
-      __syncthreads();
-      if (a.top_p < 1.0 && t < nk && before >= goal) atomicMin(&sh.keep, t);
-      __syncthreads();
-      const int kept = sh.keep;         // at least 1: before is 0 at the first, the goal is not
-      if (t == kept - 1) {
-        sh.z = upto;
-        sh.key = key;
-        sh.cut = idx;
+      const int idx = t < n ? (int)~(u32)sh.sorted[t] : 0;
+      const float qv = d.mode == kDrawRest && t < n ? d.q[idx] : 0.f;      // on its way over the next step
+      if (t < 64) {                     // the first wave, four a lane: what of the top_k lies before the mass
+        double w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * t + i;
+          w[i] = j < n && !(a.top_k && j >= a.top_k)
+                     ? weight(val_of_key<HALF>((int)(sh.sorted[j] >> 32) - (1 << 15)), mx, a.c, mc) : 0.0;
+          if (j < n) sh.w[j] = w[i];
+        }
+        double zk;
+        double run = scan4(w, zk);
+        const double goal = a.top_p * (a.top_k ? zk : total);
+        const int nk = a.top_k ? min(a.top_k, n) : n;
+        int kept = nk;                  // tokens of this lane or before it that are kept, if the cut is here
+        double z = zk;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {  // the first at which the goal is reached, from the lane's last
+          const double before = i == 0 ? run : i == 1 ? run + w[0] : i == 2 ? run + w[0] + w[1] : run + w[0] + w[1] + w[2];
+          if (4 * t + i < nk && before >= goal && a.top_p < 1.0) {
+            kept = 4 * t + i;
+            z = before;
+          }
+        }
+        const unsigned long long hit = __ballot(kept < nk);
+        if (hit) {
+          const int at = __ffsll(hit) - 1;
+          kept = __builtin_amdgcn_readlane(kept, at);
+          z = lane_value(z, at);
+        }
+        if (t == 0) {
+          sh.keep = kept;               // at least 1: before is 0 at the first, the goal is not
+          sh.z = z;
+          sh.key = (int)(sh.sorted[kept - 1] >> 32) - (1 << 15);
+          sh.cut = (int)~(u32)sh.sorted[kept - 1];
+        }
       }
       __syncthreads();
+      const int kept = sh.keep;
       out.z = sh.z;
       out.thr = sh.key;
       out.cut = sh.cut;
-      out.listed = kept;
-      if (out_idx && t < kept) {
-        put_far(out_idx + t, idx);
-        put_far(reinterpret_cast<uint64_t*>(out_w) + t, __builtin_bit_cast(uint64_t, w));
+      out.px = px_of<HALF>(a, out, draft, xd);
+      if (d.mode < 0) return out;
+      // the draw: r by index, then the first wave, four a lane
+      if (t < kept) {
+        int at = 0;
+        for (int i = 0; i < kept; ++i) at += (int)~(u32)sh.sorted[i] < idx;
+        double r = sh.w[t];
+        if (d.mode == kDrawRest) r = __builtin_fmax(r / out.z - (double)qv, 0.0);
+        else if (d.mode == kDrawOther && idx == d.skip) r = 0;
+        sh.r[at] = r;
+        sh.order[at] = t;
       }
-      const int dk = key_of<HALF>(dbits);
-      if (draft >= 0 && draft < a.V && (dk > out.thr || (dk == out.thr && draft <= out.cut)))
-        out.px = weight(val<HALF>(dbits), mx, a.c) / out.z;
+      __syncthreads();
+      if (t < 64) {
+        double r[4], all = 0, run = 0;
+        for (int tries = 0; tries < 2; ++tries) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = 4 * t + i;
+            r[i] = j < kept ? (tries ? sh.w[sh.order[j]] : sh.r[j]) : 0.0;      // r zero throughout: p
+          }
+          run = scan4(r, all);
+          if (all > 0) break;
+        }
+        const double goal = d.u * all;
+        int pick = kListed, last = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          run += r[i];
+          if (r[i] > 0) {
+            last = 4 * t + i;
+            if (run > goal && pick == kListed) pick = last;
+          }
+        }
+        const unsigned long long hit = __ballot(pick < kListed), any = __ballot(last >= 0);
+        // the last one with any mass where none passes the goal by a rounding
+        const int j = hit ? __builtin_amdgcn_readlane(pick, __ffsll(hit) - 1)
+                          : any ? __builtin_amdgcn_readlane(last, 63 - __clzll(any)) : -1;
+        if (t == 0) sh.token = j >= 0 ? (int)~(u32)sh.sorted[sh.order[j]] : 0;
+      }
+      __syncthreads();
+      token = sh.token;
       return out;
     }
     __syncthreads();
@@ -290,16 +401,22 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
         count_keys<HALF>(a, x, off, sh, nlist, hi, lo);
         loaded = hi == top ? lo : 1 << 17;
       }
-      const int nb = hi - lo + 1, each = (nb + kRowThreads - 1) / kRowThreads;
+      // a run of bins a thread, an odd number of them: neighbours read other banks
+      const int nb = hi - lo + 1, each = ((nb + kRowThreads - 1) / kRowThreads) | 1;
+      static_assert(kBins / kRowThreads < 64, "a lane for every bin of a run");
       const int b0 = min(t * each, nb), b1 = min(b0 + each, nb);
       int cn = 0;
       double cm = 0;
-      for (int b = b0; b < b1; ++b) {
-        int n = sh.bins[b];
-        if (!n) continue;
-        if (after_k && hi - b == thr_k) n = keep_k;
-        cn += n;
-        cm += (double)n * weight(val_of_key<HALF>(hi - b), mx, a.c);
+      if (b0 < b1) {
+        FallingWeights<HALF> f;
+        f.start(hi - b0, mx, a.c, mc);
+        for (int b = b0; b < b1; ++b) {
+          int n = sh.bins[b];
+          if (after_k && hi - b == thr_k) n = keep_k;
+          cn += n;
+          cm += (double)n * f.w;
+          if (b + 1 < b1) f.next(mx, a.c, mc);
+        }
       }
       if (t == 0) sh.owner = kRowThreads;
       int cnt_all, cnt_end;
@@ -310,40 +427,38 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
       const bool mine = pass == 0 ? seen + cnt_end >= a.top_k && cn : mass + mass_end >= goal && cn;
       if (mine) atomicMin(&sh.owner, t);
       __syncthreads();
-      if (sh.owner == t) {
-        int run = seen + cnt_before, r = 0;
-        double m0 = mass + mass_before;
-        bool hit = false;
-        for (int b = b0; b < b1 && !hit; ++b) {
-          int n = sh.bins[b];
-          if (!n) continue;
-          const int all = n;
-          if (after_k && hi - b == thr_k) n = keep_k;
-          const double w = weight(val_of_key<HALF>(hi - b), mx, a.c);
-          if (pass == 0) {
-            hit = run + n >= a.top_k;
-            r = hit ? a.top_k - run : n;
-          } else {
-            hit = m0 + (double)n * w >= goal;
-            r = n;
-            if (hit) {                  // tokens of this value before which less than the goal lies
-              r = (int)fmin(fmax(__builtin_ceil((goal - m0) / w), 1.0), (double)n);
-              while (r > 1 && m0 + (double)(r - 1) * w >= goal) --r;
-              while (r < n && m0 + (double)r * w < goal) ++r;
-            }
+      const int owner = sh.owner;
+      if (owner < kRowThreads && (t >> 6) == (owner >> 6)) {     // its wave, a bin a lane
+        const int run_c = __builtin_amdgcn_readlane(seen + cnt_before, owner & 63);
+        const double run_m = lane_value(mass + mass_before, owner & 63);
+        const int b = owner * each + lane;
+        const bool in = lane < each && b < nb;
+        const int n_all = in ? sh.bins[b] : 0;
+        const int n = after_k && hi - b == thr_k && in ? keep_k : n_all;
+        const double w = in ? weight(val_of_key<HALF>(hi - b), mx, a.c, mc) : 0.0;
+        const int c_end = run_c + wave_scan(n), c0 = c_end - n;
+        const double m_in = wave_scan((double)n * w), m0 = run_m + lane_before(m_in), m_end = run_m + m_in;
+        const bool reach = n && (pass == 0 ? c_end >= a.top_k : m_end >= goal);
+        const unsigned long long hit = __ballot(reach), any = __ballot(n > 0);
+        const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(any);       // the last of the run but for a rounding
+        if (lane == at) {
+          int r = n;
+          if (hit && pass == 0) r = a.top_k - c0;
+          if (hit && pass == 1) {       // tokens of this value before which less than the goal lies
+            r = (int)fmin(fmax(__builtin_ceil((goal - m0) / w), 1.0), (double)n);
+            while (r > 1 && m0 + (double)(r - 1) * w >= goal) --r;
+            while (r < n && m0 + (double)r * w < goal) ++r;
           }
-          run += n;
-          m0 += (double)r * w;
           sh.key = hi - b;
           sh.keep = r;
-          sh.ties = all;
-          sh.z = m0;
+          sh.ties = n_all;
+          sh.z = m0 + (double)r * w;
         }
       }
       __syncthreads();
       seen += cnt_all;
       mass += mass_all;
-      found = sh.owner < kRowThreads;
+      found = owner < kRowThreads;
       if (found) {
         thr = sh.key;
         keep = sh.keep;
@@ -363,38 +478,42 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
   out.z = z;
   out.cut = ties ? a.V : kNoTies;       // without a threshold value (thr = kb - 1) no token has that key
   if (keep < ties) {                    // the index of the last kept token of the threshold's value
-    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int i, const u32x4_t& v) {
-      int n = 0;
+    if (t == 0) sh.nlist = 0;
+    if (t < a.nseg) sh.cnt[t] = 0;
+    __syncthreads();
+    nlist = list_segments(sh, a.nseg, thr);
+    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
+      int n = 0, ks[8];
+      keys8(v, ks);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) n += __popcll(__ballot(key_of<HALF>(bits_of(v, j)) == thr));
-      if (lane == 0) sh.cnt[i] = n;
+      for (int j = 0; j < 8; ++j) n += __popcll(__ballot(ks[j] == thr));
+      if (lane == 0) sh.cnt[s] = n;
     });
     __syncthreads();
-    const int c = t < nlist ? sh.cnt[t] : 0;
+    const int c = t < a.nseg ? sh.cnt[t] : 0;
     int upto, all;
     const int before = block_scan(c, sh.red_i, upto, all);
     if (before < keep && keep <= upto) {
-      sh.owner = sh.list[t];
+      sh.owner = t;
       sh.keep = keep - before;
     }
     __syncthreads();
     if (t < 64) {
       const int v0 = sh.owner * kSegVals + 8 * lane - off, want = sh.keep;
       const u32x4_t v = load8<HALF>(x, v0, a.V);
-      int n = 0;
+      int n = 0, ks[8];
+      keys8(v, ks);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) n += key_of<HALF>(bits_of(v, j)) == thr;
+      for (int j = 0; j < 8; ++j) n += ks[j] == thr;
       int run = wave_scan(n) - n;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (key_of<HALF>(bits_of(v, j)) == thr && ++run == want) sh.cut = v0 + j;
+        if (ks[j] == thr && ++run == want) sh.cut = v0 + j;
     }
     __syncthreads();
     out.cut = sh.cut;
   }
-  const int dk = key_of<HALF>(dbits);
-  if (draft >= 0 && draft < a.V && z > 0 && (dk > out.thr || (dk == out.thr && draft <= out.cut)))
-    out.px = weight(val<HALF>(dbits), mx, a.c) / z;
+  out.px = px_of<HALF>(a, out, draft, xd);
   return out;
 }
 
@@ -415,7 +534,15 @@ __device__ __forceinline__ bool refused(const SampleArgs& a, const VerifyIn& in,
   return !(inside && uniform_at(in, (long)seq * a.per + i) * q < px);
 }
 
-enum { kDrawRow = 0, kDrawRest = 1, kDrawOther = 2 };   // r = p, max(p - q, 0), p without one token
+// How the token of row i is drawn if its draft is the first refused, or it is the row after the last draft.
+__device__ __forceinline__ DrawIn draw_in(const SampleArgs& a, const VerifyIn& in, int seq, int i, int len) {
+  DrawIn d;
+  d.mode = i == len ? kDrawRow : in.q ? kDrawRest : kDrawOther;
+  d.q = d.mode == kDrawRest ? in.q + seq * in.qb + i * in.qr : nullptr;
+  d.skip = i < len ? in.draft[(long)seq * (a.per - 1) + i] : -1;
+  d.u = uniform_at(in, (long)seq * a.per + a.per - 1);
+  return d;
+}
 
 // r of 8 logits from index v0 (logits outside the row are -inf: no weight, q not read). Without a cut every
 // logit's weight is formed; with one, those of which some lane keeps its own.
@@ -423,14 +550,15 @@ template <bool HALF, bool CUT>
 __device__ __forceinline__ void rest8(const SampleArgs& a, const RowInfo& r, double inv, const u32x4_t& x, int v0, int mode,
                                       const float* q, int skip, double (&out)[8]) {
   const double mc = -(double)r.m * a.c;
+  int ks[8];
+  keys8(x, ks);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const u32 b = bits_of(x, j);
-    const int k = key_of<HALF>(b), v = v0 + j;
-    const bool kept = k > r.thr || (k == r.thr && v <= r.cut);
+    const int k = ks[j], v = v0 + j;
+    const bool kept = k > r.thr || (k == r.thr && v <= r.cut);       // a NaN's weight is 0
     double w = 0;
     if (!CUT || __any(kept)) {
-      w = weight(val<HALF>(b), r.m, a.c, mc);
+      w = weight(val<HALF>(bits_of(x, j)), r.m, a.c, mc);
       if (mode == kDrawRest) w = __builtin_fmax(w * inv - (kept && v >= 0 && v < a.V ? (double)q[v] : 0.0), 0.0);
       else if (mode == kDrawOther && v == skip) w = 0;
       w = kept ? w : 0.0;
@@ -441,88 +569,48 @@ __device__ __forceinline__ void rest8(const SampleArgs& a, const RowInfo& r, dou
 
 struct DrawShared {
   double sums[kMaxSegs];
-  double r[kListed];
-  int list[kMaxSegs];                  // segments with a kept token; or the listed tokens, then in order of index
   double red[kRowWaves];
   double before;
-  int red_i[kRowWaves];
-  int seg, last, token, first;
+  int list[kMaxSegs];                  // segments with a kept token
+  int nlist, seg, last, token, first;
 };
 
 // The token drawn from row ri of a sequence: the first whose running sum of r passes u times the whole.
-// `rest`: segment sums of max(p - q, 0) (no cut), `idx` / `w`: the listed tokens (RowInfo::listed >= 0).
+// `rest`: segment sums of max(p - q, 0) (no cut).
 template <bool HALF, bool CUT>
-__device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r, int seq, int ri, int mode, const float* q,
-                                          int skip, double u, const double* rest, const int* idx, const double* w_list,
-                                          DrawShared& sh) {
+__device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r, int seq, int ri, const DrawIn& d,
+                                          const double* rest, DrawShared& sh) {
   const int t = threadIdx.x, lane = t & 63;
   const u16* x = row_ptr(a, seq, ri);
   const int off = row_off(x);
   const long row = (long)seq * a.per + ri;
   const double inv = r.z > 0 ? 1.0 / r.z : 0.0;
+  int mode = d.mode;
   if (t == 0) {
     sh.token = 0;
     sh.seg = kMaxSegs;
     sh.last = -1;
-  }
-  if (CUT && r.listed >= 0) {           // one token a thread, in the order of their indexes
-    const int n = r.listed;
-    int me = 0;
-    double v = 0;
-    if (t < n) {
-      me = get_far(idx + t);
-      const double w = __builtin_bit_cast(double, get_far(reinterpret_cast<const uint64_t*>(w_list) + t));
-      v = w;
-      if (mode == kDrawRest) v = __builtin_fmax(w * inv - (double)q[me], 0.0);
-      else if (mode == kDrawOther && me == skip) v = 0;
-      sh.list[t] = me;
-      sh.sums[t] = w;
-    }
-    __syncthreads();
-    int at = 0;
-    if (t < n)
-      for (int i = 0; i < n; ++i) at += sh.list[i] < me;
-    double all = 0, upto = 0;
-    for (int tries = 0; tries < 2; ++tries) {
-      if (t < n) {
-        sh.r[at] = tries ? sh.sums[t] : v;
-        sh.list[kListed + at] = me;
-      }
-      __syncthreads();
-      block_scan(t < n ? sh.r[t] : 0.0, sh.red, upto, all);
-      if (all > 0 || mode == kDrawRow) break;
-      mode = kDrawRow;                  // r is zero throughout: p
-    }
-    if (t < n && sh.r[t] > 0) {
-      atomicMax(&sh.last, t);
-      if (upto > u * all) atomicMin(&sh.seg, t);
-    }
-    __syncthreads();
-    const int pick = sh.seg < kMaxSegs ? sh.seg : sh.last;
-    return pick >= 0 ? sh.list[kListed + pick] : 0;
+    sh.nlist = 0;
   }
   // sums of r over the segments; where r is zero throughout, of p
   const float sm = t < a.nseg ? a.segm[row * a.nseg + t] : -INFINITY;
   double all = 0, before = 0, upto = 0, mine = 0;
+  if constexpr (CUT) {
+    __syncthreads();
+    const bool f = r.z > 0 && t < a.nseg && key_of_float<HALF>(sm) >= r.thr;
+    if (f) sh.list[atomicAdd(&sh.nlist, 1)] = t;
+    sh.sums[t] = 0;                     // kMaxSegs == kRowThreads
+    __syncthreads();
+  }
   for (int tries = 0; tries < 2; ++tries) {
     if constexpr (CUT) {
-      sh.sums[t] = 0;                   // kMaxSegs == kRowThreads
-      __syncthreads();
-      int n;
-      {
-        const int f = r.z > 0 && t < a.nseg && key_of_float<HALF>(sm) >= r.thr;
-        int up;
-        const int at = block_scan(f, sh.red_i, up, n);
-        if (f) sh.list[at] = t;
-      }
-      __syncthreads();
-      each_listed<HALF>(a, x, off, sh.list, n, [&](int i, const u32x4_t& v) {
+      each_listed<HALF>(a, x, off, sh.list, sh.nlist, [&](int s, const u32x4_t& v) {
         double w[8], sum = 0;
-        rest8<HALF, true>(a, r, inv, v, sh.list[i] * kSegVals + 8 * lane - off, mode, q, skip, w);
+        rest8<HALF, true>(a, r, inv, v, s * kSegVals + 8 * lane - off, mode, d.q, d.skip, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += w[j];
         sum = wave_total(sum);
-        if (lane == 0) sh.sums[sh.list[i]] = sum;
+        if (lane == 0) sh.sums[s] = sum;
       });
     } else {
       if (t < a.nseg) {
@@ -530,10 +618,10 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
         else sh.sums[t] = r.z > 0 ? a.segs[row * a.nseg + t] * weight(sm, r.m, a.c) : 0.0;
       }
       __syncthreads();
-      if (mode == kDrawOther && skip >= 0 && skip < a.V && t < 64) {   // the token's own segment again, without it
-        const int s = (skip + off) / kSegVals, v0 = s * kSegVals + 8 * lane - off;
+      if (mode == kDrawOther && d.skip >= 0 && d.skip < a.V && t < 64) {   // the token's own segment again, without it
+        const int s = (d.skip + off) / kSegVals, v0 = s * kSegVals + 8 * lane - off;
         double w[8], sum = 0;
-        rest8<HALF, false>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, nullptr, skip, w);
+        rest8<HALF, false>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, nullptr, d.skip, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += w[j];
         sum = wave_total(sum);
@@ -547,7 +635,7 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
     mode = kDrawRow;
   }
   // the first segment whose running sum passes the goal (the last one with any mass if none does by a rounding)
-  const double goal = u * all;
+  const double goal = d.u * all;
   if (mine > 0) {
     atomicMax(&sh.last, t);
     if (upto > goal) atomicMin(&sh.seg, t);
@@ -560,7 +648,7 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
     if (t < 64) {
       const int v0 = s * kSegVals + 8 * lane - off;
       double w[8], sum = 0;
-      rest8<HALF, CUT>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, q, skip, w);
+      rest8<HALF, CUT>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, d.q, d.skip, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += w[j];
       const double to = sh.before + wave_scan(sum);
@@ -598,45 +686,59 @@ struct CutShared {
   DrawShared draw;
 };
 
-// With a cut: one row a workgroup; the last of a sequence accepts and draws (VERIFY).
+// With a cut: one row a workgroup. Where its candidates are few it draws its token too, in case its draft is the
+// first refused (the random number of the draw is there from the start); the last workgroup of a sequence
+// accepts, and draws from the row it comes to where that is still to do (VERIFY).
 template <bool HALF, bool VERIFY>
 __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
-                                                                 int* list_idx, double* list_w) {
+                                                                 uint64_t* drawn) {
   __shared__ CutShared sh;
   const int ri = blockIdx.x, seq = blockIdx.y, m = a.per - 1, t = threadIdx.x;
   const long row = (long)seq * a.per + ri;
-  const int draft = VERIFY && ri < m ? in.draft[(long)seq * m + ri] : -1;
-  const RowInfo mine = select_row<HALF>(a, seq, ri, draft, sh.row, VERIFY ? list_idx + row * kListed : nullptr,
-                                        VERIFY ? list_w + row * kListed : nullptr);
+  DrawIn d = {-1, -1, nullptr, 0.0};
+  int draft = -1, len = 0;
+  double uq = 0;
+  if constexpr (VERIFY) {
+    len = drafts_of(a, in, seq);
+    if (ri < m) draft = in.draft[(long)seq * m + ri];
+    if (ri <= len) d = draw_in(a, in, seq, ri, len);
+    const bool inside = draft >= 0 && draft < a.V;
+    if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
+  }
+  int token;
+  const RowInfo mine = select_row<HALF>(a, seq, ri, draft, d, sh.row, token);
   static_assert(sizeof(RowInfo) == 32, "four words");
-  if (t < 4) {
+  if (t < 4 && (!VERIFY || token < 0)) {
     uint64_t w[4];
     __builtin_memcpy(w, &mine, 32);
     put_far(info + 4 * row + t, t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3]);
   }
   if constexpr (!VERIFY) return;
-  if (t == 0 && ri < m) in.px[(long)seq * m + ri] = (float)mine.px;
+  if (t == 0) {
+    if (ri < m) in.px[(long)seq * m + ri] = (float)mine.px;
+    put_far(drawn + row, (uint64_t)(ri >= len || !(uq < mine.px)) << 32 | (u32)token);
+  }
   if (!arrives_last(a.arrived + seq, a.per, &sh.row.last)) return;
-  const int len = drafts_of(a, in, seq);
   if (t == 0) sh.draw.first = len;
   __syncthreads();
-  if (t < len) {                        // kMaxDraft < kRowThreads
-    const double px = __builtin_bit_cast(double, get_far(info + 4 * ((long)seq * a.per + t) + 1));
-    if (refused(a, in, seq, t, px)) atomicMin(&sh.draw.first, t);
+  uint64_t res = 0;
+  if (t <= len) {                       // kMaxDraft < kRowThreads
+    res = get_far(drawn + (long)seq * a.per + t);
+    if (res >> 32) atomicMin(&sh.draw.first, t);
   }
   __syncthreads();
   const int n = sh.draw.first;
-  const long at = (long)seq * a.per + n;
-  uint64_t w[4];
+  if (t == n) sh.row.token = (int)(u32)res;
+  __syncthreads();
+  token = sh.row.token;
+  if (token < 0) {
+    uint64_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = get_far(info + 4 * at + i);
-  RowInfo r;
-  __builtin_memcpy(&r, w, 32);
-  const float* q = in.q && n < len ? in.q + seq * in.qb + n * in.qr : nullptr;
-  const int skip = n < len ? in.draft[(long)seq * m + n] : -1;
-  const int token = draw_token<HALF, true>(a, r, seq, n, n == len ? kDrawRow : q ? kDrawRest : kDrawOther, q, skip,
-                                           uniform_at(in, (long)seq * a.per + m), nullptr, list_idx + at * kListed,
-                                           list_w + at * kListed, sh.draw);
+    for (int i = 0; i < 4; ++i) w[i] = get_far(info + 4 * ((long)seq * a.per + n) + i);
+    RowInfo r;
+    __builtin_memcpy(&r, w, 32);
+    token = draw_token<HALF, true>(a, r, seq, n, draw_in(a, in, seq, n, len), nullptr, sh.draw);
+  }
   write_tokens(a, in, seq, n, token);
 }
 
@@ -678,7 +780,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_whole_kernel(const SampleA
   r.m = sh.m[n];
   r.thr = kLowKey<HALF>;
   r.cut = kNoTies;
-  r.listed = -1;
   const bool dense = in.q && n < len;
   const float* q = dense ? in.q + seq * in.qb + n * in.qr : nullptr;
   double* sums = rest + (long)seq * a.nseg;
@@ -699,9 +800,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_whole_kernel(const SampleA
   } else if (blockIdx.x) {
     return;
   }
-  const int skip = n < len ? in.draft[(long)seq * m + n] : -1;
-  const int token = draw_token<HALF, false>(a, r, seq, n, n == len ? kDrawRow : q ? kDrawRest : kDrawOther, q, skip,
-                                            uniform_at(in, (long)seq * a.per + m), sums, nullptr, nullptr, sh.draw);
+  const int token = draw_token<HALF, false>(a, r, seq, n, draw_in(a, in, seq, n, len), sums, sh.draw);
   write_tokens(a, in, seq, n, token);
 }
 
@@ -757,20 +856,19 @@ __global__ __launch_bounds__(kStatThreads) void sample_probs_kernel(const Sample
 // ---------------------------------------------------------------- host
 
 struct Layout {
-  size_t segs, rest, list_w, info, segm, list_idx, arrived, bytes;
+  size_t segs, rest, info, drawn, segm, arrived, bytes;
 };
 
 Layout layout(int64_t rows, int64_t V, int64_t sequences) {
-  const size_t n = (size_t)((V + 7 + kSegVals - 1) / kSegVals), listed = sequences ? (size_t)rows * kListed : 0;
+  const size_t n = (size_t)((V + 7 + kSegVals - 1) / kSegVals);
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   Layout l;
   l.segs = 0;
   l.rest = up(l.segs + (size_t)rows * n * 8);
-  l.list_w = up(l.rest + (size_t)sequences * n * 8);
-  l.info = up(l.list_w + listed * 8);
-  l.segm = up(l.info + (size_t)rows * sizeof(RowInfo));
-  l.list_idx = up(l.segm + (size_t)rows * n * 4);
-  l.arrived = up(l.list_idx + listed * 4);
+  l.info = up(l.rest + (size_t)sequences * n * 8);
+  l.drawn = up(l.info + (size_t)rows * sizeof(RowInfo));
+  l.segm = up(l.drawn + (sequences ? (size_t)rows * 8 : 0));
+  l.arrived = up(l.segm + (size_t)rows * n * 4);
   l.bytes = up(l.arrived + (size_t)sequences * 4);
   return l;
 }
@@ -815,7 +913,7 @@ void probs(const SampleArgs& a, uint64_t* info, float* out, long ldo, hipStream_
   launch_segments<HALF>(a, s);
   if (a.top_k || a.top_p < 1.0) {
     hipLaunchKernelGGL((sample_cut_kernel<HALF, false>), dim3(1, (unsigned)a.rows), dim3(kRowThreads), 0, s, a, VerifyIn{}, info,
-                       nullptr, nullptr);
+                       nullptr);
     hipLaunchKernelGGL((sample_probs_kernel<HALF, true, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
   } else {
     hipLaunchKernelGGL((sample_probs_kernel<HALF, false, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
@@ -828,8 +926,7 @@ void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, h
   launch_segments<HALF>(a, s);
   if (a.top_k || a.top_p < 1.0) {
     hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in,
-                       reinterpret_cast<uint64_t*>(w + l.info), reinterpret_cast<int*>(w + l.list_idx),
-                       reinterpret_cast<double*>(w + l.list_w));
+                       reinterpret_cast<uint64_t*>(w + l.info), reinterpret_cast<uint64_t*>(w + l.drawn));
   } else {
     // where there are draft probabilities, a workgroup a CU over the refused rows, at most one a wave and segment
     const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
