@@ -52,7 +52,7 @@ struct SampleArgs {
   int top_k;                           // 0: none
   float* segm;                         // [rows][nseg] segment maxima
   double* segs;                        // [rows][nseg] segment sums
-  int* arrived;                        // [sequences] workgroups that are done, cleared by the first launch
+  int* arrived;                        // [sequences], [rows]: workgroups that are done, cleared by the first launch
 };
 
 struct RowInfo {                       // what is sampled from of a row
@@ -263,16 +263,29 @@ __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >>
 
 __device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int seq, int i) { return a.x + seq * a.ldb + i * a.ldr; }
 
-// Maximum and normaliser of a row without a cut, the join of its segments, by one wave.
+// Maximum and normaliser of a row without a cut, the join of its segments, by one wave: four values a lane at once.
 __device__ __forceinline__ double join_wave(const float* segm, const double* segs, int nseg, double c, float& m) {
   const int lane = threadIdx.x & 63;
-  float mx = -INFINITY;
-  for (int s = lane; s < nseg; s += 64) mx = fmaxf(mx, segm[s]);
-  mx = wave_max(mx);
+  float mx = -INFINITY;                // of this lane so far; z against it
   double z = 0;
-  for (int s = lane; s < nseg; s += 64) z += segs[s] * weight(segm[s], mx, c);
-  m = mx;
-  return mx > -INFINITY ? wave_total(z) : 0.0;
+  for (int s0 = lane; s0 < nseg; s0 += 256) {
+    float sm[4];
+    double ss[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + 64 * i;
+      sm[i] = s < nseg ? segm[s] : -INFINITY;
+      ss[i] = s < nseg ? segs[s] : 0.0;
+    }
+    const float to = fmaxf(fmaxf(mx, fmaxf(sm[0], sm[1])), fmaxf(sm[2], sm[3]));
+    z *= weight(mx, to, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z += ss[i] * weight(sm[i], to, c);
+    mx = to;
+  }
+  m = wave_max(mx);
+  const double all = wave_total(m > -INFINITY ? z * weight(mx, m, c) : 0.0);
+  return all;
 }
 
 }  // namespace dspark

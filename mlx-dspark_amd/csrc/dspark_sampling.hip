@@ -18,7 +18,10 @@ constexpr int kStatThreads = 256;
 template <bool HALF, int SPW, bool SUM>
 __global__ __launch_bounds__(kStatThreads) void sample_segments_kernel(const SampleArgs a) {
   const int lane = threadIdx.x & 63, seq = blockIdx.z;
-  if (a.arrived && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.arrived[seq] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (blockIdx.y == 0) a.arrived[seq] = 0;
+    a.arrived[gridDim.z + (long)seq * a.per + blockIdx.y] = 0;
+  }
   const int s0 = (blockIdx.x * (kStatThreads / 64) + uniform(threadIdx.x >> 6)) * SPW;
   const u16* x = row_ptr(a, seq, blockIdx.y);
   const int off = row_off(x);
@@ -42,6 +45,99 @@ __global__ __launch_bounds__(kStatThreads) void sample_segments_kernel(const Sam
       if (lane == 0) a.segs[at] = m > -INFINITY ? s : 0.0;
     }
     if (lane == 0) a.segm[at] = m;
+  }
+}
+
+// The same over many segments of bf16 logits, uncut: a value's weight against 0, 2^(c x), from a table in LDS.
+// bf16 has 128 values an octave; 22 octaves, 2^-14 to 2^8, and both signs are 45 KB, formed once by each workgroup
+// (one a CU, its waves then walk through the segments). A look-up and its sum are 6 instructions, one of them fp64;
+// the weight itself is 16, nearly all fp64, and bounds the pass above (76032 segments: 37 us; the table's: TABLE_US).
+// The sums stand against 0, so no maximum is looked for. A value the table does not have turns the sum into NaN, one
+// below -256 counts as none; a segment of either kind, or too light for what was left out, is summed plainly.
+constexpr int kTabLow = (127 - 14) << 7, kTabHalf = 22 << 7;
+constexpr int kTabSlots = kTabHalf + 2;               // of one sign: below, the values, above
+constexpr int kTabThreads = 1024, kTabAhead = 3;
+constexpr double kTabMaxC = 3.5;       // 2^(c 256) stays far below the largest double
+
+typedef u16 u16x2_t __attribute__((ext_vector_type(2)));
+
+__global__ __launch_bounds__(kTabThreads) void sample_table_kernel(const SampleArgs a, const int total, const int steps) {
+  __shared__ double tab[2 * kTabSlots];
+  const int t = threadIdx.x, lane = t & 63;
+  if (blockIdx.x == 0)
+    for (int i = t; i < a.rows / a.per; i += kTabThreads) a.arrived[i] = 0;
+  // a run of segments a wave, one row after another; the first loads before the table
+  const int g0 = (blockIdx.x * (kTabThreads / 64) + uniform(t >> 6)) * steps, g1 = min(g0 + steps, total);
+  int row = g0 / a.nseg, s = g0 - row * a.nseg, ahead = g0;            // of the next load
+  const u16* x = row_ptr(a, row / a.per, row % a.per);
+  const auto load = [&]() {
+    const u32x4_t v = ahead < g1 ? load8<false>(x, s * kSegVals + 8 * lane - row_off(x), a.V) : u32x4_t{};
+    ++ahead;
+    if (++s == a.nseg) {
+      s = 0;
+      ++row;
+      if (ahead < g1) x = row_ptr(a, row / a.per, row % a.per);
+    }
+    return v;
+  };
+  u32x4_t v[kTabAhead];
+#pragma unroll
+  for (int i = 0; i < kTabAhead; ++i) v[i] = load();
+  if (t < 2 * kTabHalf / 8) {           // 8 values a thread, inside an octave: one after another by a ratio
+    const int sign = t >= kTabHalf / 8, i0 = 8 * t - (sign ? kTabHalf : 0);
+    const u32 b = (u32)(kTabLow + i0) | (sign ? 0x8000u : 0u);
+    double w = exp2_neg((double)bf2f(b) * a.c);
+    const double ratio = exp2_neg(((double)bf2f(b + 1) - (double)bf2f(b)) * a.c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      tab[sign * kTabSlots + 1 + i0 + i] = w;
+      w *= ratio;
+    }
+  }
+  if (t < 4) tab[(t >> 1) * kTabSlots + (t & 1) * (kTabHalf + 1)] = t == 3 ? 0.0 : __builtin_nan("");
+  __syncthreads();
+  const double light = __builtin_ldexp(1.0, (int)(80.0 - 256.0 * a.c));      // V values below -256 weigh nothing beside it
+  for (int g = g0; g < g1; g += kTabAhead) {
+#pragma unroll
+    for (int i = 0; i < kTabAhead; ++i) {
+      if (g + i >= g1) break;
+      const u32x4_t now = v[i];
+      double sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32 two = now[j];
+        const u16x2_t b = __builtin_bit_cast(u16x2_t, two);
+        const u16x2_t sign = (b >> (u16)15) * (u16)kTabSlots;
+        const u16x2_t slot = __builtin_elementwise_min(__builtin_elementwise_sub_sat((u16x2_t)(b & (u16)0x7FFF), (u16x2_t)(u16)(kTabLow - 1)),
+                                                       (u16x2_t)(u16)(kTabHalf + 1)) + sign;
+        sum += tab[slot[0]];
+        sum += tab[slot[1]];
+      }
+      v[i] = load();
+      sum = wave_total(sum);
+      float m = 0;
+      if (!(sum >= light)) {            // also NaN
+        m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, val<false>(bits_of(now, j)));
+        m = wave_max(m);
+        sum = 0;
+        if (m > -INFINITY) {
+          const double mc = -(double)m * a.c;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            const u32 two = j == 0 ? now[0] : j == 1 ? now[1] : j == 2 ? now[2] : now[3];
+            sum += weight(bf2f(two & 0xFFFFu), m, a.c, mc);
+            sum += weight(bf2f(two >> 16), m, a.c, mc);
+          }
+          sum = wave_total(sum);
+        }
+      }
+      if (lane == 0) {
+        a.segs[g + i] = sum;            // [rows][nseg], the order of the walk
+        a.segm[g + i] = m;
+      }
+    }
   }
 }
 
@@ -69,28 +165,40 @@ struct RowShared {
   double z;
 };
 
-// The largest key that at least k of the n (<= kMaxSegs) values reach: 4 bits a round, a wave for each of the 16
-// keys a round tries. `counts`: a slot a wave.
-__device__ __forceinline__ int kth_key(const int* v, int n, int k, int* counts) {
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  int key = -(1 << 15);
-  for (int shift = 12; shift >= 0; shift -= 4) {
-    const int tried = key + (wave << shift);
-    int c = 0;
-    for (int i = 0; i < n; i += 64) c += __popcll(__ballot(i + lane < n && v[i + lane] >= tried));
-    if (lane == 0) counts[wave] = c;
+// The largest key that at least k of the threads' keys reach (`in`: a thread that has one; there are at least k):
+// counts of the high bytes in falling order, then of the low bytes of the one the k-th lies in. `hist`: 512 zeros.
+__device__ __forceinline__ int kth_key(bool in, int key, int k, int* hist) {
+  const int lane = threadIdx.x & 63;
+  const u32 u = (u32)(key + (1 << 15));
+  int high = 0;
+  for (int round = 0; round < 2; ++round) {
+    const int bin = 255 - (round ? (int)(u & 255) : (int)(u >> 8));
+    if (in && (!round || (int)(u >> 8) == high)) atomicAdd(&hist[256 * round + bin], 1);
     __syncthreads();
-    const unsigned long long enough = __ballot(lane < kRowWaves && counts[lane & (kRowWaves - 1)] >= k);
-    key += (enough ? 63 - __clzll(enough) : 0) << shift;
-    __syncthreads();
+    int c[4], sum = 0;                   // four bins a lane, every wave for itself
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += c[i] = hist[256 * round + 4 * lane + i];
+    const int upto = wave_scan(sum);
+    int before = upto - sum, at = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (at == i && before + c[i] < k) {
+        before += c[i];
+        at = i + 1;
+      }
+    const int owner = __ffsll(__ballot(upto >= k)) - 1;
+    const int got = 255 - (4 * owner + __builtin_amdgcn_readlane(at, owner));
+    k -= __builtin_amdgcn_readlane(before, owner);
+    if (round == 0) high = got;
+    else return (high << 8 | got) - (1 << 15);
   }
-  return key;
+  return 0;
 }
 
-// The segments whose maximum reaches `lo`, into sh.list; their number in sh.nlist (0 on entry).
-__device__ __forceinline__ int list_segments(RowShared& sh, int nseg, int lo) {
+// The segments of s0 .. s1 whose maximum reaches `lo`, into sh.list; their number in sh.nlist (0 on entry).
+__device__ __forceinline__ int list_segments(RowShared& sh, int s0, int s1, int lo) {
   const int t = threadIdx.x, lane = t & 63;
-  const bool f = t < nseg && sh.skey[t] >= lo;                 // kMaxSegs <= kRowThreads
+  const bool f = t >= s0 && t < s1 && sh.skey[t] >= lo;        // kMaxSegs <= kRowThreads
   const unsigned long long on = __ballot(f);
   int base = 0;
   if (on) {
@@ -187,11 +295,19 @@ struct DrawIn {                        // what a row's own draw goes by
   double u;
 };
 
+constexpr int kGroup = 16;             // most workgroups that count a row together
+struct Group {                         // a row counted by several workgroups, each over its own run of segments
+  uint64_t* counts;                    // of each workgroup, 4 bins of 16 bits a word; null: one workgroup a row
+  int* arrived;                        // workgroups of this row that are done
+  int g, n;
+};
+
 // The part of one row that is sampled from: its threshold and normaliser (RowInfo), and px of token `draft`. Where
-// the candidates are few, the token drawn from the row too (d.mode >= 0; -1 where it was not).
+// the candidates are few, the token drawn from the row too (d.mode >= 0; -1 where it was not). False in the
+// workgroups of a group that leave the row to another.
 template <bool HALF>
-__device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, RowShared& sh,
-                                              int& token) {
+__device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, const Group& gr,
+                                           RowShared& sh, RowInfo& out, int& token) {
   const int t = threadIdx.x, lane = t & 63;
   const u16* x = row_ptr(a, seq, ri);
   const int off = row_off(x);
@@ -199,12 +315,12 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
   const float sm = t < a.nseg ? a.segm[row * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
   const double ss = !a.top_k && t < a.nseg ? a.segs[row * a.nseg + t] : 0;
   const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
-  RowInfo out;
   token = -1;
   float mx = wave_max(sm);
   if (lane == 0) sh.red_f[t >> 6] = mx;
   if (t < a.nseg) sh.skey[t] = key_of_float<HALF>(sm);
   if (t == 0) sh.ncand = sh.nlist = 0;
+  if (t < 512) sh.cnt[t] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) mx = fmaxf(mx, sh.red_f[i]);
@@ -216,7 +332,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
     out.thr = 1 << 16;
     out.cut = kNoTies;
     token = 0;
-    return out;
+    return gr.g == 0;
   }
   const double mc = -(double)mx * a.c;
   double total = 0;                     // of the whole row; needed where the mass itself is cut
@@ -237,7 +353,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
     const double w = (1.0 - a.top_p) * total / (double)a.V;
     kb = key_of_float<HALF>((float)((double)mx + log2(w) / a.c)) - 1;
   } else if (a.nseg >= a.top_k) {
-    kb = kth_key(sh.skey, a.nseg, a.top_k, sh.red_i);
+    kb = kth_key(t < a.nseg, key_of_float<HALF>(sm), a.top_k, sh.cnt);
   } else if (8 * a.nseg >= a.top_k && a.nseg <= kMaxSegs / 8) {
     // few segments: the maxima of groups of 8 lanes instead
     for (int s = uniform(t >> 6); s < a.nseg; s += kRowWaves) {
@@ -249,17 +365,20 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
       k = max(k, dpp_i<0xB1, 0xF>(k));   // the exchanges of sum8_lanes
       k = max(k, dpp_i<0x4E, 0xF>(k));
       k = max(k, dpp_i<0x141, 0xF>(k));
-      if ((lane & 7) == 0) sh.cnt[8 * s + (lane >> 3)] = k;
+      if ((lane & 7) == 0) sh.list[8 * s + (lane >> 3)] = k;
     }
     __syncthreads();
-    kb = kth_key(sh.cnt, 8 * a.nseg, a.top_k, sh.red_i);
+    kb = kth_key(t < 8 * a.nseg, sh.list[t], a.top_k, sh.cnt);
+    __syncthreads();
   }
   kb = min(max(kb, kLowKey<HALF> + 1), top);
-  int nlist = list_segments(sh, a.nseg, kb);
+  int nlist = list_segments(sh, 0, a.nseg, kb);
 
   // Few candidates are sorted. A top_k leaves little more than that many; a mass alone may leave most of a segment,
   // so that only rows where few segments reach are tried.
-  if (nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves)) {
+  const bool few = nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves);
+  if (few && gr.g) return false;        // the first workgroup's alone
+  if (few) {
     each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
       const int v0 = s * kSegVals + 8 * lane - off;
       int n = 0, ks[8];
@@ -332,7 +451,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
       out.thr = sh.key;
       out.cut = sh.cut;
       out.px = px_of<HALF>(a, out, draft, xd);
-      if (d.mode < 0) return out;
+      if (d.mode < 0) return true;
       // the draw: r by index, then the first wave, four a lane
       if (t < kept) {
         int at = 0;
@@ -373,13 +492,47 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
       }
       __syncthreads();
       token = sh.token;
-      return out;
+      return true;
     }
     __syncthreads();
   }
 
   int thr = kb - 1, keep = 0, ties = 0;  // thr = kb - 1: every listed token
   int loaded = 1 << 17;                  // the range of keys now in the bins starts here
+  const int spg = (a.nseg + gr.n - 1) / gr.n;         // segments of a workgroup of the group
+  const int words = (top - kb + 4) >> 2;
+  const bool grouped = gr.counts && !few && top - kb < kBins;
+  if (gr.counts && !few && !grouped && gr.g) return false;       // too many values for one pass: the first's alone
+  if (grouped) {
+    __syncthreads();
+    if (t == 0) sh.nlist = 0;
+    __syncthreads();
+    const int mine = list_segments(sh, gr.g * spg, min((gr.g + 1) * spg, a.nseg), kb);
+    count_keys<HALF>(a, x, off, sh, mine, top, kb);
+    uint64_t* out_c = gr.counts + (long)gr.g * (kBins / 4);
+    for (int i = t; i < words; i += kRowThreads) {    // a value at most as often as spg segments have logits: below 2^16
+      uint64_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w |= (uint64_t)(4 * i + j <= top - kb ? sh.bins[4 * i + j] : 0) << (16 * j);
+      put_far(out_c + i, w);
+    }
+    if (!arrives_last(gr.arrived, gr.n, &sh.last)) return false;
+    for (int i = t; i < words; i += kRowThreads) {
+      int c[4] = {};
+      uint64_t w[kGroup];                // every workgroup's word at once
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) w[g] = g < gr.n ? get_far(gr.counts + (long)g * (kBins / 4) + i) : 0;
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] += (int)(w[g] >> (16 * j) & 0xFFFF);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * i + j < kBins) sh.bins[4 * i + j] = c[j];
+    }
+    __syncthreads();
+    loaded = kb;
+  }
   double z = 0;
   bool found = false;
   // two passes over the values in falling order: the top_k-th token, then the mass top_p
@@ -425,7 +578,8 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
       const double mass_before = block_scan(cm, sh.red_d, mass_end, mass_all);
       // the thread whose bins the goal falls into (the first: running sums may step back by a rounding)
       const bool mine = pass == 0 ? seen + cnt_end >= a.top_k && cn : mass + mass_end >= goal && cn;
-      if (mine) atomicMin(&sh.owner, t);
+      const unsigned long long reached = __ballot(mine);
+      if (lane == 0 && reached) atomicMin(&sh.owner, t + __ffsll(reached) - 1);
       __syncthreads();
       const int owner = sh.owner;
       if (owner < kRowThreads && (t >> 6) == (owner >> 6)) {     // its wave, a bin a lane
@@ -480,8 +634,18 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
   if (keep < ties) {                    // the index of the last kept token of the threshold's value
     if (t == 0) sh.nlist = 0;
     if (t < a.nseg) sh.cnt[t] = 0;
+    int s0 = 0, s1 = a.nseg;
+    if (grouped) {                      // the run of segments it lies in, by the groups' own counts
+      const int b = top - thr;
+      const int c = lane < gr.n ? (int)(get_far(gr.counts + (long)lane * (kBins / 4) + (b >> 2)) >> (16 * (b & 3)) & 0xFFFF) : 0;
+      const int upto = wave_scan(c);
+      const int at = __ffsll(__ballot(upto >= keep)) - 1;
+      keep -= __builtin_amdgcn_readlane(upto - c, at);
+      s0 = at * spg;
+      s1 = min(s0 + spg, a.nseg);
+    }
     __syncthreads();
-    nlist = list_segments(sh, a.nseg, thr);
+    nlist = list_segments(sh, s0, s1, thr);
     each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
       int n = 0, ks[8];
       keys8(v, ks);
@@ -514,7 +678,7 @@ __device__ __forceinline__ RowInfo select_row(const SampleArgs& a, int seq, int 
     out.cut = sh.cut;
   }
   out.px = px_of<HALF>(a, out, draft, xd);
-  return out;
+  return true;
 }
 
 // ---------------------------------------------------------------- the accept rule
@@ -544,11 +708,26 @@ __device__ __forceinline__ DrawIn draw_in(const SampleArgs& a, const VerifyIn& i
   return d;
 }
 
-// r of 8 logits from index v0 (logits outside the row are -inf: no weight, q not read). Without a cut every
+// q of a lane's 8 tokens from index v0, 0 outside the row.
+__device__ __forceinline__ void load_q8(const float* q, int v0, int V, float (&out)[8]) {
+  if (v0 >= 0 && v0 + 8 <= V && (reinterpret_cast<uintptr_t>(q + v0) & 15) == 0) {
+    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(q + v0), b = *reinterpret_cast<const f32x4_t*>(q + v0 + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      out[j] = a[j];
+      out[4 + j] = b[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = v0 + j >= 0 && v0 + j < V ? q[v0 + j] : 0.f;
+  }
+}
+
+// r of 8 logits from index v0 (q: of the same tokens, where the mode asks for it). Without a cut every
 // logit's weight is formed; with one, those of which some lane keeps its own.
 template <bool HALF, bool CUT>
 __device__ __forceinline__ void rest8(const SampleArgs& a, const RowInfo& r, double inv, const u32x4_t& x, int v0, int mode,
-                                      const float* q, int skip, double (&out)[8]) {
+                                      const float (&q)[8], int skip, double (&out)[8]) {
   const double mc = -(double)r.m * a.c;
   int ks[8];
   keys8(x, ks);
@@ -559,7 +738,7 @@ __device__ __forceinline__ void rest8(const SampleArgs& a, const RowInfo& r, dou
     double w = 0;
     if (!CUT || __any(kept)) {
       w = weight(val<HALF>(bits_of(x, j)), r.m, a.c, mc);
-      if (mode == kDrawRest) w = __builtin_fmax(w * inv - (kept && v >= 0 && v < a.V ? (double)q[v] : 0.0), 0.0);
+      if (mode == kDrawRest) w = __builtin_fmax(w * inv - (double)q[j], 0.0);
       else if (mode == kDrawOther && v == skip) w = 0;
       w = kept ? w : 0.0;
     }
@@ -576,7 +755,7 @@ struct DrawShared {
 };
 
 // The token drawn from row ri of a sequence: the first whose running sum of r passes u times the whole.
-// `rest`: segment sums of max(p - q, 0) (no cut).
+// `rest`: segment sums of r (null: formed here; without a cut, only where r is max(p - q, 0)).
 template <bool HALF, bool CUT>
 __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r, int seq, int ri, const DrawIn& d,
                                           const double* rest, DrawShared& sh) {
@@ -599,14 +778,17 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
     __syncthreads();
     const bool f = r.z > 0 && t < a.nseg && key_of_float<HALF>(sm) >= r.thr;
     if (f) sh.list[atomicAdd(&sh.nlist, 1)] = t;
-    sh.sums[t] = 0;                     // kMaxSegs == kRowThreads
+    sh.sums[t] = rest && t < a.nseg ? __builtin_bit_cast(double, get_far(reinterpret_cast<const uint64_t*>(rest) + t)) : 0;
+    static_assert(kMaxSegs == kRowThreads, "a slot a thread");
     __syncthreads();
   }
   for (int tries = 0; tries < 2; ++tries) {
     if constexpr (CUT) {
-      each_listed<HALF>(a, x, off, sh.list, sh.nlist, [&](int s, const u32x4_t& v) {
+      if (!rest || tries) each_listed<HALF>(a, x, off, sh.list, sh.nlist, [&](int s, const u32x4_t& v) {
         double w[8], sum = 0;
-        rest8<HALF, true>(a, r, inv, v, s * kSegVals + 8 * lane - off, mode, d.q, d.skip, w);
+        float q[8] = {};
+        if (mode == kDrawRest) load_q8(d.q, s * kSegVals + 8 * lane - off, a.V, q);
+        rest8<HALF, true>(a, r, inv, v, s * kSegVals + 8 * lane - off, mode, q, d.skip, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += w[j];
         sum = wave_total(sum);
@@ -621,7 +803,8 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
       if (mode == kDrawOther && d.skip >= 0 && d.skip < a.V && t < 64) {   // the token's own segment again, without it
         const int s = (d.skip + off) / kSegVals, v0 = s * kSegVals + 8 * lane - off;
         double w[8], sum = 0;
-        rest8<HALF, false>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, nullptr, d.skip, w);
+        const float q[8] = {};
+        rest8<HALF, false>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, q, d.skip, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += w[j];
         sum = wave_total(sum);
@@ -636,9 +819,10 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
   }
   // the first segment whose running sum passes the goal (the last one with any mass if none does by a rounding)
   const double goal = d.u * all;
-  if (mine > 0) {
-    atomicMax(&sh.last, t);
-    if (upto > goal) atomicMin(&sh.seg, t);
+  const unsigned long long any_mass = __ballot(mine > 0), passes = __ballot(mine > 0 && upto > goal);
+  if (lane == 0 && any_mass) {          // t: the wave's first thread
+    atomicMax(&sh.last, t + 63 - __clzll(any_mass));
+    if (passes) atomicMin(&sh.seg, t + __ffsll(passes) - 1);
   }
   __syncthreads();
   const int s = sh.seg < kMaxSegs ? sh.seg : sh.last;
@@ -648,7 +832,9 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
     if (t < 64) {
       const int v0 = s * kSegVals + 8 * lane - off;
       double w[8], sum = 0;
-      rest8<HALF, CUT>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, d.q, d.skip, w);
+      float q[8] = {};
+      if (mode == kDrawRest) load_q8(d.q, v0, a.V, q);
+      rest8<HALF, CUT>(a, r, inv, load8<HALF>(x, v0, a.V), v0, mode, q, d.skip, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += w[j];
       const double to = sh.before + wave_scan(sum);
@@ -706,7 +892,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
     if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
   }
   int token;
-  const RowInfo mine = select_row<HALF>(a, seq, ri, draft, d, sh.row, token);
+  RowInfo mine;
+  select_row<HALF>(a, seq, ri, draft, d, Group{nullptr, nullptr, 0, 1}, sh.row, mine, token);
   static_assert(sizeof(RowInfo) == 32, "four words");
   if (t < 4 && (!VERIFY || token < 0)) {
     uint64_t w[4];
@@ -742,65 +929,118 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
   write_tokens(a, in, seq, n, token);
 }
 
-struct WholeShared {
+// The same in two launches where a row's candidates may be many and the rows are few: a group of workgroups a row
+// counts and selects, workgroups over the refused row's segments draw (sample_spread_kernel).
+template <bool HALF>
+__global__ __launch_bounds__(kRowThreads) void sample_group_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
+                                                                   uint64_t* counts, int* arrived) {
+  __shared__ RowShared sh;
+  const int ri = blockIdx.y, seq = blockIdx.z, m = a.per - 1;
+  const long row = (long)seq * a.per + ri;
+  const int draft = in.draft && ri < m ? in.draft[(long)seq * m + ri] : -1;
+  const Group gr = {counts + row * gridDim.x * (kBins / 4), arrived + row, (int)blockIdx.x, (int)gridDim.x};
+  int token;
+  RowInfo mine;
+  if (!select_row<HALF>(a, seq, ri, draft, DrawIn{-1, -1, nullptr, 0.0}, gr, sh, mine, token)) return;
+  if (threadIdx.x < 4) {
+    uint64_t w[4];
+    __builtin_memcpy(w, &mine, 32);
+    const int t = threadIdx.x;
+    info[4 * row + t] = t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3];
+  }
+  if (threadIdx.x == 0 && draft != -1) in.px[(long)seq * m + ri] = (float)mine.px;
+  else if (threadIdx.x == 0 && in.draft && ri < m) in.px[(long)seq * m + ri] = 0.f;
+}
+
+struct SpreadShared {
   double z[kMaxDraft + 1], px[kMaxDraft + 1];
   float m[kMaxDraft + 1];
   DrawShared draw;
   int last;
 };
 
-// Without a cut: workgroups over the segments of a sequence. Each joins its rows and accepts; where draft
-// probabilities are given, each sums max(p - q, 0) over its segments of the refused row and the last draws.
-template <bool HALF>
-__global__ __launch_bounds__(kRowThreads) void sample_whole_kernel(const SampleArgs a, const VerifyIn in, double* rest) {
-  __shared__ WholeShared sh;
+// Workgroups over the segments of a sequence. Each accepts (without a cut it joins the rows first); where r is not
+// known from the segment sums (a cut, or draft probabilities and a refused draft), each sums r over its segments of
+// the row to draw from, and the last draws.
+template <bool HALF, bool CUT>
+__global__ __launch_bounds__(kRowThreads) void sample_spread_kernel(const SampleArgs a, const VerifyIn in,
+                                                                    const uint64_t* __restrict__ info, double* rest) {
+  __shared__ SpreadShared sh;
   const int seq = blockIdx.y, m = a.per - 1, t = threadIdx.x, lane = t & 63;
   const int len = drafts_of(a, in, seq);
-  for (int i = uniform(t >> 6); i < a.per; i += kRowWaves) {
-    const long row = (long)seq * a.per + i;
-    const int draft = i < m ? in.draft[(long)seq * m + i] : -1;
-    const bool inside = draft >= 0 && draft < a.V;
-    const float xd = inside ? val<HALF>(row_ptr(a, seq, i)[draft]) : -INFINITY;
-    float mx;
-    const double z = join_wave(a.segm + row * a.nseg, a.segs + row * a.nseg, a.nseg, a.c, mx);
-    if (lane == 0) {
-      sh.z[i] = z;
-      sh.m[i] = mx;
-      sh.px[i] = z > 0 && xd > -INFINITY ? weight(xd, mx, a.c) / z : 0.0;
+  if constexpr (CUT) {
+    if (t < m) sh.px[t] = __builtin_bit_cast(double, info[4 * ((long)seq * a.per + t) + 1]);
+  } else {
+    for (int i = uniform(t >> 6); i < a.per; i += kRowWaves) {
+      const long row = (long)seq * a.per + i;
+      const int draft = i < m ? in.draft[(long)seq * m + i] : -1;
+      const bool inside = draft >= 0 && draft < a.V;
+      const float xd = inside ? val<HALF>(row_ptr(a, seq, i)[draft]) : -INFINITY;
+      float mx;
+      const double z = join_wave(a.segm + row * a.nseg, a.segs + row * a.nseg, a.nseg, a.c, mx);
+      if (lane == 0) {
+        sh.z[i] = z;
+        sh.m[i] = mx;
+        sh.px[i] = z > 0 && xd > -INFINITY ? weight(xd, mx, a.c) / z : 0.0;
+      }
     }
   }
   if (t == 0) sh.draw.first = len;
   __syncthreads();
-  if (blockIdx.x == 0 && t < m) in.px[(long)seq * m + t] = (float)sh.px[t];
+  if (!CUT && blockIdx.x == 0 && t < m) in.px[(long)seq * m + t] = (float)sh.px[t];
   if (t < len && refused(a, in, seq, t, sh.px[t])) atomicMin(&sh.draw.first, t);
   __syncthreads();
   const int n = sh.draw.first;
+  const DrawIn d = draw_in(a, in, seq, n, len);
   RowInfo r;
-  r.z = sh.z[n];
-  r.m = sh.m[n];
-  r.thr = kLowKey<HALF>;
-  r.cut = kNoTies;
-  const bool dense = in.q && n < len;
-  const float* q = dense ? in.q + seq * in.qb + n * in.qr : nullptr;
+  if constexpr (CUT) {
+    __builtin_memcpy(&r, info + 4 * ((long)seq * a.per + n), 32);
+  } else {
+    r.z = sh.z[n];
+    r.m = sh.m[n];
+    r.thr = kLowKey<HALF>;
+    r.cut = kNoTies;
+  }
   double* sums = rest + (long)seq * a.nseg;
-  if (dense) {
+  if (CUT || d.mode == kDrawRest) {
     const u16* x = row_ptr(a, seq, n);
     const int off = row_off(x);
     const double inv = r.z > 0 ? 1.0 / r.z : 0.0;
-    for (int s = blockIdx.x * kRowWaves + uniform(t >> 6); s < a.nseg; s += gridDim.x * kRowWaves) {
-      const int v0 = s * kSegVals + 8 * lane - off;
-      double w[8], sum = 0;
-      rest8<HALF, false>(a, r, inv, load8<HALF>(x, v0, a.V), v0, kDrawRest, q, -1, w);
+    const int stride = gridDim.x * kRowWaves, s0 = blockIdx.x * kRowWaves + uniform(t >> 6);
+    constexpr int kOut = 2;             // segments of a wave whose loads are out together
+    for (int s1 = s0; s1 < a.nseg; s1 += kOut * stride) {
+      u32x4_t v[kOut];
+      float q[kOut][8] = {};
+      bool on[kOut];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += w[j];
-      sum = wave_total(sum);
-      if (lane == 0) put_far(reinterpret_cast<uint64_t*>(sums) + s, __builtin_bit_cast(uint64_t, r.z > 0 ? sum : 0.0));
+      for (int i = 0; i < kOut; ++i) {
+        const int s = s1 + i * stride, v0 = s * kSegVals + 8 * lane - off;
+        on[i] = s < a.nseg && r.z > 0;
+        if (CUT && on[i]) on[i] = key_of_float<HALF>(a.segm[((long)seq * a.per + n) * a.nseg + s]) >= r.thr;
+        if (!on[i]) continue;
+        v[i] = load8<HALF>(x, v0, a.V);
+        if (d.mode == kDrawRest) load_q8(d.q, v0, a.V, q[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kOut; ++i) {
+        const int s = s1 + i * stride;
+        if (s >= a.nseg) break;
+        double sum = 0;
+        if (on[i]) {
+          double w[8];
+          rest8<HALF, CUT>(a, r, inv, v[i], s * kSegVals + 8 * lane - off, d.mode, q[i], d.skip, w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum += w[j];
+          sum = wave_total(sum);
+        }
+        if (lane == 0) put_far(reinterpret_cast<uint64_t*>(sums) + s, __builtin_bit_cast(uint64_t, sum));
+      }
     }
     if (!arrives_last(a.arrived + seq, gridDim.x, &sh.last)) return;
   } else if (blockIdx.x) {
     return;
   }
-  const int token = draw_token<HALF, false>(a, r, seq, n, draw_in(a, in, seq, n, len), sums, sh.draw);
+  const int token = draw_token<HALF, CUT>(a, r, seq, n, d, sums, sh.draw);
   write_tokens(a, in, seq, n, token);
 }
 
@@ -838,7 +1078,8 @@ __global__ __launch_bounds__(kStatThreads) void sample_probs_kernel(const Sample
     float p[8] = {};
     if (!CUT || key_of_float<HALF>(sm[i]) >= r.thr) {
       double w[8];
-      rest8<HALF, CUT>(a, r, inv, v[i], v0, kDrawRow, nullptr, -1, w);
+      const float q[8] = {};
+      rest8<HALF, CUT>(a, r, inv, v[i], v0, kDrawRow, q, -1, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j] = (float)(w[j] * inv);
     }
@@ -855,8 +1096,17 @@ __global__ __launch_bounds__(kStatThreads) void sample_probs_kernel(const Sample
 
 // ---------------------------------------------------------------- host
 
+// Workgroups that count a row together: a CU each, at least a segment a wave, at most kGroup; 0 for one a row.
+constexpr int kGroupSegs = 65535 / kSegVals;          // counts of 16 bits
+int group_size(int64_t rows, int nseg) {
+  const int64_t g = rows < 256 ? 256 / rows : 1, most = (nseg + kRowWaves - 1) / kRowWaves;
+  const int64_t n = g < most ? g : most;
+  const int size = (int)(n < kGroup ? n : kGroup);
+  return size < 2 || (nseg + size - 1) / size > kGroupSegs ? 0 : size;
+}
+
 struct Layout {
-  size_t segs, rest, info, drawn, segm, arrived, bytes;
+  size_t segs, rest, info, drawn, segm, arrived, counts, bytes;
 };
 
 Layout layout(int64_t rows, int64_t V, int64_t sequences) {
@@ -867,9 +1117,10 @@ Layout layout(int64_t rows, int64_t V, int64_t sequences) {
   l.rest = up(l.segs + (size_t)rows * n * 8);
   l.info = up(l.rest + (size_t)sequences * n * 8);
   l.drawn = up(l.info + (size_t)rows * sizeof(RowInfo));
-  l.segm = up(l.drawn + (sequences ? (size_t)rows * 8 : 0));
+  l.segm = up(l.drawn + (size_t)rows * 8);
   l.arrived = up(l.segm + (size_t)rows * n * 4);
-  l.bytes = up(l.arrived + (size_t)sequences * 4);
+  l.counts = up(l.arrived + (size_t)(sequences + rows) * 4);
+  l.bytes = l.counts + (size_t)rows * group_size(rows, (int)n) * kBins * 2;
   return l;
 }
 
@@ -898,22 +1149,44 @@ int sample_args(const char* what, int64_t dtype, const void* logits, int64_t row
   return DSPARK_OK;
 }
 
+constexpr long kTabSegs = 16384;       // segments from which the table pays
+
 unsigned groups(int nseg, int spw) { return (unsigned)((nseg + spw * (kStatThreads / 64) - 1) / (spw * (kStatThreads / 64))); }
 
 template <bool HALF>
 void launch_segments(const SampleArgs& a, hipStream_t s) {
+  const long total = (long)a.rows * a.nseg;
+  if (!HALF && !a.top_k && !(a.top_p < 1.0) && a.c <= kTabMaxC && total >= kTabSegs && total < (1l << 30)) {
+    const int waves = 256 * (kTabThreads / 64), steps = (int)((total + waves - 1) / waves);
+    const unsigned blocks = (unsigned)((total + (long)steps * (kTabThreads / 64) - 1) / ((long)steps * (kTabThreads / 64)));
+    hipLaunchKernelGGL(sample_table_kernel, dim3(blocks), dim3(kTabThreads), 0, s, a, (int)total, steps);
+    return;
+  }
   const dim3 grid(groups(a.nseg, 4), (unsigned)a.per, (unsigned)(a.rows / a.per)), block(kStatThreads);
   if (a.top_k) hipLaunchKernelGGL((sample_segments_kernel<HALF, 4, false>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((sample_segments_kernel<HALF, 4, true>), grid, block, 0, s, a);
 }
 
+// Whether a row may well have more candidates than are sorted: what the mass alone cuts, a large top_k.
+bool many(const SampleArgs& a) { return !a.top_k || a.top_k > 128; }
+
 template <bool HALF>
-void probs(const SampleArgs& a, uint64_t* info, float* out, long ldo, hipStream_t s) {
+void launch_groups(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, int group, hipStream_t s) {
+  hipLaunchKernelGGL((sample_group_kernel<HALF>), dim3((unsigned)group, (unsigned)a.per, (unsigned)(a.rows / a.per)),
+                     dim3(kRowThreads), 0, s, a, in, reinterpret_cast<uint64_t*>(w + l.info),
+                     reinterpret_cast<uint64_t*>(w + l.counts), a.arrived + a.rows / a.per);
+}
+
+template <bool HALF>
+void probs(const SampleArgs& a, char* w, const Layout& l, float* out, long ldo, hipStream_t s) {
   const dim3 grid(groups(a.nseg, 4), (unsigned)a.rows);
+  uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
+  const int group = many(a) ? group_size(a.rows, a.nseg) : 0;
   launch_segments<HALF>(a, s);
   if (a.top_k || a.top_p < 1.0) {
-    hipLaunchKernelGGL((sample_cut_kernel<HALF, false>), dim3(1, (unsigned)a.rows), dim3(kRowThreads), 0, s, a, VerifyIn{}, info,
-                       nullptr);
+    if (group) launch_groups<HALF>(a, VerifyIn{}, w, l, group, s);
+    else hipLaunchKernelGGL((sample_cut_kernel<HALF, false>), dim3(1, (unsigned)a.rows), dim3(kRowThreads), 0, s, a, VerifyIn{},
+                            info, nullptr);
     hipLaunchKernelGGL((sample_probs_kernel<HALF, true, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
   } else {
     hipLaunchKernelGGL((sample_probs_kernel<HALF, false, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
@@ -923,16 +1196,23 @@ void probs(const SampleArgs& a, uint64_t* info, float* out, long ldo, hipStream_
 template <bool HALF>
 void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, hipStream_t s) {
   const unsigned B = (unsigned)(a.rows / a.per);
+  uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
+  double* rest = reinterpret_cast<double*>(w + l.rest);
+  const bool cut = a.top_k || a.top_p < 1.0;
+  const int group = cut && many(a) ? group_size(a.rows, a.nseg) : 0;
+  // over the rows that are drawn from, a workgroup a CU, at most one a wave and segment
+  const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
+  const unsigned spread = most < fill ? most : fill;
   launch_segments<HALF>(a, s);
-  if (a.top_k || a.top_p < 1.0) {
-    hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in,
-                       reinterpret_cast<uint64_t*>(w + l.info), reinterpret_cast<uint64_t*>(w + l.drawn));
+  if (group) {
+    launch_groups<HALF>(a, in, w, l, group, s);
+    hipLaunchKernelGGL((sample_spread_kernel<HALF, true>), dim3(spread, B), dim3(kRowThreads), 0, s, a, in, info, rest);
+  } else if (cut) {
+    hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in, info,
+                       reinterpret_cast<uint64_t*>(w + l.drawn));
   } else {
-    // where there are draft probabilities, a workgroup a CU over the refused rows, at most one a wave and segment
-    const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
-    const unsigned g = in.q ? (most < fill ? most : fill) : 1;
-    hipLaunchKernelGGL((sample_whole_kernel<HALF>), dim3(g, B), dim3(kRowThreads), 0, s, a, in,
-                       reinterpret_cast<double*>(w + l.rest));
+    hipLaunchKernelGGL((sample_spread_kernel<HALF, false>), dim3(in.q ? spread : 1, B), dim3(kRowThreads), 0, s, a, in, info,
+                       rest);
   }
 }
 
@@ -943,7 +1223,7 @@ using namespace dspark;
 
 extern "C" size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences) {
   if (!shape_ok(rows, V) || sequences < 0 || sequences > rows) return 0;
-  return layout(rows, V, sequences).bytes;
+  return layout(rows, V, sequences ? sequences : rows).bytes;
 }
 
 extern "C" int dspark_sampling_probs(const dspark_sampling_probs_args* p, dspark_stream stream) {
@@ -952,7 +1232,7 @@ extern "C" int dspark_sampling_probs(const dspark_sampling_probs_args* p, dspark
   if (!shape_ok(p->rows, p->V) || (p->rows > 1 && (p->ld < p->V || p->ldo < p->V)))
     return fail(DSPARK_ERR_SHAPE, "%s: rows=%lld V=%lld ld=%lld", what, (long long)p->rows, (long long)p->V, (long long)p->ld);
   if (!aligned(p->out, 4)) return fail(DSPARK_ERR_ALIGN, "%s: out needs 4-byte alignment", what);
-  const Layout l = layout(p->rows, p->V, 0);
+  const Layout l = layout(p->rows, p->V, p->rows);
   SampleArgs a;
   const int st = sample_args(what, p->dtype, p->logits, p->rows, p->V, p->temperature, p->top_k, p->top_p, p->workspace,
                              p->workspace_bytes, l, a);
@@ -960,11 +1240,11 @@ extern "C" int dspark_sampling_probs(const dspark_sampling_probs_args* p, dspark
   a.ldb = p->ld;
   a.ldr = 0;
   a.per = 1;
-  a.arrived = nullptr;
-  uint64_t* info = reinterpret_cast<uint64_t*>(static_cast<char*>(p->workspace) + l.info);
+  char* w = static_cast<char*>(p->workspace);
+  a.arrived = reinterpret_cast<int*>(w + l.arrived);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p->dtype == DSPARK_DTYPE_F16) probs<true>(a, info, p->out, p->ldo, s);
-  else probs<false>(a, info, p->out, p->ldo, s);
+  if (p->dtype == DSPARK_DTYPE_F16) probs<true>(a, w, l, p->out, p->ldo, s);
+  else probs<false>(a, w, l, p->out, p->ldo, s);
   return check_launch(what);
 }
 

@@ -234,3 +234,59 @@ def test_streams_and_graphs(dev, cut):
     sets[0][2].copy_(torch.rand(2, 4, generator=g))         # new random numbers in place, as a serving loop draws them
     graphs[0][0].replay()
     assert all(torch.equal(a, b) for a, b in zip(call(sets[0]), graphs[0][1]))
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.5, 3.0])
+def test_many_rows_uncut(dev, temperature):
+    """A batch large enough for its weights to come from a table of the values: plain rows, values near 0, beyond
+    256 and below -256 (all of a row, and beside others), infinities, NaN, rows that leave nothing."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(6)
+    n, V = 60, 151931
+    x = 3.0 * torch.randn(n, V, generator=g)
+    x[1] = x[1] * torch.exp2(torch.randint(-140, 2, (V,), generator=g).float())
+    x[2] = x[2] * 200
+    x[3] = x[3] - 300
+    x[4] -= 200
+    x[5, ::2] = torch.finfo(torch.bfloat16).min
+    x[6] = float("-inf")
+    x[7] = float("nan")
+    x[8, ::3], x[8, 1::3] = float("nan"), float("-inf")
+    x[9, 77] = x[9, 100000] = float("inf")
+    x[10] = 0.0
+    x[11, ::2], x[11, 1::2] = -0.0, -256.0
+    x[12] = 255.0 + x[12]
+    x[13] = -1e-30
+    x = x.to(torch.bfloat16)
+    want = [ref.probs(r, temperature=temperature) for r in _np(x)]
+    got = ops.sampling_probs(x.to(dev), temperature=temperature)
+    close(got, np.stack(want))
+    d, q = _drafts(g, x.view(15, 4, V), "plain", 3)
+    u = torch.rand(15, 4, generator=g)
+    got = ops.speculative_verify(x.view(15, 4, V).to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev), temperature=temperature)
+    ns, tokens, px = ref.verify(_np(x).reshape(15, 4, V), d.numpy(), u.numpy(), q.numpy(), temperature=temperature)
+    assert np.array_equal(got[0].cpu().numpy(), ns) and np.array_equal(got[1].cpu().numpy(), tokens)
+    close(got[2], px)
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.5, temperature=2.0), dict(top_k=400), dict(top_k=500, top_p=0.7)])
+@pytest.mark.parametrize("n,V,dtype", [(100, 20000, "bf16"), (30, 60000, "f16"), (200, 3000, "f16"), (3, 400001, "bf16")])
+def test_many_candidates(dev, n, V, dtype, kw):
+    """Rows counted by several workgroups each, and more rows than that: wide and tied values, a row of one value,
+    one with too many distinct values for one pass."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(n)
+    x = torch.cat([rows(g, n - 3, V, DT[dtype]), rows(g, 1, V, DT[dtype], "same"), rows(g, 1, V, DT[dtype], "far"),
+                   rows(g, 1, V, DT[dtype], "ties")]) if n > 3 else rows(g, n, V, DT[dtype], "ties")
+    close(ops.sampling_probs(x.to(dev), **kw), np.stack([ref.probs(r, **kw) for r in _np(x)]))
+    m = 2 if n % 3 == 0 else 1
+    x = x[:n // (m + 1) * (m + 1)].view(-1, m + 1, V)
+    d, q = _drafts(g, x, "plain", m)
+    u = torch.rand(x.shape[0], m + 1, generator=g)
+    for dense in (False, True):
+        got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev) if dense else None, **kw)
+        ns, tokens, px = ref.verify(_np(x), d.numpy(), u.numpy(), q.numpy() if dense else None, **kw)
+        assert np.array_equal(got[0].cpu().numpy(), ns) and np.array_equal(got[1].cpu().numpy(), tokens)
+        close(got[2], px)
