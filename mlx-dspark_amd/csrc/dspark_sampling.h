@@ -37,6 +37,7 @@ constexpr int kSegVals = 512;          // logits of a segment
 constexpr int kMaxSegs = 1024;         // segments of a row: one LDS slot each in the kernels of a row
 constexpr int kMaxDraft = 255;         // drafts of a sequence
 constexpr int kBins = 30720;           // distinct logit values counted at a time: most of the LDS
+constexpr int kChunk = 4096;           // of them joined at a time
 constexpr int kRowThreads = 1024;      // threads of the kernels that work on one row or sequence
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kListed = 256;           // candidates of a row that are sorted instead of counted

@@ -498,7 +498,8 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
   }
 
   int thr = kb - 1, keep = 0, ties = 0;  // thr = kb - 1: every listed token
-  int loaded = 1 << 17;                  // the range of keys now in the bins starts here
+  int range_hi = -(1 << 17), range_lo = 0;             // the keys now in the bins, bin range_hi - key
+  int merged = top + 1;                  // of a group's counts: from this key up
   const int spg = (a.nseg + gr.n - 1) / gr.n;         // segments of a workgroup of the group
   const int words = (top - kb + 4) >> 2;
   const bool grouped = gr.counts && !few && top - kb < kBins;
@@ -517,21 +518,8 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
       put_far(out_c + i, w);
     }
     if (!arrives_last(gr.arrived, gr.n, &sh.last)) return false;
-    for (int i = t; i < words; i += kRowThreads) {
-      int c[4] = {};
-      uint64_t w[kGroup];                // every workgroup's word at once
-#pragma unroll
-      for (int g = 0; g < kGroup; ++g) w[g] = g < gr.n ? get_far(gr.counts + (long)g * (kBins / 4) + i) : 0;
-#pragma unroll
-      for (int g = 0; g < kGroup; ++g)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] += (int)(w[g] >> (16 * j) & 0xFFFF);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * i + j < kBins) sh.bins[4 * i + j] = c[j];
-    }
-    __syncthreads();
-    loaded = kb;
+    range_hi = top;
+    range_lo = kb;
   }
   double z = 0;
   bool found = false;
@@ -548,15 +536,34 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
     int seen = 0;
     double mass = 0;
     found = false;
-    for (int hi = top; hi >= lowest && !found; hi -= kBins) {
-      const int lo = max(lowest, hi - kBins + 1);
-      if (!(hi == top && loaded <= lo && top - loaded < kBins)) {
-        count_keys<HALF>(a, x, off, sh, nlist, hi, lo);
-        loaded = hi == top ? lo : 1 << 17;
+    for (int hi = top, lo; hi >= lowest && !found; hi = lo - 1) {
+      if (hi > range_hi || hi < range_lo) {
+        range_hi = hi;
+        range_lo = max(kb, hi - kBins + 1);
+        count_keys<HALF>(a, x, off, sh, nlist, range_hi, range_lo);
       }
+      // a few thousand values at a time: the goal is mostly in the first
+      lo = max(max(lowest, range_lo), hi - kChunk + 1);
+      if (grouped && lo < merged) {
+        for (int i = ((top - merged + 1) >> 2) + t; i <= (top - lo) >> 2; i += kRowThreads) {
+          int c[4] = {};
+          uint64_t w[kGroup];            // every workgroup's word at once
+#pragma unroll
+          for (int g = 0; g < kGroup; ++g) w[g] = g < gr.n ? get_far(gr.counts + (long)g * (kBins / 4) + i) : 0;
+#pragma unroll
+          for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[j] += (int)(w[g] >> (16 * j) & 0xFFFF);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sh.bins[4 * i + j] = c[j];
+        }
+        merged = lo;
+        __syncthreads();
+      }
+      const int base = range_hi - hi;    // the bin of hi
       // a run of bins a thread, an odd number of them: neighbours read other banks
       const int nb = hi - lo + 1, each = ((nb + kRowThreads - 1) / kRowThreads) | 1;
-      static_assert(kBins / kRowThreads < 64, "a lane for every bin of a run");
+      static_assert(kChunk / kRowThreads < 64, "a lane for every bin of a run");
       const int b0 = min(t * each, nb), b1 = min(b0 + each, nb);
       int cn = 0;
       double cm = 0;
@@ -564,7 +571,7 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
         FallingWeights<HALF> f;
         f.start(hi - b0, mx, a.c, mc);
         for (int b = b0; b < b1; ++b) {
-          int n = sh.bins[b];
+          int n = sh.bins[base + b];
           if (after_k && hi - b == thr_k) n = keep_k;
           cn += n;
           cm += (double)n * f.w;
@@ -587,7 +594,7 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
         const double run_m = lane_value(mass + mass_before, owner & 63);
         const int b = owner * each + lane;
         const bool in = lane < each && b < nb;
-        const int n_all = in ? sh.bins[b] : 0;
+        const int n_all = in ? sh.bins[base + b] : 0;
         const int n = after_k && hi - b == thr_k && in ? keep_k : n_all;
         const double w = in ? weight(val_of_key<HALF>(hi - b), mx, a.c, mc) : 0.0;
         const int c_end = run_c + wave_scan(n), c0 = c_end - n;
@@ -730,11 +737,11 @@ __device__ __forceinline__ void rest8(const SampleArgs& a, const RowInfo& r, dou
                                       const float (&q)[8], int skip, double (&out)[8]) {
   const double mc = -(double)r.m * a.c;
   int ks[8];
-  keys8(x, ks);
+  if constexpr (CUT) keys8(x, ks);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int k = ks[j], v = v0 + j;
-    const bool kept = k > r.thr || (k == r.thr && v <= r.cut);       // a NaN's weight is 0
+    const int v = v0 + j;
+    const bool kept = !CUT || ks[j] > r.thr || (ks[j] == r.thr && v <= r.cut);       // a NaN's weight is 0
     double w = 0;
     if (!CUT || __any(kept)) {
       w = weight(val<HALF>(bits_of(x, j)), r.m, a.c, mc);
@@ -800,7 +807,7 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
         else sh.sums[t] = r.z > 0 ? a.segs[row * a.nseg + t] * weight(sm, r.m, a.c) : 0.0;
       }
       __syncthreads();
-      if (mode == kDrawOther && d.skip >= 0 && d.skip < a.V && t < 64) {   // the token's own segment again, without it
+      if (mode == kDrawOther && r.z > 0 && d.skip >= 0 && d.skip < a.V && t < 64) {   // the token's own segment again, without it
         const int s = (d.skip + off) / kSegVals, v0 = s * kSegVals + 8 * lane - off;
         double w[8], sum = 0;
         const float q[8] = {};
