@@ -20,6 +20,7 @@ namespace dspark {
 namespace {
 
 constexpr int kKvThreads = 256;
+constexpr int kKvOut = 2;                      // stores of a thread that reads back
 
 struct KvSide {                                // keys or values
   char* x;                                     // plain rows (read, or the output of a read back)
@@ -136,57 +137,78 @@ __global__ __launch_bounds__(kKvThreads) void kv_quantize_kernel(const KvArgs a)
   }
 }
 
-// SRC: type of scales and biases; DST: type of the rows written; ALIGNED as above
+// SRC: type of scales and biases; DST: type of the rows written; ALIGNED as above. An item is one store of 16 bytes
+// (4 or 8 values), the lanes' next to each other; a thread takes kOut of them, their loads first.
 template <int SRC, int DST, int BITS, bool ALIGNED>
 __global__ __launch_bounds__(kKvThreads) void kv_dequantize_kernel(const KvArgs a) {
-  const u32 i = blockIdx.x * kKvThreads + threadIdx.x;
-  if (i >= a.items) return;
+  constexpr int W = DST == DSPARK_DTYPE_F32 ? 4 : 8, kOut = kKvOut, kPerWord = 32 / BITS;
+  const u32 i0 = blockIdx.x * (kKvThreads * kOut) + threadIdx.x, items = a.items * (8 / W), per = a.D8 * (8 / W);
   const int bh = blockIdx.y % (a.B * a.H), b = bh / a.H, h = bh % a.H;
   const KvSide& s = a.side[blockIdx.y >= (unsigned)(a.B * a.H)];
-  const u32 t = i / (u32)a.D8, c = i - t * a.D8;
-  const u32* w = s.w + b * s.wb + h * s.wh + (long)t * s.wt + (BITS / 4) * c;
-  u32x2_t f;
-  if constexpr (BITS == 8) {
-    if constexpr (ALIGNED) f = ldg64(w);
-    else f = u32x2_t{w[0], w[1]};
-  } else {
-    f = u32x2_t{w[0], 0};
-  }
-  const long g = b * s.sb + h * s.sh + (long)t * s.st + (c >> 3);
-  const float sc = kv_get<SRC>(s.s[g]), bias = kv_get<SRC>(s.b[g]);
-  float v[8];
+  u32 w[kOut][2], t[kOut], c[kOut];
+  u16 sc[kOut], bi[kOut];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const u32 q = BITS == 8 ? (f[j >> 2] >> (8 * (j & 3))) & 0xFFu : (f[0] >> (4 * j)) & 0xFu;
-    v[j] = (float)q * sc + bias;
-  }
-  const long at = b * s.xb + h * s.xh + (long)t * s.xt + 8 * c;
-  if constexpr (DST == DSPARK_DTYPE_F32) {
-    float* y = reinterpret_cast<float*>(s.x) + at;
-    if constexpr (ALIGNED) {
-      *reinterpret_cast<f32x4_t*>(y) = f32x4_t{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4_t*>(y + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+  for (int k = 0; k < kOut; ++k) {
+    const u32 i = i0 + k * kKvThreads;
+    if (i >= items) continue;
+    t[k] = i / per;
+    c[k] = (i - t[k] * per) * W;        // first value
+    const u32* p = s.w + b * s.wb + h * s.wh + (long)t[k] * s.wt + c[k] / kPerWord;
+    if constexpr (W > kPerWord) {
+      if constexpr (ALIGNED) {
+        const u32x2_t two = ldg64(p);
+        w[k][0] = two[0];
+        w[k][1] = two[1];
+      } else {
+        w[k][0] = p[0];
+        w[k][1] = p[1];
+      }
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = v[j];
+      w[k][0] = *p >> (W < kPerWord ? (c[k] & (kPerWord - 1)) * BITS : 0);
     }
-  } else {
-    u16* y = reinterpret_cast<u16*>(s.x) + at;
-    if constexpr (ALIGNED) {
-      u32x4_t o;
+    const long g = b * s.sb + h * s.sh + (long)t[k] * s.st + (c[k] >> 6);
+    sc[k] = s.s[g];
+    bi[k] = s.b[g];
+  }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = (u32)kv_put<DST>(v[2 * j]) | ((u32)kv_put<DST>(v[2 * j + 1]) << 16);
-      *reinterpret_cast<u32x4_t*>(y) = o;
+  for (int k = 0; k < kOut; ++k) {
+    if (i0 + k * kKvThreads >= items) break;
+    const float scale = kv_get<SRC>(sc[k]), bias = kv_get<SRC>(bi[k]);
+    float v[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const u32 q = (w[k][j / kPerWord] >> (BITS * (j % kPerWord))) & ((1u << BITS) - 1);
+      v[j] = (float)q * scale + bias;
+    }
+    const long at = b * s.xb + h * s.xh + (long)t[k] * s.xt + c[k];
+    if constexpr (DST == DSPARK_DTYPE_F32) {
+      float* y = reinterpret_cast<float*>(s.x) + at;
+      if constexpr (ALIGNED) {
+        __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4_t*>(y));
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) y[j] = v[j];
+      }
     } else {
+      u16* y = reinterpret_cast<u16*>(s.x) + at;
+      if constexpr (ALIGNED) {
+        u32x4_t o;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = kv_put<DST>(v[j]);
+        for (int j = 0; j < 4; ++j) o[j] = (u32)kv_put<DST>(v[2 * j]) | ((u32)kv_put<DST>(v[2 * j + 1]) << 16);
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4_t*>(y));
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) y[j] = kv_put<DST>(v[j]);
+      }
     }
   }
 }
 
 template <bool WRITE, int A, int C, int BITS, bool AL>
 void launch_kv(const KvArgs& a, hipStream_t s) {
-  const dim3 grid((a.items + kKvThreads - 1) / kKvThreads, (unsigned)(2 * a.B * a.H)), block(kKvThreads);
+  const u32 per = WRITE ? kKvThreads : kKvThreads * kKvOut;
+  const u32 items = WRITE ? a.items : a.items * (C == DSPARK_DTYPE_F32 ? 2 : 1);
+  const dim3 grid((items + per - 1) / per, (unsigned)(2 * a.B * a.H)), block(kKvThreads);
   if constexpr (WRITE) hipLaunchKernelGGL((kv_quantize_kernel<A, C, BITS, AL>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((kv_dequantize_kernel<A, C, BITS, AL>), grid, block, 0, s, a);
 }

@@ -7,7 +7,7 @@
 // the fp64 one by 1e-10. The rotation is fp32, rounded once to the tensors' type.
 //
 // Bound by the bytes of x and y: 16 bytes a lane and access where addresses and strides allow, else one
-// value (the same code at a width of one).
+// value.
 #include "dspark_common.h"
 
 namespace dspark {
@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeHalf = 128;                 // pairs of a head
-constexpr int kRopeTab = 512;                  // (cos, sin) pairs of a workgroup
+constexpr int kRopeRows = 4;                   // most rows of a workgroup
+constexpr int kRopeTab = kRopeRows * kRopeHalf;
 
 struct RopeSide {                              // queries or keys
   const char* x;
@@ -60,15 +61,14 @@ struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
 
-// An item is W pairs (half layout: W values of each half; interleaved: the W values of W / 2 pairs, at
-// W = 1 one pair) or W copied values.
-template <int DT, int W, bool INTER>
-__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
-  using E = Elem<DT>;
-  using T = typename E::t;
-  using P = Pack<T, W>;
-  __shared__ float2 tab[kRopeTab];
-  const int r0 = blockIdx.x * a.tok, nr = min(a.tok, a.rows - r0);
+template <typename T, int W>
+__device__ __forceinline__ void store(T* p, const Pack<T, W>& v) {
+  static_assert(sizeof(v) == 16, "one access");
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p));
+}
+
+// (cos, sin) of a workgroup's rows
+__device__ __forceinline__ void fill_table(const RopeArgs& a, float2* tab, int r0, int nr) {
   for (int i = threadIdx.x; i < nr * a.half; i += kRopeThreads) {
     const int r = r0 + i / a.half, f = i % a.half, b = r / a.L, l = r % a.L;
     long p = a.pos0 + l;
@@ -81,6 +81,90 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
     sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &sn, &cs);
     tab[i] = make_float2(cs * a.scale, sn * a.scale);
   }
+}
+
+template <int DT>
+__device__ __forceinline__ void turn(const float2 cs, typename Elem<DT>::t& x1, typename Elem<DT>::t& x2) {
+  const float u = Elem<DT>::get(x1), v = Elem<DT>::get(x2);
+  x1 = Elem<DT>::put(u * cs.x - v * cs.y);
+  x2 = Elem<DT>::put(u * cs.y + v * cs.x);
+}
+
+// 16 bytes an access, W values, written past the caches (2048 rows of 72 x 128: 14.9 us, 15.8 with plain stores; a
+// copy of the bytes: 14.7). An item of a head is W pairs (half layout: two accesses), the W / 2 pairs of W values
+// (interleaved), or W copied values. A thread keeps its item over the heads of all its workgroup's rows, kOut of
+// them at once: no division in the loop.
+template <int DT, int W, bool INTER>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
+  using T = typename Elem<DT>::t;
+  using P = Pack<T, W>;
+  constexpr int kOut = 3;
+  __shared__ float2 tab[kRopeTab];
+  __shared__ long at_x[2][kRopeRows], at_y[2][kRopeRows];
+  const int r0 = blockIdx.x * a.tok, nr = min(a.tok, a.rows - r0), t = threadIdx.x;
+  if (t < 2 * kRopeRows) {              // where a row starts, queries and keys
+    const int side = t / kRopeRows, i = t % kRopeRows, r = min(r0 + i, a.rows - 1), b = r / a.L, l = r - b * a.L;
+    const RopeSide& s = a.s[side];
+    at_x[side][i] = b * s.xb + l * s.xl;
+    at_y[side][i] = b * s.yb + l * s.yl;
+  }
+  fill_table(a, tab, r0, nr);
+  __syncthreads();
+  const int heads_at_once = kRopeThreads / a.per, first = t / a.per, c = t - first * a.per;
+  if (first >= heads_at_once) return;
+  const int step = gridDim.y * heads_at_once;
+  const bool rot = c < a.rot;
+  const int d = rot ? c * W : 2 * a.half + (c - a.rot) * W;
+  int h = blockIdx.y * heads_at_once + first, r = 0;
+  while (h >= a.heads) {
+    h -= a.heads;
+    ++r;
+  }
+  while (r < nr) {
+    P x1[kOut], x2[kOut];
+    T* y[kOut];
+    int row[kOut];
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      row[i] = r;
+      if (r >= nr) continue;
+      const int side = h >= a.heads0, hs = h - (side ? a.heads0 : 0);
+      const RopeSide& s = a.s[side];
+      const T* x = reinterpret_cast<const T*>(s.x) + at_x[side][r] + hs * s.xh + d;
+      y[i] = reinterpret_cast<T*>(s.y) + at_y[side][r] + hs * s.yh + d;
+      x1[i] = *reinterpret_cast<const P*>(x);
+      if (!INTER && rot) x2[i] = *reinterpret_cast<const P*>(x + a.half);
+      h += step;
+      while (h >= a.heads) {
+        h -= a.heads;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      if (row[i] >= nr) break;
+      const float2* cs = tab + row[i] * a.half;
+      if (rot) {
+#pragma unroll
+        for (int e = 0; e < W; e += INTER ? 2 : 1) {
+          if constexpr (INTER) turn<DT>(cs[(d + e) >> 1], x1[i].v[e], x1[i].v[e + 1]);
+          else turn<DT>(cs[d + e], x1[i].v[e], x2[i].v[e]);
+        }
+      }
+      store(y[i], x1[i]);
+      if (!INTER && rot) store(y[i] + a.half, x2[i]);
+    }
+  }
+}
+
+// The same a value at a time, for addresses, strides and sizes that have no 16 bytes together: an item is a pair or a
+// copied value.
+template <int DT, bool INTER>
+__global__ __launch_bounds__(kRopeThreads) void rope_single_kernel(const RopeArgs a) {
+  using T = typename Elem<DT>::t;
+  __shared__ float2 tab[kRopeTab];
+  const int r0 = blockIdx.x * a.tok, nr = min(a.tok, a.rows - r0);
+  fill_table(a, tab, r0, nr);
   __syncthreads();
   const int per_row = a.heads * a.per, n = nr * per_row;
   for (int i = blockIdx.y * kRopeThreads + threadIdx.x; i < n; i += gridDim.y * kRopeThreads) {
@@ -93,38 +177,14 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
     const RopeSide& s = a.s[side];
     const T* x = reinterpret_cast<const T*>(s.x) + b * s.xb + h * s.xh + l * s.xl;
     T* y = reinterpret_cast<T*>(s.y) + b * s.yb + h * s.yh + l * s.yl;
-    const float2* t = tab + tr * a.half;
-    if (c >= a.rot) {                          // beyond the rotated part
-      const int d = 2 * a.half + (c - a.rot) * W;
-      *reinterpret_cast<P*>(y + d) = *reinterpret_cast<const P*>(x + d);
-    } else if constexpr (!INTER) {
-      const int d = c * W;
-      P x1 = *reinterpret_cast<const P*>(x + d), x2 = *reinterpret_cast<const P*>(x + d + a.half);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const float2 cs = t[d + e];
-        const float u = E::get(x1.v[e]), v = E::get(x2.v[e]);
-        x1.v[e] = E::put(u * cs.x - v * cs.y);
-        x2.v[e] = E::put(u * cs.y + v * cs.x);
-      }
-      *reinterpret_cast<P*>(y + d) = x1;
-      *reinterpret_cast<P*>(y + d + a.half) = x2;
-    } else if constexpr (W == 1) {
-      const float2 cs = t[c];
-      const float u = E::get(x[2 * c]), v = E::get(x[2 * c + 1]);
-      y[2 * c] = E::put(u * cs.x - v * cs.y);
-      y[2 * c + 1] = E::put(u * cs.y + v * cs.x);
+    if (c >= a.rot) {                   // beyond the rotated part
+      y[a.half + c] = x[a.half + c];
     } else {
-      const int d = c * W;
-      P v = *reinterpret_cast<const P*>(x + d);
-#pragma unroll
-      for (int e = 0; e < W; e += 2) {
-        const float2 cs = t[(d + e) >> 1];
-        const float p = E::get(v.v[e]), q = E::get(v.v[e + 1]);
-        v.v[e] = E::put(p * cs.x - q * cs.y);
-        v.v[e + 1] = E::put(p * cs.y + q * cs.x);
-      }
-      *reinterpret_cast<P*>(y + d) = v;
+      const int d1 = INTER ? 2 * c : c, d2 = INTER ? 2 * c + 1 : c + a.half;
+      T u = x[d1], v = x[d2];
+      turn<DT>(tab[tr * a.half + c], u, v);
+      y[d1] = u;
+      y[d2] = v;
     }
   }
 }
@@ -133,13 +193,22 @@ template <int DT, int W>
 void launch_rope(RopeArgs a, bool inter, hipStream_t s) {
   a.rot = inter ? (W == 1 ? a.half : 2 * a.half / W) : a.half / W;
   a.per = a.rot + (a.D - 2 * a.half) / W;
-  // rows of a workgroup: a table of up to 512 (cos, sin), one row where there are few
-  a.tok = a.rows >= 1024 ? kRopeTab / kRopeHalf : 1;
+  // Rows of a workgroup: one, its heads spread over workgroups until there are two a CU where rows are few. Many rows
+  // of few heads share one until a thread has two items (2048 rows of 10 heads x 64: 4.0 us, 4.5 at one row each;
+  // of 72 x 128: 15.5 at two rows, 14.9 at one).
+  const int row_items = a.heads * a.per, fit = (2 * kRopeThreads + row_items - 1) / row_items;
+  a.tok = a.rows >= 1024 ? (fit < kRopeRows ? fit : kRopeRows) : 1;
   const unsigned gx = (unsigned)((a.rows + a.tok - 1) / a.tok);
   const unsigned most = (unsigned)((a.tok * a.heads * a.per + kRopeThreads - 1) / kRopeThreads);
   const unsigned gy = gx >= 512 ? 1u : (most < 512 / gx ? most : (512 / gx ? 512 / gx : 1u));
-  if (inter) hipLaunchKernelGGL((rope_kernel<DT, W, true>), dim3(gx, gy), dim3(kRopeThreads), 0, s, a);
-  else hipLaunchKernelGGL((rope_kernel<DT, W, false>), dim3(gx, gy), dim3(kRopeThreads), 0, s, a);
+  const dim3 grid(gx, gy), block(kRopeThreads);
+  if constexpr (W == 1) {
+    if (inter) hipLaunchKernelGGL((rope_single_kernel<DT, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rope_single_kernel<DT, false>), grid, block, 0, s, a);
+  } else {
+    if (inter) hipLaunchKernelGGL((rope_kernel<DT, W, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rope_kernel<DT, W, false>), grid, block, 0, s, a);
+  }
 }
 
 }  // namespace
