@@ -1,10 +1,11 @@
 // The kernels and entry points of dspark_sampling.h: the truncated softmax of a row
 // (dspark_sampling_probs) and the accept rule of a sampled round (dspark_speculative_verify).
 //
-// A call is two launches (probabilities: three where something is cut). The first leaves every segment's
-// maximum and sum; in the second, with a cut, a workgroup a row finds what is kept of it, and the last one of
-// a sequence to arrive accepts and draws; without a cut, workgroups over a sequence's segments join its rows,
-// accept, sum max(p - q, 0) over their own segments of the refused row, and the last one draws.
+// The first launch leaves every segment's maximum and sum. Then
+//   verify, few candidates a row (a small top_k): a workgroup a row selects and draws, the last of a sequence accepts;
+//   verify, else: one launch selects where something is cut, one of workgroups over a sequence's segments joins its
+//   rows where nothing is, accepts, sums r over the row drawn from, and its last workgroup draws;
+//   probabilities: a launch selects where something is cut, one writes.
 #include "dspark_sampling.h"
 
 namespace dspark {
@@ -13,6 +14,10 @@ namespace {
 // ---------------------------------------------------------------- segments of every row
 
 constexpr int kStatThreads = 256;
+// Segments of a wave in the first pass: its sums are fp64 work that many waves share better (15 rows of 151936 cut by
+// a mass, 30.9 us at 4, 28.7 at 2, 28.4 at 1; 128 rows uncut in fp16 47.9 at 2, 49.2 at 1). Writing probabilities, where
+// a wave joins its row first: 4 (128 rows uncut 39 us, 42 at 2), 2 behind a cut, which has joined it.
+constexpr int kSegWave = 2, kProbWave = 4, kProbCutWave = 2;
 
 // Maximum and sum of weights of every segment: a wave takes SPW segments, their loads first.
 template <bool HALF, int SPW, bool SUM>
@@ -879,35 +884,30 @@ struct CutShared {
   DrawShared draw;
 };
 
-// With a cut: one row a workgroup. Where its candidates are few it draws its token too, in case its draft is the
-// first refused (the random number of the draw is there from the start); the last workgroup of a sequence
-// accepts, and draws from the row it comes to where that is still to do (VERIFY).
-template <bool HALF, bool VERIFY>
+// Rows of few candidates, as a small top_k leaves them: one row a workgroup. It draws its token too, in case its draft
+// is the first refused (the random number of the draw is there from the start); the last workgroup of a sequence
+// accepts, and draws from the row it comes to where that row's candidates were many after all.
+template <bool HALF>
 __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
                                                                  uint64_t* drawn) {
   __shared__ CutShared sh;
   const int ri = blockIdx.x, seq = blockIdx.y, m = a.per - 1, t = threadIdx.x;
   const long row = (long)seq * a.per + ri;
   DrawIn d = {-1, -1, nullptr, 0.0};
-  int draft = -1, len = 0;
+  const int len = drafts_of(a, in, seq), draft = ri < m ? in.draft[(long)seq * m + ri] : -1;
+  if (ri <= len) d = draw_in(a, in, seq, ri, len);
+  const bool inside = draft >= 0 && draft < a.V;
   double uq = 0;
-  if constexpr (VERIFY) {
-    len = drafts_of(a, in, seq);
-    if (ri < m) draft = in.draft[(long)seq * m + ri];
-    if (ri <= len) d = draw_in(a, in, seq, ri, len);
-    const bool inside = draft >= 0 && draft < a.V;
-    if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
-  }
+  if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
   int token;
   RowInfo mine;
   select_row<HALF>(a, seq, ri, draft, d, Group{nullptr, nullptr, 0, 1}, sh.row, mine, token);
   static_assert(sizeof(RowInfo) == 32, "four words");
-  if (t < 4 && (!VERIFY || token < 0)) {
+  if (t < 4 && token < 0) {
     uint64_t w[4];
     __builtin_memcpy(w, &mine, 32);
     put_far(info + 4 * row + t, t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3]);
   }
-  if constexpr (!VERIFY) return;
   if (t == 0) {
     if (ri < m) in.px[(long)seq * m + ri] = (float)mine.px;
     put_far(drawn + row, (uint64_t)(ri >= len || !(uq < mine.px)) << 32 | (u32)token);
@@ -936,16 +936,16 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
   write_tokens(a, in, seq, n, token);
 }
 
-// The same in two launches where a row's candidates may be many and the rows are few: a group of workgroups a row
-// counts and selects, workgroups over the refused row's segments draw (sample_spread_kernel).
+// What is kept of a row, for a launch behind this one: by a group of workgroups where the rows are few (gridDim.x).
 template <bool HALF>
-__global__ __launch_bounds__(kRowThreads) void sample_group_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
+__global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
                                                                    uint64_t* counts, int* arrived) {
   __shared__ RowShared sh;
   const int ri = blockIdx.y, seq = blockIdx.z, m = a.per - 1;
   const long row = (long)seq * a.per + ri;
   const int draft = in.draft && ri < m ? in.draft[(long)seq * m + ri] : -1;
-  const Group gr = {counts + row * gridDim.x * (kBins / 4), arrived + row, (int)blockIdx.x, (int)gridDim.x};
+  const Group gr = {gridDim.x > 1 ? counts + row * gridDim.x * (kBins / 4) : nullptr, arrived + row, (int)blockIdx.x,
+                    (int)gridDim.x};
   int token;
   RowInfo mine;
   if (!select_row<HALF>(a, seq, ri, draft, DrawIn{-1, -1, nullptr, 0.0}, gr, sh, mine, token)) return;
@@ -1169,34 +1169,35 @@ void launch_segments(const SampleArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(sample_table_kernel, dim3(blocks), dim3(kTabThreads), 0, s, a, (int)total, steps);
     return;
   }
-  const dim3 grid(groups(a.nseg, 4), (unsigned)a.per, (unsigned)(a.rows / a.per)), block(kStatThreads);
-  if (a.top_k) hipLaunchKernelGGL((sample_segments_kernel<HALF, 4, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((sample_segments_kernel<HALF, 4, true>), grid, block, 0, s, a);
+  const dim3 grid(groups(a.nseg, kSegWave), (unsigned)a.per, (unsigned)(a.rows / a.per)), block(kStatThreads);
+  if (a.top_k) hipLaunchKernelGGL((sample_segments_kernel<HALF, kSegWave, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((sample_segments_kernel<HALF, kSegWave, true>), grid, block, 0, s, a);
 }
 
-// Whether a row may well have more candidates than are sorted: what the mass alone cuts, a large top_k.
-bool many(const SampleArgs& a) { return !a.top_k || a.top_k > 128; }
+// Whether a row may well have more candidates than are sorted: what the mass alone cuts, a large top_k. Its counting
+// and its draw are then worth more workgroups than one, and a launch each.
+bool many(const SampleArgs& a) { return !a.top_k || a.top_k > kListed / 2; }
 
 template <bool HALF>
-void launch_groups(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, int group, hipStream_t s) {
-  hipLaunchKernelGGL((sample_group_kernel<HALF>), dim3((unsigned)group, (unsigned)a.per, (unsigned)(a.rows / a.per)),
+void launch_select(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, hipStream_t s) {
+  const int group = many(a) ? group_size(a.rows, a.nseg) : 0;
+  hipLaunchKernelGGL((sample_select_kernel<HALF>), dim3(group ? group : 1, (unsigned)a.per, (unsigned)(a.rows / a.per)),
                      dim3(kRowThreads), 0, s, a, in, reinterpret_cast<uint64_t*>(w + l.info),
                      reinterpret_cast<uint64_t*>(w + l.counts), a.arrived + a.rows / a.per);
 }
 
 template <bool HALF>
 void probs(const SampleArgs& a, char* w, const Layout& l, float* out, long ldo, hipStream_t s) {
-  const dim3 grid(groups(a.nseg, 4), (unsigned)a.rows);
-  uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
-  const int group = many(a) ? group_size(a.rows, a.nseg) : 0;
+  const uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
+  const dim3 block(kStatThreads);
   launch_segments<HALF>(a, s);
   if (a.top_k || a.top_p < 1.0) {
-    if (group) launch_groups<HALF>(a, VerifyIn{}, w, l, group, s);
-    else hipLaunchKernelGGL((sample_cut_kernel<HALF, false>), dim3(1, (unsigned)a.rows), dim3(kRowThreads), 0, s, a, VerifyIn{},
-                            info, nullptr);
-    hipLaunchKernelGGL((sample_probs_kernel<HALF, true, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
+    launch_select<HALF>(a, VerifyIn{}, w, l, s);
+    hipLaunchKernelGGL((sample_probs_kernel<HALF, true, kProbCutWave>), dim3(groups(a.nseg, kProbCutWave), (unsigned)a.rows),
+                       block, 0, s, a, info, out, ldo);
   } else {
-    hipLaunchKernelGGL((sample_probs_kernel<HALF, false, 4>), grid, dim3(kStatThreads), 0, s, a, info, out, ldo);
+    hipLaunchKernelGGL((sample_probs_kernel<HALF, false, kProbWave>), dim3(groups(a.nseg, kProbWave), (unsigned)a.rows), block,
+                       0, s, a, info, out, ldo);
   }
 }
 
@@ -1206,16 +1207,15 @@ void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, h
   uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
   double* rest = reinterpret_cast<double*>(w + l.rest);
   const bool cut = a.top_k || a.top_p < 1.0;
-  const int group = cut && many(a) ? group_size(a.rows, a.nseg) : 0;
   // over the rows that are drawn from, a workgroup a CU, at most one a wave and segment
   const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
   const unsigned spread = most < fill ? most : fill;
   launch_segments<HALF>(a, s);
-  if (group) {
-    launch_groups<HALF>(a, in, w, l, group, s);
+  if (cut && many(a)) {
+    launch_select<HALF>(a, in, w, l, s);
     hipLaunchKernelGGL((sample_spread_kernel<HALF, true>), dim3(spread, B), dim3(kRowThreads), 0, s, a, in, info, rest);
   } else if (cut) {
-    hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in, info,
+    hipLaunchKernelGGL((sample_cut_kernel<HALF>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in, info,
                        reinterpret_cast<uint64_t*>(w + l.drawn));
   } else {
     hipLaunchKernelGGL((sample_spread_kernel<HALF, false>), dim3(in.q ? spread : 1, B), dim3(kRowThreads), 0, s, a, in, info,

@@ -885,7 +885,10 @@ def _call_on(dev: torch.device, name: str, args: bytes) -> None:
     """``name(args, current stream of dev)`` with dev as the current device (a launch needs its stream's to be)."""
     index = dev.index
     if index == torch.cuda.current_device():
-        _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None else _raw_stream(index))
+        status = getattr(_lib.load(), name)(args, torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None
+                                            else _raw_stream(index))
+        if status:
+            _lib.check(name, status)
     else:
         with torch.cuda.device(dev):
             _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
@@ -901,11 +904,11 @@ def _no_autograd(what: str, *ts: torch.Tensor) -> None:
 def _one_device(what: str, first: torch.Tensor, *ts) -> torch.device:
     if not first.is_cuda:
         raise ValueError("dspark kernels need tensors on a ROCm device (cuda:N)")
-    dev = first.device
+    index = first.get_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != index:       # -1 for the CPU
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    return first.device
 
 
 def check_sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
@@ -1035,8 +1038,8 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
         ld_seq, ld_row, _ = logits.stride()
     uniforms = uniforms.contiguous()
     n = torch.empty(B, dtype=torch.int32, device=dev)
-    tokens = torch.empty((B, R), dtype=torch.int32, device=dev)
-    draft_p = torch.empty((B, m), dtype=torch.float32, device=dev)
+    tokens = torch.empty(B, R, dtype=torch.int32, device=dev)
+    draft_p = torch.empty(B, m, dtype=torch.float32, device=dev)
     if B:
         ws = _sampling_workspace(workspace, dev, B * R, V, B)
         _call_on(dev, "dspark_speculative_verify",
@@ -1119,7 +1122,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
         q = q.contiguous()
         sq = q.stride()
     if q_out is None:
-        q_out = torch.empty(shape, dtype=dtype, device=dev)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rope_out("q_out", q, q_out)
     so = q_out.stride()
@@ -1130,7 +1133,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
             k = k.contiguous()
             sk = k.stride()
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=dtype, device=dev)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         else:
             _check_rope_out("k_out", k, k_out)
         if k.numel():
@@ -1147,20 +1150,26 @@ KV_CACHE_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _KV_ARGS = struct.Struct("=34q")
 
 
-def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple, cache_dtype) -> tuple:
+def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple, cache_dtype, written: bool) -> tuple:
     """The fields of one ``dspark_kv_side``: plain rows x and the (words, scales, biases) they belong to."""
     w, s, b = trip
-    _require_packed(w)
+    if w.dtype is not torch.int32:
+        _require_packed(w)
     if s.dtype != cache_dtype or b.dtype != cache_dtype:
         raise TypeError(f"{what}: scales and biases of {cache_dtype}, {s.dtype} and {b.dtype}")
-    ws, ss = w.stride(), s.stride()
     if w.shape != words or s.shape != groups or b.shape != groups:
         raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
-    if ws[3] != 1 or ss[3] != 1 or ss != b.stride():
-        if groups[3] > 1 or ws[3] != 1 or ss[:3] != b.stride()[:3]:
-            raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
-    xs = x.stride()
-    return (x.data_ptr(), xs[0], xs[1], xs[2], w.data_ptr(), s.data_ptr(), b.data_ptr(), ws[0], ws[1], ws[2], ss[0], ss[1], ss[2])
+    w0, w1, w2, w3 = w.stride()
+    ss = s.stride()
+    bs = b.stride()
+    s0, s1, s2, s3 = ss
+    if w3 != 1 or ss[:3] != bs[:3] or ((s3 != 1 or bs[3] != 1) and groups[3] > 1):
+        raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
+    if written and not (w0 and w1 and w2 and s0 and s1 and s2):
+        for t in trip:
+            _no_repeats(what, t)
+    x0, x1, x2, _ = x.stride()
+    return x.data_ptr(), x0, x1, x2, w.data_ptr(), s.data_ptr(), b.data_ptr(), w0, w1, w2, s0, s1, s2
 
 
 def _kv_shape(what: str, keys, bits: int, group_size: int):
@@ -1200,10 +1209,8 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     if values.stride(3) != 1:
         values = values.contiguous()
     words = k_rows[0].shape
-    for t in (*k_rows, *v_rows):
-        _no_repeats(what, t)
-    args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt),
-            *_kv_side(what, values, v_rows, words, groups, cdt))
+    args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt, True),
+            *_kv_side(what, values, v_rows, words, groups, cdt, True))
     if B * H * T:
         _call_on(dev, "dspark_kv_quantize", _KV_ARGS.pack(*args))
 
@@ -1219,7 +1226,8 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
         raise TypeError(f"{what}: dtype {dtype} (bfloat16, float16 or float32)")
     shape, groups, cdt = _kv_shape(what, keys, bits, group_size)
     if out is None:
-        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        k = torch.empty(*shape, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t in out:
@@ -1227,8 +1235,8 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
                 raise ValueError(f"{what}: out must be two {dtype} {list(shape)} with unit last stride")
             _no_repeats(what, t)
     words = keys[0].shape
-    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt),
-            *_kv_side(what, v, values, words, groups, cdt))
+    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt, False),
+            *_kv_side(what, v, values, words, groups, cdt, False))
     if shape[0] * shape[1] * shape[2]:
         _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v
