@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kStatThreads) void sample_segments_kernel(const Sam
 // The same over many segments of bf16 logits, uncut: a value's weight against 0, 2^(c x), from a table in LDS.
 // bf16 has 128 values an octave; 22 octaves, 2^-14 to 2^8, and both signs are 45 KB, formed once by each workgroup
 // (one a CU, its waves then walk through the segments). A look-up and its sum are 6 instructions, one of them fp64;
-// the weight itself is 16, nearly all fp64, and bounds the pass above (76032 segments: 37 us; the table's: TABLE_US).
+// the weight itself is 16, nearly all fp64, and bounds the pass above (76032 segments: 37 us; the table's: 21).
 // The sums stand against 0, so no maximum is looked for. A value the table does not have turns the sum into NaN, one
 // below -256 counts as none; a segment of either kind, or too light for what was left out, is summed plainly.
 constexpr int kTabLow = (127 - 14) << 7, kTabHalf = 22 << 7;

@@ -290,3 +290,56 @@ def test_many_candidates(dev, n, V, dtype, kw):
         ns, tokens, px = ref.verify(_np(x), d.numpy(), u.numpy(), q.numpy() if dense else None, **kw)
         assert np.array_equal(got[0].cpu().numpy(), ns) and np.array_equal(got[1].cpu().numpy(), tokens)
         close(got[2], px)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=3), dict(top_p=0.8), dict(top_k=130, top_p=0.9)])
+def test_many_short_rows_and_long_blocks(dev, kw):
+    """The most rows and the most drafts a call takes; one more of either is refused."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(8)
+    x = rows(g, 60000, 40, torch.bfloat16).view(30000, 2, 40)
+    d, q = _drafts(g, x, "plain", 1)
+    u = torch.rand(30000, 2, generator=g)
+    got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev), **kw)
+    pick = slice(0, 30000, 37)
+    n, tokens, px = ref.verify(_np(x[pick]), d[pick].numpy(), u[pick].numpy(), q[pick].numpy(), **kw)
+    assert np.array_equal(got[0][pick].cpu().numpy(), n) and np.array_equal(got[1][pick].cpu().numpy(), tokens)
+    close(got[2][pick], px)
+    close(ops.sampling_probs(x[pick].to(dev), **kw), np.stack([[ref.probs(r, **kw) for r in s] for s in _np(x[pick])]))
+    x = rows(g, 512, 3000, torch.float16).view(2, 256, 3000)
+    x[:, :, 7] = 30.0
+    d = torch.full((2, 255), 7)
+    d[1, 200] = 8
+    u = torch.rand(2, 256, generator=g)
+    got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), **kw)
+    n, tokens, px = ref.verify(_np(x), d.numpy(), u.numpy(), **kw)
+    assert n[0] > 200 and np.array_equal(got[0].cpu().numpy(), n) and np.array_equal(got[1].cpu().numpy(), tokens)
+    close(got[2], px)
+    with pytest.raises(ValueError):
+        ops.speculative_verify(x[:, :1].expand(2, 257, 3000).to(dev), d[:, :1].expand(2, 256).to(dev), torch.rand(2, 257, device=dev))
+    with pytest.raises(ValueError):
+        ops.sampling_probs(torch.zeros(65536, 2, dtype=torch.bfloat16, device=dev))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20), dict(top_p=0.9)])
+def test_the_same_bits_each_time(dev, kw):
+    """Repeated calls on one input, with other calls between on another stream: nothing depends on which workgroup
+    arrives last."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(12)
+    x = rows(g, 24, 100003, torch.bfloat16, "ties").view(4, 6, 100003)
+    d, q = _drafts(g, x, "plain", 5)
+    args = x.to(dev), d.to(dev), torch.rand(4, 6, generator=g).to(dev)
+    q = q.to(dev)
+    want = ops.speculative_verify(*args, draft_probs=q, **kw)
+    probs = ops.sampling_probs(args[0], **kw)
+    other = torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(other):
+            ops.sampling_probs(args[0], **kw)
+        got = ops.speculative_verify(*args, draft_probs=q, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(ops.sampling_probs(args[0], **kw), probs)
+    torch.cuda.synchronize()
