@@ -597,6 +597,7 @@ int dspark_argmax_accept(const void* logits, int64_t ld, int64_t M, int64_t V, c
  *   are ordered by index. A row with nothing but -inf and NaN gives zeros.
  * logits bf16 or fp16 [rows, V] (row stride ld, any alignment), V <= 524280, rows <= 65535. Weights and
  * sums are fp64. workspace >= dspark_sampling_workspace(rows, V, 0) bytes, 256-byte aligned, of any content.
+ * One call at a time uses it: calls on two streams, or graphs that may run together, need one each.
  * Covers the reference's truncate_probs (sampling.py) with the softmax before it.
  */
 size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences);
@@ -632,7 +633,7 @@ int dspark_sampling_probs(const dspark_sampling_probs_args* args, dspark_stream 
  * n_accepted int32 [sequences]; tokens int32 [sequences, drafts + 1]; draft_p fp32 [sequences, drafts]
  *            (p_i(draft_i) of every draft, those after the first refused one too)
  * workspace >= dspark_sampling_workspace(sequences * (drafts + 1), V, sequences) bytes, 256-byte aligned,
- * of any content. The sampling counterpart of dspark_argmax_accept (generate.py's sampling accept).
+ * of any content, one call's at a time. The sampling counterpart of dspark_argmax_accept (generate.py's sampling accept).
  */
 typedef struct dspark_speculative_verify_args { /* every field is 8 bytes */
   int64_t dtype;
@@ -665,10 +666,10 @@ int dspark_speculative_verify(const dspark_speculative_verify_args* args, dspark
  * for the pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved, of the first dims values of a head; the
  * other D - dims are copied. fp32 with the angle reduced in fp64, rounded once to dtype (bf16, fp16, fp32).
  * Strides (batch, head, row) in elements, unit stride along D; 16-byte accesses where every address and
- * stride allows, else single values. y may be x itself (the same address and strides), not overlap it
- * otherwise. positions: int32 or (positions_i64) int64 of row (b, l) at b * stride[0] + l * stride[1];
+ * stride allows, else single values. y may be x itself (the same address and strides); what is written
+ * shares no element with anything else that is read or written. positions: int32 or (positions_i64) int64 of row (b, l) at b * stride[0] + l * stride[1];
  * NULL: pos0 + l. freqs fp64 [dims / 2] on the device, in radians a position.
- * D <= 1024, dims even and <= 256, B * L <= 2^24. Covers mx.fast.rope as mlx-lm's layers call it
+ * D <= 1024, dims even and <= 256, B * L < 2^24. Covers mx.fast.rope as mlx-lm's layers call it
  * (traditional or not, dims below the head, offset and freqs arrays), which dspark_qk_norm_rope_kv fuses
  * for one layout.
  */
@@ -694,7 +695,8 @@ int dspark_rope(const dspark_rope_args* args, dspark_stream stream);
  * Per group of 64 values of x [B, H, T, D] (bf16, fp16 or fp32), every step one fp32 operation:
  *   scale = (max - min) * fl(1 / (2^bits - 1)) and bias = min, rounded to cache_dtype (bf16 or fp16);
  *   field = clamp(round_half_even((x - bias) / scale), 0, 2^bits - 1), a scale of 0 dividing as 1
- * (dspark_qk_norm_rope_kv_quantized's rule but for the quotient by 2^bits - 1). A NaN makes its group's scale and bias NaN, its fields 0.
+ * (dspark_qk_norm_rope_kv_quantized's rule but for the quotient by 2^bits - 1). A NaN makes its group's scale
+ * and bias NaN, its fields 0. The six arrays written share no element with each other or with x.
  * words uint32 [B, H, T, D * bits / 32], scales and biases [B, H, T, D / 64] (shared strides), unit stride
  * along the last dim: rows of a cache view. D % 64 == 0, group_size 64, 2 * B * H <= 65535.
  */

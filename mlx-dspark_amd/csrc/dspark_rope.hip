@@ -224,7 +224,8 @@ extern "C" int dspark_rope(const dspark_rope_args* p, dspark_stream stream) {
     return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %lld", what, (long long)dt);
   if (D < 2 || D > 1024 || dims < 2 || dims > 2 * kRopeHalf || dims % 2 || dims > D)
     return fail(DSPARK_ERR_SHAPE, "%s: head_dim %lld (2..1024), rotated part %lld (even, up to it and to 256)", what, (long long)D, (long long)dims);
-  if (B < 1 || L < 1 || B > (1 << 24) || L > (1 << 24) || B * L > (1 << 24) || Hq < 1 || Hk < 0 || Hq > 4096 || Hk > 4096 ||
+  // a workgroup a row: fewer than 2^32 threads
+  if (B < 1 || L < 1 || B > (1 << 24) || L > (1 << 24) || B * L >= (1 << 24) || Hq < 1 || Hk < 0 || Hq > 4096 || Hk > 4096 ||
       Hq + Hk > 4096)
     return fail(DSPARK_ERR_SHAPE, "%s: B=%lld L=%lld Hq=%lld Hk=%lld", what, (long long)B, (long long)L, (long long)Hq, (long long)Hk);
   const int64_t es = dt == DSPARK_DTYPE_F32 ? 4 : 2, wide = 16 / es;

@@ -234,7 +234,7 @@ __device__ __forceinline__ V get_far(const V* p) { return __hip_atomic_load(p, _
 
 // True in every thread of the workgroup that arrives last of `n`; what the others put before it is there to get.
 __device__ __forceinline__ bool arrives_last(int* counter, int n, int* slot) {
-  __builtin_amdgcn_s_waitcnt(0);       // this thread's stores are complete
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");     // this thread's stores are complete
   __syncthreads();
   if (threadIdx.x == 0) *slot = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
   __syncthreads();

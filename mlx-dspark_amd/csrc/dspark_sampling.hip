@@ -1265,7 +1265,9 @@ extern "C" int dspark_speculative_verify(const dspark_speculative_verify_args* p
                 (long long)p->drafts, (long long)p->V);
   if (p->ld_seq < 0 || p->ld_row < 0 || (p->draft_probs && (p->q_seq < 0 || p->q_row < 0)))
     return fail(DSPARK_ERR_SHAPE, "%s: negative strides", what);
-  if (!aligned(p->uniforms, p->uniforms_f64 ? 8 : 4)) return fail(DSPARK_ERR_ALIGN, "%s: uniforms alignment", what);
+  if (!aligned(p->uniforms, p->uniforms_f64 ? 8 : 4) || !aligned(p->draft, 4) || !aligned(p->draft_probs, 4) ||
+      !aligned(p->draft_lens, 4) || !aligned(p->n_accepted, 4) || !aligned(p->tokens, 4) || !aligned(p->draft_p, 4))
+    return fail(DSPARK_ERR_ALIGN, "%s: arrays need the alignment of their type", what);
   const int64_t rows = p->sequences * (p->drafts + 1);
   const Layout l = layout(rows, p->V, p->sequences);
   SampleArgs a;

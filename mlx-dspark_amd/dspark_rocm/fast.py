@@ -108,9 +108,12 @@ def read_back_kernel(q, q_keys, q_values, bits, group_size) -> bool:
     if not all(isinstance(t, torch.Tensor) for t in (q, *ts)) or not ops.eager_inference(q, *ts):
         return False
     (kw, ks, kb), (vw, vs, vb) = q_keys, q_values
-    if kw.dim() != 4 or bits not in ops.KV_BITS or group_size != ops.GROUP or kw.shape[3] * 32 // bits % ops.GROUP:
+    if kw.dim() != 4 or bits not in ops.KV_BITS or group_size != ops.GROUP:
         return False
-    groups = (*kw.shape[:3], kw.shape[3] * 32 // bits // ops.GROUP)
+    d = kw.shape[3] * 32 // bits
+    if d % ops.GROUP or d > 4096:
+        return False
+    groups = (*kw.shape[:3], d // ops.GROUP)
     return (kw.numel() > 0 and kw.dtype in (torch.int32, torch.uint32) and vw.dtype == kw.dtype and vw.shape == kw.shape
             and ks.dtype in ops.KV_CACHE_DTYPES and 2 * kw.shape[0] * kw.shape[1] <= 65535
             and all(t.dtype == ks.dtype and tuple(t.shape) == groups for t in (ks, kb, vs, vb))

@@ -147,6 +147,8 @@ class QuantizedKVCache:
         return (keys.shape == values.shape and keys.dim() == 4 and keys.dtype == values.dtype
                 and keys.dtype in ops.DEQUANT_DTYPES and self.dtype in ops.KV_CACHE_DTYPES and keys.shape[2] > 0
                 and tuple(keys.shape[:2]) == (self.batch, self.kv_heads) and keys.shape[3] == self.head_dim
+                and self.bits in ops.KV_BITS and self.group_size == ops.GROUP
+                and self.head_dim % ops.GROUP == 0 and self.head_dim <= 4096
                 and 2 * self.batch * self.kv_heads <= 65535
                 and all(t.device == keys.device for t in (values, *self.keys, *self.values)))
 

@@ -165,7 +165,7 @@ class Attention(nn.Module):
         if self._rope is None or self._rope[0].device != q.device:
             self._rope = a.rope_table(q.device)
         freqs, scale = self._rope
-        if ops.eager_inference(q, k) and q.dtype in ops.ROPE_DTYPES:
+        if ops.eager_inference(q, k) and q.dtype in ops.ROPE_DTYPES and freqs.numel() <= 128 and a.head_dim <= 1024:
             return ops.rope(q, k, freqs, pos0, interleaved=a.rope_traditional, scale=scale)
         return tuple(rope_tables.rotate(t, freqs, pos0, interleaved=a.rope_traditional, scale=scale) for t in (q, k))
 
@@ -714,6 +714,8 @@ class Target:
                                         or draft_probs.requires_grad):
             raise ValueError(f"draft_probs: fp32 [{m}, {V}] without gradients, got {draft_probs.dtype} {list(draft_probs.shape)}")
         ops.check_sampler(temperature, top_k, top_p)
+        if not ops.sampling_workspace_bytes(M, V, 1):
+            raise ValueError(f"a vocabulary of {V} (up to 524280)")
         probs = None if draft_probs is None else draft_probs.to(dev)[None]
         logits, fused = self.verify(torch.tensor([[pending] + list(draft)], dtype=torch.int64), cache, tap)
         _, tokens, _ = ops.speculative_verify(logits, torch.tensor([list(draft)], dtype=torch.int32, device=dev).view(1, m),

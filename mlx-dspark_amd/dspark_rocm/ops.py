@@ -948,7 +948,7 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     which less than ``top_p`` of their mass lies, 0 elsewhere. Equal logits are ordered by index; a row
     of nothing but -inf and NaN gives zeros. What a drafter samples its tokens from and hands to
     :func:`speculative_verify`. ``out`` contiguous; ``workspace`` (any content) of
-    :func:`sampling_workspace_bytes`, else allocated."""
+    :func:`sampling_workspace_bytes` for one call at a time, else allocated."""
     dev = _one_device("sampling_probs", logits, out, workspace)
     dt = LOGIT_DTYPES.get(logits.dtype)
     if dt is None:
@@ -999,7 +999,8 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
     from ``max(p - q, 0)`` of the refused row, or from p of the row after the last draft, then -1; the
     committed tokens then follow p whatever the drafter proposed. ``draft_p``: p of every draft.
     ``draft_lens`` [B] (padded batches): how many drafts each sequence has. ``uniforms`` [B, m + 1] fp32 or
-    fp64 in [0, 1). Drafts outside the vocabulary are refused. m up to 255."""
+    fp64 in [0, 1). Drafts outside the vocabulary are refused. m up to 255. ``workspace`` as in
+    :func:`sampling_probs`: two streams, or two graphs that may run together, need one each."""
     what = "speculative_verify"
     dev = _one_device(what, logits, draft, uniforms, draft_probs, draft_lens, workspace)
     dt = LOGIT_DTYPES.get(logits.dtype)
@@ -1065,6 +1066,13 @@ def _no_repeats(what: str, out: torch.Tensor) -> None:
         raise ValueError(f"{what}: the output is an expanded view ({list(out.shape)}, strides {list(out.stride())})")
 
 
+def _no_aliases(what: str, *ts: torch.Tensor) -> None:
+    """Each of ``ts`` starts elsewhere: the same rows given twice would be written by two workgroups."""
+    at = [t.data_ptr() for t in ts]
+    if len(set(at)) != len(at):
+        raise ValueError(f"{what}: the same rows given twice")
+
+
 def _check_rope_out(name: str, x: torch.Tensor, out: torch.Tensor) -> None:
     if out.dtype != x.dtype or out.shape != x.shape or out.stride(3) != 1:
         raise ValueError(f"rope: {name} must be {x.dtype} {list(x.shape)} with unit last stride")
@@ -1087,7 +1095,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
     ``scale`` multiplies; the rest is copied. ``positions``: an int (row l stands at ``positions + l``), or
     an int32 / int64 tensor [L] or [B or 1, L or 1] with the position of every row, as tree rows need. The
     angle is reduced in fp64; one rounding to the tensors' type. ``q_out`` / ``k_out``: where to write,
-    e.g. a cache's rows, or q and k themselves."""
+    e.g. a cache's rows, or q and k themselves; elements that nothing else of the call uses."""
     dev = _one_device("rope", q, k, freqs, q_out, k_out)
     dtype, shape = q.dtype, q.shape
     dt = ROPE_DTYPES.get(dtype)
@@ -1101,7 +1109,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
         raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(freqs.shape)}")
     if k is None and k_out is not None:
         raise ValueError("rope: k_out without k")
-    _no_autograd("rope", q, *(() if k is None else (k,)))
+    _no_autograd("rope", *(t for t in (q, k, freqs, q_out, k_out) if t is not None))
     freqs = freqs.contiguous()
     pos, pos64, pb, pl, pos0 = 0, 0, 0, 0, 0
     if isinstance(positions, torch.Tensor):
@@ -1137,6 +1145,10 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
         else:
             _check_rope_out("k_out", k, k_out)
         if k.numel():
+            if q.numel():
+                _no_aliases("rope", q_out, k_out)
+                if q_out.data_ptr() == k.data_ptr() or k_out.data_ptr() == q.data_ptr():
+                    raise ValueError("rope: the queries' output is the keys' input, or the other way round")
             sko = k_out.stride()
             keys = (k.data_ptr(), k_out.data_ptr(), sk[0], sk[1], sk[2], sko[0], sko[1], sko[2], k.shape[1])
     if q.numel() or keys is not _NO_KEYS:
@@ -1212,6 +1224,7 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt, True),
             *_kv_side(what, values, v_rows, words, groups, cdt, True))
     if B * H * T:
+        _no_aliases(what, *k_rows, *v_rows)
         _call_on(dev, "dspark_kv_quantize", _KV_ARGS.pack(*args))
 
 
@@ -1238,5 +1251,6 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt, False),
             *_kv_side(what, v, values, words, groups, cdt, False))
     if shape[0] * shape[1] * shape[2]:
+        _no_aliases(what, k, v)
         _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v

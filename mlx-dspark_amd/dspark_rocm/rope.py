@@ -11,7 +11,7 @@ values, and the factor its rotated values are multiplied with. ``scaling`` is th
   over the original length stands between the two factors;
 * ``yarn``: pairs that turn more than ``beta_fast`` (32) times over the original length kept, under
   ``beta_slow`` (1) divided by ``factor``, in between weighted by the pair's index; rotated values times
-  ``attention_factor`` (``0.1 ln(factor) + 1``).
+  ``attention_factor`` (``0.1 ln(factor) + 1``). ``mscale``, ``mscale_all_dim`` and ``truncate`` are refused.
 
 :func:`rotate` is the same rotation in torch ops, for tensors the kernel does not take (CPU, autograd).
 """
@@ -53,6 +53,8 @@ def frequencies(dims: int, base: float, scaling: dict | None = None, *, device=N
             f[i] = v * (kept + (1.0 - kept) / factor)
     elif kind == "yarn":
         length, = _need(scaling, "original_max_position_embeddings")
+        if scaling.get("mscale") or scaling.get("mscale_all_dim") or not scaling.get("truncate", True):
+            raise ValueError(f"rope scaling {scaling}: mscale, mscale_all_dim and truncate are not taken")
         if not (base > 1 and length > 0):
             raise ValueError(f"rope scaling {scaling}: base={base} (over 1), a positive original length")
         given = lambda name, default: float(default if scaling.get(name) is None else scaling[name])

@@ -201,3 +201,39 @@ def test_stream_and_graph(dev):
         kept = [t.clone() for t in z]
         ops.quantize_kv(*x, *trips, bits=8)
         assert all(torch.equal(a, b) for a, b in zip(kept, ops.dequantize_kv(*trips, bits=8)))
+
+
+def test_rows_given_twice(dev):
+    """Rows that two workgroups would write, or one write while another reads: refused."""
+    from dspark_rocm import ops, rope
+
+    x = torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16, device=dev)
+    t, u = (cache(1, 2, 3, 64, 8, torch.bfloat16, dev) for _ in range(2))
+    for k_rows, v_rows in ((t, t), ((t[0], t[1], t[1]), u), (t, (u[0], t[1], u[2]))):
+        with pytest.raises(ValueError, match="twice"):
+            ops.quantize_kv(x, x, k_rows, v_rows, bits=8)
+    out = torch.empty_like(x, dtype=torch.float32)
+    with pytest.raises(ValueError, match="twice"):
+        ops.dequantize_kv(t, u, bits=8, out=(out, out))
+    f, y = rope.frequencies(64, 1e4, device=dev)[0], torch.zeros_like(x)
+    for args, kw in (((x, y), dict(q_out=x, k_out=x)), ((x, x), dict(q_out=x)), ((x, y), dict(k_out=x)), ((x, y), dict(q_out=y))):
+        with pytest.raises(ValueError):
+            ops.rope(*args, f, 0, **kw)
+    with pytest.raises(ValueError, match="backward"):
+        ops.rope(x, None, f.clone().requires_grad_(), 0)
+    ops.rope(x, y, f, 0, q_out=x, k_out=y)
+
+
+def test_heads_past_the_kernel(dev):
+    """Heads wider than the kernels take: the cache and its read back go by torch ops, as they did."""
+    from dspark_rocm import fast
+    from dspark_rocm.kv_cache import QuantizedKVCache
+    from dspark_rocm.quant import quantize_rows
+
+    D = 4096 + 64
+    x = torch.randn(1, 1, 2, D, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(dev)
+    c = QuantizedKVCache(1, 1, D, bits=8, device=dev)
+    keys, values = c.update_and_fetch(x, x)
+    for got, want in zip(keys, quantize_rows(x, 8, 64, torch.bfloat16)):
+        assert torch.equal(got, want)
+    assert not fast.read_back_kernel(x, keys, values, 8, 64)

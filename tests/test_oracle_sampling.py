@@ -104,3 +104,16 @@ def test_host_checks():
         with pytest.raises(ValueError):
             ops.check_sampler(**{**dict(temperature=1.0, top_k=0, top_p=1.0), **bad})
     assert ops.sampling_workspace_bytes(16, 151936, 1) > 16 * 297 * 12
+
+
+@pytest.mark.parametrize("at", [7, 8, 11, 17, 18, 19])
+def test_speculative_verify_refuses_odd_addresses(at):
+    """Each array of 4-byte elements (field ``at`` of the struct) two bytes off: refused on the host."""
+    from dspark_rocm import ops
+
+    lib = _lib()
+    fake = 1 << 20
+    fields = [0, fake, 400, 100, 2, 3, 100, fake, fake, 300, 100, fake, fake, 0, 1.0, 0, 1.0, fake, fake, fake, fake,
+              lib.dspark_sampling_workspace(8, 100, 2)]
+    fields[at] = fake + 2
+    assert lib.dspark_speculative_verify(ops._VERIFY_ARGS.pack(*fields), None) == -3

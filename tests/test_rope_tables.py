@@ -139,3 +139,17 @@ def test_host_checks():
         ops.quantize_kv(x, x, (w, s, s), (w, s, s), bits=8)
     with pytest.raises(ValueError, match="ROCm device"):
         ops.dequantize_kv((w, s, s), (w, s, s), bits=8)
+
+
+@pytest.mark.parametrize("extra", [dict(mscale=1.0), dict(mscale_all_dim=0.7), dict(truncate=False)])
+def test_yarn_settings_that_are_not_taken(extra):
+    with pytest.raises(ValueError, match="not taken"):
+        rope.frequencies(64, 1e4, dict(type="yarn", factor=4.0, original_max_position_embeddings=4096, **extra))
+
+
+def test_rows_past_one_launch():
+    """A workgroup a row: 2^24 rows are 2^32 threads."""
+    fake, six = 1 << 20, (64,) * 6
+    pack = lambda B, L: ops._ROPE_ARGS.pack(0, fake, fake, *six, 1, 0, 0, *six, 0, B, L, 64, 64, 0, fake, 1.0, 0, 0, 0, 0, 0)
+    for B, L in ((1, 1 << 24), (1 << 24, 1), (1 << 12, 1 << 12)):
+        assert _lib.load().dspark_rope(pack(B, L), None) == -2
