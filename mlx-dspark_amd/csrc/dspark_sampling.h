@@ -51,6 +51,7 @@ struct SampleArgs {
   double c;                            // log2(e) / T
   double top_p;
   int top_k;                           // 0: none
+  int parts;                           // of a segment, whose maxima bound the top_k (0: whole segments)
   float* segm;                         // [rows][nseg] segment maxima
   double* segs;                        // [rows][nseg] segment sums
   int* arrived;                        // [sequences], [rows]: workgroups that are done, cleared by the first launch
@@ -250,15 +251,12 @@ __device__ __forceinline__ int row_off(const u16* row) { return (int)((reinterpr
 template <bool HALF>
 __device__ __forceinline__ u32x4_t load8(const u16* row, int v0, int V) {
   if (v0 >= 0 && v0 + 8 <= V) return ldg128(row + v0);
-  uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-  for (int i = 0; i < 8; ++i) {        // a row's ends: one at a time, the first shifted down to the lowest bits
-    const int v = v0 + i;
-    const uint64_t b = v >= 0 && v < V ? row[v] : 0x8000u | kInfBits<HALF>;
-    lo = lo >> 16 | hi << 48;
-    hi = hi >> 16 | b << 48;
-  }
-  return u32x4_t{(u32)lo, (u32)(lo >> 32), (u32)hi, (u32)(hi >> 32)};
+  u32 b[8];                            // a row's ends: each on its own, from inside the row
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = row[min(max(v0 + i, 0), V - 1)];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = v0 + i >= 0 && v0 + i < V ? b[i] : 0x8000u | kInfBits<HALF>;
+  return u32x4_t{b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16};
 }
 __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >> 1] >> (16 * (j & 1))) & 0xFFFFu; }
 

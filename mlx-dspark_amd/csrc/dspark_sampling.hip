@@ -6,6 +6,8 @@
 //   verify, else: one launch selects where something is cut, one of workgroups over a sequence's segments joins its
 //   rows where nothing is, accepts, sums r over the row drawn from, and its last workgroup draws;
 //   probabilities: a launch selects where something is cut, one writes.
+#include <cmath>
+
 #include "dspark_sampling.h"
 
 namespace dspark {
@@ -150,16 +152,7 @@ __global__ __launch_bounds__(kTabThreads) void sample_table_kernel(const SampleA
 
 constexpr int kAhead = 4;              // segments of a wave whose loads are out together
 
-struct RowShared {
-  union {
-    int bins[kBins];
-    struct {                           // a few candidates, one by one
-      uint64_t cand[kListed];          // (key + 2^15) << 32 | ~index: the larger the earlier in falling order
-      uint64_t sorted[kListed];
-      double w[kListed], r[kListed];   // weights in falling order; what is drawn from, by index
-      int order[kListed];              // the kept tokens by index
-    };
-  };
+struct RowState {
   int skey[kMaxSegs];                  // key of each segment's maximum
   int list[kMaxSegs];                  // the segments that may hold a kept token, in no order
   int cnt[kMaxSegs];
@@ -170,38 +163,58 @@ struct RowShared {
   double z;
 };
 
+struct Few {                           // a few candidates, one by one
+  uint64_t cand[kListed];              // (key + 2^15) << 32 | ~index: the larger the earlier in falling order
+  uint64_t sorted[kListed];
+  double w[kListed], r[kListed];       // weights in falling order; what is drawn from, by index
+  int order[kListed];                  // the kept tokens by index
+};
+
+struct RowShared : RowState {
+  union {
+    int bins[kBins];
+    Few few;
+  };
+};
+
+// The bin, of 256 in falling order, that the k-th of what they count lies in; k: which of that bin's it is. Every
+// wave for itself, four bins a lane.
+__device__ __forceinline__ int nth_bin(const int* hist, int& k) {
+  const int lane = threadIdx.x & 63;
+  int c[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * lane + i];
+  const int upto = wave_scan(sum);
+  int before = upto - sum, at = 0;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (at == i && before + c[i] < k) {
+      before += c[i];
+      at = i + 1;
+    }
+  const int owner = __ffsll(__ballot(upto >= k)) - 1;
+  k -= __builtin_amdgcn_readlane(before, owner);
+  return 4 * owner + __builtin_amdgcn_readlane(at, owner);
+}
+
 // The largest key that at least k of the threads' keys reach (`in`: a thread that has one; there are at least k):
 // counts of the high bytes in falling order, then of the low bytes of the one the k-th lies in. `hist`: 512 zeros.
 __device__ __forceinline__ int kth_key(bool in, int key, int k, int* hist) {
-  const int lane = threadIdx.x & 63;
   const u32 u = (u32)(key + (1 << 15));
-  int high = 0;
+  int high = 0, low = 0;
   for (int round = 0; round < 2; ++round) {
     const int bin = 255 - (round ? (int)(u & 255) : (int)(u >> 8));
     if (in && (!round || (int)(u >> 8) == high)) atomicAdd(&hist[256 * round + bin], 1);
     __syncthreads();
-    int c[4], sum = 0;                   // four bins a lane, every wave for itself
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum += c[i] = hist[256 * round + 4 * lane + i];
-    const int upto = wave_scan(sum);
-    int before = upto - sum, at = 0;
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (at == i && before + c[i] < k) {
-        before += c[i];
-        at = i + 1;
-      }
-    const int owner = __ffsll(__ballot(upto >= k)) - 1;
-    const int got = 255 - (4 * owner + __builtin_amdgcn_readlane(at, owner));
-    k -= __builtin_amdgcn_readlane(before, owner);
+    const int got = 255 - nth_bin(hist + 256 * round, k);
     if (round == 0) high = got;
-    else return (high << 8 | got) - (1 << 15);
+    else low = got;
   }
-  return 0;
+  return (high << 8 | low) - (1 << 15);
 }
 
 // The segments of s0 .. s1 whose maximum reaches `lo`, into sh.list; their number in sh.nlist (0 on entry).
-__device__ __forceinline__ int list_segments(RowShared& sh, int s0, int s1, int lo) {
+__device__ __forceinline__ int list_segments(RowState& sh, int s0, int s1, int lo) {
   const int t = threadIdx.x, lane = t & 63;
   const bool f = t >= s0 && t < s1 && sh.skey[t] >= lo;        // kMaxSegs <= kRowThreads
   const unsigned long long on = __ballot(f);
@@ -236,21 +249,25 @@ __device__ __forceinline__ void each_listed(const SampleArgs& a, const u16* x, i
   }
 }
 
-// Counts the logits of the listed segments by key, bin hi - key for lo <= key <= hi.
+// Counts 8 logits of a lane by key, bin hi - key for lo <= key <= hi.
+template <bool HALF>
+__device__ __forceinline__ void count_seg(const u32x4_t& v, RowShared& sh, int hi, int lo) {
+  int k[8];
+  keys8(v, k);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const u32 b = (u32)(hi - k[j]);
+    if (b <= (u32)(hi - lo)) atomicAdd(&sh.bins[b], 1);
+  }
+}
+
+// The same of the listed segments.
 template <bool HALF>
 __device__ __forceinline__ void count_keys(const SampleArgs& a, const u16* x, int off, RowShared& sh, int nlist, int hi,
                                            int lo) {
   for (int i = threadIdx.x; i <= hi - lo; i += kRowThreads) sh.bins[i] = 0;
   __syncthreads();
-  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) {
-    int k[8];
-    keys8(v, k);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const u32 b = (u32)(hi - k[j]);
-      if (b <= (u32)(hi - lo)) atomicAdd(&sh.bins[b], 1);
-    }
-  });
+  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) { count_seg<HALF>(v, sh, hi, lo); });
   __syncthreads();
 }
 
@@ -301,44 +318,301 @@ struct DrawIn {                        // what a row's own draw goes by
 };
 
 constexpr int kGroup = 16;             // most workgroups that count a row together
+constexpr int kOwn = 2;                // segments of a wave whose loads are out together
 struct Group {                         // a row counted by several workgroups, each over its own run of segments
   uint64_t* counts;                    // of each workgroup, 4 bins of 16 bits a word; null: one workgroup a row
   int* arrived;                        // workgroups of this row that are done
   int g, n;
 };
 
-// The part of one row that is sampled from: its threshold and normaliser (RowInfo), and px of token `draft`. Where
-// the candidates are few, the token drawn from the row too (d.mode >= 0; -1 where it was not). False in the
-// workgroups of a group that leave the row to another.
+// Starts on a row: the keys of its segments' maxima (sm: of this thread's), the row's maximum; what is counted later, 0.
 template <bool HALF>
-__device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, const Group& gr,
-                                           RowShared& sh, RowInfo& out, int& token) {
-  const int t = threadIdx.x, lane = t & 63;
-  const u16* x = row_ptr(a, seq, ri);
-  const int off = row_off(x);
-  const long row = (long)seq * a.per + ri;
-  const float sm = t < a.nseg ? a.segm[row * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
-  const double ss = !a.top_k && t < a.nseg ? a.segs[row * a.nseg + t] : 0;
-  const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
-  token = -1;
+__device__ __forceinline__ float row_start(const SampleArgs& a, float sm, RowState& sh) {
+  const int t = threadIdx.x;
   float mx = wave_max(sm);
-  if (lane == 0) sh.red_f[t >> 6] = mx;
+  if ((t & 63) == 0) sh.red_f[t >> 6] = mx;
   if (t < a.nseg) sh.skey[t] = key_of_float<HALF>(sm);
   if (t == 0) sh.ncand = sh.nlist = 0;
   if (t < 512) sh.cnt[t] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowWaves; ++i) mx = fmaxf(mx, sh.red_f[i]);
+  return mx;
+}
+
+// Of a row without any logit over -inf: nothing to draw from.
+__device__ __forceinline__ RowInfo empty_row(float mx) { return RowInfo{0.0, 0.0, mx, 1 << 16, kNoTies, 0}; }
+
+// A key that the top_k largest logits of a row reach (top: the largest): the k-th largest maximum of its segments, or
+// of their parts.
+template <bool HALF>
+__device__ __forceinline__ int top_k_bound(const SampleArgs& a, const u16* x, int off, float sm, int top, RowState& sh) {
+  const int t = threadIdx.x, lane = t & 63;
+  if (a.parts) {
+    for (int s = uniform(t >> 6); s < a.nseg; s += kRowWaves) {
+      const u32x4_t v = load8<HALF>(x, s * kSegVals + 8 * lane - off, a.V);
+      int ks[8], k = kLowKey<HALF>;
+      keys8(v, ks);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k = max(k, ks[j] <= top ? ks[j] : k);
+      k = max(k, dpp_i<0xB1, 0xF>(k));   // the exchanges of sum8_lanes
+      k = max(k, dpp_i<0x4E, 0xF>(k));
+      k = max(k, dpp_i<0x141, 0xF>(k));
+      if (a.parts == 4) k = max(k, dpp_i<0x140, 0xF>(k));
+      const int each = 64 / a.parts;
+      if ((lane & (each - 1)) == 0) sh.list[a.parts * s + lane / each] = k;
+    }
+    __syncthreads();
+    const int k = kth_key(t < a.parts * a.nseg, sh.list[t], a.top_k, sh.cnt);
+    __syncthreads();
+    return k;
+  }
+  return a.nseg >= a.top_k ? kth_key(t < a.nseg, key_of_float<HALF>(sm), a.top_k, sh.cnt) : kLowKey<HALF>;
+}
+
+// Logits that `take` (of a lane's keys: which of the 8) picks from the listed segments, into fw.cand as far as there is
+// room; how many (sh.ncand, 0 on entry).
+template <bool HALF, typename F>
+__device__ __forceinline__ int gather(const SampleArgs& a, const u16* x, int off, int nlist, RowState& sh, Few& fw, F&& take) {
+  const int lane = threadIdx.x & 63;
+  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
+    const int v0 = s * kSegVals + 8 * lane - off;
+    int ks[8];
+    keys8(v, ks);
+    const u32 on = take(s, ks);
+    const int n = __popc(on), upto = wave_scan(n);
+    int base = 0;
+    if (lane == 63) base = atomicAdd(&sh.ncand, upto);
+    int at = __builtin_amdgcn_readlane(base, 63) + upto - n;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (on >> j & 1) {
+        if (at < kListed) fw.cand[at] = (uint64_t)(u32)(ks[j] + (1 << 15)) << 32 | (u32)~(v0 + j);
+        ++at;
+      }
+    }
+  });
+  __syncthreads();
+  return sh.ncand;
+}
+
+// More candidates than are sorted: the top_k themselves. Their least key by counts of its bytes over the candidates, what
+// is above it, and the first by index of what equals it.
+template <bool HALF>
+__device__ __forceinline__ int gather_top(const SampleArgs& a, const u16* x, int off, int nlist, int kb, int top, RowState& sh,
+                                          Few& fw) {
+  const int t = threadIdx.x, lane = t & 63;
+  int k = a.top_k, high = 0, low = 0;
+  __syncthreads();
+  if (t < 512) sh.cnt[t] = 0;
+  if (t == 0) sh.ncand = 0;
+  __syncthreads();
+  for (int round = 0; round < 2; ++round) {
+    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) {
+      int ks[8];
+      keys8(v, ks);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int u = ks[j] + (1 << 15);
+        if (ks[j] >= kb && ks[j] <= top && (!round || u >> 8 == high))
+          atomicAdd(&sh.cnt[256 * round + 255 - (round ? u & 255 : u >> 8)], 1);
+      }
+    });
+    __syncthreads();
+    const int got = 255 - nth_bin(sh.cnt + 256 * round, k);
+    if (round == 0) high = got;
+    else low = got;
+  }
+  const int thr = (high << 8 | low) - (1 << 15);       // k of the logits that equal it
+  __syncthreads();
+  if (t < a.nseg) sh.cnt[t] = 0;
+  __syncthreads();
+  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
+    int n = 0, ks[8];
+    keys8(v, ks);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n += __popcll(__ballot(ks[j] == thr));
+    if (lane == 0) sh.cnt[s] = n;
+  });
+  __syncthreads();
+  int upto, all;
+  const int before = block_scan(t < a.nseg ? sh.cnt[t] : 0, sh.red_i, upto, all);
+  if (t < a.nseg) sh.cnt[t] = before;
+  __syncthreads();
+  return gather<HALF>(a, x, off, nlist, sh, fw, [&](int s, const int (&ks)[8]) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n += ks[j] == thr;
+    int rank = sh.cnt[s] + wave_scan(n) - n;
+    u32 on = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if ((ks[j] > thr && ks[j] <= top) || (ks[j] == thr && rank < k)) on |= 1u << j;
+      rank += ks[j] == thr;
+    }
+    return on;
+  });
+}
+
+// What is kept of the n candidates of fw.cand (total: the mass of the whole row, where there is no top_k), px of token
+// `draft`, and the token drawn (d.mode >= 0; else -1).
+template <bool HALF>
+__device__ __forceinline__ void sorted_row(const SampleArgs& a, int n, float mx, double total, int draft, float xd,
+                                           const DrawIn& d, RowState& sh, Few& fw, RowInfo& out, int& token) {
+  const int t = threadIdx.x;
+  const double mc = -(double)mx * a.c;
   out.m = mx;
-  out.px = 0;
   out.pad = 0;
-  if (!(mx > -INFINITY)) {              // nothing to draw from
-    out.z = 0;
-    out.thr = 1 << 16;
-    out.cut = kNoTies;
+  if (t < n) {
+    const uint64_t me = fw.cand[t];
+    int r = 0;
+    for (int i = 0; i < n; ++i) r += fw.cand[i] > me;
+    fw.sorted[r] = me;
+  }
+  __syncthreads();
+  const int idx = t < n ? (int)~(u32)fw.sorted[t] : 0;
+  const float qv = d.mode == kDrawRest && t < n ? d.q[idx] : 0.f;      // on its way over the next step
+  if (t < 64) {                     // the first wave, four a lane: what of the top_k lies before the mass
+    double w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = 4 * t + i;
+      w[i] = j < n && !(a.top_k && j >= a.top_k)
+                 ? weight(val_of_key<HALF>((int)(fw.sorted[j] >> 32) - (1 << 15)), mx, a.c, mc) : 0.0;
+      if (j < n) fw.w[j] = w[i];
+    }
+    double zk;
+    double run = scan4(w, zk);
+    const double goal = a.top_p * (a.top_k ? zk : total);
+    const int nk = a.top_k ? min(a.top_k, n) : n;
+    int kept = nk;                  // tokens of this lane or before it that are kept, if the cut is here
+    double z = zk;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {  // the first at which the goal is reached, from the lane's last
+      const double before = i == 0 ? run : i == 1 ? run + w[0] : i == 2 ? run + w[0] + w[1] : run + w[0] + w[1] + w[2];
+      if (4 * t + i < nk && before >= goal && a.top_p < 1.0) {
+        kept = 4 * t + i;
+        z = before;
+      }
+    }
+    const unsigned long long hit = __ballot(kept < nk);
+    if (hit) {
+      const int at = __ffsll(hit) - 1;
+      kept = __builtin_amdgcn_readlane(kept, at);
+      z = lane_value(z, at);
+    }
+    if (t == 0) {
+      sh.keep = kept;               // at least 1: before is 0 at the first, the goal is not
+      sh.z = z;
+      sh.key = (int)(fw.sorted[kept - 1] >> 32) - (1 << 15);
+      sh.cut = (int)~(u32)fw.sorted[kept - 1];
+    }
+  }
+  __syncthreads();
+  const int kept = sh.keep;
+  out.z = sh.z;
+  out.thr = sh.key;
+  out.cut = sh.cut;
+  out.px = px_of<HALF>(a, out, draft, xd);
+  token = -1;
+  if (d.mode < 0) return;
+  // the draw: r by index, then the first wave, four a lane
+  if (t < kept) {
+    int at = 0;
+    for (int i = 0; i < kept; ++i) at += (int)~(u32)fw.sorted[i] < idx;
+    double r = fw.w[t];
+    if (d.mode == kDrawRest) r = __builtin_fmax(r / out.z - (double)qv, 0.0);
+    else if (d.mode == kDrawOther && idx == d.skip) r = 0;
+    fw.r[at] = r;
+    fw.order[at] = t;
+  }
+  __syncthreads();
+  if (t < 64) {
+    double r[4], all = 0, run = 0;
+    for (int tries = 0; tries < 2; ++tries) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 4 * t + i;
+        r[i] = j < kept ? (tries ? fw.w[fw.order[j]] : fw.r[j]) : 0.0;      // r zero throughout: p
+      }
+      run = scan4(r, all);
+      if (all > 0) break;
+    }
+    const double goal = d.u * all;
+    int pick = kListed, last = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      run += r[i];
+      if (r[i] > 0) {
+        last = 4 * t + i;
+        if (run > goal && pick == kListed) pick = last;
+      }
+    }
+    const unsigned long long hit = __ballot(pick < kListed), any = __ballot(last >= 0);
+    // the last one with any mass where none passes the goal by a rounding
+    const int j = hit ? __builtin_amdgcn_readlane(pick, __ffsll(hit) - 1)
+                      : any ? __builtin_amdgcn_readlane(last, 63 - __clzll(any)) : -1;
+    if (t == 0) sh.token = j >= 0 ? (int)~(u32)fw.sorted[fw.order[j]] : 0;
+  }
+  __syncthreads();
+  token = sh.token;
+}
+
+// A row of a small top_k: what is kept of it, px of token `draft`, and the token drawn from it.
+template <bool HALF>
+__device__ __forceinline__ void cut_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, RowState& sh, Few& fw,
+                                        RowInfo& out, int& token) {
+  const int t = threadIdx.x;
+  const u16* x = row_ptr(a, seq, ri);
+  const int off = row_off(x);
+  const float sm = t < a.nseg ? a.segm[((long)seq * a.per + ri) * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
+  const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
+  const float mx = row_start<HALF>(a, sm, sh);
+  if (!(mx > -INFINITY)) {
+    out = empty_row(mx);
     token = 0;
+    return;
+  }
+  const int top = key_of_float<HALF>(mx);
+  const int kb = min(max(top_k_bound<HALF>(a, x, off, sm, top, sh), kLowKey<HALF> + 1), top);
+  const int nlist = list_segments(sh, 0, a.nseg, kb);
+  int n = gather<HALF>(a, x, off, nlist, sh, fw, [&](int, const int (&ks)[8]) {
+    u32 on = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) on |= (u32)(ks[j] >= kb && ks[j] <= top) << j;
+    return on;
+  });
+  if (n > kListed) n = gather_top<HALF>(a, x, off, nlist, kb, top, sh, fw);
+  sorted_row<HALF>(a, n, mx, 0.0, draft, xd, d, sh, fw, out, token);
+}
+
+// The part of one row that is sampled from: its threshold and normaliser (RowInfo), and px of token `draft`. False in
+// the workgroups of a group that leave the row to another.
+template <bool HALF>
+__device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri, int draft, const Group& gr, RowShared& sh,
+                                           RowInfo& out) {
+  const int t = threadIdx.x, lane = t & 63;
+  const u16* x = row_ptr(a, seq, ri);
+  const int off = row_off(x);
+  const long row = (long)seq * a.per + ri;
+  const float sm = t < a.nseg ? a.segm[row * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
+  const double ss = !a.top_k && t < a.nseg ? a.segs[row * a.nseg + t] : 0;
+  // of a group: this workgroup's run of segments, those of a wave kRowWaves apart, its first ones on their way
+  const int wave = uniform(t >> 6), spg = (a.nseg + gr.n - 1) / gr.n, s_end = min((gr.g + 1) * spg, a.nseg);
+  u32x4_t own[kOwn];
+  const auto load_own = [&](int s) {
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u)
+      if (s + u * kRowWaves < s_end) own[u] = load8<HALF>(x, (s + u * kRowWaves) * kSegVals + 8 * lane - off, a.V);
+  };
+  if (gr.counts) load_own(gr.g * spg + wave);
+  const float mx = row_start<HALF>(a, sm, sh);
+  if (!(mx > -INFINITY)) {
+    out = empty_row(mx);
     return gr.g == 0;
   }
+  out.m = mx;
+  out.pad = 0;
   const double mc = -(double)mx * a.c;
   double total = 0;                     // of the whole row; needed where the mass itself is cut
   if (!a.top_k) {
@@ -349,154 +623,50 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
     for (int i = 0; i < kRowWaves; ++i) total += sh.red_d[i];
   }
   const int top = key_of_float<HALF>(mx);
+  const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
 
   // a key that every kept token reaches
   int kb = kLowKey<HALF>;
   if (!a.top_k) {
-    // tokens of weight (1 - top_p) S / V or less: all together less than (1 - top_p) S. One key of room for the
-    // rounding to 16 bits.
-    const double w = (1.0 - a.top_p) * total / (double)a.V;
-    kb = key_of_float<HALF>((float)((double)mx + log2(w) / a.c)) - 1;
-  } else if (a.nseg >= a.top_k) {
-    kb = kth_key(t < a.nseg, key_of_float<HALF>(sm), a.top_k, sh.cnt);
-  } else if (8 * a.nseg >= a.top_k && a.nseg <= kMaxSegs / 8) {
-    // few segments: the maxima of groups of 8 lanes instead
-    for (int s = uniform(t >> 6); s < a.nseg; s += kRowWaves) {
-      const u32x4_t v = load8<HALF>(x, s * kSegVals + 8 * lane - off, a.V);
-      int ks[8], k = kLowKey<HALF>;
-      keys8(v, ks);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) k = max(k, ks[j] <= top ? ks[j] : k);
-      k = max(k, dpp_i<0xB1, 0xF>(k));   // the exchanges of sum8_lanes
-      k = max(k, dpp_i<0x4E, 0xF>(k));
-      k = max(k, dpp_i<0x141, 0xF>(k));
-      if ((lane & 7) == 0) sh.list[8 * s + (lane >> 3)] = k;
-    }
-    __syncthreads();
-    kb = kth_key(t < 8 * a.nseg, sh.list[t], a.top_k, sh.cnt);
-    __syncthreads();
+    // tokens of weight (1 - top_p) S / V or less: all together less than (1 - top_p) S. Room for an fp32 logarithm,
+    // and one key for the rounding to 16 bits.
+    const float w = (float)((1.0 - a.top_p) * total) / (float)a.V;
+    kb = key_of_float<HALF>(mx + (__builtin_amdgcn_logf(w) - 1e-4f) / (float)a.c) - 1;
+  } else {
+    kb = top_k_bound<HALF>(a, x, off, sm, top, sh);
   }
   kb = min(max(kb, kLowKey<HALF> + 1), top);
-  int nlist = list_segments(sh, 0, a.nseg, kb);
+  int nlist;
+  if (gr.counts) {                      // their number alone
+    const unsigned long long on = __ballot(t < a.nseg && sh.skey[t] >= kb);
+    if (lane == 0 && on) atomicAdd(&sh.nlist, __popcll(on));
+    __syncthreads();
+    nlist = sh.nlist;
+  } else {
+    nlist = list_segments(sh, 0, a.nseg, kb);
+  }
 
   // Few candidates are sorted. A top_k leaves little more than that many; a mass alone may leave most of a segment,
   // so that only rows where few segments reach are tried.
   const bool few = nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves);
-  if (few && gr.g) return false;        // the first workgroup's alone
-  if (few) {
-    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
-      const int v0 = s * kSegVals + 8 * lane - off;
-      int n = 0, ks[8];
-      keys8(v, ks);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n += ks[j] >= kb && ks[j] <= top;
-      const int upto = wave_scan(n);
-      int base = 0;
-      if (lane == 63) base = atomicAdd(&sh.ncand, upto);
-      int at = __builtin_amdgcn_readlane(base, 63) + upto - n;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (ks[j] >= kb && ks[j] <= top) {
-          if (at < kListed) sh.cand[at] = (uint64_t)(u32)(ks[j] + (1 << 15)) << 32 | (u32)~(v0 + j);
-          ++at;
-        }
-      }
-    });
+  const bool grouped = gr.counts && !few && top - kb < kBins;
+  if (gr.counts && !grouped) {          // few, or too many values for one pass: the first workgroup's alone
+    if (gr.g) return false;
     __syncthreads();
-    const int n = sh.ncand;
+    if (t == 0) sh.nlist = 0;
+    __syncthreads();
+    list_segments(sh, 0, a.nseg, kb);
+  }
+  if (few) {
+    const int n = gather<HALF>(a, x, off, nlist, sh, sh.few, [&](int, const int (&ks)[8]) {
+      u32 on = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) on |= (u32)(ks[j] >= kb && ks[j] <= top) << j;
+      return on;
+    });
     if (n <= kListed) {
-      if (t < n) {
-        const uint64_t me = sh.cand[t];
-        int r = 0;
-        for (int i = 0; i < n; ++i) r += sh.cand[i] > me;
-        sh.sorted[r] = me;
-      }
-      __syncthreads();
-      const int idx = t < n ? (int)~(u32)sh.sorted[t] : 0;
-      const float qv = d.mode == kDrawRest && t < n ? d.q[idx] : 0.f;      // on its way over the next step
-      if (t < 64) {                     // the first wave, four a lane: what of the top_k lies before the mass
-        double w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = 4 * t + i;
-          w[i] = j < n && !(a.top_k && j >= a.top_k)
-                     ? weight(val_of_key<HALF>((int)(sh.sorted[j] >> 32) - (1 << 15)), mx, a.c, mc) : 0.0;
-          if (j < n) sh.w[j] = w[i];
-        }
-        double zk;
-        double run = scan4(w, zk);
-        const double goal = a.top_p * (a.top_k ? zk : total);
-        const int nk = a.top_k ? min(a.top_k, n) : n;
-        int kept = nk;                  // tokens of this lane or before it that are kept, if the cut is here
-        double z = zk;
-#pragma unroll
-        for (int i = 3; i >= 0; --i) {  // the first at which the goal is reached, from the lane's last
-          const double before = i == 0 ? run : i == 1 ? run + w[0] : i == 2 ? run + w[0] + w[1] : run + w[0] + w[1] + w[2];
-          if (4 * t + i < nk && before >= goal && a.top_p < 1.0) {
-            kept = 4 * t + i;
-            z = before;
-          }
-        }
-        const unsigned long long hit = __ballot(kept < nk);
-        if (hit) {
-          const int at = __ffsll(hit) - 1;
-          kept = __builtin_amdgcn_readlane(kept, at);
-          z = lane_value(z, at);
-        }
-        if (t == 0) {
-          sh.keep = kept;               // at least 1: before is 0 at the first, the goal is not
-          sh.z = z;
-          sh.key = (int)(sh.sorted[kept - 1] >> 32) - (1 << 15);
-          sh.cut = (int)~(u32)sh.sorted[kept - 1];
-        }
-      }
-      __syncthreads();
-      const int kept = sh.keep;
-      out.z = sh.z;
-      out.thr = sh.key;
-      out.cut = sh.cut;
-      out.px = px_of<HALF>(a, out, draft, xd);
-      if (d.mode < 0) return true;
-      // the draw: r by index, then the first wave, four a lane
-      if (t < kept) {
-        int at = 0;
-        for (int i = 0; i < kept; ++i) at += (int)~(u32)sh.sorted[i] < idx;
-        double r = sh.w[t];
-        if (d.mode == kDrawRest) r = __builtin_fmax(r / out.z - (double)qv, 0.0);
-        else if (d.mode == kDrawOther && idx == d.skip) r = 0;
-        sh.r[at] = r;
-        sh.order[at] = t;
-      }
-      __syncthreads();
-      if (t < 64) {
-        double r[4], all = 0, run = 0;
-        for (int tries = 0; tries < 2; ++tries) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = 4 * t + i;
-            r[i] = j < kept ? (tries ? sh.w[sh.order[j]] : sh.r[j]) : 0.0;      // r zero throughout: p
-          }
-          run = scan4(r, all);
-          if (all > 0) break;
-        }
-        const double goal = d.u * all;
-        int pick = kListed, last = -1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          run += r[i];
-          if (r[i] > 0) {
-            last = 4 * t + i;
-            if (run > goal && pick == kListed) pick = last;
-          }
-        }
-        const unsigned long long hit = __ballot(pick < kListed), any = __ballot(last >= 0);
-        // the last one with any mass where none passes the goal by a rounding
-        const int j = hit ? __builtin_amdgcn_readlane(pick, __ffsll(hit) - 1)
-                          : any ? __builtin_amdgcn_readlane(last, 63 - __clzll(any)) : -1;
-        if (t == 0) sh.token = j >= 0 ? (int)~(u32)sh.sorted[sh.order[j]] : 0;
-      }
-      __syncthreads();
-      token = sh.token;
+      int token;
+      sorted_row<HALF>(a, n, mx, total, draft, xd, DrawIn{-1, -1, nullptr, 0.0}, sh, sh.few, out, token);
       return true;
     }
     __syncthreads();
@@ -505,16 +675,19 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
   int thr = kb - 1, keep = 0, ties = 0;  // thr = kb - 1: every listed token
   int range_hi = -(1 << 17), range_lo = 0;             // the keys now in the bins, bin range_hi - key
   int merged = top + 1;                  // of a group's counts: from this key up
-  const int spg = (a.nseg + gr.n - 1) / gr.n;         // segments of a workgroup of the group
   const int words = (top - kb + 4) >> 2;
-  const bool grouped = gr.counts && !few && top - kb < kBins;
-  if (gr.counts && !few && !grouped && gr.g) return false;       // too many values for one pass: the first's alone
   if (grouped) {
+    for (int i = t; i <= top - kb; i += kRowThreads) sh.bins[i] = 0;
     __syncthreads();
-    if (t == 0) sh.nlist = 0;
+    for (int s = gr.g * spg + wave; s < s_end; s += kOwn * kRowWaves) {
+      if (s >= gr.g * spg + kOwn * kRowWaves) load_own(s);
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) {
+        const int at = s + u * kRowWaves;
+        if (at < s_end && uniform(sh.skey[at]) >= kb) count_seg<HALF>(own[u], sh, top, kb);
+      }
+    }
     __syncthreads();
-    const int mine = list_segments(sh, gr.g * spg, min((gr.g + 1) * spg, a.nseg), kb);
-    count_keys<HALF>(a, x, off, sh, mine, top, kb);
     uint64_t* out_c = gr.counts + (long)gr.g * (kBins / 4);
     for (int i = t; i < words; i += kRowThreads) {    // a value at most as often as spg segments have logits: below 2^16
       uint64_t w = 0;
@@ -583,27 +756,35 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
           if (b + 1 < b1) f.next(mx, a.c, mc);
         }
       }
-      if (t == 0) sh.owner = kRowThreads;
-      int cnt_all, cnt_end;
-      double mass_all, mass_end;
-      const int cnt_before = block_scan(cn, sh.red_i, cnt_end, cnt_all);
-      const double mass_before = block_scan(cm, sh.red_d, mass_end, mass_all);
-      // the thread whose bins the goal falls into (the first: running sums may step back by a rounding)
-      const bool mine = pass == 0 ? seen + cnt_end >= a.top_k && cn : mass + mass_end >= goal && cn;
-      const unsigned long long reached = __ballot(mine);
-      if (lane == 0 && reached) atomicMin(&sh.owner, t + __ffsll(reached) - 1);
+      // running sums over the waves, a wave a lane, and the first wave with tokens in which the goal is reached
+      const double m_in = wave_scan(cm);
+      const int c_in = wave_scan(cn);
+      if (lane == 63) {
+        sh.red_d[wave] = m_in;
+        sh.red_i[wave] = c_in;
+      }
       __syncthreads();
-      const int owner = sh.owner;
-      if (owner < kRowThreads && (t >> 6) == (owner >> 6)) {     // its wave, a bin a lane
-        const int run_c = __builtin_amdgcn_readlane(seen + cnt_before, owner & 63);
-        const double run_m = lane_value(mass + mass_before, owner & 63);
-        const int b = owner * each + lane;
+      const double m_w = lane < kRowWaves ? sh.red_d[lane] : 0.0, m_to = wave_scan(m_w);
+      const int c_w = lane < kRowWaves ? sh.red_i[lane] : 0, c_to = wave_scan(c_w);
+      const unsigned long long there = __ballot(c_w && (pass == 0 ? seen + c_to >= a.top_k : mass + m_to >= goal));
+      const int owner = there ? __ffsll(there) - 1 : kRowWaves;
+      const double mass_before = mass + lane_value(lane_before(m_to), wave);
+      const int cnt_before = seen + __builtin_amdgcn_readlane(c_to - c_w, wave);
+      mass += lane_value(m_to, 63);
+      seen += __builtin_amdgcn_readlane(c_to, 63);
+      if (wave == owner) {              // its lane's bins, a bin a lane
+        const unsigned long long reached = __ballot(cn && (pass == 0 ? cnt_before + c_in >= a.top_k : mass_before + m_in >= goal));
+        const unsigned long long some = __ballot(cn > 0);
+        const int from = reached ? __ffsll(reached) - 1 : 63 - __clzll(some);
+        const int run_c = __builtin_amdgcn_readlane(cnt_before + lane_before(c_in), from);
+        const double run_m = lane_value(mass_before + lane_before(m_in), from);
+        const int b = (64 * wave + from) * each + lane;
         const bool in = lane < each && b < nb;
         const int n_all = in ? sh.bins[base + b] : 0;
         const int n = after_k && hi - b == thr_k && in ? keep_k : n_all;
         const double w = in ? weight(val_of_key<HALF>(hi - b), mx, a.c, mc) : 0.0;
         const int c_end = run_c + wave_scan(n), c0 = c_end - n;
-        const double m_in = wave_scan((double)n * w), m0 = run_m + lane_before(m_in), m_end = run_m + m_in;
+        const double mb = wave_scan((double)n * w), m0 = run_m + lane_before(mb), m_end = run_m + mb;
         const bool reach = n && (pass == 0 ? c_end >= a.top_k : m_end >= goal);
         const unsigned long long hit = __ballot(reach), any = __ballot(n > 0);
         const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(any);       // the last of the run but for a rounding
@@ -622,9 +803,7 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
         }
       }
       __syncthreads();
-      seen += cnt_all;
-      mass += mass_all;
-      found = owner < kRowThreads;
+      found = owner < kRowWaves;
       if (found) {
         thr = sh.key;
         keep = sh.keep;
@@ -644,39 +823,8 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
   out.z = z;
   out.cut = ties ? a.V : kNoTies;       // without a threshold value (thr = kb - 1) no token has that key
   if (keep < ties) {                    // the index of the last kept token of the threshold's value
-    if (t == 0) sh.nlist = 0;
-    if (t < a.nseg) sh.cnt[t] = 0;
-    int s0 = 0, s1 = a.nseg;
-    if (grouped) {                      // the run of segments it lies in, by the groups' own counts
-      const int b = top - thr;
-      const int c = lane < gr.n ? (int)(get_far(gr.counts + (long)lane * (kBins / 4) + (b >> 2)) >> (16 * (b & 3)) & 0xFFFF) : 0;
-      const int upto = wave_scan(c);
-      const int at = __ffsll(__ballot(upto >= keep)) - 1;
-      keep -= __builtin_amdgcn_readlane(upto - c, at);
-      s0 = at * spg;
-      s1 = min(s0 + spg, a.nseg);
-    }
-    __syncthreads();
-    nlist = list_segments(sh, s0, s1, thr);
-    each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
-      int n = 0, ks[8];
-      keys8(v, ks);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n += __popcll(__ballot(ks[j] == thr));
-      if (lane == 0) sh.cnt[s] = n;
-    });
-    __syncthreads();
-    const int c = t < a.nseg ? sh.cnt[t] : 0;
-    int upto, all;
-    const int before = block_scan(c, sh.red_i, upto, all);
-    if (before < keep && keep <= upto) {
-      sh.owner = t;
-      sh.keep = keep - before;
-    }
-    __syncthreads();
-    if (t < 64) {
-      const int v0 = sh.owner * kSegVals + 8 * lane - off, want = sh.keep;
-      const u32x4_t v = load8<HALF>(x, v0, a.V);
+    // the keep-th logit of the threshold's value among a lane's 8 from index v0, by one wave
+    const auto place = [&](const u32x4_t& v, int v0, int want) {
       int n = 0, ks[8];
       keys8(v, ks);
 #pragma unroll
@@ -685,8 +833,77 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (ks[j] == thr && ++run == want) sh.cut = v0 + j;
+    };
+    const auto count = [&](const u32x4_t& v) {
+      int n = 0, ks[8];
+      keys8(v, ks);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n += __popcll(__ballot(ks[j] == thr));
+      return n;
+    };
+    if (grouped) {                      // the run of segments it lies in, by the groups' own counts
+      const int b = top - thr;
+      const int c = lane < gr.n ? (int)(get_far(gr.counts + (long)lane * (kBins / 4) + (b >> 2)) >> (16 * (b & 3)) & 0xFFFF) : 0;
+      const int upto = wave_scan(c), at = __ffsll(__ballot(upto >= keep)) - 1;
+      keep -= __builtin_amdgcn_readlane(upto - c, at);
+      const int s0 = at * spg, s1 = min(s0 + spg, a.nseg);
+      for (int s = s0 + wave; s < s1; s += kOwn * kRowWaves) {
+#pragma unroll
+        for (int u = 0; u < kOwn; ++u)
+          if (s + u * kRowWaves < s1) own[u] = load8<HALF>(x, (s + u * kRowWaves) * kSegVals + 8 * lane - off, a.V);
+#pragma unroll
+        for (int u = 0; u < kOwn; ++u) {
+          if (s + u * kRowWaves >= s1) break;
+          const int n = count(own[u]);
+          if (lane == 0) sh.cnt[s + u * kRowWaves - s0] = n;
+        }
+      }
+      __syncthreads();
+      int first = 0;                    // the segment, by every wave for itself
+      for (int i = 0; i < s1 - s0; i += 64) {
+        const int n = i + lane < s1 - s0 ? sh.cnt[i + lane] : 0, end = wave_scan(n);
+        const unsigned long long hit = __ballot(end >= keep);
+        if (hit) {
+          const int l = __ffsll(hit) - 1;
+          first = i + l;
+          keep -= __builtin_amdgcn_readlane(end - n, l);
+          break;
+        }
+        keep -= __builtin_amdgcn_readlane(end, 63);
+      }
+      if ((first & (kRowWaves - 1)) == wave) {
+        const int v0 = (s0 + first) * kSegVals + 8 * lane - off;
+        static_assert(kOwn == 2, "own[0], own[1]");
+        u32x4_t v = own[0];
+        if (s1 - s0 > kOwn * kRowWaves) v = load8<HALF>(x, v0, a.V);
+        else if (first >= kRowWaves) v = own[1];
+        place(v, v0, keep);
+      }
+      __syncthreads();
+    } else {
+      if (t == 0) sh.nlist = 0;
+      if (t < a.nseg) sh.cnt[t] = 0;
+      __syncthreads();
+      nlist = list_segments(sh, 0, a.nseg, thr);
+      each_listed<HALF>(a, x, off, sh.list, nlist, [&](int s, const u32x4_t& v) {
+        const int n = count(v);
+        if (lane == 0) sh.cnt[s] = n;
+      });
+      __syncthreads();
+      const int c = t < a.nseg ? sh.cnt[t] : 0;
+      int upto, all;
+      const int before = block_scan(c, sh.red_i, upto, all);
+      if (before < keep && keep <= upto) {
+        sh.owner = t;
+        sh.keep = keep - before;
+      }
+      __syncthreads();
+      if (t < 64) {
+        const int v0 = sh.owner * kSegVals + 8 * lane - off;
+        place(load8<HALF>(x, v0, a.V), v0, sh.keep);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     out.cut = sh.cut;
   }
   out.px = px_of<HALF>(a, out, draft, xd);
@@ -879,17 +1096,15 @@ __device__ __forceinline__ void write_tokens(const SampleArgs& a, const VerifyIn
   if (threadIdx.x == 0) in.n[seq] = n;
 }
 
-struct CutShared {
-  RowShared row;
-  DrawShared draw;
+struct CutShared : RowState {
+  Few few;
+  int first;
 };
 
-// Rows of few candidates, as a small top_k leaves them: one row a workgroup. It draws its token too, in case its draft
-// is the first refused (the random number of the draw is there from the start); the last workgroup of a sequence
-// accepts, and draws from the row it comes to where that row's candidates were many after all.
+// Rows of a small top_k: one row a workgroup. It draws its token too, in case its draft is the first refused (the random
+// number of the draw is there from the start); the last workgroup of a sequence accepts.
 template <bool HALF>
-__global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
-                                                                 uint64_t* drawn) {
+__global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArgs a, const VerifyIn in, uint64_t* drawn) {
   __shared__ CutShared sh;
   const int ri = blockIdx.x, seq = blockIdx.y, m = a.per - 1, t = threadIdx.x;
   const long row = (long)seq * a.per + ri;
@@ -901,39 +1116,24 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
   if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
   int token;
   RowInfo mine;
-  select_row<HALF>(a, seq, ri, draft, d, Group{nullptr, nullptr, 0, 1}, sh.row, mine, token);
-  static_assert(sizeof(RowInfo) == 32, "four words");
-  if (t < 4 && token < 0) {
-    uint64_t w[4];
-    __builtin_memcpy(w, &mine, 32);
-    put_far(info + 4 * row + t, t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3]);
-  }
+  cut_row<HALF>(a, seq, ri, draft, d, sh, sh.few, mine, token);
   if (t == 0) {
     if (ri < m) in.px[(long)seq * m + ri] = (float)mine.px;
     put_far(drawn + row, (uint64_t)(ri >= len || !(uq < mine.px)) << 32 | (u32)token);
   }
-  if (!arrives_last(a.arrived + seq, a.per, &sh.row.last)) return;
-  if (t == 0) sh.draw.first = len;
+  if (!arrives_last(a.arrived + seq, a.per, &sh.last)) return;
+  if (t == 0) sh.first = len;
   __syncthreads();
   uint64_t res = 0;
   if (t <= len) {                       // kMaxDraft < kRowThreads
     res = get_far(drawn + (long)seq * a.per + t);
-    if (res >> 32) atomicMin(&sh.draw.first, t);
+    if (res >> 32) atomicMin(&sh.first, t);
   }
   __syncthreads();
-  const int n = sh.draw.first;
-  if (t == n) sh.row.token = (int)(u32)res;
+  const int n = sh.first;
+  if (t == n) sh.token = (int)(u32)res;
   __syncthreads();
-  token = sh.row.token;
-  if (token < 0) {
-    uint64_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = get_far(info + 4 * ((long)seq * a.per + n) + i);
-    RowInfo r;
-    __builtin_memcpy(&r, w, 32);
-    token = draw_token<HALF, true>(a, r, seq, n, draw_in(a, in, seq, n, len), nullptr, sh.draw);
-  }
-  write_tokens(a, in, seq, n, token);
+  write_tokens(a, in, seq, n, sh.token);
 }
 
 // What is kept of a row, for a launch behind this one: by a group of workgroups where the rows are few (gridDim.x).
@@ -946,9 +1146,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const Sample
   const int draft = in.draft && ri < m ? in.draft[(long)seq * m + ri] : -1;
   const Group gr = {gridDim.x > 1 ? counts + row * gridDim.x * (kBins / 4) : nullptr, arrived + row, (int)blockIdx.x,
                     (int)gridDim.x};
-  int token;
   RowInfo mine;
-  if (!select_row<HALF>(a, seq, ri, draft, DrawIn{-1, -1, nullptr, 0.0}, gr, sh, mine, token)) return;
+  if (!select_row<HALF>(a, seq, ri, draft, gr, sh, mine)) return;
   if (threadIdx.x < 4) {
     uint64_t w[4];
     __builtin_memcpy(w, &mine, 32);
@@ -1135,6 +1334,16 @@ constexpr int64_t kMaxVocab = (int64_t)kMaxSegs * kSegVals - 8;
 
 bool shape_ok(int64_t rows, int64_t V) { return rows >= 1 && rows <= 65535 && V >= 1 && V <= kMaxVocab; }
 
+// Parts a segment that a top_k's bound goes by, 0 for whole segments. The k-th largest of n maxima is reached by
+// n ln(n / (n - k)) logits or so; where that is near what can be sorted, and where there are fewer segments than k, the
+// maxima of parts, at another pass over the row (24 rows of 70000, top 128: 24.4 us, 46.9 by whole segments).
+int bound_parts(int nseg, int top_k) {
+  if (!top_k) return 0;
+  const int parts = nseg <= kMaxSegs / 8 ? 8 : nseg <= kMaxSegs / 4 ? 4 : 0;
+  if (nseg < top_k) return parts * nseg >= top_k ? parts : 0;
+  return top_k <= kListed / 2 && nseg * std::log(nseg / (nseg - top_k + 0.5)) > 0.7 * kListed ? parts : 0;
+}
+
 int sample_args(const char* what, int64_t dtype, const void* logits, int64_t rows, int64_t V, double temperature, int64_t top_k,
                 double top_p, void* ws, int64_t ws_bytes, const Layout& l, SampleArgs& a) {
   if (!logits || !ws) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
@@ -1151,6 +1360,7 @@ int sample_args(const char* what, int64_t dtype, const void* logits, int64_t row
   a.c = 1.4426950408889634 / temperature;
   a.top_p = top_p;
   a.top_k = top_k < V ? (int)top_k : 0;
+  a.parts = bound_parts(a.nseg, a.top_k);
   a.segm = reinterpret_cast<float*>(w + l.segm);
   a.segs = reinterpret_cast<double*>(w + l.segs);
   return DSPARK_OK;
@@ -1215,7 +1425,7 @@ void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, h
     launch_select<HALF>(a, in, w, l, s);
     hipLaunchKernelGGL((sample_spread_kernel<HALF, true>), dim3(spread, B), dim3(kRowThreads), 0, s, a, in, info, rest);
   } else if (cut) {
-    hipLaunchKernelGGL((sample_cut_kernel<HALF>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in, info,
+    hipLaunchKernelGGL((sample_cut_kernel<HALF>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in,
                        reinterpret_cast<uint64_t*>(w + l.drawn));
   } else {
     hipLaunchKernelGGL((sample_spread_kernel<HALF, false>), dim3(in.q ? spread : 1, B), dim3(kRowThreads), 0, s, a, in, info,

@@ -343,3 +343,36 @@ def test_the_same_bits_each_time(dev, kw):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert torch.equal(ops.sampling_probs(args[0], **kw), probs)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("top_p", [1.0, 0.85])
+@pytest.mark.parametrize("top_k", [1, 31, 64, 65, 128, 129])
+@pytest.mark.parametrize("V,dtype", [(600, "bf16"), (40961, "f16"), (70001, "bf16"), (140000, "bf16")])
+def test_tied_candidates(dev, V, dtype, top_k, top_p):
+    """Rows of which more tokens tie for the top_k than are looked at one by one, and rows without ties whose
+    candidates are about as many: the first by index count, over every segment."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(V + top_k)
+    B, m = 4, 2
+    x = rows(g, B * (m + 1), V, DT[dtype])
+    x[0] = 1.5                                           # nothing but ties
+    x[1] = torch.round(x[1].float() / 4).to(x.dtype) * 4     # thousands at each value
+    x[2, torch.randperm(V, generator=g)[:400]] = 20.0    # more than are sorted, spread, above the others
+    x[3, V - 300:] = 9.5                                 # in the last segments
+    x[4, :70] = 30.0                                     # some above a tie
+    x[4, 70:] = torch.where(torch.rand(V - 70, generator=g) < 0.5, -2.0, -3.0).to(x.dtype)
+    x[5] = float("-inf")
+    x[5, ::2] = float("nan")
+    x[5, 100:400] = -1.0
+    x = x.reshape(B, m + 1, V)
+    d, q = _drafts(g, x, "odd", m)
+    u = torch.rand(B, m + 1, generator=g, dtype=torch.float64)
+    for qq in (None, q):
+        got = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=None if qq is None else qq.to(dev),
+                                     top_k=top_k, top_p=top_p)
+        want = ref.verify(_np(x), d.numpy(), u.numpy(), None if qq is None else qq.numpy(), top_k=top_k, top_p=top_p)
+        assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1])
+        close(got[2], want[2])
+    flat = x.reshape(-1, V)[:6]
+    close(ops.sampling_probs(flat.to(dev), top_k=top_k, top_p=top_p), np.stack([ref.probs(r, top_k=top_k, top_p=top_p) for r in _np(flat)]))
