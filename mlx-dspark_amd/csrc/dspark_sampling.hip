@@ -249,25 +249,25 @@ __device__ __forceinline__ void each_listed(const SampleArgs& a, const u16* x, i
   }
 }
 
-// Counts 8 logits of a lane by key, bin hi - key for lo <= key <= hi.
-template <bool HALF>
-__device__ __forceinline__ void count_seg(const u32x4_t& v, RowShared& sh, int hi, int lo) {
+// Counts 8 logits of a lane by key, bin hi - key for lo <= key <= hi; PAIRS: two bins of 16 bits an int.
+template <bool HALF, bool PAIRS>
+__device__ __forceinline__ void count_seg(const u32x4_t& v, int* bins, int hi, int lo) {
   int k[8];
   keys8(v, k);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const u32 b = (u32)(hi - k[j]);
-    if (b <= (u32)(hi - lo)) atomicAdd(&sh.bins[b], 1);
+    if (b <= (u32)(hi - lo)) atomicAdd(&bins[PAIRS ? b >> 1 : b], PAIRS ? 1 << (16 * (b & 1)) : 1);
   }
 }
 
-// The same of the listed segments.
+// All logits of the listed segments.
 template <bool HALF>
 __device__ __forceinline__ void count_keys(const SampleArgs& a, const u16* x, int off, RowShared& sh, int nlist, int hi,
                                            int lo) {
   for (int i = threadIdx.x; i <= hi - lo; i += kRowThreads) sh.bins[i] = 0;
   __syncthreads();
-  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) { count_seg<HALF>(v, sh, hi, lo); });
+  each_listed<HALF>(a, x, off, sh.list, nlist, [&](int, const u32x4_t& v) { count_seg<HALF, false>(v, sh.bins, hi, lo); });
   __syncthreads();
 }
 
@@ -318,6 +318,7 @@ struct DrawIn {                        // what a row's own draw goes by
 };
 
 constexpr int kGroup = 16;             // most workgroups that count a row together
+constexpr int kGroupBins = 2 * kBins;  // values that they count: 16-bit counts
 constexpr int kOwn = 2;                // segments of a wave whose loads are out together
 struct Group {                         // a row counted by several workgroups, each over its own run of segments
   uint64_t* counts;                    // of each workgroup, 4 bins of 16 bits a word; null: one workgroup a row
@@ -649,15 +650,16 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
   // Few candidates are sorted. A top_k leaves little more than that many; a mass alone may leave most of a segment,
   // so that only rows where few segments reach are tried.
   const bool few = nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves);
-  const bool grouped = gr.counts && !few && top - kb < kBins;
-  if (gr.counts && !grouped) {          // few, or too many values for one pass: the first workgroup's alone
-    if (gr.g) return false;
+  const bool grouped = gr.counts && !few;
+  const auto list_all = [&]() {
     __syncthreads();
     if (t == 0) sh.nlist = 0;
     __syncthreads();
-    list_segments(sh, 0, a.nseg, kb);
-  }
+    nlist = list_segments(sh, 0, a.nseg, kb);
+  };
   if (few) {
+    if (gr.g) return false;             // the first workgroup's alone
+    if (gr.counts) list_all();
     const int n = gather<HALF>(a, x, off, nlist, sh, sh.few, [&](int, const int (&ks)[8]) {
       u32 on = 0;
 #pragma unroll
@@ -674,31 +676,27 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
 
   int thr = kb - 1, keep = 0, ties = 0;  // thr = kb - 1: every listed token
   int range_hi = -(1 << 17), range_lo = 0;             // the keys now in the bins, bin range_hi - key
-  int merged = top + 1;                  // of a group's counts: from this key up
-  const int words = (top - kb + 4) >> 2;
+  int merged_hi = -(1 << 17), merged_lo = 0;           // of a group's counts: joined in the bins, bin merged_hi - key
+  const int group_lo = max(kb, top - kGroupBins + 1);  // a group counts this far; what is below, its last workgroup alone
+  const int words = (top - group_lo + 4) >> 2;
   if (grouped) {
-    for (int i = t; i <= top - kb; i += kRowThreads) sh.bins[i] = 0;
+    // a value at most as often as spg segments have logits: below 2^16
+    for (int i = t; i < 2 * words; i += kRowThreads) sh.bins[i] = 0;
     __syncthreads();
     for (int s = gr.g * spg + wave; s < s_end; s += kOwn * kRowWaves) {
       if (s >= gr.g * spg + kOwn * kRowWaves) load_own(s);
 #pragma unroll
       for (int u = 0; u < kOwn; ++u) {
         const int at = s + u * kRowWaves;
-        if (at < s_end && uniform(sh.skey[at]) >= kb) count_seg<HALF>(own[u], sh, top, kb);
+        if (at < s_end && uniform(sh.skey[at]) >= kb) count_seg<HALF, true>(own[u], sh.bins, top, group_lo);
       }
     }
     __syncthreads();
-    uint64_t* out_c = gr.counts + (long)gr.g * (kBins / 4);
-    for (int i = t; i < words; i += kRowThreads) {    // a value at most as often as spg segments have logits: below 2^16
-      uint64_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w |= (uint64_t)(4 * i + j <= top - kb ? sh.bins[4 * i + j] : 0) << (16 * j);
-      put_far(out_c + i, w);
-    }
+    uint64_t* out_c = gr.counts + (long)gr.g * (kGroupBins / 4);
+    for (int i = t; i < words; i += kRowThreads) put_far(out_c + i, (uint64_t)(u32)sh.bins[2 * i] | (uint64_t)(u32)sh.bins[2 * i + 1] << 32);
     if (!arrives_last(gr.arrived, gr.n, &sh.last)) return false;
-    range_hi = top;
-    range_lo = kb;
   }
+  bool exchanged = grouped;              // the counts are a group's
   double z = 0;
   bool found = false;
   // two passes over the values in falling order: the top_k-th token, then the mass top_p
@@ -715,33 +713,46 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
     double mass = 0;
     found = false;
     for (int hi = top, lo; hi >= lowest && !found; hi = lo - 1) {
-      if (hi > range_hi || hi < range_lo) {
-        range_hi = hi;
-        range_lo = max(kb, hi - kBins + 1);
-        count_keys<HALF>(a, x, off, sh, nlist, range_hi, range_lo);
+      // a few thousand values first: the goal is mostly there
+      lo = max(lowest, hi - (hi == top ? kChunk : kBins - 4) + 1);
+      if (exchanged && hi < group_lo) {
+        list_all();
+        exchanged = false;
       }
-      // a few thousand values at a time: the goal is mostly in the first
-      lo = max(max(lowest, range_lo), hi - kChunk + 1);
-      if (grouped && lo < merged) {
-        for (int i = ((top - merged + 1) >> 2) + t; i <= (top - lo) >> 2; i += kRowThreads) {
-          int c[4] = {};
-          uint64_t w[kGroup];            // every workgroup's word at once
+      int base;                          // the bin of hi
+      if (exchanged) {
+        lo = max(lo, group_lo);
+        if (merged_hi != hi || merged_lo > lo) {
+          const int w0 = (top - hi) >> 2;
+          for (int i = w0 + t; i <= (top - lo) >> 2; i += kRowThreads) {
+            int c[4] = {};
+            uint64_t w[kGroup];          // every workgroup's word at once
 #pragma unroll
-          for (int g = 0; g < kGroup; ++g) w[g] = g < gr.n ? get_far(gr.counts + (long)g * (kBins / 4) + i) : 0;
+            for (int g = 0; g < kGroup; ++g) w[g] = g < gr.n ? get_far(gr.counts + (long)g * (kGroupBins / 4) + i) : 0;
 #pragma unroll
-          for (int g = 0; g < kGroup; ++g)
+            for (int g = 0; g < kGroup; ++g)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] += (int)(w[g] >> (16 * j) & 0xFFFF);
+              for (int j = 0; j < 4; ++j) c[j] += (int)(w[g] >> (16 * j) & 0xFFFF);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sh.bins[4 * i + j] = c[j];
+            for (int j = 0; j < 4; ++j) sh.bins[4 * (i - w0) + j] = c[j];
+          }
+          merged_hi = hi;
+          merged_lo = lo;
+          __syncthreads();
         }
-        merged = lo;
-        __syncthreads();
+        base = (top - hi) & 3;
+      } else {
+        if (hi > range_hi || hi < range_lo) {
+          range_hi = hi;
+          range_lo = max(kb, hi - kBins + 1);
+          count_keys<HALF>(a, x, off, sh, nlist, range_hi, range_lo);
+        }
+        lo = max(lo, range_lo);
+        base = range_hi - hi;
       }
-      const int base = range_hi - hi;    // the bin of hi
       // a run of bins a thread, an odd number of them: neighbours read other banks
       const int nb = hi - lo + 1, each = ((nb + kRowThreads - 1) / kRowThreads) | 1;
-      static_assert(kChunk / kRowThreads < 64, "a lane for every bin of a run");
+      static_assert(kBins / kRowThreads < 64, "a lane for every bin of a run");
       const int b0 = min(t * each, nb), b1 = min(b0 + each, nb);
       int cn = 0;
       double cm = 0;
@@ -841,9 +852,9 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
       for (int j = 0; j < 8; ++j) n += __popcll(__ballot(ks[j] == thr));
       return n;
     };
-    if (grouped) {                      // the run of segments it lies in, by the groups' own counts
+    if (grouped && thr >= group_lo) {   // the run of segments it lies in, by the groups' own counts
       const int b = top - thr;
-      const int c = lane < gr.n ? (int)(get_far(gr.counts + (long)lane * (kBins / 4) + (b >> 2)) >> (16 * (b & 3)) & 0xFFFF) : 0;
+      const int c = lane < gr.n ? (int)(get_far(gr.counts + (long)lane * (kGroupBins / 4) + (b >> 2)) >> (16 * (b & 3)) & 0xFFFF) : 0;
       const int upto = wave_scan(c), at = __ffsll(__ballot(upto >= keep)) - 1;
       keep -= __builtin_amdgcn_readlane(upto - c, at);
       const int s0 = at * spg, s1 = min(s0 + spg, a.nseg);
@@ -1144,7 +1155,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const Sample
   const int ri = blockIdx.y, seq = blockIdx.z, m = a.per - 1;
   const long row = (long)seq * a.per + ri;
   const int draft = in.draft && ri < m ? in.draft[(long)seq * m + ri] : -1;
-  const Group gr = {gridDim.x > 1 ? counts + row * gridDim.x * (kBins / 4) : nullptr, arrived + row, (int)blockIdx.x,
+  const Group gr = {gridDim.x > 1 ? counts + row * gridDim.x * (kGroupBins / 4) : nullptr, arrived + row, (int)blockIdx.x,
                     (int)gridDim.x};
   RowInfo mine;
   if (!select_row<HALF>(a, seq, ri, draft, gr, sh, mine)) return;
@@ -1326,7 +1337,7 @@ Layout layout(int64_t rows, int64_t V, int64_t sequences) {
   l.segm = up(l.drawn + (size_t)rows * 8);
   l.arrived = up(l.segm + (size_t)rows * n * 4);
   l.counts = up(l.arrived + (size_t)(sequences + rows) * 4);
-  l.bytes = l.counts + (size_t)rows * group_size(rows, (int)n) * kBins * 2;
+  l.bytes = l.counts + (size_t)rows * group_size(rows, (int)n) * kGroupBins * 2;
   return l;
 }
 

@@ -376,3 +376,20 @@ def test_tied_candidates(dev, V, dtype, top_k, top_p):
         close(got[2], want[2])
     flat = x.reshape(-1, V)[:6]
     close(ops.sampling_probs(flat.to(dev), top_k=top_k, top_p=top_p), np.stack([ref.probs(r, top_k=top_k, top_p=top_p) for r in _np(flat)]))
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.3), dict(top_p=0.9), dict(top_p=0.9999), dict(top_k=9000, top_p=0.999), dict(top_k=19990)])
+@pytest.mark.parametrize("n", [2, 300])
+@pytest.mark.parametrize("dtype,t", [("f16", 2e5), ("f16", 3.0), ("bf16", 1e30), ("bf16", 1.0)])
+def test_every_value_of_the_type(dev, dtype, t, n, kw):
+    """Logits of any finite bits at a temperature of the type's range: the cut lies thousands of values below the
+    largest, past what is counted at a time, near and below zero."""
+    from dspark_rocm import ops
+
+    V = 20000
+    g = torch.Generator().manual_seed(n)
+    x = torch.randint(-2 ** 15, 2 ** 15, (n, V), generator=g, dtype=torch.int32).to(torch.int16).view(DT[dtype])
+    x = torch.where(torch.isfinite(x), x, 0.0)
+    got = ops.sampling_probs(x.to(dev), temperature=t, **kw)
+    pick = range(n) if n < 10 else range(0, n, 61)
+    close(got[list(pick)], np.stack([ref.probs(r, temperature=t, **kw) for r in _np(x[list(pick)])]))
