@@ -930,14 +930,6 @@ __device__ __forceinline__ int drafts_of(const SampleArgs& a, const VerifyIn& in
   return in.lens ? min(max(in.lens[seq], 0), a.per - 1) : a.per - 1;
 }
 
-// Whether draft i of sequence seq, with probability px, is refused.
-__device__ __forceinline__ bool refused(const SampleArgs& a, const VerifyIn& in, int seq, int i, double px) {
-  const int v = in.draft[(long)seq * (a.per - 1) + i];
-  const bool inside = v >= 0 && v < a.V;
-  const double q = in.q ? (inside ? (double)in.q[seq * in.qb + i * in.qr + v] : 0.0) : 1.0;
-  return !(inside && uniform_at(in, (long)seq * a.per + i) * q < px);
-}
-
 // How the token of row i is drawn if its draft is the first refused, or it is the row after the last draft.
 __device__ __forceinline__ DrawIn draw_in(const SampleArgs& a, const VerifyIn& in, int seq, int i, int len) {
   DrawIn d;
@@ -1170,8 +1162,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const Sample
 }
 
 struct SpreadShared {
-  double z[kMaxDraft + 1], px[kMaxDraft + 1];
+  double z[kMaxDraft + 1];             // of the rows: RowInfo, without px
   float m[kMaxDraft + 1];
+  int thr[kMaxDraft + 1], cut[kMaxDraft + 1], draft[kMaxDraft + 1];
   DrawShared draw;
   int last;
 };
@@ -1185,39 +1178,55 @@ __global__ __launch_bounds__(kRowThreads) void sample_spread_kernel(const Sample
   __shared__ SpreadShared sh;
   const int seq = blockIdx.y, m = a.per - 1, t = threadIdx.x, lane = t & 63;
   const int len = drafts_of(a, in, seq);
-  if constexpr (CUT) {
-    if (t < m) sh.px[t] = __builtin_bit_cast(double, info[4 * ((long)seq * a.per + t) + 1]);
-  } else {
-    for (int i = uniform(t >> 6); i < a.per; i += kRowWaves) {
-      const long row = (long)seq * a.per + i;
-      const int draft = i < m ? in.draft[(long)seq * m + i] : -1;
-      const bool inside = draft >= 0 && draft < a.V;
-      const float xd = inside ? val<HALF>(row_ptr(a, seq, i)[draft]) : -INFINITY;
+  const double u_last = uniform_at(in, (long)seq * a.per + m);
+  // the last threads, a row each: what its draft is accepted by, on its way while the rows are joined
+  const int i = kRowThreads - 1 - t;
+  double px = 0, uq = 0;
+  float xd = -INFINITY;
+  RowInfo mine = {0.0, 0.0, 0.f, kLowKey<HALF>, kNoTies, 0};
+  if (i < a.per) {
+    const long row = (long)seq * a.per + i;
+    if constexpr (CUT) __builtin_memcpy(&mine, info + 4 * row, 32);
+    const int draft = i < m ? in.draft[(long)seq * m + i] : -1;
+    const bool inside = draft >= 0 && draft < a.V;
+    sh.draft[i] = draft;
+    uq = inside ? uniform_at(in, row) * (in.q ? (double)in.q[seq * in.qb + i * in.qr + draft] : 1.0) : INFINITY;
+    if (!CUT && inside) xd = val<HALF>(row_ptr(a, seq, i)[draft]);
+  }
+  if constexpr (!CUT) {
+    for (int r = uniform(t >> 6); r < a.per; r += kRowWaves) {
+      const long row = (long)seq * a.per + r;
       float mx;
       const double z = join_wave(a.segm + row * a.nseg, a.segs + row * a.nseg, a.nseg, a.c, mx);
       if (lane == 0) {
-        sh.z[i] = z;
-        sh.m[i] = mx;
-        sh.px[i] = z > 0 && xd > -INFINITY ? weight(xd, mx, a.c) / z : 0.0;
+        sh.z[r] = z;
+        sh.m[r] = mx;
       }
     }
   }
   if (t == 0) sh.draw.first = len;
   __syncthreads();
-  if (!CUT && blockIdx.x == 0 && t < m) in.px[(long)seq * m + t] = (float)sh.px[t];
-  if (t < len && refused(a, in, seq, t, sh.px[t])) atomicMin(&sh.draw.first, t);
+  if (i < a.per) {
+    if constexpr (CUT) {
+      px = mine.px;
+      sh.z[i] = mine.z;
+      sh.m[i] = mine.m;
+    } else {
+      px = sh.z[i] > 0 && xd > -INFINITY ? weight(xd, sh.m[i], a.c) / sh.z[i] : 0.0;
+      if (blockIdx.x == 0 && i < m) in.px[(long)seq * m + i] = (float)px;
+    }
+    sh.thr[i] = mine.thr;
+    sh.cut[i] = mine.cut;
+    if (i < len && !(uq < px)) atomicMin(&sh.draw.first, i);
+  }
   __syncthreads();
   const int n = sh.draw.first;
-  const DrawIn d = draw_in(a, in, seq, n, len);
-  RowInfo r;
-  if constexpr (CUT) {
-    __builtin_memcpy(&r, info + 4 * ((long)seq * a.per + n), 32);
-  } else {
-    r.z = sh.z[n];
-    r.m = sh.m[n];
-    r.thr = kLowKey<HALF>;
-    r.cut = kNoTies;
-  }
+  DrawIn d;
+  d.mode = n == len ? kDrawRow : in.q ? kDrawRest : kDrawOther;
+  d.q = d.mode == kDrawRest ? in.q + seq * in.qb + n * in.qr : nullptr;
+  d.skip = n < len ? sh.draft[n] : -1;
+  d.u = u_last;
+  const RowInfo r = {sh.z[n], 0.0, sh.m[n], sh.thr[n], sh.cut[n], 0};
   double* sums = rest + (long)seq * a.nseg;
   if (CUT || d.mode == kDrawRest) {
     const u16* x = row_ptr(a, seq, n);
@@ -1228,13 +1237,14 @@ __global__ __launch_bounds__(kRowThreads) void sample_spread_kernel(const Sample
     for (int s1 = s0; s1 < a.nseg; s1 += kOut * stride) {
       u32x4_t v[kOut];
       float q[kOut][8] = {};
+      float sm[kOut];
       bool on[kOut];
 #pragma unroll
       for (int i = 0; i < kOut; ++i) {
         const int s = s1 + i * stride, v0 = s * kSegVals + 8 * lane - off;
         on[i] = s < a.nseg && r.z > 0;
-        if (CUT && on[i]) on[i] = key_of_float<HALF>(a.segm[((long)seq * a.per + n) * a.nseg + s]) >= r.thr;
         if (!on[i]) continue;
+        if constexpr (CUT) sm[i] = a.segm[((long)seq * a.per + n) * a.nseg + s];
         v[i] = load8<HALF>(x, v0, a.V);
         if (d.mode == kDrawRest) load_q8(d.q, v0, a.V, q[i]);
       }
@@ -1243,7 +1253,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_spread_kernel(const Sample
         const int s = s1 + i * stride;
         if (s >= a.nseg) break;
         double sum = 0;
-        if (on[i]) {
+        if (on[i] && (!CUT || key_of_float<HALF>(sm[i]) >= r.thr)) {
           double w[8];
           rest8<HALF, CUT>(a, r, inv, v[i], s * kSegVals + 8 * lane - off, d.mode, q[i], d.skip, w);
 #pragma unroll
