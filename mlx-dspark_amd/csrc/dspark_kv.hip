@@ -10,7 +10,9 @@
 // bias NaN and its fields 0.
 //
 // Bound by bytes: 8 lanes hold a group, 8 values a lane (16 bytes of a 16-bit row), the group's extremes
-// joined over the 8 lanes with DPP.
+// joined over the 8 lanes with DPP. 2048 rows of 4 x 256 in bf16 to 4 bits: 7.3 us for 10.8 MB, of which the launch and
+// one round of loads are 4; 32768 rows of 8 x 128 read back to fp32 from 8 bits: 49 us for 340 MB, 6.9 TB/s, the rate
+// of a fill of the same size.
 #include "dspark_common.h"
 
 // A product and a sum stay two roundings: a fused one does not overflow between them.
@@ -20,7 +22,8 @@ namespace dspark {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvOut = 2;                      // stores of a thread that reads back
+// Stores of a thread that reads back (32768 rows of 8 x 128: 52 us at 2, 85 at 1, 53 at 4; 4017 rows: 6.0, 11.1, 7.3).
+constexpr int kKvOut = 2;
 
 struct KvSide {                                // keys or values
   char* x;                                     // plain rows (read, or the output of a read back)

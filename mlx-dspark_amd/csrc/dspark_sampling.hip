@@ -16,9 +16,9 @@ namespace {
 // ---------------------------------------------------------------- segments of every row
 
 constexpr int kStatThreads = 256;
-// Segments of a wave in the first pass: its sums are fp64 work that many waves share better (15 rows of 151936 cut by
-// a mass, 30.9 us at 4, 28.7 at 2, 28.4 at 1; 128 rows uncut in fp16 47.9 at 2, 49.2 at 1). Writing probabilities, where
-// a wave joins its row first: 4 (128 rows uncut 39 us, 42 at 2), 2 behind a cut, which has joined it.
+// Segments of a wave in the first pass: its sums are fp64 work that many waves share better (15 rows of 151936 cut by a
+// mass: 24.7 us at 2, 26.3 at 4, 24.9 at 1; 128 rows uncut in fp16: 47.2, 47.7, 48.3). Writing probabilities: 4 where a
+// wave joins its row first (128 rows: 49.7 us at 2), 2 behind a cut, which has joined it (15 rows: 26.6 us at 4).
 constexpr int kSegWave = 2, kProbWave = 4, kProbCutWave = 2;
 
 // Maximum and sum of weights of every segment: a wave takes SPW segments, their loads first.
@@ -317,7 +317,9 @@ struct DrawIn {                        // what a row's own draw goes by
   double u;
 };
 
-constexpr int kGroup = 16;             // most workgroups that count a row together
+// Most workgroups that count a row together: each hands over its counts, which the last one joins (15 rows of 151936: 36.7
+// us by one workgroup a row, 25.1 by 4, 23.8 by 8, 24.8 by 16; one row 22.4 by 4, 20.5 by 8 and by 16).
+constexpr int kGroup = 8;
 constexpr int kGroupBins = 2 * kBins;  // values that they count: 16-bit counts
 constexpr int kOwn = 2;                // segments of a wave whose loads are out together
 struct Group {                         // a row counted by several workgroups, each over its own run of segments
@@ -649,7 +651,7 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
 
   // Few candidates are sorted. A top_k leaves little more than that many; a mass alone may leave most of a segment,
   // so that only rows where few segments reach are tried.
-  const bool few = nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves);
+  const bool few = nlist <= (a.top_k ? kAhead * kRowWaves : kRowWaves / 2);
   const bool grouped = gr.counts && !few;
   const auto list_all = [&]() {
     __syncthreads();
@@ -712,9 +714,8 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
     int seen = 0;
     double mass = 0;
     found = false;
-    for (int hi = top, lo; hi >= lowest && !found; hi = lo - 1) {
-      // a few thousand values first: the goal is mostly there
-      lo = max(lowest, hi - (hi == top ? kChunk : kBins - 4) + 1);
+    for (int hi = top, lo, span = kChunk<HALF>; hi >= lowest && !found; hi = lo - 1, span = min(4 * span, kBins - 4)) {
+      lo = max(lowest, hi - span + 1);
       if (exchanged && hi < group_lo) {
         list_all();
         exchanged = false;
@@ -756,7 +757,9 @@ __device__ __forceinline__ bool select_row(const SampleArgs& a, int seq, int ri,
       const int b0 = min(t * each, nb), b1 = min(b0 + each, nb);
       int cn = 0;
       double cm = 0;
-      if (b0 < b1) {
+      int some = 0;                      // values near zero are many, and mostly nobody's
+      for (int b = b0; b < b1; ++b) some |= sh.bins[base + b];
+      if (some) {
         FallingWeights<HALF> f;
         f.start(hi - b0, mx, a.c, mc);
         for (int b = b0; b < b1; ++b) {
@@ -1387,7 +1390,9 @@ int sample_args(const char* what, int64_t dtype, const void* logits, int64_t row
   return DSPARK_OK;
 }
 
-constexpr long kTabSegs = 16384;       // segments from which the table pays
+// Segments from which the table pays: 8 rows of 151936 9.9 us without it, 10.8 with; 24 rows 15.3, 15.1; 55 rows 27.2, 24.6;
+// 256 rows verified 53.0, 37.9.
+constexpr long kTabSegs = 8192;
 
 unsigned groups(int nseg, int spw) { return (unsigned)((nseg + spw * (kStatThreads / 64) - 1) / (spw * (kStatThreads / 64))); }
 

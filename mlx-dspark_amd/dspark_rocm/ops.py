@@ -1066,9 +1066,9 @@ def _no_repeats(what: str, out: torch.Tensor) -> None:
         raise ValueError(f"{what}: the output is an expanded view ({list(out.shape)}, strides {list(out.stride())})")
 
 
-def _no_aliases(what: str, *ts: torch.Tensor) -> None:
-    """Each of ``ts`` starts elsewhere: the same rows given twice would be written by two workgroups."""
-    at = [t.data_ptr() for t in ts]
+def _distinct(what: str, *at: int) -> None:
+    """Addresses of what is written, and of what else must not be there: the same rows given twice would be written by
+    two workgroups, or read while they are."""
     if len(set(at)) != len(at):
         raise ValueError(f"{what}: the same rows given twice")
 
@@ -1146,9 +1146,10 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
             _check_rope_out("k_out", k, k_out)
         if k.numel():
             if q.numel():
-                _no_aliases("rope", q_out, k_out)
-                if q_out.data_ptr() == k.data_ptr() or k_out.data_ptr() == q.data_ptr():
-                    raise ValueError("rope: the queries' output is the keys' input, or the other way round")
+                at_q, at_k = q_out.data_ptr(), k_out.data_ptr()
+                _distinct("rope", at_q, at_k)
+                _distinct("rope", at_q, k.data_ptr())
+                _distinct("rope", at_k, q.data_ptr())
             sko = k_out.stride()
             keys = (k.data_ptr(), k_out.data_ptr(), sk[0], sk[1], sk[2], sko[0], sko[1], sko[2], k.shape[1])
     if q.numel() or keys is not _NO_KEYS:
@@ -1224,7 +1225,7 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt, True),
             *_kv_side(what, values, v_rows, words, groups, cdt, True))
     if B * H * T:
-        _no_aliases(what, *k_rows, *v_rows)
+        _distinct(what, *args[12:15], *args[25:28])         # words, scales and biases of both
         _call_on(dev, "dspark_kv_quantize", _KV_ARGS.pack(*args))
 
 
@@ -1251,6 +1252,6 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt, False),
             *_kv_side(what, v, values, words, groups, cdt, False))
     if shape[0] * shape[1] * shape[2]:
-        _no_aliases(what, k, v)
+        _distinct(what, k.data_ptr(), v.data_ptr())
         _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v
