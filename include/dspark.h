@@ -5,7 +5,8 @@
  *   1. the small-M affine-quantized matmul (4/8-bit, group 64, M = 1..16 verify rows);
  *   2. multi-row causal GQA verify attention over a strided KV cache (split-KV + combine);
  *   3. MoE top-k routing plus the grouped expert qmm (gather_qmm / SwitchGLU).
- * plus the small elementwise kernels a dense verify forward needs around them.
+ * plus the small elementwise kernels a dense verify forward needs around them, and the operators of a round at a
+ * temperature: its distributions and accept rule, rotary positions by a table, rows of quantized caches.
  *
  * Conventions (every entry point):
  *   - Plain pointers and sizes only; device pointers come from the caller (torch tensors).

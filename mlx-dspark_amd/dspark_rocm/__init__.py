@@ -10,6 +10,7 @@ Modules:
   sdpa_split    row-split fallback scope (reference: sdpa_split.py)
   moe           routing, gather_qmm, SwitchGLU (reference: mlx-lm SparseMoeBlock / SwitchGLU)
   kv_cache      bf16 KV cache with O(1) trim (reference: BatchCache / mlx-lm KVCache)
+  rope          rotary frequency tables (reference: mlx-lm's rope_scaling configurations)
 """
 
 __version__ = "0.1.0"
