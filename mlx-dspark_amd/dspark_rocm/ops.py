@@ -7,6 +7,7 @@ These are the product path: every function here launches a hand-written gfx950 k
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
@@ -894,10 +895,10 @@ def _call_on(dev: torch.device, name: str, args: bytes) -> None:
             _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _no_autograd(what: str, *ts: torch.Tensor) -> None:
+def _no_autograd(what: str, *ts) -> None:
     if torch.is_grad_enabled():
         for t in ts:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: has no backward pass; detach its inputs or use torch.no_grad()")
 
 
@@ -922,7 +923,7 @@ def check_sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
 
 
 def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> torch.Tensor:
-    nbytes = _lib.load().dspark_sampling_workspace(rows, vocab, sequences)
+    nbytes = sampling_workspace_bytes(rows, vocab, sequences)
     if nbytes == 0:
         raise ValueError(f"{rows} rows of {vocab} logits (up to 65535 rows of 524280)")
     if ws is None:
@@ -932,6 +933,7 @@ def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> to
     return ws
 
 
+@functools.lru_cache(maxsize=256)
 def sampling_workspace_bytes(rows: int, vocab: int, sequences: int = 0) -> int:
     """Workspace bytes of :func:`sampling_probs` over ``rows`` rows, or of :func:`speculative_verify`
     over ``sequences`` sequences of ``rows`` rows together."""
@@ -1096,66 +1098,72 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
     an int32 / int64 tensor [L] or [B or 1, L or 1] with the position of every row, as tree rows need. The
     angle is reduced in fp64; one rounding to the tensors' type. ``q_out`` / ``k_out``: where to write,
     e.g. a cache's rows, or q and k themselves; elements that nothing else of the call uses."""
-    dev = _one_device("rope", q, k, freqs, q_out, k_out)
-    dtype, shape = q.dtype, q.shape
+    tensor = isinstance(positions, torch.Tensor)
+    dev = _one_device("rope", q, k, freqs, q_out, k_out, positions if tensor else None)
+    dtype = q.dtype
     dt = ROPE_DTYPES.get(dtype)
-    if dt is None or (k is not None and k.dtype != dtype):
+    if dt is None or (k is not None and k.dtype is not dtype):
         raise TypeError(f"rope: q {dtype}, k {None if k is None else k.dtype} (one of bfloat16, float16, float32)")
-    if len(shape) != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (shape[0], *shape[2:]))):
-        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(shape)} and {None if k is None else list(k.shape)}")
-    B, Hq, L, D = shape
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(q.shape)} and {None if k is None else list(k.shape)}")
+    B, Hq, L, D = q.shape
+    Hk = 0
+    if k is not None:
+        Bk, Hk, Lk, Dk = k.shape
+        if Bk != B or Lk != L or Dk != D:
+            raise ValueError(f"rope: q {list(q.shape)} and k {list(k.shape)}")
+    elif k_out is not None:
+        raise ValueError("rope: k_out without k")
     half = freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not 1 <= half <= min(128, D // 2):
         raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(freqs.shape)}")
-    if k is None and k_out is not None:
-        raise ValueError("rope: k_out without k")
-    _no_autograd("rope", *(t for t in (q, k, freqs, q_out, k_out) if t is not None))
+    _no_autograd("rope", q, k, freqs, q_out, k_out)
     freqs = freqs.contiguous()
     pos, pos64, pb, pl, pos0 = 0, 0, 0, 0, 0
-    if isinstance(positions, torch.Tensor):
-        ps = positions.shape
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev or len(ps) not in (1, 2):
-            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L] on {dev}, got {positions.dtype} {list(ps)}")
-        if ps[-1] not in (1, L) or (len(ps) == 2 and ps[0] not in (1, B)):
-            raise ValueError(f"rope: positions {list(ps)} for {B} sequences of {L} rows")
-        pos, pos64, st = positions.data_ptr(), int(positions.dtype is torch.int64), positions.stride()
-        pl = st[-1] if ps[-1] > 1 else 0
-        pb = st[0] if len(ps) == 2 and ps[0] > 1 else 0
+    if tensor:
+        pos64 = positions.dtype is torch.int64
+        axes = positions.dim()
+        if not (pos64 or positions.dtype is torch.int32) or not 1 <= axes <= 2:
+            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L], got {positions.dtype} {list(positions.shape)}")
+        nb, nl = positions.shape if axes == 2 else (1, positions.shape[0])
+        if nl not in (1, L) or nb not in (1, B):
+            raise ValueError(f"rope: positions {list(positions.shape)} for {B} sequences of {L} rows")
+        pos, st = positions.data_ptr(), positions.stride()
+        pl = st[-1] if nl > 1 else 0
+        pb = st[0] if nb > 1 else 0
     else:
         pos0 = int(positions)
         if abs(pos0) >= 1 << 52:
             raise ValueError(f"rope: position {pos0}")
-    sq = q.stride()
-    if sq[3] != 1:
+    s0, s1, s2, unit = q.stride()
+    if unit != 1:
         q = q.contiguous()
-        sq = q.stride()
+        s0, s1, s2, _ = q.stride()
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_rope_out("q_out", q, q_out)
-    so = q_out.stride()
+    o0, o1, o2, _ = q_out.stride()
+    at_q, at_qo = q.data_ptr(), q_out.data_ptr()
     keys = _NO_KEYS
     if k is not None:
-        sk = k.stride()
-        if sk[3] != 1:
+        k0, k1, k2, unit = k.stride()
+        if unit != 1:
             k = k.contiguous()
-            sk = k.stride()
+            k0, k1, k2, _ = k.stride()
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         else:
             _check_rope_out("k_out", k, k_out)
-        if k.numel():
-            if q.numel():
-                at_q, at_k = q_out.data_ptr(), k_out.data_ptr()
-                _distinct("rope", at_q, at_k)
-                _distinct("rope", at_q, k.data_ptr())
-                _distinct("rope", at_k, q.data_ptr())
-            sko = k_out.stride()
-            keys = (k.data_ptr(), k_out.data_ptr(), sk[0], sk[1], sk[2], sko[0], sko[1], sko[2], k.shape[1])
-    if q.numel() or keys is not _NO_KEYS:
+        if B and L and Hk:
+            at_k, at_ko = k.data_ptr(), k_out.data_ptr()
+            if Hq and (at_ko == at_qo or at_ko == at_q or at_qo == at_k):
+                raise ValueError("rope: the same rows given twice")
+            keys = (at_k, at_ko, k0, k1, k2, *k_out.stride()[:3], Hk)
+    if B and L and (Hq or Hk):
         _call_on(dev, "dspark_rope",
-                 _ROPE_ARGS.pack(dt, q.data_ptr(), q_out.data_ptr(), sq[0], sq[1], sq[2], so[0], so[1], so[2], Hq, *keys, B, L,
-                                 D, 2 * half, bool(interleaved), freqs.data_ptr(), scale, pos, pos64, pb, pl, pos0))
+                 _ROPE_ARGS.pack(dt, at_q, at_qo, s0, s1, s2, o0, o1, o2, Hq, *keys, B, L, D, 2 * half, bool(interleaved),
+                                 freqs.data_ptr(), scale, pos, pos64, pb, pl, pos0))
     return q_out, k_out
 
 
@@ -1168,15 +1176,14 @@ def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple,
     w, s, b = trip
     if w.dtype is not torch.int32:
         _require_packed(w)
-    if s.dtype != cache_dtype or b.dtype != cache_dtype:
+    if s.dtype is not cache_dtype or b.dtype is not cache_dtype:
         raise TypeError(f"{what}: scales and biases of {cache_dtype}, {s.dtype} and {b.dtype}")
     if w.shape != words or s.shape != groups or b.shape != groups:
         raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
     w0, w1, w2, w3 = w.stride()
-    ss = s.stride()
-    bs = b.stride()
-    s0, s1, s2, s3 = ss
-    if w3 != 1 or ss[:3] != bs[:3] or ((s3 != 1 or bs[3] != 1) and groups[3] > 1):
+    s0, s1, s2, s3 = s.stride()
+    b0, b1, b2, b3 = b.stride()
+    if w3 != 1 or s0 != b0 or s1 != b1 or s2 != b2 or ((s3 != 1 or b3 != 1) and groups[3] > 1):
         raise ValueError(f"{what}: unit last strides, and shared ones of scales and biases, needed")
     if written and not (w0 and w1 and w2 and s0 and s1 and s2):
         for t in trip:
