@@ -265,24 +265,27 @@ __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >>
 
 __device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int seq, int i) { return a.x + seq * a.ldb + i * a.ldr; }
 
-// Maximum and normaliser of a row without a cut, the join of its segments, by one wave: four values a lane at once.
+// Maximum and normaliser of a row without a cut, the join of its segments, by one wave: eight values a lane at once.
 __device__ __forceinline__ double join_wave(const float* segm, const double* segs, int nseg, double c, float& m) {
+  constexpr int kAtOnce = 8;
   const int lane = threadIdx.x & 63;
   float mx = -INFINITY;                // of this lane so far; z against it
   double z = 0;
-  for (int s0 = lane; s0 < nseg; s0 += 256) {
-    float sm[4];
-    double ss[4];
+  for (int s0 = lane; s0 < nseg; s0 += 64 * kAtOnce) {
+    float sm[kAtOnce], to = mx;
+    double ss[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kAtOnce; ++i) {
       const int s = s0 + 64 * i;
       sm[i] = s < nseg ? segm[s] : -INFINITY;
       ss[i] = s < nseg ? segs[s] : 0.0;
     }
-    const float to = fmaxf(fmaxf(mx, fmaxf(sm[0], sm[1])), fmaxf(sm[2], sm[3]));
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, sm[i]);
     z *= weight(mx, to, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z += ss[i] * weight(sm[i], to, c);
+    for (int i = 0; i < kAtOnce; ++i)
+      if (s0 - lane + 64 * i < nseg) z += ss[i] * weight(sm[i], to, c);
     mx = to;
   }
   m = wave_max(mx);
