@@ -1142,7 +1142,26 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
   write_tokens(a, in, seq, n, sh.token);
 }
 
-// What is kept of a row, for a launch behind this one: by a group of workgroups where the rows are few (gridDim.x).
+__device__ __forceinline__ void write_info(uint64_t* info, long row, const RowInfo& r) {
+  static_assert(sizeof(RowInfo) == 32, "four words");
+  const int t = threadIdx.x;
+  if (t >= 4) return;
+  uint64_t w[4];
+  __builtin_memcpy(w, &r, 32);
+  info[4 * row + t] = t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3];
+}
+
+// What is kept of a row of a small top_k, for the launch that writes probabilities.
+template <bool HALF>
+__global__ __launch_bounds__(kRowThreads) void sample_few_kernel(const SampleArgs a, uint64_t* info) {
+  __shared__ CutShared sh;
+  int token;
+  RowInfo mine;
+  cut_row<HALF>(a, blockIdx.x, 0, -1, DrawIn{-1, -1, nullptr, 0.0}, sh, sh.few, mine, token);
+  write_info(info, blockIdx.x, mine);
+}
+
+// The same by counts, for either launch behind this one: by a group of workgroups where the rows are few (gridDim.x).
 template <bool HALF>
 __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const SampleArgs a, const VerifyIn in, uint64_t* info,
                                                                    uint64_t* counts, int* arrived) {
@@ -1154,12 +1173,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_select_kernel(const Sample
                     (int)gridDim.x};
   RowInfo mine;
   if (!select_row<HALF>(a, seq, ri, draft, gr, sh, mine)) return;
-  if (threadIdx.x < 4) {
-    uint64_t w[4];
-    __builtin_memcpy(w, &mine, 32);
-    const int t = threadIdx.x;
-    info[4 * row + t] = t == 0 ? w[0] : t == 1 ? w[1] : t == 2 ? w[2] : w[3];
-  }
+  write_info(info, row, mine);
   if (threadIdx.x == 0 && draft != -1) in.px[(long)seq * m + ri] = (float)mine.px;
   else if (threadIdx.x == 0 && in.draft && ri < m) in.px[(long)seq * m + ri] = 0.f;
 }
@@ -1416,7 +1430,7 @@ bool many(const SampleArgs& a) { return !a.top_k || a.top_k > kListed / 2; }
 
 template <bool HALF>
 void launch_select(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, hipStream_t s) {
-  const int group = many(a) ? group_size(a.rows, a.nseg) : 0;
+  const int group = group_size(a.rows, a.nseg);
   hipLaunchKernelGGL((sample_select_kernel<HALF>), dim3(group ? group : 1, (unsigned)a.per, (unsigned)(a.rows / a.per)),
                      dim3(kRowThreads), 0, s, a, in, reinterpret_cast<uint64_t*>(w + l.info),
                      reinterpret_cast<uint64_t*>(w + l.counts), a.arrived + a.rows / a.per);
@@ -1428,7 +1442,8 @@ void probs(const SampleArgs& a, char* w, const Layout& l, float* out, long ldo, 
   const dim3 block(kStatThreads);
   launch_segments<HALF>(a, s);
   if (a.top_k || a.top_p < 1.0) {
-    launch_select<HALF>(a, VerifyIn{}, w, l, s);
+    if (many(a)) launch_select<HALF>(a, VerifyIn{}, w, l, s);
+    else hipLaunchKernelGGL((sample_few_kernel<HALF>), dim3((unsigned)a.rows), dim3(kRowThreads), 0, s, a, reinterpret_cast<uint64_t*>(w + l.info));
     hipLaunchKernelGGL((sample_probs_kernel<HALF, true, kProbCutWave>), dim3(groups(a.nseg, kProbCutWave), (unsigned)a.rows),
                        block, 0, s, a, info, out, ldo);
   } else {
