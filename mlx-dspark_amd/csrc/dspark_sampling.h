@@ -263,6 +263,15 @@ __device__ __forceinline__ u32x4_t load8(const u16* row, int v0, int V) {
 }
 __device__ __forceinline__ u32 bits_of(const u32x4_t& v, int j) { return (v[j >> 1] >> (16 * (j & 1))) & 0xFFFFu; }
 
+// The largest of a segment's logits (NaN: none), in every lane.
+template <bool HALF>
+__device__ __forceinline__ float max8_wave(const u32x4_t& v) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, val<HALF>(bits_of(v, j)));
+  return wave_max(m);
+}
+
 __device__ __forceinline__ const u16* row_ptr(const SampleArgs& a, int seq, int i) { return a.x + seq * a.ldb + i * a.ldr; }
 
 // Maximum and normaliser of a row without a cut, the join of its segments, by one wave: eight values a lane at once.

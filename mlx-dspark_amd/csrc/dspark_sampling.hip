@@ -2,10 +2,11 @@
 // (dspark_sampling_probs) and the accept rule of a sampled round (dspark_speculative_verify).
 //
 // The first launch leaves every segment's maximum and sum. Then
-//   verify, few candidates a row (a small top_k): a workgroup a row selects and draws, the last of a sequence accepts;
+//   verify, a small top_k: a workgroup a row selects and draws, the last of a sequence accepts;
 //   verify, else: one launch selects where something is cut, one of workgroups over a sequence's segments joins its
 //   rows where nothing is, accepts, sums r over the row drawn from, and its last workgroup draws;
 //   probabilities: a launch selects where something is cut, one writes.
+// A small top_k of rows that are not long, without drafts, is one launch: a workgroup takes its row whole.
 #include <cmath>
 
 #include "dspark_sampling.h"
@@ -38,10 +39,7 @@ __global__ __launch_bounds__(kStatThreads) void sample_segments_kernel(const Sam
 #pragma unroll
   for (int i = 0; i < SPW; ++i) {
     if (s0 + i >= a.nseg) return;
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, val<HALF>(bits_of(v[i], j)));
-    m = wave_max(m);
+    const float m = max8_wave<HALF>(v[i]);
     const long at = ((long)seq * a.per + blockIdx.y) * a.nseg + s0 + i;
     if constexpr (SUM) {
       const double mc = -(double)m * a.c;
@@ -124,10 +122,7 @@ __global__ __launch_bounds__(kTabThreads) void sample_table_kernel(const SampleA
       sum = wave_total(sum);
       float m = 0;
       if (!(sum >= light)) {            // also NaN
-        m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, val<false>(bits_of(now, j)));
-        m = wave_max(m);
+        m = max8_wave<false>(now);
         sum = 0;
         if (m > -INFINITY) {
           const double mc = -(double)m * a.c;
@@ -163,11 +158,19 @@ struct RowState {
   double z;
 };
 
+// Most segments of a row that a workgroup takes whole, without a launch before it (a token drawn from one row of 70000: 9.9
+// us, 10.6 in two launches; of 100000: 11.1, 10.6; from each of 600 rows of 50257: 29.6, 35.9).
+constexpr int kWholeSegs = 160;
+static_assert(kWholeSegs <= kListed, "one room");
+
 struct Few {                           // a few candidates, one by one
   uint64_t cand[kListed];              // (key + 2^15) << 32 | ~index: the larger the earlier in falling order
   uint64_t sorted[kListed];
   double w[kListed], r[kListed];       // weights in falling order; what is drawn from, by index
-  int order[kListed];                  // the kept tokens by index
+  union {
+    int order[kListed];                // the kept tokens by index
+    float segm[kWholeSegs];            // before that: the segments' maxima
+  };
 };
 
 struct RowShared : RowState {
@@ -561,14 +564,33 @@ __device__ __forceinline__ void sorted_row(const SampleArgs& a, int n, float mx,
   token = sh.token;
 }
 
-// A row of a small top_k: what is kept of it, px of token `draft`, and the token drawn from it.
-template <bool HALF>
+// A row of a small top_k: what is kept of it, px of token `draft`, and the token drawn from it. WHOLE: there was no launch
+// before this one, the segments' maxima are formed here.
+template <bool HALF, bool WHOLE>
 __device__ __forceinline__ void cut_row(const SampleArgs& a, int seq, int ri, int draft, const DrawIn& d, RowState& sh, Few& fw,
                                         RowInfo& out, int& token) {
   const int t = threadIdx.x;
   const u16* x = row_ptr(a, seq, ri);
   const int off = row_off(x);
-  const float sm = t < a.nseg ? a.segm[((long)seq * a.per + ri) * a.nseg + t] : -INFINITY;      // kMaxSegs <= kRowThreads
+  float sm = -INFINITY;                 // kMaxSegs <= kRowThreads
+  if constexpr (WHOLE) {
+    for (int s0 = uniform(t >> 6); s0 < a.nseg; s0 += kAhead * kRowWaves) {
+      u32x4_t v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (s0 + u * kRowWaves < a.nseg) v[u] = load8<HALF>(x, (s0 + u * kRowWaves) * kSegVals + 8 * (t & 63) - off, a.V);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (s0 + u * kRowWaves >= a.nseg) break;
+        const float m = max8_wave<HALF>(v[u]);
+        if ((t & 63) == 0) fw.segm[s0 + u * kRowWaves] = m;
+      }
+    }
+    __syncthreads();
+    if (t < a.nseg) sm = fw.segm[t];
+  } else {
+    if (t < a.nseg) sm = a.segm[((long)seq * a.per + ri) * a.nseg + t];
+  }
   const float xd = draft >= 0 && draft < a.V ? val<HALF>(x[draft]) : -INFINITY;
   const float mx = row_start<HALF>(a, sm, sh);
   if (!(mx > -INFINITY)) {
@@ -1109,7 +1131,7 @@ struct CutShared : RowState {
 
 // Rows of a small top_k: one row a workgroup. It draws its token too, in case its draft is the first refused (the random
 // number of the draw is there from the start); the last workgroup of a sequence accepts.
-template <bool HALF>
+template <bool HALF, bool WHOLE>
 __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArgs a, const VerifyIn in, uint64_t* drawn) {
   __shared__ CutShared sh;
   const int ri = blockIdx.x, seq = blockIdx.y, m = a.per - 1, t = threadIdx.x;
@@ -1122,7 +1144,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_cut_kernel(const SampleArg
   if (ri < len) uq = inside ? uniform_at(in, row) * (in.q ? (double)d.q[draft] : 1.0) : INFINITY;
   int token;
   RowInfo mine;
-  cut_row<HALF>(a, seq, ri, draft, d, sh, sh.few, mine, token);
+  cut_row<HALF, WHOLE>(a, seq, ri, draft, d, sh, sh.few, mine, token);
+  if constexpr (WHOLE) {                // rows without drafts
+    write_tokens(a, in, seq, 0, token);
+    return;
+  }
   if (t == 0) {
     if (ri < m) in.px[(long)seq * m + ri] = (float)mine.px;
     put_far(drawn + row, (uint64_t)(ri >= len || !(uq < mine.px)) << 32 | (u32)token);
@@ -1157,8 +1183,27 @@ __global__ __launch_bounds__(kRowThreads) void sample_few_kernel(const SampleArg
   __shared__ CutShared sh;
   int token;
   RowInfo mine;
-  cut_row<HALF>(a, blockIdx.x, 0, -1, DrawIn{-1, -1, nullptr, 0.0}, sh, sh.few, mine, token);
+  cut_row<HALF, false>(a, blockIdx.x, 0, -1, DrawIn{-1, -1, nullptr, 0.0}, sh, sh.few, mine, token);
   write_info(info, blockIdx.x, mine);
+}
+
+// The probabilities of a row of a small top_k, by a workgroup that takes it whole: zeros while its logits are on their
+// way, then the few that are not.
+template <bool HALF>
+__global__ __launch_bounds__(kRowThreads) void sample_whole_kernel(const SampleArgs a, float* __restrict__ out, long ldo) {
+  __shared__ CutShared sh;
+  const int t = threadIdx.x;
+  float* y = out + (long)blockIdx.x * ldo;
+  const int head = min((int)(-(reinterpret_cast<uintptr_t>(y) >> 2) & 3), a.V), quads = (a.V - head) / 4;
+  if (t < head) y[t] = 0.f;
+  for (int i = t; i < quads; i += kRowThreads) *reinterpret_cast<f32x4_t*>(y + head + 4 * i) = f32x4_t{};
+  if (t < a.V - head - 4 * quads) y[head + 4 * quads + t] = 0.f;
+  int token;
+  RowInfo mine;
+  cut_row<HALF, true>(a, blockIdx.x, 0, -1, DrawIn{-1, -1, nullptr, 0.0}, sh, sh.few, mine, token);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // the zeros are there, every thread's
+  __syncthreads();
+  if (mine.z > 0 && t < sh.keep) y[(int)~(u32)sh.few.sorted[t]] = (float)(sh.few.w[t] * (1.0 / mine.z));
 }
 
 // The same by counts, for either launch behind this one: by a group of workgroups where the rows are few (gridDim.x).
@@ -1440,10 +1485,16 @@ template <bool HALF>
 void probs(const SampleArgs& a, char* w, const Layout& l, float* out, long ldo, hipStream_t s) {
   const uint64_t* info = reinterpret_cast<uint64_t*>(w + l.info);
   const dim3 block(kStatThreads);
+  const dim3 grid((unsigned)a.rows), row(kRowThreads);
+  const bool cut = a.top_k || a.top_p < 1.0;
+  if (cut && !many(a) && a.nseg <= kWholeSegs) {
+    hipLaunchKernelGGL((sample_whole_kernel<HALF>), grid, row, 0, s, a, out, ldo);
+    return;
+  }
   launch_segments<HALF>(a, s);
-  if (a.top_k || a.top_p < 1.0) {
+  if (cut) {
     if (many(a)) launch_select<HALF>(a, VerifyIn{}, w, l, s);
-    else hipLaunchKernelGGL((sample_few_kernel<HALF>), dim3((unsigned)a.rows), dim3(kRowThreads), 0, s, a, reinterpret_cast<uint64_t*>(w + l.info));
+    else hipLaunchKernelGGL((sample_few_kernel<HALF>), grid, row, 0, s, a, reinterpret_cast<uint64_t*>(w + l.info));
     hipLaunchKernelGGL((sample_probs_kernel<HALF, true, kProbCutWave>), dim3(groups(a.nseg, kProbCutWave), (unsigned)a.rows),
                        block, 0, s, a, info, out, ldo);
   } else {
@@ -1461,12 +1512,17 @@ void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, h
   // over the rows that are drawn from, a workgroup a CU, at most one a wave and segment
   const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
   const unsigned spread = most < fill ? most : fill;
+  if (cut && !many(a) && a.per == 1 && a.nseg <= kWholeSegs) {
+    hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3(1, B), dim3(kRowThreads), 0, s, a, in,
+                       reinterpret_cast<uint64_t*>(w + l.drawn));
+    return;
+  }
   launch_segments<HALF>(a, s);
   if (cut && many(a)) {
     launch_select<HALF>(a, in, w, l, s);
     hipLaunchKernelGGL((sample_spread_kernel<HALF, true>), dim3(spread, B), dim3(kRowThreads), 0, s, a, in, info, rest);
   } else if (cut) {
-    hipLaunchKernelGGL((sample_cut_kernel<HALF>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in,
+    hipLaunchKernelGGL((sample_cut_kernel<HALF, false>), dim3((unsigned)a.per, B), dim3(kRowThreads), 0, s, a, in,
                        reinterpret_cast<uint64_t*>(w + l.drawn));
   } else {
     hipLaunchKernelGGL((sample_spread_kernel<HALF, false>), dim3(in.q ? spread : 1, B), dim3(kRowThreads), 0, s, a, in, info,

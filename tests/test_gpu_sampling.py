@@ -393,3 +393,25 @@ def test_every_value_of_the_type(dev, dtype, t, n, kw):
     got = ops.sampling_probs(x.to(dev), temperature=t, **kw)
     pick = range(n) if n < 10 else range(0, n, 61)
     close(got[list(pick)], np.stack([ref.probs(r, temperature=t, **kw) for r in _np(x[list(pick)])]))
+
+
+@pytest.mark.parametrize("kind", ["plain", "ties", "same", "masked", "odd", "far"])
+@pytest.mark.parametrize("V,dtype", [(1, "bf16"), (9, "f16"), (513, "bf16"), (8192, "f16"), (50257, "bf16"), (81905, "bf16"),
+                                     (81913, "f16"), (81920, "bf16"), (100001, "f16")])
+def test_rows_without_drafts(dev, V, dtype, kind):
+    """The next token of each row, sampled; around the length to which a row is taken whole."""
+    from dspark_rocm import ops
+
+    n = 5
+    g = torch.Generator().manual_seed(V)
+    x = rows(g, n, V, DT[dtype], kind).reshape(n, 1, V)
+    none = torch.zeros(n, 0, dtype=torch.int32, device=dev)
+    for kw in (dict(top_k=1), dict(top_k=20, top_p=0.9), dict(top_k=128), dict(top_k=100, top_p=0.7, temperature=0.5)):
+        u = torch.rand(n, 1, generator=g, dtype=torch.float64)
+        got = ops.speculative_verify(x.to(dev), none, u.to(dev), **kw)
+        want = ref.verify(_np(x), np.zeros((n, 0), np.int32), u.numpy(), None, None, **kw)
+        assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1]), (kw, got, want)
+        buf = torch.full((n * V + 8,), 7.0, device=dev)
+        out = buf[3:3 + n * V].view(n, 1, V)
+        close(ops.sampling_probs(x.to(dev), out=out, **kw)[:, 0], np.stack([ref.probs(r, **kw) for r in _np(x[:, 0])]))
+        assert (buf[:3] == 7).all() and (buf[3 + n * V:] == 7).all()
