@@ -415,3 +415,26 @@ def test_rows_without_drafts(dev, V, dtype, kind):
         out = buf[3:3 + n * V].view(n, 1, V)
         close(ops.sampling_probs(x.to(dev), out=out, **kw)[:, 0], np.stack([ref.probs(r, **kw) for r in _np(x[:, 0])]))
         assert (buf[:3] == 7).all() and (buf[3 + n * V:] == 7).all()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.8), dict(top_k=300)])
+def test_offsets_past_32_bits(dev, kw):
+    """Sequences and rows whose logits and draft probabilities lie more than 2^31 elements apart."""
+    from dspark_rocm import ops
+
+    V, far = 5001, (1 << 31) + 17
+    g = torch.Generator().manual_seed(3)
+    x = rows(g, 4, V, torch.bfloat16).reshape(2, 2, V)
+    d, q = _drafts(g, x, "plain", 1)
+    u = torch.rand(2, 2, generator=g, dtype=torch.float64)
+    want = ops.speculative_verify(x.to(dev), d.to(dev), u.to(dev), draft_probs=q.to(dev), **kw)
+    buf, qbuf = torch.empty(far + 2 * V, dtype=torch.bfloat16, device=dev), torch.empty(far + 2 * V, device=dev)
+    qs = qbuf.as_strided((2, 1, V), (far, V, 1)).copy_(q)
+    for strides in ((far, V, 1), (V, far, 1)):
+        xs = buf.as_strided((2, 2, V), strides).copy_(x)
+        got = ops.speculative_verify(xs, d.to(dev), u.to(dev), draft_probs=qs, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    xs = buf.as_strided((2, V), (far, 1)).copy_(x[:, 0])
+    assert torch.equal(ops.sampling_probs(xs, **kw), ops.sampling_probs(x[:, 0].contiguous().to(dev), **kw))
+    del buf, qbuf, qs, xs
+    torch.cuda.empty_cache()
