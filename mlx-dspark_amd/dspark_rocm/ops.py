@@ -958,7 +958,7 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     shape = logits.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"sampling_probs: logits {list(shape)}")
-    _no_autograd("sampling_probs", logits)
+    _no_autograd("sampling_probs", logits, out)
     t, k, p = check_sampler(temperature, top_k, top_p)
     V = shape[-1]
     x = logits if len(shape) == 2 else logits.reshape(-1, V)
@@ -1223,7 +1223,7 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     (B, H, T, D), groups, cdt = _kv_shape(what, k_rows, bits, group_size)
     if keys.shape != (B, H, T, D) or values.shape != keys.shape:
         raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)} for rows [{B}, {H}, {T}, {D}]")
-    _no_autograd(what, keys, values)
+    _no_autograd(what, keys, values, *k_rows[1:], *v_rows[1:])
     if keys.stride(3) != 1:
         keys = keys.contiguous()
     if values.stride(3) != 1:
@@ -1246,6 +1246,7 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     if dt is None:
         raise TypeError(f"{what}: dtype {dtype} (bfloat16, float16 or float32)")
     shape, groups, cdt = _kv_shape(what, keys, bits, group_size)
+    _no_autograd(what, *keys[1:], *values[1:], *(out or ()))
     if out is None:
         k = torch.empty(*shape, dtype=dtype, device=dev)
         v = torch.empty_like(k)

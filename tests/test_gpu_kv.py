@@ -237,3 +237,19 @@ def test_heads_past_the_kernel(dev):
     for got, want in zip(keys, quantize_rows(x, 8, 64, torch.bfloat16)):
         assert torch.equal(got, want)
     assert not fast.read_back_kernel(x, keys, values, 8, 64)
+
+
+def test_a_cache_that_records(dev):
+    """Scales and biases with gradients: neither written nor read back without them."""
+    from dspark_rocm import ops
+
+    x = torch.zeros(1, 2, 3, 64, dtype=torch.bfloat16, device=dev)
+    t, u = (cache(1, 2, 3, 64, 8, torch.bfloat16, dev) for _ in range(2))
+    for i in (1, 2):
+        grad = tuple(a.clone().requires_grad_() if j == i else a for j, a in enumerate(t))
+        for call in (lambda: ops.quantize_kv(x, x, grad, u, bits=8), lambda: ops.quantize_kv(x, x, u, grad, bits=8),
+                     lambda: ops.dequantize_kv(grad, u, bits=8), lambda: ops.dequantize_kv(u, grad, bits=8)):
+            with pytest.raises(ValueError, match="backward"):
+                call()
+        with torch.no_grad():
+            assert torch.equal(ops.dequantize_kv(grad, u, bits=8)[0], ops.dequantize_kv(t, u, bits=8)[0])

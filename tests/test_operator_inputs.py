@@ -1,0 +1,72 @@
+"""CPU: tensors whose values are not what lies at their address, or that autograd follows, at the operators without a
+backward pass. The launches are left out: what is refused is refused on the host before them."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from dspark_rocm import ops
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The operators' host code on CPU tensors; the calls that would have been made."""
+    calls = []
+    monkeypatch.setattr(ops, "_one_device", lambda what, first, *ts: first.device)
+    monkeypatch.setattr(ops, "_call_on", lambda dev, name, args: calls.append(name))
+    return calls
+
+
+def _triple(dtype=torch.bfloat16):
+    return [torch.zeros(1, 2, 3, 16, dtype=torch.int32), torch.zeros(1, 2, 3, 1, dtype=dtype), torch.zeros(1, 2, 3, 1, dtype=dtype)]
+
+
+def _probs(logits, out):
+    ops.sampling_probs(logits, out=out)
+
+
+def _verify(logits, draft_probs):
+    ops.speculative_verify(logits, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 3), draft_probs=draft_probs)
+
+
+def _rope(q, k, freqs, q_out, k_out):
+    ops.rope(q, k, freqs, 3, q_out=q_out, k_out=k_out)
+
+
+def _quantize(keys, values, ks, kb, vs, vb):
+    (kw, _, _), (vw, _, _) = _triple(), _triple()
+    ops.quantize_kv(keys, values, (kw, ks, kb), (vw, vs, vb), bits=8)
+
+
+def _dequantize(ks, kb, vs, vb, k_out, v_out):
+    (kw, _, _), (vw, _, _) = _triple(), _triple()
+    ops.dequantize_kv((kw, ks, kb), (vw, vs, vb), bits=8, out=(k_out, v_out))
+
+
+def _inputs():
+    """Each operator with the tensors whose gradients it would have."""
+    head = lambda: torch.zeros(1, 2, 3, 64)
+    scale = lambda: torch.zeros(1, 2, 3, 1, dtype=torch.bfloat16)
+    return [(_probs, dict(logits=torch.zeros(2, 9, dtype=torch.bfloat16), out=torch.zeros(2, 9))),
+            (_verify, dict(logits=torch.zeros(2, 3, 9, dtype=torch.float16), draft_probs=torch.zeros(2, 2, 9))),
+            (_rope, dict(q=head(), k=head(), freqs=torch.zeros(32, dtype=torch.float64), q_out=head(), k_out=head())),
+            (_quantize, dict(keys=head(), values=head(), ks=scale(), kb=scale(), vs=scale(), vb=scale())),
+            (_dequantize, dict(ks=scale(), kb=scale(), vs=scale(), vb=scale(), k_out=head(), v_out=head()))]
+
+
+EACH = [(i, name) for i, (_, kw) in enumerate(_inputs()) for name in kw]
+
+
+@pytest.mark.parametrize("i,name", EACH)
+def test_gradients_are_not_dropped(host, i, name):
+    call, kw = _inputs()[i]
+    call(**kw)
+    assert len(host) == 1
+    kw[name].requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        call(**kw)
+    assert len(host) == 1
+    with torch.no_grad():
+        call(**kw)
+    assert len(host) == 2
