@@ -713,6 +713,7 @@ class Target:
         if draft_probs is not None and (draft_probs.dtype != torch.float32 or tuple(draft_probs.shape) != (m, V)
                                         or draft_probs.requires_grad):
             raise ValueError(f"draft_probs: fp32 [{m}, {V}] without gradients, got {draft_probs.dtype} {list(draft_probs.shape)}")
+        ops._no_autograd("sampled_round", draft_probs)
         ops.check_sampler(temperature, top_k, top_p)
         if not ops.sampling_workspace_bytes(M, V, 1):
             raise ValueError(f"a vocabulary of {V} (up to 524280)")

@@ -11,6 +11,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -896,10 +897,16 @@ def _call_on(dev: torch.device, name: str, args: bytes) -> None:
 
 
 def _no_autograd(what: str, *ts) -> None:
+    """ValueError where autograd follows one of the tensors: gradients while they are recorded, tangents always
+    (forward mode asks neither for requires_grad nor for grad mode)."""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: has no backward pass; detach its inputs or use torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:       # without that name every tensor is asked
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what}: has no derivative for a tangent; take the primal of its inputs")
 
 
 def _one_device(what: str, first: torch.Tensor, *ts) -> torch.device:

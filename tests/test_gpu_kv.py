@@ -253,3 +253,26 @@ def test_a_cache_that_records(dev):
                 call()
         with torch.no_grad():
             assert torch.equal(ops.dequantize_kv(grad, u, bits=8)[0], ops.dequantize_kv(t, u, bits=8)[0])
+
+
+def test_tangents(dev):
+    """Duals are refused by the operators; the cache and the stock attention keep the torch ops for them."""
+    from torch.autograd import forward_ad
+
+    from dspark_rocm import fast, ops
+    from dspark_rocm.kv_cache import QuantizedKVCache
+
+    g = torch.Generator().manual_seed(0)
+    rows = [torch.randn(1, 2, 30, 64, generator=g).to(dev) for _ in range(2)]
+    q = torch.randn(1, 2, 3, 64, generator=g).to(dev)
+    t, u = (cache(1, 2, 30, 64, 8, torch.bfloat16, dev) for _ in range(2))
+    c = QuantizedKVCache(1, 2, 64, bits=8, device=dev)
+    keys, values = c.update_and_fetch(*rows)
+    attend = lambda q: fast.quantized_scaled_dot_product_attention(q, keys, values, scale=0.125, bits=8)
+    want = attend(q)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(rows[0], torch.ones_like(rows[0]))
+        with pytest.raises(ValueError, match="tangent"):
+            ops.quantize_kv(dual, rows[1], t, u, bits=8)
+        out = forward_ad.unpack_dual(attend(forward_ad.make_dual(q, torch.ones_like(q))))
+        assert torch.equal(out.primal, want) and bool(out.tangent.abs().sum() > 0)

@@ -70,3 +70,56 @@ def test_gradients_are_not_dropped(host, i, name):
     with torch.no_grad():
         call(**kw)
     assert len(host) == 2
+
+
+@pytest.mark.parametrize("i,name", EACH)
+def test_tangents_are_not_dropped(host, i, name):
+    """Forward mode does not ask for requires_grad, nor for grad mode."""
+    from torch.autograd import forward_ad
+
+    call, kw = _inputs()[i]
+    with forward_ad.dual_level():
+        call(**kw)                      # a level alone is no tangent
+        assert len(host) == 1
+        plain = kw[name]
+        kw[name] = forward_ad.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(ValueError, match="tangent"):
+            call(**kw)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+            call(**kw)
+        assert len(host) == 1
+        kw[name] = forward_ad.unpack_dual(kw[name]).primal
+        call(**kw)
+        assert len(host) == 2
+
+
+class _Round:
+    """What Target.sampled_round asks of a target, on the CPU; counts the verify steps."""
+
+    max_rows = 16
+
+    def __init__(self):
+        from types import SimpleNamespace
+
+        self.engine = SimpleNamespace(ids=torch.zeros(16, dtype=torch.int64))
+        self.model = SimpleNamespace(args=SimpleNamespace(vocab_size=9))
+        self.steps = 0
+
+    def verify(self, ids, cache, tap):
+        self.steps += 1
+        return torch.zeros(1, ids.numel(), 9, dtype=torch.bfloat16), None
+
+    def rollback(self, cache, n):
+        pass
+
+
+def test_round_refuses_tangents_before_the_caches_take_rows(host):
+    from dspark_rocm.model import Target
+    from torch.autograd import forward_ad
+
+    r = _Round()
+    with forward_ad.dual_level():
+        q = forward_ad.make_dual(torch.zeros(2, 9), torch.ones(2, 9))
+        with pytest.raises(ValueError):
+            Target.sampled_round(r, 3, [1, 2], [], draft_probs=q)
+    assert not r.steps
