@@ -896,6 +896,11 @@ def _call_on(dev: torch.device, name: str, args: bytes) -> None:
             _lib.call(name, args, torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _forward_level() -> bool:
+    """Whether tensors may have tangents (without the name torch keeps to itself: every one is asked)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def _no_autograd(what: str, *ts) -> None:
     """ValueError where autograd follows one of the tensors: gradients while they are recorded, tangents always
     (forward mode asks neither for requires_grad nor for grad mode)."""
@@ -903,10 +908,18 @@ def _no_autograd(what: str, *ts) -> None:
         for t in ts:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: has no backward pass; detach its inputs or use torch.no_grad()")
-    if getattr(forward_ad, "_current_level", 0) >= 0:       # without that name every tensor is asked
+    if _forward_level():
         for t in ts:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError(f"{what}: has no derivative for a tangent; take the primal of its inputs")
+
+
+def _as_stored(what: str, *ts) -> None:
+    """ValueError for a view that negates its memory where it is read: what a kernel writes there, or reads as a cache,
+    is the memory itself. (Plain inputs of this kind are copied: resolve_neg.)"""
+    for t in ts:
+        if t is not None and t.is_neg():
+            raise ValueError(f"{what}: a view that negates its memory; take its resolve_neg()")
 
 
 def _one_device(what: str, first: torch.Tensor, *ts) -> torch.device:
@@ -966,6 +979,8 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"sampling_probs: logits {list(shape)}")
     _no_autograd("sampling_probs", logits, out)
+    if logits.is_neg():
+        logits = logits.resolve_neg()
     t, k, p = check_sampler(temperature, top_k, top_p)
     V = shape[-1]
     x = logits if len(shape) == 2 else logits.reshape(-1, V)
@@ -976,6 +991,8 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
         out = torch.empty(shape, dtype=torch.float32, device=dev)
     elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"sampling_probs: out must be contiguous fp32 {list(shape)}")
+    else:
+        _as_stored("sampling_probs", out)
     if rows:
         ws = _sampling_workspace(workspace, dev, rows, V, 0)
         _call_on(dev, "dspark_sampling_probs",
@@ -1022,31 +1039,34 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
     m = R - 1
     if m > 255:
         raise ValueError(f"{what}: {m} drafts (up to 255)")
-    u64 = uniforms.dtype is torch.float64
-    if not (u64 or uniforms.dtype is torch.float32) or uniforms.shape != (B, R):
+    udt = uniforms.dtype
+    u64 = udt is torch.float64
+    if not (u64 or udt is torch.float32) or uniforms.shape != (B, R):
         raise ValueError(f"{what}: uniforms must be fp32 or fp64 [{B}, {R}], got {uniforms.dtype} {list(uniforms.shape)}")
     t, k, p = check_sampler(temperature, top_k, top_p)
+    _no_autograd(what, logits, draft_probs)
     draft = _ints(what, "draft", draft, (B, m))
     q = q_seq = q_row = 0
     if draft_probs is not None:
         if draft_probs.dtype is not torch.float32 or draft_probs.shape != (B, m, V):
             raise ValueError(f"{what}: draft_probs must be fp32 [{B}, {m}, {V}], got {draft_probs.dtype} {list(draft_probs.shape)}")
-        _no_autograd(what, draft_probs)
         q_seq, q_row, unit = draft_probs.stride()
-        if unit != 1 and V > 1:
-            draft_probs = draft_probs.contiguous()
+        if (unit != 1 and V > 1) or draft_probs.is_neg():
+            draft_probs = draft_probs.resolve_neg().contiguous()
             q_seq, q_row, _ = draft_probs.stride()
         q = draft_probs.data_ptr()
-    _no_autograd(what, logits)
+        if not q and draft_probs.numel():
+            raise ValueError(f"{what}: draft_probs without memory")
     lens = 0
     if draft_lens is not None:
         draft_lens = _ints(what, "draft_lens", draft_lens, (B,))
         lens = draft_lens.data_ptr()
     ld_seq, ld_row, unit = logits.stride()
-    if unit != 1 and V > 1:
-        logits = logits.contiguous()
+    if (unit != 1 and V > 1) or logits.is_neg():
+        logits = logits.resolve_neg().contiguous()
         ld_seq, ld_row, _ = logits.stride()
-    uniforms = uniforms.contiguous()
+    if uniforms.is_neg() or not uniforms.is_contiguous():
+        uniforms = uniforms.resolve_neg().contiguous()
     n = torch.empty(B, dtype=torch.int32, device=dev)
     tokens = torch.empty(B, R, dtype=torch.int32, device=dev)
     draft_p = torch.empty(B, m, dtype=torch.float32, device=dev)
@@ -1083,6 +1103,7 @@ def _distinct(what: str, *at: int) -> None:
 
 
 def _check_rope_out(name: str, x: torch.Tensor, out: torch.Tensor) -> None:
+    _as_stored("rope", out)
     if out.dtype != x.dtype or out.shape != x.shape or out.stride(3) != 1:
         raise ValueError(f"rope: {name} must be {x.dtype} {list(x.shape)} with unit last stride")
     _no_repeats("rope", out)
@@ -1111,30 +1132,33 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
     dt = ROPE_DTYPES.get(dtype)
     if dt is None or (k is not None and k.dtype is not dtype):
         raise TypeError(f"rope: q {dtype}, k {None if k is None else k.dtype} (one of bfloat16, float16, float32)")
-    if q.dim() != 4 or (k is not None and k.dim() != 4):
-        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(q.shape)} and {None if k is None else list(k.shape)}")
-    B, Hq, L, D = q.shape
+    q_shape, k_shape = q.shape, None if k is None else k.shape
+    if len(q_shape) != 4 or (k_shape is not None and len(k_shape) != 4):
+        raise ValueError(f"rope: q and k must be [B, H, L, D], got {list(q_shape)} and {None if k is None else list(k_shape)}")
+    B, Hq, L, D = q_shape
     Hk = 0
     if k is not None:
-        Bk, Hk, Lk, Dk = k.shape
+        Bk, Hk, Lk, Dk = k_shape
         if Bk != B or Lk != L or Dk != D:
-            raise ValueError(f"rope: q {list(q.shape)} and k {list(k.shape)}")
+            raise ValueError(f"rope: q {list(q_shape)} and k {list(k_shape)}")
     elif k_out is not None:
         raise ValueError("rope: k_out without k")
-    half = freqs.numel()
-    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not 1 <= half <= min(128, D // 2):
-        raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(freqs.shape)}")
+    f_shape = freqs.shape
+    half = f_shape[0] if len(f_shape) == 1 else 0
+    if freqs.dtype is not torch.float64 or not 1 <= half <= min(128, D // 2):
+        raise ValueError(f"rope: freqs must be fp64 [dims / 2], dims up to the head dim and 256, got {freqs.dtype} {list(f_shape)}")
     _no_autograd("rope", q, k, freqs, q_out, k_out)
-    freqs = freqs.contiguous()
+    if freqs.is_neg() or not freqs.is_contiguous():
+        freqs = freqs.resolve_neg().contiguous()
     pos, pos64, pb, pl, pos0 = 0, 0, 0, 0, 0
     if tensor:
-        pos64 = positions.dtype is torch.int64
-        axes = positions.dim()
-        if not (pos64 or positions.dtype is torch.int32) or not 1 <= axes <= 2:
-            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L], got {positions.dtype} {list(positions.shape)}")
-        nb, nl = positions.shape if axes == 2 else (1, positions.shape[0])
+        pdt, p_shape = positions.dtype, positions.shape
+        pos64 = pdt is torch.int64
+        if not (pos64 or pdt is torch.int32) or not 1 <= len(p_shape) <= 2:
+            raise ValueError(f"rope: positions must be int32 or int64 [L] or [B, L], got {pdt} {list(p_shape)}")
+        nb, nl = p_shape if len(p_shape) == 2 else (1, p_shape[0])
         if nl not in (1, L) or nb not in (1, B):
-            raise ValueError(f"rope: positions {list(positions.shape)} for {B} sequences of {L} rows")
+            raise ValueError(f"rope: positions {list(p_shape)} for {B} sequences of {L} rows")
         pos, st = positions.data_ptr(), positions.stride()
         pl = st[-1] if nl > 1 else 0
         pb = st[0] if nb > 1 else 0
@@ -1143,30 +1167,33 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
         if abs(pos0) >= 1 << 52:
             raise ValueError(f"rope: position {pos0}")
     s0, s1, s2, unit = q.stride()
-    if unit != 1:
-        q = q.contiguous()
+    if unit != 1 or q.is_neg():
+        q = q.resolve_neg().contiguous()
         s0, s1, s2, _ = q.stride()
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        o0, o1, o2 = Hq * L * D, L * D, D
     else:
         _check_rope_out("q_out", q, q_out)
-    o0, o1, o2, _ = q_out.stride()
+        o0, o1, o2, _ = q_out.stride()
     at_q, at_qo = q.data_ptr(), q_out.data_ptr()
     keys = _NO_KEYS
     if k is not None:
         k0, k1, k2, unit = k.stride()
-        if unit != 1:
-            k = k.contiguous()
+        if unit != 1 or k.is_neg():
+            k = k.resolve_neg().contiguous()
             k0, k1, k2, _ = k.stride()
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            ko = (Hk * L * D, L * D, D)
         else:
             _check_rope_out("k_out", k, k_out)
+            ko = k_out.stride()[:3]
         if B and L and Hk:
             at_k, at_ko = k.data_ptr(), k_out.data_ptr()
             if Hq and (at_ko == at_qo or at_ko == at_q or at_qo == at_k):
                 raise ValueError("rope: the same rows given twice")
-            keys = (at_k, at_ko, k0, k1, k2, *k_out.stride()[:3], Hk)
+            keys = (at_k, at_ko, k0, k1, k2, *ko, Hk)
     if B and L and (Hq or Hk):
         _call_on(dev, "dspark_rope",
                  _ROPE_ARGS.pack(dt, at_q, at_qo, s0, s1, s2, o0, o1, o2, Hq, *keys, B, L, D, 2 * half, bool(interleaved),
@@ -1178,15 +1205,21 @@ KV_CACHE_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _KV_ARGS = struct.Struct("=34q")
 
 
-def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple, cache_dtype, written: bool) -> tuple:
-    """The fields of one ``dspark_kv_side``: plain rows x and the (words, scales, biases) they belong to."""
+def _kv_side(what: str, at: int, strides: tuple, trip, words: torch.Size, groups: tuple, cache_dtype, dual: bool,
+             written: bool) -> tuple:
+    """The fields of one ``dspark_kv_side``: plain rows at ``at`` and the (words, scales, biases) they belong to (words
+    None: its shape is where the sizes came from)."""
     w, s, b = trip
     if w.dtype is not torch.int32:
         _require_packed(w)
     if s.dtype is not cache_dtype or b.dtype is not cache_dtype:
         raise TypeError(f"{what}: scales and biases of {cache_dtype}, {s.dtype} and {b.dtype}")
-    if w.shape != words or s.shape != groups or b.shape != groups:
+    if (words is not None and w.shape != words) or s.shape != groups or b.shape != groups:
         raise ValueError(f"{what}: words {list(w.shape)}, scales {list(s.shape)}, biases {list(b.shape)}")
+    if s.requires_grad or b.requires_grad or dual:
+        _no_autograd(what, s, b)
+    if s.is_neg() or b.is_neg():
+        _as_stored(what, s, b)
     w0, w1, w2, w3 = w.stride()
     s0, s1, s2, s3 = s.stride()
     b0, b1, b2, b3 = b.stride()
@@ -1195,26 +1228,37 @@ def _kv_side(what: str, x: torch.Tensor, trip, words: torch.Size, groups: tuple,
     if written and not (w0 and w1 and w2 and s0 and s1 and s2):
         for t in trip:
             _no_repeats(what, t)
-    x0, x1, x2, _ = x.stride()
-    return x.data_ptr(), x0, x1, x2, w.data_ptr(), s.data_ptr(), b.data_ptr(), w0, w1, w2, s0, s1, s2
+    x0, x1, x2, _ = strides
+    return at, x0, x1, x2, w.data_ptr(), s.data_ptr(), b.data_ptr(), w0, w1, w2, s0, s1, s2
 
 
 def _kv_shape(what: str, keys, bits: int, group_size: int):
-    """((B, H, T, D), shape of the scales, their type) of a triple of cache views."""
+    """((B, H, T, D), shape of the words, of the scales, type of these) of a triple of cache views."""
     if bits not in KV_BITS or group_size != GROUP:
         raise ValueError(f"{what}: bits={bits} (4 or 8), group_size={group_size} (64)")
-    kw = keys[0]
-    if kw.dim() != 4:
-        raise ValueError(f"{what}: words must be [B, H, rows, D * bits / 32], got {list(kw.shape)}")
-    B, H, T, W = kw.shape
+    kw, ks, _ = keys
+    words = kw.shape
+    if len(words) != 4:
+        raise ValueError(f"{what}: words must be [B, H, rows, D * bits / 32], got {list(words)}")
+    B, H, T, W = words
     D = W * 32 // bits
     if D % GROUP or D == 0:
-        raise ValueError(f"{what}: words {list(kw.shape)} at {bits} bits")
-    if keys[1].dtype not in KV_CACHE_DTYPES:
-        raise TypeError(f"{what}: scales {keys[1].dtype} (bfloat16 or float16)")
+        raise ValueError(f"{what}: words {list(words)} at {bits} bits")
+    cdt = ks.dtype
+    if cdt not in KV_CACHE_DTYPES:
+        raise TypeError(f"{what}: scales {cdt} (bfloat16 or float16)")
     if 2 * B * H > 65535:
         raise ValueError(f"{what}: {B} x {H} heads (up to 32767)")
-    return (B, H, T, D), (B, H, T, D // GROUP), keys[1].dtype
+    return (B, H, T, D), words, (B, H, T, D // GROUP), cdt
+
+
+def _kv_rows(t: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """Plain rows as a kernel reads them (a copy where the last stride is not 1 or the memory is negated), their strides."""
+    st = t.stride()
+    if st[3] != 1 or t.is_neg():
+        t = t.resolve_neg().contiguous()
+        st = t.stride()
+    return t, st
 
 
 def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bits: int, group_size: int = GROUP) -> None:
@@ -1224,21 +1268,22 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     bit (a group with a NaN gets a NaN scale and bias), both tensors in one launch."""
     what = "quantize_kv"
     dev = _one_device(what, keys, values, *k_rows, *v_rows)
-    dt = DEQUANT_DTYPES.get(keys.dtype)
-    if dt is None or values.dtype != keys.dtype:
-        raise TypeError(f"{what}: rows {keys.dtype} and {values.dtype} (one of bfloat16, float16, float32)")
-    (B, H, T, D), groups, cdt = _kv_shape(what, k_rows, bits, group_size)
-    if keys.shape != (B, H, T, D) or values.shape != keys.shape:
-        raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)} for rows [{B}, {H}, {T}, {D}]")
-    _no_autograd(what, keys, values, *k_rows[1:], *v_rows[1:])
-    if keys.stride(3) != 1:
-        keys = keys.contiguous()
-    if values.stride(3) != 1:
-        values = values.contiguous()
-    words = k_rows[0].shape
-    args = (dt, KV_CACHE_DTYPES[cdt], B, H, T, D, bits, group_size, *_kv_side(what, keys, k_rows, words, groups, cdt, True),
-            *_kv_side(what, values, v_rows, words, groups, cdt, True))
-    if B * H * T:
+    xdt = keys.dtype
+    dt = DEQUANT_DTYPES.get(xdt)
+    if dt is None or values.dtype != xdt:
+        raise TypeError(f"{what}: rows {xdt} and {values.dtype} (one of bfloat16, float16, float32)")
+    shape, words, groups, cdt = _kv_shape(what, k_rows, bits, group_size)
+    if keys.shape != shape or values.shape != shape:
+        raise ValueError(f"{what}: keys {list(keys.shape)}, values {list(values.shape)} for rows {list(shape)}")
+    dual = _forward_level()
+    if dual or keys.requires_grad or values.requires_grad:
+        _no_autograd(what, keys, values)
+    keys, k_st = _kv_rows(keys)
+    values, v_st = _kv_rows(values)
+    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size,
+            *_kv_side(what, keys.data_ptr(), k_st, k_rows, None, groups, cdt, dual, True),
+            *_kv_side(what, values.data_ptr(), v_st, v_rows, words, groups, cdt, dual, True))
+    if shape[0] * shape[1] * shape[2]:
         _distinct(what, *args[12:15], *args[25:28])         # words, scales and biases of both
         _call_on(dev, "dspark_kv_quantize", _KV_ARGS.pack(*args))
 
@@ -1252,21 +1297,26 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     dt = DEQUANT_DTYPES.get(dtype)
     if dt is None:
         raise TypeError(f"{what}: dtype {dtype} (bfloat16, float16 or float32)")
-    shape, groups, cdt = _kv_shape(what, keys, bits, group_size)
-    _no_autograd(what, *keys[1:], *values[1:], *(out or ()))
+    shape, words, groups, cdt = _kv_shape(what, keys, bits, group_size)
     if out is None:
-        k = torch.empty(*shape, dtype=dtype, device=dev)
+        k = torch.empty(shape, dtype=dtype, device=dev)
         v = torch.empty_like(k)
+        k_st = v_st = (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1)
     else:
         k, v = out
+        _no_autograd(what, k, v)
+        _as_stored(what, k, v)
         for t in out:
             if t.dtype != dtype or t.shape != shape or t.stride(3) != 1:
                 raise ValueError(f"{what}: out must be two {dtype} {list(shape)} with unit last stride")
             _no_repeats(what, t)
-    words = keys[0].shape
-    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size, *_kv_side(what, k, keys, words, groups, cdt, False),
-            *_kv_side(what, v, values, words, groups, cdt, False))
+        k_st, v_st = k.stride(), v.stride()
+        if shape[0] * shape[1] * shape[2]:
+            _distinct(what, k.data_ptr(), v.data_ptr())
+    dual = _forward_level()
+    args = (dt, KV_CACHE_DTYPES[cdt], *shape, bits, group_size,
+            *_kv_side(what, k.data_ptr(), k_st, keys, None, groups, cdt, dual, False),
+            *_kv_side(what, v.data_ptr(), v_st, values, words, groups, cdt, dual, False))
     if shape[0] * shape[1] * shape[2]:
-        _distinct(what, k.data_ptr(), v.data_ptr())
         _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v

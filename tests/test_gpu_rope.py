@@ -149,3 +149,16 @@ def test_stream_and_graph(dev):
         want = ops.rope(q, k, f, pos)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(z, want))
+
+
+def test_negated_views(dev):
+    """The imaginary part of a conjugate, and one whose memory could be read as it lies: their values are rotated."""
+    from dspark_rocm import ops, rope
+
+    g = torch.Generator().manual_seed(6)
+    f = rope.frequencies(64, 1e4, device=dev)[0]
+    z = torch.randn(1, 2, 3, 64, dtype=torch.complex64, generator=g).to(dev)
+    for q in (z.conj().imag, torch._neg_view(z.imag.clone())):
+        assert q.is_neg()
+        for y in ops.rope(q, q, f, 5):
+            check(-z.imag, y, torch.arange(5, 8)[None], f, False)

@@ -3,6 +3,8 @@ backward pass. The launches are left out: what is refused is refused on the host
 
 from __future__ import annotations
 
+import struct
+
 import pytest
 import torch
 
@@ -123,3 +125,38 @@ def test_round_refuses_tangents_before_the_caches_take_rows(host):
         with pytest.raises(ValueError):
             Target.sampled_round(r, 3, [1, 2], [], draft_probs=q)
     assert not r.steps
+
+
+@pytest.mark.parametrize("i,name", EACH)
+def test_negated_views_are_not_read_as_stored(host, monkeypatch, i, name):
+    """A view that negates when it is read (as the imaginary part of a conjugate is): its memory holds other values.
+    Plain inputs are copied, caches and outputs refused."""
+    fields = []
+    monkeypatch.setattr(ops, "_call_on", lambda dev, name, args: fields.append(struct.unpack(f"={len(args) // 8}q", args)))
+    call, kw = _inputs()[i]
+    call(**kw)
+    assert kw[name].data_ptr() in fields[0]
+    view = kw[name] = torch._neg_view(kw[name])
+    if name in ("logits", "draft_probs", "q", "k", "freqs", "keys", "values"):
+        call(**kw)
+        assert len(fields) == 2 and view.data_ptr() not in fields[1]
+    else:
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call(**kw)
+        assert len(fields) == 1
+
+
+def test_negated_uniforms(host, monkeypatch):
+    fields = []
+    monkeypatch.setattr(ops, "_call_on", lambda dev, name, args: fields.append(struct.unpack(f"={len(args) // 8}q", args)))
+    u = torch.full((2, 3), -0.25)
+    for v in (u, torch._neg_view(u)):
+        ops.speculative_verify(torch.zeros(2, 3, 9, dtype=torch.float16), torch.zeros(2, 2, dtype=torch.int32), v)
+    assert u.data_ptr() in fields[0] and u.data_ptr() not in fields[1]
+
+
+def test_zero_tensors_have_no_address(host):
+    """A given tensor without memory is not taken for one that was not given."""
+    with pytest.raises(ValueError):
+        _verify(torch.zeros(2, 3, 9, dtype=torch.float16), torch._efficientzerotensor((2, 2, 9)))
+    assert not host
