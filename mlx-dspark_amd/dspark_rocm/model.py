@@ -718,9 +718,10 @@ class Target:
         if not ops.sampling_workspace_bytes(M, V, 1):
             raise ValueError(f"a vocabulary of {V} (up to 524280)")
         probs = None if draft_probs is None else draft_probs.to(dev)[None]
+        uniforms = uniforms.to(dev).reshape(1, M)
         logits, fused = self.verify(torch.tensor([[pending] + list(draft)], dtype=torch.int64), cache, tap)
         _, tokens, _ = ops.speculative_verify(logits, torch.tensor([list(draft)], dtype=torch.int32, device=dev).view(1, m),
-                                              uniforms.to(dev).view(1, M), draft_probs=probs, temperature=temperature,
+                                              uniforms, draft_probs=probs, temperature=temperature,
                                               top_k=top_k, top_p=top_p)
         out = [t for t in tokens[0].tolist() if t >= 0]         # the round's one host read
         n = len(out) - 1

@@ -127,3 +127,15 @@ def test_table_targets_step_as_their_module_path(dev, rope, kv_bits):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(e.logits, got[-1][0])
+
+
+def test_round_takes_uniforms_of_any_strides(dev):
+    """Random numbers that lie in memory in another order than they count in: read in theirs, and the caches advance by
+    the accepted rows."""
+    tgt = _target(dev)
+    draft = torch.randint(0, 512, (15,), generator=torch.Generator().manual_seed(4)).tolist()
+    u = torch.rand(4, 4, generator=torch.Generator().manual_seed(5))
+    a, b = tgt.make_cache(8), tgt.make_cache(8)
+    want = tgt.sampled_round(3, draft, a, uniforms=u.t().reshape(-1).clone(), top_k=50)
+    got = tgt.sampled_round(3, draft, b, uniforms=u.t(), top_k=50)
+    assert got[:2] == want[:2] and a[0].offset == b[0].offset == got[0] + 1

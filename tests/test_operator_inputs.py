@@ -160,3 +160,20 @@ def test_zero_tensors_have_no_address(host):
     with pytest.raises(ValueError):
         _verify(torch.zeros(2, 3, 9, dtype=torch.float16), torch._efficientzerotensor((2, 2, 9)))
     assert not host
+
+
+def test_round_takes_uniforms_of_any_strides(host, monkeypatch):
+    """They are formed before the verify step: one that cannot be viewed as a row would raise behind it, with the rows
+    in the caches."""
+    from dspark_rocm.model import Target
+
+    seen = []
+
+    def accept(logits, draft, uniforms, **kw):
+        seen.append(uniforms)
+        return None, torch.tensor([[4] + [-1] * 15]), None
+
+    monkeypatch.setattr(ops, "speculative_verify", accept)
+    u, r = torch.rand(4, 4), _Round()
+    assert Target.sampled_round(r, 3, [1] * 15, [], uniforms=u.t())[:2] == (0, [4])
+    assert r.steps == 1 and torch.equal(seen[0], u.t().reshape(1, 16))
