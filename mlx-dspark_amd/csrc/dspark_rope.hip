@@ -4,7 +4,8 @@
 // for the pairs (i, i + half) or, interleaved, (2i, 2i + 1) of a head's first 2 half values; the others
 // are copied. cos and sin of a position serve every head of its row: a workgroup forms them once for its
 // rows in LDS. The angle is reduced in fp64, in turns: at position 1e6 an fp32 product is off by 0.06 rad,
-// the fp64 one by 1e-10. The rotation is fp32, rounded once to the tensors' type.
+// the fp64 one by 1e-10; its sine and cosine are fp32, within a few units of their own size also near zero. The rotation
+// is fp32, rounded once to the tensors' type.
 //
 // Bound by the bytes of x and y: 16 bytes a lane and access where addresses and strides allow, else one
 // value.
@@ -36,7 +37,7 @@ struct RopeArgs {
   long pb, pl;                                 // strides of the positions
   long pos0;                                   // without pos: row l stands at pos0 + l
   const double* freqs;
-  float scale;
+  double scale;
 };
 
 template <int DT> struct Elem;
@@ -77,9 +78,14 @@ __device__ __forceinline__ void fill_table(const RopeArgs& a, float2* tab, int r
       p = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : (long)static_cast<const int32_t*>(a.pos)[at];
     }
     const double turns = (double)p * (a.freqs[f] * 0.15915494309189535);
+    const double halves = 2.0 * (turns - __builtin_rint(turns));
+    const float hi = (float)halves;
     float sn, cs;
-    sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &sn, &cs);
-    tab[i] = make_float2(cs * a.scale, sn * a.scale);
+    sincospif(hi, &sn, &cs);
+    // What fp32 leaves of the angle (up to 1e-7 rad: all of a cosine near zero), to first order, and the factor in fp64:
+    // one rounding of each.
+    const double lo = 3.141592653589793 * (halves - (double)hi);
+    tab[i] = make_float2((float)(((double)cs - lo * (double)sn) * a.scale), (float)(((double)sn + lo * (double)cs) * a.scale));
   }
 }
 
@@ -253,7 +259,7 @@ extern "C" int dspark_rope(const dspark_rope_args* p, dspark_stream stream) {
   a.pl = p->position_strides[1];
   a.pos0 = p->pos0;
   a.freqs = p->freqs;
-  a.scale = (float)p->scale;
+  a.scale = p->scale;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dt == DSPARK_DTYPE_BF16) vec ? launch_rope<DSPARK_DTYPE_BF16, 8>(a, inter, s) : launch_rope<DSPARK_DTYPE_BF16, 1>(a, inter, s);
   else if (dt == DSPARK_DTYPE_F16) vec ? launch_rope<DSPARK_DTYPE_F16, 8>(a, inter, s) : launch_rope<DSPARK_DTYPE_F16, 1>(a, inter, s);

@@ -151,6 +151,26 @@ def test_stream_and_graph(dev):
         assert all(torch.equal(a, b) for a, b in zip(z, want))
 
 
+@pytest.mark.parametrize("scale", [1.0, 1.25, 0.1 * np.log(4.0) + 1.0])
+@pytest.mark.parametrize("inter", [False, True])
+def test_small_values_of_a_turn(dev, inter, scale):
+    """Unit vectors in fp32: their turn is the table itself, also where a cosine or sine is near zero. Each is within 4
+    units of its own value (2^-21, the bound of sinpi and cospi), half a step for the rounding after the factor, and the
+    angle: up to 2^13 radians, four roundings of 2^-53 and what an fp32 remainder of the half turns leaves (2^-50): under
+    2^-37 together."""
+    from dspark_rocm import ops, rope
+
+    freqs, _ = rope.frequencies(128, 1e6, device=dev)
+    L = 5000
+    x = torch.zeros(1, 1, L, 128, device=dev)
+    x[..., slice(0, 128, 2) if inter else slice(0, 64)] = 1.0
+    y = ops.rope(x, None, freqs, 0, interleaved=inter, scale=scale)[0][0, 0].double().cpu().numpy()
+    c, s = (y[:, ::2], y[:, 1::2]) if inter else (y[:, :64], y[:, 64:])
+    a = np.arange(L)[:, None].astype(np.longdouble) * freqs.cpu().numpy().astype(np.longdouble)
+    for got, want in ((c, np.cos(a) * scale), (s, np.sin(a) * scale)):
+        assert (np.abs(got - want) <= np.abs(want) * (2.0 ** -21 + 2.0 ** -24) + 2.0 ** -37).all()
+
+
 def test_negated_views(dev):
     """The imaginary part of a conjugate, and one whose memory could be read as it lies: their values are rotated."""
     from dspark_rocm import ops, rope
