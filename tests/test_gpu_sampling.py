@@ -438,3 +438,21 @@ def test_offsets_past_32_bits(dev, kw):
     assert torch.equal(ops.sampling_probs(xs, **kw), ops.sampling_probs(x[:, 0].contiguous().to(dev), **kw))
     del buf, qbuf, qs, xs
     torch.cuda.empty_cache()
+
+
+def test_border_of_two_tokens(dev):
+    """Rows of two logits x < 0 and 0: the first token weighs w = 2^(x c), and is drawn while u (1 + w) < w. With
+    |x c| <= 1/2, w is within 5.2e-16 of itself (3.2e-16 of the interpolation, 1.4e-16 of its steps' roundings, the rest the
+    argument's); in u = w / (1 + w) that counts 0.59 times, beside the roundings of 1 + w, u (1 + w) and u (2.2e-16):
+    5.3e-16. So random numbers 6e-16 beside the border fall on either side."""
+    from dspark_rocm import ops
+
+    x = -torch.arange(0x3C80, 0x3EB1, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    assert float(x.float().min()) > -0.3466
+    logits = torch.stack([x, torch.zeros_like(x)], -1)[:, None].to(dev)
+    w = np.exp(x.double().numpy().astype(np.longdouble))
+    none = torch.zeros(len(x), 0, dtype=torch.int32, device=dev)
+    for side, token in ((-1, 0), (1, 1)):
+        u = (w / (1 + w) * (1 + side * np.longdouble(6e-16))).astype(np.float64)
+        got = ops.speculative_verify(logits, none, torch.from_numpy(u)[:, None].to(dev))[1]
+        assert (got == token).all(), int((got != token).sum())
