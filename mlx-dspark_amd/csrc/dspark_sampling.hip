@@ -1012,7 +1012,8 @@ struct DrawShared {
 };
 
 // The token drawn from row ri of a sequence: the first whose running sum of r passes u times the whole.
-// `rest`: segment sums of r (null: formed here; without a cut, only where r is max(p - q, 0)).
+// `rest`: segment sums of r, by every workgroup of the launch (without a cut, only where r is max(p - q, 0): else they
+// follow from the segments' own).
 template <bool HALF, bool CUT>
 __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r, int seq, int ri, const DrawIn& d,
                                           const double* rest, DrawShared& sh) {
@@ -1035,17 +1036,16 @@ __device__ __forceinline__ int draw_token(const SampleArgs& a, const RowInfo& r,
     __syncthreads();
     const bool f = r.z > 0 && t < a.nseg && key_of_float<HALF>(sm) >= r.thr;
     if (f) sh.list[atomicAdd(&sh.nlist, 1)] = t;
-    sh.sums[t] = rest && t < a.nseg ? __builtin_bit_cast(double, get_far(reinterpret_cast<const uint64_t*>(rest) + t)) : 0;
+    sh.sums[t] = t < a.nseg ? __builtin_bit_cast(double, get_far(reinterpret_cast<const uint64_t*>(rest) + t)) : 0;
     static_assert(kMaxSegs == kRowThreads, "a slot a thread");
     __syncthreads();
   }
   for (int tries = 0; tries < 2; ++tries) {
     if constexpr (CUT) {
-      if (!rest || tries) each_listed<HALF>(a, x, off, sh.list, sh.nlist, [&](int s, const u32x4_t& v) {
+      if (tries) each_listed<HALF>(a, x, off, sh.list, sh.nlist, [&](int s, const u32x4_t& v) {      // p
         double w[8], sum = 0;
-        float q[8] = {};
-        if (mode == kDrawRest) load_q8(d.q, s * kSegVals + 8 * lane - off, a.V, q);
-        rest8<HALF, true>(a, r, inv, v, s * kSegVals + 8 * lane - off, mode, q, d.skip, w);
+        const float q[8] = {};
+        rest8<HALF, true>(a, r, inv, v, s * kSegVals + 8 * lane - off, kDrawRow, q, -1, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += w[j];
         sum = wave_total(sum);
