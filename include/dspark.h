@@ -597,11 +597,15 @@ int dspark_argmax_accept(const void* logits, int64_t ld, int64_t M, int64_t V, c
  *   less than top_p of their mass lies (1: all); out = w / their sum on these, 0 elsewhere. Equal logits
  *   are ordered by index. A row with nothing but -inf and NaN gives zeros.
  * logits bf16 or fp16 [rows, V] (row stride ld, any alignment), V <= 524280, rows <= 65535. Weights and
- * sums are fp64. workspace >= dspark_sampling_workspace(rows, V, 0) bytes, 256-byte aligned, of any content.
+ * sums are fp64. workspace >= dspark_sampling_workspace(rows, V, 0) bytes, or as many as dspark_sampling_workspace_for says
+ * of this sampler, 256-byte aligned, of any content.
  * One call at a time uses it: calls on two streams, or graphs that may run together, need one each.
  * Covers the reference's truncate_probs (sampling.py) with the softmax before it.
  */
 size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences);
+
+/* The same for calls with these settings alone: without the counts (up to 31 MB) that only a mass, or a large top_k, needs. */
+size_t dspark_sampling_workspace_for(int64_t rows, int64_t V, int64_t sequences, int64_t top_k, double top_p);
 
 typedef struct dspark_sampling_probs_args { /* every field is 8 bytes */
   int64_t dtype;
@@ -633,7 +637,7 @@ int dspark_sampling_probs(const dspark_sampling_probs_args* args, dspark_stream 
  * uniforms   [sequences, drafts + 1] in [0, 1), fp32 or (uniforms_f64) fp64; the last one draws the token
  * n_accepted int32 [sequences]; tokens int32 [sequences, drafts + 1]; draft_p fp32 [sequences, drafts]
  *            (p_i(draft_i) of every draft, those after the first refused one too)
- * workspace >= dspark_sampling_workspace(sequences * (drafts + 1), V, sequences) bytes, 256-byte aligned,
+ * workspace >= dspark_sampling_workspace(sequences * (drafts + 1), V, sequences) bytes (or _for this sampler), 256-byte aligned,
  * of any content, one call's at a time. The sampling counterpart of dspark_argmax_accept (generate.py's sampling accept).
  */
 typedef struct dspark_speculative_verify_args { /* every field is 8 bytes */

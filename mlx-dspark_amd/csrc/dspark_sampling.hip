@@ -1415,6 +1415,13 @@ Layout layout(int64_t rows, int64_t V, int64_t sequences) {
 
 constexpr int64_t kMaxVocab = (int64_t)kMaxSegs * kSegVals - 8;
 
+// Whether what is kept may well be more than can be sorted: what the mass alone cuts, a large top_k. Its counting and its
+// draw are then worth more workgroups than one, and a launch each.
+bool many(int top_k) { return !top_k || top_k > kListed / 2; }
+int top_k_of(int64_t top_k, int64_t V) { return top_k < V ? (int)top_k : 0; }
+// Bytes of a layout that a sampler uses: all of it where it counts.
+size_t needed(const Layout& l, int top_k, double top_p) { return (top_k || top_p < 1.0) && many(top_k) ? l.bytes : l.counts; }
+
 bool shape_ok(int64_t rows, int64_t V) { return rows >= 1 && rows <= 65535 && V >= 1 && V <= kMaxVocab; }
 
 // Parts a segment that a top_k's bound goes by, 0 for whole segments. The k-th largest of n maxima is reached by
@@ -1434,7 +1441,8 @@ int sample_args(const char* what, int64_t dtype, const void* logits, int64_t row
   if (!(temperature >= 1e-30 && temperature <= 1e30)) return fail(DSPARK_ERR_ARG, "%s: temperature %g (greedy: argmax_accept)", what, temperature);
   if (!(top_p > 0.0 && top_p <= 1.0) || top_k < 0) return fail(DSPARK_ERR_ARG, "%s: top_k %lld, top_p %g", what, (long long)top_k, top_p);
   if (!aligned(logits, 2) || !aligned(ws, 256)) return fail(DSPARK_ERR_ALIGN, "%s: logits need 2-byte, the workspace 256-byte alignment", what);
-  if (ws_bytes < (int64_t)l.bytes) return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %lld < %zu bytes", what, (long long)ws_bytes, l.bytes);
+  const size_t need = needed(l, top_k_of(top_k, V), top_p);
+  if (ws_bytes < (int64_t)need) return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %lld < %zu bytes", what, (long long)ws_bytes, need);
   char* w = static_cast<char*>(ws);
   a.x = static_cast<const u16*>(logits);
   a.rows = (int)rows;
@@ -1442,7 +1450,7 @@ int sample_args(const char* what, int64_t dtype, const void* logits, int64_t row
   a.nseg = (int)((V + 7 + kSegVals - 1) / kSegVals);
   a.c = 1.4426950408889634 / temperature;
   a.top_p = top_p;
-  a.top_k = top_k < V ? (int)top_k : 0;
+  a.top_k = top_k_of(top_k, V);
   a.parts = bound_parts(a.nseg, a.top_k);
   a.segm = reinterpret_cast<float*>(w + l.segm);
   a.segs = reinterpret_cast<double*>(w + l.segs);
@@ -1469,10 +1477,6 @@ void launch_segments(const SampleArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((sample_segments_kernel<HALF, kSegWave, true>), grid, block, 0, s, a);
 }
 
-// Whether a row may well have more candidates than are sorted: what the mass alone cuts, a large top_k. Its counting
-// and its draw are then worth more workgroups than one, and a launch each.
-bool many(const SampleArgs& a) { return !a.top_k || a.top_k > kListed / 2; }
-
 template <bool HALF>
 void launch_select(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, hipStream_t s) {
   const int group = group_size(a.rows, a.nseg);
@@ -1487,13 +1491,13 @@ void probs(const SampleArgs& a, char* w, const Layout& l, float* out, long ldo, 
   const dim3 block(kStatThreads);
   const dim3 grid((unsigned)a.rows), row(kRowThreads);
   const bool cut = a.top_k || a.top_p < 1.0;
-  if (cut && !many(a) && a.nseg <= kWholeSegs) {
+  if (cut && !many(a.top_k) && a.nseg <= kWholeSegs) {
     hipLaunchKernelGGL((sample_whole_kernel<HALF>), grid, row, 0, s, a, out, ldo);
     return;
   }
   launch_segments<HALF>(a, s);
   if (cut) {
-    if (many(a)) launch_select<HALF>(a, VerifyIn{}, w, l, s);
+    if (many(a.top_k)) launch_select<HALF>(a, VerifyIn{}, w, l, s);
     else hipLaunchKernelGGL((sample_few_kernel<HALF>), grid, row, 0, s, a, reinterpret_cast<uint64_t*>(w + l.info));
     hipLaunchKernelGGL((sample_probs_kernel<HALF, true, kProbCutWave>), dim3(groups(a.nseg, kProbCutWave), (unsigned)a.rows),
                        block, 0, s, a, info, out, ldo);
@@ -1512,13 +1516,13 @@ void verify(const SampleArgs& a, const VerifyIn& in, char* w, const Layout& l, h
   // over the rows that are drawn from, a workgroup a CU, at most one a wave and segment
   const unsigned most = (unsigned)((a.nseg + kRowWaves - 1) / kRowWaves), fill = B < 256 ? 256 / B : 1;
   const unsigned spread = most < fill ? most : fill;
-  if (cut && !many(a) && a.per == 1 && a.nseg <= kWholeSegs) {
+  if (cut && !many(a.top_k) && a.per == 1 && a.nseg <= kWholeSegs) {
     hipLaunchKernelGGL((sample_cut_kernel<HALF, true>), dim3(1, B), dim3(kRowThreads), 0, s, a, in,
                        reinterpret_cast<uint64_t*>(w + l.drawn));
     return;
   }
   launch_segments<HALF>(a, s);
-  if (cut && many(a)) {
+  if (cut && many(a.top_k)) {
     launch_select<HALF>(a, in, w, l, s);
     hipLaunchKernelGGL((sample_spread_kernel<HALF, true>), dim3(spread, B), dim3(kRowThreads), 0, s, a, in, info, rest);
   } else if (cut) {
@@ -1538,6 +1542,11 @@ using namespace dspark;
 extern "C" size_t dspark_sampling_workspace(int64_t rows, int64_t V, int64_t sequences) {
   if (!shape_ok(rows, V) || sequences < 0 || sequences > rows) return 0;
   return layout(rows, V, sequences ? sequences : rows).bytes;
+}
+
+extern "C" size_t dspark_sampling_workspace_for(int64_t rows, int64_t V, int64_t sequences, int64_t top_k, double top_p) {
+  if (!shape_ok(rows, V) || sequences < 0 || sequences > rows) return 0;
+  return needed(layout(rows, V, sequences ? sequences : rows), top_k_of(top_k, V), top_p);
 }
 
 extern "C" int dspark_sampling_probs(const dspark_sampling_probs_args* p, dspark_stream stream) {

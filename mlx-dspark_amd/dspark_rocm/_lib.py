@@ -184,6 +184,7 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_argmax_accept": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
                                      c_size_t, c_void_p]),
     "dspark_sampling_workspace": (c_size_t, [c_i64, c_i64, c_i64]),
+    "dspark_sampling_workspace_for": (c_size_t, [c_i64, c_i64, c_i64, c_i64, ctypes.c_double]),
     # args: the bytes of the struct of 8-byte fields (include/dspark.h)
     "dspark_sampling_probs": (c_int, [c_char_p, c_void_p]),
     "dspark_speculative_verify": (c_int, [c_char_p, c_void_p]),

@@ -942,8 +942,8 @@ def check_sampler(temperature, top_k, top_p) -> tuple[float, int, float]:
     return t, k, p
 
 
-def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> torch.Tensor:
-    nbytes = sampling_workspace_bytes(rows, vocab, sequences)
+def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int, top_k: int, top_p: float) -> torch.Tensor:
+    nbytes = sampling_workspace_bytes(rows, vocab, sequences, top_k, top_p)
     if nbytes == 0:
         raise ValueError(f"{rows} rows of {vocab} logits (up to 65535 rows of 524280)")
     if ws is None:
@@ -954,10 +954,13 @@ def _sampling_workspace(ws, device, rows: int, vocab: int, sequences: int) -> to
 
 
 @functools.lru_cache(maxsize=256)
-def sampling_workspace_bytes(rows: int, vocab: int, sequences: int = 0) -> int:
+def sampling_workspace_bytes(rows: int, vocab: int, sequences: int = 0, top_k: int | None = None, top_p: float = 1.0) -> int:
     """Workspace bytes of :func:`sampling_probs` over ``rows`` rows, or of :func:`speculative_verify`
-    over ``sequences`` sequences of ``rows`` rows together."""
-    return int(_lib.load().dspark_sampling_workspace(rows, vocab, sequences))
+    over ``sequences`` sequences of ``rows`` rows together: with any settings, or (``top_k`` given) with these."""
+    lib = _lib.load()
+    if top_k is None:
+        return int(lib.dspark_sampling_workspace(rows, vocab, sequences))
+    return int(lib.dspark_sampling_workspace_for(rows, vocab, sequences, top_k, top_p))
 
 
 _PROBS_ARGS = struct.Struct("=5qdqd4q")
@@ -994,7 +997,7 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     else:
         _as_stored("sampling_probs", out)
     if rows:
-        ws = _sampling_workspace(workspace, dev, rows, V, 0)
+        ws = _sampling_workspace(workspace, dev, rows, V, 0, k, p)
         _call_on(dev, "dspark_sampling_probs",
                  _PROBS_ARGS.pack(dt, x.data_ptr(), ld, rows, V, t, k, p, out.data_ptr(), V, ws.data_ptr(), ws.nbytes))
     return out
@@ -1071,7 +1074,7 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
     tokens = torch.empty(B, R, dtype=torch.int32, device=dev)
     draft_p = torch.empty(B, m, dtype=torch.float32, device=dev)
     if B:
-        ws = _sampling_workspace(workspace, dev, B * R, V, B)
+        ws = _sampling_workspace(workspace, dev, B * R, V, B, k, p)
         _call_on(dev, "dspark_speculative_verify",
                  _VERIFY_ARGS.pack(dt, logits.data_ptr(), ld_seq, ld_row, B, m, V, draft.data_ptr(), q, q_seq, q_row, lens,
                                    uniforms.data_ptr(), u64, t, k, p, n.data_ptr(), tokens.data_ptr(), draft_p.data_ptr(),

@@ -456,3 +456,28 @@ def test_border_of_two_tokens(dev):
         u = (w / (1 + w) * (1 + side * np.longdouble(6e-16))).astype(np.float64)
         got = ops.speculative_verify(logits, none, torch.from_numpy(u)[:, None].to(dev))[1]
         assert (got == token).all(), int((got != token).sum())
+
+
+@pytest.mark.parametrize("kw", CUTS + [dict(top_k=128, top_p=0.9), dict(top_k=129), dict(top_k=10 ** 6)])
+def test_a_workspace_for_the_sampler(dev, kw):
+    """As much as its sampler needs, between guards that stay as they were: the results of a workspace for any."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(11)
+    B, m, V = 5, 3, 50257
+    x = rows(g, B * (m + 1), V, torch.bfloat16).view(B, m + 1, V)
+    d, q = _drafts(g, x, "plain", m)
+    args = x.to(dev), d.to(dev), torch.rand(B, m + 1, generator=g).to(dev)
+    q, k, p = q.to(dev), kw.get("top_k", 0), kw.get("top_p", 1.0)
+    calls = [(0, lambda ws: (ops.sampling_probs(args[0].view(-1, V), workspace=ws, **kw),)),
+             (B, lambda ws: ops.speculative_verify(*args, draft_probs=q, workspace=ws, **kw)),
+             (B, lambda ws: ops.speculative_verify(*args, workspace=ws, **kw))]
+    for seqs, call in calls:
+        need, most = (ops.sampling_workspace_bytes(B * (m + 1), V, seqs, *s) for s in ((k, p), ()))
+        want = call(torch.full((most,), 0xFF, dtype=torch.uint8, device=dev))
+        buf = torch.full((need + 512,), 0xA5, dtype=torch.uint8, device=dev)
+        got = call(buf[256:256 + need])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert (buf[:256] == 0xA5).all() and (buf[256 + need:] == 0xA5).all()
+        with pytest.raises(ValueError):
+            call(buf[256:255 + need])

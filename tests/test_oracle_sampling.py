@@ -117,3 +117,27 @@ def test_speculative_verify_refuses_odd_addresses(at):
               lib.dspark_sampling_workspace(8, 100, 2)]
     fields[at] = fake + 2
     assert lib.dspark_speculative_verify(ops._VERIFY_ARGS.pack(*fields), None) == -3
+
+
+@pytest.mark.parametrize("rows,V,per", [(1, 151936, 1), (16, 151936, 16), (20, 50257, 4), (256, 151936, 8), (3, 1000, 1)])
+def test_workspace_of_a_sampler(rows, V, per):
+    """Only what cuts by a mass, or by a top_k that is counted, needs room for counts; a call with less is refused."""
+    from dspark_rocm import ops
+
+    lib = _lib()
+    fake = 1 << 20
+    for seqs in (0, rows // per):
+        most = lib.dspark_sampling_workspace(rows, V, seqs)
+        for k, p in ((0, 1.0), (1, 1.0), (20, 0.9), (128, 0.5), (V, 1.0), (1 << 31, 1.0), (0, 0.9), (129, 1.0), (700, 0.9), (V, 0.9)):
+            need = lib.dspark_sampling_workspace_for(rows, V, seqs, k, p)
+            counted = (k > 128 and k < V) or (p < 1.0 and (k == 0 or k >= V))
+            groups = min(256 // rows, (-(-(V + 7) // 512) + 15) // 16, 8)
+            assert most - need == (0 if counted or groups < 2 else rows * groups * 61440 * 2)
+            assert need == ops.sampling_workspace_bytes(rows, V, seqs, k, p)
+            if seqs:
+                fields = [0, fake, per * V, V, seqs, per - 1, V, fake, 0, 0, 0, 0, fake, 0, 1.0, k, p, fake, fake, fake, fake, need - 1]
+                assert lib.dspark_speculative_verify(ops._VERIFY_ARGS.pack(*fields), None) == -4
+            else:
+                assert lib.dspark_sampling_probs(ops._PROBS_ARGS.pack(0, fake, V, rows, V, 1.0, k, p, fake, V, fake, need - 1), None) == -4
+    assert ops.sampling_workspace_bytes(rows, V) == lib.dspark_sampling_workspace(rows, V, 0)
+    assert lib.dspark_sampling_workspace_for(0, V, 0, 0, 1.0) == 0 and lib.dspark_sampling_workspace_for(rows, 524281, 0, 0, 1.0) == 0
