@@ -150,7 +150,17 @@ class QuantizedKVCache:
                 and self.bits in ops.KV_BITS and self.group_size == ops.GROUP
                 and self.head_dim % ops.GROUP == 0 and self.head_dim <= 4096
                 and 2 * self.batch * self.kv_heads <= 65535
-                and all(t.device == keys.device for t in (values, *self.keys, *self.values)))
+                and self._buffers_fit(self.keys) and self._buffers_fit(self.values))
+
+    def _buffers_fit(self, trip) -> bool:
+        """Whether a triple is as :meth:`_alloc` makes it, but for its capacity: buffers put in its place may not be."""
+        w, s, b = trip
+        B, H, cap, n = w.shape
+        st = s.stride()
+        return (w.dtype in (torch.int32, torch.uint32) and (B, H, 32 * n) == (self.batch, self.kv_heads, self.head_dim * self.bits)
+                and s.dtype is self.dtype and b.dtype is self.dtype
+                and s.shape == b.shape == (B, H, cap, self.head_dim // self.group_size)
+                and w.stride(3) == 1 and st[3] == 1 and st == b.stride())
 
     def reserve(self, t: int) -> None:
         """Make room for ``t`` more rows at ``offset`` (a kernel then writes them in place)."""

@@ -177,3 +177,51 @@ def test_round_takes_uniforms_of_any_strides(host, monkeypatch):
     u, r = torch.rand(4, 4), _Round()
     assert Target.sampled_round(r, 3, [1] * 15, [], uniforms=u.t())[:2] == (0, [4])
     assert r.steps == 1 and torch.equal(seen[0], u.t().reshape(1, 16))
+
+
+def _other_buffers(name, trip):
+    w, s, b = trip
+    if name == "fp32 scales":
+        return w, s.float(), b.float()
+    if name == "biases of other strides":
+        return w, s, b.transpose(1, 2).contiguous().transpose(1, 2)
+    if name == "words of another stride":
+        return w.transpose(2, 3).contiguous().transpose(2, 3), s, b
+    return w.view(torch.uint32), s, b
+
+
+@pytest.mark.parametrize("name", ["fp32 scales", "biases of other strides", "words of another stride"])
+@pytest.mark.parametrize("side", ["keys", "values"])
+def test_a_cache_given_other_buffers(monkeypatch, side, name):
+    """Buffers the cache did not allocate (restored, views of one's own): what the kernel does not take is written by the
+    torch ops, as it was."""
+    from dspark_rocm.kv_cache import QuantizedKVCache
+
+    monkeypatch.setattr(ops, "eager_inference", lambda *ts: True)
+
+    def kernel(keys, values, k_rows, v_rows, *, bits, group_size):
+        raise AssertionError("buffers that the kernel refuses")
+
+    monkeypatch.setattr(ops, "quantize_kv", kernel)
+    x = torch.randn(1, 2, 5, 128, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    c, want = (QuantizedKVCache(1, 2, 128, bits=8, device="cpu") for _ in range(2))
+    setattr(c, side, _other_buffers(name, getattr(c, side)))
+    got = c.update_and_fetch(x, x + 1)
+    monkeypatch.setattr(ops, "eager_inference", lambda *ts: False)
+    for g, w in zip(got, want.update_and_fetch(x, x + 1)):
+        assert all(torch.equal(a.to(b.dtype), b) for a, b in zip(g, w))
+
+
+def test_a_cache_of_its_own_buffers_goes_by_the_kernel(monkeypatch):
+    from dspark_rocm.kv_cache import QuantizedKVCache
+
+    monkeypatch.setattr(ops, "eager_inference", lambda *ts: True)
+    calls = []
+    monkeypatch.setattr(ops, "quantize_kv", lambda *a, **k: calls.append(a))
+    x = torch.zeros(1, 2, 5, 128, dtype=torch.bfloat16)
+    c = QuantizedKVCache(1, 2, 128, bits=4, device="cpu")
+    c.update_and_fetch(x, x)
+    c.keys = _other_buffers("uint32 words", c.keys)
+    c.values = _other_buffers("uint32 words", c.values)
+    c.update_and_fetch(x, x)
+    assert len(calls) == 2
