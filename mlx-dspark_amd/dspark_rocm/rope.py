@@ -72,13 +72,15 @@ def frequencies(dims: int, base: float, scaling: dict | None = None, *, device=N
 
 
 def rotate(x: torch.Tensor, freqs: torch.Tensor, positions, *, interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
-    """:func:`dspark_rocm.ops.rope` of one tensor [B, H, L, D] in torch ops (angles in fp64)."""
+    """:func:`dspark_rocm.ops.rope` of one tensor [B, H, L, D] in torch ops: angles in fp64, the rotation in fp32 (in fp64
+    for fp64 tensors, which the kernel does not take)."""
     L, half = x.shape[2], freqs.numel()
     if not isinstance(positions, torch.Tensor):
         positions = torch.arange(int(positions), int(positions) + L, device=x.device)
     ang = positions.expand(x.shape[0], L).to(torch.float64)[:, None, :, None] * freqs.to(x.device)
-    c, s = (torch.cos(ang) * scale).to(torch.float32), (torch.sin(ang) * scale).to(torch.float32)
-    r, rest = x[..., :2 * half].to(torch.float32), x[..., 2 * half:]
+    ft = torch.float64 if x.dtype is torch.float64 else torch.float32
+    c, s = (torch.cos(ang) * scale).to(ft), (torch.sin(ang) * scale).to(ft)
+    r, rest = x[..., :2 * half].to(ft), x[..., 2 * half:]
     a, b = (r[..., 0::2], r[..., 1::2]) if interleaved else (r[..., :half], r[..., half:])
     a, b = a * c - b * s, a * s + b * c
     y = torch.stack([a, b], dim=-1).flatten(-2) if interleaved else torch.cat([a, b], dim=-1)

@@ -153,3 +153,18 @@ def test_rows_past_one_launch():
     pack = lambda B, L: ops._ROPE_ARGS.pack(0, fake, fake, *six, 1, 0, 0, *six, 0, B, L, 64, 64, 0, fake, 1.0, 0, 0, 0, 0, 0)
     for B, L in ((1, 1 << 24), (1 << 24, 1), (1 << 12, 1 << 12)):
         assert _lib.load().dspark_rope(pack(B, L), None) == -2
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotate_in_64_bits(inter):
+    """fp64 tensors are rotated in fp64: within the angle's and four operations' roundings; gradients and tangents
+    against differences."""
+    f, _ = rope.frequencies(8, 1e4)
+    x = torch.randn(2, 3, 5, 12, dtype=torch.float64, generator=torch.Generator().manual_seed(0))
+    pos = torch.arange(10).view(2, 5)
+    y = rope.rotate(x, f, pos, interleaved=inter, scale=1.25)
+    a, b = (x[..., 0:8:2], x[..., 1:8:2]) if inter else (x[..., :4], x[..., 4:8])
+    z = torch.complex(a, b) * torch.polar(torch.full((), 1.25, dtype=torch.float64), pos[:, None, :, None] * f)
+    want = torch.stack([z.real, z.imag], -1).flatten(-2) if inter else torch.cat([z.real, z.imag], -1)
+    assert torch.equal(y[..., 8:], x[..., 8:]) and (y[..., :8] - want).abs().max() <= 8 * 2.0 ** -52 * 1.25 * float(x.abs().max())
+    assert torch.autograd.gradcheck(lambda t: rope.rotate(t, f, pos, interleaved=inter), x.requires_grad_(), check_forward_ad=True)
