@@ -701,7 +701,7 @@ int dspark_rope(const dspark_rope_args* args, dspark_stream stream);
  *   scale = (max - min) * fl(1 / (2^bits - 1)) and bias = min, rounded to cache_dtype (bf16 or fp16);
  *   field = clamp(round_half_even((x - bias) / scale), 0, 2^bits - 1), a scale of 0 dividing as 1
  * (dspark_qk_norm_rope_kv_quantized's rule but for the quotient by 2^bits - 1). A NaN makes its group's scale
- * and bias NaN, its fields 0. The six arrays written share no element with each other or with x.
+ * and bias NaN, its fields 0; a bias of zero may be -0. The six arrays written share no element with each other or with x.
  * words uint32 [B, H, T, D * bits / 32], scales and biases [B, H, T, D / 64] (shared strides), unit stride
  * along the last dim: rows of a cache view. D % 64 == 0, group_size 64, 2 * B * H <= 65535.
  */

@@ -7,11 +7,12 @@
 // q/k/v kernel, which divides, rounds about one scale in 2^16 to the other side):
 //   scale = T((max - min) * fl(1 / (2^bits - 1))), bias = T(min), f = clamp(round_half_even((x - bias) / scale))
 // with a scale of 0 dividing as 1; read back: T'(fl(f * scale) + bias). A NaN in a group makes its scale and
-// bias NaN and its fields 0.
+// bias NaN and its fields 0. "Bit for bit" is but for the sign of a bias of zero: a group whose least values are +0 and
+// -0 gets -0 here, what its order gives in torch; the values read back are the same.
 //
 // Bound by bytes: 8 lanes hold a group, 8 values a lane (16 bytes of a 16-bit row), the group's extremes
-// joined over the 8 lanes with DPP. 2048 rows of 4 x 256 in bf16 to 4 bits: 7.3 us for 10.8 MB, of which the launch and
-// one round of loads are 4; 32768 rows of 8 x 128 read back to fp32 from 8 bits: 49 us for 340 MB, 6.9 TB/s, the rate
+// joined over the 8 lanes with DPP. 2048 rows of 4 x 256 in bf16 to 4 bits: 7.1 us for 10.8 MB, of which the launch and
+// one round of loads are 4; 32768 rows of 8 x 128 read back to fp32 from 8 bits: 50 us for 340 MB, 6.8 TB/s, the rate
 // of a fill of the same size.
 #include "dspark_common.h"
 
@@ -22,8 +23,8 @@ namespace dspark {
 namespace {
 
 constexpr int kKvThreads = 256;
-// Stores of a thread that reads back (one row written and 32768 of 8 x 128 read back: 52 us at 2, 85 at 1, 53 at 4; 16
-// written and 4017 read back: 9.8, 14.9, 11.1).
+// Stores of a thread that reads back (one row written and 32768 of 8 x 128 read back, both kernels from a replayed graph:
+// 51.7 us at 2, 85.4 at 1, 52.9 at 4; 16 written and 4017 read back: 9.8, 14.9, 11.2).
 constexpr int kKvOut = 2;
 
 struct KvSide {                                // keys or values

@@ -140,7 +140,7 @@ class QuantizedKVCache:
         return self.fetch()
 
     def _kernel(self, keys: torch.Tensor, values: torch.Tensor) -> bool:
-        """Whether ``ops.quantize_kv`` writes these rows (the same bits in one launch): rows and cache on
+        """Whether ``ops.quantize_kv`` writes these rows (the same values in one launch): rows and cache on
         one GPU, whole rows of the cache's own shape, nothing recording gradients."""
         if not ops.eager_inference(keys, values, *self.keys, *self.values):
             return False

@@ -973,7 +973,7 @@ def sampling_probs(logits: torch.Tensor, *, temperature: float = 1.0, top_k: int
     which less than ``top_p`` of their mass lies, 0 elsewhere. Equal logits are ordered by index; a row
     of nothing but -inf and NaN gives zeros. What a drafter samples its tokens from and hands to
     :func:`speculative_verify`. ``out`` contiguous; ``workspace`` (any content) of
-    :func:`sampling_workspace_bytes` for one call at a time, else allocated."""
+    :func:`sampling_workspace_bytes`, 256-byte aligned, for one call at a time, else allocated."""
     dev = _one_device("sampling_probs", logits, out, workspace)
     dt = LOGIT_DTYPES.get(logits.dtype)
     if dt is None:
@@ -1128,7 +1128,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, freqs: torch.Tensor, positions
     ``scale`` multiplies; the rest is copied. ``positions``: an int (row l stands at ``positions + l``), or
     an int32 / int64 tensor [L] or [B or 1, L or 1] with the position of every row, as tree rows need. The
     angle is reduced in fp64; one rounding to the tensors' type. ``q_out`` / ``k_out``: where to write,
-    e.g. a cache's rows, or q and k themselves; elements that nothing else of the call uses."""
+    e.g. a cache's rows, or q and k themselves; elements that nothing else of the call uses (refused where the
+    addresses from its first to its last element meet its input's and it is not the same view)."""
     tensor = isinstance(positions, torch.Tensor)
     dev = _one_device("rope", q, k, freqs, q_out, k_out, positions if tensor else None)
     dtype = q.dtype
@@ -1268,7 +1269,8 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
     """Quantize ``keys`` / ``values`` [B, H, T, D] (bf16, fp16 or fp32, any strides) into the cache rows
     ``k_rows`` / ``v_rows``: (words int32 [B, H, T, D*bits/32], scales [B, H, T, D/64], biases) views of a
     quantized cache, scales in bf16 or fp16. The values of :func:`dspark_rocm.quant.quantize_rows`, bit for
-    bit (a group with a NaN gets a NaN scale and bias), both tensors in one launch."""
+    bit but for the sign of a zero bias (a group with a NaN gets a NaN scale and bias), both tensors in one launch.
+    The six arrays written share no element with each other or with the rows."""
     what = "quantize_kv"
     dev = _one_device(what, keys, values, *k_rows, *v_rows)
     xdt = keys.dtype
@@ -1294,7 +1296,8 @@ def quantize_kv(keys: torch.Tensor, values: torch.Tensor, k_rows, v_rows, *, bit
 def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: torch.dtype = torch.float32, out=None):
     """A quantized cache (or rows of it) read back: the triples of :func:`quantize_kv` -> ``(keys, values)``
     [B, H, T, D] of ``dtype``, ``scale * field + bias`` with an fp32 product rounded, then an fp32 sum
-    rounded, then rounded to ``dtype``; both tensors in one launch. ``out``: two tensors to write."""
+    rounded, then rounded to ``dtype``; both tensors in one launch. ``out``: two tensors to write, sharing no
+    element with each other or with the cache."""
     what = "dequantize_kv"
     dev = _one_device(what, *keys, *values, *(out or ()))
     dt = DEQUANT_DTYPES.get(dtype)
