@@ -113,7 +113,9 @@ __global__ __launch_bounds__(kKvThreads) void kv_quantize_kernel(const KvArgs a)
   lo = min8_lanes(lo);
   hi = max8_lanes(hi);
   if (max8_lanes(bad) != 0.f) lo = hi = __builtin_nanf("");
-  const u16 sbits = kv_put<DST>((hi - lo) * (1.0f / kLevels)), bbits = kv_put<DST>(lo);
+  float range = (hi - lo) * (1.0f / kLevels);
+  asm("" : "+v"(range));                       // in fp32 first: else product and conversion to fp16 are one instruction, rounded once
+  const u16 sbits = kv_put<DST>(range), bbits = kv_put<DST>(lo);
   const float sc = kv_get<DST>(sbits), bias = kv_get<DST>(bbits);
   const float div = sc == 0.f ? 1.f : sc;
   u32 f[8];

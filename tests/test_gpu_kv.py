@@ -276,3 +276,32 @@ def test_tangents(dev):
             ops.quantize_kv(dual, rows[1], t, u, bits=8)
         out = forward_ad.unpack_dual(attend(forward_ad.make_dual(q, torch.ones_like(q))))
         assert torch.equal(out.primal, want) and bool(out.tangent.abs().sum() > 0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("cdt", ["f16", "bf16"])
+def test_scales_round_twice(dev, bits, cdt):
+    """Ranges whose product with the reciprocal lies beside the middle of two scales, so close that it is there in fp32:
+    the scale is the even one, as two roundings give it, on whichever side of the middle the product lies."""
+    from dspark_rocm import ops, quant
+
+    dt = DT[cdt]
+    levels, ulp = 2 ** bits - 1, torch.finfo(dt).eps
+    recip = torch.tensor(1.0 / levels, dtype=torch.float32).double()
+    mid = 1.0 + ulp * (torch.arange(1 / ulp if cdt == "f16" else 128).double() + 0.5)
+    d = torch.cat([(mid * levels).to(torch.float32).view(torch.int32) + i for i in (-1, 0, 1)]).view(torch.float32)
+    exact, near = d.double() * recip, (d.double() * recip).to(torch.float32)
+    m3 = mid.repeat(3)
+    once = torch.where(exact > m3, m3 + ulp / 2, m3 - ulp / 2)
+    twice = near.to(dt).double()
+    d = d[(near.double() == m3) & (exact != m3) & (once != twice)]
+    assert len(d) > 10
+    x = torch.zeros(1, 1, len(d), 64)
+    x[0, 0, :, 5] = d
+    x = x.to(dev)
+    trips = [cache(1, 1, len(d), 64, bits, dt, dev) for _ in range(2)]
+    ops.quantize_kv(x, x, *trips, bits=bits)
+    f, s, b = rule(x, bits, dt)
+    for trip, q in zip(zip(*trips), quant.quantize_rows(x, bits, dtype=dt)):
+        assert torch.equal(trip[0], trip[1]) and torch.equal(trip[0], q)
+    assert torch.equal(trips[0][1].cpu(), s) and torch.equal(fields(trips[0][0], bits), f)
