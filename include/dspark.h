@@ -724,6 +724,79 @@ int dspark_kv_quantize(const dspark_kv_args* args, dspark_stream stream);
 /* Such rows read back: x = scale * field (rounded to fp32) + bias (rounded to fp32), rounded to x_dtype. */
 int dspark_kv_dequantize(const dspark_kv_args* args, dspark_stream stream);
 
+/* ------------------------------------------------------------------ paged caches of many sequences */
+
+/*
+ * Keys or values of a pool of pages: [pool, Hk, P, D], P = 16, 32, 64 or 128 positions, D = 64, 128 or 256, of the
+ * model's type, or (codes) e4m3 codes c that stand for c * 2^(e - 127) with a byte e (e8m0) for each page and head in
+ * exponents [pool, Hk]. Strides in elements, of 16-byte multiples, unit stride along D.
+ */
+typedef struct dspark_pages { /* every field is 8 bytes; strides are (page, head, position) and (page, head) */
+  void* data;
+  int64_t strides[3];
+  void* exponents;
+  int64_t exponent_strides[2];
+} dspark_pages;
+
+/*
+ * The sequences of a call, on the device: int32 table [count, width] (row stride ld_table) of page ids, position p of a
+ * sequence in row p % P of its page p / P; int32 starts [count + 1]: rows starts[b] .. starts[b + 1] - 1 of the call are
+ * sequence b's, the last of its lens[b] (int32) positions. Whatever these hold, nothing outside the tensors is touched:
+ * a sequence whose rows are not among the call's `rows` has none, and positions before the first, past the table or
+ * in a page that is not one of the pool's are not there. count <= 4096, rows < 2^22.
+ */
+typedef struct dspark_sequences { /* every field is 8 bytes */
+  const int32_t* table;
+  const int32_t* starts;
+  const int32_t* lens;
+  int64_t ld_table, count, width, rows;
+} dspark_sequences;
+
+/*
+ * A step's rows into their sequences' pages, rotated on the way, in one launch. q [rows, Hq, D] (Hq = 0: none), k and v
+ * [rows, Hk, D], bf16 or fp16, strides (row, head) in elements, 16-byte aligned. Of the first dims values of a head (a
+ * multiple of 16, interleaved of 8; 0: nothing is rotated) the pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved,
+ * turn by position * freqs[i] (fp64): cos and sin, times scale, rounded to fp32, then fl(fl(x1 c) - fl(x2 s)) and
+ * fl(fl(x1 s) + fl(x2 c)) in fp32, rounded to dtype. positions (int32 or int64 [rows]) replaces the rows' own.
+ * q_out may be q itself. Pages of codes: the exponent of a page and head becomes the least with |x| <= 448 2^(e - 127)
+ * for the finite values of the rows new in it, at least 17, and at least what it was where the page holds rows of this
+ * sequence before them, which are shifted to it; codes are rounded to nearest even, infinities become NaN. A page that is
+ * written to belongs to one sequence.
+ */
+typedef struct dspark_paged_append_args { /* every field is 8 bytes */
+  int64_t dtype, codes, Hq, Hk, D, P, pool, dims, interleaved;
+  const double* freqs;
+  double scale;
+  const void* positions;
+  int64_t positions_i64, position_stride;
+  const void* q;
+  int64_t q_strides[2];
+  void* q_out;
+  int64_t q_out_strides[2];
+  int64_t q_clear; /* rows of no sequence: zeros in q_out, else left as they are */
+  const void* k;
+  int64_t k_strides[2];
+  const void* v;
+  int64_t v_strides[2];
+  dspark_pages k_pages, v_pages;
+  dspark_sequences seqs;
+} dspark_paged_append_args;
+
+int dspark_paged_append(const dspark_paged_append_args* args, dspark_stream stream);
+
+/* Pages by id (int32 [count]), keys and values [count, Hk, P, D] of dtype, contiguous: the values the codes stand for,
+ * rounded once; zeros for an id that is not one of the pool's. */
+typedef struct dspark_paged_read_args { /* every field is 8 bytes */
+  int64_t dtype, codes, Hk, D, P, pool;
+  const int32_t* ids;
+  int64_t count;
+  dspark_pages k_pages, v_pages;
+  void* k_out;
+  void* v_out;
+} dspark_paged_read_args;
+
+int dspark_paged_read(const dspark_paged_read_args* args, dspark_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -191,6 +191,8 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_rope": (c_int, [c_char_p, c_void_p]),
     "dspark_kv_quantize": (c_int, [c_char_p, c_void_p]),
     "dspark_kv_dequantize": (c_int, [c_char_p, c_void_p]),
+    "dspark_paged_append": (c_int, [c_char_p, c_void_p]),
+    "dspark_paged_read": (c_int, [c_char_p, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -1326,3 +1326,194 @@ def dequantize_kv(keys, values, *, bits: int, group_size: int = GROUP, dtype: to
     if shape[0] * shape[1] * shape[2]:
         _call_on(dev, "dspark_kv_dequantize", _KV_ARGS.pack(*args))
     return k, v
+
+
+# ---------------------------------------------------------------------------- paged caches of many sequences
+
+PAGE_POSITIONS = (16, 32, 64, 128)
+PAGE_CODES, PAGE_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu     # 8-bit pages: codes, and scales of a page and head
+
+
+def _pages_side(what: str, pages, shape, dtype, written: bool) -> tuple[bool, torch.Size, tuple]:
+    """(codes?, [pool, Hk, P, D], the fields of one ``dspark_pages``) of keys or values."""
+    scales = None
+    data = pages
+    if isinstance(pages, (tuple, list)):
+        data, scales = pages
+        if data.dtype is not PAGE_CODES or scales.dtype is not PAGE_SCALES:
+            raise TypeError(f"{what}: 8-bit pages are {PAGE_CODES} codes and {PAGE_SCALES} scales, got {data.dtype} and {scales.dtype}")
+    elif data.dtype is not dtype:
+        raise TypeError(f"{what}: pages {data.dtype} for rows of {dtype} (or codes with their scales)")
+    s = data.shape
+    if len(s) != 4 or (shape is not None and s != shape):
+        raise ValueError(f"{what}: pages must be [pages, Hk, positions, D], keys and values alike, got {list(s)}")
+    if s[2] not in PAGE_POSITIONS or s[3] not in QUANT_HEAD_DIMS:
+        raise ValueError(f"{what}: pages of {s[2]} positions {PAGE_POSITIONS} of {s[3]} values {QUANT_HEAD_DIMS}")
+    _no_autograd(what, data)
+    _as_stored(what, data)
+    p0, p1, p2, unit = data.stride()
+    if unit != 1:
+        raise ValueError(f"{what}: pages need unit stride along their values")
+    if written:
+        _no_repeats(what, data)
+    if scales is None:
+        return False, s, (data.data_ptr(), p0, p1, p2, 0, 0, 0)
+    if scales.shape != s[:2]:
+        raise ValueError(f"{what}: scales must be {list(s[:2])}, got {list(scales.shape)}")
+    if written:
+        _no_repeats(what, scales)
+    return True, s, (data.data_ptr(), p0, p1, p2, scales.data_ptr(), *scales.stride())
+
+
+def _pages_parts(pages) -> tuple:
+    return tuple(pages) if isinstance(pages, (tuple, list)) else (pages,)
+
+
+def _both_pages(what: str, k_pages, v_pages, dtype, written: bool):
+    """(codes?, shape, fields of both, tensors written)."""
+    codes, shape, k = _pages_side(what, k_pages, None, dtype, written)
+    v_codes, _, v = _pages_side(what, v_pages, shape, dtype, written)
+    if codes != v_codes:
+        raise TypeError(f"{what}: keys and values in 8 bits, or neither")
+    return codes, shape, k + v
+
+
+def _sequences(what: str, table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, rows: int) -> tuple:
+    """The fields of ``dspark_sequences``, and what has to stay alive for them."""
+    if table.dim() != 2 or table.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: table must be int32 [sequences, pages], got {table.dtype} {list(table.shape)}")
+    B, W = table.shape
+    if B > 4096:
+        raise ValueError(f"{what}: {B} sequences (up to 4096)")
+    if table.dtype is not torch.int32:
+        table = _ints(what, "table", table, table.shape)
+    if W > 1 and table.stride(1) != 1 or table.stride(0) < W:
+        table = table.contiguous()
+    starts, lens = _ints(what, "starts", starts, (B + 1,)), _ints(what, "lens", lens, (B,))
+    return (table.data_ptr(), starts.data_ptr(), lens.data_ptr(), max(table.stride(0), W), B, W, rows), (table, starts, lens)
+
+
+def _paged_rows(what: str, name: str, t: torch.Tensor, T: int, H: int, D: int, dtype) -> tuple:
+    """Rows [T, H, D] as a kernel reads them (a copy where their addresses have no 16 bytes together), their strides."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} {t.dtype} beside {dtype}")
+    if t.shape != (T, H, D):
+        raise ValueError(f"{what}: {name} must be [{T}, {H}, {D}], got {list(t.shape)}")
+    if t.is_neg():
+        t = t.resolve_neg()
+    s0, s1, unit = t.stride()
+    if unit != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, _ = t.stride()
+    return t, s0, s1
+
+
+_APPEND_ARGS = struct.Struct("=10qd37q")
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torch.Tensor, starts: torch.Tensor,
+                 lens: torch.Tensor, *, q: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None, interleaved: bool = False, scale: float = 1.0,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """A step's rows into their sequences' pages, rotated to their positions on the way, in one launch; returns the
+    rotated queries (None without ``q``).
+
+    ``k`` / ``v`` [T, Hk, D] and ``q`` [T, Hq, D], bf16 or fp16, D 64, 128 or 256: the rows of all sequences, one after
+    the other: ``starts`` [B + 1] says where each one's begin, ``lens`` [B] how many positions it has with them (both
+    int32 on the device), ``table`` int32 [B, pages] in which pages: position p lies in row p % P of page
+    ``table[b, p // P]``. ``k_pages`` / ``v_pages`` [pages, Hk, P, D] (P 16, 32, 64 or 128) are of the rows' type, or
+    (codes e4m3 [pages, Hk, P, D], scales e8m0 [pages, Hk]): 8 bits with one power of two for each page and head, the least
+    that fits the rows new in it and those it held before them, which are shifted to it.
+
+    ``freqs`` fp64 [dims / 2] (:func:`dspark_rocm.rope.frequencies`) rotates the first ``dims`` values of queries and keys as
+    :func:`rope` does, ``dims`` a multiple of 16 (interleaved: of 8); None: nothing is rotated. ``positions`` int32 / int64
+    [T]: rotate by these instead. Rows of a position that the table, or the pool, does not have are not written; rows
+    behind the last sequence's are left out, and ``q_out`` there as it is. A page that is written to belongs to one
+    sequence. ``q_out``: where the queries go, e.g. ``q`` itself; else new, with zeros in rows of no sequence."""
+    what = "paged_append"
+    tensors = (v, *_pages_parts(k_pages), *_pages_parts(v_pages), table, starts, lens, q, freqs, positions, q_out)
+    dev = _one_device(what, k, *tensors)
+    dtype = k.dtype
+    dt = ATTN_DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"{what}: rows {dtype} (bfloat16 or float16)")
+    codes, (pool, Hk, P, D), pages = _both_pages(what, k_pages, v_pages, dtype, True)
+    if k.dim() != 3:
+        raise ValueError(f"{what}: k must be [rows, {Hk}, {D}], got {list(k.shape)}")
+    T = k.shape[0]
+    _no_autograd(what, k, v, q, freqs, q_out)
+    k, *k_st = _paged_rows(what, "k", k, T, Hk, D, dtype)
+    v, *v_st = _paged_rows(what, "v", v, T, Hk, D, dtype)
+    seqs, keep = _sequences(what, table, starts, lens, T)
+    at_f = dims = 0
+    if freqs is not None:
+        if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= D // 2:
+            raise ValueError(f"{what}: freqs must be fp64 [dims / 2], dims up to {D}, got {freqs.dtype} {list(freqs.shape)}")
+        dims = 2 * freqs.numel()
+        if dims % (8 if interleaved else 16):
+            raise ValueError(f"{what}: {dims} rotated values (a multiple of 16, interleaved of 8; others: rope, then paged_append)")
+        freqs = freqs.resolve_neg().contiguous()
+        at_f = freqs.data_ptr()
+    at_p = p_st = p64 = 0
+    if positions is not None:
+        p64 = positions.dtype is torch.int64
+        if not (p64 or positions.dtype is torch.int32) or positions.shape != (T,):
+            raise ValueError(f"{what}: positions must be int32 or int64 [{T}], got {positions.dtype} {list(positions.shape)}")
+        at_p, p_st = positions.data_ptr(), positions.stride(0)
+    q_fields, Hq = (0,) * 7, 0
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError(f"{what}: q must be [{T}, heads, {D}], got {list(q.shape)}")
+        Hq = q.shape[1]
+        clear = True
+        if q_out is None:
+            q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
+            q_out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+        else:
+            clear = False
+            same = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
+            if q_out.dtype is not dtype or q_out.shape != q.shape or q_out.stride(2) != 1 or q_out.stride(0) % 8 \
+                    or q_out.stride(1) % 8 or q_out.data_ptr() % 16:
+                raise ValueError(f"{what}: q_out must be {dtype} {list(q.shape)} with unit last stride, aligned to 16 bytes")
+            _as_stored(what, q_out)
+            _no_repeats(what, q_out)
+            if not same and q.numel() and _spans_meet(q, q_out):
+                raise ValueError(f"{what}: q_out overlaps q (in place: the same view)")
+            q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
+        q_fields = (q.data_ptr(), *q_st, q_out.data_ptr(), *q_out.stride()[:2], clear)
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out without q")
+    if T and seqs[4] and seqs[5] and pool and Hk:
+        for t in (k, v):                # what is written shares no place with what is read, k and v may
+            _distinct(what, t.data_ptr(), *(f for f in (*pages[::7], *pages[4::7]) if f), *((q_out.data_ptr(),) if Hq else ()))
+        _call_on(dev, "dspark_paged_append",
+                 _APPEND_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, dims, bool(interleaved), at_f, scale, at_p, p64, p_st, *q_fields,
+                                   k.data_ptr(), *k_st, v.data_ptr(), *v_st, *pages, *seqs))
+    elif Hq and clear:
+        q_out.zero_()
+    return q_out
+
+
+_READ_ARGS = struct.Struct("=24q")
+
+
+def paged_read(k_pages, v_pages, pages: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16):
+    """Pages by id (``pages`` int32 [N] on the device) as dense ``(keys, values)`` [N, Hk, P, D] of ``dtype`` (bf16 or fp16;
+    for pages that are not in 8 bits their own): what :func:`paged_append` keeps, the values that 8-bit codes stand for
+    rounded once. Zeros for ids that are none of the pool's."""
+    what = "paged_read"
+    parts = (*_pages_parts(k_pages), *_pages_parts(v_pages))
+    dev = _one_device(what, *parts, pages)
+    dt = ATTN_DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"{what}: dtype {dtype} (bfloat16 or float16)")
+    codes, (pool, Hk, P, D), fields = _both_pages(what, k_pages, v_pages, dtype, False)
+    if pages.dim() != 1:
+        raise ValueError(f"{what}: pages must be int32 [N], got {list(pages.shape)}")
+    ids = _ints(what, "pages", pages, pages.shape)
+    N = ids.numel()
+    k, v = (torch.empty((N, Hk, P, D), dtype=dtype, device=dev) for _ in range(2))
+    if N and Hk and pool:
+        _call_on(dev, "dspark_paged_read",
+                 _READ_ARGS.pack(dt, codes, Hk, D, P, pool, ids.data_ptr(), N, *fields, k.data_ptr(), v.data_ptr()))
+    return (k, v) if pool else (k.zero_(), v.zero_())
