@@ -797,6 +797,34 @@ typedef struct dspark_paged_read_args { /* every field is 8 bytes */
 
 int dspark_paged_read(const dspark_paged_read_args* args, dspark_stream stream);
 
+/*
+ * Attention of a step's rows over their sequences' pages: q and out [rows, Hq, D] of dtype (strides (row, head), 16-byte
+ * aligned), query head g of Hq reading KV head g / (Hq / Hk). Row i of sequence b's n sees, of the positions that are there,
+ * 0 .. lens[b] - n + i (causal) or all lens[b]: out = softmax(scale q . k) . v in fp32, rounded once; zeros where it sees
+ * none. Values that are not finite count only where a row sees them. Rows of no sequence: zeros (clear), else left as they
+ * are. max_rows: rows of one sequence, at most; a sequence with more is served too, only slower. scale > 0, finite.
+ * workspace: dspark_paged_attention_workspace bytes with max_len = width * P, 16-byte aligned, of any content, one call's at
+ * a time: calls on two streams, or graphs that may run together, need one each. The result does not depend on what else is
+ * in the call, but for the order in which partial sums are joined.
+ */
+typedef struct dspark_paged_attention_args { /* every field is 8 bytes */
+  int64_t dtype, codes, Hq, Hk, D, P, pool, causal, clear, max_rows;
+  double scale;
+  const void* q;
+  int64_t q_strides[2];
+  void* out;
+  int64_t out_strides[2];
+  dspark_pages k_pages, v_pages;
+  dspark_sequences seqs;
+  void* workspace;
+  int64_t workspace_bytes;
+} dspark_paged_attention_args;
+
+size_t dspark_paged_attention_workspace(int64_t count, int64_t Hq, int64_t Hk, int64_t D, int64_t rows, int64_t max_rows,
+                                        int64_t max_len);
+
+int dspark_paged_attention(const dspark_paged_attention_args* args, dspark_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

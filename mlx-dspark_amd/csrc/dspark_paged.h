@@ -58,34 +58,33 @@ __device__ __forceinline__ int page_of(const Seqs& s, int b, long pos) {
   return (unsigned)id < (unsigned)s.pool ? id : -1;
 }
 
-// Sum of v over the lanes up to this one
-__device__ __forceinline__ int wave_scan(int v) {
+// Sum of v over the lanes up to this one, at most 2^32 - 1
+__device__ __forceinline__ u32 wave_scan(u32 v) {
   const int lane = __lane_id();
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int o = __builtin_amdgcn_ds_bpermute((lane - d) << 2, v);
-    if (lane >= d) v += o;
+    const u32 o = (u32)__builtin_amdgcn_ds_bpermute((lane - d) << 2, (int)v);
+    v = __builtin_elementwise_add_sat(v, lane >= d ? o : 0u);
   }
   return v;
 }
 
-// The sequence that holds item `item` of a list in which every sequence b has count(b) items (no more than `most`, so that
-// sums stay in 32 bits), and the item's place among them. Every wave finds it for itself; false past the list's end.
+// The sequence that holds item `item` of a list in which every sequence b has count(b) items, and the item's place among
+// them. Every wave finds it for itself; false past the list's end.
 template <class F>
-__device__ __forceinline__ bool locate(int item, int B, int most, F count, int& b, int& local) {
+__device__ __forceinline__ bool locate(u32 item, int B, F count, int& b, int& local) {
   const int lane = __lane_id();
-  int before = 0;
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int c = b0 + lane < B ? min(max(count(b0 + lane), 0), most) : 0;
-    const int upto = wave_scan(c);
-    const int all = __builtin_amdgcn_readlane(upto, 63);
-    if (item - before < all) {
-      const int first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > item - before));
+    const u32 c = b0 + lane < B ? count(b0 + lane) : 0u;
+    const u32 upto = wave_scan(c);
+    const u32 all = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+    if (item < all) {
+      const int first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > item));
       b = uniform(b0 + first);
-      local = uniform(item - before - __builtin_amdgcn_readlane(upto - c, first));
+      local = uniform((int)(item - (u32)__builtin_amdgcn_readlane((int)(upto - c), first)));
       return true;
     }
-    before += all;
+    item -= all;
   }
   return false;
 }

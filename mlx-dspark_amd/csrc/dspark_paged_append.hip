@@ -227,11 +227,11 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, float2* tab, u
   int b, j;
   const auto count = [&](int i) {
     const Seq q = sequence(a.s, i);
-    if (!q.n) return 0;
+    if (!q.n) return 0u;
     const long p0 = first_position(a.s, i, q), p1 = p0 + q.n;      // of the rows, their end
-    return p1 <= 0 ? 0 : (int)(((p1 - 1) >> a.s.log2P) - ((p0 < 0 ? 0 : p0) >> a.s.log2P) + 1);
+    return p1 <= 0 ? 0u : (u32)(((p1 - 1) >> a.s.log2P) - ((p0 < 0 ? 0 : p0) >> a.s.log2P) + 1);
   };
-  if (!locate((item >> 1) / a.Hk, a.s.B, a.s.T, count, b, j)) return;
+  if (!locate((u32)((item >> 1) / a.Hk), a.s.B, count, b, j)) return;
   const Seq q = sequence(a.s, b);
   const long p0 = first_position(a.s, b, q), base = (((p0 < 0 ? 0 : p0) >> a.s.log2P) + j) << a.s.log2P;
   const int id = page_of(a.s, b, base);
@@ -384,7 +384,7 @@ int check_pool(const char* what, int64_t pool, int64_t Hk, int64_t P, int64_t D)
 int take_seqs(const char* what, const dspark_sequences* p, int64_t P, int64_t pool, Seqs* out) {
   if (!p->table || !p->starts || !p->lens) return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
   if (p->count < 1 || p->count > 4096 || p->width < 1 || p->width > (1 << 24) || p->rows < 1 || p->rows >= (1 << 22) ||
-      p->ld_table < p->width || p->width * P >= (1L << 31))
+      p->ld_table < p->width || p->width * P > (1L << 30))
     return fail(DSPARK_ERR_SHAPE, "%s: %ld sequences (up to 4096) of %ld pages, %ld rows (up to 2^22)", what, (long)p->count,
                 (long)p->width, (long)p->rows);
   *out = Seqs{p->table, p->starts, p->lens, p->ld_table, (int)p->count, (int)p->width, (int)p->rows, (int)P,

@@ -1,0 +1,594 @@
+// Attention over paged caches for gfx950: few rows of each sequence (decoded tokens, verify blocks).
+//
+// out[row] = softmax(scale q . k^T) . v over the keys that the row sees: keys 0 .. len - n + i of its sequence for row i of
+// n (causal), or all of them; fp32 scores, running maximum and sum in one pass over the keys. The rows of a sequence and
+// KV head, R = n times the query heads of the group, are (token, query head), heads fastest.
+//
+// Bound by the bytes of K and V. Hence:
+//   * the work is the list of all (sequence, KV head, row group, 128 keys), dealt in equal runs to a fixed number of
+//     workgroups, whatever the lengths: a workgroup's run covers the end of one KV head, whole ones, and the start of
+//     another. What is not whole goes to the workspace as unnormalised fp32 outputs with their maxima and sums, two slots a
+//     workgroup, and a second launch joins them in the order of the keys. Lengths stay on the device;
+//   * a wave takes 32 of the 128 keys by itself: no barrier in the loop. The next keys and values are in flight in
+//     registers while the present ones are multiplied; one page's 16 positions have one address, so page ids are kept 64 a
+//     wave in a register and read by the lane number;
+//   * S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32: a lane holds 4 + 4 keys of one row, which are, in place, what
+//     the second product needs. K goes from memory to the operand, V through LDS (the transposing read), 16-byte
+//     chunks XOR-swizzled by the row;
+//   * 8-bit pages are turned into the model's type as they are used: one conversion for two values with the page's power of
+//     two in it, exact.
+// Probabilities go to the matrix cores as two pieces of the type (16 bits of bf16, 22 of fp16, there of p 2^15): at these
+// row counts the second piece costs nothing.
+//
+// Values that are not finite are only let through where a row sees them: a row with such an output is computed again in
+// plain fp32 from the keys it sees (plain_row).
+#pragma once
+
+#include "dspark_attn.h"
+#include "dspark_paged.h"
+
+namespace dspark {
+namespace paged {
+
+using attn::BF16;
+using attn::F16;
+
+constexpr int kAttnThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kWaveKeys = 32;                       // keys of a wave's step
+constexpr int kUnit = kWaves * kWaveKeys;           // of a workgroup's
+constexpr float kLowest = -3.402823466e38f;
+constexpr u32 kMostUnits = 1u << 30;                // of a call
+
+struct AttnArgs {
+  Seqs s;
+  Pages k, v;
+  const u16* q;
+  u16* out;
+  long qrow, qhead, orow, ohead;                    // element strides
+  float* opart;                                     // [workgroup][2 slots][16 RT rows][D], unnormalised
+  float* mpart;                                     // [workgroup][2 slots][16 RT rows]: maxima, then sums
+  int Hq, Hk, gqa, causal;
+  int whole;                                        // a workgroup takes whole (sequence, KV head, row group)s: nothing to join
+  int least;                                        // units of a run, at least
+  int rows_up_to;                                   // sequences with more rows of a KV head are another kernel's
+  int clear;                                        // rows of no sequence: zeros
+  float scale_log2;
+};
+
+// A sequence's share of the work list
+struct Work {
+  int start, n, len;                                // first row, rows, keys
+  int rows, groups, tiles;                          // rows and row groups of a KV head, units along the keys
+};
+
+template <int RT>
+__device__ __forceinline__ Work work_of(const AttnArgs& a, int b) {
+  const Seq q = sequence(a.s, b);
+  Work w{q.start, q.n, q.len, q.n * a.gqa, 0, 0};
+  if (w.rows > a.rows_up_to || q.n == 0) w.rows = 0;
+  w.groups = (w.rows + 16 * RT - 1) / (16 * RT);
+  w.tiles = a.whole ? 1 : (q.len + kUnit - 1) / kUnit;
+  return w;
+}
+
+template <int RT>
+__device__ __forceinline__ u32 units_of(const AttnArgs& a, int b) {
+  const Work w = work_of<RT>(a, b);
+  const unsigned long long n = (unsigned long long)a.Hk * (unsigned)w.groups * (unsigned)w.tiles;
+  return n > kMostUnits ? kMostUnits + 1 : (u32)n;
+}
+
+// Units of all sequences, and of those before `upto`; none where they are more than a call may have (the entry point
+// checks that: only sequences that share their rows come to that here)
+template <int RT>
+__device__ __forceinline__ int all_units(const AttnArgs& a, int upto, int* before) {
+  const int lane = __lane_id();
+  u32 sum = 0, first = 0;
+  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+    const u32 n = b0 + lane < a.s.B ? units_of<RT>(a, b0 + lane) : 0u;
+    sum = __builtin_elementwise_add_sat(sum, n);
+    if (b0 + lane < upto) first += n;
+  }
+  const u32 all = (u32)__builtin_amdgcn_readlane((int)wave_scan(sum), 63);
+  if (all > kMostUnits) return 0;
+  if (before) *before = __builtin_amdgcn_readlane((int)wave_scan(first), 63);
+  return (int)all;
+}
+
+__device__ __forceinline__ int run_of(const AttnArgs& a, int units, int workgroups) {
+  const int even = (units + workgroups - 1) / workgroups;
+  return even > a.least ? even : a.least;
+}
+
+template <class T, bool CODES>
+__device__ __forceinline__ float element(const Pages& p, long at, float unit) {
+  if constexpr (CODES) return __builtin_amdgcn_cvt_f32_fp8((int)(unsigned char)p.data[at], 0) * unit;
+  else return attn::to_f32<T>(reinterpret_cast<const u16*>(p.data)[at]);
+}
+
+// One row again, by one wave, in plain fp32 over the keys it sees: largest score, sum, then probabilities times values.
+template <class T, int D, bool CODES>
+__device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int head, int keys) {
+  const int lane = __lane_id(), h = head / a.gqa;
+  const u16* q = a.q + t * a.qrow + head * a.qhead;
+  auto unit = [&](const Pages& p, int id) {
+    return CODES ? __builtin_bit_cast(float, (u32)p.exps[id * p.epage + h * p.ehead] << 23) : 1.f;
+  };
+  auto score = [&](int key) {
+    const int id = key < keys ? page_of(a.s, b, key) : -1;
+    if (id < 0) return -__builtin_inff();
+    const long at = id * a.k.page + h * a.k.head + (key & (a.s.P - 1)) * a.k.row;
+    const float u = unit(a.k, id);
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) s = __builtin_fmaf(attn::to_f32<T>(q[d]), element<T, CODES>(a.k, at + d, u), s);
+    return s;
+  };
+  auto seen = [&](int key) { return key < keys && page_of(a.s, b, key) >= 0; };
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < keys; k0 += 64) m = fmaxf(m, score(k0 + lane));
+#pragma unroll 1
+  for (int x = 1; x < 64; x *= 2) m = fmaxf(m, shfl_xor(m, x));
+  auto weight = [&](int key) { return seen(key) ? __builtin_amdgcn_exp2f((score(key) - m) * a.scale_log2) : 0.f; };
+#pragma unroll 1
+  for (int k0 = 0; k0 < keys; k0 += 64) l += weight(k0 + lane);
+#pragma unroll 1
+  for (int x = 1; x < 64; x *= 2) l += shfl_xor(l, x);
+  float sum[D / 64] = {};
+  bool any = false;
+#pragma unroll 1
+  for (int k0 = 0; k0 < keys; k0 += 64) {
+    const float p = weight(k0 + lane) / l;
+#pragma unroll 1
+    for (int j = 0; j < min(64, keys - k0); ++j) {
+      const int id = page_of(a.s, b, k0 + j);
+      if (id < 0) continue;
+      any = true;
+      const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j)), u = unit(a.v, id);
+      const long at = id * a.v.page + h * a.v.head + ((k0 + j) & (a.s.P - 1)) * a.v.row + lane * (D / 64);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) sum[c] = __builtin_fmaf(pj, element<T, CODES>(a.v, at + c, u), sum[c]);
+    }
+  }
+  u16* o = a.out + t * a.orow + head * a.ohead + lane * (D / 64);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) o[c] = attn::from_f32<T>(any ? sum[c] : 0.f);
+}
+
+// Keys that row i of a sequence's n sees
+__device__ __forceinline__ int keys_seen(const AttnArgs& a, int b, int n, int len, int i) {
+  if (!a.causal) return len;
+  const long k = (long)a.s.lens[b] - n + i + 1;
+  return (int)(k < 0 ? 0 : k < len ? k : len);
+}
+
+// 16 codes as 16 values of T
+template <class T>
+__device__ __forceinline__ void decode(u32x4_t c, float unit, u32x4_t& lo, u32x4_t& hi) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u32 x, y;
+    if constexpr (T::kF16) {
+      x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], unit, false));
+      y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[i], unit, true));
+    } else {
+      x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], unit, false));
+      y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], unit, true));
+    }
+    if (i < 2) lo[2 * i] = x, lo[2 * i + 1] = y;
+    else hi[2 * i - 4] = x, hi[2 * i - 3] = y;
+  }
+}
+
+// The 16-byte chunk c of row r of a V tile lies at chunk c ^ tile_swz(r): a transposing read takes two chunks of 16 rows
+template <int D>
+__device__ __forceinline__ int tile_swz(int r) { return D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
+
+__device__ __forceinline__ u32x2_t lds_transposed(const u16* p) {
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
+}
+
+// What a wave writes to LDS for itself is in place before it reads it
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <class T, int D, int RT, bool CODES>
+__global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) void rows_kernel(const AttnArgs a) {
+  constexpr int ROWS = 16 * RT, NC = D / 32, ND = D / 16;
+  constexpr int CH = D / 8;                                  // 16-byte chunks of a row in T
+  constexpr int KL = CODES ? D / 64 : D / 32;                // 16-byte loads of a lane for 16 keys
+  constexpr int VCH = CODES ? D / 16 : D / 8;                // 16-byte chunks of a row in memory
+  constexpr int VL = kWaveKeys * VCH / 64;                   // of a lane for the wave's keys
+  __shared__ __attribute__((aligned(16))) u16 tiles[kWaves][kWaveKeys * D];      // V; then the waves' outputs
+  __shared__ float wm[kWaves][ROWS], wl[kWaves][ROWS];
+  __shared__ int again[ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int c16 = lane & 15, q4 = lane >> 4;
+  u16* const vt = tiles[wave];
+
+  if (a.clear) {
+    for (int t = blockIdx.x; t < a.s.T; t += gridDim.x) {
+      bool has = false;
+      for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+        const Seq q = sequence(a.s, min(b0 + lane, a.s.B - 1));
+        has |= q.n > 0 && t >= q.start && t < q.start + q.n;
+      }
+      if (__builtin_amdgcn_ballot_w64(has)) continue;
+      for (int i = tid; i < a.Hq * CH; i += kAttnThreads)
+        *reinterpret_cast<u32x4_t*>(a.out + t * a.orow + i / CH * a.ohead + 8 * (i % CH)) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  }
+
+  const int units = all_units<RT>(a, 0, nullptr), run = a.whole ? 1 : run_of(a, units, gridDim.x);
+  if ((long)blockIdx.x * run >= units) return;
+  int u = blockIdx.x * run;
+  const int u_end = min(u + run, units);
+  int b, local;
+  if (!locate((u32)u, a.s.B, [&](int i) { return units_of<RT>(a, i); }, b, local)) return;
+  Work w = work_of<RT>(a, b);
+  w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+
+  while (u < u_end) {
+    // the KV head and row group, and the units [t0, t1) of it
+    const int seg = local / w.tiles, t0 = local - seg * w.tiles;
+    const int t1 = min(w.tiles, t0 + (u_end - u));
+    const int h = seg / w.groups, r0 = (seg - h * w.groups) * ROWS;
+    const int key0 = t0 * kUnit, key1 = a.whole ? w.len : min(w.len, t1 * kUnit);
+
+    u32x4_t qf[RT][NC];
+    int lim[RT];                                             // keys that this lane's rows see
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = min(r0 + 16 * rt + c16, w.rows - 1), i = r / a.gqa;
+      lim[rt] = keys_seen(a, b, w.n, w.len, i);
+      const u16* qp = a.q + (w.start + i) * a.qrow + (h * a.gqa + r - i * a.gqa) * a.qhead;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        qf[rt][c] = CODES ? ldg128(qp + 64 * (c >> 1) + 16 * q4 + 8 * (c & 1)) : ldg128(qp + 32 * c + 8 * q4);
+    }
+    const int all_see = uniform(keys_seen(a, b, w.n, w.len, min(r0, w.rows - 1) / a.gqa));
+
+    // page ids (and scales) of 64 pages, a lane each
+    const int* const row = a.s.table + b * a.s.ldt;
+    int ids = -1, ids_at = -1 << 30;                         // of page ids_at + lane
+    float ku = 1.f, vu = 1.f;
+    auto fetch_ids = [&](int first) {
+      ids_at = first;
+      const int p = first + lane;
+      const int id = p <= (w.len - 1) >> a.s.log2P ? row[p] : -1;
+      ids = (unsigned)id < (unsigned)a.s.pool ? id : -1;
+      if constexpr (CODES) {
+        ku = vu = 0.f;
+        if (ids >= 0) {
+          ku = __builtin_bit_cast(float, (u32)a.k.exps[ids * a.k.epage + h * a.k.ehead] << 23);
+          vu = __builtin_bit_cast(float, (u32)a.v.exps[ids * a.v.epage + h * a.v.ehead] << 23);
+        }
+      }
+    };
+
+    u32x4_t kr[2][KL], vr[VL];
+    int id0 = -1, id1 = -1;                                  // pages of the two 16-key halves in flight
+    float ku0 = 1.f, ku1 = 1.f, vu0 = 1.f, vu1 = 1.f;
+    auto lane_of = [&](float x, int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l)); };
+    auto find_pages = [&](int key) {
+      const int p0 = key >> a.s.log2P, p1 = (key + 16) >> a.s.log2P;
+      if (p0 < ids_at || p1 >= ids_at + 64) fetch_ids(p0);
+      id0 = __builtin_amdgcn_readlane(ids, p0 - ids_at);
+      id1 = __builtin_amdgcn_readlane(ids, p1 - ids_at);
+      if constexpr (CODES) {
+        ku0 = lane_of(ku, p0 - ids_at), ku1 = lane_of(ku, p1 - ids_at);
+        vu0 = lane_of(vu, p0 - ids_at), vu1 = lane_of(vu, p1 - ids_at);
+      }
+    };
+    constexpr int ES = CODES ? 1 : 2;
+    auto at = [&](const Pages& p, int id, int key) {         // of a half's first row; pages that are not there: any
+      return p.data + (max(id, 0) * p.page + h * p.head + (key & (a.s.P - 1)) * p.row) * ES;
+    };
+    auto load_k = [&](int key) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const char* p = at(a.k, s ? id1 : id0, key + 16 * s) + (c16 * (int)a.k.row * ES + 16 * q4);
+#pragma unroll
+        for (int c = 0; c < KL; ++c) kr[s][c] = ldg128(p + 64 * c);
+      }
+    };
+    auto load_v = [&](int key) {
+#pragma unroll
+      for (int j = 0; j < VL; ++j) {
+        const int chunk = j * 64 + lane, r = chunk / VCH;    // rows of one load lie in one half
+        const bool second = j >= VL / 2;
+        vr[j] = ldg128(at(a.v, second ? id1 : id0, key + (second ? 16 : 0)) + ((r & 15) * (int)a.v.row * ES + 16 * (chunk % VCH)));
+      }
+    };
+
+    f32x4_t o[RT][ND];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kLowest;
+      l[rt] = 0.f;
+#pragma unroll
+      for (int t = 0; t < ND; ++t) o[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int key = key0 + wave * kWaveKeys;
+    if (key < key1) {
+      find_pages(key);
+      load_k(key);
+      load_v(key);
+    }
+    while (key < key1) {
+      const bool bad0 = id0 < 0, bad1 = id1 < 0;
+      // S^T of the two halves
+      f32x4_t s[RT][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KL; ++c) {
+          if constexpr (CODES) {
+            u32x4_t lo, hi;
+            decode<T>(kr[j][c], j ? ku1 : ku0, lo, hi);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              s[rt][j] = attn::mfma<T>(lo, qf[rt][2 * c], s[rt][j]);
+              s[rt][j] = attn::mfma<T>(hi, qf[rt][2 * c + 1], s[rt][j]);
+            }
+          } else {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt][j] = attn::mfma<T>(kr[j][c], qf[rt][c], s[rt][j]);
+          }
+        }
+      }
+      // V of these keys to LDS; rows past the sequence's are nobody's, and zero
+      wave_lds_fence();
+      const bool short_tile = key + kWaveKeys > w.len;
+#pragma unroll
+      for (int j = 0; j < VL; ++j) {
+        const int chunk = j * 64 + lane, r = chunk / VCH, c = chunk % VCH;
+        u32x4_t x = vr[j];
+        if constexpr (CODES) {
+          u32x4_t lo, hi;
+          decode<T>(x, j >= VL / 2 ? vu1 : vu0, lo, hi);
+          if (short_tile && key + r >= w.len) lo = hi = u32x4_t{0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4_t*>(vt + r * D + (((2 * c) ^ tile_swz<D>(r)) << 3)) = lo;
+          *reinterpret_cast<u32x4_t*>(vt + r * D + (((2 * c + 1) ^ tile_swz<D>(r)) << 3)) = hi;
+        } else {
+          if (short_tile && key + r >= w.len) x = u32x4_t{0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4_t*>(vt + r * D + ((c ^ tile_swz<D>(r)) << 3)) = x;
+        }
+      }
+      wave_lds_fence();
+      const int cur = key;
+      key += kUnit;
+      if (key < key1) {
+        find_pages(key);
+        load_k(key);
+        load_v(key);
+      }
+
+      u32x4_t ph[RT], pl[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        if (cur + kWaveKeys > all_see || bad0 || bad1) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (cur + 16 * j + 4 * q4 + i >= lim[rt] || (j ? bad1 : bad0)) s[rt][j][i] = -__builtin_inff();
+        }
+        float mx = m[rt];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][j][i]);
+        mx = max_xor32(max_xor16(mx));
+        if (__builtin_amdgcn_ballot_w64(mx > m[rt])) {
+          const float alpha = __builtin_amdgcn_exp2f((m[rt] - mx) * a.scale_log2);
+          m[rt] = mx;
+          l[rt] *= alpha;
+#pragma unroll
+          for (int t = 0; t < ND; ++t) o[rt][t] *= alpha;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = __builtin_amdgcn_exp2f((s[rt][j][i] - mx) * a.scale_log2);
+            if constexpr (T::kF16) x *= 32768.f;
+            p[4 * j + i] = x;
+            l[rt] += x;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const u32 hi = attn::pack2<T>(p[2 * i], p[2 * i + 1]);
+          ph[rt][i] = hi;
+          pl[rt][i] = attn::pack2<T>(p[2 * i] - attn::to_f32<T>(hi & 0xFFFFu), p[2 * i + 1] - attn::to_f32<T>(hi >> 16));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const int r = 4 * q4 + (c16 >> 2);
+        const u16* vp = vt + r * D + (((2 * t + ((c16 & 3) >> 1)) ^ tile_swz<D>(r)) << 3) + 4 * (c16 & 1);
+        const u32x2_t lo = lds_transposed(vp), hi = lds_transposed(vp + 16 * D);
+        const u32x4_t vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          o[rt][t] = attn::mfma<T>(vf, ph[rt], o[rt][t]);
+          o[rt][t] = attn::mfma<T>(vf, pl[rt], o[rt][t]);
+        }
+      }
+    }
+
+    // the waves' parts together: a common maximum, then sums row tile by row tile
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += shfl_xor(l[rt], 16);
+      l[rt] += shfl_xor(l[rt], 32);
+      if (q4 == 0) {
+        wm[wave][16 * rt + c16] = m[rt];
+        wl[wave][16 * rt + c16] = l[rt];
+      }
+    }
+    if (tid < ROWS) again[tid] = 0;
+    __syncthreads();
+    const bool complete = t0 == 0 && t1 == w.tiles;
+    const long slot = (2 * (long)blockIdx.x + (t0 == 0 ? 1 : 0)) * ROWS;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int rw = 16 * rt + c16;
+      const float mt = fmaxf(fmaxf(wm[0][rw], wm[1][rw]), fmaxf(wm[2][rw], wm[3][rw]));
+      const float f = __builtin_amdgcn_exp2f((m[rt] - mt) * a.scale_log2);
+      f32x4_t* const mine = reinterpret_cast<f32x4_t*>(vt);
+#pragma unroll
+      for (int t = 0; t < ND; ++t) mine[t * 64 + lane] = o[rt][t] * f;
+      __syncthreads();
+      float lt = 0.f;                                        // of the row whose outputs this thread sums
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) lt += wl[i][rw] * __builtin_amdgcn_exp2f((wm[i][rw] - mt) * a.scale_log2);
+      const int r = r0 + rw, i = r / a.gqa;
+      if (r < w.rows) {
+        const float inv = lt > 0.f ? 1.f / lt : 0.f;
+        float zero = lt - lt;                                // NaN once an output is not finite
+        for (int x = wave; x < ND; x += kWaves) {
+          f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < kWaves; ++k) sum += reinterpret_cast<const f32x4_t*>(tiles[k])[x * 64 + lane];
+          if (complete) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) zero = __builtin_fmaf(sum[k], 0.f, zero);
+            *reinterpret_cast<u32x2_t*>(a.out + (w.start + i) * a.orow + (h * a.gqa + r - i * a.gqa) * a.ohead + 16 * x + 4 * q4) =
+                u32x2_t{attn::pack2<T>(sum[0] * inv, sum[1] * inv), attn::pack2<T>(sum[2] * inv, sum[3] * inv)};
+          } else {
+            *reinterpret_cast<f32x4_t*>(a.opart + (slot + rw) * D + 16 * x + 4 * q4) = sum;
+          }
+        }
+        if (complete) {
+          if (zero != 0.f) again[rw] = 1;
+        } else if (wave == 0 && q4 == 0) {
+          a.mpart[2 * slot + rw] = mt;
+          a.mpart[2 * slot + ROWS + rw] = lt;
+        }
+      }
+      __syncthreads();
+    }
+    if (complete) {
+      __threadfence_block();
+      for (int r = wave; r < ROWS; r += kWaves)
+        if (again[r]) {
+          const int i = (r0 + r) / a.gqa;
+          plain_row<T, D, CODES>(a, b, w.start + i, h * a.gqa + r0 + r - i * a.gqa, keys_seen(a, b, w.n, w.len, i));
+        }
+    }
+    __syncthreads();
+
+    u += t1 - t0;
+    local += t1 - t0;
+    if (u < u_end && local == a.Hk * w.groups * w.tiles) {
+      local = 0;
+      do {
+        ++b;
+        w = work_of<RT>(a, b);
+        w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+      } while (w.rows == 0 && b < a.s.B - 1);
+      if (w.rows == 0) return;
+    }
+  }
+}
+
+// Joins the parts of a KV head's rows: out = sum 2^(m_j - m) o_j / sum 2^(m_j - m) l_j over the runs j that have some of its
+// keys, in their order. A wave a row.
+template <class T, int D, int RT, bool CODES>
+__global__ __launch_bounds__(kAttnThreads) void join_kernel(const AttnArgs a, int workgroups) {
+  constexpr int ROWS = 16 * RT, C = D / 64;
+  typedef float cols_t __attribute__((ext_vector_type(C)));
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
+  Work w = work_of<RT>(a, b);
+  w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+  if ((int)blockIdx.y * kWaves >= w.rows) return;
+  // units before this sequence, and of all
+  int before = 0;
+  const int units = all_units<RT>(a, b, &before);
+  if (!units) return;
+  const int run = run_of(a, units, workgroups);
+  for (int r = blockIdx.y * kWaves + wave; r < w.rows; r += gridDim.y * kWaves) {
+    const int group = r / ROWS, rw = r - group * ROWS;
+    const int u0 = before + (h * w.groups + group) * w.tiles, u1 = u0 + w.tiles;
+    const int j0 = u0 / run, j1 = (u1 - 1) / run;
+    if (j0 == j1) continue;
+    auto slot = [&](int j) { return (2 * (long)j + (j == j0 ? 1 : 0)) * ROWS; };
+    float m = kLowest;
+    for (int j = j0 + lane; j <= j1; j += 64) m = fmaxf(m, a.mpart[2 * slot(j) + rw]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, shfl_xor(m, x));
+    cols_t acc;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    float l = 0.f;
+    for (int j = j0; j <= j1; ++j) {
+      const float f = __builtin_amdgcn_exp2f((a.mpart[2 * slot(j) + rw] - m) * a.scale_log2);
+      l += f * a.mpart[2 * slot(j) + ROWS + rw];
+      const cols_t x = *reinterpret_cast<const cols_t*>(a.opart + (slot(j) + rw) * D + C * lane);
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(f, x[c], acc[c]);
+    }
+    const int i = r / a.gqa, head = h * a.gqa + r - i * a.gqa;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    u16* op = a.out + (w.start + i) * a.orow + head * a.ohead + C * lane;
+    float zero = l - l;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      zero = __builtin_fmaf(acc[c], 0.f, zero);
+      op[c] = attn::from_f32<T>(acc[c] * inv);
+    }
+    if (__builtin_amdgcn_ballot_w64(zero != 0.f))
+      plain_row<T, D, CODES>(a, b, w.start + i, head, keys_seen(a, b, w.n, w.len, i));
+  }
+}
+
+template <class T, int D, int RT, bool CODES>
+int launch_rows(const AttnArgs& a, int workgroups, int most_rows, hipStream_t s) {
+  hipLaunchKernelGGL((rows_kernel<T, D, RT, CODES>), dim3((unsigned)workgroups), dim3(kAttnThreads), 0, s, a);
+  const int st = check_launch("paged_attention");
+  if (st || a.whole) return st;
+  const unsigned y = (unsigned)((std::min(most_rows, 16 * RT) + kWaves - 1) / kWaves);     // more rows: a loop
+  hipLaunchKernelGGL((join_kernel<T, D, RT, CODES>), dim3((unsigned)(a.s.B * a.Hk), y), dim3(kAttnThreads), 0, s, a, workgroups);
+  return check_launch("paged_attention(join)");
+}
+
+// Each (element type, head dim) in its own translation unit
+template <class T, int D>
+int launch(const AttnArgs& a, int rt, bool codes, int workgroups, int most_rows, hipStream_t s);
+
+#define DSPARK_PAGED_ATTN(T, D)                                                                                       \
+  template <>                                                                                                        \
+  int launch<T, D>(const AttnArgs& a, int rt, bool codes, int workgroups, int most_rows, hipStream_t s)
+DSPARK_PAGED_ATTN(BF16, 64);
+DSPARK_PAGED_ATTN(BF16, 128);
+DSPARK_PAGED_ATTN(BF16, 256);
+DSPARK_PAGED_ATTN(F16, 64);
+DSPARK_PAGED_ATTN(F16, 128);
+DSPARK_PAGED_ATTN(F16, 256);
+
+template <class T, int D>
+int launch_rt(const AttnArgs& a, int rt, bool codes, int workgroups, int most_rows, hipStream_t s) {
+#define DSPARK_ROWS(RT) \
+  (codes ? launch_rows<T, D, RT, true>(a, workgroups, most_rows, s) : launch_rows<T, D, RT, false>(a, workgroups, most_rows, s))
+  if constexpr (D <= 128) {
+    if (rt == 4) return DSPARK_ROWS(4);
+  }
+  return rt >= 2 ? DSPARK_ROWS(2) : DSPARK_ROWS(1);
+#undef DSPARK_ROWS
+}
+
+}  // namespace paged
+}  // namespace dspark

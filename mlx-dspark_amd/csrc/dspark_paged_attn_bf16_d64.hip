@@ -1,0 +1,10 @@
+// Attention over paged caches: bf16, head dim 64.
+#include "dspark_paged_attn.h"
+
+namespace dspark {
+namespace paged {
+
+DSPARK_PAGED_ATTN(BF16, 64) { return launch_rt<BF16, 64>(a, rt, codes, workgroups, most_rows, s); }
+
+}  // namespace paged
+}  // namespace dspark

@@ -1517,3 +1517,79 @@ def paged_read(k_pages, v_pages, pages: torch.Tensor, *, dtype: torch.dtype = to
         _call_on(dev, "dspark_paged_read",
                  _READ_ARGS.pack(dt, codes, Hk, D, P, pool, ids.data_ptr(), N, *fields, k.data_ptr(), v.data_ptr()))
     return (k, v) if pool else (k.zero_(), v.zero_())
+
+
+@functools.lru_cache(maxsize=256)
+def paged_attention_workspace_bytes(sequences: int, hq: int, hk: int, d: int, rows: int, max_rows: int, max_len: int) -> int:
+    """Workspace bytes of :func:`paged_attention` (``max_len``: positions of the table's pages); 0 where it refuses the call."""
+    return int(_lib.load().dspark_paged_attention_workspace(sequences, hq, hk, d, rows, max_rows, max_len))
+
+
+_PAGED_ATTN_ARGS = struct.Struct("=10qd29q")
+
+
+def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, *,
+                    scale: float, causal: bool = True, max_rows: int | None = None, max_len: int | None = None,
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a step's rows over their sequences' pages -> [T, Hq, D]: decoded tokens, verify blocks and prompt chunks
+    of any lengths together, the sequences, pages and arguments as in :func:`paged_append`, which writes the rows' own keys
+    and values first.
+
+    Row i of a sequence's n sees the positions up to its own, ``lens[b] - n + i`` (``causal``), or all ``lens[b]``: an
+    encoder's states, kept in pages. fp32 scores, probabilities and sums; zeros for a row that sees nothing; values that
+    are not finite count only where a row sees them. Positions of pages that the pool does not have are not seen.
+
+    ``max_rows`` (rows of one sequence) and ``max_len`` (positions; default: what the table has room for) are the
+    host's bounds: positions from ``max_len`` on, rounded up to a page, are not seen; more rows than ``max_rows`` are
+    served too, only slower. ``out``: rows of no sequence are left as they are there; in a new one they are zeros.
+    ``workspace`` of :func:`paged_attention_workspace_bytes`, 16-byte aligned, any content, for one call at a time, else
+    allocated."""
+    what = "paged_attention"
+    dev = _one_device(what, q, *_pages_parts(k_pages), *_pages_parts(v_pages), table, starts, lens, out, workspace)
+    dtype = q.dtype
+    dt = ATTN_DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"{what}: q {dtype} (bfloat16 or float16)")
+    codes, (pool, Hk, P, D), pages = _both_pages(what, k_pages, v_pages, dtype, False)
+    if q.dim() != 3 or q.shape[2] != D or (Hk and q.shape[1] % Hk):
+        raise ValueError(f"{what}: q must be [rows, a multiple of {Hk} heads, {D}], got {list(q.shape)}")
+    scale = float(scale)
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"{what}: scale={scale} (positive)")
+    T, Hq, _ = q.shape
+    _no_autograd(what, q, out)
+    clear = out is None
+    if not clear:
+        if out.dtype is not dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 \
+                or out.data_ptr() % 16:
+            raise ValueError(f"{what}: out must be {dtype} {list(q.shape)} with unit last stride, aligned to 16 bytes")
+        _as_stored(what, out)
+        _no_repeats(what, out)
+        if q.numel() and _spans_meet(q, out):
+            raise ValueError(f"{what}: out overlaps q")
+    q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
+    if clear:
+        out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+    seqs, keep = _sequences(what, table, starts, lens, T)
+    B, W = seqs[4], seqs[5]
+    rows = T if max_rows is None else min(int(max_rows), T)
+    if max_len is not None:
+        W = min(W, -(-int(max_len) // P))
+    if rows < 1 and T or W < 0:
+        raise ValueError(f"{what}: max_rows={max_rows}, max_len={max_len}")
+    if T and Hq:
+        if B and W and pool:
+            nbytes = paged_attention_workspace_bytes(B, Hq, Hk, D, T, rows, W * P)
+            if nbytes == 0:
+                raise ValueError(f"{what}: {T} rows of {Hq} / {Hk} heads, {B} sequences of {W} pages: {_lib.last_error()}")
+            if workspace is None:
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            elif workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.data_ptr() % 16:
+                raise ValueError(f"{what}: workspace: {nbytes} contiguous bytes, aligned to 16, needed")
+            _call_on(dev, "dspark_paged_attention",
+                     _PAGED_ATTN_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, bool(causal), clear, rows, scale, q.data_ptr(), *q_st,
+                                           out.data_ptr(), *out.stride()[:2], *pages, *seqs[:5], W, T, workspace.data_ptr(),
+                                           workspace.nbytes))
+        elif clear:
+            out.zero_()
+    return out

@@ -80,3 +80,16 @@ def test_logprobs_closed_forms():
     lp, h, ids, best = paged_ref.logprobs([-np.inf, np.nan], 0, 2)
     assert lp == -np.inf and h == 0 and ids.tolist() == [0, 1] and (best == -np.inf).all()
     assert paged_ref.logprobs([1.0, 2.0], 7)[0] == -np.inf
+
+
+def test_attention_of_many_keys_is_the_loops():
+    from tests._paged import attention
+
+    g = np.random.default_rng(1)
+    k, v = (paged_ref.Pages(g.standard_normal((6, 2, 4, 8))) for _ in range(2))
+    q = g.standard_normal((9, 4, 8))
+    table = np.array([[2, 0, 5], [1, -1, 7], [3, 4, 0]])
+    for starts, lens in (([0, 2, 5, 8], [6, 12, 5]), ([0, 5, 5, 6], [3, 12, 99]), ([0, 1, 99, 6], [1, 1, 1])):
+        for causal in (True, False):
+            np.testing.assert_allclose(attention(q, k, v, table, starts, lens, 0.3, causal)[0],
+                                       paged_ref.attention(q, k, v, table, starts, lens, 0.3, causal), rtol=1e-12, atol=1e-14)
