@@ -825,6 +825,36 @@ size_t dspark_paged_attention_workspace(int64_t count, int64_t Hq, int64_t Hk, i
 
 int dspark_paged_attention(const dspark_paged_attention_args* args, dspark_stream stream);
 
+/* ------------------------------------------------------------------ what tokens are reported with */
+
+/*
+ * Of every row of logits [rows, V] (bf16, fp16 or fp32, row stride ld, any alignment; V up to 2^28, rows up to 2^20), with
+ * log p the logarithm of softmax(x / temperature):
+ *   logprobs[r] = log p(tokens[r]) (-inf for a token outside 0..V-1), entropy[r] = -sum p log p, and the `top` (up to 64, and
+ *   V) largest logits' tokens, falling, equal ones by index, with their log p (row stride top).
+ * NaN counts as -inf; infinite logits share all the probability; a row of nothing but -inf and NaN has log p = -inf
+ * throughout and an entropy of 0. workspace >= dspark_token_logprobs_workspace(rows, V, top) bytes, 16-byte aligned, of any
+ * content, one call's at a time.
+ */
+typedef struct dspark_token_logprobs_args { /* every field is 8 bytes */
+  int64_t dtype;
+  const void* logits;
+  int64_t ld, rows, V;
+  const int32_t* tokens;
+  int64_t top;
+  double temperature;
+  float* logprobs;
+  float* entropy;
+  int32_t* top_tokens;
+  float* top_logprobs;
+  void* workspace;
+  int64_t workspace_bytes;
+} dspark_token_logprobs_args;
+
+size_t dspark_token_logprobs_workspace(int64_t rows, int64_t V, int64_t top);
+
+int dspark_token_logprobs(const dspark_token_logprobs_args* args, dspark_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,434 @@
+// Log probabilities of given tokens, the entropy of their distributions and the best alternatives (gfx950).
+//
+// With z = (x - max x) / temperature over a row's logits, S = sum e^z and U = sum z e^z:
+//   log p(token) = z_token - ln S,   entropy = ln S - U / S,   alternatives: the largest x, equal ones by index.
+// One pass: every lane keeps its running maximum with S and U relative to it (U' = f (U + delta S) where the maximum
+// rises by -delta in the exponent), in fp32 and units of log 2; ln S and the differences that leave the call are fp64. NaN
+// counts as -inf; with infinite logits those share all of it; a row of nothing has -inf everywhere and no entropy.
+//
+// The alternatives come out of the same pass. A candidate is a 64-bit key, value before inverted index, so that no two are
+// equal and the order is total. A wave keeps a list of candidates in LDS and a least key, under which k better ones are
+// known; 32 values a lane are compared by their maximum, which the sums need anyway, and looked at only where it reaches the
+// least key. The least key starts as the k-th of the 64 lanes' maxima, rises when a full list is cut to its k best, and
+// is shared by the workgroup's waves.
+//
+// Bound by the bytes of the logits, with the exponential (a quarter of the rate) and about 10 more instructions a value
+// close behind. Many rows: a workgroup a row; few: up to 64 workgroups, joined by a second launch.
+#include <algorithm>
+#include <cmath>
+
+#include "dspark_common.h"
+
+namespace dspark {
+namespace {
+
+using u64 = unsigned long long;
+
+constexpr int kScoreThreads = 256;
+constexpr int kScoreWaves = kScoreThreads / 64;
+constexpr int kPer = 32;                       // values of a lane's step
+constexpr int kMostTop = 64;
+constexpr int kList = 320;                     // candidates of a wave
+constexpr int kMostSegments = 64;              // of a row: a lane each where they are joined
+constexpr float kScoreLowest = -3.402823466e38f;
+constexpr float kNothing = -1e4f;              // an exponent whose power of two is 0, times which 0 is 0
+
+struct ScoreArgs {
+  const char* x;
+  long ld;                                     // row stride in elements
+  int rows, V, top, segments;
+  float c;                                     // log2(e) / temperature
+  double temperature;
+  const int* tokens;
+  float* given;
+  float* entropy;
+  int* ids;                                    // [rows][top]
+  float* best;
+  float* stats;                                // [rows][segments][3]
+  u64* keys;                                   // [rows][segments][top], falling; 0: none
+};
+
+template <int DT> struct Logit;
+template <> struct Logit<DSPARK_DTYPE_BF16> {
+  using t = u16;
+  static __device__ __forceinline__ float get(u16 v) { return bf2f(v); }
+};
+template <> struct Logit<DSPARK_DTYPE_F16> {
+  using t = u16;
+  static __device__ __forceinline__ float get(u16 v) { return (float)__builtin_bit_cast(_Float16, v); }
+};
+template <> struct Logit<DSPARK_DTYPE_F32> {
+  using t = float;
+  static __device__ __forceinline__ float get(float v) { return v; }
+};
+
+// A key falls with the value, then with the index; NaN as -inf, -0 as 0. Never 0.
+__device__ __forceinline__ u64 key_of(float x, int i) {
+  x = x == x ? x + 0.f : -__builtin_inff();
+  const u32 b = __builtin_bit_cast(u32, x);
+  return (u64)(b ^ ((int)b < 0 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (u32)~i;
+}
+__device__ __forceinline__ float value_of(u64 k) {
+  const u32 b = (u32)(k >> 32);
+  return __builtin_bit_cast(float, b ^ ((int)b < 0 ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int index_of(u64 k) { return (int)~(u32)k; }
+
+__device__ __forceinline__ u64 lane_key(u64 k, int l) {
+  return (u64)(u32)__builtin_amdgcn_readlane((int)(k >> 32), l) << 32 | (u32)__builtin_amdgcn_readlane((int)(u32)k, l);
+}
+__device__ __forceinline__ u64 xor_key(u64 k, int m) {
+  const int at = (__lane_id() ^ m) << 2;
+  return (u64)(u32)__builtin_amdgcn_ds_bpermute(at, (int)(k >> 32)) << 32 | (u32)__builtin_amdgcn_ds_bpermute(at, (int)(u32)k);
+}
+
+struct Stats {
+  float m, s, u;                               // maximum, sum of 2^d, sum of d 2^d, d = (x - m) c
+};
+
+__device__ __forceinline__ Stats join(Stats a, Stats b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = fmaxf((a.m - m) * c, kNothing), db = fmaxf((b.m - m) * c, kNothing);
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  return Stats{m, fa * a.s + fb * b.s, fa * (a.u + da * a.s) + fb * (b.u + db * b.s)};
+}
+__device__ __forceinline__ Stats join_wave(Stats s, float c) {
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) s = join(s, Stats{shfl_xor(s.m, x), shfl_xor(s.s, x), shfl_xor(s.u, x)}, c);
+  return s;
+}
+
+// The k best of a wave's list of n, in order at its start; how many there are
+__device__ __forceinline__ int cut_list(u64* list, int n, int k) {
+  constexpr int N = kList / 64;
+  const int lane = __lane_id();
+  u64 mine[N];
+  int rank[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mine[i] = 64 * i + lane < n ? list[64 * i + lane] : 0;
+    rank[i] = 0;
+  }
+  for (int j = 0; j < n; ++j) {
+    const u64 o = list[j];
+#pragma unroll
+    for (int i = 0; i < N; ++i) rank[i] += o > mine[i] ? 1 : 0;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (mine[i] && rank[i] < k) list[rank[i]] = mine[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return min(n, k);
+}
+
+// Infinite logits of a row, counted by one wave
+template <int DT>
+__device__ __forceinline__ int infinite_logits(const ScoreArgs& a, long row) {
+  using T = typename Logit<DT>::t;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  int n = 0;
+#pragma unroll 1
+  for (int i = __lane_id(); i < a.V; i += 64) n += Logit<DT>::get(x[i]) == __builtin_inff() ? 1 : 0;
+#pragma unroll 1
+  for (int d = 1; d < 64; d *= 2) n += __builtin_amdgcn_ds_bpermute((__lane_id() ^ d) << 2, n);
+  return n;
+}
+
+// What a row's sums and keys (falling, in LDS or memory) come to; by one wave
+template <int DT>
+__device__ __forceinline__ void finish_row(const ScoreArgs& a, long row, Stats s, u64 mine) {
+  using T = typename Logit<DT>::t;
+  const int lane = __lane_id();
+  double log_sum = log((double)s.s), entropy = log_sum - 0.69314718055994531 * ((double)s.u / (double)s.s);
+  const bool infinite = s.m == __builtin_inff();
+  if (infinite) entropy = log_sum = log((double)infinite_logits<DT>(a, row));
+  const bool none = !infinite && !(s.s > 0.f);
+  auto log_p = [&](float x) {
+    if (infinite) return x == s.m ? (float)-log_sum : -__builtin_inff();
+    if (none || x != x) return -__builtin_inff();
+    return (float)(((double)x - (double)s.m) / a.temperature - log_sum);
+  };
+  if (lane == 0) {
+    const int t = a.tokens[row];
+    a.given[row] = (unsigned)t < (unsigned)a.V ? log_p(Logit<DT>::get((reinterpret_cast<const T*>(a.x) + row * a.ld)[t])) : -__builtin_inff();
+    a.entropy[row] = none ? 0.f : (float)(entropy > 0. ? entropy : 0.);
+  }
+  if (lane < a.top) {
+    a.ids[row * a.top + lane] = index_of(mine);
+    a.best[row * a.top + lane] = log_p(value_of(mine));
+  }
+}
+
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a) {
+  using T = typename Logit<DT>::t;
+  constexpr int E = 16 / sizeof(T), NL = kPer / E;           // values of a 16-byte load, loads of a step
+  struct alignas(16) Vec { T v[E]; };
+  __shared__ u64 lists[kScoreWaves][TOP ? kList : 1];
+  __shared__ u64 least_of_all;
+  __shared__ Stats parts[kScoreWaves];
+  __shared__ int counts[kScoreWaves];
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  const long row = blockIdx.x / a.segments;
+  const int seg = blockIdx.x - (int)row * a.segments;
+  const T* const x0 = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  // 16-byte chunks from the one that the row starts in: value i is number i + off of them
+  const int off = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
+  const Vec* const chunks = reinterpret_cast<const Vec*>(x0 - off);
+  const int nc = (int)(((long)a.V + off + E - 1) / E), per = (nc + a.segments - 1) / a.segments;
+  const int c0 = (int)min((long)seg * per, (long)nc), c1 = min(c0 + per, nc);
+  u64* const list = lists[wave];
+  int n = 0;                                                 // of the list
+  const int full = min(kList - 64, 2 * a.top + 64);
+  u64 least = 0;
+  if (TOP) {
+    if (threadIdx.x == 0) least_of_all = 0;
+    __syncthreads();
+  }
+
+  auto load = [&](Vec (&v)[NL], int c) {
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int k = c + 64 * j + lane;
+      if (k < c1 && k * E >= off && (long)(k + 1) * E <= (long)a.V + off) {
+        v[j] = chunks[k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const long i = (long)k * E + e - off;
+          T t;
+          if constexpr (sizeof(T) == 4) t = __builtin_nanf("");
+          else t = 0x7FFF;                                   // NaN: nothing
+          if (k < c1 && i >= 0 && i < a.V) t = x0[i];
+          v[j].v[e] = t;
+        }
+      }
+    }
+  };
+
+  Stats st{kScoreLowest, 0.f, 0.f};
+  const int step = 64 * NL * kScoreWaves;
+  int c = c0 + wave * 64 * NL;
+  Vec next[NL];
+  if (c < c1) load(next, c);
+  while (c < c1) {
+    float x[kPer];
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[j * E + e] = Logit<DT>::get(next[j].v[e]);
+    const int cur = c;
+    c += step;
+    if (c < c1) load(next, c);
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i]);
+    const float m = fmaxf(st.m, top);
+    const float d0 = fmaxf((st.m - m) * a.c, kNothing), f = __builtin_amdgcn_exp2f(d0);
+    st.u = f * (st.u + d0 * st.s);
+    st.s *= f;
+    st.m = m;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float d = fmaxf((x[i] - m) * a.c, kNothing), e = __builtin_amdgcn_exp2f(d);
+      st.s += e;
+      st.u = __builtin_fmaf(e, d, st.u);
+    }
+    if constexpr (TOP) {
+      const u64 shared = least_of_all;
+      least = shared > least ? shared : least;
+      const u64 some = __builtin_amdgcn_ballot_w64(top >= (least ? value_of(least) : -__builtin_inff()));
+      if (!some) continue;
+      auto index = [&](int i) { return (int)((long)(cur + 64 * (i / E) + lane) * E + i % E - off); };
+      auto key = [&](int i) {
+        const int at = index(i);
+        return at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1 ? key_of(x[i], at) : 0;
+      };
+      if (__builtin_popcountll(some) >= a.top) {
+        // the k-th of the lanes' best: k values at least reach it
+        u64 best = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const u64 k = key(i);
+          best = k > best ? k : best;
+        }
+        int rank = 0;
+        for (int j = 0; j < 64; ++j) rank += lane_key(best, j) > best ? 1 : 0;
+        const u64 kth = __builtin_amdgcn_ballot_w64(rank == a.top - 1 && best != 0);
+        if (kth) {
+          const u64 k = lane_key(best, __builtin_ctzll(kth));
+          if (k > least) {
+            least = k;
+            if (lane == 0) atomicMax(&least_of_all, k);
+          }
+        }
+      }
+      const float least_value = least ? value_of(least) : -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        // (NaN counts as -inf)
+        const bool maybe = !(x[i] < least_value);
+        if (!__builtin_amdgcn_ballot_w64(maybe)) continue;
+        const u64 k = maybe ? key(i) : 0;
+        const u64 in = __builtin_amdgcn_ballot_w64(k != 0 && k >= least);
+        if (!in) continue;
+        if (k != 0 && k >= least) list[n + __builtin_popcountll(in & ((1ull << lane) - 1))] = k;
+        n = uniform(n + __builtin_popcountll(in));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (n > full) {
+          n = uniform(cut_list(list, n, a.top));
+          const u64 k = list[a.top - 1];
+          if (k > least) {
+            least = k;
+            if (lane == 0) atomicMax(&least_of_all, k);
+          }
+        }
+      }
+    }
+  }
+
+  st = join_wave(st, a.c);
+  if (TOP) {
+    n = uniform(cut_list(list, n, a.top));
+    if (lane == 0) counts[wave] = n;
+  }
+  if (lane == 0) parts[wave] = st;
+  __syncthreads();
+  if (TOP && kScoreWaves > 1) {
+    // every wave's keys find their places among all
+    u64 mine[kScoreWaves];
+    int rank[kScoreWaves];
+    for (int w = 0; w < kScoreWaves; ++w) {
+      mine[w] = lane < counts[w] ? lists[w][lane] : 0;
+      rank[w] = 0;
+    }
+    if (wave == 0) {
+      for (int w = 0; w < kScoreWaves; ++w)
+        for (int j = 0; j < counts[w]; ++j) {
+          const u64 o = lists[w][j];
+#pragma unroll
+          for (int v = 0; v < kScoreWaves; ++v) rank[v] += o > mine[v] ? 1 : 0;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (lane < a.top) lists[0][lane] = 0;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int v = 0; v < kScoreWaves; ++v)
+        if (mine[v] && rank[v] < a.top) lists[0][rank[v]] = mine[v];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < kScoreWaves; ++w) st = join(st, parts[w], a.c);
+  const u64 mine = TOP && lane < a.top ? lists[0][lane] : 0;
+  if (a.segments == 1) {
+    finish_row<DT>(a, row, st, mine);
+    return;
+  }
+  if (lane == 0) {
+    float* to = a.stats + 3 * (row * a.segments + seg);
+    to[0] = st.m, to[1] = st.s, to[2] = st.u;
+  }
+  if (TOP && lane < a.top) a.keys[(row * a.segments + seg) * a.top + lane] = mine;
+}
+
+// A row's segments together, by one wave: a lane has a segment's sums, and the head of its keys
+template <int DT>
+__global__ __launch_bounds__(64) void join_scores_kernel(const ScoreArgs a) {
+  const long row = blockIdx.x;
+  const int lane = __lane_id();
+  Stats s{kScoreLowest, 0.f, 0.f};
+  if (lane < a.segments) {
+    const float* from = a.stats + 3 * (row * a.segments + lane);
+    s = Stats{from[0], from[1], from[2]};
+  }
+  s = join_wave(s, a.c);
+  const u64* keys = a.keys + (row * a.segments + lane) * a.top;
+  int at = 0;
+  u64 head = lane < a.segments && a.top ? keys[0] : 0, mine = 0;
+  for (int i = 0; i < a.top; ++i) {
+    u64 best = head;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const u64 o = xor_key(best, x);
+      best = o > best ? o : best;
+    }
+    if (lane == i) mine = best;
+    if (head == best && head) head = ++at < a.top ? keys[at] : 0;
+  }
+  finish_row<DT>(a, row, s, mine);
+}
+
+// Workgroups of a row: enough for two a CU together, each with at least 2048 values
+int score_segments(int64_t rows, int64_t V) {
+  const int64_t want = (512 + rows - 1) / rows;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, kMostSegments, V / 2048}));
+}
+
+template <int DT>
+int launch_score(const ScoreArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.rows * (long)a.segments)), block(kScoreThreads);
+  if (a.top) hipLaunchKernelGGL((score_kernel<DT, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((score_kernel<DT, false>), grid, block, 0, s, a);
+  const int st = check_launch("token_logprobs");
+  if (st || a.segments == 1) return st;
+  hipLaunchKernelGGL((join_scores_kernel<DT>), dim3((unsigned)a.rows), dim3(64), 0, s, a);
+  return check_launch("token_logprobs(join)");
+}
+
+}  // namespace
+}  // namespace dspark
+
+using namespace dspark;
+
+extern "C" size_t dspark_token_logprobs_workspace(int64_t rows, int64_t V, int64_t top) {
+  if (rows < 1 || rows > (1 << 20) || V < 1 || V > (1 << 28) || top < 0 || top > kMostTop || top > V) return 0;
+  const int64_t n = score_segments(rows, V);
+  return n == 1 ? 256 : (size_t)(rows * n * (8 * top + 12) + 256);
+}
+
+extern "C" int dspark_token_logprobs(const dspark_token_logprobs_args* p, dspark_stream stream) {
+  const char* what = "token_logprobs";
+  if (!p || !p->logits || !p->tokens || !p->logprobs || !p->entropy || !p->workspace || (p->top && (!p->top_tokens || !p->top_logprobs)))
+    return fail(DSPARK_ERR_ARG, "%s: null pointer", what);
+  const size_t need = dspark_token_logprobs_workspace(p->rows, p->V, p->top);
+  if (!need)
+    return fail(DSPARK_ERR_SHAPE, "%s: %ld rows (up to 2^20) of %ld logits (up to 2^28), the best %ld (up to %d and all)", what,
+                (long)p->rows, (long)p->V, (long)p->top, kMostTop);
+  if (!(p->temperature >= 1e-30 && p->temperature <= 1e30)) return fail(DSPARK_ERR_ARG, "%s: temperature %g", what, p->temperature);
+  const int es = p->dtype == DSPARK_DTYPE_F32 ? 4 : 2;
+  if (!aligned(p->logits, es)) return fail(DSPARK_ERR_ALIGN, "%s: logits need the alignment of their type", what);
+  if (!aligned(p->workspace, 16) || (size_t)p->workspace_bytes < need)
+    return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %ld < %zu bytes, or not 16-byte aligned", what, (long)p->workspace_bytes, need);
+  ScoreArgs a = {};
+  a.x = static_cast<const char*>(p->logits);
+  a.ld = p->ld;
+  a.rows = (int)p->rows;
+  a.V = (int)p->V;
+  a.top = (int)p->top;
+  a.segments = score_segments(p->rows, p->V);
+  a.c = (float)(1.44269504088896340736 / p->temperature);
+  a.temperature = p->temperature;
+  a.tokens = p->tokens;
+  a.given = p->logprobs;
+  a.entropy = p->entropy;
+  a.ids = p->top_tokens;
+  a.best = p->top_logprobs;
+  a.keys = static_cast<u64*>(p->workspace);
+  a.stats = reinterpret_cast<float*>(a.keys + p->rows * a.segments * p->top);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (p->dtype) {
+    case DSPARK_DTYPE_BF16: return launch_score<DSPARK_DTYPE_BF16>(a, s);
+    case DSPARK_DTYPE_F16: return launch_score<DSPARK_DTYPE_F16>(a, s);
+    case DSPARK_DTYPE_F32: return launch_score<DSPARK_DTYPE_F32>(a, s);
+    default: return fail(DSPARK_ERR_UNSUPPORTED, "%s: dtype %ld", what, (long)p->dtype);
+  }
+}

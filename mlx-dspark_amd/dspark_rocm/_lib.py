@@ -195,6 +195,8 @@ SIGNATURES: dict[str, tuple] = {
     "dspark_paged_read": (c_int, [c_char_p, c_void_p]),
     "dspark_paged_attention_workspace": (c_size_t, [c_i64] * 7),
     "dspark_paged_attention": (c_int, [c_char_p, c_void_p]),
+    "dspark_token_logprobs_workspace": (c_size_t, [c_i64] * 3),
+    "dspark_token_logprobs": (c_int, [c_char_p, c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -1082,6 +1082,67 @@ def speculative_verify(logits: torch.Tensor, draft: torch.Tensor, uniforms: torc
     return n, tokens, draft_p
 
 
+# ---------------------------------------------------------------------------- what tokens are reported with
+
+MOST_ALTERNATIVES = 64
+
+
+@functools.lru_cache(maxsize=256)
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top: int = 0) -> int:
+    """Workspace bytes of :func:`token_logprobs`; 0 where it refuses the sizes."""
+    return int(_lib.load().dspark_token_logprobs_workspace(rows, vocab, top))
+
+
+_SCORE_ARGS = struct.Struct("=7qd6q")
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, temperature: float = 1.0,
+                   workspace: torch.Tensor | None = None):
+    """What a token is reported with, in one pass over its logits: ``(logprobs fp32 [...], entropy fp32 [...], top_tokens int32
+    [..., top], top_logprobs fp32 [..., top])`` for logits bf16, fp16 or fp32 [..., V] and tokens int32 / int64 [...].
+
+    ``logprobs``: the logarithm of each token's probability under softmax(logits / temperature), the whole distribution that
+    :func:`sampling_probs` cuts (-inf for a token outside the vocabulary); ``entropy`` of that distribution, in nats;
+    ``top`` (up to 64): the tokens of the largest logits, falling, equal ones by index, and their log probabilities.
+    NaN counts as -inf, infinite logits share all the probability, and a row of nothing but -inf and NaN has -inf
+    throughout and an entropy of 0. ``workspace`` of :func:`token_logprobs_workspace_bytes`, 16-byte aligned, any content, for
+    one call at a time, else allocated."""
+    what = "token_logprobs"
+    dev = _one_device(what, logits, tokens, workspace)
+    dt = DEQUANT_DTYPES.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"{what}: logits {logits.dtype} (bfloat16, float16 or float32)")
+    shape = logits.shape
+    top = int(top)
+    if len(shape) < 1 or shape[-1] < 1 or not 0 <= top <= min(MOST_ALTERNATIVES, shape[-1]):
+        raise ValueError(f"{what}: logits {list(shape)}, top={top} (up to {MOST_ALTERNATIVES} and the vocabulary)")
+    t, _, _ = check_sampler(temperature, 0, 1.0)
+    _no_autograd(what, logits)
+    tokens = _ints(what, "tokens", tokens, shape[:-1])
+    if logits.is_neg():
+        logits = logits.resolve_neg()
+    V = shape[-1]
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    rows, (ld, unit) = x.shape[0], x.stride()
+    if (unit != 1 and V > 1) or ld < 0:
+        x, ld = x.contiguous(), V
+    given, entropy = (torch.empty(shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
+    ids = torch.empty((*shape[:-1], top), dtype=torch.int32, device=dev)
+    best = torch.empty((*shape[:-1], top), dtype=torch.float32, device=dev)
+    if rows:
+        nbytes = token_logprobs_workspace_bytes(rows, V, top)
+        if nbytes == 0:
+            raise ValueError(f"{what}: {rows} rows (up to 2^20) of {V} logits (up to 2^28)")
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        elif workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.data_ptr() % 16:
+            raise ValueError(f"{what}: workspace: {nbytes} contiguous bytes, aligned to 16, needed")
+        _call_on(dev, "dspark_token_logprobs",
+                 _SCORE_ARGS.pack(dt, x.data_ptr(), ld, rows, V, tokens.data_ptr(), top, t, given.data_ptr(), entropy.data_ptr(),
+                                  ids.data_ptr(), best.data_ptr(), workspace.data_ptr(), workspace.nbytes))
+    return given, entropy, ids, best
+
+
 # ---------------------------------------------------------------------------- rotary positions, quantized cache rows
 
 ROPE_DTYPES = DEQUANT_DTYPES
