@@ -198,10 +198,26 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Zeros in rows of no sequence
+template <int D>
+__device__ __forceinline__ void clear_rows(const AttnArgs& a) {
+  constexpr int CH = D / 8;
+  const int lane = __lane_id();
+  for (int t = blockIdx.x; t < a.s.T; t += gridDim.x) {
+    bool has = false;
+    for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+      const Seq q = sequence(a.s, min(b0 + lane, a.s.B - 1));
+      has |= q.n > 0 && t >= q.start && t < q.start + q.n;
+    }
+    if (__builtin_amdgcn_ballot_w64(has)) continue;
+    for (int i = threadIdx.x; i < a.Hq * CH; i += kAttnThreads)
+      *reinterpret_cast<u32x4_t*>(a.out + t * a.orow + i / CH * a.ohead + 8 * (i % CH)) = u32x4_t{0u, 0u, 0u, 0u};
+  }
+}
+
 template <class T, int D, int RT, bool CODES>
 __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) void rows_kernel(const AttnArgs a) {
   constexpr int ROWS = 16 * RT, NC = D / 32, ND = D / 16;
-  constexpr int CH = D / 8;                                  // 16-byte chunks of a row in T
   constexpr int KL = CODES ? D / 64 : D / 32;                // 16-byte loads of a lane for 16 keys
   constexpr int VCH = CODES ? D / 16 : D / 8;                // 16-byte chunks of a row in memory
   constexpr int VL = kWaveKeys * VCH / 64;                   // of a lane for the wave's keys
@@ -212,19 +228,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
   const int c16 = lane & 15, q4 = lane >> 4;
   u16* const vt = tiles[wave];
 
-  if (a.clear) {
-    for (int t = blockIdx.x; t < a.s.T; t += gridDim.x) {
-      bool has = false;
-      for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-        const Seq q = sequence(a.s, min(b0 + lane, a.s.B - 1));
-        has |= q.n > 0 && t >= q.start && t < q.start + q.n;
-      }
-      if (__builtin_amdgcn_ballot_w64(has)) continue;
-      for (int i = tid; i < a.Hq * CH; i += kAttnThreads)
-        *reinterpret_cast<u32x4_t*>(a.out + t * a.orow + i / CH * a.ohead + 8 * (i % CH)) = u32x4_t{0u, 0u, 0u, 0u};
-    }
-  }
-
+  if (a.clear) clear_rows<D>(a);
   const int units = all_units<RT>(a, 0, nullptr), run = a.whole ? 1 : run_of(a, units, gridDim.x);
   if ((long)blockIdx.x * run >= units) return;
   int u = blockIdx.x * run;

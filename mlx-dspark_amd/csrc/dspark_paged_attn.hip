@@ -2,24 +2,36 @@
 #include <algorithm>
 #include <cmath>
 
-#include "dspark_paged_attn.h"
+#include "dspark_paged_tiles.h"
 
 namespace dspark {
 namespace paged {
 namespace {
 
 struct Plan {
-  int rt, workgroups, most_rows, whole, least;
-  size_t part_floats;
+  int rt, workgroups, most_rows, whole, least;   // few rows (workgroups = 0: not launched)
+  int rows_up_to;                                // of a sequence and KV head that are few
+  unsigned items;                                // many rows: workgroups, 0: not launched
+  size_t part_floats, tile_floats;
 };
 
 Plan make_plan(long B, long Hq, long Hk, long D, long T, long max_rows, long max_len) {
   Plan p{};
   const long gqa = Hq / Hk, rows = std::min(T, max_rows) * gqa;
-  p.rt = rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
+  const bool tiles_too = rows > (D == 256 ? 32 : 64);
+  // Beside prompt chunks the few-rows kernel has decoded tokens only: one row tile, and what is more goes to the other
+  p.rows_up_to = tiles_too ? 16 : 1 << 30;
+  p.rt = tiles_too || rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
+  if (tiles_too) {
+    if (B == 1) p.rows_up_to = 0;                // one sequence: the one launch takes it as it is
+    const long long_ones = std::min(B, T * gqa / (p.rows_up_to + 1) + 1);
+    p.items = (unsigned)(((T * gqa / kTileRows + long_ones) * Hk + kParts + 7) / 8 * 8);
+    p.tile_floats = (size_t)kParts * kTileRows * (D + 2);
+    if (B == 1) return p;
+  }
   const long tiles = (max_len + kUnit - 1) / kUnit, height = 16 * p.rt;
   const long groups = T * gqa / height + std::min(B, T);                // of all sequences, at most
-  p.most_rows = (int)std::min(T * gqa, std::max(rows, 1L));
+  p.most_rows = (int)std::min(T * gqa, std::max(tiles_too ? 16L : rows, 1L));
   p.whole = tiles <= 4;
   p.least = p.rt == 4 ? 4 : 2;
   if (p.whole) {
@@ -51,7 +63,8 @@ using namespace dspark;
 extern "C" size_t dspark_paged_attention_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t rows, int64_t max_rows,
                                                    int64_t max_len) {
   if (paged::check(B, Hq, Hk, D, rows, max_rows, max_len)) return 0;
-  return std::max<size_t>(paged::make_plan(B, Hq, Hk, D, rows, max_rows, max_len).part_floats * sizeof(float), 256);
+  const paged::Plan p = paged::make_plan(B, Hq, Hk, D, rows, max_rows, max_len);
+  return std::max<size_t>(std::max(p.part_floats, p.tile_floats) * sizeof(float), 256);
 }
 
 extern "C" int dspark_paged_attention(const dspark_paged_attention_args* p, dspark_stream stream) {
@@ -76,8 +89,9 @@ extern "C" int dspark_paged_attention(const dspark_paged_attention_args* p, dspa
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->workspace, 16))
     return fail(DSPARK_ERR_ALIGN, "%s: queries, outputs and workspace must be 16-byte aligned", what);
   const paged::Plan plan = paged::make_plan(a.s.B, p->Hq, p->Hk, p->D, a.s.T, p->max_rows, max_len);
-  if ((size_t)p->workspace_bytes < plan.part_floats * sizeof(float))
-    return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %ld < %zu bytes", what, (long)p->workspace_bytes, plan.part_floats * sizeof(float));
+  const size_t need = std::max(plan.part_floats, plan.tile_floats) * sizeof(float);      // one after the other
+  if ((size_t)p->workspace_bytes < need)
+    return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %ld < %zu bytes", what, (long)p->workspace_bytes, need);
   a.q = static_cast<const u16*>(p->q);
   a.out = static_cast<u16*>(p->out);
   a.qrow = p->q_strides[0], a.qhead = p->q_strides[1];
@@ -90,16 +104,27 @@ extern "C" int dspark_paged_attention(const dspark_paged_attention_args* p, dspa
   a.causal = p->causal != 0;
   a.whole = plan.whole;
   a.least = plan.least;
-  a.rows_up_to = 1 << 30;
+  a.rows_up_to = plan.rows_up_to;
   a.clear = p->clear != 0;
   a.scale_log2 = (float)(p->scale * 1.44269504088896340736);
   hipStream_t s = static_cast<hipStream_t>(stream);
   using paged::BF16;
   using paged::F16;
   const bool bf = p->dtype == DSPARK_DTYPE_BF16;
+  if (plan.workgroups) {
 #define DSPARK_PAGED_CALL(D) \
   (bf ? paged::launch<BF16, D>(a, plan.rt, codes, plan.workgroups, plan.most_rows, s) \
       : paged::launch<F16, D>(a, plan.rt, codes, plan.workgroups, plan.most_rows, s))
+    st = p->D == 64 ? DSPARK_PAGED_CALL(64) : p->D == 128 ? DSPARK_PAGED_CALL(128) : DSPARK_PAGED_CALL(256);
+#undef DSPARK_PAGED_CALL
+    if (st) return st;
+    a.clear = 0;
+  }
+  if (!plan.items) return DSPARK_OK;
+  paged::TileArgs ta{a, static_cast<float*>(p->workspace), nullptr};
+  ta.mpart = ta.opart + (size_t)paged::kParts * paged::kTileRows * p->D;
+#define DSPARK_PAGED_CALL(D) \
+  (bf ? paged::launch_tiles<BF16, D>(ta, codes, plan.items, s) : paged::launch_tiles<F16, D>(ta, codes, plan.items, s))
   return p->D == 64 ? DSPARK_PAGED_CALL(64) : p->D == 128 ? DSPARK_PAGED_CALL(128) : DSPARK_PAGED_CALL(256);
 #undef DSPARK_PAGED_CALL
 }

@@ -1,0 +1,468 @@
+// Attention over paged caches for gfx950: many rows of each sequence (prompt chunks).
+//
+// The same attention as dspark_paged_attn.h, bound by the matrix cores and, close behind, by the softmax's instructions.
+// Hence, as for prompts over contiguous caches:
+//   * a workgroup of 4 waves takes 128 rows of a (sequence, KV head), (token, query head) heads fastest, 32 a wave, so
+//     that 64 keys and values in LDS serve them all; S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16, where the scores
+//     of a lane (32 keys of one row) are, in place, what the second product needs;
+//   * K and V tiles are double buffered, one barrier a tile; each wave brings 16 positions, which lie in one page: pages of
+//     the model's type go to LDS without passing registers, 8-bit codes through registers, where they are turned into the
+//     model's type once for the workgroup;
+//   * sequences of unequal lengths: those with more keys than one and a half times the average share of a workgroup slot are
+//     split along the keys, into parts that a second launch joins (fp32, in the order of the keys). Everything is found on
+//     the device from the lengths as they are;
+//   * the rows of one KV head are consecutive on one XCD, whose L2 then holds its pages, long causal tiles first.
+// Probabilities are two pieces of the type, as in dspark_paged_attn.h: the second costs a third of the products, and one
+// piece alone would add an error of the size of the output's own rounding.
+//
+// The running maximum is only raised (and the outputs rescaled) where it grew by more than 2^8: fp32 sums do not mind
+// probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
+#pragma once
+
+#include "dspark_attn_prefill.h"
+#include "dspark_paged_attn.h"
+
+namespace dspark {
+namespace paged {
+
+constexpr int kTileRows = 128;    // rows of a workgroup
+constexpr int kTileKeys = 64;
+constexpr int kSlots = 512;       // workgroups that run together: two a CU
+constexpr int kParts = 704;       // parts of split sequences, at most: 2 kSlots / 1.5 and what rounding adds
+constexpr int kLeastTiles = 8;    // key tiles of a part, at least
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+struct TileArgs {
+  AttnArgs a;                     // rows_up_to: sequences with more rows of a KV head are these kernels'
+  float* opart;                   // [part][128 rows][D], unnormalised; then maxima and sums
+  float* mpart;
+};
+
+struct TileWork {
+  int start, n, len, rows, row_tiles, key_tiles;
+};
+
+__device__ __forceinline__ TileWork tile_work(const AttnArgs& a, int b) {
+  const Seq q = sequence(a.s, b);
+  TileWork w{q.start, q.n, q.len, q.n * a.gqa, 0, (q.len + kTileKeys - 1) / kTileKeys};
+  if (w.rows <= a.rows_up_to) w.rows = 0;
+  w.row_tiles = (w.rows + kTileRows - 1) / kTileRows;
+  return w;
+}
+
+// Key tiles that a part may have before it is split: 1.5 times the average share of a slot
+__device__ __forceinline__ int target_tiles(const AttnArgs& a) {
+  const int lane = __lane_id();
+  float sum = 0.f;                // a rule, not a count: rounding does not matter
+  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+    if (b0 + lane >= a.s.B) continue;
+    const TileWork w = tile_work(a, b0 + lane);
+    sum += (float)w.row_tiles * (float)w.key_tiles;
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) sum += shfl_xor(sum, x);
+  const float t = 1.5f * sum * (float)a.Hk / kSlots;
+  return uniform(t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1);
+}
+
+__device__ __forceinline__ int parts_of(const TileWork& w, int target) { return (w.key_tiles + target - 1) / target; }
+
+// Items of the list (and of the split ones among them) of a sequence
+__device__ __forceinline__ u32 items_of(const AttnArgs& a, int b, int target) {
+  const TileWork w = tile_work(a, b);
+  const unsigned long long n = (unsigned long long)a.Hk * (unsigned)w.row_tiles * (unsigned)parts_of(w, target);
+  return n > kMostUnits ? kMostUnits + 1 : (u32)n;
+}
+
+// Parts before sequence b among the split sequences
+__device__ __forceinline__ int parts_before(const AttnArgs& a, int b, int target) {
+  const int lane = __lane_id();
+  u32 n = 0;
+  for (int b0 = 0; b0 < b; b0 += 64)
+    if (b0 + lane < b) {
+      const TileWork w = tile_work(a, b0 + lane);
+      if (parts_of(w, target) > 1) n = __builtin_elementwise_add_sat(n, items_of(a, b0 + lane, target));
+    }
+  const u32 all = (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+  return (int)(all > (u32)kParts ? (u32)kParts : all);
+}
+
+__device__ __forceinline__ u32 items_of_all(const AttnArgs& a, int target) {
+  const int lane = __lane_id();
+  u32 n = 0;
+  for (int b0 = 0; b0 < a.s.B; b0 += 64)
+    if (b0 + lane < a.s.B) n = __builtin_elementwise_add_sat(n, items_of(a, b0 + lane, target));
+  return (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+}
+
+// Eight probabilities as two pieces of T whose sum they are: the upper one cut off, so that both are positive
+template <class T>
+__device__ __forceinline__ void two_pieces(const f32x16_t& p, int r0, u32x4_t& hi, u32x4_t& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = p[r0 + 2 * i], b = p[r0 + 2 * i + 1];
+    if constexpr (T::kF16) {
+      const attn::f16x2_t h = __builtin_bit_cast(attn::f16x2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+      const float m1 = __builtin_bit_cast(float, opaque_sgpr(0xBF800000u));     // keeps it one v_fma_mix
+      hi[i] = __builtin_bit_cast(u32, h);
+      lo[i] = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h.x, m1, a), __builtin_fmaf((float)h.y, m1, b)));
+    } else {
+      const u32 x = __builtin_bit_cast(u32, a), y = __builtin_bit_cast(u32, b);
+      hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+      lo[i] = pack_bf16x2(a - __builtin_bit_cast(float, x & 0xFFFF0000u), b - __builtin_bit_cast(float, y & 0xFFFF0000u));
+    }
+  }
+}
+
+template <class T, int D, bool CODES>
+__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(const TileArgs ta) {
+  using prefill::k_swz;
+  using prefill::lds_tr;
+  using prefill::mfma32;
+  using prefill::v_swz;
+  constexpr int KT = kTileKeys, SUB = KT / 32, CH = D / 8, ND = D / 32, NK = D / 16;
+  constexpr int NJ = 16 * CH / 64;                           // 16-byte pieces of T that a lane brings of 16 positions
+  constexpr int CJ = CODES ? D / 64 : 1;                     // of codes
+  constexpr float kTop = T::kF16 ? 128.f : 1.f;              // fp16 probabilities up to 2^15
+  __shared__ __attribute__((aligned(16))) u16 sm[2][2][KT * D];      // [buffer][K, V]
+  typedef __attribute__((address_space(3))) u16 lds_u16;
+  typedef const __attribute__((address_space(1))) u16 glb_u16;
+  const AttnArgs& a = ta.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15;
+
+  if (a.clear) clear_rows<D>(a);
+  const int target = target_tiles(a);
+  const u32 all = items_of_all(a, target);
+  if (all > kMostUnits) return;
+  const u32 per_xcd = (all + 7) / 8, item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per_xcd || item >= all) return;
+  int b, local;
+  if (!locate(item, a.s.B, [&](int i) { return items_of(a, i, target); }, b, local)) return;
+  TileWork w = tile_work(a, b);
+  w = TileWork{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.row_tiles), uniform(w.key_tiles)};
+  const int parts = parts_of(w, target);
+  const int h = local / (w.row_tiles * parts), rest = local - h * w.row_tiles * parts;
+  const int tile = w.row_tiles - 1 - rest / parts, z = rest % parts;
+
+  const int r0 = tile * kTileRows, rw = r0 + 32 * wave;
+  const int r = min(rw + l31, w.rows - 1), tok = r / a.gqa, head = h * a.gqa + (r - tok * a.gqa);
+  // keys that this lane's row sees, the wave's least and most, the workgroup's most
+  const int lim = keys_seen(a, b, w.n, w.len, tok);
+  const int wmin = uniform(keys_seen(a, b, w.n, w.len, min(rw, w.rows - 1) / a.gqa));
+  const int wmax = uniform(keys_seen(a, b, w.n, w.len, min(rw + 31, w.rows - 1) / a.gqa));
+  const int bmax = uniform(keys_seen(a, b, w.n, w.len, min(r0 + kTileRows - 1, w.rows - 1) / a.gqa));
+  const int ntile = (bmax + KT - 1) / KT;
+  const int t0 = (int)((long)ntile * z / parts), t1 = (int)((long)ntile * (z + 1) / parts);
+
+  // page ids (and scales), 64 at a time
+  const int* const row = a.s.table + b * a.s.ldt;
+  const int last_page = (w.len - 1) >> a.s.log2P;
+  int ids = -1, ids_at = -1 << 30;
+  bool whole_window = true;
+  float ku = 1.f, vu = 1.f;
+  auto fetch_ids = [&](int first) {
+    ids_at = first;
+    const int p = first + lane;
+    const int id = p <= last_page ? row[p] : 0;
+    ids = (unsigned)id < (unsigned)a.s.pool ? id : -1;
+    whole_window = __builtin_amdgcn_ballot_w64(ids < 0) == 0;
+    if constexpr (CODES) {
+      ku = vu = 0.f;
+      if (ids >= 0) {
+        ku = __builtin_bit_cast(float, (u32)a.k.exps[ids * a.k.epage + h * a.k.ehead] << 23);
+        vu = __builtin_bit_cast(float, (u32)a.v.exps[ids * a.v.epage + h * a.v.ehead] << 23);
+      }
+    }
+  };
+  auto window = [&](int t) {      // pages of tile t are in the window
+    const int p0 = (t * KT) >> a.s.log2P, p1 = (t * KT + KT - 1) >> a.s.log2P;
+    if (p0 < ids_at || p1 >= ids_at + 64) fetch_ids(p0);
+  };
+
+  // This wave's 16 positions of tile t: rows past the keys repeat the last one (and are masked)
+  constexpr int ES = CODES ? 1 : 2;
+  u32x4_t kc[CJ], vc[CJ];         // codes in flight
+  float kc_unit = 1.f, vc_unit = 1.f;
+  auto bring = [&](int t, int buf) {
+    window(t);
+    const int pos = min(t * KT + 16 * wave, (w.len - 1) & ~15), rmax = min(15, w.len - 1 - pos);
+    const int p = (pos >> a.s.log2P) - ids_at, id = max(__builtin_amdgcn_readlane(ids, p), 0);
+    const long in = pos & (a.s.P - 1);
+    const char* kp = a.k.data + (id * a.k.page + h * a.k.head + in * a.k.row) * ES;
+    const char* vp = a.v.data + (id * a.v.page + h * a.v.head + in * a.v.row) * ES;
+    if constexpr (CODES) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j) {
+        const int i = j * 64 + lane, rr = i / (D / 16), c = i % (D / 16);
+        kc[j] = ldg128(kp + min(rr, rmax) * (int)a.k.row + 16 * c);
+        vc[j] = ldg128(vp + min(rr, rmax) * (int)a.v.row + 16 * c);
+      }
+      auto unit = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), p)); };
+      kc_unit = unit(ku);
+      vc_unit = unit(vu);
+    } else {
+      const u32 ks = (u32)a.k.row * 2, vs = (u32)a.v.row * 2;          // < 2^24
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int i = j * 64 + lane, rr = i / CH;
+        const u32 off = __umul24((u32)min(rr, rmax), ks) + (u32)((i % CH ^ k_swz<D>(16 * wave + rr)) << 4);
+        __builtin_amdgcn_global_load_lds((glb_u16*)(kp + off), (lds_u16*)&sm[buf][0][16 * wave * D + j * 512], 16, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int i = j * 64 + lane, rr = i / CH;
+        const u32 off = __umul24((u32)min(rr, rmax), vs) + (u32)((i % CH ^ v_swz<D>(16 * wave + rr)) << 4);
+        __builtin_amdgcn_global_load_lds((glb_u16*)(vp + off), (lds_u16*)&sm[buf][1][16 * wave * D + j * 512], 16, 0, 0);
+      }
+    }
+  };
+  auto put_codes = [&](int buf) {
+    if constexpr (CODES) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j) {
+        const int i = j * 64 + lane, rr = 16 * wave + i / (D / 16), c = 2 * (i % (D / 16));
+        u32x4_t lo, hi;
+        decode<T>(kc[j], kc_unit, lo, hi);
+        *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + ((c ^ k_swz<D>(rr)) << 3)]) = lo;
+        *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + (((c + 1) ^ k_swz<D>(rr)) << 3)]) = hi;
+        decode<T>(vc[j], vc_unit, lo, hi);
+        *reinterpret_cast<u32x4_t*>(&sm[buf][1][rr * D + ((c ^ v_swz<D>(rr)) << 3)]) = lo;
+        *reinterpret_cast<u32x4_t*>(&sm[buf][1][rr * D + (((c + 1) ^ v_swz<D>(rr)) << 3)]) = hi;
+      }
+    }
+  };
+
+  if (t0 < t1) {
+    bring(t0, 0);
+    put_codes(0);
+  }
+  u32x4_t qf[NK];
+  const u16* qp = a.q + (w.start + tok) * a.qrow + head * a.qhead + 8 * half;
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk) qf[kk] = ldg128(qp + 16 * kk);
+
+  f32x16_t o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  const float c = a.scale_log2;
+  float m = kLowest, mc = -1e30f, l = 0.f;                   // reference of the exponents: raw, and times c; this half's sum
+  const int kswz = k_swz<D>(l31), kbase = l31 * D;
+  const int vrow = 4 * half + (l16 >> 2), vswz = v_swz<D>(l16 >> 2);
+  const int vchunk = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1), vbase = vrow * D + 4 * (l16 & 1);
+
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    // tile t has landed once every wave's copies have; every read of the other buffer is done
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    u32 gone = 0;                                            // 16-position groups of this tile in pages that are not there
+    if (!whole_window) {
+      window(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = (t * KT + 16 * i) >> a.s.log2P;
+        if (p <= last_page && __builtin_amdgcn_readlane(ids, p - ids_at) < 0) gone |= 1u << i;
+      }
+    }
+    const int key0 = t * KT;
+    if (t + 1 < t1) bring(t + 1, buf ^ 1);
+    if (key0 < wmax) {                                       // wave-uniform
+      const u16* ks = sm[buf][0];
+      const u16* vs = sm[buf][1];
+      f32x16_t s[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+          s[u] = mfma32<T>(*reinterpret_cast<const u32x4_t*>(ks + u * 32 * D + kbase + (((2 * kk + half) ^ kswz) << 3)),
+                           qf[kk], s[u]);
+      if (key0 + KT > wmin || gone) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
+            if (key0 + k >= lim || (gone >> (k >> 4) & 1)) s[u][i] = -__builtin_inff();
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+      mx = max_xor32(mx);
+      // (the first keys that a row sees raise it from its lowest)
+      if (__builtin_amdgcn_ballot_w64(mx > m && __builtin_fmaf(mx, c, -mc) > 8.f)) {
+        const float to = fmaxf(m, mx), toc = to == kLowest ? -1e30f : to * c;
+        const float alpha = __builtin_amdgcn_exp2f(mc - toc);
+        m = to;
+        mc = toc;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mc));
+          if constexpr (T::kF16) p *= kTop;
+          s[u][i] = p;
+          sum += p;
+        }
+      l += sum;
+      auto v_frag = [&](int uj, int d) {                     // V^T of keys 16 uj .. 16 uj + 15, columns 32 d ..
+        const u16* vp = vs + 16 * uj * D + vbase + (((4 * d + vchunk) ^ vswz) << 3);
+        const u32x2_t lo = lds_tr(vp), hi = lds_tr(vp + 8 * D);
+        return u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      };
+      constexpr int DB = ND < 4 ? ND : 4;                    // V fragments in flight
+#pragma unroll
+      for (int uj = 0; uj < 2 * SUB; ++uj) {
+        u32x4_t ph, pl;
+        two_pieces<T>(s[uj >> 1], 8 * (uj & 1), ph, pl);
+#pragma unroll
+        for (int d0 = 0; d0 < ND; d0 += DB) {
+          u32x4_t vf[DB];
+#pragma unroll
+          for (int d = 0; d < DB; ++d) vf[d] = v_frag(uj, d0 + d);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[d], ph, o[d0 + d]);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[d], pl, o[d0 + d]);
+        }
+      }
+    }
+    if (t + 1 < t1) put_codes(buf ^ 1);
+  }
+
+  l += shfl_xor(l, 32);
+  const bool own = rw + l31 < w.rows;
+  if (parts > 1) {
+    const int part = parts_before(a, b, target) + local;
+    if (part >= kParts || !own) return;
+    const long pr = (long)part * kTileRows + 32 * wave + l31;
+    if (half == 0) {
+      ta.mpart[2 * pr] = mc;
+      ta.mpart[2 * pr + 1] = l;
+    }
+    float* op = ta.opart + pr * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * g) = f32x4_t{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    return;
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  float zero = l - l;             // NaN once an output is not finite
+  if (own) {
+    u16* op = a.out + (w.start + tok) * a.orow + head * a.ohead + 4 * half;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = __builtin_fmaf(o[d][4 * g + i], 0.f, zero);
+        *reinterpret_cast<u32x2_t*>(op + 32 * d + 8 * g) =
+            u32x2_t{attn::pack2<T>(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                    attn::pack2<T>(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv)};
+      }
+  }
+  const unsigned long long bad = __builtin_amdgcn_ballot_w64(own && zero != 0.f);
+  if (!bad) return;
+  __threadfence_block();
+  for (u32 rows = (u32)bad | (u32)(bad >> 32); rows; rows &= rows - 1) {
+    const int i = rw + __builtin_ctz(rows), ti = i / a.gqa;
+    plain_row<T, D, CODES>(a, b, w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, b, w.n, w.len, ti));
+  }
+}
+
+// Joins the parts of split sequences; a wave a row
+template <class T, int D, bool CODES>
+__global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs ta) {
+  constexpr int C = D / 64;
+  typedef float cols_t __attribute__((ext_vector_type(C)));
+  const AttnArgs& a = ta.a;
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  const int target = target_tiles(a);
+  if (items_of_all(a, target) > kMostUnits) return;
+  int base = 0;                   // parts before sequence b
+  for (int b = 0; b < a.s.B && base < kParts; ++b) {
+    TileWork w = tile_work(a, b);
+    w = TileWork{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.row_tiles), uniform(w.key_tiles)};
+    const int parts = parts_of(w, target);
+    if (w.rows == 0 || parts == 1) continue;
+    const int count = a.Hk * w.row_tiles * parts;
+    if (base + count > kParts) return;
+    for (long x = (long)blockIdx.x * kWaves + wave; x < (long)a.Hk * w.rows; x += (long)gridDim.x * kWaves) {
+      const int h = (int)(x / w.rows), r = (int)(x - (long)h * w.rows);
+      const int tile = r / kTileRows, first = base + (h * w.row_tiles + w.row_tiles - 1 - tile) * parts;
+      const int at = r - tile * kTileRows;
+      float mc = -1e30f;
+      for (int z = 0; z < parts; ++z) mc = fmaxf(mc, ta.mpart[2 * ((long)(first + z) * kTileRows + at)]);
+      cols_t acc;
+#pragma unroll
+      for (int i = 0; i < C; ++i) acc[i] = 0.f;
+      float l = 0.f;
+      for (int z = 0; z < parts; ++z) {
+        const long pr = (long)(first + z) * kTileRows + at;
+        const float f = __builtin_amdgcn_exp2f(ta.mpart[2 * pr] - mc);
+        l += f * ta.mpart[2 * pr + 1];
+        const cols_t v = *reinterpret_cast<const cols_t*>(ta.opart + pr * D + C * lane);
+#pragma unroll
+        for (int i = 0; i < C; ++i) acc[i] = __builtin_fmaf(f, v[i], acc[i]);
+      }
+      const int tok = r / a.gqa, head = h * a.gqa + r - tok * a.gqa;
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      u16* op = a.out + (w.start + tok) * a.orow + head * a.ohead + C * lane;
+      float zero = l - l;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        zero = __builtin_fmaf(acc[i], 0.f, zero);
+        op[i] = attn::from_f32<T>(acc[i] * inv);
+      }
+      if (__builtin_amdgcn_ballot_w64(zero != 0.f))
+        plain_row<T, D, CODES>(a, b, w.start + tok, head, keys_seen(a, b, w.n, w.len, tok));
+    }
+    base += count;
+  }
+}
+
+// Each (element type, head dim) in its own translation unit
+template <class T, int D>
+int launch_tiles(const TileArgs& ta, bool codes, unsigned items, hipStream_t s);
+
+#define DSPARK_PAGED_TILES(T, D) \
+  template <>                   \
+  int launch_tiles<T, D>(const TileArgs& ta, bool codes, unsigned items, hipStream_t s)
+DSPARK_PAGED_TILES(BF16, 64);
+DSPARK_PAGED_TILES(BF16, 128);
+DSPARK_PAGED_TILES(BF16, 256);
+DSPARK_PAGED_TILES(F16, 64);
+DSPARK_PAGED_TILES(F16, 128);
+DSPARK_PAGED_TILES(F16, 256);
+
+template <class T, int D, bool CODES>
+int launch_tiles_of(const TileArgs& ta, unsigned items, hipStream_t s) {
+  hipLaunchKernelGGL((tiles_kernel<T, D, CODES>), dim3(items), dim3(kAttnThreads), 0, s, ta);
+  const int st = check_launch("paged_attention(tiles)");
+  if (st) return st;
+  hipLaunchKernelGGL((join_tiles_kernel<T, D, CODES>), dim3(kSlots), dim3(kAttnThreads), 0, s, ta);
+  return check_launch("paged_attention(join tiles)");
+}
+
+}  // namespace paged
+}  // namespace dspark

@@ -1,0 +1,10 @@
+// Attention over paged caches, many rows: bf16, head dim 128.
+#include "dspark_paged_tiles.h"
+
+namespace dspark {
+namespace paged {
+
+DSPARK_PAGED_TILES(BF16, 128) { return codes ? launch_tiles_of<BF16, 128, true>(ta, items, s) : launch_tiles_of<BF16, 128, false>(ta, items, s); }
+
+}  // namespace paged
+}  // namespace dspark

@@ -294,3 +294,130 @@ def test_encoder_states(dev):
         kk, vv = (t[lo:lo + n].double().repeat_interleave(2, 1) for t in (k, v))
         p = torch.softmax((q[s:e].double()[:, None] * kk[None]).sum(-1) * 0.2, 1)
         assert (got[s:e].double() - (p[..., None] * vv[None]).sum(1)).abs().max() < 2e-3
+
+
+TILES = [  # Hq, Hk, D, P, lens, rows: prompt chunks, alone and beside others
+    (4, 2, 64, 16, [1000], [1000]),
+    (4, 1, 128, 64, [129], [65]),
+    (8, 2, 128, 16, [700, 33, 1, 400, 90], [300, 1, 1, 64, 17]),
+    (6, 1, 256, 128, [513, 77], [512, 30]),
+    (9, 3, 64, 32, [5000, 64, 65], [150, 64, 65]),
+    (2, 2, 128, 64, [3000, 300, 20, 2], [33, 300, 16, 2]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", TILES, ids=str)
+def test_prompt_chunks(dev, shape, dtype, bits, causal):
+    Hq, Hk, D, P, lens, rows = shape
+    run(dev, dtype, bits, Hq, Hk, D, P, lens, rows, causal=causal, behind=3, max_rows=max(rows))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_chunks_of_many_sequences(dev, bits):
+    """More sequences than a wave has lanes; more items than workgroups run together; long ones split beside short ones."""
+    run(dev, "bf16", bits, 2, 1, 64, 16, [40 + i % 90 for i in range(140)], [1 + (i * 7) % 40 for i in range(140)], max_rows=40)
+    run(dev, "bf16", bits, 8, 8, 64, 16, [1200, 900], [1100, 800], max_rows=1100)
+    run(dev, "f16", bits, 4, 2, 64, 64, [9000, 200, 100, 4000], [40, 200, 100, 33], max_rows=200)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_chunk_rows_that_see_nothing(dev, bits):
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(12)
+    D, P, pool, T = 64, 16, 9, 150
+    q = torch.randn(T, 4, D, generator=g).to(torch.bfloat16).to(dev)
+    for table, starts, lens in (([[0, 1, 2, 3, 4]], [0, 120], [60]), ([[0, 1, -3, 3, 40, 5, 6, 7]], [0, 100], [120]), ([[0, 1, 2]], [3, 150], [999]),
+                                ([[1, 2, 3, 4], [5, 6, 7, 8]], [0, 60, 90], [64, 64]), ([[1, 2], [5, 6]], [0, 160, 10], [32, 32]),
+                                ([[-1] * 8], [0, 100], [128])):
+        kp, vp = (make_pages(g, pool, 2, P, D, torch.bfloat16, bits, dev) for _ in range(2))
+        args = (q, kp, vp, ints(table, dev), ints(starts, dev), ints(lens, dev))
+        for causal in (True, False):
+            got = ops.paged_attention(*args, scale=0.2, causal=causal)
+            check(args, got, 0.2, causal)
+            out = torch.full_like(q, 7.0)
+            ops.paged_attention(*args, scale=0.2, causal=causal, out=out)
+            none = np.isnan(attention(host(q), oracle_pages(kp), oracle_pages(vp), np.array(table), starts, lens, 0.2, causal)[0])
+            none = torch.from_numpy(none).to(dev)
+            assert (out[none] == 7).all() and torch.equal(out[~none], got[~none])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("split", [False, True])
+def test_chunk_values_that_are_not_finite(dev, dtype, bits, split):
+    """Behind the end and in keys that a row does not see they leave it alone; where it sees them they count."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(13)
+    n, L = 80, 3000 if split else 200
+    q, kp, vp, table, starts, lens = make(g, dev, dtype, bits, 4, 2, 64, 16, [L, 17], [n, 1])
+    clean = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.125)
+    data = lambda p: p[0] if bits == 8 else p
+    as_bits = lambda t: t.view(torch.uint8) if bits == 8 else t.view(torch.int16)
+    bad = torch.full(data(kp).shape, float("nan"), device=dev).to(data(kp).dtype)
+    used = torch.zeros(bad.shape[0], 16, dtype=torch.bool)
+    for b, m in enumerate((L, 17)):
+        for i in range(m):
+            used[table[b, i // 16].item(), i % 16] = True
+    for p in (kp, vp):
+        as_bits(data(p)).copy_(torch.where((~used).to(dev)[:, None, :, None], as_bits(bad), as_bits(data(p))))
+    assert torch.equal(ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.125), clean)
+    at = L - 10                                         # seen by the last ten rows
+    for p in (kp, vp):
+        keep = data(p).clone()
+        as_bits(data(p))[table[0, at // 16].item(), :, at % 16] = as_bits(bad)[0, 0, 0, 0]
+        got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.125)
+        assert not got[n - 10:n].isfinite().any() and got[:n - 10].isfinite().all() and torch.equal(got[n:], clean[n:])
+        assert (got[:n - 10].double() - clean[:n - 10].double()).abs().max() <= 2 ** -7 * clean.double().abs().max()
+        data(p).copy_(keep)
+    if bits == 16:
+        vp[table[0, 1].item(), :, 3, 5] = float("inf")
+        got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.125)
+        assert (got[:n, :, 5] == float("inf")).all() and got[:n, :, :5].isfinite().all() and got[:n, :, 6:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_chunk_scores_that_rise_and_fall(dev, dtype):
+    """Scores that rise by little and by much from tile to tile, fall, and stand far under the first; values near the end of
+    the type's range."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(14)
+    q, kp, vp, table, starts, lens = make(g, dev, dtype, 16, 2, 1, 64, 16, [900], [70])
+    q[:] = q[:1, :1]
+    args = (q, kp, vp, table, starts, lens)
+    for f in (lambda i: 0.001 * i, lambda i: 0.1 * i, lambda i: -0.1 * i, lambda i: 30.0 * (i == 0), lambda i: 3.0 * (i // 64 % 2), lambda i: -60 + 0.0 * i):
+        for i in range(900):
+            kp[table[0, i // 16].item(), :, i % 16] = q[0, 0] * (f(i) / 8)
+        check(args, ops.paged_attention(*args, scale=0.125), 0.125)
+    kp.zero_()
+    vp.fill_(torch.finfo(DT[dtype]).max * 0.9)
+    got = ops.paged_attention(*args, scale=0.125)
+    assert torch.allclose(got.double(), vp[0, 0, 0, 0].double().expand(got.shape), rtol=2 ** -7, atol=0)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_captured_chunks(dev, bits):
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(15)
+    q, kp, vp, table, _, _ = make(g, dev, "bf16", bits, 8, 2, 128, 16, [2000, 800, 40], [100, 3, 2])
+    starts, lens = ints([0, 80, 83, 84], dev), ints([1500, 700, 3], dev)
+    call = lambda: ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.1)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(4):
+        lens += 7
+        starts[1:] += 3
+        q.copy_(torch.randn(q.shape, generator=g))
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        check((q, kp, vp, table, starts, lens), out, 0.1)
