@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
 
     // page ids (and scales) of 64 pages, a lane each
     const int* const row = a.s.table + b * a.s.ldt;
-    int ids = -1, ids_at = -1 << 30;                         // of page ids_at + lane
+    int ids = -1, ids_at = -(1 << 30);                        // of page ids_at + lane
     float ku = 1.f, vu = 1.f;
     auto fetch_ids = [&](int first) {
       ids_at = first;

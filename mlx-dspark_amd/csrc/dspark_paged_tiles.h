@@ -11,9 +11,14 @@
 //   * sequences of unequal lengths: those with more keys than one and a half times the average share of a workgroup slot are
 //     split along the keys, into parts that a second launch joins (fp32, in the order of the keys). Everything is found on
 //     the device from the lengths as they are;
-//   * the rows of one KV head are consecutive on one XCD, whose L2 then holds its pages, long causal tiles first.
+//   * items with many keys first: sequences by their length, long causal tiles first within one. Consecutive items are a
+//     tile's KV heads, which go to consecutive XCDs: with 8 heads each XCD's L2 has the pages of one.
 // Probabilities are two pieces of the type, as in dspark_paged_attn.h: the second costs a third of the products, and one
-// piece alone would add an error of the size of the output's own rounding.
+// bf16 piece alone would add an error of the size of the output's own rounding. Codes of a page are, but for extreme
+// scales, fp16 numbers when multiplied by 2^10, and one fp16 piece of a probability is off by an eighth of a bf16
+// rounding: so 8-bit pages of bf16 models go to LDS as fp16 and take one product, and only a workgroup that comes to a page
+// that does not fit begins again with two bf16 pieces (seven chunks of 1 to 700 rows: 182 -> 165 us). For bf16 pages what the
+// conversion costs is what the products save.
 //
 // The running maximum is only raised (and the outputs rescaled) where it grew by more than 2^8: fp32 sums do not mind
 // probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
@@ -30,6 +35,8 @@ constexpr int kTileKeys = 64;
 constexpr int kSlots = 512;       // workgroups that run together: two a CU
 constexpr int kParts = 704;       // parts of split sequences, at most: 2 kSlots / 1.5 and what rounding adds
 constexpr int kLeastTiles = 8;    // key tiles of a part, at least
+
+constexpr int kAluMayCross = 0x2 | 0x4;     // of a scheduling barrier: vector and scalar arithmetic
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -96,6 +103,59 @@ __device__ __forceinline__ u32 items_of_all(const AttnArgs& a, int target) {
   return (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
 }
 
+// 16 bytes a lane from `base` + `off` to LDS, the wave's 1 KB from `to` on. In assembly, and waited for by hand: the
+// compiler takes every later LDS read for one of these bytes and would have it wait for the copies just begun.
+__device__ __forceinline__ void copy_to_lds(const char* base, u32 off, u16* to) {
+  typedef __attribute__((address_space(3))) u16 lds_u16;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"((u32)(uintptr_t)(lds_u16*)to)
+               : "memory", "m0");
+}
+
+constexpr int kNarrow = 10;       // what codes are multiplied by as fp16: 2^10
+
+// The sequence of the item, and its place among the sequence's, where sequences (64 at a time) stand in the order of
+// the keys that their items have, most first
+__device__ __forceinline__ bool locate_longest(const AttnArgs& a, u32 item, int target, int& b, int& local) {
+  const int lane = __lane_id();
+  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+    const int n = min(64, a.s.B - b0);
+    const u32 count = lane < n ? items_of(a, b0 + lane, target) : 0u;
+    int keys = -1;
+    if (lane < n) {
+      const TileWork w = tile_work(a, b0 + lane);
+      keys = w.key_tiles / max(parts_of(w, target), 1);
+    }
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+      const int k = __builtin_amdgcn_readlane(keys, j);
+      rank += k > keys || (k == keys && j < lane) ? 1 : 0;
+    }
+    rank = lane < n ? rank : lane;
+    const u32 c = (u32)__builtin_amdgcn_ds_permute(rank << 2, (int)count);
+    const int from = __builtin_amdgcn_ds_permute(rank << 2, lane);
+    const u32 upto = wave_scan(c);
+    const u32 all = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+    if (item < all) {
+      const int first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > item));
+      b = uniform(b0 + __builtin_amdgcn_readlane(from, first));
+      local = uniform((int)(item - (u32)__builtin_amdgcn_readlane((int)(upto - c), first)));
+      return true;
+    }
+    item -= all;
+  }
+  return false;
+}
+
+// Eight probabilities as fp16
+__device__ __forceinline__ u32x4_t one_piece(const f32x16_t& p, int r0) {
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = attn::pack2<F16>(p[r0 + 2 * i], p[r0 + 2 * i + 1]);
+  return o;
+}
+
 // Eight probabilities as two pieces of T whose sum they are: the upper one cut off, so that both are positive
 template <class T>
 __device__ __forceinline__ void two_pieces(const f32x16_t& p, int r0, u32x4_t& hi, u32x4_t& lo) {
@@ -115,8 +175,15 @@ __device__ __forceinline__ void two_pieces(const f32x16_t& p, int r0, u32x4_t& h
   }
 }
 
-template <class T, int D, bool CODES>
-__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(const TileArgs ta) {
+template <int D>
+struct TileLds {
+  u16 kv[2][2][kTileKeys * D];    // [buffer][K, V]
+  u32 fits[2][4];                 // V of 16 positions fits fp16
+};
+
+// A workgroup's item; false if it was given up at a tile whose V does not fit fp16
+template <class T, int D, bool CODES, bool FP16>
+__device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   using prefill::k_swz;
   using prefill::lds_tr;
   using prefill::mfma32;
@@ -124,27 +191,29 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
   constexpr int KT = kTileKeys, SUB = KT / 32, CH = D / 8, ND = D / 32, NK = D / 16;
   constexpr int NJ = 16 * CH / 64;                           // 16-byte pieces of T that a lane brings of 16 positions
   constexpr int CJ = CODES ? D / 64 : 1;                     // of codes
-  constexpr float kTop = T::kF16 ? 128.f : 1.f;              // fp16 probabilities up to 2^15
-  __shared__ __attribute__((aligned(16))) u16 sm[2][2][KT * D];      // [buffer][K, V]
-  typedef __attribute__((address_space(3))) u16 lds_u16;
-  typedef const __attribute__((address_space(1))) u16 glb_u16;
+  constexpr float kTop = 7.f;                                // probabilities times 2^7: up to 2^15
+  constexpr float kUnscale = FP16 ? 1.f / (1 << kNarrow) : 1.f;
+  auto& sm = lds.kv;
+  auto& fits = lds.fits;
   const AttnArgs& a = ta.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15;
 
-  if (a.clear) clear_rows<D>(a);
   const int target = target_tiles(a);
   const u32 all = items_of_all(a, target);
-  if (all > kMostUnits) return;
-  const u32 per_xcd = (all + 7) / 8, item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per_xcd || item >= all) return;
+  if (all > kMostUnits) return true;
+  // Of the 512 that start together, two a CU, the second 256 in turned order: a long causal tile shares its CU with a
+  // short one (2048 rows behind 2953 keys: 193.4 -> 191.6 us)
+  const u32 nth = blockIdx.x >> 3, rounds = (all + 7) / 8;
+  const u32 turned = nth / 32 == 1 && rounds > 32 ? 32 + min(63u, rounds - 1) - nth : nth;
+  const u32 item = turned * 8 + (blockIdx.x & 7);
+  if (nth >= rounds || item >= all) return true;
   int b, local;
-  if (!locate(item, a.s.B, [&](int i) { return items_of(a, i, target); }, b, local)) return;
+  if (!locate_longest(a, item, target, b, local)) return true;
   TileWork w = tile_work(a, b);
   w = TileWork{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.row_tiles), uniform(w.key_tiles)};
   const int parts = parts_of(w, target);
-  const int h = local / (w.row_tiles * parts), rest = local - h * w.row_tiles * parts;
-  const int tile = w.row_tiles - 1 - rest / parts, z = rest % parts;
+  const int z = local % parts, h = local / parts % a.Hk, tile = w.row_tiles - 1 - local / (parts * a.Hk);
 
   const int r0 = tile * kTileRows, rw = r0 + 32 * wave;
   const int r = min(rw + l31, w.rows - 1), tok = r / a.gqa, head = h * a.gqa + (r - tok * a.gqa);
@@ -159,7 +228,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
   // page ids (and scales), 64 at a time
   const int* const row = a.s.table + b * a.s.ldt;
   const int last_page = (w.len - 1) >> a.s.log2P;
-  int ids = -1, ids_at = -1 << 30;
+  int ids = -1, ids_at = -(1 << 30);
   bool whole_window = true;
   float ku = 1.f, vu = 1.f;
   auto fetch_ids = [&](int first) {
@@ -185,40 +254,52 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
   constexpr int ES = CODES ? 1 : 2;
   u32x4_t kc[CJ], vc[CJ];         // codes in flight
   float kc_unit = 1.f, vc_unit = 1.f;
-  auto bring = [&](int t, int buf) {
+  const char* v_at = nullptr;     // of the positions whose keys were brought last, and its last row
+  int rmax = 0;
+  auto bring_k = [&](int t, int buf) {
     window(t);
-    const int pos = min(t * KT + 16 * wave, (w.len - 1) & ~15), rmax = min(15, w.len - 1 - pos);
+    const int pos = min(t * KT + 16 * wave, (w.len - 1) & ~15);
+    rmax = min(15, w.len - 1 - pos);
     const int p = (pos >> a.s.log2P) - ids_at, id = max(__builtin_amdgcn_readlane(ids, p), 0);
     const long in = pos & (a.s.P - 1);
     const char* kp = a.k.data + (id * a.k.page + h * a.k.head + in * a.k.row) * ES;
-    const char* vp = a.v.data + (id * a.v.page + h * a.v.head + in * a.v.row) * ES;
+    v_at = a.v.data + (id * a.v.page + h * a.v.head + in * a.v.row) * ES;
     if constexpr (CODES) {
 #pragma unroll
       for (int j = 0; j < CJ; ++j) {
         const int i = j * 64 + lane, rr = i / (D / 16), c = i % (D / 16);
         kc[j] = ldg128(kp + min(rr, rmax) * (int)a.k.row + 16 * c);
-        vc[j] = ldg128(vp + min(rr, rmax) * (int)a.v.row + 16 * c);
       }
       auto unit = [&](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), p)); };
       kc_unit = unit(ku);
       vc_unit = unit(vu);
     } else {
-      const u32 ks = (u32)a.k.row * 2, vs = (u32)a.v.row * 2;          // < 2^24
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int i = j * 64 + lane, rr = i / CH;
-        const u32 off = __umul24((u32)min(rr, rmax), ks) + (u32)((i % CH ^ k_swz<D>(16 * wave + rr)) << 4);
-        __builtin_amdgcn_global_load_lds((glb_u16*)(kp + off), (lds_u16*)&sm[buf][0][16 * wave * D + j * 512], 16, 0, 0);
-      }
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int i = j * 64 + lane, rr = i / CH;
-        const u32 off = __umul24((u32)min(rr, rmax), vs) + (u32)((i % CH ^ v_swz<D>(16 * wave + rr)) << 4);
-        __builtin_amdgcn_global_load_lds((glb_u16*)(vp + off), (lds_u16*)&sm[buf][1][16 * wave * D + j * 512], 16, 0, 0);
+        const u32 off = __umul24((u32)min(rr, rmax), (u32)a.k.row * 2) + (u32)((i % CH ^ k_swz<D>(16 * wave + rr)) << 4);    // < 2^28
+        copy_to_lds(kp, off, &sm[buf][0][16 * wave * D + j * 512]);
       }
     }
   };
-  auto put_codes = [&](int buf) {
+  auto bring_v = [&](int buf) {
+    if constexpr (CODES) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j) {
+        const int i = j * 64 + lane, rr = i / (D / 16), c = i % (D / 16);
+        vc[j] = ldg128(v_at + min(rr, rmax) * (int)a.v.row + 16 * c);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int i = j * 64 + lane, rr = i / CH;
+        const u32 off = __umul24((u32)min(rr, rmax), (u32)a.v.row * 2) + (u32)((i % CH ^ v_swz<D>(16 * wave + rr)) << 4);
+        copy_to_lds(v_at, off, &sm[buf][1][16 * wave * D + j * 512]);
+      }
+    }
+  };
+  // What passes registers goes to LDS
+  auto put = [&](int buf) {
     if constexpr (CODES) {
 #pragma unroll
       for (int j = 0; j < CJ; ++j) {
@@ -227,21 +308,27 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
         decode<T>(kc[j], kc_unit, lo, hi);
         *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + ((c ^ k_swz<D>(rr)) << 3)]) = lo;
         *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + (((c + 1) ^ k_swz<D>(rr)) << 3)]) = hi;
-        decode<T>(vc[j], vc_unit, lo, hi);
+        if constexpr (FP16) decode<F16>(vc[j], vc_unit * (1 << kNarrow), lo, hi);
+        else decode<T>(vc[j], vc_unit, lo, hi);
         *reinterpret_cast<u32x4_t*>(&sm[buf][1][rr * D + ((c ^ v_swz<D>(rr)) << 3)]) = lo;
         *reinterpret_cast<u32x4_t*>(&sm[buf][1][rr * D + (((c + 1) ^ v_swz<D>(rr)) << 3)]) = hi;
       }
+      // codes are up to 448 in size and multiples of 2^-9
+      if (FP16 && lane == 0) fits[buf][wave] = vc_unit <= 0.125f && vc_unit >= 1.f / (1 << 25);
     }
   };
 
   if (t0 < t1) {
-    bring(t0, 0);
-    put_codes(0);
+    bring_k(t0, 0);
+    bring_v(0);
   }
   u32x4_t qf[NK];
   const u16* qp = a.q + (w.start + tok) * a.qrow + head * a.qhead + 8 * half;
 #pragma unroll
   for (int kk = 0; kk < NK; ++kk) qf[kk] = ldg128(qp + 16 * kk);
+  // vmcnt(0): the queries are here, or their first use, in the loop, would wait for a tile's copies in every round
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __builtin_amdgcn_sched_barrier(0);
 
   f32x16_t o[ND];
 #pragma unroll
@@ -254,6 +341,7 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
   const int vrow = 4 * half + (l16 >> 2), vswz = v_swz<D>(l16 >> 2);
   const int vchunk = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1), vbase = vrow * D + 4 * (l16 & 1);
 
+  if (t0 < t1) put(0);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     // tile t has landed once every wave's copies have; every read of the other buffer is done
@@ -270,8 +358,14 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
       }
     }
     const int key0 = t * KT;
-    if (t + 1 < t1) bring(t + 1, buf ^ 1);
-    if (key0 < wmax) {                                       // wave-uniform
+    if constexpr (FP16) {
+      const u32x4_t f = *reinterpret_cast<const u32x4_t*>(fits[buf]);
+      if (!uniform((int)(f.x & f.y & f.z & f.w))) return false;
+    }
+    if (t + 1 < t1) bring_k(t + 1, buf ^ 1);
+    if (key0 >= wmax) {                                      // wave-uniform
+      if (t + 1 < t1) bring_v(buf ^ 1);
+    } else {
       const u16* ks = sm[buf][0];
       const u16* vs = sm[buf][1];
       f32x16_t s[SUB];
@@ -279,12 +373,39 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk)
+      // K operands are asked for KA steps ahead of their products, V operands one (left to itself the compiler reads one and
+      // waits for it)
+      constexpr int KA = NK < 4 ? NK : 4;
+      u32x4_t kf[KA][SUB];
+      auto read_k = [&](int kk) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
-          s[u] = mfma32<T>(*reinterpret_cast<const u32x4_t*>(ks + u * 32 * D + kbase + (((2 * kk + half) ^ kswz) << 3)),
-                           qf[kk], s[u]);
+          kf[kk % KA][u] = *reinterpret_cast<const u32x4_t*>(ks + u * 32 * D + kbase + (((2 * kk + half) ^ kswz) << 3));
+      };
+#pragma unroll
+      for (int kk = 0; kk < KA; ++kk) read_k(kk);
+      __builtin_amdgcn_sched_barrier(kAluMayCross);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) s[u] = mfma32<T>(kf[kk % KA][u], qf[kk], s[u]);
+        if (kk + KA < NK) read_k(kk + KA);
+        __builtin_amdgcn_sched_barrier(kAluMayCross);
+      }
+      if (t + 1 < t1) bring_v(buf ^ 1);             // (its registers are free now)
+      auto v_frag = [&](int uj, int d) {                     // V^T of keys 16 uj .. 16 uj + 15, columns 32 d ..
+        const u16* vp = vs + 16 * uj * D + vbase + (((4 * d + vchunk) ^ vswz) << 3);
+        const u32x2_t lo = lds_tr(vp), hi = lds_tr(vp + 8 * D);
+        return u32x4_t{lo.x, lo.y, hi.x, hi.y};
+      };
+      constexpr int DB = ND < 4 ? ND : 4, NG = 2 * SUB * (ND / DB);    // V operands of a step, steps
+      u32x4_t vf[2][DB];
+      auto read_v = [&](int g) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vf[g & 1][d] = v_frag(g / (ND / DB), g % (ND / DB) * DB + d);
+      };
+      read_v(0);
+      __builtin_amdgcn_sched_barrier(kAluMayCross);
       if (key0 + KT > wmin || gone) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
@@ -312,47 +433,50 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
       }
+      const float up = kTop - mc;
       float sum = 0.f;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mc));
-          if constexpr (T::kF16) p *= kTop;
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, up));
           s[u][i] = p;
           sum += p;
         }
       l += sum;
-      auto v_frag = [&](int uj, int d) {                     // V^T of keys 16 uj .. 16 uj + 15, columns 32 d ..
-        const u16* vp = vs + 16 * uj * D + vbase + (((4 * d + vchunk) ^ vswz) << 3);
-        const u32x2_t lo = lds_tr(vp), hi = lds_tr(vp + 8 * D);
-        return u32x4_t{lo.x, lo.y, hi.x, hi.y};
-      };
-      constexpr int DB = ND < 4 ? ND : 4;                    // V fragments in flight
+      u32x4_t ph, pl;
+      if constexpr (FP16) {
 #pragma unroll
-      for (int uj = 0; uj < 2 * SUB; ++uj) {
-        u32x4_t ph, pl;
-        two_pieces<T>(s[uj >> 1], 8 * (uj & 1), ph, pl);
+        for (int g = 0; g < NG; ++g) {
+          const int uj = g / (ND / DB), d0 = g % (ND / DB) * DB;
+          if (g + 1 < NG) read_v(g + 1);
+          __builtin_amdgcn_sched_barrier(kAluMayCross);
+          if (d0 == 0) ph = one_piece(s[uj >> 1], 8 * (uj & 1));
 #pragma unroll
-        for (int d0 = 0; d0 < ND; d0 += DB) {
-          u32x4_t vf[DB];
+          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<F16>(vf[g & 1][d], ph, o[d0 + d]);
+        }
+      } else {
 #pragma unroll
-          for (int d = 0; d < DB; ++d) vf[d] = v_frag(uj, d0 + d);
+        for (int g = 0; g < NG; ++g) {
+          const int uj = g / (ND / DB), d0 = g % (ND / DB) * DB;
+          if (g + 1 < NG) read_v(g + 1);
+          __builtin_amdgcn_sched_barrier(kAluMayCross);
+          if (d0 == 0) two_pieces<T>(s[uj >> 1], 8 * (uj & 1), ph, pl);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[d], ph, o[d0 + d]);
+          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[g & 1][d], ph, o[d0 + d]);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[d], pl, o[d0 + d]);
+          for (int d = 0; d < DB; ++d) o[d0 + d] = mfma32<T>(vf[g & 1][d], pl, o[d0 + d]);
         }
       }
     }
-    if (t + 1 < t1) put_codes(buf ^ 1);
+    if (t + 1 < t1) put(buf ^ 1);
   }
 
   l += shfl_xor(l, 32);
   const bool own = rw + l31 < w.rows;
   if (parts > 1) {
     const int part = parts_before(a, b, target) + local;
-    if (part >= kParts || !own) return;
+    if (part >= kParts || !own) return true;
     const long pr = (long)part * kTileRows + 32 * wave + l31;
     if (half == 0) {
       ta.mpart[2 * pr] = mc;
@@ -363,10 +487,11 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * g) = f32x4_t{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-    return;
+        *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * g) =
+            f32x4_t{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]} * kUnscale;
+    return true;
   }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const float inv = l > 0.f ? kUnscale / l : 0.f;
   float zero = l - l;             // NaN once an output is not finite
   if (own) {
     u16* op = a.out + (w.start + tok) * a.orow + head * a.ohead + 4 * half;
@@ -382,12 +507,26 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
       }
   }
   const unsigned long long bad = __builtin_amdgcn_ballot_w64(own && zero != 0.f);
-  if (!bad) return;
+  if (!bad) return true;
   __threadfence_block();
   for (u32 rows = (u32)bad | (u32)(bad >> 32); rows; rows &= rows - 1) {
     const int i = rw + __builtin_ctz(rows), ti = i / a.gqa;
     plain_row<T, D, CODES>(a, b, w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, b, w.n, w.len, ti));
   }
+  return true;
+}
+
+template <class T, int D, bool CODES>
+__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(const TileArgs ta) {
+  __shared__ __attribute__((aligned(16))) TileLds<D> lds;
+  if (ta.a.clear) clear_rows<D>(ta.a);
+  // (At head dim 256 the two paths together are past the registers of one wave)
+  if constexpr (CODES && !T::kF16 && D <= 128) {
+    if (take_item<T, D, CODES, true>(ta, lds)) return;
+    __syncthreads();              // every wave has read what does not fit
+    asm volatile("" ::: "memory");
+  }
+  take_item<T, D, CODES, false>(ta, lds);
 }
 
 // Joins the parts of split sequences; a wave a row
@@ -409,7 +548,7 @@ __global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs
     if (base + count > kParts) return;
     for (long x = (long)blockIdx.x * kWaves + wave; x < (long)a.Hk * w.rows; x += (long)gridDim.x * kWaves) {
       const int h = (int)(x / w.rows), r = (int)(x - (long)h * w.rows);
-      const int tile = r / kTileRows, first = base + (h * w.row_tiles + w.row_tiles - 1 - tile) * parts;
+      const int tile = r / kTileRows, first = base + ((w.row_tiles - 1 - tile) * a.Hk + h) * parts;
       const int at = r - tile * kTileRows;
       float mc = -1e30f;
       for (int z = 0; z < parts; ++z) mc = fmaxf(mc, ta.mpart[2 * ((long)(first + z) * kTileRows + at)]);
@@ -460,7 +599,7 @@ int launch_tiles_of(const TileArgs& ta, unsigned items, hipStream_t s) {
   hipLaunchKernelGGL((tiles_kernel<T, D, CODES>), dim3(items), dim3(kAttnThreads), 0, s, ta);
   const int st = check_launch("paged_attention(tiles)");
   if (st) return st;
-  hipLaunchKernelGGL((join_tiles_kernel<T, D, CODES>), dim3(kSlots), dim3(kAttnThreads), 0, s, ta);
+  hipLaunchKernelGGL((join_tiles_kernel<T, D, CODES>), dim3(4 * kSlots), dim3(kAttnThreads), 0, s, ta);
   return check_launch("paged_attention(join tiles)");
 }
 

@@ -25,8 +25,12 @@ def make(g, dev, dtype, bits, Hq, Hk, D, P, lens, rows, behind=0):
 
 
 def check(args, got, scale, causal=True):
+    """Probabilities are two pieces of the type, 2^-16 off together; over 8-bit pages of a bf16 model prompt chunks take one fp16
+    piece: half a step, 2^-11 of the probability at most."""
     q, kp, vp, table, starts, lens = args
-    want, tol = attention(host(q), oracle_pages(kp), oracle_pages(vp), table.cpu().numpy(), starts.tolist(), lens.tolist(), scale, causal)
+    pieces = 2.0 ** -11 if isinstance(kp, tuple) and q.dtype is torch.bfloat16 else 2.0 ** -16
+    want, tol = attention(host(q), oracle_pages(kp), oracle_pages(vp), table.cpu().numpy(), starts.tolist(), lens.tolist(), scale, causal,
+                          pieces)
     check_rows(got, want, tol)
 
 
@@ -421,3 +425,17 @@ def test_captured_chunks(dev, bits):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         check((q, kp, vp, table, starts, lens), out, 0.1)
+
+
+def test_chunks_over_pages_of_extreme_scales(dev):
+    """8-bit pages whose values do not fit fp16: the largest and the smallest scales, alone and beside ordinary ones."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(16)
+    for low, high in ((-60, -59), (20, 21), (-30, 5)):
+        q, kp, vp, table, starts, lens = make(g, dev, "bf16", 8, 4, 2, 64, 16, [400, 90], [100, 90])
+        some = torch.randint(low, high, vp[1].shape, generator=g)
+        some[torch.rand(vp[1].shape, generator=g) < 0.5] = low
+        vp = (vp[0], (some + 127).to(torch.uint8).view(torch.float8_e8m0fnu).to(dev))
+        args = (q, kp, vp, table, starts, lens)
+        check(args, ops.paged_attention(*args, scale=0.125), 0.125)
