@@ -508,54 +508,103 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
   }
 }
 
-// Joins the parts of a KV head's rows: out = sum 2^(m_j - m) o_j / sum 2^(m_j - m) l_j over the runs j that have some of its
-// keys, in their order. A wave a row.
+// Parts of a row, joined by a wave: out = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z in the order of the keys. `part(z)`:
+// where part z's row stands among the outputs; its maximum (times `c` in the exponent) and sum at `stat(z)` and `stat(z)` +
+// `sums`. A lane looks at a part's maximum and sum, then N parts' outputs are on their way at a time.
+template <int C>
+struct Joined {
+  float v[C];                    // unnormalised columns of the lane
+  float m, l;
+};
+template <int D, int N, class Part, class Stat>
+__device__ __forceinline__ Joined<D / 64> join_parts(const float* o, const float* stats, int sums, float c, int parts, int first,
+                                                     int step, Part part, Stat stat) {
+  constexpr int C = D / 64;
+  typedef float cols_t __attribute__((ext_vector_type(C)));
+  const int lane = __lane_id();
+  Joined<C> r;
+#pragma unroll
+  for (int i = 0; i < C; ++i) r.v[i] = 0.f;
+  r.m = kLowest;
+  for (int z = lane; z < parts; z += 64) r.m = fmaxf(r.m, stats[stat(z)]);
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) r.m = fmaxf(r.m, shfl_xor(r.m, x));
+  r.l = 0.f;
+  for (int z0 = 0; z0 < parts; z0 += 64) {
+    const int z = min(z0 + lane, parts - 1);
+    const float f = z0 + lane < parts ? __builtin_amdgcn_exp2f((stats[stat(z)] - r.m) * c) : 0.f;
+    r.l += f * stats[stat(z) + sums];
+    const int n = min(64, parts - z0);
+    for (int j = first; j < n; j += step * N) {
+      cols_t x[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        x[k] = *reinterpret_cast<const cols_t*>(o + part(z0 + min(j + k * step, n - 1)) * D + C * lane);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float fk = j + k * step < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(j + k * step, n - 1))) : 0.f;
+        // (a part of weight 0 may hold what is not finite: it would have to count, were it there)
+#pragma unroll
+        for (int i = 0; i < C; ++i) r.v[i] = j + k * step < n ? __builtin_fmaf(fk, x[k][i], r.v[i]) : r.v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) r.l += shfl_xor(r.l, x);
+  return r;
+}
+
+// A joined row to its place, by a wave
+template <class T, int D, bool CODES>
+__device__ __forceinline__ void put_row(const AttnArgs& a, const float (&v)[D / 64], float l, int b, int t, int head, int keys) {
+  constexpr int C = D / 64;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  u16* op = a.out + t * a.orow + head * a.ohead + C * (int)__lane_id();
+  float zero = l - l;
+  u16 x[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    zero = __builtin_fmaf(v[i], 0.f, zero);
+    x[i] = attn::from_f32<T>(v[i] * inv);
+  }
+  if constexpr (C == 4) *reinterpret_cast<u32x2_t*>(op) = u32x2_t{x[0] | (u32)x[1] << 16, x[2] | (u32)x[3] << 16};
+  else if constexpr (C == 2) *reinterpret_cast<u32*>(op) = x[0] | (u32)x[1] << 16;
+  else op[0] = x[0];
+  if (__builtin_amdgcn_ballot_w64(zero != 0.f)) plain_row<T, D, CODES>(a, b, t, head, keys);
+}
+
+// Joins the parts of a KV head's rows, a workgroup a row: its waves take every fourth part
 template <class T, int D, int RT, bool CODES>
 __global__ __launch_bounds__(kAttnThreads) void join_kernel(const AttnArgs a, int workgroups) {
   constexpr int ROWS = 16 * RT, C = D / 64;
-  typedef float cols_t __attribute__((ext_vector_type(C)));
+  __shared__ float sm[kWaves][D];
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
   Work w = work_of<RT>(a, b);
   w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
-  if ((int)blockIdx.y * kWaves >= w.rows) return;
-  // units before this sequence, and of all
+  if ((int)blockIdx.y >= w.rows) return;
   int before = 0;
   const int units = all_units<RT>(a, b, &before);
   if (!units) return;
   const int run = run_of(a, units, workgroups);
-  for (int r = blockIdx.y * kWaves + wave; r < w.rows; r += gridDim.y * kWaves) {
+  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
     const int group = r / ROWS, rw = r - group * ROWS;
     const int u0 = before + (h * w.groups + group) * w.tiles, u1 = u0 + w.tiles;
     const int j0 = u0 / run, j1 = (u1 - 1) / run;
     if (j0 == j1) continue;
-    auto slot = [&](int j) { return (2 * (long)j + (j == j0 ? 1 : 0)) * ROWS; };
-    float m = kLowest;
-    for (int j = j0 + lane; j <= j1; j += 64) m = fmaxf(m, a.mpart[2 * slot(j) + rw]);
+    auto slot = [&](int z) { return (2 * (long)(j0 + z) + (z == 0 ? 1 : 0)) * ROWS; };
+    Joined<C> x = join_parts<D, (C == 4 ? 8 : 16)>(a.opart, a.mpart, ROWS, a.scale_log2, j1 - j0 + 1, wave, kWaves,
+                                                  [&](int z) { return slot(z) + rw; }, [&](int z) { return 2 * slot(z) + rw; });
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, shfl_xor(m, x));
-    cols_t acc;
+    for (int i = 0; i < C; ++i) sm[wave][C * lane + i] = x.v[i];
+    __syncthreads();
+    if (wave == 0) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = 0.f;
-    float l = 0.f;
-    for (int j = j0; j <= j1; ++j) {
-      const float f = __builtin_amdgcn_exp2f((a.mpart[2 * slot(j) + rw] - m) * a.scale_log2);
-      l += f * a.mpart[2 * slot(j) + ROWS + rw];
-      const cols_t x = *reinterpret_cast<const cols_t*>(a.opart + (slot(j) + rw) * D + C * lane);
-#pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(f, x[c], acc[c]);
+      for (int i = 0; i < C; ++i) x.v[i] = (sm[0][C * lane + i] + sm[1][C * lane + i]) + (sm[2][C * lane + i] + sm[3][C * lane + i]);
+      const int i = r / a.gqa;
+      put_row<T, D, CODES>(a, x.v, x.l, b, w.start + i, h * a.gqa + r - i * a.gqa, keys_seen(a, b, w.n, w.len, i));
     }
-    const int i = r / a.gqa, head = h * a.gqa + r - i * a.gqa;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    u16* op = a.out + (w.start + i) * a.orow + head * a.ohead + C * lane;
-    float zero = l - l;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      zero = __builtin_fmaf(acc[c], 0.f, zero);
-      op[c] = attn::from_f32<T>(acc[c] * inv);
-    }
-    if (__builtin_amdgcn_ballot_w64(zero != 0.f))
-      plain_row<T, D, CODES>(a, b, w.start + i, head, keys_seen(a, b, w.n, w.len, i));
+    __syncthreads();
   }
 }
 
@@ -564,7 +613,7 @@ int launch_rows(const AttnArgs& a, int workgroups, int most_rows, hipStream_t s)
   hipLaunchKernelGGL((rows_kernel<T, D, RT, CODES>), dim3((unsigned)workgroups), dim3(kAttnThreads), 0, s, a);
   const int st = check_launch("paged_attention");
   if (st || a.whole) return st;
-  const unsigned y = (unsigned)((std::min(most_rows, 16 * RT) + kWaves - 1) / kWaves);     // more rows: a loop
+  const unsigned y = (unsigned)std::min(most_rows, 16 * RT);     // more rows: a loop
   hipLaunchKernelGGL((join_kernel<T, D, RT, CODES>), dim3((unsigned)(a.s.B * a.Hk), y), dim3(kAttnThreads), 0, s, a, workgroups);
   return check_launch("paged_attention(join)");
 }

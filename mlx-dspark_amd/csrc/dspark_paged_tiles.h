@@ -32,8 +32,9 @@ namespace paged {
 
 constexpr int kTileRows = 128;    // rows of a workgroup
 constexpr int kTileKeys = 64;
-constexpr int kSlots = 512;       // workgroups that run together: two a CU
-constexpr int kParts = 704;       // parts of split sequences, at most: 2 kSlots / 1.5 and what rounding adds
+template <int D>
+constexpr int kSlots = D == 256 ? 256 : 512;     // workgroups that run together: two a CU, at head dim 256 one
+constexpr int kParts = 704;       // parts of split sequences, at most: 2 * 512 / 1.5 and what rounding adds
 constexpr int kLeastTiles = 8;    // key tiles of a part, at least
 
 constexpr int kAluMayCross = 0x2 | 0x4;     // of a scheduling barrier: vector and scalar arithmetic
@@ -59,6 +60,7 @@ __device__ __forceinline__ TileWork tile_work(const AttnArgs& a, int b) {
 }
 
 // Key tiles that a part may have before it is split: 1.5 times the average share of a slot
+template <int D>
 __device__ __forceinline__ int target_tiles(const AttnArgs& a) {
   const int lane = __lane_id();
   float sum = 0.f;                // a rule, not a count: rounding does not matter
@@ -69,7 +71,7 @@ __device__ __forceinline__ int target_tiles(const AttnArgs& a) {
   }
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) sum += shfl_xor(sum, x);
-  const float t = 1.5f * sum * (float)a.Hk / kSlots;
+  const float t = 1.5f * sum * (float)a.Hk / kSlots<D>;
   return uniform(t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1);
 }
 
@@ -199,7 +201,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15;
 
-  const int target = target_tiles(a);
+  const int target = target_tiles<D>(a);
   const u32 all = items_of_all(a, target);
   if (all > kMostUnits) return true;
   // Of the 512 that start together, two a CU, the second 256 in turned order: a long causal tile shares its CU with a
@@ -533,10 +535,9 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(c
 template <class T, int D, bool CODES>
 __global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs ta) {
   constexpr int C = D / 64;
-  typedef float cols_t __attribute__((ext_vector_type(C)));
   const AttnArgs& a = ta.a;
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-  const int target = target_tiles(a);
+  const int wave = uniform((int)(threadIdx.x >> 6));
+  const int target = target_tiles<D>(a);
   if (items_of_all(a, target) > kMostUnits) return;
   int base = 0;                   // parts before sequence b
   for (int b = 0; b < a.s.B && base < kParts; ++b) {
@@ -550,31 +551,11 @@ __global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs
       const int h = (int)(x / w.rows), r = (int)(x - (long)h * w.rows);
       const int tile = r / kTileRows, first = base + ((w.row_tiles - 1 - tile) * a.Hk + h) * parts;
       const int at = r - tile * kTileRows;
-      float mc = -1e30f;
-      for (int z = 0; z < parts; ++z) mc = fmaxf(mc, ta.mpart[2 * ((long)(first + z) * kTileRows + at)]);
-      cols_t acc;
-#pragma unroll
-      for (int i = 0; i < C; ++i) acc[i] = 0.f;
-      float l = 0.f;
-      for (int z = 0; z < parts; ++z) {
-        const long pr = (long)(first + z) * kTileRows + at;
-        const float f = __builtin_amdgcn_exp2f(ta.mpart[2 * pr] - mc);
-        l += f * ta.mpart[2 * pr + 1];
-        const cols_t v = *reinterpret_cast<const cols_t*>(ta.opart + pr * D + C * lane);
-#pragma unroll
-        for (int i = 0; i < C; ++i) acc[i] = __builtin_fmaf(f, v[i], acc[i]);
-      }
-      const int tok = r / a.gqa, head = h * a.gqa + r - tok * a.gqa;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      u16* op = a.out + (w.start + tok) * a.orow + head * a.ohead + C * lane;
-      float zero = l - l;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        zero = __builtin_fmaf(acc[i], 0.f, zero);
-        op[i] = attn::from_f32<T>(acc[i] * inv);
-      }
-      if (__builtin_amdgcn_ballot_w64(zero != 0.f))
-        plain_row<T, D, CODES>(a, b, w.start + tok, head, keys_seen(a, b, w.n, w.len, tok));
+      const Joined<C> v = join_parts<D, 8>(ta.opart, ta.mpart, 1, 1.f, parts, 0, 1,
+                                           [&](int z) { return (long)(first + z) * kTileRows + at; },
+                                           [&](int z) { return 2 * ((long)(first + z) * kTileRows + at); });
+      const int tok = r / a.gqa;
+      put_row<T, D, CODES>(a, v.v, v.l, b, w.start + tok, h * a.gqa + r - tok * a.gqa, keys_seen(a, b, w.n, w.len, tok));
     }
     base += count;
   }
@@ -599,7 +580,7 @@ int launch_tiles_of(const TileArgs& ta, unsigned items, hipStream_t s) {
   hipLaunchKernelGGL((tiles_kernel<T, D, CODES>), dim3(items), dim3(kAttnThreads), 0, s, ta);
   const int st = check_launch("paged_attention(tiles)");
   if (st) return st;
-  hipLaunchKernelGGL((join_tiles_kernel<T, D, CODES>), dim3(4 * kSlots), dim3(kAttnThreads), 0, s, ta);
+  hipLaunchKernelGGL((join_tiles_kernel<T, D, CODES>), dim3(2048), dim3(kAttnThreads), 0, s, ta);
   return check_launch("paged_attention(join tiles)");
 }
 
