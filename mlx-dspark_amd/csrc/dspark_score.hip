@@ -8,12 +8,15 @@
 //
 // The alternatives come out of the same pass. A candidate is a 64-bit key, value before inverted index, so that no two are
 // equal and the order is total. A wave keeps a list of candidates in LDS and a least key, under which k better ones are
-// known; 32 values a lane are compared by their maximum, which the sums need anyway, and looked at only where it reaches the
-// least key. The least key starts as the k-th of the 64 lanes' maxima, rises when a full list is cut to its k best, and
-// is shared by the workgroup's waves.
+// known; a lane's values of a step are compared by their maximum, which the sums need anyway, and looked at only where it
+// reaches the least key (passes it, once the wave is behind the least key's index: rows of equal values, as of forbidden
+// tokens, cost no more). The least key starts as the k-th of the 64 lanes' maxima, rises when a full list is cut to its k best,
+// and is shared by the workgroup's waves.
 //
-// Bound by the bytes of the logits, with the exponential (a quarter of the rate) and about 10 more instructions a value
-// close behind. Many rows: a workgroup a row; few: up to 64 workgroups, joined by a second launch.
+// Bound by the bytes of the logits, with the exponential (a quarter of the rate) and about 6 more instructions a value
+// close behind. Many rows: a workgroup of four waves a row; few: up to 64 waves a row, a workgroup each, joined by a second
+// launch. bf16, 900 rows of 128255: 54 us (4.3 TB/s), 74 with the best 5; one row of 151936: 6 us, 18 with the best 20,
+// of which the list takes its time from a wave that has nothing beside it on its SIMD.
 #include <algorithm>
 #include <cmath>
 
@@ -24,11 +27,9 @@ namespace {
 
 using u64 = unsigned long long;
 
-constexpr int kScoreThreads = 256;
-constexpr int kScoreWaves = kScoreThreads / 64;
-constexpr int kPer = 32;                       // values of a lane's step
+constexpr int kScoreWaves = 4;                 // of a workgroup that takes a whole row
 constexpr int kMostTop = 64;
-constexpr int kList = 320;                     // candidates of a wave
+constexpr int kList = 192;                     // candidates of a wave: 1.5 times the most, 16, and a key of every lane
 constexpr int kMostSegments = 64;              // of a row: a lane each where they are joined
 constexpr float kScoreLowest = -3.402823466e38f;
 constexpr float kNothing = -1e4f;              // an exponent whose power of two is 0, times which 0 is 0
@@ -77,11 +78,6 @@ __device__ __forceinline__ int index_of(u64 k) { return (int)~(u32)k; }
 __device__ __forceinline__ u64 lane_key(u64 k, int l) {
   return (u64)(u32)__builtin_amdgcn_readlane((int)(k >> 32), l) << 32 | (u32)__builtin_amdgcn_readlane((int)(u32)k, l);
 }
-__device__ __forceinline__ u64 xor_key(u64 k, int m) {
-  const int at = (__lane_id() ^ m) << 2;
-  return (u64)(u32)__builtin_amdgcn_ds_bpermute(at, (int)(k >> 32)) << 32 | (u32)__builtin_amdgcn_ds_bpermute(at, (int)(u32)k);
-}
-
 struct Stats {
   float m, s, u;                               // maximum, sum of 2^d, sum of d 2^d, d = (x - m) c
 };
@@ -98,9 +94,9 @@ __device__ __forceinline__ Stats join_wave(Stats s, float c) {
   return s;
 }
 
-// The k best of a wave's list of n, in order at its start; how many there are
+// The k best of a wave's list of n (up to 64 N), in order at its start; how many there are
+template <int N>
 __device__ __forceinline__ int cut_list(u64* list, int n, int k) {
-  constexpr int N = kList / 64;
   const int lane = __lane_id();
   u64 mine[N];
   int rank[N];
@@ -109,6 +105,7 @@ __device__ __forceinline__ int cut_list(u64* list, int n, int k) {
     mine[i] = 64 * i + lane < n ? list[64 * i + lane] : 0;
     rank[i] = 0;
   }
+#pragma unroll 4
   for (int j = 0; j < n; ++j) {
     const u64 o = list[j];
 #pragma unroll
@@ -162,16 +159,64 @@ __device__ __forceinline__ void finish_row(const ScoreArgs& a, long row, Stats s
   }
 }
 
-template <int DT, bool TOP>
-__global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a) {
+// Keys of a wave's list, and the least one under which k better ones are known
+struct List {
+  u64* keys;
+  int n, top, full;
+  u64 least;
+  u64* shared;                                 // the workgroup's least key (null: one wave)
+
+  __device__ __forceinline__ void raise(u64 k) {
+    if (k <= least) return;
+    least = k;
+    if (shared && __lane_id() == 0) atomicMax(shared, k);
+  }
+  // Where 64 lanes' best keys come to k of at least some key, that is a least key
+  __device__ __forceinline__ void raise_by(u64 best) {
+    keys[n + __lane_id()] = best;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) rank += keys[n + j] > best ? 1 : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u64 kth = __builtin_amdgcn_ballot_w64(rank == top - 1 && best != 0);
+    if (kth) raise(lane_key(best, __builtin_ctzll(kth)));
+  }
+  // A key of every lane (0: none)
+  __device__ __forceinline__ void push(u64 k) {
+    const u64 in = __builtin_amdgcn_ballot_w64(k != 0 && k >= least);
+    if (!in) return;
+    if (k != 0 && k >= least) keys[n + __builtin_popcountll(in & ((1ull << __lane_id()) - 1))] = k;
+    n = uniform(n + __builtin_popcountll(in));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (n > full) cut();
+  }
+  __device__ __forceinline__ void cut() {
+    n = uniform(n <= 64 ? cut_list<1>(keys, n, top) : cut_list<kList / 64>(keys, n, top));
+    if (n == top) raise(keys[top - 1]);
+  }
+};
+__device__ __forceinline__ List new_list(u64* keys, int top, u64* shared) {
+  return List{keys, 0, top, top + top / 2 + 16, 0, shared};
+}
+
+// kPer: values of a lane's step. A wave that has a row's part for itself takes 8: it is alone on its SIMD, and what counts is
+// how many instructions it issues until it is done.
+template <int DT, bool TOP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void score_kernel(const ScoreArgs a) {
   using T = typename Logit<DT>::t;
+  constexpr int kPer = WAVES == 1 ? 8 : 32;
   constexpr int E = 16 / sizeof(T), NL = kPer / E;           // values of a 16-byte load, loads of a step
+  constexpr int STEP = 64 * NL;                              // 16-byte chunks of a wave's step
   struct alignas(16) Vec { T v[E]; };
-  __shared__ u64 lists[kScoreWaves][TOP ? kList : 1];
+  __shared__ u64 lists[WAVES][TOP ? kList : 1];
   __shared__ u64 least_of_all;
-  __shared__ Stats parts[kScoreWaves];
-  __shared__ int counts[kScoreWaves];
-  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  __shared__ Stats parts[WAVES];
+  __shared__ int counts[WAVES];
+  const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : uniform((int)(threadIdx.x >> 6));
   const long row = blockIdx.x / a.segments;
   const int seg = blockIdx.x - (int)row * a.segments;
   const T* const x0 = reinterpret_cast<const T*>(a.x) + row * a.ld;
@@ -180,20 +225,25 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a)
   const Vec* const chunks = reinterpret_cast<const Vec*>(x0 - off);
   const int nc = (int)(((long)a.V + off + E - 1) / E), per = (nc + a.segments - 1) / a.segments;
   const int c0 = (int)min((long)seg * per, (long)nc), c1 = min(c0 + per, nc);
-  u64* const list = lists[wave];
-  int n = 0;                                                 // of the list
-  const int full = min(kList - 64, 2 * a.top + 64);
-  u64 least = 0;
-  if (TOP) {
+  const int w0 = off ? 1 : 0, w1 = min(c1, (int)(((long)a.V + off) / E));      // chunks that are all the row's
+  List list = new_list(lists[wave], a.top, WAVES > 1 ? &least_of_all : nullptr);
+  if (TOP && WAVES > 1) {
     if (threadIdx.x == 0) least_of_all = 0;
     __syncthreads();
   }
 
+  auto whole = [&](int c) { return c >= w0 && c + STEP <= w1; };
   auto load = [&](Vec (&v)[NL], int c) {
+    if (whole(c)) {
+      const Vec* p = chunks + c + lane;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) v[j] = p[64 * j];
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int k = c + 64 * j + lane;
-      if (k < c1 && k * E >= off && (long)(k + 1) * E <= (long)a.V + off) {
+      if (k >= w0 && k < w1) {
         v[j] = chunks[k];
       } else {
 #pragma unroll
@@ -210,18 +260,19 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a)
   };
 
   Stats st{kScoreLowest, 0.f, 0.f};
-  const int step = 64 * NL * kScoreWaves;
-  int c = c0 + wave * 64 * NL;
+  int c = c0 + wave * STEP;
   Vec next[NL];
   if (c < c1) load(next, c);
   while (c < c1) {
+    u64 shared = 0;
+    if (TOP && WAVES > 1) shared = *(volatile u64*)&least_of_all;
     float x[kPer];
 #pragma unroll
     for (int j = 0; j < NL; ++j)
 #pragma unroll
       for (int e = 0; e < E; ++e) x[j * E + e] = Logit<DT>::get(next[j].v[e]);
     const int cur = c;
-    c += step;
+    c += WAVES * STEP;
     if (c < c1) load(next, c);
     float top = -__builtin_inff();
 #pragma unroll
@@ -231,104 +282,75 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a)
     st.u = f * (st.u + d0 * st.s);
     st.s *= f;
     st.m = m;
+    float s1 = 0.f, u1 = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const float d = fmaxf((x[i] - m) * a.c, kNothing), e = __builtin_amdgcn_exp2f(d);
-      st.s += e;
-      st.u = __builtin_fmaf(e, d, st.u);
+      (i & 1 ? s1 : st.s) += e;
+      if (i & 1) u1 = __builtin_fmaf(e, d, u1);
+      else st.u = __builtin_fmaf(e, d, st.u);
     }
+    st.s += s1;
+    st.u += u1;
     if constexpr (TOP) {
-      const u64 shared = least_of_all;
-      least = shared > least ? shared : least;
-      const u64 some = __builtin_amdgcn_ballot_w64(top >= (least ? value_of(least) : -__builtin_inff()));
-      if (!some) continue;
-      auto index = [&](int i) { return (int)((long)(cur + 64 * (i / E) + lane) * E + i % E - off); };
-      auto key = [&](int i) {
-        const int at = index(i);
-        return at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1 ? key_of(x[i], at) : 0;
+      list.least = shared > list.least ? shared : list.least;
+      // what a value has to reach: the least key's, or the next one up where all of the step's indices lie behind its
+      auto needed = [&] {
+        if (!list.least) return -__builtin_inff();
+        const bool behind = (long)cur * E - off > (long)index_of(list.least);
+        return value_of(behind ? list.least + (1ull << 32) : list.least);
       };
-      if (__builtin_popcountll(some) >= a.top) {
-        // the k-th of the lanes' best: k values at least reach it
-        u64 best = 0;
+      const u64 some = __builtin_amdgcn_ballot_w64(top >= needed());
+      if (!some) continue;
+      const bool all = whole(cur);
+      auto index = [&](int i) { return (int)((long)(cur + 64 * (i / E) + lane) * E + i % E - off); };
+      auto there = [&](int i) {
+        const int at = index(i);
+        return all || (at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1);
+      };
+      if (__builtin_popcountll(some) >= max(a.top, 16)) {
+        u64 best = 0;                                        // the lane's: the first of its largest
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const u64 k = key(i);
-          best = k > best ? k : best;
-        }
-        int rank = 0;
-        for (int j = 0; j < 64; ++j) rank += lane_key(best, j) > best ? 1 : 0;
-        const u64 kth = __builtin_amdgcn_ballot_w64(rank == a.top - 1 && best != 0);
-        if (kth) {
-          const u64 k = lane_key(best, __builtin_ctzll(kth));
-          if (k > least) {
-            least = k;
-            if (lane == 0) atomicMax(&least_of_all, k);
-          }
-        }
+        for (int i = kPer - 1; i >= 0; --i)
+          if ((x[i] == top || top == -__builtin_inff()) && there(i)) best = (u32)~index(i);
+        if (best) best |= key_of(top, 0) & 0xFFFFFFFF00000000ull;
+        list.raise_by(best);
       }
-      const float least_value = least ? value_of(least) : -__builtin_inff();
+      // Bit i: value i reaches the least key's (NaN counts as -inf). Such values are read again: there are few, and one
+      // copy of the code that lists a value, where 32 would not fit the instruction cache
+      const float least_value = needed();
+      const bool nan_too = least_value == -__builtin_inff();
+      u32 mask = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        // (NaN counts as -inf)
-        const bool maybe = !(x[i] < least_value);
-        if (!__builtin_amdgcn_ballot_w64(maybe)) continue;
-        const u64 k = maybe ? key(i) : 0;
-        const u64 in = __builtin_amdgcn_ballot_w64(k != 0 && k >= least);
-        if (!in) continue;
-        if (k != 0 && k >= least) list[n + __builtin_popcountll(in & ((1ull << lane) - 1))] = k;
-        n = uniform(n + __builtin_popcountll(in));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (n > full) {
-          n = uniform(cut_list(list, n, a.top));
-          const u64 k = list[a.top - 1];
-          if (k > least) {
-            least = k;
-            if (lane == 0) atomicMax(&least_of_all, k);
-          }
-        }
+      for (int i = kPer - 1; i >= 0; --i) mask = mask + mask + (x[i] >= least_value ? 1u : 0u);
+      if (nan_too) mask = 0xFFFFFFFFu >> (32 - kPer);
+      while (__builtin_amdgcn_ballot_w64(mask != 0)) {
+        const int i = mask ? __builtin_ctz(mask) : 0, at = (int)((long)(cur + 64 * (i / E) + lane) * E + i % E - off);
+        u64 k = 0;
+        if (mask && at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1) k = key_of(Logit<DT>::get(x0[at]), at);
+        mask &= mask - 1;
+        list.push(k);
       }
     }
   }
 
   st = join_wave(st, a.c);
-  if (TOP) {
-    n = uniform(cut_list(list, n, a.top));
-    if (lane == 0) counts[wave] = n;
-  }
-  if (lane == 0) parts[wave] = st;
-  __syncthreads();
-  if (TOP && kScoreWaves > 1) {
-    // every wave's keys find their places among all
-    u64 mine[kScoreWaves];
-    int rank[kScoreWaves];
-    for (int w = 0; w < kScoreWaves; ++w) {
-      mine[w] = lane < counts[w] ? lists[w][lane] : 0;
-      rank[w] = 0;
+  if (TOP) list.cut();
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      parts[wave] = st;
+      counts[wave] = list.n;
     }
-    if (wave == 0) {
-      for (int w = 0; w < kScoreWaves; ++w)
-        for (int j = 0; j < counts[w]; ++j) {
-          const u64 o = lists[w][j];
-#pragma unroll
-          for (int v = 0; v < kScoreWaves; ++v) rank[v] += o > mine[v] ? 1 : 0;
-        }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (lane < a.top) lists[0][lane] = 0;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int v = 0; v < kScoreWaves; ++v)
-        if (mine[v] && rank[v] < a.top) lists[0][rank[v]] = mine[v];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll 1
+    for (int w = 1; w < WAVES; ++w) {
+      st = join(st, parts[w], a.c);
+      if (TOP) list.push(lane < counts[w] ? lists[w][lane] : 0);
     }
+    if (TOP) list.cut();
   }
-  if (wave != 0) return;
-#pragma unroll
-  for (int w = 1; w < kScoreWaves; ++w) st = join(st, parts[w], a.c);
-  const u64 mine = TOP && lane < a.top ? lists[0][lane] : 0;
+  const u64 mine = TOP && lane < list.n ? list.keys[lane] : 0;
   if (a.segments == 1) {
     finish_row<DT>(a, row, st, mine);
     return;
@@ -340,9 +362,10 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const ScoreArgs a)
   if (TOP && lane < a.top) a.keys[(row * a.segments + seg) * a.top + lane] = mine;
 }
 
-// A row's segments together, by one wave: a lane has a segment's sums, and the head of its keys
+// A row's segments together, by one wave: a lane has a segment's sums, and its keys, which fall
 template <int DT>
 __global__ __launch_bounds__(64) void join_scores_kernel(const ScoreArgs a) {
+  __shared__ u64 keys[kList];
   const long row = blockIdx.x;
   const int lane = __lane_id();
   Stats s{kScoreLowest, 0.f, 0.f};
@@ -350,38 +373,43 @@ __global__ __launch_bounds__(64) void join_scores_kernel(const ScoreArgs a) {
     const float* from = a.stats + 3 * (row * a.segments + lane);
     s = Stats{from[0], from[1], from[2]};
   }
-  s = join_wave(s, a.c);
-  const u64* keys = a.keys + (row * a.segments + lane) * a.top;
-  int at = 0;
-  u64 head = lane < a.segments && a.top ? keys[0] : 0, mine = 0;
-  for (int i = 0; i < a.top; ++i) {
-    u64 best = head;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) {
-      const u64 o = xor_key(best, x);
-      best = o > best ? o : best;
+  u64 mine = 0;
+  if (a.top) {
+    List list = new_list(keys, a.top, nullptr);
+    const u64* from = a.keys + (row * a.segments + min(lane, a.segments - 1)) * a.top;
+    u64 k = lane < a.segments ? from[0] : 0;
+    if (a.segments >= a.top) list.raise_by(k);
+#pragma unroll 1
+    for (int i = 1; __builtin_amdgcn_ballot_w64(k != 0 && k >= list.least); ++i) {
+      const u64 next = lane < a.segments && i < a.top ? from[i] : 0;
+      list.push(k);
+      k = next;
     }
-    if (lane == i) mine = best;
-    if (head == best && head) head = ++at < a.top ? keys[at] : 0;
+    list.cut();
+    if (lane < list.n) mine = keys[lane];
   }
-  finish_row<DT>(a, row, s, mine);
+  finish_row<DT>(a, row, join_wave(s, a.c), mine);
 }
 
-// Workgroups of a row: enough for two a CU together, each with at least 2048 values
+// Segments of a row: 1 from 512 rows on, a workgroup each; fewer rows are dealt to 2048 waves, of at least 1024 values
 int score_segments(int64_t rows, int64_t V) {
-  const int64_t want = (512 + rows - 1) / rows;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, kMostSegments, V / 2048}));
+  if (rows >= 512) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + rows - 1) / rows, kMostSegments, V / 1024}));
 }
 
-template <int DT>
+template <int DT, bool TOP>
 int launch_score(const ScoreArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.rows * (long)a.segments)), block(kScoreThreads);
-  if (a.top) hipLaunchKernelGGL((score_kernel<DT, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((score_kernel<DT, false>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)(a.rows * (long)a.segments));
+  if (a.segments == 1) hipLaunchKernelGGL((score_kernel<DT, TOP, kScoreWaves>), grid, dim3(64 * kScoreWaves), 0, s, a);
+  else hipLaunchKernelGGL((score_kernel<DT, TOP, 1>), grid, dim3(64), 0, s, a);
   const int st = check_launch("token_logprobs");
   if (st || a.segments == 1) return st;
   hipLaunchKernelGGL((join_scores_kernel<DT>), dim3((unsigned)a.rows), dim3(64), 0, s, a);
   return check_launch("token_logprobs(join)");
+}
+template <int DT>
+int launch_score(const ScoreArgs& a, hipStream_t s) {
+  return a.top ? launch_score<DT, true>(a, s) : launch_score<DT, false>(a, s);
 }
 
 }  // namespace
