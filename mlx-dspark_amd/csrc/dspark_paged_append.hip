@@ -12,7 +12,11 @@
 // of the earlier rows shifted where E grew. Infinities and NaN become NaN codes.
 //
 // Bound by bytes. Rows: a workgroup forms cos and sin of its row once in LDS for all heads. 8-bit pages: a workgroup a
-// (page, KV head, keys or values), since the scale needs all its rows first; they wait in LDS.
+// (page, KV head, keys or values), since the scale needs all its rows first; they wait in LDS. Its threads take the
+// angles that they need themselves, as no other head shares them there; a page's chain of loads and angles is what takes
+// the time of a step with fewer pages than the card has compute units (workgroups of 512 and 1024 threads shorten it by
+// 15% there, and cost as much and more where there are many). bf16: one row of 32 / 8 heads of 128 3.5 us, 2048 rows of 64 / 8
+// 18 to 20 us (4.3 to 4.6 TB/s); 8-bit pages, 48 single rows 5 us, chunks of 77 to 600 rows of 24 / 4 heads of 256 14 us.
 #include <algorithm>
 
 #include "dspark_paged.h"
@@ -25,7 +29,6 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTab = 2048;       // (cos, sin) pairs of a workgroup
 
 struct Rows {                    // [T, heads, D]; strides in elements
   const char* x;
@@ -45,7 +48,8 @@ struct AppendArgs {
   const void* pos;               // null: the positions that the rows are written to
   int pos64;
   long pstride;
-  int row_blocks, parts;         // workgroups of the rows, of one row
+  int page_blocks;               // workgroups of the pages, which come before those of the rows
+  int parts;                     // workgroups of a row
 };
 
 template <int DT>
@@ -94,34 +98,34 @@ struct Item {
   int d, d2;                     // d2 < 0: no second part
 };
 
-template <int DT, bool INTER>
-__device__ __forceinline__ Item rotated_item(const AppendArgs& a, const u16* x, const float2* tab, int c) {
+template <bool INTER>
+__device__ __forceinline__ Item load_item(const AppendArgs& a, const u16* x, int c) {
   Item it;
   const int rot = INTER ? a.half / 4 : a.half / 8;
-  it.d2 = -1;
-  if (c >= rot) {
-    it.d = 2 * a.half + 8 * (c - rot);
-    it.lo = ldg128(x + it.d);
-    return it;
-  }
-  it.d = 8 * c;
+  it.d = c < rot ? 8 * c : 2 * a.half + 8 * (c - rot);
+  it.d2 = !INTER && c < rot ? it.d + a.half : -1;
   it.lo = ldg128(x + it.d);
+  if (it.d2 >= 0) it.hi = ldg128(x + it.d2);
+  return it;
+}
+
+template <int DT, bool INTER, class F>
+__device__ __forceinline__ void turn_item(const AppendArgs& a, Item& it, F turn) {
+  if (INTER ? it.d >= 2 * a.half : it.d2 < 0) return;
   if constexpr (INTER) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 cs = tab[4 * c + i];
+      const float2 cs = turn(it.d / 2 + i);
       const float u = get<DT>(it.lo[i]), v = get<DT>(it.lo[i] >> 16);
       it.lo[i] = put<DT>(u * cs.x - v * cs.y) | put<DT>(u * cs.y + v * cs.x) << 16;
     }
   } else {
-    it.d2 = it.d + a.half;
-    it.hi = ldg128(x + it.d2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32 y1[2], y2[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float2 cs = tab[8 * c + 2 * i + j];
+        const float2 cs = turn(it.d + 2 * i + j);
         const float u = get<DT>(it.lo[i] >> (16 * j)), v = get<DT>(it.hi[i] >> (16 * j));
         y1[j] = put<DT>(u * cs.x - v * cs.y);
         y2[j] = put<DT>(u * cs.y + v * cs.x);
@@ -130,7 +134,6 @@ __device__ __forceinline__ Item rotated_item(const AppendArgs& a, const u16* x, 
       it.hi[i] = y2[0] | y2[1] << 16;
     }
   }
-  return it;
 }
 
 __device__ __forceinline__ void stg128(void* p, u32x4_t v) { *static_cast<u32x4_t*>(p) = v; }
@@ -138,7 +141,10 @@ __device__ __forceinline__ void stg128(void* p, u32x4_t v) { *static_cast<u32x4_
 // One row: its queries rotated, and into pages of the model's type its keys and values
 template <int DT, bool INTER, bool KV>
 __device__ __forceinline__ void append_row(const AppendArgs& a, float2* tab) {
-  const int t = blockIdx.x / a.parts, part = blockIdx.x - t * a.parts, lane = __lane_id();
+  const int unit = blockIdx.x - a.page_blocks, t = unit / a.parts, part = unit - t * a.parts, lane = __lane_id();
+  const int plain = a.D / 8, log_plain = __builtin_ctz(plain);
+  const int rot = INTER ? a.half / 4 : a.half / 8, per = rot + (a.D - 2 * a.half) / 8;
+  const int heads = a.Hq + (KV ? a.Hk : 0), turned = heads * per, all = turned + (KV ? a.Hk * plain : 0);
   // its sequence
   int b = -1, n0 = 0, n1 = 0;
   for (int b0 = 0; b0 < a.s.B && b < 0; b0 += 64) {
@@ -153,16 +159,13 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, float2* tab) {
     }
   }
   if (b < 0) {                   // a row of no sequence
-    for (int i = part * kThreads + threadIdx.x; a.clear && i < a.Hq * (a.D / 8); i += a.parts * kThreads)
-      stg128(reinterpret_cast<u16*>(a.qo) + t * a.qo_row + i / (a.D / 8) * a.qo_head + 8 * (i % (a.D / 8)), u32x4_t{0u, 0u, 0u, 0u});
+    for (int i = part * kThreads + threadIdx.x; a.clear && i < a.Hq * plain; i += a.parts * kThreads)
+      stg128(reinterpret_cast<u16*>(a.qo) + t * a.qo_row + (i >> log_plain) * a.qo_head + 8 * (i & (plain - 1)), u32x4_t{0u, 0u, 0u, 0u});
     return;
   }
-  const long p = (long)a.s.lens[b] - n1 + (t - n0);
-  const long rp = rotary_position(a, t, p);
+  const long p = (long)a.s.lens[b] - n1 + (t - n0), rp = rotary_position(a, t, p);
   for (int i = threadIdx.x; i < a.half; i += kThreads) tab[i] = cos_sin((double)rp * a.freqs[i], a.scale);
   __syncthreads();
-  const int rot = INTER ? a.half / 4 : a.half / 8, per = rot + (a.D - 2 * a.half) / 8, plain = a.D / 8;
-  const int heads = a.Hq + (KV ? a.Hk : 0), turned = heads * per, all = turned + (KV ? a.Hk * plain : 0);
   const int id = KV ? page_of(a.s, b, p) : -1;
   const long off = p & (a.s.P - 1);
   for (int i = part * kThreads + threadIdx.x; i < all; i += a.parts * kThreads) {
@@ -172,13 +175,14 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, float2* tab) {
       if (key && id < 0) continue;
       const Rows& r = key ? a.k : a.q;
       const int hs = key ? h - a.Hq : h;
-      const Item it = rotated_item<DT, INTER>(a, reinterpret_cast<const u16*>(r.x) + t * r.row + hs * r.head, tab, c);
+      Item it = load_item<INTER>(a, reinterpret_cast<const u16*>(r.x) + t * r.row + hs * r.head, c);
+      turn_item<DT, INTER>(a, it, [&](int j) { return tab[j]; });
       u16* y = key ? reinterpret_cast<u16*>(a.kp.data) + id * a.kp.page + hs * a.kp.head + off * a.kp.row
                    : reinterpret_cast<u16*>(a.qo) + t * a.qo_row + hs * a.qo_head;
       stg128(y + it.d, it.lo);
       if (it.d2 >= 0) stg128(y + it.d2, it.hi);
     } else if (id >= 0) {
-      const int j = i - turned, h = j / plain, c = j - h * plain;
+      const int j = i - turned, h = j >> log_plain, c = j & (plain - 1);
       stg128(reinterpret_cast<u16*>(a.vp.data) + id * a.vp.page + h * a.vp.head + off * a.vp.row + 8 * c,
              ldg128(reinterpret_cast<const u16*>(a.v.x) + t * a.v.row + h * a.v.head + 8 * c));
     }
@@ -222,8 +226,8 @@ __device__ __forceinline__ float exp2_of(int e) { return __builtin_bit_cast(floa
 
 // The rows new in one page of one KV head, keys or values
 template <int DT, bool INTER>
-__device__ __forceinline__ void append_page8(const AppendArgs& a, float2* tab, u16* stash, u32* joined) {
-  const int item = blockIdx.x - a.row_blocks, kind = item & 1, h = (item >> 1) % a.Hk;
+__device__ __forceinline__ void append_page8(const AppendArgs& a, u16* stash, u32* joined) {
+  const int item = blockIdx.x, kind = item & 1, h = (item >> 1) % a.Hk;
   int b, j;
   const auto count = [&](int i) {
     const Seq q = sequence(a.s, i);
@@ -241,37 +245,37 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, float2* tab, u
   const Pages& pg = kind ? a.vp : a.kp;
   const Rows& src = kind ? a.v : a.k;
   unsigned char* ep = pg.exps + id * pg.epage + h * pg.ehead;
-  const int half = kind ? 0 : a.half, D = a.D;
+  const int half = kind ? 0 : a.half, D = a.D, log8 = __builtin_ctz(D / 8);
   const int rot = INTER ? half / 4 : half / 8, per = rot + (D - 2 * half) / 8;
-  const int at_once = half ? kTab / half : rows;
   u32 m = 0;
-  for (int r0 = 0; r0 < rows; r0 += at_once) {
-    const int nr = min(at_once, rows - r0);
-    if (half) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < nr * half; i += kThreads) {
-        const int r = i / half, f = i - r * half;
-        tab[i] = cos_sin((double)rotary_position(a, t0 + r0 + r, base + lo + r0 + r) * a.freqs[f], a.scale);
+  if (half) {
+    const auto load = [&](int i) {
+      const int r = i / per;
+      return load_item<INTER>(a, reinterpret_cast<const u16*>(src.x) + (t0 + r) * src.row + h * src.head, i - r * per);
+    };
+    Item next = {};
+    if ((int)threadIdx.x < rows * per) next = load(threadIdx.x);
+    for (int i = threadIdx.x; i < rows * per;) {
+      Item it = next;
+      const int r = i / per;
+      i += kThreads;
+      if (i < rows * per) next = load(i);
+      const double at = (double)rotary_position(a, t0 + r, base + lo + r);
+      turn_item<DT, INTER>(a, it, [&](int f) { return cos_sin(at * a.freqs[f], a.scale); });
+      m = largest<DT>(it.lo, m);
+      stg128(stash + r * D + it.d, it.lo);
+      if (it.d2 >= 0) {
+        m = largest<DT>(it.hi, m);
+        stg128(stash + r * D + it.d2, it.hi);
       }
-      __syncthreads();
     }
-    for (int i = threadIdx.x; i < nr * per; i += kThreads) {
-      const int r = i / per, c = i - r * per;
-      const u16* x = reinterpret_cast<const u16*>(src.x) + (t0 + r0 + r) * src.row + h * src.head;
-      u16* y = stash + (r0 + r) * D;
-      if (half) {
-        const Item it = rotated_item<DT, INTER>(a, x, tab + r * half, c);
-        m = largest<DT>(it.lo, m);
-        stg128(y + it.d, it.lo);
-        if (it.d2 >= 0) {
-          m = largest<DT>(it.hi, m);
-          stg128(y + it.d2, it.hi);
-        }
-      } else {
-        const u32x4_t v = ldg128(x + 8 * c);
-        m = largest<DT>(v, m);
-        stg128(y + 8 * c, v);
-      }
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows << log8; i += kThreads) {
+      const int r = i >> log8, c = i - (r << log8);
+      const u32x4_t v = ldg128(reinterpret_cast<const u16*>(src.x) + (t0 + r) * src.row + h * src.head + 8 * c);
+      m = largest<DT>(v, m);
+      stg128(stash + 8 * i, v);
     }
   }
 #pragma unroll
@@ -289,16 +293,15 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, float2* tab, u
   e = max(e, old);
   const float unit = exp2_of(-e);
   unsigned char* to = reinterpret_cast<unsigned char*>(pg.data) + id * pg.page + h * pg.head;
-  for (int i = threadIdx.x; i < rows * (D / 8); i += kThreads) {
-    const int r = i / (D / 8), c = i - r * (D / 8);
-    *reinterpret_cast<u32x2_t*>(to + (lo + r) * pg.row + 8 * c) =
-        codes8<DT>(*reinterpret_cast<const u32x4_t*>(stash + r * D + 8 * c), unit);
+  for (int i = threadIdx.x; i < rows << log8; i += kThreads) {
+    const int r = i >> log8, c = i - (r << log8);
+    *reinterpret_cast<u32x2_t*>(to + (lo + r) * pg.row + 8 * c) = codes8<DT>(*reinterpret_cast<const u32x4_t*>(stash + 8 * i), unit);
   }
   if (lo && e > old) {
     const int by = old - e;
     const float f = by < -126 ? 0.f : exp2_of(by);
-    for (int i = threadIdx.x; i < lo * (D / 16); i += kThreads) {
-      const int r = i / (D / 16), c = i - r * (D / 16);
+    for (int i = threadIdx.x; i < lo << (log8 - 1); i += kThreads) {
+      const int r = i >> (log8 - 1), c = i - (r << (log8 - 1));
       u32x4_t* p = reinterpret_cast<u32x4_t*>(to + r * pg.row + 16 * c);
       u32x4_t v = *p;
 #pragma unroll
@@ -312,11 +315,15 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, float2* tab, u
 
 template <int DT, bool INTER, bool CODES>
 __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
-  extern __shared__ __attribute__((aligned(16))) char dynamic[];      // (cos, sin) pairs; codes: then a page's rows
-  __shared__ u32 joined[kThreads / 64];
-  float2* tab = reinterpret_cast<float2*>(dynamic);
-  if (!CODES || (int)blockIdx.x < a.row_blocks) append_row<DT, INTER, !CODES>(a, tab);
-  else append_page8<DT, INTER>(a, tab, reinterpret_cast<u16*>(tab + kTab), joined);
+  extern __shared__ __attribute__((aligned(16))) char dynamic[];      // (cos, sin) pairs of a row, or a page's rows
+  if constexpr (CODES) {
+    __shared__ u32 joined[kThreads / 64];
+    if ((int)blockIdx.x < a.page_blocks) {
+      append_page8<DT, INTER>(a, reinterpret_cast<u16*>(dynamic), joined);
+      return;
+    }
+  }
+  append_row<DT, INTER, !CODES>(a, reinterpret_cast<float2*>(dynamic));
 }
 
 // Pages by id as dense values [N, Hk, P, D], zeros for ids that the pool does not have
@@ -399,15 +406,15 @@ using namespace dspark;
 
 namespace {
 
-template <int DT, bool INTER, bool CODES>
-void launch_append(const paged::AppendArgs& a, unsigned blocks, size_t lds, hipStream_t s) {
-  hipLaunchKernelGGL((paged::append_kernel<DT, INTER, CODES>), dim3(blocks), dim3(paged::kThreads), lds, s, a);
+template <int DT, bool INTER>
+void launch_append(const paged::AppendArgs& a, bool codes, unsigned blocks, size_t lds, hipStream_t s) {
+  const dim3 grid(blocks), block(paged::kThreads);
+  if (codes) hipLaunchKernelGGL((paged::append_kernel<DT, INTER, true>), grid, block, lds, s, a);
+  else hipLaunchKernelGGL((paged::append_kernel<DT, INTER, false>), grid, block, lds, s, a);
 }
-
 template <int DT>
 void launch_append(const paged::AppendArgs& a, bool inter, bool codes, unsigned blocks, size_t lds, hipStream_t s) {
-  if (codes) inter ? launch_append<DT, true, true>(a, blocks, lds, s) : launch_append<DT, false, true>(a, blocks, lds, s);
-  else inter ? launch_append<DT, true, false>(a, blocks, lds, s) : launch_append<DT, false, false>(a, blocks, lds, s);
+  inter ? launch_append<DT, true>(a, codes, blocks, lds, s) : launch_append<DT, false>(a, codes, blocks, lds, s);
 }
 
 int take_rows(const char* what, const void* x, const int64_t st[2], paged::Rows* out) {
@@ -457,15 +464,14 @@ extern "C" int dspark_paged_append(const dspark_paged_append_args* p, dspark_str
   const int items = (a.Hq + (codes ? 0 : a.Hk)) * per + (codes ? 0 : a.Hk * (a.D / 8));
   a.parts = a.s.T >= 512 ? 1 : (items + paged::kThreads - 1) / paged::kThreads;
   if (a.parts < 1) a.parts = 1;
-  long blocks = 0;
-  if (items) blocks = (long)a.s.T * a.parts;
-  a.row_blocks = (int)blocks;
+  long blocks = items ? (long)a.s.T * a.parts : 0;
   size_t lds = (size_t)a.half * sizeof(float2);
   if (codes) {
     // a sequence's rows reach into one page more than they fill, at each end
-    const long segments = std::min<long>(a.s.T, a.s.T / p->P + 2L * a.s.B);
-    blocks += segments * a.Hk * 2;
-    lds = paged::kTab * sizeof(float2) + (size_t)(p->P * p->D) * 2;
+    const long pages = std::min<long>(a.s.T, a.s.T / p->P + 2L * a.s.B) * a.Hk * 2;
+    a.page_blocks = (int)std::min<long>(pages, INT32_MAX);
+    blocks += pages;
+    lds = std::max(lds, (size_t)(std::min<long>(p->P, a.s.T) * p->D * 2));
   }
   if (blocks >= (1L << 31) / paged::kThreads) return fail(DSPARK_ERR_SHAPE, "%s: %ld workgroups", what, blocks);
   hipStream_t s = static_cast<hipStream_t>(stream);
