@@ -840,8 +840,8 @@ typedef struct dspark_token_logprobs_args { /* every field is 8 bytes */
   int64_t dtype;
   const void* logits;
   int64_t ld, rows, V;
-  const int32_t* tokens;
-  int64_t top;
+  const void* tokens;           /* int32, or tokens_i64: int64 */
+  int64_t tokens_i64, top;
   double temperature;
   float* logprobs;
   float* entropy;

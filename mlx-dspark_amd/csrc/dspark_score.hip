@@ -15,10 +15,11 @@
 //
 // Bound by the bytes of the logits, with the exponential (a quarter of the rate) and about 6 more instructions a value
 // close behind. Many rows: a workgroup of four waves a row; few: up to 64 waves a row, a workgroup each, joined by a second
-// launch. bf16, 900 rows of 128255: 54 us (4.3 TB/s), 74 with the best 5; one row of 151936: 6 us, 18 with the best 20,
-// of which the list takes its time from a wave that has nothing beside it on its SIMD.
+// launch. bf16, 900 rows of 128255: 54 us (4.3 TB/s), 66 with the best 5, 74 with the best 20; one row of 151936: 6 us, 14
+// with the best 20, of which the list takes its time from a wave that has nothing beside it on its SIMD.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dspark_common.h"
 
@@ -40,7 +41,8 @@ struct ScoreArgs {
   int rows, V, top, segments;
   float c;                                     // log2(e) / temperature
   double temperature;
-  const int* tokens;
+  const void* tokens;
+  int tokens64;
   float* given;
   float* entropy;
   int* ids;                                    // [rows][top]
@@ -149,8 +151,8 @@ __device__ __forceinline__ void finish_row(const ScoreArgs& a, long row, Stats s
     return (float)(((double)x - (double)s.m) / a.temperature - log_sum);
   };
   if (lane == 0) {
-    const int t = a.tokens[row];
-    a.given[row] = (unsigned)t < (unsigned)a.V ? log_p(Logit<DT>::get((reinterpret_cast<const T*>(a.x) + row * a.ld)[t])) : -__builtin_inff();
+    const int64_t t = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : (int64_t)static_cast<const int32_t*>(a.tokens)[row];
+    a.given[row] = t >= 0 && t < a.V ? log_p(Logit<DT>::get((reinterpret_cast<const T*>(a.x) + row * a.ld)[t])) : -__builtin_inff();
     a.entropy[row] = none ? 0.f : (float)(entropy > 0. ? entropy : 0.);
   }
   if (lane < a.top) {
@@ -203,16 +205,19 @@ __device__ __forceinline__ List new_list(u64* keys, int top, u64* shared) {
   return List{keys, 0, top, top + top / 2 + 16, 0, shared};
 }
 
-// kPer: values of a lane's step. A wave that has a row's part for itself takes 8: it is alone on its SIMD, and what counts is
-// how many instructions it issues until it is done.
+// Values of a lane's step. A wave that has a row's part for itself is alone on its SIMD, and what counts is how many
+// instructions it issues until it is done: one step for most vocabularies.
+template <int WAVES> constexpr int kPerLane = WAVES == 1 ? 40 : 32;
+
 template <int DT, bool TOP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void score_kernel(const ScoreArgs a) {
   using T = typename Logit<DT>::t;
-  constexpr int kPer = WAVES == 1 ? 8 : 32;
+  constexpr int kPer = kPerLane<WAVES>;
   constexpr int E = 16 / sizeof(T), NL = kPer / E;           // values of a 16-byte load, loads of a step
   constexpr int STEP = 64 * NL;                              // 16-byte chunks of a wave's step
   struct alignas(16) Vec { T v[E]; };
   __shared__ u64 lists[WAVES][TOP ? kList : 1];
+  __shared__ float staged[WAVES][TOP ? kPer * 64 : 1];
   __shared__ u64 least_of_all;
   __shared__ Stats parts[WAVES];
   __shared__ int counts[WAVES];
@@ -316,18 +321,23 @@ __global__ __launch_bounds__(64 * WAVES) void score_kernel(const ScoreArgs a) {
         if (best) best |= key_of(top, 0) & 0xFFFFFFFF00000000ull;
         list.raise_by(best);
       }
-      // Bit i: value i reaches the least key's (NaN counts as -inf). Such values are read again: there are few, and one
-      // copy of the code that lists a value, where 32 would not fit the instruction cache
+      // Bit i: value i reaches the least key's (NaN counts as -inf). They are listed out of LDS, where a lane finds value i:
+      // one copy of the code, where one for every value would not fit the instruction cache
+      using Mask = std::conditional_t<(kPer > 32), u64, u32>;
       const float least_value = needed();
-      const bool nan_too = least_value == -__builtin_inff();
-      u32 mask = 0;
+      Mask mask = 0;
 #pragma unroll
       for (int i = kPer - 1; i >= 0; --i) mask = mask + mask + (x[i] >= least_value ? 1u : 0u);
-      if (nan_too) mask = 0xFFFFFFFFu >> (32 - kPer);
+      if (least_value == -__builtin_inff()) mask = ~Mask(0) >> (8 * sizeof(Mask) - kPer);
+      float* const mine = &staged[wave][lane];
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine[64 * i] = x[i];
+      }
       while (__builtin_amdgcn_ballot_w64(mask != 0)) {
-        const int i = mask ? __builtin_ctz(mask) : 0, at = (int)((long)(cur + 64 * (i / E) + lane) * E + i % E - off);
+        const int i = mask ? __builtin_ctzll(mask) : 0, at = index(i);
         u64 k = 0;
-        if (mask && at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1) k = key_of(Logit<DT>::get(x0[at]), at);
+        if (mask && at >= 0 && at < a.V && cur + 64 * (i / E) + lane < c1) k = key_of(mine[64 * i], at);
         mask &= mask - 1;
         list.push(k);
       }
@@ -391,10 +401,12 @@ __global__ __launch_bounds__(64) void join_scores_kernel(const ScoreArgs a) {
   finish_row<DT>(a, row, join_wave(s, a.c), mine);
 }
 
-// Segments of a row: 1 from 512 rows on, a workgroup each; fewer rows are dealt to 2048 waves, of at least 1024 values
+// Segments of a row: 1 from 512 rows on, a workgroup each; fewer rows are dealt to 2048 waves, of whole steps
 int score_segments(int64_t rows, int64_t V) {
   if (rows >= 512) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + rows - 1) / rows, kMostSegments, V / 1024}));
+  constexpr int64_t step = 64 * kPerLane<1>;
+  const int64_t n = std::min<int64_t>((2048 + rows - 1) / rows, kMostSegments), steps = (V + n * step - 1) / (n * step);
+  return (int)((V + steps * step - 1) / (steps * step));
 }
 
 template <int DT, bool TOP>
@@ -431,6 +443,7 @@ extern "C" int dspark_token_logprobs(const dspark_token_logprobs_args* p, dspark
   if (!need)
     return fail(DSPARK_ERR_SHAPE, "%s: %ld rows (up to 2^20) of %ld logits (up to 2^28), the best %ld (up to %d and all)", what,
                 (long)p->rows, (long)p->V, (long)p->top, kMostTop);
+  if (!aligned(p->tokens, p->tokens_i64 ? 8 : 4)) return fail(DSPARK_ERR_ALIGN, "%s: tokens need the alignment of their type", what);
   if (!(p->temperature >= 1e-30 && p->temperature <= 1e30)) return fail(DSPARK_ERR_ARG, "%s: temperature %g", what, p->temperature);
   const int es = p->dtype == DSPARK_DTYPE_F32 ? 4 : 2;
   if (!aligned(p->logits, es)) return fail(DSPARK_ERR_ALIGN, "%s: logits need the alignment of their type", what);
@@ -446,6 +459,7 @@ extern "C" int dspark_token_logprobs(const dspark_token_logprobs_args* p, dspark
   a.c = (float)(1.44269504088896340736 / p->temperature);
   a.temperature = p->temperature;
   a.tokens = p->tokens;
+  a.tokens64 = p->tokens_i64 != 0;
   a.given = p->logprobs;
   a.entropy = p->entropy;
   a.ids = p->top_tokens;

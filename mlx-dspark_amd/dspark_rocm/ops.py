@@ -1093,7 +1093,7 @@ def token_logprobs_workspace_bytes(rows: int, vocab: int, top: int = 0) -> int:
     return int(_lib.load().dspark_token_logprobs_workspace(rows, vocab, top))
 
 
-_SCORE_ARGS = struct.Struct("=7qd6q")
+_SCORE_ARGS = struct.Struct("=8qd6q")
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, temperature: float = 1.0,
@@ -1118,7 +1118,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
         raise ValueError(f"{what}: logits {list(shape)}, top={top} (up to {MOST_ALTERNATIVES} and the vocabulary)")
     t, _, _ = check_sampler(temperature, 0, 1.0)
     _no_autograd(what, logits)
-    tokens = _ints(what, "tokens", tokens, shape[:-1])
+    wide = tokens.dtype is torch.int64
+    if not (wide or tokens.dtype is torch.int32) or tokens.shape != shape[:-1]:
+        raise ValueError(f"{what}: tokens must be int32 or int64 {list(shape[:-1])}, got {tokens.dtype} {list(tokens.shape)}")
+    tokens = tokens.contiguous()
     if logits.is_neg():
         logits = logits.resolve_neg()
     V = shape[-1]
@@ -1138,7 +1141,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
         elif workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.data_ptr() % 16:
             raise ValueError(f"{what}: workspace: {nbytes} contiguous bytes, aligned to 16, needed")
         _call_on(dev, "dspark_token_logprobs",
-                 _SCORE_ARGS.pack(dt, x.data_ptr(), ld, rows, V, tokens.data_ptr(), top, t, given.data_ptr(), entropy.data_ptr(),
+                 _SCORE_ARGS.pack(dt, x.data_ptr(), ld, rows, V, tokens.data_ptr(), wide, top, t, given.data_ptr(), entropy.data_ptr(),
                                   ids.data_ptr(), best.data_ptr(), workspace.data_ptr(), workspace.nbytes))
     return given, entropy, ids, best
 
@@ -1545,8 +1548,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     elif q_out is not None:
         raise ValueError(f"{what}: q_out without q")
     if T and seqs[4] and seqs[5] and pool and Hk:
-        for t in (k, v):                # what is written shares no place with what is read, k and v may
-            _distinct(what, t.data_ptr(), *(f for f in (*pages[::7], *pages[4::7]) if f), *((q_out.data_ptr(),) if Hq else ()))
+        # what is written shares no place with what is read; k and v may
+        written = [pages[0], pages[7]] + ([pages[4], pages[11]] if codes else []) + ([q_out.data_ptr()] if Hq else [])
+        places = {*written}
+        if len(places) < len(written) or k.data_ptr() in places or v.data_ptr() in places:
+            raise ValueError(f"{what}: the same rows given twice")
         _call_on(dev, "dspark_paged_append",
                  _APPEND_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, dims, bool(interleaved), at_f, scale, at_p, p64, p_st, *q_fields,
                                    k.data_ptr(), *k_st, v.data_ptr(), *v_st, *pages, *seqs))

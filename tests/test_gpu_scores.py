@@ -106,6 +106,16 @@ def test_infinite_and_nan_logits(dev):
             check(x, tokens, ops.token_logprobs(x, tokens, top=9), 9)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [2559, 2560, 2561, 5121, 163839, 163841])
+def test_rows_that_end_where_a_step_does(dev, V, dtype):
+    """A wave of a split row takes 2560 values a step; rows at every offset from 16 bytes reach one load further."""
+    g = torch.Generator().manual_seed(V)
+    wide = logits(g, 2, V + 9, dtype, dev)
+    for off in (0, 1, 7):
+        run(wide[:, off:off + V], 20, seed=off)
+
+
 def test_views_streams_and_workspaces(dev):
     from dspark_rocm import ops
 
