@@ -245,11 +245,12 @@ def test_score_fields(host):
     x = torch.zeros(2, 3, 10, dtype=torch.float16)[..., :9]
     g, h, i, b = ops.token_logprobs(x[:, :2], torch.zeros(2, 2, dtype=torch.int64), top=4, temperature=0.5)
     name, f = host.pop()
-    assert name == "dspark_token_logprobs" and f[0] == 1 and f[3:5] == (4, 9) and f[6] == 4
-    assert f[8:12] == (g.data_ptr(), h.data_ptr(), i.data_ptr(), b.data_ptr()) and i.shape == b.shape == (2, 2, 4)
+    assert name == "dspark_token_logprobs" and f[0] == 1 and f[3:5] == (4, 9) and f[6:8] == (1, 4)
+    assert f[9:13] == (g.data_ptr(), h.data_ptr(), i.data_ptr(), b.data_ptr()) and i.shape == b.shape == (2, 2, 4)
     y = torch.zeros(5, 9)
     ops.token_logprobs(y, ids(0, 1, 2, 3, 4))
-    assert host.pop()[1][1:5] == (y.data_ptr(), 9, 5, 9)
+    f = host.pop()[1]
+    assert f[1:5] == (y.data_ptr(), 9, 5, 9) and f[6] == 0
     ops.token_logprobs(torch._neg_view(y), ids(0, 1, 2, 3, 4))
     assert host.pop()[1][1] != y.data_ptr()
     assert ops.token_logprobs(y[:0], ids(), top=3)[2].shape == (0, 3) and not host
