@@ -37,19 +37,29 @@ struct Seqs {
 };
 
 struct Seq {
-  int start, n, len;             // first row, rows, positions with them; n = 0 where they do not fit the call
+  int start, n, len;             // first row, rows, positions with them that the table has; n = 0 where they do not fit
+  int full;                      // positions as given: the rows' own count from there
 };
 
 __device__ __forceinline__ Seq sequence(const Seqs& s, int b) {
   const int s0 = s.starts[b], s1 = s.starts[b + 1], len = s.lens[b];
   const bool ok = s0 >= 0 && s1 > s0 && s1 <= s.T && len > 0;
   const long most = (long)s.width << s.log2P;
-  return Seq{s0, ok ? s1 - s0 : 0, (int)((long)len < most ? (long)len : most)};
+  return Seq{s0, ok ? s1 - s0 : 0, (int)((long)len < most ? (long)len : most), len};
 }
 
-// A sequence whose positions go past its table keeps those that the table has: its rows' positions count from the
-// length it was given with.
-__device__ __forceinline__ long first_position(const Seqs& s, int b, const Seq& q) { return (long)s.lens[b] - q.n; }
+__device__ __forceinline__ long first_position(const Seq& q) { return (long)q.full - q.n; }
+
+// Every row of the call is a sequence's: what a step usually is
+__device__ __forceinline__ bool all_rows_taken(const Seqs& s) {
+  const int lane = __lane_id();
+  bool open = s.starts[0] != 0 || s.starts[s.B] != s.T;
+  for (int b = lane; b < s.B; b += 64) {
+    const int s0 = s.starts[b], s1 = s.starts[b + 1];
+    open |= s1 < s0 || (s1 > s0 && s.lens[b] <= 0);
+  }
+  return !__builtin_amdgcn_ballot_w64(open);
+}
 
 // The page of a sequence's position, -1 where there is none
 __device__ __forceinline__ int page_of(const Seqs& s, int b, long pos) {

@@ -232,12 +232,12 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, u16* stash, u3
   const auto count = [&](int i) {
     const Seq q = sequence(a.s, i);
     if (!q.n) return 0u;
-    const long p0 = first_position(a.s, i, q), p1 = p0 + q.n;      // of the rows, their end
+    const long p0 = first_position(q), p1 = p0 + q.n;      // of the rows, their end
     return p1 <= 0 ? 0u : (u32)(((p1 - 1) >> a.s.log2P) - ((p0 < 0 ? 0 : p0) >> a.s.log2P) + 1);
   };
   if (!locate((u32)((item >> 1) / a.Hk), a.s.B, count, b, j)) return;
   const Seq q = sequence(a.s, b);
-  const long p0 = first_position(a.s, b, q), base = (((p0 < 0 ? 0 : p0) >> a.s.log2P) + j) << a.s.log2P;
+  const long p0 = first_position(q), base = (((p0 < 0 ? 0 : p0) >> a.s.log2P) + j) << a.s.log2P;
   const int id = page_of(a.s, b, base);
   if (id < 0) return;
   const int lo = (int)(p0 > base ? p0 - base : 0), hi = (int)(p0 + q.n < base + a.s.P ? p0 + q.n - base : a.s.P);

@@ -58,43 +58,60 @@ struct AttnArgs {
 
 // A sequence's share of the work list
 struct Work {
-  int start, n, len;                                // first row, rows, keys
+  int start, n, len, full;                          // first row, rows, keys that the table has, and as given
   int rows, groups, tiles;                          // rows and row groups of a KV head, units along the keys
 };
 
 template <int RT>
 __device__ __forceinline__ Work work_of(const AttnArgs& a, int b) {
   const Seq q = sequence(a.s, b);
-  Work w{q.start, q.n, q.len, q.n * a.gqa, 0, 0};
+  Work w{q.start, q.n, q.len, q.full, q.n * a.gqa, 0, 0};
   if (w.rows > a.rows_up_to || q.n == 0) w.rows = 0;
   w.groups = (w.rows + 16 * RT - 1) / (16 * RT);
   w.tiles = a.whole ? 1 : (q.len + kUnit - 1) / kUnit;
   return w;
 }
 
-template <int RT>
-__device__ __forceinline__ u32 units_of(const AttnArgs& a, int b) {
-  const Work w = work_of<RT>(a, b);
+__device__ __forceinline__ Work lane_work(const Work& w, int l) {
+  auto at = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+  return Work{at(w.start), at(w.n), at(w.len), at(w.full), at(w.rows), at(w.groups), at(w.tiles)};
+}
+
+__device__ __forceinline__ u32 units_of(const AttnArgs& a, const Work& w) {
   const unsigned long long n = (unsigned long long)a.Hk * (unsigned)w.groups * (unsigned)w.tiles;
   return n > kMostUnits ? kMostUnits + 1 : (u32)n;
 }
 
-// Units of all sequences, and of those before `upto`; none where they are more than a call may have (the entry point
-// checks that: only sequences that share their rows come to that here)
+// The work of all sequences: that of the first 64 is looked up once, a lane each
 template <int RT>
-__device__ __forceinline__ int all_units(const AttnArgs& a, int upto, int* before) {
-  const int lane = __lane_id();
-  u32 sum = 0, first = 0;
-  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-    const u32 n = b0 + lane < a.s.B ? units_of<RT>(a, b0 + lane) : 0u;
-    sum = __builtin_elementwise_add_sat(sum, n);
-    if (b0 + lane < upto) first += n;
+struct Works {
+  const AttnArgs& a;
+  Work first;
+
+  __device__ __forceinline__ explicit Works(const AttnArgs& args) : a(args), first(work_of<RT>(args, min((int)__lane_id(), args.s.B - 1))) {}
+  __device__ __forceinline__ u32 units(int b) const {        // of sequence b = 64 i + lane
+    return b >= a.s.B ? 0u : b < 64 ? units_of(a, first) : units_of(a, work_of<RT>(a, b));
   }
-  const u32 all = (u32)__builtin_amdgcn_readlane((int)wave_scan(sum), 63);
-  if (all > kMostUnits) return 0;
-  if (before) *before = __builtin_amdgcn_readlane((int)wave_scan(first), 63);
-  return (int)all;
-}
+  __device__ __forceinline__ Work at(int b) const {          // b: the wave's
+    if (b < 64) return lane_work(first, b);
+    return lane_work(work_of<RT>(a, b), 0);
+  }
+  // Units of all sequences, and of those before `upto`; none where they are more than a call may have (the entry point
+  // checks that: only sequences that share their rows come to that here)
+  __device__ __forceinline__ int all(int upto, int* before) const {
+    const int lane = __lane_id();
+    u32 sum = 0, some = 0;
+    for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+      const u32 n = units(b0 + lane);
+      sum = __builtin_elementwise_add_sat(sum, n);
+      if (b0 + lane < upto) some += n;
+    }
+    const u32 total = (u32)__builtin_amdgcn_readlane((int)wave_scan(sum), 63);
+    if (total > kMostUnits) return 0;
+    if (before) *before = __builtin_amdgcn_readlane((int)wave_scan(some), 63);
+    return (int)total;
+  }
+};
 
 __device__ __forceinline__ int run_of(const AttnArgs& a, int units, int workgroups) {
   const int even = (units + workgroups - 1) / workgroups;
@@ -158,10 +175,11 @@ __device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int h
 }
 
 // Keys that row i of a sequence's n sees
-__device__ __forceinline__ int keys_seen(const AttnArgs& a, int b, int n, int len, int i) {
-  if (!a.causal) return len;
-  const long k = (long)a.s.lens[b] - n + i + 1;
-  return (int)(k < 0 ? 0 : k < len ? k : len);
+template <class W>
+__device__ __forceinline__ int keys_seen(const AttnArgs& a, const W& w, int i) {
+  if (!a.causal) return w.len;
+  const int k = w.full - w.n + i + 1;                        // full > 0
+  return k < 0 ? 0 : k < w.len ? k : w.len;
 }
 
 // 16 codes as 16 values of T
@@ -203,6 +221,7 @@ template <int D>
 __device__ __forceinline__ void clear_rows(const AttnArgs& a) {
   constexpr int CH = D / 8;
   const int lane = __lane_id();
+  if (all_rows_taken(a.s)) return;
   for (int t = blockIdx.x; t < a.s.T; t += gridDim.x) {
     bool has = false;
     for (int b0 = 0; b0 < a.s.B; b0 += 64) {
@@ -229,14 +248,14 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
   u16* const vt = tiles[wave];
 
   if (a.clear) clear_rows<D>(a);
-  const int units = all_units<RT>(a, 0, nullptr), run = a.whole ? 1 : run_of(a, units, gridDim.x);
+  const Works<RT> works(a);
+  const int units = works.all(0, nullptr), run = a.whole ? 1 : run_of(a, units, gridDim.x);
   if ((long)blockIdx.x * run >= units) return;
   int u = blockIdx.x * run;
   const int u_end = min(u + run, units);
   int b, local;
-  if (!locate((u32)u, a.s.B, [&](int i) { return units_of<RT>(a, i); }, b, local)) return;
-  Work w = work_of<RT>(a, b);
-  w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+  if (!locate((u32)u, a.s.B, [&](int i) { return works.units(i); }, b, local)) return;
+  Work w = works.at(b);
 
   while (u < u_end) {
     // the KV head and row group, and the units [t0, t1) of it
@@ -250,13 +269,13 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = min(r0 + 16 * rt + c16, w.rows - 1), i = r / a.gqa;
-      lim[rt] = keys_seen(a, b, w.n, w.len, i);
+      lim[rt] = keys_seen(a, w, i);
       const u16* qp = a.q + (w.start + i) * a.qrow + (h * a.gqa + r - i * a.gqa) * a.qhead;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         qf[rt][c] = CODES ? ldg128(qp + 64 * (c >> 1) + 16 * q4 + 8 * (c & 1)) : ldg128(qp + 32 * c + 8 * q4);
     }
-    const int all_see = uniform(keys_seen(a, b, w.n, w.len, min(r0, w.rows - 1) / a.gqa));
+    const int all_see = uniform(keys_seen(a, w, min(r0, w.rows - 1) / a.gqa));
 
     // page ids (and scales) of 64 pages, a lane each
     const int* const row = a.s.table + b * a.s.ldt;
@@ -489,7 +508,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
       for (int r = wave; r < ROWS; r += kWaves)
         if (again[r]) {
           const int i = (r0 + r) / a.gqa;
-          plain_row<T, D, CODES>(a, b, w.start + i, h * a.gqa + r0 + r - i * a.gqa, keys_seen(a, b, w.n, w.len, i));
+          plain_row<T, D, CODES>(a, b, w.start + i, h * a.gqa + r0 + r - i * a.gqa, keys_seen(a, w, i));
         }
     }
     __syncthreads();
@@ -500,8 +519,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
       local = 0;
       do {
         ++b;
-        w = work_of<RT>(a, b);
-        w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+        w = works.at(b);
       } while (w.rows == 0 && b < a.s.B - 1);
       if (w.rows == 0) return;
     }
@@ -510,7 +528,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
 
 // Parts of a row, joined by a wave: out = sum_z 2^(m_z - m) o_z / sum_z 2^(m_z - m) l_z in the order of the keys. `part(z)`:
 // where part z's row stands among the outputs; its maximum (times `c` in the exponent) and sum at `stat(z)` and `stat(z)` +
-// `sums`. A lane looks at a part's maximum and sum, then N parts' outputs are on their way at a time.
+// `sums`. A lane looks at a part's maximum and sum, while N parts' outputs are on their way.
 template <int C>
 struct Joined {
   float v[C];                    // unnormalised columns of the lane
@@ -522,27 +540,35 @@ __device__ __forceinline__ Joined<D / 64> join_parts(const float* o, const float
   constexpr int C = D / 64;
   typedef float cols_t __attribute__((ext_vector_type(C)));
   const int lane = __lane_id();
+  cols_t x[N];
+  auto load = [&](int z) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      x[k] = *reinterpret_cast<const cols_t*>(o + part(min(z + k * step, parts - 1)) * D + C * lane);
+  };
+  load(first);
+  float ms = stats[stat(min(lane, parts - 1))], ls = stats[stat(min(lane, parts - 1)) + sums];
   Joined<C> r;
 #pragma unroll
   for (int i = 0; i < C; ++i) r.v[i] = 0.f;
-  r.m = kLowest;
-  for (int z = lane; z < parts; z += 64) r.m = fmaxf(r.m, stats[stat(z)]);
+  r.m = ms;
+  for (int z = lane + 64; z < parts; z += 64) r.m = fmaxf(r.m, stats[stat(z)]);
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) r.m = fmaxf(r.m, shfl_xor(r.m, x));
+  for (int y = 1; y < 64; y *= 2) r.m = fmaxf(r.m, shfl_xor(r.m, y));
   r.l = 0.f;
   for (int z0 = 0; z0 < parts; z0 += 64) {
-    const int z = min(z0 + lane, parts - 1);
-    const float f = z0 + lane < parts ? __builtin_amdgcn_exp2f((stats[stat(z)] - r.m) * c) : 0.f;
-    r.l += f * stats[stat(z) + sums];
+    if (z0) {
+      const int z = min(z0 + lane, parts - 1);
+      ms = stats[stat(z)], ls = stats[stat(z) + sums];
+    }
+    const float f = z0 + lane < parts ? __builtin_amdgcn_exp2f((ms - r.m) * c) : 0.f;
+    r.l += f * ls;
     const int n = min(64, parts - z0);
     for (int j = first; j < n; j += step * N) {
-      cols_t x[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        x[k] = *reinterpret_cast<const cols_t*>(o + part(z0 + min(j + k * step, n - 1)) * D + C * lane);
+      if (z0 + j != first) load(z0 + j);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float fk = j + k * step < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(j + k * step, n - 1))) : 0.f;
+        const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(j + k * step, n - 1)));
         // (a part of weight 0 may hold what is not finite: it would have to count, were it there)
 #pragma unroll
         for (int i = 0; i < C; ++i) r.v[i] = j + k * step < n ? __builtin_fmaf(fk, x[k][i], r.v[i]) : r.v[i];
@@ -550,7 +576,7 @@ __device__ __forceinline__ Joined<D / 64> join_parts(const float* o, const float
     }
   }
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) r.l += shfl_xor(r.l, x);
+  for (int y = 1; y < 64; y *= 2) r.l += shfl_xor(r.l, y);
   return r;
 }
 
@@ -580,11 +606,11 @@ __global__ __launch_bounds__(kAttnThreads) void join_kernel(const AttnArgs a, in
   __shared__ float sm[kWaves][D];
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
-  Work w = work_of<RT>(a, b);
-  w = Work{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.groups), uniform(w.tiles)};
+  const Works<RT> works(a);
+  const Work w = works.at(b);
   if ((int)blockIdx.y >= w.rows) return;
   int before = 0;
-  const int units = all_units<RT>(a, b, &before);
+  const int units = works.all(b, &before);
   if (!units) return;
   const int run = run_of(a, units, workgroups);
   for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
@@ -602,7 +628,7 @@ __global__ __launch_bounds__(kAttnThreads) void join_kernel(const AttnArgs a, in
 #pragma unroll
       for (int i = 0; i < C; ++i) x.v[i] = (sm[0][C * lane + i] + sm[1][C * lane + i]) + (sm[2][C * lane + i] + sm[3][C * lane + i]);
       const int i = r / a.gqa;
-      put_row<T, D, CODES>(a, x.v, x.l, b, w.start + i, h * a.gqa + r - i * a.gqa, keys_seen(a, b, w.n, w.len, i));
+      put_row<T, D, CODES>(a, x.v, x.l, b, w.start + i, h * a.gqa + r - i * a.gqa, keys_seen(a, w, i));
     }
     __syncthreads();
   }

@@ -48,62 +48,100 @@ struct TileArgs {
 };
 
 struct TileWork {
-  int start, n, len, rows, row_tiles, key_tiles;
+  int start, n, len, full, rows, row_tiles, key_tiles;
 };
 
 __device__ __forceinline__ TileWork tile_work(const AttnArgs& a, int b) {
   const Seq q = sequence(a.s, b);
-  TileWork w{q.start, q.n, q.len, q.n * a.gqa, 0, (q.len + kTileKeys - 1) / kTileKeys};
+  TileWork w{q.start, q.n, q.len, q.full, q.n * a.gqa, 0, (q.len + kTileKeys - 1) / kTileKeys};
   if (w.rows <= a.rows_up_to) w.rows = 0;
   w.row_tiles = (w.rows + kTileRows - 1) / kTileRows;
   return w;
 }
 
-// Key tiles that a part may have before it is split: 1.5 times the average share of a slot
+// The list of items: how many key tiles a part may have, and what every sequence has. That of the first 64 is looked up
+// once, a lane each.
 template <int D>
-__device__ __forceinline__ int target_tiles(const AttnArgs& a) {
-  const int lane = __lane_id();
-  float sum = 0.f;                // a rule, not a count: rounding does not matter
-  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-    if (b0 + lane >= a.s.B) continue;
-    const TileWork w = tile_work(a, b0 + lane);
-    sum += (float)w.row_tiles * (float)w.key_tiles;
-  }
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) sum += shfl_xor(sum, x);
-  const float t = 1.5f * sum * (float)a.Hk / kSlots<D>;
-  return uniform(t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1);
-}
+struct TileList {
+  const AttnArgs& a;
+  TileWork first;
+  int target;                     // key tiles that a part may have before it is split: 1.5 times the average share of a slot
 
-__device__ __forceinline__ int parts_of(const TileWork& w, int target) { return (w.key_tiles + target - 1) / target; }
-
-// Items of the list (and of the split ones among them) of a sequence
-__device__ __forceinline__ u32 items_of(const AttnArgs& a, int b, int target) {
-  const TileWork w = tile_work(a, b);
-  const unsigned long long n = (unsigned long long)a.Hk * (unsigned)w.row_tiles * (unsigned)parts_of(w, target);
-  return n > kMostUnits ? kMostUnits + 1 : (u32)n;
-}
-
-// Parts before sequence b among the split sequences
-__device__ __forceinline__ int parts_before(const AttnArgs& a, int b, int target) {
-  const int lane = __lane_id();
-  u32 n = 0;
-  for (int b0 = 0; b0 < b; b0 += 64)
-    if (b0 + lane < b) {
-      const TileWork w = tile_work(a, b0 + lane);
-      if (parts_of(w, target) > 1) n = __builtin_elementwise_add_sat(n, items_of(a, b0 + lane, target));
+  __device__ __forceinline__ explicit TileList(const AttnArgs& args) : a(args), first(tile_work(args, min((int)__lane_id(), args.s.B - 1))) {
+    const int lane = __lane_id();
+    float sum = 0.f;              // a rule, not a count: rounding does not matter
+    for (int b = lane; b < a.s.B; b += 64) {
+      const TileWork w = lanes(b);
+      sum += (float)w.row_tiles * (float)w.key_tiles;
     }
-  const u32 all = (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
-  return (int)(all > (u32)kParts ? (u32)kParts : all);
-}
-
-__device__ __forceinline__ u32 items_of_all(const AttnArgs& a, int target) {
-  const int lane = __lane_id();
-  u32 n = 0;
-  for (int b0 = 0; b0 < a.s.B; b0 += 64)
-    if (b0 + lane < a.s.B) n = __builtin_elementwise_add_sat(n, items_of(a, b0 + lane, target));
-  return (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
-}
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) sum += shfl_xor(sum, x);
+    const float t = 1.5f * sum * (float)a.Hk / kSlots<D>;
+    target = uniform(t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1);
+  }
+  __device__ __forceinline__ TileWork lanes(int b) const {   // of sequence b = 64 i + lane
+    if (b < 64) return first;
+    return tile_work(a, min(b, a.s.B - 1));
+  }
+  __device__ __forceinline__ TileWork at(int b) const {      // b: the wave's
+    const TileWork w = b < 64 ? first : tile_work(a, b);
+    const int l = b < 64 ? b : 0;
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+    return TileWork{of(w.start), of(w.n), of(w.len), of(w.full), of(w.rows), of(w.row_tiles), of(w.key_tiles)};
+  }
+  __device__ __forceinline__ int parts(const TileWork& w) const { return (w.key_tiles + target - 1) / target; }
+  // Items of the list (and of the split ones among them) of a sequence
+  __device__ __forceinline__ u32 items(int b) const {
+    if (b >= a.s.B) return 0;
+    const TileWork w = lanes(b);
+    const unsigned long long n = (unsigned long long)a.Hk * (unsigned)w.row_tiles * (unsigned)parts(w);
+    return n > kMostUnits ? kMostUnits + 1 : (u32)n;
+  }
+  __device__ __forceinline__ u32 split_items(int b) const { return b < a.s.B && parts(lanes(b)) > 1 ? items(b) : 0u; }
+  __device__ __forceinline__ u32 all() const {
+    u32 n = 0;
+    for (int b0 = 0; b0 < a.s.B; b0 += 64) n = __builtin_elementwise_add_sat(n, items(b0 + (int)__lane_id()));
+    return (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+  }
+  // Parts before sequence b among the split sequences
+  __device__ __forceinline__ int parts_before(int b) const {
+    const int lane = __lane_id();
+    u32 n = 0;
+    for (int b0 = 0; b0 < b; b0 += 64)
+      if (b0 + lane < b) n = __builtin_elementwise_add_sat(n, split_items(b0 + lane));
+    const u32 sum = (u32)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+    return (int)(sum > (u32)kParts ? (u32)kParts : sum);
+  }
+  // The sequence of the item, and its place among the sequence's, where sequences (64 at a time) stand in the order of
+  // the keys that their items have, most first
+  __device__ __forceinline__ bool locate(u32 item, int& b, int& local) const {
+    const int lane = __lane_id();
+    for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+      const int n = min(64, a.s.B - b0);
+      const u32 count = items(b0 + lane);
+      const TileWork w = lanes(b0 + lane);
+      const int keys = lane < n ? w.key_tiles / max(parts(w), 1) : -1;
+      int rank = 0;
+      for (int j = 0; j < n; ++j) {
+        const int k = __builtin_amdgcn_readlane(keys, j);
+        rank += k > keys || (k == keys && j < lane) ? 1 : 0;
+      }
+      rank = lane < n ? rank : lane;
+      const u32 c = (u32)__builtin_amdgcn_ds_permute(rank << 2, (int)count);
+      const int from = __builtin_amdgcn_ds_permute(rank << 2, lane);
+      const u32 upto = wave_scan(c);
+      const u32 sum = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+      if (item < sum) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > item));
+        b = uniform(b0 + __builtin_amdgcn_readlane(from, at));
+        local = uniform((int)(item - (u32)__builtin_amdgcn_readlane((int)(upto - c), at)));
+        return true;
+      }
+      item -= sum;
+    }
+    return false;
+  }
+};
 
 // 16 bytes a lane from `base` + `off` to LDS, the wave's 1 KB from `to` on. In assembly, and waited for by hand: the
 // compiler takes every later LDS read for one of these bytes and would have it wait for the copies just begun.
@@ -116,39 +154,6 @@ __device__ __forceinline__ void copy_to_lds(const char* base, u32 off, u16* to) 
 }
 
 constexpr int kNarrow = 10;       // what codes are multiplied by as fp16: 2^10
-
-// The sequence of the item, and its place among the sequence's, where sequences (64 at a time) stand in the order of
-// the keys that their items have, most first
-__device__ __forceinline__ bool locate_longest(const AttnArgs& a, u32 item, int target, int& b, int& local) {
-  const int lane = __lane_id();
-  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-    const int n = min(64, a.s.B - b0);
-    const u32 count = lane < n ? items_of(a, b0 + lane, target) : 0u;
-    int keys = -1;
-    if (lane < n) {
-      const TileWork w = tile_work(a, b0 + lane);
-      keys = w.key_tiles / max(parts_of(w, target), 1);
-    }
-    int rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const int k = __builtin_amdgcn_readlane(keys, j);
-      rank += k > keys || (k == keys && j < lane) ? 1 : 0;
-    }
-    rank = lane < n ? rank : lane;
-    const u32 c = (u32)__builtin_amdgcn_ds_permute(rank << 2, (int)count);
-    const int from = __builtin_amdgcn_ds_permute(rank << 2, lane);
-    const u32 upto = wave_scan(c);
-    const u32 all = (u32)__builtin_amdgcn_readlane((int)upto, 63);
-    if (item < all) {
-      const int first = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > item));
-      b = uniform(b0 + __builtin_amdgcn_readlane(from, first));
-      local = uniform((int)(item - (u32)__builtin_amdgcn_readlane((int)(upto - c), first)));
-      return true;
-    }
-    item -= all;
-  }
-  return false;
-}
 
 // Eight probabilities as fp16
 __device__ __forceinline__ u32x4_t one_piece(const f32x16_t& p, int r0) {
@@ -201,8 +206,8 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15;
 
-  const int target = target_tiles<D>(a);
-  const u32 all = items_of_all(a, target);
+  const TileList<D> list(a);
+  const u32 all = list.all();
   if (all > kMostUnits) return true;
   // Of the 512 that start together, two a CU, the second 256 in turned order: a long causal tile shares its CU with a
   // short one (2048 rows behind 2953 keys: 193.4 -> 191.6 us)
@@ -211,19 +216,18 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   const u32 item = turned * 8 + (blockIdx.x & 7);
   if (nth >= rounds || item >= all) return true;
   int b, local;
-  if (!locate_longest(a, item, target, b, local)) return true;
-  TileWork w = tile_work(a, b);
-  w = TileWork{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.row_tiles), uniform(w.key_tiles)};
-  const int parts = parts_of(w, target);
+  if (!list.locate(item, b, local)) return true;
+  const TileWork w = list.at(b);
+  const int parts = list.parts(w);
   const int z = local % parts, h = local / parts % a.Hk, tile = w.row_tiles - 1 - local / (parts * a.Hk);
 
   const int r0 = tile * kTileRows, rw = r0 + 32 * wave;
   const int r = min(rw + l31, w.rows - 1), tok = r / a.gqa, head = h * a.gqa + (r - tok * a.gqa);
   // keys that this lane's row sees, the wave's least and most, the workgroup's most
-  const int lim = keys_seen(a, b, w.n, w.len, tok);
-  const int wmin = uniform(keys_seen(a, b, w.n, w.len, min(rw, w.rows - 1) / a.gqa));
-  const int wmax = uniform(keys_seen(a, b, w.n, w.len, min(rw + 31, w.rows - 1) / a.gqa));
-  const int bmax = uniform(keys_seen(a, b, w.n, w.len, min(r0 + kTileRows - 1, w.rows - 1) / a.gqa));
+  const int lim = keys_seen(a, w, tok);
+  const int wmin = uniform(keys_seen(a, w, min(rw, w.rows - 1) / a.gqa));
+  const int wmax = uniform(keys_seen(a, w, min(rw + 31, w.rows - 1) / a.gqa));
+  const int bmax = uniform(keys_seen(a, w, min(r0 + kTileRows - 1, w.rows - 1) / a.gqa));
   const int ntile = (bmax + KT - 1) / KT;
   const int t0 = (int)((long)ntile * z / parts), t1 = (int)((long)ntile * (z + 1) / parts);
 
@@ -477,7 +481,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   l += shfl_xor(l, 32);
   const bool own = rw + l31 < w.rows;
   if (parts > 1) {
-    const int part = parts_before(a, b, target) + local;
+    const int part = TileList<D>(a).parts_before(b) + local;      // (kept from the start, the list costs registers)
     if (part >= kParts || !own) return true;
     const long pr = (long)part * kTileRows + 32 * wave + l31;
     if (half == 0) {
@@ -513,7 +517,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   __threadfence_block();
   for (u32 rows = (u32)bad | (u32)(bad >> 32); rows; rows &= rows - 1) {
     const int i = rw + __builtin_ctz(rows), ti = i / a.gqa;
-    plain_row<T, D, CODES>(a, b, w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, b, w.n, w.len, ti));
+    plain_row<T, D, CODES>(a, b, w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, w, ti));
   }
   return true;
 }
@@ -536,28 +540,33 @@ template <class T, int D, bool CODES>
 __global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs ta) {
   constexpr int C = D / 64;
   const AttnArgs& a = ta.a;
-  const int wave = uniform((int)(threadIdx.x >> 6));
-  const int target = target_tiles<D>(a);
-  if (items_of_all(a, target) > kMostUnits) return;
-  int base = 0;                   // parts before sequence b
-  for (int b = 0; b < a.s.B && base < kParts; ++b) {
-    TileWork w = tile_work(a, b);
-    w = TileWork{uniform(w.start), uniform(w.n), uniform(w.len), uniform(w.rows), uniform(w.row_tiles), uniform(w.key_tiles)};
-    const int parts = parts_of(w, target);
-    if (w.rows == 0 || parts == 1) continue;
-    const int count = a.Hk * w.row_tiles * parts;
-    if (base + count > kParts) return;
-    for (long x = (long)blockIdx.x * kWaves + wave; x < (long)a.Hk * w.rows; x += (long)gridDim.x * kWaves) {
-      const int h = (int)(x / w.rows), r = (int)(x - (long)h * w.rows);
-      const int tile = r / kTileRows, first = base + ((w.row_tiles - 1 - tile) * a.Hk + h) * parts;
-      const int at = r - tile * kTileRows;
-      const Joined<C> v = join_parts<D, 8>(ta.opart, ta.mpart, 1, 1.f, parts, 0, 1,
+  const int lane = __lane_id(), wave = uniform((int)(threadIdx.x >> 6));
+  const TileList<D> list(a);
+  if (list.all() > kMostUnits) return;
+  int base = 0;                   // parts before sequence b0
+  for (int b0 = 0; b0 < a.s.B && base < kParts; b0 += 64) {
+    // a lane has a sequence's parts and rows, and those before
+    const TileWork w = list.lanes(b0 + lane);
+    const u32 count = list.split_items(b0 + lane), rows = count ? (u32)a.Hk * (u32)w.rows : 0u;
+    const u32 upto = wave_scan(count), rows_upto = wave_scan(rows);
+    const u32 all = (u32)__builtin_amdgcn_readlane((int)rows_upto, 63);
+    for (u32 x = blockIdx.x * kWaves + wave; x < all; x += gridDim.x * kWaves) {
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(rows_upto > x)), b = b0 + l;
+      auto of = [&](u32 y) { return __builtin_amdgcn_readlane((int)y, l); };
+      const long before = (long)base + (u32)of(upto - count);
+      if (before + (u32)of(count) > kParts) break;
+      const TileWork v = TileWork{of(w.start), of(w.n), of(w.len), of(w.full), of(w.rows), of(w.row_tiles), of(w.key_tiles)};
+      const int parts = list.parts(v), i = (int)(x - (u32)of(rows_upto - rows)), h = i / v.rows, r = i - h * v.rows;
+      const int tile = r / kTileRows, at = r - tile * kTileRows;
+      const int first = (int)before + ((v.row_tiles - 1 - tile) * a.Hk + h) * parts;
+      const Joined<C> y = join_parts<D, 8>(ta.opart, ta.mpart, 1, 1.f, parts, 0, 1,
                                            [&](int z) { return (long)(first + z) * kTileRows + at; },
                                            [&](int z) { return 2 * ((long)(first + z) * kTileRows + at); });
       const int tok = r / a.gqa;
-      put_row<T, D, CODES>(a, v.v, v.l, b, w.start + tok, h * a.gqa + r - tok * a.gqa, keys_seen(a, b, w.n, w.len, tok));
+      put_row<T, D, CODES>(a, y.v, y.l, b, v.start + tok, h * a.gqa + r - tok * a.gqa, keys_seen(a, v, tok));
     }
-    base += count;
+    const u32 sum = (u32)__builtin_amdgcn_readlane((int)upto, 63);
+    base = sum > (u32)(kParts - base) ? kParts : base + (int)sum;
   }
 }
 
