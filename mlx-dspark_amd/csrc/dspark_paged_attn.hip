@@ -15,19 +15,22 @@ struct Plan {
   size_t part_floats, tile_floats;
 };
 
-Plan make_plan(long B, long Hq, long Hk, long D, long T, long max_rows, long max_len) {
+Plan make_plan(long B, long Hq, long Hk, long D, long T, long max_rows, long max_len, bool codes) {
   Plan p{};
   const long gqa = Hq / Hk, rows = std::min(T, max_rows) * gqa;
   const bool tiles_too = rows > (D == 256 ? 32 : 64);
-  // Beside prompt chunks the few-rows kernel has decoded tokens only: one row tile, and what is more goes to the other
-  p.rows_up_to = tiles_too ? 16 : 1 << 30;
+  // Beside prompt chunks the few-rows kernel has decoded tokens only: one row tile, and what is more goes to the other.
+  // Pages of the model's type up to head dim 128: both are bound by the bytes, and the one launch takes all (32 / 8 heads of
+  // 128, a chunk of 512 rows and 31 tokens behind 100 to 8000: 182 -> 168 us, a chunk of 256 and 127 tokens 181 -> 150; a
+  // chunk of 100 and three behind 30000 122 -> 129). 8-bit pages and head dim 256 lose: 137 -> 155 us, 236 -> 252.
+  const bool one_launch = B == 1 || (!codes && D <= 128);
+  p.rows_up_to = !tiles_too ? 1 << 30 : one_launch ? 0 : 16;
   p.rt = tiles_too || rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4;
   if (tiles_too) {
-    if (B == 1) p.rows_up_to = 0;                // one sequence: the one launch takes it as it is
     const long long_ones = std::min(B, T * gqa / (p.rows_up_to + 1) + 1);
     p.items = (unsigned)(((T * gqa / kTileRows + long_ones) * Hk + kParts + 7) / 8 * 8);
     p.tile_floats = (size_t)kParts * kTileRows * (D + 2);
-    if (B == 1) return p;
+    if (one_launch) return p;
   }
   const long tiles = (max_len + kUnit - 1) / kUnit, height = 16 * p.rt;
   const long groups = T * gqa / height + std::min(B, T);                // of all sequences, at most
@@ -63,8 +66,12 @@ using namespace dspark;
 extern "C" size_t dspark_paged_attention_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t rows, int64_t max_rows,
                                                    int64_t max_len) {
   if (paged::check(B, Hq, Hk, D, rows, max_rows, max_len)) return 0;
-  const paged::Plan p = paged::make_plan(B, Hq, Hk, D, rows, max_rows, max_len);
-  return std::max<size_t>(std::max(p.part_floats, p.tile_floats) * sizeof(float), 256);
+  size_t floats = 64;
+  for (const bool codes : {false, true}) {
+    const paged::Plan p = paged::make_plan(B, Hq, Hk, D, rows, max_rows, max_len, codes);
+    floats = std::max({floats, p.part_floats, p.tile_floats});
+  }
+  return floats * sizeof(float);
 }
 
 extern "C" int dspark_paged_attention(const dspark_paged_attention_args* p, dspark_stream stream) {
@@ -88,7 +95,7 @@ extern "C" int dspark_paged_attention(const dspark_paged_attention_args* p, dspa
       return fail(DSPARK_ERR_ALIGN, "%s: strides of queries and outputs must be multiples of 16 bytes", what);
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->workspace, 16))
     return fail(DSPARK_ERR_ALIGN, "%s: queries, outputs and workspace must be 16-byte aligned", what);
-  const paged::Plan plan = paged::make_plan(a.s.B, p->Hq, p->Hk, p->D, a.s.T, p->max_rows, max_len);
+  const paged::Plan plan = paged::make_plan(a.s.B, p->Hq, p->Hk, p->D, a.s.T, p->max_rows, max_len, codes);
   const size_t need = std::max(plan.part_floats, plan.tile_floats) * sizeof(float);      // one after the other
   if ((size_t)p->workspace_bytes < need)
     return fail(DSPARK_ERR_WORKSPACE, "%s: workspace %ld < %zu bytes", what, (long)p->workspace_bytes, need);

@@ -8,9 +8,9 @@
 //   * K and V tiles are double buffered, one barrier a tile; each wave brings 16 positions, which lie in one page: pages of
 //     the model's type go to LDS without passing registers, 8-bit codes through registers, where they are turned into the
 //     model's type once for the workgroup;
-//   * sequences of unequal lengths: those with more keys than one and a half times the average share of a workgroup slot are
-//     split along the keys, into parts that a second launch joins (fp32, in the order of the keys). Everything is found on
-//     the device from the lengths as they are;
+//   * sequences of unequal lengths: those with more keys than one to one and a half times the average share of a workgroup
+//     slot are split along the keys, into parts that a second launch joins (fp32, in the order of the keys).
+//     Everything is found on the device from the lengths as they are;
 //   * items with many keys first: sequences by their length, long causal tiles first within one. Consecutive items are a
 //     tile's KV heads, which go to consecutive XCDs: with 8 heads each XCD's L2 has the pages of one.
 // Probabilities are two pieces of the type, as in dspark_paged_attn.h: the second costs a third of the products, and one
@@ -65,7 +65,10 @@ template <int D>
 struct TileList {
   const AttnArgs& a;
   TileWork first;
-  int target;                     // key tiles that a part may have before it is split: 1.5 times the average share of a slot
+  // Key tiles that a part may have: 1.5 times the average share of a slot. With one workgroup a CU (head dim 256) the least
+  // from the share on with which all items run together, if that is less: six verify blocks of 18 to 96 rows 66.7 -> 62.4 us
+  // (with two a CU, where a lone one runs faster, seven chunks lose 8% by it)
+  int target;
 
   __device__ __forceinline__ explicit TileList(const AttnArgs& args) : a(args), first(tile_work(args, min((int)__lane_id(), args.s.B - 1))) {
     const int lane = __lane_id();
@@ -76,8 +79,20 @@ struct TileList {
     }
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) sum += shfl_xor(sum, x);
-    const float t = 1.5f * sum * (float)a.Hk / kSlots<D>;
-    target = uniform(t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1);
+    const float share = sum * (float)a.Hk / kSlots<D>;
+    auto whole = [](float t) { return t < kLeastTiles ? kLeastTiles : t > 1e9f ? 1000000000 : (int)t + 1; };
+    target = whole(1.5f * share);
+    if (D == 256 && a.s.B <= 64) {
+      const int mine = whole((1.f + (float)lane / 128.f) * share);       // a lane's try
+      const float inv = 1.f / (float)mine;
+      float items = 0.f;
+      for (int b = 0; b < a.s.B; ++b)
+        items += (float)__builtin_amdgcn_readlane(first.row_tiles, b) *
+                 __builtin_ceilf((float)__builtin_amdgcn_readlane(first.key_tiles, b) * inv - 1e-6f);
+      const unsigned long long fit = __builtin_amdgcn_ballot_w64(items * (float)a.Hk <= (float)kSlots<D>);
+      if (fit) target = __builtin_amdgcn_readlane(mine, __builtin_ctzll(fit));
+    }
+    target = uniform(target);
   }
   __device__ __forceinline__ TileWork lanes(int b) const {   // of sequence b = 64 i + lane
     if (b < 64) return first;
