@@ -1129,9 +1129,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     rows, (ld, unit) = x.shape[0], x.stride()
     if (unit != 1 and V > 1) or ld < 0:
         x, ld = x.contiguous(), V
-    given, entropy = (torch.empty(shape[:-1], dtype=torch.float32, device=dev) for _ in range(2))
+    given = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(given)
     ids = torch.empty((*shape[:-1], top), dtype=torch.int32, device=dev)
-    best = torch.empty((*shape[:-1], top), dtype=torch.float32, device=dev)
+    best = torch.empty_like(ids, dtype=torch.float32)
     if rows:
         nbytes = token_logprobs_workspace_bytes(rows, V, top)
         if nbytes == 0:
@@ -1398,48 +1399,47 @@ PAGE_POSITIONS = (16, 32, 64, 128)
 PAGE_CODES, PAGE_SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu     # 8-bit pages: codes, and scales of a page and head
 
 
-def _pages_side(what: str, pages, shape, dtype, written: bool) -> tuple[bool, torch.Size, tuple]:
-    """(codes?, [pool, Hk, P, D], the fields of one ``dspark_pages``) of keys or values."""
-    scales = None
-    data = pages
-    if isinstance(pages, (tuple, list)):
-        data, scales = pages
-        if data.dtype is not PAGE_CODES or scales.dtype is not PAGE_SCALES:
-            raise TypeError(f"{what}: 8-bit pages are {PAGE_CODES} codes and {PAGE_SCALES} scales, got {data.dtype} and {scales.dtype}")
-    elif data.dtype is not dtype:
-        raise TypeError(f"{what}: pages {data.dtype} for rows of {dtype} (or codes with their scales)")
-    s = data.shape
-    if len(s) != 4 or (shape is not None and s != shape):
-        raise ValueError(f"{what}: pages must be [pages, Hk, positions, D], keys and values alike, got {list(s)}")
-    if s[2] not in PAGE_POSITIONS or s[3] not in QUANT_HEAD_DIMS:
-        raise ValueError(f"{what}: pages of {s[2]} positions {PAGE_POSITIONS} of {s[3]} values {QUANT_HEAD_DIMS}")
-    _no_autograd(what, data)
-    _as_stored(what, data)
-    p0, p1, p2, unit = data.stride()
-    if unit != 1:
-        raise ValueError(f"{what}: pages need unit stride along their values")
-    if written:
-        _no_repeats(what, data)
-    if scales is None:
-        return False, s, (data.data_ptr(), p0, p1, p2, 0, 0, 0)
-    if scales.shape != s[:2]:
-        raise ValueError(f"{what}: scales must be {list(s[:2])}, got {list(scales.shape)}")
-    if written:
-        _no_repeats(what, scales)
-    return True, s, (data.data_ptr(), p0, p1, p2, scales.data_ptr(), *scales.stride())
-
-
 def _pages_parts(pages) -> tuple:
     return tuple(pages) if isinstance(pages, (tuple, list)) else (pages,)
 
 
-def _both_pages(what: str, k_pages, v_pages, dtype, written: bool):
-    """(codes?, shape, fields of both, tensors written)."""
-    codes, shape, k = _pages_side(what, k_pages, None, dtype, written)
-    v_codes, _, v = _pages_side(what, v_pages, shape, dtype, written)
-    if codes != v_codes:
+def _both_pages(what: str, k_pages, v_pages, dtype, written: bool) -> tuple[bool, torch.Size, tuple]:
+    """(codes?, [pool, Hk, P, D], the fields of the two ``dspark_pages``) of keys and values. Decoding calls this for every
+    layer and token: what can go wrong is looked at first, what exactly did afterwards."""
+    k, v, ks, vs = k_pages, v_pages, None, None
+    if isinstance(k, (tuple, list)):
+        k, ks = k
+    if isinstance(v, (tuple, list)):
+        v, vs = v
+    codes = ks is not None
+    want = PAGE_CODES if codes else dtype
+    if codes != (vs is not None):
         raise TypeError(f"{what}: keys and values in 8 bits, or neither")
-    return codes, shape, k + v
+    if k.dtype is not want or v.dtype is not want or codes and (ks.dtype is not PAGE_SCALES or vs.dtype is not PAGE_SCALES):
+        raise TypeError(f"{what}: pages {k.dtype} and {v.dtype} for rows of {dtype} (8-bit pages are {PAGE_CODES} codes with "
+                        f"{PAGE_SCALES} scales)")
+    s = k.shape
+    if len(s) != 4 or v.shape != s:
+        raise ValueError(f"{what}: pages must be [pages, Hk, positions, D], keys and values alike, got {list(s)} and {list(v.shape)}")
+    if s[2] not in PAGE_POSITIONS or s[3] not in QUANT_HEAD_DIMS:
+        raise ValueError(f"{what}: pages of {s[2]} positions {PAGE_POSITIONS} of {s[3]} values {QUANT_HEAD_DIMS}")
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if k3 != 1 or v3 != 1:
+        raise ValueError(f"{what}: pages need unit stride along their values")
+    if k.is_neg() or v.is_neg():
+        _as_stored(what, k, v)
+    if written and not (k0 and k1 and k2 and v0 and v1 and v2):
+        _no_repeats(what, k)
+        _no_repeats(what, v)
+    if not codes:
+        return False, s, (k.data_ptr(), k0, k1, k2, 0, 0, 0, v.data_ptr(), v0, v1, v2, 0, 0, 0)
+    if ks.shape != s[:2] or vs.shape != s[:2]:
+        raise ValueError(f"{what}: scales must be {list(s[:2])}, got {list(ks.shape)} and {list(vs.shape)}")
+    if written:
+        _no_repeats(what, ks)
+        _no_repeats(what, vs)
+    return True, s, (k.data_ptr(), k0, k1, k2, ks.data_ptr(), *ks.stride(), v.data_ptr(), v0, v1, v2, vs.data_ptr(), *vs.stride())
 
 
 def _sequences(what: str, table: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, rows: int) -> tuple:
@@ -1451,14 +1451,17 @@ def _sequences(what: str, table: torch.Tensor, starts: torch.Tensor, lens: torch
         raise ValueError(f"{what}: {B} sequences (up to 4096)")
     if table.dtype is not torch.int32:
         table = _ints(what, "table", table, table.shape)
-    if W > 1 and table.stride(1) != 1 or table.stride(0) < W:
+    ld, unit = table.stride()
+    if unit != 1 and W > 1 or ld < W:
         table = table.contiguous()
+        ld = W
     starts, lens = _ints(what, "starts", starts, (B + 1,)), _ints(what, "lens", lens, (B,))
-    return (table.data_ptr(), starts.data_ptr(), lens.data_ptr(), max(table.stride(0), W), B, W, rows), (table, starts, lens)
+    return (table.data_ptr(), starts.data_ptr(), lens.data_ptr(), ld, B, W, rows), (table, starts, lens)
 
 
 def _paged_rows(what: str, name: str, t: torch.Tensor, T: int, H: int, D: int, dtype) -> tuple:
-    """Rows [T, H, D] as a kernel reads them (a copy where their addresses have no 16 bytes together), their strides."""
+    """Rows [T, H, D] as a kernel reads them (a copy where their addresses have no 16 bytes together), their address and
+    strides."""
     if t.dtype is not dtype:
         raise TypeError(f"{what}: {name} {t.dtype} beside {dtype}")
     if t.shape != (T, H, D):
@@ -1466,10 +1469,11 @@ def _paged_rows(what: str, name: str, t: torch.Tensor, T: int, H: int, D: int, d
     if t.is_neg():
         t = t.resolve_neg()
     s0, s1, unit = t.stride()
-    if unit != 1 or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
+    at = t.data_ptr()
+    if unit != 1 or s0 % 8 or s1 % 8 or at % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        s0, s1, _ = t.stride()
-    return t, s0, s1
+        at, s0, s1 = t.data_ptr(), H * D, D
+    return t, at, s0, s1
 
 
 _APPEND_ARGS = struct.Struct("=10qd37q")
@@ -1505,9 +1509,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     if k.dim() != 3:
         raise ValueError(f"{what}: k must be [rows, {Hk}, {D}], got {list(k.shape)}")
     T = k.shape[0]
-    _no_autograd(what, k, v, q, freqs, q_out)
-    k, *k_st = _paged_rows(what, "k", k, T, Hk, D, dtype)
-    v, *v_st = _paged_rows(what, "v", v, T, Hk, D, dtype)
+    _no_autograd(what, k, *tensors)
+    k, *k_at = _paged_rows(what, "k", k, T, Hk, D, dtype)
+    v, *v_at = _paged_rows(what, "v", v, T, Hk, D, dtype)
     seqs, keep = _sequences(what, table, starts, lens, T)
     at_f = dims = 0
     if freqs is not None:
@@ -1518,7 +1522,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
             raise ValueError(f"{what}: {dims} rotated values (a multiple of 16, interleaved of 8; others: rope, then paged_append)")
         freqs = freqs.resolve_neg().contiguous()
         at_f = freqs.data_ptr()
-    at_p = p_st = p64 = 0
+    at_p = p_st = p64 = at_o = 0
     if positions is not None:
         p64 = positions.dtype is torch.int64
         if not (p64 or positions.dtype is torch.int32) or positions.shape != (T,):
@@ -1529,12 +1533,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
         if q.dim() != 3:
             raise ValueError(f"{what}: q must be [{T}, heads, {D}], got {list(q.shape)}")
         Hq = q.shape[1]
-        clear = True
-        if q_out is None:
-            q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
-            q_out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+        clear = q_out is None
+        if clear:
+            q, *q_at = _paged_rows(what, "q", q, T, Hq, D, dtype)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            o_st = Hq * D, D
         else:
-            clear = False
             same = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
             if q_out.dtype is not dtype or q_out.shape != q.shape or q_out.stride(2) != 1 or q_out.stride(0) % 8 \
                     or q_out.stride(1) % 8 or q_out.data_ptr() % 16:
@@ -1543,19 +1547,21 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
             _no_repeats(what, q_out)
             if not same and q.numel() and _spans_meet(q, q_out):
                 raise ValueError(f"{what}: q_out overlaps q (in place: the same view)")
-            q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
-        q_fields = (q.data_ptr(), *q_st, q_out.data_ptr(), *q_out.stride()[:2], clear)
+            q, *q_at = _paged_rows(what, "q", q, T, Hq, D, dtype)
+            o_st = q_out.stride()[:2]
+        at_o = q_out.data_ptr()
+        q_fields = (*q_at, at_o, *o_st, clear)
     elif q_out is not None:
         raise ValueError(f"{what}: q_out without q")
     if T and seqs[4] and seqs[5] and pool and Hk:
         # what is written shares no place with what is read; k and v may
-        written = [pages[0], pages[7]] + ([pages[4], pages[11]] if codes else []) + ([q_out.data_ptr()] if Hq else [])
+        written = [pages[0], pages[7]] + ([pages[4], pages[11]] if codes else []) + ([at_o] if Hq else [])
         places = {*written}
-        if len(places) < len(written) or k.data_ptr() in places or v.data_ptr() in places:
+        if len(places) < len(written) or k_at[0] in places or v_at[0] in places:
             raise ValueError(f"{what}: the same rows given twice")
         _call_on(dev, "dspark_paged_append",
                  _APPEND_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, dims, bool(interleaved), at_f, scale, at_p, p64, p_st, *q_fields,
-                                   k.data_ptr(), *k_st, v.data_ptr(), *v_st, *pages, *seqs))
+                                   *k_at, *v_at, *pages, *seqs))
     elif Hq and clear:
         q_out.zero_()
     return q_out
@@ -1571,6 +1577,7 @@ def paged_read(k_pages, v_pages, pages: torch.Tensor, *, dtype: torch.dtype = to
     what = "paged_read"
     parts = (*_pages_parts(k_pages), *_pages_parts(v_pages))
     dev = _one_device(what, *parts, pages)
+    _no_autograd(what, *parts)
     dt = ATTN_DTYPES.get(dtype)
     if dt is None:
         raise TypeError(f"{what}: dtype {dtype} (bfloat16 or float16)")
@@ -1579,7 +1586,8 @@ def paged_read(k_pages, v_pages, pages: torch.Tensor, *, dtype: torch.dtype = to
         raise ValueError(f"{what}: pages must be int32 [N], got {list(pages.shape)}")
     ids = _ints(what, "pages", pages, pages.shape)
     N = ids.numel()
-    k, v = (torch.empty((N, Hk, P, D), dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty((N, Hk, P, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     if N and Hk and pool:
         _call_on(dev, "dspark_paged_read",
                  _READ_ARGS.pack(dt, codes, Hk, D, P, pool, ids.data_ptr(), N, *fields, k.data_ptr(), v.data_ptr()))
@@ -1612,7 +1620,8 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
     ``workspace`` of :func:`paged_attention_workspace_bytes`, 16-byte aligned, any content, for one call at a time, else
     allocated."""
     what = "paged_attention"
-    dev = _one_device(what, q, *_pages_parts(k_pages), *_pages_parts(v_pages), table, starts, lens, out, workspace)
+    parts = (*_pages_parts(k_pages), *_pages_parts(v_pages))
+    dev = _one_device(what, q, *parts, table, starts, lens, out, workspace)
     dtype = q.dtype
     dt = ATTN_DTYPES.get(dtype)
     if dt is None:
@@ -1624,7 +1633,7 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
     if not 1e-30 < scale < 1e30:
         raise ValueError(f"{what}: scale={scale} (positive)")
     T, Hq, _ = q.shape
-    _no_autograd(what, q, out)
+    _no_autograd(what, q, out, *parts)
     clear = out is None
     if not clear:
         if out.dtype is not dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 \
@@ -1634,9 +1643,9 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
         _no_repeats(what, out)
         if q.numel() and _spans_meet(q, out):
             raise ValueError(f"{what}: out overlaps q")
-    q, *q_st = _paged_rows(what, "q", q, T, Hq, D, dtype)
+    q, *q_at = _paged_rows(what, "q", q, T, Hq, D, dtype)
     if clear:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     seqs, keep = _sequences(what, table, starts, lens, T)
     B, W = seqs[4], seqs[5]
     rows = T if max_rows is None else min(int(max_rows), T)
@@ -1654,7 +1663,7 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
             elif workspace.nbytes < nbytes or not workspace.is_contiguous() or workspace.data_ptr() % 16:
                 raise ValueError(f"{what}: workspace: {nbytes} contiguous bytes, aligned to 16, needed")
             _call_on(dev, "dspark_paged_attention",
-                     _PAGED_ATTN_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, bool(causal), clear, rows, scale, q.data_ptr(), *q_st,
+                     _PAGED_ATTN_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, bool(causal), clear, rows, scale, *q_at,
                                            out.data_ptr(), *out.stride()[:2], *pages, *seqs[:5], W, T, workspace.data_ptr(),
                                            workspace.nbytes))
         elif clear:
