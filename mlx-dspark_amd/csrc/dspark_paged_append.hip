@@ -13,10 +13,11 @@
 //
 // Bound by bytes. Rows: a workgroup forms cos and sin of its row once in LDS for all heads. 8-bit pages: a workgroup a
 // (page, KV head, keys or values), since the scale needs all its rows first; they wait in LDS. Its threads take the
-// angles that they need themselves, as no other head shares them there; a page's chain of loads and angles is what takes
+// angles that they need themselves, as no other head shares them there (what rows become goes past the caches, 19.5 -> 19.0 us for the
+// 2048 below; read past them too they took 18.4 there, but the chunks 20.2 with their read for 18.1); a page's chain of loads and angles is what takes
 // the time of a step with fewer pages than the card has compute units (workgroups of 512 and 1024 threads shorten it by
 // 15% there, and cost as much and more where there are many). bf16: one row of 32 / 8 heads of 128 3.5 us, 2048 rows of 64 / 8
-// 18 to 20 us (4.3 to 4.6 TB/s); 8-bit pages, 48 single rows 5 us, chunks of 77 to 600 rows of 24 / 4 heads of 256 14 us.
+// 19 us (4.4 TB/s); 8-bit pages, 48 single rows 5 us, chunks of 77 to 600 rows of 24 / 4 heads of 256 14 us.
 #include <algorithm>
 
 #include "dspark_paged.h"
@@ -136,6 +137,7 @@ __device__ __forceinline__ void turn_item(const AppendArgs& a, Item& it, F turn)
   }
 }
 
+__device__ __forceinline__ void stg128_nt(void* p, u32x4_t v) { __builtin_nontemporal_store(v, static_cast<u32x4_t*>(p)); }
 __device__ __forceinline__ void stg128(void* p, u32x4_t v) { *static_cast<u32x4_t*>(p) = v; }
 
 // One row: its queries rotated, and into pages of the model's type its keys and values
@@ -179,11 +181,11 @@ __device__ __forceinline__ void append_row(const AppendArgs& a, float2* tab) {
       turn_item<DT, INTER>(a, it, [&](int j) { return tab[j]; });
       u16* y = key ? reinterpret_cast<u16*>(a.kp.data) + id * a.kp.page + hs * a.kp.head + off * a.kp.row
                    : reinterpret_cast<u16*>(a.qo) + t * a.qo_row + hs * a.qo_head;
-      stg128(y + it.d, it.lo);
-      if (it.d2 >= 0) stg128(y + it.d2, it.hi);
+      stg128_nt(y + it.d, it.lo);
+      if (it.d2 >= 0) stg128_nt(y + it.d2, it.hi);
     } else if (id >= 0) {
       const int j = i - turned, h = j >> log_plain, c = j & (plain - 1);
-      stg128(reinterpret_cast<u16*>(a.vp.data) + id * a.vp.page + h * a.vp.head + off * a.vp.row + 8 * c,
+      stg128_nt(reinterpret_cast<u16*>(a.vp.data) + id * a.vp.page + h * a.vp.head + off * a.vp.row + 8 * c,
              ldg128(reinterpret_cast<const u16*>(a.v.x) + t * a.v.row + h * a.v.head + 8 * c));
     }
   }

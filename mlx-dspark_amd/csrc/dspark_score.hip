@@ -15,8 +15,9 @@
 //
 // Bound by the bytes of the logits, with the exponential (a quarter of the rate) and about 6 more instructions a value
 // close behind. Many rows: a workgroup of four waves a row; few: up to 64 waves a row, a workgroup each, joined by a second
-// launch. bf16, 900 rows of 128255: 54 us (4.3 TB/s), 66 with the best 5, 74 with the best 20; one row of 151936: 6 us, 14
-// with the best 20, of which the list takes its time from a wave that has nothing beside it on its SIMD.
+// launch. bf16, 900 rows of 128255 with the best 5: 59 us (3.9 TB/s; 66 with loads that fill the caches, 61 and 72 with 16
+// and 48 values a lane's step instead of 32); one row of 151936: 6 us, 13 with the best 20, of which the list takes its time
+// from a wave that has nothing beside it on its SIMD.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(64 * WAVES) void score_kernel(const ScoreArgs a) {
     if (whole(c)) {
       const Vec* p = chunks + c + lane;
 #pragma unroll
-      for (int j = 0; j < NL; ++j) v[j] = p[64 * j];
+      for (int j = 0; j < NL; ++j) v[j] = __builtin_bit_cast(Vec, ldg128_nt(p + 64 * j));
       return;
     }
 #pragma unroll
