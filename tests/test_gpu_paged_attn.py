@@ -439,3 +439,68 @@ def test_chunks_over_pages_of_extreme_scales(dev):
         vp = (vp[0], (some + 127).to(torch.uint8).view(torch.float8_e8m0fnu).to(dev))
         args = (q, kp, vp, table, starts, lens)
         check(args, ops.paged_attention(*args, scale=0.125), 0.125)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("D,Hq,Hk", [(128, 8, 2), (256, 6, 1), (64, 4, 4)])
+def test_chunks_beside_decoded_tokens(dev, D, Hq, Hk, bits):
+    """One launch or two, by pages and head dim: tokens and short blocks behind short and long caches beside a chunk, long ones
+    split, sequences past the 64th among the split ones, rows of no sequence between and behind."""
+    n = 70
+    lens = [(53 * i) % 300 + 1 for i in range(n)]
+    rows = [1 if i % 9 else 0 for i in range(n)]
+    for i, L, r in ((3, 5000, 1), (40, 900, 250), (65, 7000, 2), (67, 3000, 33), (69, 4100, 16)):
+        lens[i], rows[i] = L, r
+    args, got = run(dev, "bf16", bits, Hq, Hk, D, 32, lens, rows, behind=5, max_rows=250, max_len=7000)
+    q, kp, vp, table, starts, lens = args
+    moved = starts.clone()
+    moved[66:] += 3                             # three rows more for 65
+    moved[65] -= 1                              # and one that was 64's
+    args = q, kp, vp, table, moved, lens
+    from dspark_rocm import ops
+
+    check(args, ops.paged_attention(*args, scale=0.1, max_rows=250), 0.1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,lens", [([18, 40, 96, 3, 33, 64], [1500, 4007, 2900, 700, 64, 1111]), ([50], [6000]),
+                                       ([11] * 64, [64 * i + 11 for i in range(64)]), ([11] * 66, [70 * i + 11 for i in range(66)])])
+def test_verify_blocks_at_head_dim_256(dev, rows, lens, dtype):
+    """Parts that all run together, where 64 sequences or fewer allow it."""
+    run(dev, dtype, 16, 6, 1, 256, 32, [max(a, b) for a, b in zip(lens, rows)], rows, max_rows=max(rows))
+
+
+def test_starts_that_fall(dev):
+    """Starts whose differences pass 31 bits, and sequences that share rows, leave no row of a new output unwritten."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(21)
+    kp, vp = (make_pages(g, 4, 1, 16, 64, torch.bfloat16, 16, dev) for _ in range(2))
+    junk = [torch.full((1 << 16,), float("nan"), device=dev) for _ in range(4)]
+    del junk                                    # what a new tensor finds in memory
+    for T in (9, 200):
+        q = torch.randn(T, 2, 64, generator=g).to(torch.bfloat16).to(dev)
+        table = ints([[0, 1, 2, 3]] * 3, dev)
+        for starts in ([0, 2 ** 31 - 1, -2, T], [0, T + 1, 0, T - 1], [0, 0, 0, 0], [T, T, T, T], [0, -2 ** 31, 2 ** 31 - 1, T]):
+            args = q, kp, vp, table, ints(starts, dev), ints([30, 40, 50], dev)
+            check(args, ops.paged_attention(*args, scale=0.2), 0.2)
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap read the same pages, each with a workspace of its own."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(22)
+    many = make(g, dev, "bf16", 16, 8, 2, 128, 64, [3000, 700], [200, 60])
+    few = make(g, dev, "bf16", 16, 8, 2, 128, 64, [5000, 64, 1200], [1, 1, 4])
+    want = [ops.paged_attention(*a, scale=0.1, max_rows=m) for a, m in ((many, 200), (few, 4))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, a, m in zip(streams, (many, few), (200, 4)):
+            with torch.cuda.stream(s):
+                got.append([ops.paged_attention(*a, scale=0.1, max_rows=m) for _ in range(4)])
+        for s in streams:
+            s.synchronize()
+        assert all(torch.equal(x, w) for xs, w in zip(got, want) for x in xs)
