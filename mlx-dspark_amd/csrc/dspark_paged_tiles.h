@@ -22,6 +22,11 @@
 //
 // The running maximum is only raised (and the outputs rescaled) where it grew by more than 2^8: fp32 sums do not mind
 // probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
+// 2048 rows behind 2953 keys, 32 / 8 heads of 128, bf16: 196 us (680 TFLOP/s of the two products, 1020 with the pieces); seven
+// chunks of 1 to 700 rows over 8-bit pages, 16 / 4 heads of 128: 134 us; six verify blocks of 18 to 96 rows of a KV head behind
+// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 60 us with what joins them. Tried and not kept: two groups of
+// four waves in a workgroup, one in its products while the other is in its softmax, a barrier between the phases (198 -> 234
+// us: as many cycles a tile, and lengths that fit together worse).
 #pragma once
 
 #include "dspark_attn_prefill.h"
@@ -574,7 +579,7 @@ __global__ __launch_bounds__(kAttnThreads) void join_tiles_kernel(const TileArgs
       const int parts = list.parts(v), i = (int)(x - (u32)of(rows_upto - rows)), h = i / v.rows, r = i - h * v.rows;
       const int tile = r / kTileRows, at = r - tile * kTileRows;
       const int first = (int)before + ((v.row_tiles - 1 - tile) * a.Hk + h) * parts;
-      const Joined<C> y = join_parts<D, 8>(ta.opart, ta.mpart, 1, 1.f, parts, 0, 1,
+      const Joined<C> y = join_parts<D, 4>(ta.opart, ta.mpart, 1, 1.f, parts, 0, 1,
                                            [&](int z) { return (long)(first + z) * kTileRows + at; },
                                            [&](int z) { return 2 * ((long)(first + z) * kTileRows + at); });
       const int tok = r / a.gqa;
