@@ -4,7 +4,7 @@
 // n (causal), or all of them; fp32 scores, running maximum and sum in one pass over the keys. The rows of a sequence and
 // KV head, R = n times the query heads of the group, are (token, query head), heads fastest.
 //
-// Bound by the bytes of K and V. 32 tokens behind 90 to 8192 positions, 32 / 8 heads of 128: 524 MB in 96 us (5.4 TB/s; 111 with
+// Bound by the bytes of K and V. 32 tokens behind 90 to 8192 positions, 32 / 8 heads of 128: 524 MB in 95 us (5.5 TB/s; 111 with
 // loads that fill the caches); two behind 70001 and 100000 8-bit positions, 64 / 8 heads: 395 MB in 76 us. Hence:
 //   * the work is the list of all (sequence, KV head, row group, 128 keys), dealt in equal runs to a fixed number of
 //     workgroups, whatever the lengths: a workgroup's run covers the end of one KV head, whole ones, and the start of
@@ -600,38 +600,39 @@ __device__ __forceinline__ void put_row(const AttnArgs& a, const float (&v)[D / 
   if (__builtin_amdgcn_ballot_w64(zero != 0.f)) plain_row<T, D, CODES>(a, b, t, head, keys);
 }
 
-// Joins the parts of a KV head's rows, a workgroup a row: its waves take every fourth part
-template <class T, int D, int RT, bool CODES>
+// Joins the parts of a KV head's rows. Few parts, up to 8 on the average: a wave a row (32 tokens behind 600 to 2500 positions
+// 48.7 -> 46.4 us with the first launch, 16 blocks of 4 to 8 rows 48 -> 39); many: a workgroup a row, whose waves take every
+// fourth part (one token behind 100000 positions has 64).
+template <class T, int D, int RT, bool CODES, bool FEW>
 __global__ __launch_bounds__(kAttnThreads) void join_kernel(const AttnArgs a, int workgroups) {
-  constexpr int ROWS = 16 * RT, C = D / 64;
-  __shared__ float sm[kWaves][D];
+  constexpr int ROWS = 16 * RT, C = D / 64, AT_ONCE = FEW ? 4 : C == 4 ? 8 : 16, STEP = FEW ? kWaves : 1;
+  __shared__ float sm[kWaves][FEW ? 1 : D];
   const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
   const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
   const Works<RT> works(a);
   const Work w = works.at(b);
-  if ((int)blockIdx.y >= w.rows) return;
+  if ((int)blockIdx.y * STEP >= w.rows) return;
   int before = 0;
   const int units = works.all(b, &before);
   if (!units) return;
   const int run = run_of(a, units, workgroups);
-  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
-    const int group = r / ROWS, rw = r - group * ROWS;
+  for (int r = (int)blockIdx.y * STEP + (FEW ? wave : 0); r < w.rows; r += gridDim.y * STEP) {
+    const int group = r / ROWS, rw = r - group * ROWS, i = r / a.gqa;
     const int u0 = before + (h * w.groups + group) * w.tiles, u1 = u0 + w.tiles;
     const int j0 = u0 / run, j1 = (u1 - 1) / run;
     if (j0 == j1) continue;
     auto slot = [&](int z) { return (2 * (long)(j0 + z) + (z == 0 ? 1 : 0)) * ROWS; };
-    Joined<C> x = join_parts<D, (C == 4 ? 8 : 16)>(a.opart, a.mpart, ROWS, a.scale_log2, j1 - j0 + 1, wave, kWaves,
-                                                  [&](int z) { return slot(z) + rw; }, [&](int z) { return 2 * slot(z) + rw; });
+    Joined<C> x = join_parts<D, AT_ONCE>(a.opart, a.mpart, ROWS, a.scale_log2, j1 - j0 + 1, FEW ? 0 : wave, FEW ? 1 : kWaves,
+                                         [&](int z) { return slot(z) + rw; }, [&](int z) { return 2 * slot(z) + rw; });
+    if constexpr (!FEW) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) sm[wave][C * lane + i] = x.v[i];
-    __syncthreads();
-    if (wave == 0) {
+      for (int c = 0; c < C; ++c) sm[wave][C * lane + c] = x.v[c];
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < C; ++i) x.v[i] = (sm[0][C * lane + i] + sm[1][C * lane + i]) + (sm[2][C * lane + i] + sm[3][C * lane + i]);
-      const int i = r / a.gqa;
-      put_row<T, D, CODES>(a, x.v, x.l, b, w.start + i, h * a.gqa + r - i * a.gqa, keys_seen(a, w, i));
+      for (int c = 0; c < C; ++c) x.v[c] = (sm[0][C * lane + c] + sm[1][C * lane + c]) + (sm[2][C * lane + c] + sm[3][C * lane + c]);
     }
-    __syncthreads();
+    if (FEW || wave == 0) put_row<T, D, CODES>(a, x.v, x.l, b, w.start + i, h * a.gqa + r - i * a.gqa, keys_seen(a, w, i));
+    if (!FEW) __syncthreads();
   }
 }
 
@@ -640,8 +641,10 @@ int launch_rows(const AttnArgs& a, int workgroups, int most_rows, hipStream_t s)
   hipLaunchKernelGGL((rows_kernel<T, D, RT, CODES>), dim3((unsigned)workgroups), dim3(kAttnThreads), 0, s, a);
   const int st = check_launch("paged_attention");
   if (st || a.whole) return st;
-  const unsigned y = (unsigned)std::min(most_rows, 16 * RT);     // more rows: a loop
-  hipLaunchKernelGGL((join_kernel<T, D, RT, CODES>), dim3((unsigned)(a.s.B * a.Hk), y), dim3(kAttnThreads), 0, s, a, workgroups);
+  const unsigned x = (unsigned)(a.s.B * a.Hk), y = (unsigned)std::min(most_rows, 16 * RT);      // more rows: a loop
+  if (workgroups <= 8 * (long)x)                                 // parts of a row, on the average
+    hipLaunchKernelGGL((join_kernel<T, D, RT, CODES, true>), dim3(x, (y + kWaves - 1) / kWaves), dim3(kAttnThreads), 0, s, a, workgroups);
+  else hipLaunchKernelGGL((join_kernel<T, D, RT, CODES, false>), dim3(x, y), dim3(kAttnThreads), 0, s, a, workgroups);
   return check_launch("paged_attention(join)");
 }
 
