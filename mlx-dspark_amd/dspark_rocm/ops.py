@@ -1129,7 +1129,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     rows, (ld, unit) = x.shape[0], x.stride()
     if (unit != 1 and V > 1) or ld < 0:
         x, ld = x.contiguous(), V
-    given = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    given = torch.empty_like(tokens, dtype=torch.float32)
     entropy = torch.empty_like(given)
     ids = torch.empty((*shape[:-1], top), dtype=torch.int32, device=dev)
     best = torch.empty_like(ids, dtype=torch.float32)
@@ -1509,7 +1509,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     if k.dim() != 3:
         raise ValueError(f"{what}: k must be [rows, {Hk}, {D}], got {list(k.shape)}")
     T = k.shape[0]
-    _no_autograd(what, k, *tensors)
+    _no_autograd(what, k, v, q, freqs, q_out, *_pages_parts(k_pages), *_pages_parts(v_pages))
     k, *k_at = _paged_rows(what, "k", k, T, Hk, D, dtype)
     v, *v_at = _paged_rows(what, "v", v, T, Hk, D, dtype)
     seqs, keep = _sequences(what, table, starts, lens, T)
