@@ -24,7 +24,8 @@
 // probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
 // 2048 rows behind 2953 keys, 32 / 8 heads of 128, bf16: 196 us (680 TFLOP/s of the two products, 1020 with the pieces); seven
 // chunks of 1 to 700 rows over 8-bit pages, 16 / 4 heads of 128: 134 us; six verify blocks of 18 to 96 rows of a KV head behind
-// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 60 us with what joins them. Tried and not kept: two groups of
+// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 59 us with what joins them
+// (63 when waves without rows multiplied too). Tried and not kept: two groups of
 // four waves in a workgroup, one in its products while the other is in its softmax, a barrier between the phases (198 -> 234
 // us: as many cycles a tile, and lengths that fit together worse).
 #pragma once
@@ -246,7 +247,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   // keys that this lane's row sees, the wave's least and most, the workgroup's most
   const int lim = keys_seen(a, w, tok);
   const int wmin = uniform(keys_seen(a, w, min(rw, w.rows - 1) / a.gqa));
-  const int wmax = uniform(keys_seen(a, w, min(rw + 31, w.rows - 1) / a.gqa));
+  const int wmax = rw < w.rows ? uniform(keys_seen(a, w, min(rw + 31, w.rows - 1) / a.gqa)) : 0;      // (none for a wave without rows)
   const int bmax = uniform(keys_seen(a, w, min(r0 + kTileRows - 1, w.rows - 1) / a.gqa));
   const int ntile = (bmax + KT - 1) / KT;
   const int t0 = (int)((long)ntile * z / parts), t1 = (int)((long)ntile * (z + 1) / parts);
@@ -399,9 +400,10 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-      // K operands are asked for KA steps ahead of their products, V operands one (left to itself the compiler reads one and
-      // waits for it)
-      constexpr int KA = NK < 4 ? NK : 4;
+      // K operands are asked for KA steps ahead of their products, V operands of DB column blocks one (left to itself the
+      // compiler reads one and waits for it). Two of each at head dim 256, where what is past 256 registers moves between two
+      // files (513 rows behind 2462 positions: 87.6 -> 84.5 us)
+      constexpr int KA = D == 256 ? 2 : NK < 4 ? NK : 4;
       u32x4_t kf[KA][SUB];
       auto read_k = [&](int kk) {
 #pragma unroll
@@ -424,7 +426,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
         const u32x2_t lo = lds_tr(vp), hi = lds_tr(vp + 8 * D);
         return u32x4_t{lo.x, lo.y, hi.x, hi.y};
       };
-      constexpr int DB = ND < 4 ? ND : 4, NG = 2 * SUB * (ND / DB);    // V operands of a step, steps
+      constexpr int DB = D == 256 ? 2 : ND < 4 ? ND : 4, NG = 2 * SUB * (ND / DB);    // V operands of a step, steps
       u32x4_t vf[2][DB];
       auto read_v = [&](int g) {
 #pragma unroll
