@@ -24,10 +24,9 @@
 // probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
 // 2048 rows behind 2953 keys, 32 / 8 heads of 128, bf16: 196 us (680 TFLOP/s of the two products, 1020 with the pieces); seven
 // chunks of 1 to 700 rows over 8-bit pages, 16 / 4 heads of 128: 134 us; six verify blocks of 18 to 96 rows of a KV head behind
-// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 59 us with what joins them
-// (63 when waves without rows multiplied too). Tried and not kept: two groups of
-// four waves in a workgroup, one in its products while the other is in its softmax, a barrier between the phases (198 -> 234
-// us: as many cycles a tile, and lengths that fit together worse).
+// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 59 us with what joins them (63 when waves without rows
+// multiplied too). Tried and not kept: two groups of four waves in a workgroup, one in its products while the other is in its
+// softmax, a barrier between the phases (198 -> 234 us: as many cycles a tile, and lengths that fit together worse).
 #pragma once
 
 #include "dspark_attn_prefill.h"
