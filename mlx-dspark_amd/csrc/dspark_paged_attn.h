@@ -17,7 +17,8 @@
 //     the second product needs. K goes from memory to the operand, V through LDS (the transposing read), 16-byte
 //     chunks XOR-swizzled by the row;
 //   * 8-bit pages are turned into the model's type as they are used: one conversion for two values with the page's power of
-//     two in it, exact.
+//     two in it, exact for every page that a model of that type wrote, but for values past fp16's largest: keys take what fp16 does not
+//     hold of their power of two to the scores (key_unit), values become infinite, and their rows are computed again.
 // Probabilities go to the matrix cores as two pieces of the type (16 bits of bf16, 22 of fp16, there of p 2^15): at these
 // row counts the second piece costs nothing.
 //
@@ -201,6 +202,16 @@ __device__ __forceinline__ void decode(u32x4_t c, float unit, u32x4_t& lo, u32x4
   }
 }
 
+// What a page's power of two leaves of itself where its keys become values of T, and what multiplies their scores instead: fp16
+// has all codes, 2^-9 to 448 in size, times 2^-15 to 2^7. (fp16 rows of 63489 and more become 256 2^8 = 65536: as an fp16 infinity such a
+// key had no weight, or all of it.)
+template <class T>
+__device__ __forceinline__ float key_unit(float unit) { return T::kF16 ? fminf(fmaxf(unit, 0x1p-15f), 0x1p7f) : unit; }
+template <class T>
+__device__ __forceinline__ float key_rest(float unit) {
+  return key_unit<T>(unit) == unit ? 1.f : unit * (unit < 1.f ? 0x1p15f : 0x1p-7f);
+}
+
 // The 16-byte chunk c of row r of a V tile lies at chunk c ^ tile_swz(r): a transposing read takes two chunks of 16 rows
 template <int D>
 __device__ __forceinline__ int tile_swz(int r) { return D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
         for (int c = 0; c < KL; ++c) {
           if constexpr (CODES) {
             u32x4_t lo, hi;
-            decode<T>(kr[j][c], j ? ku1 : ku0, lo, hi);
+            decode<T>(kr[j][c], key_unit<T>(j ? ku1 : ku0), lo, hi);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               s[rt][j] = attn::mfma<T>(lo, qf[rt][2 * c], s[rt][j]);
@@ -368,6 +379,13 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
           } else {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) s[rt][j] = attn::mfma<T>(kr[j][c], qf[rt][c], s[rt][j]);
+          }
+        }
+        if constexpr (CODES && T::kF16) {
+          const float rest = key_rest<T>(j ? ku1 : ku0);
+          if (rest != 1.f) {                                 // wave-uniform
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt][j] *= rest;
           }
         }
       }

@@ -206,6 +206,7 @@ template <int D>
 struct TileLds {
   u16 kv[2][2][kTileKeys * D];    // [buffer][K, V]
   u32 fits[2][4];                 // V of 16 positions fits fp16
+  float rest[2][4];               // of fp16 models: key_rest of 16 positions
 };
 
 // A workgroup's item; false if it was given up at a tile whose V does not fit fp16
@@ -331,7 +332,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
       for (int j = 0; j < CJ; ++j) {
         const int i = j * 64 + lane, rr = 16 * wave + i / (D / 16), c = 2 * (i % (D / 16));
         u32x4_t lo, hi;
-        decode<T>(kc[j], kc_unit, lo, hi);
+        decode<T>(kc[j], key_unit<T>(kc_unit), lo, hi);
         *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + ((c ^ k_swz<D>(rr)) << 3)]) = lo;
         *reinterpret_cast<u32x4_t*>(&sm[buf][0][rr * D + (((c + 1) ^ k_swz<D>(rr)) << 3)]) = hi;
         if constexpr (FP16) decode<F16>(vc[j], vc_unit * (1 << kNarrow), lo, hi);
@@ -341,6 +342,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
       }
       // codes are up to 448 in size and multiples of 2^-9
       if (FP16 && lane == 0) fits[buf][wave] = vc_unit <= 0.125f && vc_unit >= 1.f / (1 << 25);
+      if (T::kF16 && lane == 0) lds.rest[buf][wave] = key_rest<T>(kc_unit);
     }
   };
 
@@ -418,6 +420,18 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
         for (int u = 0; u < SUB; ++u) s[u] = mfma32<T>(kf[kk % KA][u], qf[kk], s[u]);
         if (kk + KA < NK) read_k(kk + KA);
         __builtin_amdgcn_sched_barrier(kAluMayCross);
+      }
+      if constexpr (CODES && T::kF16) {
+        const u32x4_t f = *reinterpret_cast<const u32x4_t*>(lds.rest[buf]);
+        const int one = __builtin_bit_cast(int, 1.f);
+        const int f0 = uniform((int)f.x), f1 = uniform((int)f.y), f2 = uniform((int)f.z), f3 = uniform((int)f.w);
+        if (f0 != one || f1 != one || f2 != one || f3 != one) {
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)                     // (positions 16 (2 u + i / 8) ..)
+              s[u][i] *= __builtin_bit_cast(float, u ? i < 8 ? f2 : f3 : i < 8 ? f0 : f1);
+        }
       }
       if (t + 1 < t1) bring_v(buf ^ 1);             // (its registers are free now)
       auto v_frag = [&](int uj, int d) {                     // V^T of keys 16 uj .. 16 uj + 15, columns 32 d ..

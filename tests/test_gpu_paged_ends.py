@@ -1,0 +1,86 @@
+"""GPU: paged caches at the ends of their ranges: keys and scales that a narrower type does not hold, scores and scales without a
+number, chunks that begin again."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests._paged import DT, attention, check_rows, host, ints, make_pages, make_table, oracle_pages, starts_of
+
+pytestmark = pytest.mark.gpu
+
+BEHIND = {1: 40, 5: 3000, 100: 150, 33: 6000}          # rows: positions; one part and several, of either kernel
+
+
+def call(args, scale, pieces=2.0 ** -16, **kw):
+    """The operator's rows, against attention in 64 bits over the values that the pages hold."""
+    from dspark_rocm import ops
+
+    q, kp, vp, table, starts, lens = args
+    got = ops.paged_attention(*args, scale=scale, **kw)
+    want, tol = attention(host(q), oracle_pages(kp), oracle_pages(vp), table.cpu().numpy(), starts.tolist(), lens.tolist(), scale, True, pieces)
+    check_rows(got, want, tol)
+    return got
+
+
+def make(g, dev, dtype, bits, Hq, Hk, D, P, lens, rows):
+    pool = sum(-(-n // P) for n in lens) + 2
+    kp, vp = (make_pages(g, pool, Hk, P, D, DT[dtype], bits, dev) for _ in range(2))
+    q = torch.randn(sum(rows), Hq, D, generator=g).to(DT[dtype]).to(dev)
+    return q, kp, vp, make_table(g, lens, P, pool, dev), starts_of(rows, dev), ints(lens, dev)
+
+
+def with_scales(pages, e):
+    return pages[0], (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu).to(pages[0].device)
+
+
+# ---------------------------------------------------------------------------- 8-bit keys that fp16 does not hold
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", BEHIND)
+def test_the_largest_keys_of_fp16_rows(dev, n, D, both):
+    """A row's 65000 becomes the code 256 of scale 2^8: 65536, which fp16 does not have and a score does. Keys of one sign, and of
+    both; queries of either."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(1)
+    L = BEHIND[n]
+    q, kp, vp, table, starts, lens = make(g, dev, "f16", 8, 2, 1, D, 16, [L], [n])
+    k, v = (torch.randn(L, 1, D, generator=g).to(torch.float16) for _ in range(2))
+    k[::3, 0, 5] = 65000.0
+    if both:
+        k[1::3, 0, 5] = -65504.0
+    ops.paged_append(k.to(dev), v.to(dev), kp, vp, table, ints([0, L], dev), lens)
+    assert (oracle_pages(kp).values == 65536).any()
+    for far in (-1e-4, 1e-4, 3e-5):
+        q[..., 5] = far
+        call((q, kp, vp, table, starts, lens), 0.125)
+
+
+def test_one_key_that_fp16_does_not_hold(dev):
+    """The only key of a row has all of its weight, whatever its score."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(2)
+    q, kp, vp, table, starts, lens = make(g, dev, "f16", 8, 1, 1, 64, 16, [1], [1])
+    k, v = torch.full((1, 1, 64), 1.0, dtype=torch.float16, device=dev), torch.ones(1, 1, 64, dtype=torch.float16, device=dev)
+    k[..., 0] = 65000.0
+    ops.paged_append(k, v, kp, vp, table, starts, lens)
+    q[..., 0] = -1e-4
+    assert (ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.125) == 1).all()
+
+
+@pytest.mark.parametrize("low,high,size", [(8, 14, 2e-5), (-26, -20, 3e4), (-24, 12, 1e-3)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", BEHIND)
+def test_scales_of_keys_past_fp16(dev, n, D, low, high, size):
+    """Scales past both ends of fp16, pages of ordinary ones between."""
+    g = torch.Generator().manual_seed(3)
+    q, kp, vp, table, starts, lens = make(g, dev, "f16", 8, 2, 1, D, 16, [BEHIND[n]], [n])
+    e = torch.randint(low, high, kp[1].shape, generator=g)
+    e[torch.rand(e.shape, generator=g) < 0.3] = -7
+    q = (q * size).clamp(-65504, 65504)
+    call((q, with_scales(kp, e), vp, table, starts, lens), 0.05)
