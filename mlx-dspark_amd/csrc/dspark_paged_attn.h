@@ -22,8 +22,8 @@
 // Probabilities go to the matrix cores as two pieces of the type (16 bits of bf16, 22 of fp16, there of p 2^15): at these
 // row counts the second piece costs nothing.
 //
-// Values that are not finite are only let through where a row sees them: a row with such an output is computed again in
-// plain fp32 from the keys it sees (plain_row).
+// Values that are not finite are only let through where a row sees them: a row with such an output, or one that sees keys and has
+// no probability (scores of -inf), is computed again in plain fp32 from the keys it sees (plain_row).
 #pragma once
 
 #include "dspark_attn.h"
@@ -131,6 +131,14 @@ template <class T, int D, bool CODES>
 __device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int head, int keys) {
   const int lane = __lane_id(), h = head / a.gqa;
   const u16* q = a.q + t * a.qrow + head * a.qhead;
+  u16* o = a.out + t * a.orow + head * a.ohead + lane * (D / 64);
+  bool some = false;                                         // a key that is there
+  for (int p = lane; (long)p << a.s.log2P < keys; p += 64) some |= page_of(a.s, b, (long)p << a.s.log2P) >= 0;
+  if (!__builtin_amdgcn_ballot_w64(some)) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) o[c] = 0;
+    return;
+  }
   auto unit = [&](const Pages& p, int id) {
     return CODES ? __builtin_bit_cast(float, (u32)p.exps[id * p.epage + h * p.ehead] << 23) : 1.f;
   };
@@ -156,7 +164,6 @@ __device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int h
 #pragma unroll 1
   for (int x = 1; x < 64; x *= 2) l += shfl_xor(l, x);
   float sum[D / 64] = {};
-  bool any = false;
 #pragma unroll 1
   for (int k0 = 0; k0 < keys; k0 += 64) {
     const float p = weight(k0 + lane) / l;
@@ -164,16 +171,14 @@ __device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int h
     for (int j = 0; j < min(64, keys - k0); ++j) {
       const int id = page_of(a.s, b, k0 + j);
       if (id < 0) continue;
-      any = true;
       const float pj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j)), u = unit(a.v, id);
       const long at = id * a.v.page + h * a.v.head + ((k0 + j) & (a.s.P - 1)) * a.v.row + lane * (D / 64);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) sum[c] = __builtin_fmaf(pj, element<T, CODES>(a.v, at + c, u), sum[c]);
     }
   }
-  u16* o = a.out + t * a.orow + head * a.ohead + lane * (D / 64);
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) o[c] = attn::from_f32<T>(any ? sum[c] : 0.f);
+  for (int c = 0; c < D / 64; ++c) o[c] = attn::from_f32<T>(sum[c]);
 }
 
 // Keys that row i of a sequence's n sees
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
       const int r = r0 + rw, i = r / a.gqa;
       if (r < w.rows) {
         const float inv = lt > 0.f ? 1.f / lt : 0.f;
-        float zero = lt - lt;                                // NaN once an output is not finite
+        float zero = lt > 0.f || lim[rt] == 0 ? lt - lt : 1.f;       // NaN once an output is not finite
         for (int x = wave; x < ND; x += kWaves) {
           f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -605,7 +610,7 @@ __device__ __forceinline__ void put_row(const AttnArgs& a, const float (&v)[D / 
   constexpr int C = D / 64;
   const float inv = l > 0.f ? 1.f / l : 0.f;
   u16* op = a.out + t * a.orow + head * a.ohead + C * (int)__lane_id();
-  float zero = l - l;
+  float zero = l > 0.f || keys == 0 ? l - l : 1.f;
   u16 x[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {

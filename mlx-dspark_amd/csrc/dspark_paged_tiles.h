@@ -533,7 +533,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
     return true;
   }
   const float inv = l > 0.f ? kUnscale / l : 0.f;
-  float zero = l - l;             // NaN once an output is not finite
+  float zero = l > 0.f || lim == 0 ? l - l : 1.f;            // NaN once an output is not finite
   if (own) {
     u16* op = a.out + (w.start + tok) * a.orow + head * a.ohead + 4 * half;
 #pragma unroll

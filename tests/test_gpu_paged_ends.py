@@ -84,3 +84,56 @@ def test_scales_of_keys_past_fp16(dev, n, D, low, high, size):
     e[torch.rand(e.shape, generator=g) < 0.3] = -7
     q = (q * size).clamp(-65504, 65504)
     call((q, with_scales(kp, e), vp, table, starts, lens), 0.05)
+
+
+# ---------------------------------------------------------------------------- rows without a finite score
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", BEHIND)
+def test_rows_whose_scores_are_all_minus_infinity(dev, n, D, dtype):
+    """exp(-inf - -inf) is no number: an infinity in every key that a row sees is not hidden behind a zero. Rows that see nothing
+    of their sequence, or a finite score beside, are what they were."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(4)
+    L = BEHIND[n]
+    q, kp, vp, table, starts, lens = make(g, dev, dtype, 16, 2, 1, D, 16, [L, 90], [n, 1])
+    q[:, 0, 3], q[:, 1, 3] = 1.0, 0.5
+    clean = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.1)
+    for b, m in enumerate((L, 90)):
+        if b == 0:
+            kp[table[b, :-(-m // 16)].long(), :, :, 3] = -float("inf")
+    got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.1)
+    assert got[:n].isnan().all() and torch.equal(got[n:], clean[n:])
+    kp[table[0, 0].item(), :, 7, 3] = 2.0                    # one key that has a score
+    got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.1)
+    seen = torch.arange(L - n, L, device=dev) >= 7
+    assert torch.equal(got[:n][seen], vp[table[0, 0].item(), :, 7].expand(int(seen.sum()), 2, D)) and got[:n][~seen].isnan().all()
+    # of n rows the last 7 have positions: the others see nothing
+    if n > 7:
+        kp[table[0, 0].item(), :, 7, 3] = -float("inf")
+        short = lens.clone()
+        short[0] = 7
+        got = ops.paged_attention(q, kp, vp, table, starts, short, scale=0.1)
+        assert not got[:n - 7].any() and got[n - 7:n].isnan().all()
+        gone = table.clone()
+        gone[0] = -1
+        assert not ops.paged_attention(q, kp, vp, gone, starts, lens, scale=0.1)[:n].any()
+
+
+@pytest.mark.parametrize("n", BEHIND)
+def test_scores_far_below_zero(dev, n):
+    """Equal scores of -1e34, one product each: finite, and a softmax like that of zeros."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(5)
+    L = BEHIND[n]
+    q, kp, vp, table, starts, lens = make(g, dev, "bf16", 16, 2, 1, 64, 16, [L], [n])
+    q.zero_()
+    kp.zero_()
+    q[..., 0], kp[..., 0] = 1e17, -1e17
+    got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=1.0)
+    want, tol = attention(0 * host(q), oracle_pages(kp), oracle_pages(vp), table.cpu().numpy(), starts.tolist(), lens.tolist(), 1.0)
+    check_rows(got, want, tol)
