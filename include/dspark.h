@@ -728,8 +728,8 @@ int dspark_kv_dequantize(const dspark_kv_args* args, dspark_stream stream);
 
 /*
  * Keys or values of a pool of pages: [pool, Hk, P, D], P = 16, 32, 64 or 128 positions, D = 64, 128 or 256, of the
- * model's type, or (codes) e4m3 codes c that stand for c * 2^(e - 127) with a byte e (e8m0) for each page and head in
- * exponents [pool, Hk]. Strides in elements, of 16-byte multiples, unit stride along D.
+ * model's type, or (codes) e4m3 codes c that stand for c * 2^(e - 127) with a byte e (e8m0: 255 is NaN) for each page and head
+ * in exponents [pool, Hk]. Strides in elements, of 16-byte multiples, unit stride along D.
  */
 typedef struct dspark_pages { /* every field is 8 bytes; strides are (page, head, position) and (page, head) */
   void* data;
@@ -760,8 +760,8 @@ typedef struct dspark_sequences { /* every field is 8 bytes */
  * fl(fl(x1 s) + fl(x2 c)) in fp32, rounded to dtype. positions (int32 or int64 [rows]) replaces the rows' own.
  * q_out may be q itself. Pages of codes: the exponent of a page and head becomes the least with |x| <= 448 2^(e - 127)
  * for the finite values of the rows new in it, at least 17, and at least what it was where the page holds rows of this
- * sequence before them, which are shifted to it; codes are rounded to nearest even, infinities become NaN. A page that is
- * written to belongs to one sequence.
+ * sequence before them, which are shifted to it; codes are rounded to nearest even, infinities become NaN, and so do rows
+ * behind others of a NaN scale. A page that is written to belongs to one sequence.
  */
 typedef struct dspark_paged_append_args { /* every field is 8 bytes */
   int64_t dtype, codes, Hq, Hk, D, P, pool, dims, interleaved;

@@ -3,7 +3,7 @@
 // A cache is a pool of pages of P positions (a power of two) for every KV head; sequence b's position p lies in row
 // p % P of page table[b][p / P]. A step's rows of all sequences stand one after the other: starts[b] .. starts[b + 1] - 1
 // are sequence b's, the last ones of the lens[b] positions that it has with them. Pages are of the model's type, or hold
-// e4m3 codes c that stand for c 2^E, with one exponent E for each page and head (e8m0: a byte E + 127). With a power of
+// e4m3 codes c that stand for c 2^E, with one exponent E for each page and head (e8m0: a byte E + 127, NaN for 255). With a power of
 // two the codes' own precision is all there is to lose: a page whose exponent grows shifts its codes' exponents, and
 // nothing is rounded that stays normal.
 //
@@ -25,6 +25,11 @@ struct Pages {                   // keys or values
   long page, head, row;          // strides in elements
   long epage, ehead;
 };
+
+// 2^(e - 127), NaN for 255: what a scale byte stands for
+__device__ __forceinline__ float scale_of(u32 e) {
+  return __builtin_bit_cast(float, e == 0 ? 0x400000u : e == 255 ? 0x7FC00000u : e << 23);
+}
 
 // The sequences of a call
 struct Seqs {

@@ -9,7 +9,7 @@
 //
 // 8-bit pages: E of a page and head is the least exponent with |x| <= 448 2^E for the finite values of the rows new in it,
 // at least kLeastExp and the page's own where it holds rows of the sequence before them; codes are e4m3(x 2^-E), those
-// of the earlier rows shifted where E grew. Infinities and NaN become NaN codes.
+// of the earlier rows shifted where E grew. Infinities and NaN become NaN codes, and so does what is put behind rows of a NaN scale.
 //
 // Bound by bytes. Rows: a workgroup forms cos and sin of its row once in LDS for all heads. 8-bit pages: a workgroup a
 // (page, KV head, keys or values), since the scale needs all its rows first; they wait in LDS. Its threads take the
@@ -224,8 +224,6 @@ __device__ __forceinline__ u32 shift_codes(u32 c, float by) {
   return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(hi.x * by, hi.y * by, r, true);
 }
 
-__device__ __forceinline__ float exp2_of(int e) { return __builtin_bit_cast(float, (u32)(e + 127) << 23); }
-
 // The rows new in one page of one KV head, keys or values
 template <int DT, bool INTER>
 __device__ __forceinline__ void append_page8(const AppendArgs& a, u16* stash, u32* joined) {
@@ -293,7 +291,7 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, u16* stash, u3
   int e = max((int)(m >> 23) - 127 - 8 + ((m & 0x7FFFFFu) > 0x600000u ? 1 : 0), kLeastExp);
   const int old = lo ? (int)*ep - 127 : kLeastExp;
   e = max(e, old);
-  const float unit = exp2_of(-e);
+  const float unit = e > 127 ? __builtin_nanf("") : scale_of((u32)(127 - e));
   unsigned char* to = reinterpret_cast<unsigned char*>(pg.data) + id * pg.page + h * pg.head;
   for (int i = threadIdx.x; i < rows << log8; i += kThreads) {
     const int r = i >> log8, c = i - (r << log8);
@@ -301,7 +299,7 @@ __device__ __forceinline__ void append_page8(const AppendArgs& a, u16* stash, u3
   }
   if (lo && e > old) {
     const int by = old - e;
-    const float f = by < -126 ? 0.f : exp2_of(by);
+    const float f = by < -126 ? 0.f : scale_of((u32)(by + 127));
     for (int i = threadIdx.x; i < lo << (log8 - 1); i += kThreads) {
       const int r = i >> (log8 - 1), c = i - (r << (log8 - 1));
       u32x4_t* p = reinterpret_cast<u32x4_t*>(to + r * pg.row + 16 * c);
@@ -351,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadArgs a) {
       const long at = id * pg.page + h * pg.head + r * pg.row + 8 * c;
       if constexpr (CODES) {
         const u32x2_t w = *reinterpret_cast<const u32x2_t*>(pg.data + at);
-        const float unit = exp2_of((int)pg.exps[id * pg.epage + h * pg.ehead] - 127);
+        const float unit = scale_of(pg.exps[id * pg.epage + h * pg.ehead]);
         typedef float f32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {

@@ -140,7 +140,7 @@ __device__ __forceinline__ void plain_row(const AttnArgs& a, int b, int t, int h
     return;
   }
   auto unit = [&](const Pages& p, int id) {
-    return CODES ? __builtin_bit_cast(float, (u32)p.exps[id * p.epage + h * p.ehead] << 23) : 1.f;
+    return CODES ? scale_of(p.exps[id * p.epage + h * p.ehead]) : 1.f;
   };
   auto score = [&](int key) {
     const int id = key < keys ? page_of(a.s, b, key) : -1;
@@ -306,8 +306,8 @@ __global__ __launch_bounds__(kAttnThreads, RT * D > 256 || D == 256 ? 1 : 2) voi
       if constexpr (CODES) {
         ku = vu = 0.f;
         if (ids >= 0) {
-          ku = __builtin_bit_cast(float, (u32)a.k.exps[ids * a.k.epage + h * a.k.ehead] << 23);
-          vu = __builtin_bit_cast(float, (u32)a.v.exps[ids * a.v.epage + h * a.v.ehead] << 23);
+          ku = scale_of(a.k.exps[ids * a.k.epage + h * a.k.ehead]);
+          vu = scale_of(a.v.exps[ids * a.v.epage + h * a.v.ehead]);
         }
       }
     };

@@ -267,8 +267,8 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
     if constexpr (CODES) {
       ku = vu = 0.f;
       if (ids >= 0) {
-        ku = __builtin_bit_cast(float, (u32)a.k.exps[ids * a.k.epage + h * a.k.ehead] << 23);
-        vu = __builtin_bit_cast(float, (u32)a.v.exps[ids * a.v.epage + h * a.v.ehead] << 23);
+        ku = scale_of(a.k.exps[ids * a.k.epage + h * a.k.ehead]);
+        vu = scale_of(a.v.exps[ids * a.v.epage + h * a.v.ehead]);
       }
     }
   };

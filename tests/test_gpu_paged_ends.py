@@ -3,10 +3,12 @@ number, chunks that begin again."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from tests._paged import DT, attention, check_rows, host, ints, make_pages, make_table, oracle_pages, starts_of
+from oracle import paged_ref
+from tests._paged import DT, attention, check_rows, exps, host, ints, make_pages, make_table, oracle_pages, starts_of, typed
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +139,90 @@ def test_scores_far_below_zero(dev, n):
     got = ops.paged_attention(q, kp, vp, table, starts, lens, scale=1.0)
     want, tol = attention(0 * host(q), oracle_pages(kp), oracle_pages(vp), table.cpu().numpy(), starts.tolist(), lens.tolist(), 1.0)
     check_rows(got, want, tol)
+
+
+# ---------------------------------------------------------------------------- every scale byte
+
+
+def values(pages):
+    """What codes with scale bytes stand for, in 64 bits: 2^-127 for byte 0, NaN for 255."""
+    b = pages[1].view(torch.uint8).cpu().numpy().astype(np.float64)
+    return host(pages[0]) * np.where(b == 255, np.nan, np.exp2(b - 127))[:, :, None, None]
+
+
+def with_bytes(pages, b):
+    return pages[0], torch.as_tensor(b, dtype=torch.uint8).expand(pages[1].shape).contiguous().view(torch.float8_e8m0fnu).to(pages[0].device)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_read_of_every_scale_byte(dev, dtype):
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(6)
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1, 4).view(256, 1, 16, 64).view(torch.float8_e4m3fn).to(dev)
+    pages = with_bytes((codes, torch.zeros(256, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu)), torch.arange(256)[:, None])
+    other = make_pages(g, 256, 1, 16, 64, DT[dtype], 8, dev)
+    k, v = ops.paged_read(pages, other, torch.arange(256, dtype=torch.int32, device=dev), dtype=DT[dtype])
+    for got, p in ((k, pages), (v, other)):
+        np.testing.assert_array_equal(host(got), typed(DT[dtype])(values(p)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n", BEHIND)
+def test_attention_over_every_scale_byte(dev, n, dtype):
+    """A NaN scale is NaN to the rows that see its page and nothing to others; the least and the largest are numbers."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(7)
+    L = BEHIND[n]
+    q, kp, vp, table, starts, lens = make(g, dev, dtype, 8, 2, 1, 64, 16, [L, 90], [n, 1])
+    clean = ops.paged_attention(q, kp, vp, table, starts, lens, scale=0.1)
+    last = table[0, (L - 1) // 16].item()
+    sees = torch.arange(L - n, L, device=dev) >= (L - 1) // 16 * 16
+    for which in (0, 1):
+        pages = [kp, vp]
+        b = pages[which][1].view(torch.uint8).clone()
+        b[last] = 255
+        pages[which] = with_bytes(pages[which], b)
+        got = ops.paged_attention(q, *pages, table, starts, lens, scale=0.1)
+        assert got[:n][sees].isnan().all() and torch.equal(got[n:], clean[n:])
+        off = (got[:n][~sees].double() - clean[:n][~sees].double()).abs()
+        assert off.numel() == 0 or off.max() <= 2 ** -7 * clean.double().abs().max()
+    # keys and values of next to nothing, values that fp16 does not hold beside them (there: rows computed again in fp32)
+    for which in (0, 1):
+        pages = [kp, vp]
+        b = pages[which][1].view(torch.uint8).clone()
+        b[::2] = 0
+        if which and dtype == "f16":
+            b[1::2] = 127 + 8
+        pages[which] = with_bytes(pages[which], b)
+        x = host(q), *(paged_ref.Pages(values(p)) for p in pages)
+        want, tol = attention(*x, table.cpu().numpy(), starts.tolist(), lens.tolist(), 0.1, True, 2.0 ** (-11 if dtype == "bf16" else -16))
+        got = ops.paged_attention(q, *pages, table, starts, lens, scale=0.1)
+        fits = np.abs(want) < 6e4
+        check_rows(torch.where(torch.from_numpy(fits).to(dev), got, 0), np.where(fits, want, 0), tol)
+        assert fits.mean() > 0.5
+
+
+@pytest.mark.parametrize("which", [254, 255, 0])
+def test_rows_behind_the_last_scales(dev, which):
+    """A page's old scale counts where it holds rows before: 2^127 as any other, NaN for the new rows too."""
+    from dspark_rocm import ops
+
+    g = torch.Generator().manual_seed(8)
+    D, P = 64, 16
+    kp, vp = (with_bytes(make_pages(g, 2, 2, P, D, torch.bfloat16, 8, dev), torch.full((2, 2), which)) for _ in range(2))
+    k, v = (torch.randn(3, 2, D, generator=g).to(torch.bfloat16) * (1e38 if which else 1.0) for _ in range(2))
+    k, v = k.clamp(-3e38, 3e38), v.clamp(-3e38, 3e38)
+    want = []
+    for pages, x in ((kp, k), (vp, v)):
+        w = paged_ref.Pages(values(pages), np.full((2, 2), which - 127))
+        if which != 255:
+            paged_ref.append(w, host(x), np.array([[1]]), [0, 3], [8])
+        else:
+            w.values[1, :, 5:8] = np.nan
+        want.append(w)
+    ops.paged_append(k.to(dev), v.to(dev), kp, vp, ints([[1]], dev), ints([0, 3], dev), ints([8], dev))
+    for got, w in zip((kp, vp), want):
+        np.testing.assert_array_equal(exps(got[1]), w.exps)
+        np.testing.assert_array_equal(values(got)[:, :, :8], w.values[:, :, :8])
