@@ -1476,6 +1476,16 @@ def _paged_rows(what: str, name: str, t: torch.Tensor, T: int, H: int, D: int, d
     return t, at, s0, s1
 
 
+def _no_positions(k_pages, v_pages, table: torch.Tensor):
+    """A pool without pages, or a table without room, as the kernels can take it: the rows are there, none of their positions is."""
+    def one(pages):
+        if isinstance(pages, (tuple, list)):
+            return tuple(torch.zeros((1, *t.shape[1:]), dtype=torch.uint8, device=t.device).view(t.dtype) for t in pages)
+        return pages.new_zeros((1, *pages.shape[1:]))
+
+    return one(k_pages), one(v_pages), table.new_full((table.shape[0], 1), -1)
+
+
 _APPEND_ARGS = struct.Struct("=10qd37q")
 
 
@@ -1512,7 +1522,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     _no_autograd(what, k, v, q, freqs, q_out, *_pages_parts(k_pages), *_pages_parts(v_pages))
     k, *k_at = _paged_rows(what, "k", k, T, Hk, D, dtype)
     v, *v_at = _paged_rows(what, "v", v, T, Hk, D, dtype)
+    if not Hk:
+        raise ValueError(f"{what}: pages of no heads")
     seqs, keep = _sequences(what, table, starts, lens, T)
+    if not (pool and seqs[5]):
+        nowhere = _no_positions(k_pages, v_pages, table)
+        _, (pool, *_), pages = _both_pages(what, *nowhere[:2], dtype, True)
+        seqs, keep = _sequences(what, nowhere[2], starts, lens, T)
     at_f = dims = 0
     if freqs is not None:
         if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= D // 2:
@@ -1553,7 +1569,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
         q_fields = (*q_at, at_o, *o_st, clear)
     elif q_out is not None:
         raise ValueError(f"{what}: q_out without q")
-    if T and seqs[4] and seqs[5] and pool and Hk:
+    if T and seqs[4]:
         # what is written shares no place with what is read; k and v may
         written = [pages[0], pages[7]] + ([pages[4], pages[11]] if codes else []) + ([at_o] if Hq else [])
         places = {*written}
@@ -1615,7 +1631,8 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
     are not finite count only where a row sees them. Positions of pages that the pool does not have are not seen.
 
     ``max_rows`` (rows of one sequence) and ``max_len`` (positions; default: what the table has room for) are the
-    host's bounds: positions from ``max_len`` on, rounded up to a page, are not seen; more rows than ``max_rows`` are
+    host's bounds: positions from ``max_len`` on, rounded up to a page, are not seen (0 says that no sequence has any, and so
+    no rows, whatever ``lens``: nothing is done but a new ``out`` cleared); more rows than ``max_rows`` are
     served too, only slower. ``out``: rows of no sequence are left as they are there; in a new one they are zeros.
     ``workspace`` of :func:`paged_attention_workspace_bytes`, 16-byte aligned, any content, for one call at a time, else
     allocated."""
@@ -1647,6 +1664,10 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
     if clear:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     seqs, keep = _sequences(what, table, starts, lens, T)
+    if not (pool and seqs[5]) and not clear:                     # (a new out is cleared below)
+        nowhere, workspace = _no_positions(k_pages, v_pages, table), None
+        _, (pool, *_), pages = _both_pages(what, *nowhere[:2], dtype, False)
+        seqs, keep = _sequences(what, nowhere[2], starts, lens, T)
     B, W = seqs[4], seqs[5]
     rows = T if max_rows is None else min(int(max_rows), T)
     if max_len is not None:

@@ -226,3 +226,33 @@ def test_rows_behind_the_last_scales(dev, which):
     for got, w in zip((kp, vp), want):
         np.testing.assert_array_equal(exps(got[1]), w.exps)
         np.testing.assert_array_equal(values(got)[:, :, :8], w.values[:, :, :8])
+
+
+# ---------------------------------------------------------------------------- no positions at all
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_pools_and_tables_of_nothing(dev, bits):
+    """A pool without pages, a table without room: rows of sequences are turned, and see nothing; rows of none stay."""
+    from dspark_rocm import ops, rope
+
+    g = torch.Generator().manual_seed(9)
+    freqs = rope.frequencies(64, 1e4, device=dev)[0]
+    q, kp, vp, table, _, _ = make(g, dev, "bf16", bits, 4, 2, 64, 16, [40, 3], [5, 2])
+    starts, lens = ints([1, 4, 6], dev), ints([40, 3], dev)
+    k, v = (torch.randn(7, 2, 64, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+    cut = lambda p: tuple(t[:0] for t in p) if bits == 8 else p[:0]
+    want = ops.paged_append(k, v, kp, vp, torch.full_like(table, -1), starts, lens, q=q, freqs=freqs)
+    inside = torch.tensor([False] + [True] * 5 + [False], device=dev)
+    for pages, t in (((kp, vp), table[:, :0]), ((cut(kp), cut(vp)), table), ((cut(kp), cut(vp)), table[:, :0].long())):
+        assert torch.equal(ops.paged_append(k, v, *pages, t, starts, lens, q=q, freqs=freqs), want)
+        y = q.clone()
+        assert ops.paged_append(k, v, *pages, t, starts, lens, q=y, freqs=freqs, q_out=y) is y
+        assert torch.equal(y[inside], want[inside]) and torch.equal(y[~inside], q[~inside])
+        for rows in (1, 7):
+            out = torch.full_like(q, 7.0)
+            ops.paged_attention(q, *pages, t, starts, lens, scale=0.1, out=out, max_rows=rows)
+            assert not out[inside].any() and (out[~inside] == 7).all()
+            assert not ops.paged_attention(q, *pages, t, starts, lens, scale=0.1, max_rows=rows).any()
+        assert ops.paged_append(k, v, *pages, t, starts, lens) is None
+    assert not inside.all() and want[inside].any()
