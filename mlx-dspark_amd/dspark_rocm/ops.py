@@ -1476,6 +1476,67 @@ def _paged_rows(what: str, name: str, t: torch.Tensor, T: int, H: int, D: int, d
     return t, at, s0, s1
 
 
+@functools.lru_cache(maxsize=256)
+def _lie_apart(ahead: int, size_a: int, a: tuple, size_b: int, b: tuple) -> bool:
+    """Whether two views whose spans meet are known to share no byte: ``b`` begins ``ahead`` bytes behind ``a``, each is (count,
+    bytes of stride) pairs of elements of ``size`` bytes. So they are where, in steps of some stride of theirs, what
+    the others span lies side by side: heads of one row of queries, keys and values, keys and values of one page."""
+    for period in {s for n, s in a + b if n > 1 and s}:
+        reach = lambda size, dims: size + sum((n - 1) * s for n, s in dims if s % period)
+        off = ahead % period
+        if reach(size_a, a) <= off and off + reach(size_b, b) <= period:
+            return True
+    return False
+
+
+def _span(at: int, size: int, *dims: tuple) -> tuple:
+    """Where a view begins and ends, for :func:`_share`."""
+    end = at + size
+    for n, s in dims:
+        end += (n - 1) * s
+    return at, end, size, dims
+
+
+def _share(x: tuple, y: tuple) -> bool:
+    return x[0] < y[1] and y[0] < x[1] and not _lie_apart(y[0] - x[0], x[2], x[3], y[2], y[3])
+
+
+def _page_spans(codes: bool, pool: int, Hk: int, P: int, D: int, f: tuple) -> list:
+    """Spans of the parts of ``_both_pages``' fields: keys, values, and their scales."""
+    e = 1 if codes else 2
+    spans = [_span(f[i], e, (pool, e * f[i + 1]), (Hk, e * f[i + 2]), (P, e * f[i + 3]), (D, e)) for i in (0, 7)]
+    return spans + [_span(f[i], 1, (pool, f[i + 1]), (Hk, f[i + 2])) for i in (4, 11)] if codes else spans
+
+
+def _page_ends(codes: bool, pool: int, Hk: int, P: int, D: int, f: tuple) -> tuple:
+    """Where keys, values (and their scales) end."""
+    if not codes:
+        return (f[0] + 2 * ((pool - 1) * f[1] + (Hk - 1) * f[2] + (P - 1) * f[3] + D),
+                f[7] + 2 * ((pool - 1) * f[8] + (Hk - 1) * f[9] + (P - 1) * f[10] + D))
+    return (f[0] + (pool - 1) * f[1] + (Hk - 1) * f[2] + (P - 1) * f[3] + D, f[7] + (pool - 1) * f[8] + (Hk - 1) * f[9] + (P - 1) * f[10] + D,
+            f[4] + (pool - 1) * f[5] + (Hk - 1) * f[6] + 1, f[11] + (pool - 1) * f[12] + (Hk - 1) * f[13] + 1)
+
+
+def _meet_pages(at: int, end: int, codes: bool, f: tuple, ends: tuple) -> bool:
+    """Whether the bytes from ``at`` to ``end`` meet the spans of the pages."""
+    return at < ends[0] and f[0] < end or at < ends[1] and f[7] < end or codes and (at < ends[2] and f[4] < end or at < ends[3] and f[11] < end)
+
+
+def _side_by_side(ahead: int, wide_a: int, wide_b: int, step: int, size: int) -> bool:
+    """Whether, every ``step`` elements, what two views span lies beside each other; ``ahead`` in bytes."""
+    off = ahead % (step * size) if step else -1
+    return wide_a * size <= off and off + wide_b * size <= step * size
+
+
+def _overlaps(T: int, D: int, to: tuple, rows: tuple, written: list) -> bool:
+    """Whether the pages that an append writes share memory, or the queries' place (``to``: heads, address and strides; none: a new
+    one) and them or ``rows``, keys and values alike."""
+    if any(_share(x, y) for i, x in enumerate(written) for y in written[i + 1:]):
+        return True
+    span = lambda heads, at, s0, s1: _span(at, 2, (T, 2 * s0), (heads, 2 * s1), (D, 2))
+    return bool(to) and any(_share(span(*to), x) for x in (*(span(*r) for r in rows), *written))
+
+
 def _no_positions(k_pages, v_pages, table: torch.Tensor):
     """A pool without pages, or a table without room, as the kernels can take it: the rows are there, none of their positions is."""
     def one(pages):
@@ -1570,11 +1631,30 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     elif q_out is not None:
         raise ValueError(f"{what}: q_out without q")
     if T and seqs[4]:
-        # what is written shares no place with what is read; k and v may
-        written = [pages[0], pages[7]] + ([pages[4], pages[11]] if codes else []) + ([at_o] if Hq else [])
-        places = {*written}
-        if len(places) < len(written) or k_at[0] in places or v_at[0] in places:
-            raise ValueError(f"{what}: the same rows given twice")
+        # What is written shares no byte with what else is written, and the queries' place none with k and v. (k and v may be
+        # rows of the pool in pages that the call does not write, but not from its first page on.) Decoding comes by here for every
+        # layer: plain sums first, what they do not settle afterwards.
+        (at_ka, sk0, sk1), (at_va, sv0, sv1) = k_at, v_at
+        ends = _page_ends(codes, pool, Hk, P, D, pages)
+        at_k, at_v = pages[0], pages[7]
+        near = at_ka == at_k or at_ka == at_v or at_va == at_k or at_va == at_v
+        if not near and at_k < ends[1] and at_v < ends[0]:
+            wide, wide_v = ((Hk - 1) * f1 + (P - 1) * f2 + D for f1, f2 in (pages[2:4], pages[9:11]))
+            near = pages[1] != pages[8] or not _side_by_side(at_v - at_k, wide, wide_v, pages[1], 1 if codes else 2)
+        if codes and not near:
+            near = pages[4] < ends[3] and pages[11] < ends[2] and not (
+                pages[5] == pages[12] and _side_by_side(pages[11] - pages[4], (Hk - 1) * pages[6] + 1, (Hk - 1) * pages[13] + 1, pages[5], 1))
+        placed = Hq and not clear
+        if placed and not near:
+            o0, o1 = o_st
+            wide, wide_k, wide_v = (Hq - 1) * o1 + D, (Hk - 1) * sk1 + D, (Hk - 1) * sv1 + D
+            end = at_o + 2 * ((T - 1) * o0 + wide)
+            near = at_o < at_ka + 2 * ((T - 1) * sk0 + wide_k) and at_ka < end and not (o0 == sk0 and _side_by_side(at_ka - at_o, wide, wide_k, o0, 2)) \
+                or at_o < at_va + 2 * ((T - 1) * sv0 + wide_v) and at_va < end and not (o0 == sv0 and _side_by_side(at_va - at_o, wide, wide_v, o0, 2)) \
+                or _meet_pages(at_o, end, codes, pages, ends)
+        if near and (at_ka in (at_k, at_v) or at_va in (at_k, at_v) or _overlaps(
+                T, D, (Hq, at_o, *o_st) if placed else (), ((Hk, *k_at), (Hk, *v_at)), _page_spans(codes, pool, Hk, P, D, pages))):
+            raise ValueError(f"{what}: the same memory given twice (what is written overlaps)")
         _call_on(dev, "dspark_paged_append",
                  _APPEND_ARGS.pack(dt, codes, Hq, Hk, D, P, pool, dims, bool(interleaved), at_f, scale, at_p, p64, p_st, *q_fields,
                                    *k_at, *v_at, *pages, *seqs))
@@ -1660,6 +1740,10 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
         _no_repeats(what, out)
         if q.numel() and _spans_meet(q, out):
             raise ValueError(f"{what}: out overlaps q")
+        at_o, (o0, o1, _) = out.data_ptr(), out.stride()
+        if T and Hq and pool and _meet_pages(at_o, at_o + 2 * ((T - 1) * o0 + (Hq - 1) * o1 + D), codes, pages, _page_ends(codes, pool, Hk, P, D, pages)) \
+                and any(_share(_span(at_o, 2, (T, 2 * o0), (Hq, 2 * o1), (D, 2)), x) for x in _page_spans(codes, pool, Hk, P, D, pages)):
+            raise ValueError(f"{what}: out overlaps the pages")
     q, *q_at = _paged_rows(what, "q", q, T, Hq, D, dtype)
     if clear:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
