@@ -209,9 +209,34 @@ struct TileLds {
   float rest[2][4];               // of fp16 models: key_rest of 16 positions
 };
 
-// A workgroup's item; false if it was given up at a tile whose V does not fit fp16
+struct TileItem {
+  TileWork w;
+  int b, local, parts;            // its sequence, its place among the sequence's items, parts of a row tile
+};
+
+// The workgroup's item of the list
+template <int D>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, TileItem& it) {
+  const TileList<D> list(a);
+  const u32 all = list.all();
+  if (all > kMostUnits) return false;
+  // Of the 512 that start together, two a CU, the second 256 in turned order: a long causal tile shares its CU with a
+  // short one (2048 rows behind 2953 keys: 193.4 -> 191.6 us). At head dim 256 a CU has one, and the second 256 only start with
+  // their shortest; that order was not measured
+  const u32 nth = blockIdx.x >> 3, rounds = (all + 7) / 8;
+  const u32 turned = nth / 32 == 1 && rounds > 32 ? 32 + min(63u, rounds - 1) - nth : nth;
+  const u32 item = turned * 8 + (blockIdx.x & 7);
+  if (nth >= rounds || item >= all) return false;
+  if (!list.locate(item, it.b, it.local)) return false;
+  it.w = list.at(it.b);
+  it.parts = list.parts(it.w);
+  return true;
+}
+
+// A workgroup's item; false if it was given up at a tile whose V does not fit fp16. `again`: rows of the wave that plain_rows
+// has to compute
 template <class T, int D, bool CODES, bool FP16>
-__device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
+__device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds, u32& again) {
   using prefill::k_swz;
   using prefill::lds_tr;
   using prefill::mfma32;
@@ -227,20 +252,10 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15;
 
-  const TileList<D> list(a);
-  const u32 all = list.all();
-  if (all > kMostUnits) return true;
-  // Of the 512 that start together, two a CU, the second 256 in turned order: a long causal tile shares its CU with a
-  // short one (2048 rows behind 2953 keys: 193.4 -> 191.6 us)
-  const u32 nth = blockIdx.x >> 3, rounds = (all + 7) / 8;
-  const u32 turned = nth / 32 == 1 && rounds > 32 ? 32 + min(63u, rounds - 1) - nth : nth;
-  const u32 item = turned * 8 + (blockIdx.x & 7);
-  if (nth >= rounds || item >= all) return true;
-  int b, local;
-  if (!list.locate(item, b, local)) return true;
-  const TileWork w = list.at(b);
-  const int parts = list.parts(w);
-  const int z = local % parts, h = local / parts % a.Hk, tile = w.row_tiles - 1 - local / (parts * a.Hk);
+  TileItem it;
+  if (!find_item<D>(a, it)) return true;
+  const TileWork& w = it.w;
+  const int b = it.b, parts = it.parts, z = it.local % parts, h = it.local / parts % a.Hk, tile = w.row_tiles - 1 - it.local / (parts * a.Hk);
 
   const int r0 = tile * kTileRows, rw = r0 + 32 * wave;
   const int r = min(rw + l31, w.rows - 1), tok = r / a.gqa, head = h * a.gqa + (r - tok * a.gqa);
@@ -516,7 +531,7 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
   l += shfl_xor(l, 32);
   const bool own = rw + l31 < w.rows;
   if (parts > 1) {
-    const int part = TileList<D>(a).parts_before(b) + local;      // (kept from the start, the list costs registers)
+    const int part = TileList<D>(a).parts_before(b) + it.local;   // (kept from the start, the list costs registers)
     if (part >= kParts || !own) return true;
     const long pr = (long)part * kTileRows + 32 * wave + l31;
     if (half == 0) {
@@ -548,26 +563,40 @@ __device__ __forceinline__ bool take_item(const TileArgs& ta, TileLds<D>& lds) {
       }
   }
   const unsigned long long bad = __builtin_amdgcn_ballot_w64(own && zero != 0.f);
-  if (!bad) return true;
-  __threadfence_block();
-  for (u32 rows = (u32)bad | (u32)(bad >> 32); rows; rows &= rows - 1) {
-    const int i = rw + __builtin_ctz(rows), ti = i / a.gqa;
-    plain_row<T, D, CODES>(a, b, w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, w, ti));
-  }
+  again = (u32)bad | (u32)(bad >> 32);
   return true;
+}
+
+// Rows of the wave again, in plain fp32. The item is found anew: kept, what this needs would cost registers in take_item's loop
+template <class T, int D, bool CODES>
+__device__ __forceinline__ void plain_rows(const AttnArgs& a, u32 rows) {
+  TileItem it;
+  if (!find_item<D>(a, it)) return;
+  const int h = it.local / it.parts % a.Hk, tile = it.w.row_tiles - 1 - it.local / (it.parts * a.Hk);
+  const int rw = tile * kTileRows + 32 * uniform((int)threadIdx.x >> 6);
+  __threadfence_block();
+  for (; rows; rows &= rows - 1) {
+    const int i = rw + __builtin_ctz(rows), ti = i / a.gqa;
+    plain_row<T, D, CODES>(a, it.b, it.w.start + ti, h * a.gqa + i - ti * a.gqa, keys_seen(a, it.w, ti));
+  }
 }
 
 template <class T, int D, bool CODES>
 __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void tiles_kernel(const TileArgs ta) {
   __shared__ __attribute__((aligned(16))) TileLds<D> lds;
   if (ta.a.clear) clear_rows<D>(ta.a);
+  u32 again = 0;
   // (At head dim 256 the two paths together are past the registers of one wave)
   if constexpr (CODES && !T::kF16 && D <= 128) {
-    if (take_item<T, D, CODES, true>(ta, lds)) return;
-    __syncthreads();              // every wave has read what does not fit
-    asm volatile("" ::: "memory");
+    if (!take_item<T, D, CODES, true>(ta, lds, again)) {
+      __syncthreads();            // every wave has read what does not fit
+      asm volatile("" ::: "memory");
+      take_item<T, D, CODES, false>(ta, lds, again);
+    }
+  } else {
+    take_item<T, D, CODES, false>(ta, lds, again);
   }
-  take_item<T, D, CODES, false>(ta, lds);
+  if (again) plain_rows<T, D, CODES>(ta.a, again);
 }
 
 // Joins the parts of split sequences; a wave a row
