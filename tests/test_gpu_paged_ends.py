@@ -256,3 +256,81 @@ def test_pools_and_tables_of_nothing(dev, bits):
             assert not ops.paged_attention(q, *pages, t, starts, lens, scale=0.1, max_rows=rows).any()
         assert ops.paged_append(k, v, *pages, t, starts, lens) is None
     assert not inside.all() and want[inside].any()
+
+
+# ---------------------------------------------------------------------------- 8-bit chunks of bf16 models: one fp16 piece, or again with two
+
+
+def chunk(args, scale, **kw):
+    """A probability is one fp16 piece: half a step, 2^-11 of it at most, or where it is subnormal, 2^-25 with the row's reference at
+    2^7: 2^-32 of the largest weight a key."""
+    from dspark_rocm import ops
+
+    q, kp, vp, table, starts, lens = args
+    got = ops.paged_attention(*args, scale=scale, **kw)
+    values = oracle_pages(vp)
+    want, tol = attention(host(q), oracle_pages(kp), values, table.cpu().numpy(), starts.tolist(), lens.tolist(), scale, True, 2.0 ** -11)
+    check_rows(got, want, tol + int(lens.max()) * 2.0 ** -32 * np.abs(values.values).max())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("low,high", [(-60, -59), (20, 21), (-30, 5), (-3, -1)])
+def test_chunks_that_begin_again(dev, D, low, high):
+    """V that does not fit fp16 in some page of every item, early or late."""
+    g = torch.Generator().manual_seed(10)
+    q, kp, vp, table, starts, lens = make(g, dev, "bf16", 8, 4, 2, D, 16, [700, 90, 2000], [200, 90, 33])
+    e = torch.randint(low, high, vp[1].shape, generator=g)
+    e[torch.rand(e.shape, generator=g) < 0.5] = low
+    chunk((q, kp, with_scales(vp, e), table, starts, lens), 0.125)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("e", [-2, 12, -40, -110])
+@pytest.mark.parametrize("rows,L,at", [(33, 6000, 5200), (33, 6000, 40), (600, 1500, 1390), (70, 9000, 4500)])
+def test_one_page_that_does_not_fit(dev, D, e, rows, L, at):
+    """One page among many: the part, or the row tiles, that come to it begin again, the others do not, and are joined."""
+    g = torch.Generator().manual_seed(11)
+    q, kp, vp, table, starts, lens = make(g, dev, "bf16", 8, 2, 1, D, 16, [L, 300], [rows, 40])
+    b = (vp[1].view(torch.uint8).to(torch.int64) - 127).cpu()
+    b[table[0, at // 16].item()] = e
+    chunk((q, kp, with_scales(vp, b), table, starts, lens), 0.1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,L", [(100, 700), (33, 6000), (600, 1500)])
+def test_chunks_with_pages_that_are_not_there(dev, D, rows, L):
+    g = torch.Generator().manual_seed(12)
+    q, kp, vp, table, starts, lens = make(g, dev, "bf16", 8, 2, 1, D, 16, [L, 300], [rows, 40])
+    for at, bad in ((L // 2, -1), (L // 2 + 16, 10 ** 6), (L - 1, -7), (0, -1)):
+        table[0, at // 16] = bad
+        chunk((q, kp, vp, table, starts, lens), 0.1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows,L", [(70, 900), (33, 6000)])
+@pytest.mark.parametrize("shape", ["slow", "rise", "fall", "first", "steps", "low", "late"])
+def test_8_bit_scores_that_rise_and_fall(dev, D, rows, L, shape):
+    """The running maximum's rule where a probability is fp16: up to 2^8 over the reference, and far under it."""
+    from dspark_rocm import ops
+
+    f = {"slow": lambda i: 0.001 * i, "rise": lambda i: 0.02 * i, "fall": lambda i: -0.02 * i, "first": lambda i: 30.0 * (i == 0),
+         "steps": lambda i: 5.4 * (i // 64 % 2), "low": lambda i: -60 + 0.0 * i, "late": lambda i: 25.0 * (i == L - rows)}[shape]
+    g = torch.Generator().manual_seed(13)
+    q, kp, vp, table, starts, lens = make(g, dev, "bf16", 8, 2, 1, D, 16, [L], [rows])
+    q[:] = q[:1, :1]
+    size = float((q[0, 0].double() ** 2).sum()) * 0.1
+    k = (q[0, 0].double()[None, None] * f(torch.arange(L, dtype=torch.float64, device=dev))[:, None, None] / size).to(torch.bfloat16)
+    v = torch.randn(L, 1, D, generator=g).to(torch.bfloat16).to(dev)
+    ops.paged_append(k, v, kp, vp, table, ints([0, L], dev), lens)
+    chunk((q, kp, vp, table, starts, lens), 0.1)
+
+
+@pytest.mark.parametrize("Hq,Hk,D,P,lens,rows", [(4, 2, 64, 16, [1, 2, 5, 900], [1, 2, 4, 3]), (32, 8, 128, 64, [3, 700, 40], [2, 16, 1]),
+                                                 (6, 1, 256, 32, [4, 1300, 2], [1, 5, 2]), (8, 1, 128, 16, [2500, 9], [8, 6])])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_few_rows_over_8_bit_pages_have_two_pieces(dev, Hq, Hk, D, P, lens, rows, dtype):
+    """Decoded tokens and verify blocks: 2^-16 of a probability, over 8-bit pages too. Few keys, where a piece lost is not averaged
+    away."""
+    for seed in range(4):
+        g = torch.Generator().manual_seed(20 + seed)
+        call(make(g, dev, dtype, 8, Hq, Hk, D, P, lens, rows), D ** -0.5, max_rows=max(rows), max_len=max(lens))
