@@ -743,7 +743,8 @@ typedef struct dspark_pages { /* every field is 8 bytes; strides are (page, head
  * sequence in row p % P of its page p / P; int32 starts [count + 1]: rows starts[b] .. starts[b + 1] - 1 of the call are
  * sequence b's, the last of its lens[b] (int32) positions. Whatever these hold, nothing outside the tensors is touched:
  * a sequence whose rows are not among the call's `rows` has none, and positions before the first, past the table or
- * in a page that is not one of the pool's are not there. count <= 4096, rows < 2^22.
+ * in a page that is not one of the pool's are not there. Starts that do not fall give every row to one sequence at most; rows that
+ * more than one claims come out as any one's, or not at all. count <= 4096, rows < 2^22.
  */
 typedef struct dspark_sequences { /* every field is 8 bytes */
   const int32_t* table;
@@ -757,11 +758,12 @@ typedef struct dspark_sequences { /* every field is 8 bytes */
  * [rows, Hk, D], bf16 or fp16, strides (row, head) in elements, 16-byte aligned. Of the first dims values of a head (a
  * multiple of 16, interleaved of 8; 0: nothing is rotated) the pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved,
  * turn by position * freqs[i] (fp64): cos and sin, times scale, rounded to fp32, then fl(fl(x1 c) - fl(x2 s)) and
- * fl(fl(x1 s) + fl(x2 c)) in fp32, rounded to dtype. positions (int32 or int64 [rows]) replaces the rows' own.
- * q_out may be q itself. Pages of codes: the exponent of a page and head becomes the least with |x| <= 448 2^(e - 127)
- * for the finite values of the rows new in it, at least 17, and at least what it was where the page holds rows of this
- * sequence before them, which are shifted to it; codes are rounded to nearest even, infinities become NaN, and so do rows
- * behind others of a NaN scale. A page that is written to belongs to one sequence.
+ * fl(fl(x1 s) + fl(x2 c)) in fp32, rounded to dtype. positions (int32 or int64 [rows]) replaces the rows' own; angles up to 2^50.
+ * q_out may be q itself, else it shares no byte with what is read; nor do the pages of keys with those of values. Pages of
+ * codes: the exponent of a page and head becomes the least with |x| <= 448 2^(e - 127) for the finite values of the rows new in
+ * it, at least 17, and at least what it was where the page holds rows of this sequence before them, which are shifted to it;
+ * codes are rounded to nearest even, infinities become NaN, and so do rows behind others of a NaN scale. A page that is
+ * written to belongs to one sequence.
  */
 typedef struct dspark_paged_append_args { /* every field is 8 bytes */
   int64_t dtype, codes, Hq, Hk, D, P, pool, dims, interleaved;
@@ -801,11 +803,15 @@ int dspark_paged_read(const dspark_paged_read_args* args, dspark_stream stream);
  * Attention of a step's rows over their sequences' pages: q and out [rows, Hq, D] of dtype (strides (row, head), 16-byte
  * aligned), query head g of Hq reading KV head g / (Hq / Hk). Row i of sequence b's n sees, of the positions that are there,
  * 0 .. lens[b] - n + i (causal) or all lens[b]: out = softmax(scale q . k) . v in fp32, rounded once; zeros where it sees
- * none. Values that are not finite count only where a row sees them. Rows of no sequence: zeros (clear), else left as they
- * are. max_rows: rows of one sequence, at most; a sequence with more is served too, only slower. scale > 0, finite.
+ * none. Values that are not finite, and scores of nothing but -inf (NaN), count only where a row sees them. Rows of no sequence:
+ * zeros (clear), else left as they are. max_rows: rows of one sequence, at most; a sequence with more is served too, only slower.
+ * It chooses the kernels: give the step's own, 1 for decoded tokens. scale > 0, finite.
  * workspace: dspark_paged_attention_workspace bytes with max_len = width * P, 16-byte aligned, of any content, one call's at
- * a time: calls on two streams, or graphs that may run together, need one each. The result does not depend on what else is
- * in the call, but for the order in which partial sums are joined.
+ * a time: calls on two streams, or graphs that may run together, need one each.
+ * Scores, sums and outputs are fp32; a probability enters the product with the values as two pieces of dtype, off by 2^-16 of
+ * it (bf16) or 2^-20 (fp16; small ones 2^-31 of the row's largest), or, where the rows of a bf16 model's prompt chunk go over
+ * codes at D = 64 and 128, as one fp16 piece: 2^-11 of it, and 2^-32 of the row's largest. The call's bounds and the other sequences decide which a row takes, and in which
+ * parts its keys are joined: its result differs by no more than that between calls, and not at all between equal ones.
  */
 typedef struct dspark_paged_attention_args { /* every field is 8 bytes */
   int64_t dtype, codes, Hq, Hk, D, P, pool, causal, clear, max_rows;

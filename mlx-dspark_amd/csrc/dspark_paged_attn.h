@@ -19,8 +19,8 @@
 //   * 8-bit pages are turned into the model's type as they are used: one conversion for two values with the page's power of
 //     two in it, exact for every page that a model of that type wrote, but for values past fp16's largest: keys take what fp16 does not
 //     hold of their power of two to the scores (key_unit), values become infinite, and their rows are computed again.
-// Probabilities go to the matrix cores as two pieces of the type (16 bits of bf16, 22 of fp16, there of p 2^15): at these
-// row counts the second piece costs nothing.
+// Probabilities go to the matrix cores as two pieces of the type (16 bits of bf16, 20 and more of fp16, there of p 2^15), over 8-bit pages
+// too: at these row counts the second piece costs nothing.
 //
 // Values that are not finite are only let through where a row sees them: a row with such an output, or one that sees keys and has
 // no probability (scores of -inf), is computed again in plain fp32 from the keys it sees (plain_row).

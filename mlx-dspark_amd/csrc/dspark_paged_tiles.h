@@ -14,17 +14,19 @@
 //   * items with many keys first: sequences by their length, long causal tiles first within one. Consecutive items are a
 //     tile's KV heads, which go to consecutive XCDs: with 8 heads each XCD's L2 has the pages of one.
 // Probabilities are two pieces of the type, as in dspark_paged_attn.h: the second costs a third of the products, and one
-// bf16 piece alone would add an error of the size of the output's own rounding. Codes of a page are, but for extreme
-// scales, fp16 numbers when multiplied by 2^10, and one fp16 piece of a probability is off by an eighth of a bf16
-// rounding: so 8-bit pages of bf16 models go to LDS as fp16 and take one product, and only a workgroup that comes to a page
-// that does not fit begins again with two bf16 pieces (seven chunks of 1 to 700 rows: 182 -> 165 us). For bf16 pages what the
-// conversion costs is what the products save.
+// bf16 piece alone would add an error of the size of the output's own rounding. Codes of a page with a scale of 2^-25 to 2^-3
+// (values up to 56) are fp16 numbers when multiplied by 2^10, and one fp16 piece of a probability is off by an eighth of a bf16
+// rounding (2^-11 of it; one 2^21 under the reference is subnormal there, and off by 2^-32 of the reference): so 8-bit pages of
+// bf16 models go to LDS as fp16 and take one product, and a workgroup that comes to a page that does not fit begins again with
+// two bf16 pieces (seven chunks of 1 to 700 rows: 182 -> 165 us; with values past 56 throughout 101 -> 117 in seven others, with one
+// page of zeros, whose scale is 2^-110, in one sequence of them 126). Pages that are not there begin again too. For bf16 pages
+// what the conversion costs is what the products save.
 //
 // The running maximum is only raised (and the outputs rescaled) where it grew by more than 2^8: fp32 sums do not mind
 // probabilities up to 2^8, and with 32 rows a wave some row's maximum moves in most tiles.
 // 2048 rows behind 2953 keys, 32 / 8 heads of 128, bf16: 196 us (680 TFLOP/s of the two products, 1020 with the pieces); seven
-// chunks of 1 to 700 rows over 8-bit pages, 16 / 4 heads of 128: 134 us; six verify blocks of 18 to 96 rows of a KV head behind
-// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 59 us with what joins them (63 when waves without rows
+// chunks of 1 to 700 rows over 8-bit pages, 16 / 4 heads of 128: 130 us; six verify blocks of 18 to 96 rows of a KV head behind
+// 1500 to 10007 fp16 positions, 24 / 4 heads of 256: 154 MB in 56 us with what joins them (4 more when waves without rows
 // multiplied too). Tried and not kept: two groups of four waves in a workgroup, one in its products while the other is in its
 // softmax, a barrier between the phases (198 -> 234 us: as many cycles a tile, and lengths that fit together worse).
 #pragma once

@@ -1568,7 +1568,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages, v_pages, table: torc
     :func:`rope` does, ``dims`` a multiple of 16 (interleaved: of 8); None: nothing is rotated. ``positions`` int32 / int64
     [T]: rotate by these instead. Rows of a position that the table, or the pool, does not have are not written; rows
     behind the last sequence's are left out, and ``q_out`` there as it is. A page that is written to belongs to one
-    sequence. ``q_out``: where the queries go, e.g. ``q`` itself; else new, with zeros in rows of no sequence."""
+    sequence. ``q_out``: where the queries go, e.g. ``q`` itself; else new, with zeros in rows of no sequence. ``q_out`` in other memory
+    that is read or written, and pools that share some, are refused, unless a common stride sets them side by side."""
     what = "paged_append"
     tensors = (v, *_pages_parts(k_pages), *_pages_parts(v_pages), table, starts, lens, q, freqs, positions, q_out)
     dev = _one_device(what, k, *tensors)
@@ -1707,13 +1708,16 @@ def paged_attention(q: torch.Tensor, k_pages, v_pages, table: torch.Tensor, star
     and values first.
 
     Row i of a sequence's n sees the positions up to its own, ``lens[b] - n + i`` (``causal``), or all ``lens[b]``: an
-    encoder's states, kept in pages. fp32 scores, probabilities and sums; zeros for a row that sees nothing; values that
-    are not finite count only where a row sees them. Positions of pages that the pool does not have are not seen.
+    encoder's states, kept in pages. fp32 scores and sums; zeros for a row that sees nothing; values that are not finite
+    count only where a row sees them. Positions of pages that the pool does not have are not seen. A probability is held to 2^-16 of
+    it in bf16 and 2^-20 in fp16 models, and to 2^-11 (an eighth of the output's rounding) where the chunk rows of a bf16 model go
+    over 8-bit pages at D 64 and 128: by the call's bounds and the other sequences, a row may take the one or the other.
 
     ``max_rows`` (rows of one sequence) and ``max_len`` (positions; default: what the table has room for) are the
     host's bounds: positions from ``max_len`` on, rounded up to a page, are not seen (0 says that no sequence has any, and so
     no rows, whatever ``lens``: nothing is done but a new ``out`` cleared); more rows than ``max_rows`` are
-    served too, only slower. ``out``: rows of no sequence are left as they are there; in a new one they are zeros.
+    served too, only slower. ``max_rows`` chooses the kernels and the workspace, and is all of the call's rows if it is not given:
+    give the step's own, 1 for decoded tokens (32 of them over 8-bit pages take 54 us with it and 62 without). ``out``: rows of no sequence are left as they are there; in a new one they are zeros.
     ``workspace`` of :func:`paged_attention_workspace_bytes`, 16-byte aligned, any content, for one call at a time, else
     allocated."""
     what = "paged_attention"
